@@ -9,6 +9,7 @@ from .optimizers import (
     FlashAdam,
     FlashAdamW,
     FlashLion,
+    FlashMuon,
     FlashOptimizer,
     FlashSGD,
     FlashSGDW,
@@ -17,6 +18,7 @@ from .optimizers import (
     cast_model,
     compute_ecc_bits,
     enable_gradient_release,
+    newton_schulz,
     reconstruct_fp32_param,
 )
 
@@ -26,6 +28,7 @@ __all__ = [
     "FlashAdam",
     "FlashAdamW",
     "FlashLion",
+    "FlashMuon",
     "FlashOptimizer",
     "FlashSGD",
     "FlashSGDW",
@@ -34,5 +37,6 @@ __all__ = [
     "cast_model",
     "compute_ecc_bits",
     "enable_gradient_release",
+    "newton_schulz",
     "reconstruct_fp32_param",
 ]

@@ -51,6 +51,19 @@ class FoChunk(ctypes.Structure):
     ]
 
 
+class FoMatrixShape(ctypes.Structure):
+    """Mirror of ``fo_matrix_shape``."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int32),
+        ("cols", ctypes.c_int32),
+        ("count", ctypes.c_int32),
+        ("lr", ctypes.c_float),
+    ]
+
+
+MATRIX_MOST_LINES = 65536
+
 _DIAG_LIB_PATH = os.path.join(os.path.dirname(_LIB_PATH), "libflashoptim_hip_diag.so")
 
 _lock = threading.Lock()
@@ -85,6 +98,9 @@ SIGNATURES = {
     "fo_quantize_many": (_i32, [_vp, _i64, _i32, _vp]),
     "fo_ecc_join": (_i32, [_vp, _i32, _vp, _i32, _vp, _i64, _vp]),
     "fo_ecc_split": (_i32, [_vp, _vp, _i32, _vp, _i32, _i64, _vp]),
+    "fo_newton_schulz_workspace": (_i64, [_vp, _i64]),
+    "fo_newton_schulz": (_i32, [_vp, _i32] + [_i64] * 5 + [_vp, _i32, _vp, _f32, _vp, _i64, _vp]),
+    "fo_muon_step": (_i32, [_vp, _vp, _i64, _i32, _i32, _i32, _f32, _f32, _i32, _i32, _vp, _f32, _vp, _i64, _vp]),
 }
 # include/flashoptim_hip_diag.h: exported by the diagnostics build only (libflashoptim_hip_diag.so, which also
 # exports everything above)

@@ -227,6 +227,14 @@ class FlashOptimizer(torch.optim.Optimizer, abc.ABC):
     def _min_step_size_relative_to_lr(self) -> float:
         return 1.0  # sign-based updates (Lion) move every weight by exactly lr
 
+    def _order_bucket(self, items: list) -> list:
+        """The (parameter, tensors) pairs of one launch in the order its tables hold them."""
+        return items
+
+    def _make_plan(self, key: LaunchKey, tensors: list) -> Optional[BucketPlan]:
+        """The launch tables of a bucket; None to launch its tensors one by one."""
+        return BucketPlan(key.kind, key.dtype, key.ecc_bytes, key.quantized, tensors) if len(tensors) > 1 else None
+
     # True for optimizers whose kernels receive a per-parameter step number as a host value
     _step_number_by_value = False
 
@@ -437,11 +445,11 @@ class FlashOptimizer(torch.optim.Optimizer, abc.ABC):
                 cacheable = False  # sharded wrapper: keep the generic path
         buckets = []
         for key, items in planned.items():
+            items = self._order_bucket(items)
             tensors = [t for _, t in items]
             scalars = dict(key.scalars)
-            plan = None
-            if len(tensors) > 1:
-                plan = BucketPlan(key.kind, key.dtype, key.ecc_bytes, key.quantized, tensors)
+            plan = self._make_plan(key, tensors)
+            if plan is not None:
                 plan.launch(**scalars)
             else:
                 for t in tensors:

@@ -1,0 +1,337 @@
+// Matrix product core of the gfx950 kernels that multiply: C[i][j] = sum_k A[i][k] * B[j][k], both operands with k
+// contiguous, fp32 accumulation in the matrix cores.  The Newton-Schulz kernels (fo_muon.hip) run it on fp16 operands, the
+// microscaled 4-bit product (fo_mx.hip) on E2M1 codes with one E8M0 scale per 32 of them.  The two differ in the matrix
+// instruction only: either way a lane's operand of one 16x16 instruction is 16 bytes of one row, so a tile is rows of
+// bytes and the same staging serves both.
+//
+// Shape.  A workgroup is four wavefronts in a 2x2 arrangement; a wavefront owns a WT x WT piece of the tile (WT = 128, 64
+// or 32) and keeps it in its accumulators.  The operands pass through LDS in stages of 128 bytes of every row (64 fp16
+// values, 256 codes), two stages in turn.  With WT = 128 the workgroup holds 128 KiB of LDS, a wavefront 256 accumulator
+// registers and both halves of a stage's operands in registers, and one wavefront runs on each SIMD: every LDS byte read is
+// used for eight instructions, which is what keeps LDS (128 bytes a clock) behind the matrix cores.
+//
+// Flow.  Per stage two phases of (WT/16)^2 matrix instructions.  Phase 1 multiplies the first half of the stage out of
+// registers while the second half is read from LDS; then the workgroup meets (nobody reads this stage any more, and the next
+// one has arrived); phase 2 multiplies the second half while the next stage's first half is read and the loads of the
+// stage after it are issued into the buffer that has become free.  A load has one whole stage of multiplications to arrive.
+//
+// Loads go from memory straight into LDS (16 bytes a lane, no registers).  They are inline asm: the compiler would wait for
+// all of them before every LDS read.  They have no register result, and every wait for them is written out below.
+//
+// LDS layout: rows of 128 bytes, the eight 16-byte pieces of row r stored in the order piece ^ (r & 7), so that the 16 rows
+// that an instruction's operand needs lie in different banks.  The order is applied to the address that a lane loads from.
+#pragma once
+
+#include "fo_device.h"
+
+namespace fo {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kGemmThreads = 256;
+constexpr int kStageBytes = 128;   // of each row
+constexpr int kHalfBytes = 64;     // what one phase multiplies; rows are whole multiples of it
+
+// One operand: `rows` rows of `row_bytes` (a multiple of 64), `stride` bytes apart.  Rows beyond the last are read as copies of
+// the last one; what they contribute to is not stored.  scales (4-bit operands): one byte per 16 bytes of the row.
+struct Operand {
+    const char* data;
+    int64_t stride;
+    const uint8_t* scales;
+    int64_t scale_stride;
+    int rows;
+};
+
+// The matrix instructions are inline asm so that an accumulator stays in the registers it is in (the compiler's own form lets
+// result and addend differ, and with 256 accumulator registers out of 256 it spills).  What the hazard recogniser then does
+// not see: an accumulator may be read by other instructions 18 wait states after the last instruction that wrote it, see
+// multiply().  Results feed the next instruction on the same accumulator without a wait, at least three others lie between.
+struct F16Product {
+    static constexpr bool kScaled = false;
+    struct Frag { f16x8 v; };
+    __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c) {
+        asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a.v), "v"(b.v));
+    }
+};
+
+struct Mx4Product {
+    static constexpr bool kScaled = true;
+    struct Frag { i32x4 v; int scale; };
+    __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c) {
+        asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+            : "+a"(c) : "v"(a.v), "v"(b.v), "v"(a.scale), "v"(b.scale));
+    }
+};
+
+// 64 lanes x 16 (4) bytes from base + lane offset to LDS at `lds` + 16 (4) * lane.  m0, which holds that address, is a reserved
+// register: the compiler keeps no value in it, and nothing else in a kernel that multiplies uses it.
+__device__ __forceinline__ void load_to_lds16(unsigned lds, unsigned offset, const char* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_to_lds4(unsigned lds, unsigned offset, const char* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
+__device__ __forceinline__ void wait_loads_and_lds() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory"); }
+__device__ __forceinline__ void meet() {
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+__device__ __forceinline__ const char* uniform(const char* p) {
+    const uint64_t v = (uint64_t)p;
+    const u32 lo = __builtin_amdgcn_readfirstlane((u32)v), hi = __builtin_amdgcn_readfirstlane((u32)(v >> 32));
+    return (const char*)(((uint64_t)hi << 32) | lo);
+}
+
+template <class Product, int WT> struct GemmTile {
+    static constexpr int kTile = 2 * WT;          // rows and columns of a workgroup's tile
+    static constexpr int kFrags = WT / 16;        // 16-row pieces of a wavefront's operands
+    static constexpr int kRows = 2 * kTile;       // rows of a stage, A's then B's
+    static constexpr int kScaleOffset = kRows * kStageBytes;
+    static constexpr int kBuffer = kScaleOffset + (Product::kScaled ? kRows * 8 : 0);
+    static constexpr int kRowLoads = kRows / 8 / 4;                          // loads of a wavefront per stage: 8 rows each
+    static constexpr int kScaleLoads = Product::kScaled ? kRows / 32 / 4 : 0;   // 32 rows each
+    static constexpr int kLoads = kRowLoads + kScaleLoads;
+    // the epilogue moves the tile through LDS in strips of 32 rows of a wavefront, 4 floats of padding per row
+    static constexpr int kStripStride = WT + 4;
+    static constexpr int kStripBytes = 32 * kStripStride * 4;
+    static constexpr int kLds = 2 * kBuffer > 4 * kStripBytes ? 2 * kBuffer : 4 * kStripBytes;
+
+    typedef typename Product::Frag Frag;
+
+    f32x4 acc[kFrags][kFrags];
+    char* smem;
+    unsigned smem_address;
+    int wave, lane;
+
+    __device__ __forceinline__ GemmTile(char* lds)
+        : smem(lds), smem_address(lds_address(lds)), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), lane(threadIdx.x & 63) {}
+
+    // ------------------------------------------------------------------------------------------- staging
+    struct Loader {
+        unsigned row[kRowLoads];
+        unsigned scale[kScaleLoads > 0 ? kScaleLoads : 1];
+        unsigned past_half, past_half_scale;   // what a lane steps back by when the last stage is half of one
+        const char* base;
+        const char* scale_base;
+    };
+    __device__ __forceinline__ void start(Loader& l, const Operand& a, const Operand& b, int row0, int col0) const {
+        const bool first = wave < 2;  // two wavefronts load A's rows, two B's
+        const char* data = first ? a.data : b.data;
+        const int64_t stride = first ? a.stride : b.stride;
+        const int at = first ? row0 : col0, left = (first ? a.rows : b.rows) - at;
+        l.base = uniform(data + at * stride);
+        const int row = lane >> 3, piece = (lane & 7) ^ (row & 7);
+        l.past_half = piece >= 4 ? kHalfBytes : 0;
+#pragma unroll
+        for (int i = 0; i < kRowLoads; ++i) {
+            int r = (wave & 1) * (kRowLoads * 8) + i * 8 + row;
+            r = r < left ? r : left - 1;
+            l.row[i] = (unsigned)(r * stride) + piece * 16;
+        }
+        if constexpr (Product::kScaled) {
+            const int64_t scale_stride = first ? a.scale_stride : b.scale_stride;
+            l.scale_base = uniform((const char*)(first ? a.scales : b.scales) + at * scale_stride);
+            l.past_half_scale = lane & 1 ? 4 : 0;
+#pragma unroll
+            for (int i = 0; i < kScaleLoads; ++i) {
+                int r = (wave & 1) * (kScaleLoads * 32) + i * 32 + (lane >> 1);
+                r = r < left ? r : left - 1;
+                l.scale[i] = (unsigned)(r * scale_stride) + (lane & 1) * 4;
+            }
+        }
+    }
+    // The i-th load of a stage.  half: the rows end in the middle of the stage, its second half repeats the first.
+    __device__ __forceinline__ void load(const Loader& l, int i, int stage, bool half) const {
+        const unsigned buffer = smem_address + (stage & 1) * kBuffer;
+        if (i < kRowLoads) {
+            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, l.row[i] - (half ? l.past_half : 0), l.base + (int64_t)stage * kStageBytes);
+        } else if constexpr (Product::kScaled) {
+            const int k = i - kRowLoads;
+            load_to_lds4(buffer + kScaleOffset + (wave * kScaleLoads + k) * 256, l.scale[k] - (half ? l.past_half_scale : 0),
+                         l.scale_base + (int64_t)stage * (kStageBytes / 16));
+        }
+    }
+
+    // Operand piece f of the wavefront (0..kFrags-1: B's, then A's) from half `half` of a stage.
+    __device__ __forceinline__ void read(Frag (&fa)[kFrags], Frag (&fb)[kFrags], int f, int stage, int half) const {
+        const bool is_b = f < kFrags;
+        const int i = is_b ? f : f - kFrags;
+        const int row = (is_b ? kTile + (wave & 1) * WT : (wave >> 1) * WT) + i * 16 + (lane & 15);
+        const char* buffer = smem + (stage & 1) * kBuffer;
+        Frag& out = is_b ? fb[i] : fa[i];
+        out.v = *reinterpret_cast<const decltype(out.v)*>(buffer + row * kStageBytes + (((half * 4 + (lane >> 4)) ^ (row & 7)) * 16));
+        if constexpr (Product::kScaled)
+            out.scale = *reinterpret_cast<const uint8_t*>(buffer + kScaleOffset + row * 8 + half * 4 + (lane >> 4));
+    }
+
+    // Multiplies (a, b) while reading the operands of the next phase into (na, nb) and, with LOAD, issuing a stage's loads.
+    // One row of instructions at a time, fenced off from the next, so that the reads and loads stay spread among them; the
+    // reads are over well before the last row, the next phase finds its operands there.
+    template <bool LOAD>
+    __device__ __forceinline__ void phase(const Frag (&a)[kFrags], const Frag (&b)[kFrags], Frag (&na)[kFrags], Frag (&nb)[kFrags],
+                                          int read_stage, int read_half, const Loader& l, int load_stage, bool load_half) {
+        constexpr int kReads = 2 * kFrags;
+        constexpr int kReadsPerRow = kFrags >= 4 ? (kReads + kFrags - 3) / (kFrags - 2) : kReads;
+        constexpr int kLoadsPerRow = (kLoads + kFrags - 1) / kFrags;
+#pragma unroll
+        for (int i = 0; i < kFrags; ++i) {
+            if constexpr (LOAD) {
+#pragma unroll
+                for (int k = i * kLoadsPerRow; k < (i + 1) * kLoadsPerRow && k < kLoads; ++k) load(l, k, load_stage, load_half);
+            }
+#pragma unroll
+            for (int k = i * kReadsPerRow; k < (i + 1) * kReadsPerRow && k < kReads; ++k) read(na, nb, k, read_stage, read_half);
+#pragma unroll
+            for (int j = 0; j < kFrags; ++j) Product::multiply(a[i], b[j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+
+    // Says that an accumulator lives in accumulator registers here.
+    __device__ __forceinline__ static void keep(f32x4& c) { asm volatile("" : "+a"(c)); }
+
+    // acc = the product's tile at (row0, col0) over rows of `row_bytes` > 0.
+    __device__ __forceinline__ void multiply(const Operand& a, const Operand& b, int row0, int col0, int row_bytes) {
+#pragma unroll
+        for (int i = 0; i < kFrags; ++i)
+#pragma unroll
+            for (int j = 0; j < kFrags; ++j) {
+                acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                keep(acc[i][j]);
+            }
+        const int stages = (row_bytes + kStageBytes - 1) / kStageBytes;
+        const bool odd = (row_bytes / kHalfBytes) & 1;
+        Loader l;
+        start(l, a, b, row0, col0);
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) load(l, k, 0, odd && stages == 1);
+        if (stages > 1) {
+#pragma unroll
+            for (int k = 0; k < kLoads; ++k) load(l, k, 1, odd && stages == 2);
+            wait_loads<kLoads>();
+        } else {
+            wait_loads<0>();
+        }
+        meet();
+        Frag a0[kFrags], b0[kFrags], a1[kFrags], b1[kFrags];
+#pragma unroll
+        for (int f = 0; f < 2 * kFrags; ++f) read(a0, b0, f, 0, 0);
+        int s = 0;
+        for (; s + 2 < stages; ++s) {
+            phase<false>(a0, b0, a1, b1, s, 1, l, 0, false);
+            wait_loads_and_lds();  // stage s is in registers, stage s + 1 in LDS
+            meet();
+            phase<true>(a1, b1, a0, b0, s + 1, 0, l, s + 2, odd && s + 3 == stages);
+        }
+        for (;; ++s) {
+            phase<false>(a0, b0, a1, b1, s, 1, l, 0, false);
+            wait_loads_and_lds();
+            meet();
+            if (s + 1 == stages && odd) break;
+            phase<false>(a1, b1, a0, b0, s + 1, 0, l, 0, false);
+            if (s + 1 == stages) break;
+        }
+        asm volatile("s_nop 15\n\ts_nop 3" : : : "memory");  // the last results are written
+#pragma unroll
+        for (int i = 0; i < kFrags; ++i)
+#pragma unroll
+            for (int j = 0; j < kFrags; ++j) keep(acc[i][j]);
+        meet();  // the epilogue writes over the buffers
+    }
+
+    // ------------------------------------------------------------------------------------------- epilogue
+    // Hands the tile to `out` row by row: out.row(i, j, v) gets v[0..7] = C[i][j .. j+7] (i, j counted in the whole result, j
+    // a multiple of 8) and, with out.kColumns, leaves in v what out.column(i, j, w) then gets column by column: w[0..7] =
+    // rows i .. i+7 of column j.  Consecutive lanes get consecutive pieces of a row (of eight rows of a column).
+    template <class Out> __device__ __forceinline__ void finish(int row0, int col0, Out& out) {
+        float* strip = reinterpret_cast<float*>(smem + wave * kStripBytes);
+        constexpr int kPieces = WT / 8;              // 8-value pieces of a row
+        constexpr int kRowsAtOnce = 64 / kPieces;
+        const int r0 = row0 + (wave >> 1) * WT, c0 = col0 + (wave & 1) * WT;
+#pragma unroll
+        for (int s = 0; s < WT / 32; ++s) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < kFrags; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        strip[(h * 16 + (lane >> 4) * 4 + k) * kStripStride + j * 16 + (lane & 15)] = acc[2 * s + h][j][k];
+            same_wave();
+            for (int r = lane / kPieces; r < 32; r += kRowsAtOnce) {
+                f32x4* p = reinterpret_cast<f32x4*>(strip + r * kStripStride + (lane % kPieces) * 8);
+                const f32x4 lo = p[0], hi = p[1];
+                float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                out.row(r0 + s * 32 + r, c0 + (lane % kPieces) * 8, v);
+                if constexpr (Out::kColumns) {
+                    p[0] = f32x4{v[0], v[1], v[2], v[3]};
+                    p[1] = f32x4{v[4], v[5], v[6], v[7]};
+                }
+            }
+            if constexpr (Out::kColumns) {
+                same_wave();
+                for (int k = lane; k < WT * 4; k += 64) {
+                    const int col = k >> 2, rows = (k & 3) * 8;
+                    float w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = strip[(rows + e) * kStripStride + col];
+                    out.column(r0 + s * 32 + rows, c0 + col, w);
+                }
+            }
+            same_wave();
+        }
+    }
+    // A wavefront's LDS accesses take effect in order; this keeps the compiler from reordering them.
+    __device__ __forceinline__ static void same_wave() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+};
+
+// ------------------------------------------------------------------------------------------- which tile a workgroup takes
+// Workgroup b runs on accelerator die b % 8, each with an L2 of its own: every die takes a contiguous run of the tiles.
+__device__ __forceinline__ int64_t tile_of_workgroup(int64_t b, int64_t tiles) {
+    const int64_t per = tiles >> 3, rest = tiles & 7, die = b & 7;
+    return die * per + (die < rest ? die : rest) + (b >> 3);
+}
+// Tile t of a result of `rows` x `cols` tiles, in bands of four rows, column by column: 32 consecutive tiles (a die's
+// compute units) share twelve operand panels.
+__device__ __forceinline__ void tile_at(int t, int rows, int cols, int& i, int& j) {
+    const int band = t / (4 * cols), left = t - band * 4 * cols;
+    const int height = rows - band * 4 < 4 ? rows - band * 4 : 4;
+    i = band * 4 + left % height;
+    j = left / height;
+}
+// The same for the tiles on and above the diagonal of a symmetric result of n x n tiles: n (n + 1) / 2 of them.
+__device__ __forceinline__ void tile_at_symmetric(int t, int n, int& i, int& j) {
+    int first = 0;
+    for (;;) {
+        const int height = n - first < 4 ? n - first : 4;
+        const int corner = height * (height + 1) / 2, in_band = corner + (n - first - height) * height;
+        if (t < in_band) {
+            if (t < corner) {
+                int k = 0;
+                while (t >= k + 1) t -= ++k;   // column k of the corner has k + 1 tiles
+                i = first + t;
+                j = first + k;
+            } else {
+                t -= corner;
+                i = first + t % height;
+                j = first + height + t / height;
+            }
+            return;
+        }
+        t -= in_band;
+        first += 4;
+    }
+}
+
+}  // namespace fo

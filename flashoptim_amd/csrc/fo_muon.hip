@@ -1,0 +1,714 @@
+// Newton-Schulz orthogonalisation of matrices and the Muon optimizer step around it, for gfx950, with their C entry points.
+//
+// Mathematics.  For a matrix G (rows x cols; its shorter side m, its longer n; X is G with the shorter side as rows):
+//     X <- G / (|G|_F + eps),  then `steps` times  S = X X',  B = b S + c S S,  X <- a X + B X.
+// The polynomial drives every singular value towards one and leaves the singular vectors alone.
+//
+// Precision.  The products run on the matrix cores in fp16 with fp32 sums.  Rounding X itself to fp16 in every step would
+// cost up to 1e-2 of the result: an error among the small singular directions is multiplied like the signal there (3.4 per
+// step).  So X is held in two parts, hi (fp16, the operand of the products) and lo (bf16, the rest, 19 bits or more together); lo
+// enters where X is multiplied by a.  The diagonal of B, by far its largest entries on a flat spectrum, is kept apart in
+// fp32 and added to a; the products see B without it.  What is left (S and B off the diagonal in fp16) costs 1e-4 .. 8e-4
+// of the result, below the bfloat16 rounding it is handed out with.  X starts at |X|_F = 1, entries as small as 1e-4, so
+// the first X is kept times a power of two near sqrt(n), in fp16's normal range.
+//
+// Layout.  "Main" arrays have G's own orientation, padded with zeros to multiples of 64 (Rp x Cp), so that the products need no
+// bounds inside; T is hi transposed.  Every product is then rows times rows (fo_gemm.h):
+//     S = rows of X by rows of X          (X = hi where rows <= cols, else T); the tiles on and above the diagonal, written twice
+//     B = rows of S by rows of S          (S is symmetric); likewise
+//     X = rows of B by rows of T          (rows <= cols), or rows of hi by rows of B: main orientation either way
+// so the result comes out in G's orientation and the last product's epilogue writes it, or updates the weights with it.
+//
+// One launch covers matrices of many shapes: the shapes travel as kernel arguments, matrices of one shape lie one after the
+// other in the workspace.
+#include "fo_gemm.h"
+#include "fo_host.h"
+#include "fo_step.h"
+
+namespace fo {
+
+constexpr int kMaxShapes = 16;    // of one launch
+constexpr int kPad = 64;
+constexpr int kChunk = 8192;      // elements of a matrix whose squares one workgroup sums
+
+// The matrices of one shape.
+struct MatrixGroup {
+    int rows, cols, padded_rows, padded_cols, count;
+    int first;            // matrix number of the first of them
+    int chunks;           // sums of squares of each
+    float unit;           // the power of two that the first X is kept times
+    float lr;             // optimizer step: learning rate with the shape's factor
+    char* workspace;      // their arrays, see the functions below
+
+    __host__ __device__ bool tall() const { return rows > cols; }
+    __host__ __device__ int side() const { return tall() ? padded_cols : padded_rows; }
+    __host__ __device__ int64_t area() const { return (int64_t)padded_rows * padded_cols; }
+    __host__ __device__ int64_t gram_area() const { return (int64_t)side() * side(); }
+    // per matrix: two generations of hi and of T, lo, S, B, the diagonal of B, the factor that normalises, sums of squares.
+    // The update before its normalisation (fp32) lies over the second generation, which is written later.
+    __host__ __device__ int64_t bytes_each() const {
+        return area() * 10 + gram_area() * 4 + side() * 4 + 256 + ((int64_t)chunks * 8 + 255) / 256 * 256;
+    }
+    __device__ char* of(int k) const { return workspace + bytes_each() * k; }
+    __device__ _Float16* hi(int k, int generation) const { return (_Float16*)(of(k) + generation * area() * 4); }
+    __device__ _Float16* t(int k, int generation) const { return (_Float16*)(of(k) + generation * area() * 4 + area() * 2); }
+    __device__ float* update(int k) const { return (float*)(of(k) + area() * 4); }
+    __device__ u32* lo(int k) const { return (u32*)(of(k) + area() * 8); }   // pairs of bf16
+    __device__ _Float16* s(int k) const { return (_Float16*)(of(k) + area() * 10); }
+    __device__ _Float16* b(int k) const { return (_Float16*)(of(k) + area() * 10 + gram_area() * 2); }
+    __device__ float* diagonal(int k) const { return (float*)(of(k) + area() * 10 + gram_area() * 4); }
+    __device__ float* factor(int k) const { return diagonal(k) + side(); }
+    __device__ double* squares(int k) const { return (double*)((char*)factor(k) + 256); }
+};
+
+// A launch over all groups; workgroups first[g] .. first[g + 1] belong to group g.
+struct Groups {
+    MatrixGroup group[kMaxShapes];
+    int64_t begin[kMaxShapes + 1];
+    int n;
+};
+
+__device__ __forceinline__ int group_of(const Groups& a, int64_t b) {
+    int g = 0;
+    while (g + 1 < a.n && b >= a.begin[g + 1]) ++g;
+    return g;
+}
+
+// ------------------------------------------------------------------------------------------------
+// what comes before the products: momentum, norm, normalised parts
+// ------------------------------------------------------------------------------------------------
+
+// Matrices in memory: `stride` elements between those of a stack, `row_stride` between rows, columns adjacent.  Without
+// data: the update that the momentum kernel left in the workspace.
+struct MatrixSource {
+    const void* data;
+    int64_t stride, row_stride;
+    bool aligned;   // 16-byte pieces of eight values may be read
+};
+
+template <int DT> __device__ __forceinline__ void read8(const char* p, bool aligned, int valid, float (&v)[8]) {
+    constexpr int B = DTypeInfo<DT>::bytes;
+    Pack<B, 16 / B> raw[B / 2];
+    if (aligned && valid >= 8) {
+        const u32x4* q = reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+        for (int i = 0; i < B / 2; ++i) {
+            const u32x4 w = q[i];
+            raw[i].w[0] = w.x; raw[i].w[1] = w.y; raw[i].w[2] = w.z; raw[i].w[3] = w.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < B / 2; ++i) load_guarded<B, 16 / B>(raw[i], p, i * (16 / B), valid);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = widen<DT, 16 / B>(raw[k / (16 / B)], k % (16 / B));
+}
+
+__device__ __forceinline__ double workgroup_sum(double x, double* lds) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_down(x, d);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+// Sum of the squares of a run of 8-value pieces of the matrix, one number per workgroup (in order, so a step repeats to
+// the bit).  One read of the matrix.
+template <int DT> __global__ __launch_bounds__(256) void squares_kernel(Groups a, MatrixSource source) {
+    __shared__ double lds[4];
+    const int g = group_of(a, blockIdx.x);
+    const MatrixGroup& m = a.group[g];
+    const int64_t local = blockIdx.x - a.begin[g];
+    const int k = (int)(local / m.chunks), chunk = (int)(local % m.chunks);
+    const int64_t pieces = (m.cols + 7) / 8, all = pieces * m.rows, each = (all + m.chunks - 1) / m.chunks;
+    const int64_t last = (chunk + 1) * each < all ? (chunk + 1) * each : all;
+    float sum = 0.0f;
+    for (int64_t i = chunk * each + threadIdx.x; i < last; i += 256) {
+        const int64_t row = i / pieces;
+        const int col = (int)(i - row * pieces) * 8;
+        float v[8];
+        read8<DT>((const char*)source.data + (source.stride * k + source.row_stride * row + col) * DTypeInfo<DT>::bytes, source.aligned, m.cols - col, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
+    }
+    const double total = workgroup_sum((double)sum, lds);
+    if (threadIdx.x == 0) m.squares(k)[chunk] = total;
+}
+
+// unit / (|G|_F + eps) of every matrix.
+__global__ __launch_bounds__(256) void norm_kernel(Groups a, float eps) {
+    __shared__ double lds[4];
+    const int g = group_of(a, blockIdx.x);
+    const MatrixGroup& m = a.group[g];
+    const int k = (int)(blockIdx.x - a.begin[g]);
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < m.chunks; i += 256) sum += m.squares(k)[i];
+    const double total = workgroup_sum(sum, lds);
+    if (threadIdx.x == 0) *m.factor(k) = (float)((double)m.unit / (sqrt(total) + (double)eps));
+}
+
+// 64 x 64 pieces of G, normalised, as hi and lo in G's orientation and hi transposed, zeros in the padding.
+template <int DT> __global__ __launch_bounds__(256) void split_kernel(Groups a, MatrixSource source) {
+    __shared__ _Float16 lds[64][64 + 2];
+    const int g = group_of(a, blockIdx.x);
+    const MatrixGroup& m = a.group[g];
+    const int tile_cols = m.padded_cols / 64, tiles = m.padded_rows / 64 * tile_cols;
+    const int64_t local = blockIdx.x - a.begin[g];
+    const int k = (int)(local / tiles), tile = (int)(local % tiles);
+    const int row0 = tile / tile_cols * 64, col0 = tile % tile_cols * 64;
+    const float factor = *m.factor(k);
+    const char* base = source.data ? (const char*)source.data + source.stride * k * DTypeInfo<DT>::bytes : (const char*)m.update(k);
+    const int64_t row_stride = source.data ? source.row_stride : m.cols;
+    const bool aligned = source.data ? source.aligned : m.cols % 4 == 0;
+    const int piece = (threadIdx.x & 7) * 8;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        const int r = (threadIdx.x >> 3) + 32 * p, row = row0 + r, col = col0 + piece;
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (row < m.rows && col < m.cols) read8<DT>(base + (row_stride * row + col) * DTypeInfo<DT>::bytes, aligned, m.cols - col, v);
+        f16x8 hi;
+        u32x4 lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] *= factor;
+            hi[e] = (_Float16)v[e];
+            v[e] -= (float)hi[e];
+            lds[r][piece + e] = hi[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const f32x2 pair = {v[2 * e], v[2 * e + 1]};
+            lo[e] = __builtin_bit_cast(u32, __builtin_convertvector(pair, bf16x2));
+        }
+        const int64_t at = (int64_t)row * m.padded_cols + col;
+        *reinterpret_cast<f16x8*>(m.hi(k, 0) + at) = hi;
+        *reinterpret_cast<u32x4*>(m.lo(k) + at / 2) = lo;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        const int c = (threadIdx.x >> 3) + 32 * p;
+        f16x8 t;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = lds[piece + e][c];
+        *reinterpret_cast<f16x8*>(m.t(k, 0) + (int64_t)(col0 + c) * m.padded_rows + row0 + piece) = t;
+    }
+}
+
+// Momentum of the optimizer step, over the flat elements of every matrix (groups of 32 codes run on across rows):
+//     m <- mu m + (1 - mu) g,   u = nesterov ? (1 - mu) g + mu m : m
+// each product and sum rounded, requantised as the SGD / Lion kernels do; u goes to the workspace in fp32 together with the
+// sum of its squares.
+struct MomentumArgs {
+    const fo_tensor_desc* matrices;
+    float mu, one_minus_mu;
+    int nesterov;
+};
+
+template <int DT, bool QUANT, int MODE>
+__device__ __forceinline__ float momentum_span(const fo_tensor_desc& d, float* update, Where w, int64_t n, const MomentumArgs& h, const float* lut) {
+    constexpr int EPL = DTypeInfo<DT>::epl, PB = DTypeInfo<DT>::bytes, SB = QUANT ? 1 : PB;
+    Pack<PB, EPL> g;
+    Pack<SB, EPL> raw;
+    load_lane<PB, EPL, MODE>(g, d.grad, w, n);
+    load_lane<SB, EPL, MODE>(raw, d.mom, w, n);
+    const bool live = MODE == kVector || w.first() < n;
+    float scale = 1.0f;
+    if constexpr (QUANT) { if (live) scale = f16_bits_to_f32(load_scale((const uint16_t*)d.mom_scales, w)); }
+    float m[EPL], u[EPL], am = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < EPL; ++k) {
+        const float gk = widen<DT, EPL>(g, k) * h.one_minus_mu;
+        float old;
+        if constexpr (QUANT) old = lookup_mom(lut, byte_of<EPL>(raw, k)) * scale; else old = widen<DT, EPL>(raw, k);
+        m[k] = old * h.mu + gk;
+        u[k] = h.nesterov ? gk + m[k] * h.mu : m[k];
+        am = fmaxf(am, fabsf(m[k]));
+        sum = fmaf(u[k], u[k], sum);
+    }
+    if constexpr (QUANT) {
+        am = fmaxf(group_max<EPL>(am), 1e-12f);
+        if constexpr (EPL == 8) quantize_mom_quick_verified<EPL>(m, am, raw);
+        else quantize_mom(m, am, raw);
+        if (live && (threadIdx.x & (32 / EPL - 1)) == 0) store_scale((uint16_t*)d.mom_scales, w, f32_to_f16_bits(am));
+    } else {
+        narrow_all<DT, EPL>(m, raw);
+    }
+    store_lane<SB, EPL, MODE>(raw, d.mom, w, n);
+    // the update is read again at once: ordinary stores
+    float* out = update + w.first();
+    if (MODE == kVector || w.first() + EPL <= n) {
+#pragma unroll
+        for (int k = 0; k < EPL; k += 4) *reinterpret_cast<f32x4*>(out + k) = f32x4{u[k], u[k + 1], u[k + 2], u[k + 3]};
+    } else {
+        sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < EPL; ++k)
+            if (w.first() + k < n) { out[k] = u[k]; sum = fmaf(u[k], u[k], sum); }
+    }
+    return sum;
+}
+
+template <int DT, bool QUANT> __global__ __launch_bounds__(256) void momentum_kernel(Groups a, MomentumArgs h) {
+    constexpr int EPL = DTypeInfo<DT>::epl;
+    __shared__ double lds[4];
+    __shared__ __attribute__((aligned(16))) float lut[256];
+    const int g = group_of(a, blockIdx.x);
+    const MatrixGroup& m = a.group[g];
+    const int64_t local = blockIdx.x - a.begin[g], n = (int64_t)m.rows * m.cols;
+    const int k = (int)(local / m.chunks), chunk = (int)(local % m.chunks);
+    const fo_tensor_desc d = h.matrices[m.first + k];
+    if constexpr (QUANT) {
+        // (q / 127) / (2 - |q / 127|) with q times 1/127 for the first quotient: a value in the last place of the step kernels'
+        // table, without reading one.  About one code in 1e5 comes out one step apart for it.
+        const float y = (float)(int8_t)threadIdx.x * (1.0f / 127.0f);
+        lut[threadIdx.x] = y / (2.0f - fabsf(y));
+        __syncthreads();
+    }
+    const bool aligned = (((uintptr_t)d.grad | (uintptr_t)d.mom) & 15) == 0;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float sum = 0.0f;
+    for (int i = wave; i < kChunk / (64 * EPL); i += 4) {
+        const Where w{(int64_t)chunk * kChunk + i * 64 * EPL, (int)(threadIdx.x & 63) * EPL};
+        if (w.span >= n) break;
+        if (aligned && w.span + 64 * EPL <= n) sum += momentum_span<DT, QUANT, kVector>(d, m.update(k), w, n, h, lut);
+        else if (aligned) sum += momentum_span<DT, QUANT, kLane>(d, m.update(k), w, n, h, lut);
+        else sum += momentum_span<DT, QUANT, kGuarded>(d, m.update(k), w, n, h, lut);
+    }
+    const double total = workgroup_sum((double)sum, lds);
+    if (threadIdx.x == 0) m.squares(k)[chunk] = total;
+}
+
+// ------------------------------------------------------------------------------------------------
+// the products
+// ------------------------------------------------------------------------------------------------
+
+struct StepArgs {
+    float a, b, c;
+    int generation;    // of hi and T that the step starts from
+    int first;         // the parts still carry the unit
+};
+
+__device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
+    f16x8 h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = (_Float16)v[e];
+    return h;
+}
+
+// S, and B without its diagonal: rows of a symmetric matrix, each tile off the diagonal twice.
+struct SymmetricOut {
+    static constexpr bool kColumns = true;
+    const _Float16* s;      // B: the matrix that it is made of; S: null
+    _Float16* out;
+    float* diagonal;
+    int side;
+    float scale, b, c;
+    bool mirror;
+
+    __device__ __forceinline__ void row(int i, int j, float (&v)[8]) const {
+        if (i >= side || j >= side) return;
+        const int64_t at = (int64_t)i * side + j;
+        if (s) {
+            const f16x8 old = *reinterpret_cast<const f16x8*>(s + at);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = fmaf(c, v[e], b * (float)old[e]);
+                if (i == j + e) { diagonal[i] = v[e]; v[e] = 0.0f; }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= scale;
+        }
+        *reinterpret_cast<f16x8*>(out + at) = half8(v);
+    }
+    __device__ __forceinline__ void column(int i, int j, const float (&v)[8]) const {
+        if (!mirror || i >= side || j >= side) return;
+        *reinterpret_cast<f16x8*>(out + (int64_t)j * side + i) = half8(v);
+    }
+};
+
+template <int WT, bool GRAM> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2) void symmetric_kernel(Groups a, StepArgs h) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    typedef GemmTile<F16Product, WT> Tile;
+    const int64_t b = tile_of_workgroup(blockIdx.x, a.begin[a.n]);
+    const int g = group_of(a, b);
+    const MatrixGroup& m = a.group[g];
+    const int side = m.side(), n = (side + Tile::kTile - 1) / Tile::kTile, tiles = n * (n + 1) / 2;
+    const int64_t local = b - a.begin[g];
+    const int k = (int)(local / tiles);
+    int i, j;
+    tile_at_symmetric((int)(local % tiles), n, i, j);
+    const bool tall = m.tall();
+    const _Float16* x = GRAM ? (tall ? m.t(k, h.generation) : m.hi(k, h.generation)) : m.s(k);
+    const int64_t length = (GRAM ? (tall ? m.padded_rows : m.padded_cols) : side) * 2;
+    const Operand op{(const char*)x, length, nullptr, 0, side};
+    Tile tile(lds);
+    tile.multiply(op, op, i * Tile::kTile, j * Tile::kTile, (int)length);
+    SymmetricOut out{GRAM ? nullptr : m.s(k), GRAM ? m.s(k) : m.b(k), m.diagonal(k), side, h.first ? 1.0f / (m.unit * m.unit) : 1.0f, h.b, h.c, i != j};
+    tile.finish(i * Tile::kTile, j * Tile::kTile, out);
+}
+
+// X <- a X + B X, common to the steps: x = (acc + (a + d) (hi + lo)) / unit, d the diagonal entry of B.
+struct ApplyIn {
+    const _Float16* hi;
+    u32* lo;
+    const float* diagonal;
+    int rows, cols;     // padded
+    float a, scale;
+    bool tall;
+
+    __device__ __forceinline__ void x(int i, int j, float (&v)[8], u32x4& low) const {
+        const int64_t at = (int64_t)i * cols + j;
+        const f16x8 h = *reinterpret_cast<const f16x8*>(hi + at);
+        low = *reinterpret_cast<const u32x4*>(lo + at / 2);
+        float d[8];
+        if (tall) {
+            const f32x4 d0 = *reinterpret_cast<const f32x4*>(diagonal + j), d1 = *reinterpret_cast<const f32x4*>(diagonal + j + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { d[e] = a + d0[e]; d[4 + e] = a + d1[e]; }
+        } else {
+            const float one = a + diagonal[i];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = one;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float rest = as_f32(e & 1 ? low[e / 2] & 0xffff0000u : low[e / 2] << 16);
+            v[e] = fmaf(d[e], (float)h[e] + rest, v[e]) * scale;
+        }
+    }
+};
+
+struct ApplyOut : ApplyIn {
+    static constexpr bool kColumns = true;
+    _Float16 *next_hi, *next_t;
+    __device__ __forceinline__ void row(int i, int j, float (&v)[8]) const {
+        if (i >= rows || j >= cols) return;
+        u32x4 low;
+        x(i, j, v, low);
+        const f16x8 h = half8(v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const f32x2 rest = {v[2 * e] - (float)h[2 * e], v[2 * e + 1] - (float)h[2 * e + 1]};
+            low[e] = __builtin_bit_cast(u32, __builtin_convertvector(rest, bf16x2));
+        }
+        const int64_t at = (int64_t)i * cols + j;
+        *reinterpret_cast<f16x8*>(next_hi + at) = h;
+        *reinterpret_cast<u32x4*>(lo + at / 2) = low;
+    }
+    __device__ __forceinline__ void column(int i, int j, const float (&v)[8]) const {
+        if (i >= rows || j >= cols) return;
+        *reinterpret_cast<f16x8*>(next_t + (int64_t)j * rows + i) = half8(v);
+    }
+};
+
+// The last step: the result as bfloat16, or the weights moved along it.
+struct LastArgs {
+    uint16_t* result;               // rows x cols matrices one after the other; null: update the weights
+    const fo_tensor_desc* matrices;
+    int dtype, ecc_bytes;
+    float keep;                     // 1 - lr * weight decay
+};
+
+// 8 weights of a row (the first `valid` of them): p <- p * keep - lr * x at master precision.
+template <int DT, int ECCB> __device__ __forceinline__ void update8(const fo_tensor_desc& d, int64_t at, int valid, bool aligned, const float (&x)[8], float keep, float lr) {
+    constexpr int PB = DTypeInfo<DT>::bytes, EPL = DTypeInfo<DT>::epl;
+#pragma unroll
+    for (int part = 0; part < 8; part += EPL) {
+        Pack<PB, EPL> p;
+        Pack<ECCB, EPL> e;
+        const int64_t first = at + part, end = at + valid;
+        if (aligned) { load_lane<PB, EPL, kLane>(p, d.param, first, end); load_lane<ECCB, EPL, kLane>(e, d.ecc, first, end); }
+        else { load_lane<PB, EPL, kGuarded>(p, d.param, first, end); load_lane<ECCB, EPL, kGuarded>(e, d.ecc, first, end); }
+        float w[EPL];
+#pragma unroll
+        for (int k = 0; k < EPL; ++k) {
+            float master = widen<DT, EPL>(p, k);
+            if constexpr (ECCB > 0) master = ecc_join<DT, ECCB>(master, ecc_to_float<ECCB, EPL>(e, k));
+            w[k] = master * keep - x[part + k] * lr;
+        }
+        write_master<DT, ECCB, EPL>(w, p, e);
+        if (aligned) { store_lane<PB, EPL, kLane>(p, d.param, first, end); store_lane<ECCB, EPL, kLane>(e, d.ecc, first, end); }
+        else { store_lane<PB, EPL, kGuarded>(p, d.param, first, end); store_lane<ECCB, EPL, kGuarded>(e, d.ecc, first, end); }
+    }
+}
+
+struct LastOut : ApplyIn {
+    static constexpr bool kColumns = false;
+    LastArgs last;
+    fo_tensor_desc matrix;
+    uint16_t* result;
+    int true_rows, true_cols;
+    float lr;
+    bool aligned;
+
+    __device__ __forceinline__ void row(int i, int j, float (&v)[8]) const {
+        if (i >= true_rows || j >= true_cols) return;
+        u32x4 low;
+        x(i, j, v, low);
+        const int64_t at = (int64_t)i * true_cols + j;
+        const int valid = true_cols - j;
+        if (result) {
+            Pack<2, 8> p;
+            narrow_all<DT_BF16, 8>(v, p);
+            if (aligned && valid >= 8) *reinterpret_cast<u32x4*>(result + at) = u32x4{p.w[0], p.w[1], p.w[2], p.w[3]};
+            else store_guarded<2, 8>(p, result, at, at + valid);
+            return;
+        }
+        const int v8 = valid < 8 ? valid : 8;
+        switch (last.dtype * 4 + last.ecc_bytes) {
+            case DT_BF16 * 4 + 0: update8<DT_BF16, 0>(matrix, at, v8, aligned, v, last.keep, lr); break;
+            case DT_BF16 * 4 + 1: update8<DT_BF16, 1>(matrix, at, v8, aligned, v, last.keep, lr); break;
+            case DT_BF16 * 4 + 2: update8<DT_BF16, 2>(matrix, at, v8, aligned, v, last.keep, lr); break;
+            case DT_F16 * 4 + 0: update8<DT_F16, 0>(matrix, at, v8, aligned, v, last.keep, lr); break;
+            case DT_F16 * 4 + 1: update8<DT_F16, 1>(matrix, at, v8, aligned, v, last.keep, lr); break;
+            case DT_F16 * 4 + 2: update8<DT_F16, 2>(matrix, at, v8, aligned, v, last.keep, lr); break;
+            default: update8<DT_F32, 0>(matrix, at, v8, aligned, v, last.keep, lr);
+        }
+    }
+    __device__ __forceinline__ void column(int, int, const float (&)[8]) const {}
+};
+
+template <int WT, bool LAST> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2) void apply_kernel(Groups a, StepArgs h, LastArgs last) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    typedef GemmTile<F16Product, WT> Tile;
+    const int64_t b = tile_of_workgroup(blockIdx.x, a.begin[a.n]);
+    const int g = group_of(a, b);
+    const MatrixGroup& m = a.group[g];
+    const int rows = (m.padded_rows + Tile::kTile - 1) / Tile::kTile, cols = (m.padded_cols + Tile::kTile - 1) / Tile::kTile;
+    const int64_t local = b - a.begin[g];
+    const int k = (int)(local / (rows * cols));
+    int i, j;
+    tile_at((int)(local % (rows * cols)), rows, cols, i, j);
+    const bool tall = m.tall();
+    const int side = m.side();
+    const Operand poly{(const char*)m.b(k), side * 2, nullptr, 0, side};
+    const Operand main{(const char*)m.hi(k, h.generation), side * 2, nullptr, 0, m.padded_rows};
+    const Operand turned{(const char*)m.t(k, h.generation), side * 2, nullptr, 0, m.padded_cols};
+    Tile tile(lds);
+    tile.multiply(tall ? main : poly, tall ? poly : turned, i * Tile::kTile, j * Tile::kTile, side * 2);
+    const ApplyIn in{m.hi(k, h.generation), m.lo(k), m.diagonal(k), m.padded_rows, m.padded_cols, h.a, h.first ? 1.0f / m.unit : 1.0f, tall};
+    if constexpr (LAST) {
+        LastOut out{in, last, {}, nullptr, m.rows, m.cols, m.lr, true};
+        if (last.result) {
+            out.result = last.result + (int64_t)(m.first + k) * m.rows * m.cols;
+            out.aligned = m.cols % 8 == 0;
+        } else {
+            out.matrix = last.matrices[m.first + k];
+            out.aligned = m.cols % 8 == 0 && (((uintptr_t)out.matrix.param | (uintptr_t)out.matrix.ecc) & 15) == 0;
+        }
+        tile.finish(i * Tile::kTile, j * Tile::kTile, out);
+    } else {
+        ApplyOut out{in, m.hi(k, h.generation ^ 1), m.t(k, h.generation ^ 1)};
+        tile.finish(i * Tile::kTile, j * Tile::kTile, out);
+    }
+}
+
+}  // namespace fo
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+namespace {
+using namespace fo_host;
+
+constexpr int64_t kMostWorkgroups = 1 << 23;   // of 256 threads: below 2^32 work-items
+
+int64_t padded(int64_t n) { return (n + fo::kPad - 1) / fo::kPad * fo::kPad; }
+
+// Shapes without elements are left out of the launches.
+int validate_shapes(const fo_matrix_shape* shapes, int64_t n) {
+    if (n < 0 || (n > 0 && !shapes)) return fail(FO_ERR_INVALID_ARGUMENT, "shapes must not be NULL");
+    for (int64_t i = 0; i < n; ++i) {
+        const fo_matrix_shape& s = shapes[i];
+        if (s.rows < 0 || s.cols < 0 || s.count < 0) return fail(FO_ERR_INVALID_ARGUMENT, "negative size of shape %lld", (long long)i);
+        if (s.rows > FO_MATRIX_MOST_LINES || s.cols > FO_MATRIX_MOST_LINES)
+            return fail(FO_ERR_UNSUPPORTED, "a matrix of %d x %d has more than %d rows or columns", s.rows, s.cols, FO_MATRIX_MOST_LINES);
+    }
+    return 0;
+}
+
+// The groups of shapes[0..n) with their places in the workspace; returns its size.
+int64_t plan(const fo_matrix_shape* shapes, int64_t n, char* workspace, fo::Groups* out) {
+    int64_t at = 0;
+    int first = 0, used = 0;
+    for (int64_t i = 0; i < n; ++i) {
+        const fo_matrix_shape& s = shapes[i];
+        if (s.rows > 0 && s.cols > 0 && s.count > 0) {
+            fo::MatrixGroup m{};
+            m.rows = s.rows; m.cols = s.cols; m.count = s.count; m.first = first; m.lr = s.lr;
+            m.padded_rows = (int)padded(s.rows); m.padded_cols = (int)padded(s.cols);
+            m.chunks = (int)(((int64_t)s.rows * s.cols + fo::kChunk - 1) / fo::kChunk);
+            m.unit = 1.0f;
+            const int longer = s.rows > s.cols ? s.rows : s.cols;
+            while (m.unit * m.unit * 4.0f <= (float)longer) m.unit *= 2.0f;
+            m.workspace = workspace + at;
+            at += m.bytes_each() * s.count;
+            if (out) out->group[used] = m;
+            ++used;
+        }
+        first += s.count;
+    }
+    if (out) out->n = used;
+    return at;
+}
+
+// Sets the groups' ranges of workgroups, `each(group)` of them for a matrix; returns the grid.
+template <class F> int64_t spread(fo::Groups& a, F each) {
+    a.begin[0] = 0;
+    for (int g = 0; g < a.n; ++g) a.begin[g + 1] = a.begin[g] + each(a.group[g]) * a.group[g].count;
+    return a.begin[a.n];
+}
+
+int64_t tiles_across(int n, int tile) { return (n + tile - 1) / tile; }
+
+template <int WT> int64_t symmetric_tiles(fo::Groups& a) {
+    return spread(a, [](const fo::MatrixGroup& m) { const int64_t n = tiles_across(m.side(), 2 * WT); return n * (n + 1) / 2; });
+}
+template <int WT> int64_t apply_tiles(fo::Groups& a) {
+    return spread(a, [](const fo::MatrixGroup& m) { return tiles_across(m.padded_rows, 2 * WT) * tiles_across(m.padded_cols, 2 * WT); });
+}
+
+template <class K, class... Args> int launch(K kernel, int64_t grid, int lds, hipStream_t stream, const char* what, Args... args) {
+    if (grid > kMostWorkgroups) return fail(FO_ERR_UNSUPPORTED, "%s: %lld workgroups are more than one launch takes", what, (long long)grid);
+    if (lds > 65536) {
+        if (int rc = check_hip(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds), what)) return rc;
+    }
+    kernel<<<dim3((unsigned)grid), dim3(256), lds, stream>>>(args...);
+    return check_hip(hipGetLastError(), what);
+}
+
+// The largest tile that still gives every compute unit one.
+int choose(int64_t large, int64_t middle, int cus) {
+    if (large >= cus) return 128;
+    return middle >= cus ? 64 : 32;
+}
+
+template <bool GRAM> int launch_symmetric(fo::Groups& a, const fo::StepArgs& h, int cus, hipStream_t stream) {
+    const char* what = "Newton-Schulz product";
+    switch (choose(symmetric_tiles<128>(a), symmetric_tiles<64>(a), cus)) {
+        case 128: return launch(fo::symmetric_kernel<128, GRAM>, symmetric_tiles<128>(a), fo::GemmTile<fo::F16Product, 128>::kLds, stream, what, a, h);
+        case 64: return launch(fo::symmetric_kernel<64, GRAM>, symmetric_tiles<64>(a), fo::GemmTile<fo::F16Product, 64>::kLds, stream, what, a, h);
+        default: return launch(fo::symmetric_kernel<32, GRAM>, symmetric_tiles<32>(a), fo::GemmTile<fo::F16Product, 32>::kLds, stream, what, a, h);
+    }
+}
+template <bool LAST> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, int cus, hipStream_t stream) {
+    const char* what = "Newton-Schulz step";
+    switch (choose(apply_tiles<128>(a), apply_tiles<64>(a), cus)) {
+        case 128: return launch(fo::apply_kernel<128, LAST>, apply_tiles<128>(a), fo::GemmTile<fo::F16Product, 128>::kLds, stream, what, a, h, last);
+        case 64: return launch(fo::apply_kernel<64, LAST>, apply_tiles<64>(a), fo::GemmTile<fo::F16Product, 64>::kLds, stream, what, a, h, last);
+        default: return launch(fo::apply_kernel<32, LAST>, apply_tiles<32>(a), fo::GemmTile<fo::F16Product, 32>::kLds, stream, what, a, h, last);
+    }
+}
+
+struct Iteration { int steps; float a, b, c, eps; };
+
+int validate_iteration(int steps, const float* coefficients, float eps) {
+    if (steps < 1) return fail(FO_ERR_INVALID_ARGUMENT, "steps must be at least 1, not %d", steps);
+    if (!coefficients) return fail(FO_ERR_INVALID_ARGUMENT, "coefficients must not be NULL");
+    if (!(eps >= 0.0f)) return fail(FO_ERR_INVALID_ARGUMENT, "eps must not be negative");
+    return 0;
+}
+
+// From the sums of squares on.
+template <int DT> int iterate(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, const fo::LastArgs& last, hipStream_t stream) {
+    const int cus = compute_units();
+    if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
+    int64_t grid = spread(a, [](const fo::MatrixGroup&) { return (int64_t)1; });
+    if (int rc = launch(fo::norm_kernel, grid, 0, stream, "norm", a, it.eps)) return rc;
+    grid = spread(a, [](const fo::MatrixGroup& m) { return m.area() / 4096; });
+    if (int rc = launch(fo::split_kernel<DT>, grid, 0, stream, "normalisation", a, source)) return rc;
+    for (int k = 0; k < it.steps; ++k) {
+        const fo::StepArgs h{it.a, it.b, it.c, k & 1, k == 0};
+        if (int rc = launch_symmetric<true>(a, h, cus, stream)) return rc;
+        if (int rc = launch_symmetric<false>(a, h, cus, stream)) return rc;
+        if (int rc = k + 1 < it.steps ? launch_apply<false>(a, h, last, cus, stream) : launch_apply<true>(a, h, last, cus, stream)) return rc;
+    }
+    return 0;
+}
+
+template <int DT> int orthogonalise(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, const fo::LastArgs& last, hipStream_t stream) {
+    const int64_t grid = spread(a, [](const fo::MatrixGroup& m) { return (int64_t)m.chunks; });
+    if (int rc = launch(fo::squares_kernel<DT>, grid, 0, stream, "sum of squares", a, source)) return rc;
+    return iterate<DT>(a, source, it, last, stream);
+}
+
+template <int DT> int momentum(fo::Groups& a, const fo::MomentumArgs& h, int quantized, hipStream_t stream) {
+    const int64_t grid = spread(a, [](const fo::MatrixGroup& m) { return (int64_t)m.chunks; });
+    return quantized ? launch(fo::momentum_kernel<DT, true>, grid, 0, stream, "momentum", a, h)
+                     : launch(fo::momentum_kernel<DT, false>, grid, 0, stream, "momentum", a, h);
+}
+
+}  // namespace
+
+extern "C" {
+int64_t fo_newton_schulz_workspace(const fo_matrix_shape* shapes, int64_t n_shapes) {
+    if (int rc = validate_shapes(shapes, n_shapes)) return rc;
+    int64_t most = 0;
+    // lists of more shapes than a launch takes go through the workspace one part after the other
+    for (int64_t i = 0; i < n_shapes; i += fo::kMaxShapes) {
+        const int64_t n = n_shapes - i < fo::kMaxShapes ? n_shapes - i : fo::kMaxShapes;
+        const int64_t bytes = plan(shapes + i, n, nullptr, nullptr);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
+}
+
+int fo_newton_schulz(const void* x, int dtype, int64_t count, int64_t rows, int64_t cols, int64_t stride, int64_t row_stride,
+                     void* result, int steps, const float* coefficients, float eps, void* workspace, int64_t workspace_bytes,
+                     void* stream) {
+    if (dtype < FO_F32 || dtype > FO_F16) return fail(FO_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+    if (count < 0 || rows < 0 || cols < 0 || count > INT32_MAX || rows > INT32_MAX || cols > INT32_MAX)
+        return fail(FO_ERR_INVALID_ARGUMENT, "bad size");
+    if (int rc = validate_iteration(steps, coefficients, eps)) return rc;
+    const fo_matrix_shape shape{(int32_t)rows, (int32_t)cols, (int32_t)count, 0.0f};
+    if (int rc = validate_shapes(&shape, 1)) return rc;
+    if (count == 0 || rows == 0 || cols == 0) return 0;
+    if (!x || !result || !workspace) return fail(FO_ERR_INVALID_ARGUMENT, "x, result and workspace must not be NULL");
+    if ((uintptr_t)workspace & 255 || (uintptr_t)result & 15) return fail(FO_ERR_INVALID_ARGUMENT, "workspace must be aligned to 256 bytes, result to 16");
+    fo::Groups a{};
+    if (workspace_bytes < plan(&shape, 1, (char*)workspace, &a)) return fail(FO_ERR_INVALID_ARGUMENT, "workspace too small");
+    const int width = dtype == FO_F32 ? 4 : 2;
+    const bool aligned = (((uintptr_t)x | (uintptr_t)(stride * width) | (uintptr_t)(row_stride * width)) & 15) == 0;
+    const fo::MatrixSource source{x, stride, row_stride, aligned};
+    const Iteration it{steps, coefficients[0], coefficients[1], coefficients[2], eps};
+    const fo::LastArgs last{(uint16_t*)result, nullptr, 0, 0, 0.0f};
+    switch (dtype) {
+        case FO_F32: return orthogonalise<fo::DT_F32>(a, source, it, last, (hipStream_t)stream);
+        case FO_BF16: return orthogonalise<fo::DT_BF16>(a, source, it, last, (hipStream_t)stream);
+        default: return orthogonalise<fo::DT_F16>(a, source, it, last, (hipStream_t)stream);
+    }
+}
+
+int fo_muon_step(const fo_tensor_desc* matrices, const fo_matrix_shape* shapes, int64_t n_shapes, int dtype, int ecc_bytes,
+                 int quantized, float keep, float momentum_coef, int nesterov, int steps, const float* coefficients, float eps,
+                 void* workspace, int64_t workspace_bytes, void* stream) {
+    if (dtype < FO_F32 || dtype > FO_F16) return fail(FO_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+    if (ecc_bytes < 0 || ecc_bytes > 2) return fail(FO_ERR_INVALID_ARGUMENT, "ecc_bytes must be 0, 1 or 2, not %d", ecc_bytes);
+    if (dtype == FO_F32 && ecc_bytes) return fail(FO_ERR_UNSUPPORTED, "fp32 parameters have no correction term");
+    if (int rc = validate_iteration(steps, coefficients, eps)) return rc;
+    if (int rc = validate_shapes(shapes, n_shapes)) return rc;
+    const int64_t need = fo_newton_schulz_workspace(shapes, n_shapes);
+    if (need == 0) return 0;
+    if (!matrices || !workspace) return fail(FO_ERR_INVALID_ARGUMENT, "matrices and workspace must not be NULL");
+    if ((uintptr_t)workspace & 255) return fail(FO_ERR_INVALID_ARGUMENT, "workspace must be aligned to 256 bytes");
+    if (workspace_bytes < need) return fail(FO_ERR_INVALID_ARGUMENT, "workspace too small");
+    const Iteration it{steps, coefficients[0], coefficients[1], coefficients[2], eps};
+    for (int64_t i = 0; i < n_shapes; i += fo::kMaxShapes) {
+        const int64_t n = n_shapes - i < fo::kMaxShapes ? n_shapes - i : fo::kMaxShapes;
+        fo::Groups a{};
+        plan(shapes + i, n, (char*)workspace, &a);
+        if (a.n > 0) {
+            const fo::MomentumArgs h{matrices, momentum_coef, 1.0f - momentum_coef, nesterov};
+            const fo::LastArgs last{nullptr, matrices, dtype, ecc_bytes, keep};
+            hipStream_t s = (hipStream_t)stream;
+            if (int rc = dtype == FO_F32 ? momentum<fo::DT_F32>(a, h, quantized, s) : dtype == FO_BF16 ? momentum<fo::DT_BF16>(a, h, quantized, s)
+                                                                                                : momentum<fo::DT_F16>(a, h, quantized, s)) return rc;
+            if (int rc = iterate<fo::DT_F32>(a, fo::MatrixSource{nullptr, 0, 0, false}, it, last, s)) return rc;
+        }
+        for (int64_t k = 0; k < n; ++k) matrices += shapes[i + k].count;
+    }
+    return 0;
+}
+}  // extern "C"

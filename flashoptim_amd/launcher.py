@@ -101,9 +101,11 @@ def absmax_many(tensors: Sequence[torch.Tensor]) -> list[float]:
 class BucketPlan:
     """Launch tables of one bucket: tensors that share kernel kind, dtype, ECC width and quantisation."""
 
+    _kinds = ("adam", "momentum", "plain")
+
     def __init__(self, kind: str, dtype: torch.dtype, ecc_bytes: int, quantized: bool,
                  tensors: Sequence[StepTensors], tiles_per_chunk: int = 0):
-        if kind not in ("adam", "momentum", "plain"):
+        if kind not in self._kinds:
             raise ValueError(f"no multi-tensor kernel for kind {kind!r}")
         self.kind, self.dtype, self.ecc_bytes, self.quantized = kind, dtype, int(ecc_bytes), bool(quantized)
         self.device = tensors[0].param.device
@@ -134,13 +136,10 @@ class BucketPlan:
             raise RuntimeError(
                 "The launch tables of a multi-tensor step cannot be built while a HIP graph is being captured. Run one "
                 "step outside the capture first, with the gradient buffers the graph will use.")
-        host, self.n_chunks = chunk_table(numels, tiles_per_chunk)
-        self.chunks_dev = host.to(self.device)
+        self._divide(tensors, numels, tiles_per_chunk)
         nbytes = self.n_tensors * ctypes.sizeof(FoTensorDesc)
         self.descs_dev = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        # what every launch of the plan starts its argument list with
-        self._head = (self.descs_dev.data_ptr(), self.n_tensors, self.chunks_dev.data_ptr(), self.n_chunks,
-                      DTYPE_CODE[dtype], self.ecc_bytes, int(self.quantized))
+        self._head = self._launch_head()
         # two pinned staging buffers for the life of the plan, used in turn; `_staged[i]` marks the last copy out of
         # buffer i
         self._staging = [torch.empty(nbytes, dtype=torch.uint8).pin_memory() for _ in range(2)]
@@ -148,6 +147,16 @@ class BucketPlan:
         self._staged: list[Optional[torch.cuda.Event]] = [None, None]
         self._next_staging = 0
         self._dirty = True
+
+    def _divide(self, tensors: Sequence[StepTensors], numels: Sequence[int], tiles_per_chunk: int) -> None:
+        """The work of one launch as the kernels are to divide it."""
+        host, self.n_chunks = chunk_table(numels, tiles_per_chunk)
+        self.chunks_dev = host.to(self.device)
+
+    def _launch_head(self) -> tuple:
+        """What every launch of the plan starts its argument list with."""
+        return (self.descs_dev.data_ptr(), self.n_tensors, self.chunks_dev.data_ptr(), self.n_chunks,
+                DTYPE_CODE[self.dtype], self.ecc_bytes, int(self.quantized))
 
     def set_grad_ptr(self, index: int, ptr: int) -> None:
         self.table[index].grad = ptr

@@ -19,6 +19,7 @@ from .kernels import (
     reconstruct_fp32_param,
 )
 from .lion import FlashLion
+from .muon import FlashMuon, newton_schulz
 from .release import GradientReleaseHandle, enable_gradient_release
 from .sgd import FlashSGD, FlashSGDW
 from .state import QuantizedTensorSpec, _MaybeQuantizedTensor
@@ -27,6 +28,7 @@ __all__ = [
     "NumericsError",
     "FlashOptimizer",
     "FlashLion",
+    "FlashMuon",
     "FlashSGD",
     "FlashSGDW",
     "FlashAdam",
@@ -35,5 +37,6 @@ __all__ = [
     "cast_model",
     "compute_ecc_bits",
     "enable_gradient_release",
+    "newton_schulz",
     "reconstruct_fp32_param",
 ]

@@ -232,6 +232,38 @@ int fo_ecc_join_many(const fo_convert_job *jobs, int64_t n_jobs, int narrow_dtyp
  * dst2 = their ecc, as fo_ecc_split gives it for src and dst */
 int fo_ecc_narrow_many(const fo_convert_job *jobs, int64_t n_jobs, int narrow_dtype, int ecc_bytes, void *stream);
 
+/*
+ * Newton-Schulz orthogonalisation and the Muon optimizer step (no counterpart in the reference).  For a matrix G, with X its
+ * orientation of fewer rows than columns:  X <- G / (|G|_F + eps), then `steps` times X <- a X + (b S + c S S) X, S = X X'.
+ * `coefficients` (host memory) is {a, b, c}.
+ */
+#define FO_MATRIX_MOST_LINES 65536 /* rows and columns of one matrix */
+
+/* `count` matrices of one shape; lr: the optimizer step's learning rate for them */
+typedef struct fo_matrix_shape {
+    int32_t rows, cols, count;
+    float lr;
+} fo_matrix_shape;
+
+/* Bytes of device memory, aligned to 256, that the calls below need for these shapes; negative: FO_ERR_* */
+int64_t fo_newton_schulz_workspace(const fo_matrix_shape *shapes, int64_t n_shapes);
+
+/* `count` matrices of `dtype`, `stride` elements apart, rows `row_stride` apart, columns adjacent; result: bfloat16, contiguous,
+ * aligned to 16 bytes.  The workspace is free again when the call's work on `stream` is done. */
+int fo_newton_schulz(const void *x, int dtype, int64_t count, int64_t rows, int64_t cols, int64_t stride, int64_t row_stride,
+                     void *result, int steps, const float *coefficients, float eps, void *workspace, int64_t workspace_bytes,
+                     void *stream);
+
+/*
+ * One step over a list of matrices: m <- mu m + (1 - mu) g (codes and scales requantised, or `dtype` values), the update
+ * (nesterov: (1 - mu) g + mu m, else m) through the iteration above, p <- p * keep - lr * update at master precision.
+ *   matrices: device memory, those of shapes[0] first, then those of shapes[1] and so on (var, var_scales and n are not
+ *   looked at); shapes: host memory
+ */
+int fo_muon_step(const fo_tensor_desc *matrices, const fo_matrix_shape *shapes, int64_t n_shapes, int dtype, int ecc_bytes,
+                 int quantized, float keep, float momentum_coef, int nesterov, int steps, const float *coefficients, float eps,
+                 void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
