@@ -14,10 +14,17 @@ from .optimizers import (
     FlashSGD,
     FlashSGDW,
     GradientReleaseHandle,
+    MXFP4Linear,
+    MXFP4Tensor,
     NumericsError,
     cast_model,
     compute_ecc_bits,
     enable_gradient_release,
+    mxfp4_dequantize,
+    mxfp4_linear,
+    mxfp4_matmul,
+    mxfp4_quantize,
+    mxfp4_quantize_both,
     newton_schulz,
     reconstruct_fp32_param,
 )
@@ -33,10 +40,17 @@ __all__ = [
     "FlashSGD",
     "FlashSGDW",
     "GradientReleaseHandle",
+    "MXFP4Linear",
+    "MXFP4Tensor",
     "NumericsError",
     "cast_model",
     "compute_ecc_bits",
     "enable_gradient_release",
+    "mxfp4_dequantize",
+    "mxfp4_linear",
+    "mxfp4_matmul",
+    "mxfp4_quantize",
+    "mxfp4_quantize_both",
     "newton_schulz",
     "reconstruct_fp32_param",
 ]

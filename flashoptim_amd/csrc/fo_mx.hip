@@ -1,0 +1,483 @@
+// Microscaled 4-bit floating point (MXFP4) for gfx950: quantiser, dequantiser and products, with their C entry points.
+//
+// Format.  A row is cut into groups of 32 values.  A group is stored as 32 E2M1 codes (sign, magnitudes 0, 0.5, 1, 1.5, 2, 3,
+// 4, 6) and one E8M0 byte s, the power of two 2^(s - 127) that multiplies them.  With M the group's largest magnitude,
+//     s - 127 = floor(log2 M) - 2, at least -127 (M = 0 included),     code = x / 2^(s - 127) rounded to nearest, ties to the even code,
+// magnitudes above 6 (up to 8 occur) become 6.  A group that holds an infinity or a NaN has s = 255 and stands for NaNs, so that it
+// shows in whatever is made of it.  Rows are filled up with zeros to whole blocks of 128 values: 64 bytes of codes, the first of two
+// in the low half of a byte, and 4 scale bytes.
+//
+// A product contracts over rows of both operands, so the scales have to run along the contracted axis: the quantiser writes
+// the row form of a matrix, the row form of its transpose, or both from one read.
+#include "fo_gemm.h"
+#include "fo_host.h"
+
+namespace fo {
+
+constexpr int kBlock = 128;    // values that rows are filled up to
+constexpr int kMxGroup = 32;
+
+// 8-bit scale of a group from the bits of its largest magnitude as fp32.  Infinities and NaNs have the largest bits.
+__device__ __forceinline__ u32 scale_byte(u32 magnitude_bits) {
+    const u32 e = magnitude_bits >> 23;
+    return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+// The scale as the converting instructions take it; they look at the exponent alone.
+__device__ __forceinline__ float scale_value(u32 byte) { return as_f32(byte << 23); }
+
+__device__ __forceinline__ u32 largest_of_quad(u32 x) {
+    const u32 a = (u32)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true);   // lanes 1 0 3 2
+    x = x > a ? x : a;
+    const u32 b = (u32)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true);   // lanes 2 3 0 1
+    return x > b ? x : b;
+}
+
+// Two values next to each other, as they are stored.
+template <int DT> struct Pair;
+template <> struct Pair<DT_BF16> {
+    u32 v;
+    __device__ __forceinline__ u32 magnitude() const {   // the larger, as fp32 bits
+        const u32 a = (v & 0x7fffu) << 16, b = v & 0x7fff0000u;
+        return a > b ? a : b;
+    }
+    template <int BYTE> __device__ __forceinline__ u32 encode(u32 into, float scale) const {
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(into, __builtin_bit_cast(bf16x2, v), scale, BYTE);
+    }
+};
+template <> struct Pair<DT_F16> {
+    u32 v;
+    __device__ __forceinline__ u32 magnitude() const {
+        const u32 a = v & 0x7fffu, b = (v >> 16) & 0x7fffu, m = a > b ? a : b;
+        return as_u32((float)__builtin_bit_cast(_Float16, (uint16_t)m));
+    }
+    template <int BYTE> __device__ __forceinline__ u32 encode(u32 into, float scale) const {
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(into, __builtin_bit_cast(f16x2, v), scale, BYTE);
+    }
+};
+template <> struct Pair<DT_F32> {
+    float a, b;
+    __device__ __forceinline__ u32 magnitude() const {
+        const u32 x = as_u32(a) & 0x7fffffffu, y = as_u32(b) & 0x7fffffffu;
+        return x > y ? x : y;
+    }
+    template <int BYTE> __device__ __forceinline__ u32 encode(u32 into, float scale) const {
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(into, a, b, scale, BYTE);
+    }
+};
+
+template <int DT> __device__ __forceinline__ u32 encode8(const Pair<DT>* p, float scale) {
+    u32 w = p[0].template encode<0>(0u, scale);
+    w = p[1].template encode<1>(w, scale);
+    w = p[2].template encode<2>(w, scale);
+    return p[3].template encode<3>(w, scale);
+}
+
+// Four pairs from memory, the first `valid` values of them, zeros after.
+template <int DT> __device__ __forceinline__ void load_pairs(const char* p, bool aligned, int valid, Pair<DT> (&out)[4]) {
+    constexpr int B = DTypeInfo<DT>::bytes;
+    u32 w[2 * B];
+    if (aligned && valid >= 8) {
+#pragma unroll
+        for (int i = 0; i < B / 2; ++i) {
+            const u32x4 q = reinterpret_cast<const u32x4*>(p)[i];
+            w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if constexpr (B == 2) {
+                const u32 x = k < valid ? reinterpret_cast<const uint16_t*>(p)[k] : 0u;
+                w[k / 2] = k & 1 ? w[k / 2] | x << 16 : x;
+            } else {
+                w[k] = k < valid ? reinterpret_cast<const u32*>(p)[k] : 0u;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (B == 2) out[i].v = w[i]; else { out[i].a = as_f32(w[2 * i]); out[i].b = as_f32(w[2 * i + 1]); }
+    }
+}
+
+struct QuantizeArgs {
+    const char* x;
+    int64_t row_stride;   // in elements
+    int rows, cols;
+    bool aligned;
+    uint8_t *codes, *scales;                  // of the rows, or null
+    uint8_t *column_codes, *column_scales;    // of the columns, or null
+};
+
+// A 128 x 128 piece per workgroup: read once, the row form out of registers (a group is four lanes), the column form through LDS
+// (a thread takes 32 rows of a column; two neighbouring columns at once for 2-byte types).  Bound by memory: 2 bytes in, 17/32
+// out per value and form.
+template <int DT> __global__ __launch_bounds__(256) void mx_quantize_kernel(QuantizeArgs a) {
+    constexpr int B = DTypeInfo<DT>::bytes, kStride = kBlock * B / 4 + 1;   // dwords, odd: rows begin in different banks
+    extern __shared__ u32 lds[];
+    const int tile_cols = (a.cols + kBlock - 1) / kBlock;
+    const int row0 = blockIdx.x / tile_cols * kBlock, col0 = blockIdx.x % tile_cols * kBlock;
+    const int64_t row_bytes = (int64_t)tile_cols * (kBlock / 2);
+    const int piece = threadIdx.x & 15;
+    const int col = col0 + piece * 8;
+#pragma unroll
+    for (int pass = 0; pass < 8; ++pass) {
+        const int r = pass * 16 + (threadIdx.x >> 4), row = row0 + r;
+        Pair<DT> p[4] = {};
+        if (row < a.rows && col < a.cols) load_pairs<DT>(a.x + (a.row_stride * row + col) * B, a.aligned, a.cols - col, p);
+        if (a.codes) {
+            u32 m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { const u32 k = p[i].magnitude(); m = m > k ? m : k; }
+            const u32 byte = scale_byte(largest_of_quad(m));
+            const u32 w = byte == 255u ? 0u : encode8<DT>(p, scale_value(byte));
+            if (row < a.rows) {
+                *reinterpret_cast<u32*>(a.codes + row * row_bytes + col0 / 2 + piece * 4) = w;
+                if ((piece & 3) == 0) a.scales[row * (row_bytes / 16) + col0 / kMxGroup + piece / 4] = (uint8_t)byte;
+            }
+        }
+        if (a.column_codes) {
+            u32* out = lds + r * kStride + piece * 2 * B;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (B == 2) out[i] = p[i].v; else { out[2 * i] = as_u32(p[i].a); out[2 * i + 1] = as_u32(p[i].b); }
+            }
+        }
+    }
+    if (!a.column_codes) return;
+    __syncthreads();
+    const int64_t column_bytes = (int64_t)((a.rows + kBlock - 1) / kBlock) * (kBlock / 2);
+    const int group = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {   // of the wavefront's columns: even and odd ones, or left and right
+        Pair<DT> p[16];
+        const u32* in = lds + group * 32 * kStride + (B == 2 ? lane : lane + half * 64);
+        u32 m = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const u32 x = in[2 * i * kStride], y = in[(2 * i + 1) * kStride];
+            if constexpr (B == 2) p[i].v = half ? __builtin_amdgcn_perm(y, x, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
+            else { p[i].a = as_f32(x); p[i].b = as_f32(y); }
+            const u32 k = p[i].magnitude();
+            m = m > k ? m : k;
+        }
+        const u32 byte = scale_byte(m);
+        u32x4 w = {0, 0, 0, 0};
+        if (byte != 255u) {
+            const float scale = scale_value(byte);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = encode8<DT>(p + 4 * i, scale);
+        }
+        const int c = col0 + (B == 2 ? lane * 2 + half : lane + half * 64);
+        if (c < a.cols) {
+            *reinterpret_cast<u32x4*>(a.column_codes + c * column_bytes + row0 / 2 + group * 16) = w;
+            a.column_scales[c * (column_bytes / 16) + row0 / kMxGroup + group] = (uint8_t)byte;
+        }
+    }
+}
+
+// Eight values per thread.
+template <int DT> __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, char* out, int rows, int cols, bool aligned) {
+    const int blocks = (cols + kBlock - 1) / kBlock, pieces = (cols + 7) / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = i / pieces;
+    const int piece = (int)(i - row * pieces);
+    if (row >= rows) return;
+    const u32 w = *reinterpret_cast<const u32*>(codes + row * blocks * (kBlock / 2) + piece * 4);
+    const u32 byte = scales[row * blocks * 4 + piece / 4];
+    // the codes' values, then one product with the power of two, exact down to fp32's smallest numbers
+    const float scale = byte == 255u ? __builtin_nanf("") : byte ? as_f32(byte << 23) : as_f32(0x00400000u);
+    float v[8];
+    const f32x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+    const f32x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+    v[0] = v0.x * scale; v[1] = v0.y * scale; v[2] = v1.x * scale; v[3] = v1.y * scale;
+    v[4] = v2.x * scale; v[5] = v2.y * scale; v[6] = v3.x * scale; v[7] = v3.y * scale;
+    constexpr int B = DTypeInfo<DT>::bytes, EPL = 16 / B;
+    const int valid = cols - piece * 8;
+    char* p = out + (row * cols + piece * 8) * B;
+#pragma unroll
+    for (int part = 0; part < 8 / EPL; ++part) {
+        Pack<B, EPL> d;
+#pragma unroll
+        for (int k = 0; k < EPL; k += 2) { float x, y; narrow_pair<DT, EPL>(d, k, v[part * EPL + k], v[part * EPL + k + 1], x, y); }
+        if (aligned && valid >= 8) *reinterpret_cast<u32x4*>(p + part * 16) = u32x4{d.w[0], d.w[1], d.w[2], d.w[3]};
+        else store_guarded<B, EPL>(d, p, part * EPL, valid);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// products
+// ------------------------------------------------------------------------------------------------
+struct ProductArgs {
+    const char *a, *b;                  // codes
+    const uint8_t *a_scales, *b_scales;
+    char* out;
+    int rows, cols, blocks;             // of the result; 128-value blocks of the contracted axis
+    int dtype;
+    bool aligned;                       // 16-byte pieces of the result may be written
+};
+
+struct ProductOut {
+    static constexpr bool kColumns = false;
+    char* out;
+    int rows, cols, dtype;
+    bool aligned;
+    template <int DT> __device__ __forceinline__ void put(int i, int j, const float (&v)[8]) const {
+        constexpr int B = DTypeInfo<DT>::bytes, EPL = 16 / B;
+        char* p = out + ((int64_t)i * cols + j) * B;
+        const int valid = cols - j;
+#pragma unroll
+        for (int part = 0; part < 8 / EPL; ++part) {
+            Pack<B, EPL> d;
+#pragma unroll
+            for (int k = 0; k < EPL; k += 2) { float x, y; narrow_pair<DT, EPL>(d, k, v[part * EPL + k], v[part * EPL + k + 1], x, y); }
+            if (aligned && valid >= 8) *reinterpret_cast<u32x4*>(p + part * 16) = u32x4{d.w[0], d.w[1], d.w[2], d.w[3]};
+            else store_guarded<B, EPL>(d, p, part * EPL, valid);
+        }
+    }
+    __device__ __forceinline__ void row(int i, int j, float (&v)[8]) const {
+        if (i >= rows || j >= cols) return;
+        if (dtype == DT_BF16) put<DT_BF16>(i, j, v);
+        else if (dtype == DT_F16) put<DT_F16>(i, j, v);
+        else put<DT_F32>(i, j, v);
+    }
+    __device__ __forceinline__ void column(int, int, const float (&)[8]) const {}
+};
+
+template <int WT> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2) void mx_product_kernel(ProductArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typedef GemmTile<Mx4Product, WT> Tile;
+    const int rows = (p.rows + Tile::kTile - 1) / Tile::kTile, cols = (p.cols + Tile::kTile - 1) / Tile::kTile;
+    int i, j;
+    tile_at((int)tile_of_workgroup(blockIdx.x, (int64_t)rows * cols), rows, cols, i, j);
+    const int64_t row_bytes = (int64_t)p.blocks * (kBlock / 2);
+    const Operand a{p.a, row_bytes, p.a_scales, row_bytes / 16, p.rows}, b{p.b, row_bytes, p.b_scales, row_bytes / 16, p.cols};
+    Tile tile(smem);
+    tile.multiply(a, b, i * Tile::kTile, j * Tile::kTile, (int)row_bytes);
+    ProductOut out{p.out, p.rows, p.cols, p.dtype, p.aligned};
+    tile.finish(i * Tile::kTile, j * Tile::kTile, out);
+}
+
+// Few rows against many: `tokens` <= 16 TILES rows of x, a weight of `cols` rows.  Bound by the weight's bytes.  A workgroup takes 16
+// weight rows, its eight wavefronts take turns along the contracted axis, 256 values at a time, straight from memory into
+// the operand registers of 16x16x128 instructions (weight rows as their rows, tokens as their columns), and add up through
+// LDS at the end.  x comes as codes, or, with RAW, as values of type DT that every wavefront quantises as it needs them: a
+// lane's operand is one group, so the scale never leaves the lane.
+struct TokensArgs {
+    const char* x;                 // codes, or values
+    const uint8_t* x_scales;
+    const char* weight;
+    const uint8_t* weight_scales;
+    char* out;
+    int tokens, cols, inner, blocks;
+    int64_t x_stride;              // RAW: elements between rows
+    bool x_aligned;
+    int dtype;                     // of the result
+};
+constexpr int kTokenWaves = 8;
+
+template <int DT, bool RAW, int TILES> __global__ __launch_bounds__(64 * kTokenWaves) void mx_tokens_kernel(TokensArgs p) {
+    __shared__ f32x4 sums[kTokenWaves][TILES][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int line = lane & 15, group = lane >> 4;
+    const int row = blockIdx.x * 16 + line < p.cols ? blockIdx.x * 16 + line : p.cols - 1;   // past the last: copies, not stored
+    const char* w = p.weight + (int64_t)row * p.blocks * 64 + group * 16;
+    const uint8_t* ws = p.weight_scales + (int64_t)row * p.blocks * 4 + group;
+    f32x4 acc[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int first = wave * 2; first < p.blocks; first += kTokenWaves * 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int block = first + u;
+            if (block >= p.blocks) break;
+            const i32x4 wv = *reinterpret_cast<const i32x4*>(w + block * 64);
+            const int wscale = ws[block * 4];
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                const int token = t * 16 + line;
+                i32x4 xv = {0, 0, 0, 0};
+                int xscale = 127;
+                if (token < p.tokens) {
+                    if constexpr (RAW) {
+                        const int at = block * kBlock + group * kMxGroup;
+                        Pair<DT> v[16];
+                        u32 m = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            Pair<DT> q[4] = {};
+                            if (at + i * 8 < p.inner)
+                                load_pairs<DT>(p.x + (p.x_stride * token + at + i * 8) * DTypeInfo<DT>::bytes, p.x_aligned, p.inner - at - i * 8, q);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) { v[i * 4 + e] = q[e]; const u32 k = q[e].magnitude(); m = m > k ? m : k; }
+                        }
+                        const u32 byte = scale_byte(m);
+                        xscale = (int)byte;
+                        if (byte != 255u) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) xv[i] = (int)encode8<DT>(v + 4 * i, scale_value(byte));
+                        }
+                    } else {
+                        xv = *reinterpret_cast<const i32x4*>(p.x + ((int64_t)token * p.blocks + block) * 64 + group * 16);
+                        xscale = p.x_scales[((int64_t)token * p.blocks + block) * 4 + group];
+                    }
+                }
+                const i32x8 va = {wv.x, wv.y, wv.z, wv.w, 0, 0, 0, 0}, vb = {xv.x, xv.y, xv.z, xv.w, 0, 0, 0, 0};
+                acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, acc[t], 4, 4, 0, wscale, 0, xscale);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) sums[wave][t][lane] = acc[t];
+    __syncthreads();
+    for (int k = threadIdx.x; k < TILES * 64; k += 64 * kTokenWaves) {
+        f32x4 v = sums[0][k >> 6][k & 63];
+#pragma unroll
+        for (int s = 1; s < kTokenWaves; ++s) v += sums[s][k >> 6][k & 63];
+        const int token = (k >> 6) * 16 + (k & 15), col = blockIdx.x * 16 + (k >> 4 & 3) * 4;
+        if (token >= p.tokens) continue;
+        const int64_t at = (int64_t)token * p.cols + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (col + e >= p.cols) break;
+            if (p.dtype == DT_BF16) reinterpret_cast<__bf16*>(p.out)[at + e] = (__bf16)v[e];
+            else if (p.dtype == DT_F16) reinterpret_cast<_Float16*>(p.out)[at + e] = (_Float16)v[e];
+            else reinterpret_cast<float*>(p.out)[at + e] = v[e];
+        }
+    }
+}
+
+}  // namespace fo
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+namespace {
+using namespace fo_host;
+
+constexpr int64_t kMostWorkgroups = 1 << 22;
+constexpr int64_t kMostLines = INT32_MAX - 255;
+
+int validate_matrix(const char* what, int64_t rows, int64_t cols, int dtype) {
+    if (rows < 0 || cols < 0) return fail(FO_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+    if (rows > kMostLines || cols > kMostLines) return fail(FO_ERR_UNSUPPORTED, "%s: %lld x %lld is too large", what, (long long)rows, (long long)cols);
+    if (dtype < FO_F32 || dtype > FO_F16) return fail(FO_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+    return 0;
+}
+
+// What the lanes' 32-bit offsets into a tile's rows reach.
+int validate_inner(const char* what, int64_t inner) {
+    if (inner == 0) return fail(FO_ERR_UNSUPPORTED, "%s: nothing to contract over", what);
+    if (inner > 1 << 24) return fail(FO_ERR_UNSUPPORTED, "%s: rows of %lld values are too long", what, (long long)inner);
+    return 0;
+}
+
+int64_t blocks_of(int64_t n) { return (n + fo::kBlock - 1) / fo::kBlock; }
+
+template <class K, class... Args> int launch(K kernel, int64_t grid, int threads, int lds, void* stream, const char* what, Args... args) {
+    if (grid > kMostWorkgroups) return fail(FO_ERR_UNSUPPORTED, "%s: %lld workgroups are more than one launch takes", what, (long long)grid);
+    if (lds > 65536) {
+        if (int rc = check_hip(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds), what)) return rc;
+    }
+    kernel<<<dim3((unsigned)grid), dim3(threads), lds, (hipStream_t)stream>>>(args...);
+    return check_hip(hipGetLastError(), what);
+}
+
+template <int DT> int launch_quantize(const fo::QuantizeArgs& a, int64_t grid, void* stream) {
+    const int lds = a.column_codes ? fo::kBlock * (fo::kBlock * fo::DTypeInfo<DT>::bytes / 4 + 1) * 4 : 0;
+    return launch(fo::mx_quantize_kernel<DT>, grid, 256, lds, stream, "fo_mxfp4_quantize", a);
+}
+
+template <int DT, bool RAW> int launch_tokens(const fo::TokensArgs& p, void* stream) {
+    const int64_t grid = (p.cols + 15) / 16;
+    const char* what = "fo_mxfp4_product";
+    if (RAW || p.tokens <= 16) return launch(fo::mx_tokens_kernel<DT, RAW, 1>, grid, 64 * fo::kTokenWaves, 0, stream, what, p);
+    if (p.tokens <= 32) return launch(fo::mx_tokens_kernel<DT, RAW, RAW ? 1 : 2>, grid, 64 * fo::kTokenWaves, 0, stream, what, p);
+    return launch(fo::mx_tokens_kernel<DT, RAW, RAW ? 1 : 4>, grid, 64 * fo::kTokenWaves, 0, stream, what, p);
+}
+
+int64_t tiles(int64_t rows, int64_t cols, int tile) { return ((rows + tile - 1) / tile) * ((cols + tile - 1) / tile); }
+
+}  // namespace
+
+extern "C" {
+int fo_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void* codes, void* scales,
+                      void* column_codes, void* column_scales, void* stream) {
+    if (int rc = validate_matrix("fo_mxfp4_quantize", rows, cols, dtype)) return rc;
+    if (!codes != !scales || !column_codes != !column_scales || (!codes && !column_codes))
+        return fail(FO_ERR_INVALID_ARGUMENT, "codes and scales of the rows, of the columns or of both must be given");
+    if (rows == 0 || cols == 0) return 0;
+    if (!x) return fail(FO_ERR_INVALID_ARGUMENT, "x must not be NULL");
+    if (((uintptr_t)codes | (uintptr_t)column_codes) & 15) return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes");
+    const int width = dtype == FO_F32 ? 4 : 2;
+    const bool aligned = (((uintptr_t)x | (uintptr_t)(row_stride * width)) & 15) == 0;
+    const fo::QuantizeArgs a{(const char*)x, row_stride, (int)rows, (int)cols, aligned, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)column_codes, (uint8_t*)column_scales};
+    const int64_t grid = blocks_of(rows) * blocks_of(cols);
+    switch (dtype) {
+        case FO_F32: return launch_quantize<fo::DT_F32>(a, grid, stream);
+        case FO_BF16: return launch_quantize<fo::DT_BF16>(a, grid, stream);
+        default: return launch_quantize<fo::DT_F16>(a, grid, stream);
+    }
+}
+
+int fo_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype, void* stream) {
+    if (int rc = validate_matrix("fo_mxfp4_dequantize", rows, cols, dtype)) return rc;
+    if (rows == 0 || cols == 0) return 0;
+    if (!codes || !scales || !out) return fail(FO_ERR_INVALID_ARGUMENT, "codes, scales and out must not be NULL");
+    if ((uintptr_t)codes & 3) return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 4 bytes");
+    const int width = dtype == FO_F32 ? 4 : 2;
+    const bool aligned = ((uintptr_t)out & 15) == 0 && cols * width % 16 == 0;
+    const int64_t grid = (rows * ((cols + 7) / 8) + 255) / 256;
+    const char* what = "fo_mxfp4_dequantize";
+    switch (dtype) {
+        case FO_F32: return launch(fo::mx_dequantize_kernel<fo::DT_F32>, grid, 256, 0, stream, what, (const uint8_t*)codes, (const uint8_t*)scales, (char*)out, (int)rows, (int)cols, aligned);
+        case FO_BF16: return launch(fo::mx_dequantize_kernel<fo::DT_BF16>, grid, 256, 0, stream, what, (const uint8_t*)codes, (const uint8_t*)scales, (char*)out, (int)rows, (int)cols, aligned);
+        default: return launch(fo::mx_dequantize_kernel<fo::DT_F16>, grid, 256, 0, stream, what, (const uint8_t*)codes, (const uint8_t*)scales, (char*)out, (int)rows, (int)cols, aligned);
+    }
+}
+
+int fo_mxfp4_product(const void* a, const void* a_scales, int64_t rows, const void* b, const void* b_scales, int64_t cols, int64_t inner,
+                     void* out, int dtype, void* stream) {
+    if (int rc = validate_matrix("fo_mxfp4_product", rows, cols, dtype)) return rc;
+    if (int rc = validate_matrix("fo_mxfp4_product", rows, inner, dtype)) return rc;
+    if (rows == 0 || cols == 0) return 0;
+    if (int rc = validate_inner("fo_mxfp4_product", inner)) return rc;
+    if (!a || !a_scales || !b || !b_scales || !out) return fail(FO_ERR_INVALID_ARGUMENT, "operands and out must not be NULL");
+    if (((uintptr_t)a | (uintptr_t)b) & 15 || ((uintptr_t)a_scales | (uintptr_t)b_scales) & 3)
+        return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes, scales to 4");
+    const int width = dtype == FO_F32 ? 4 : 2;
+    const int64_t blocks = blocks_of(inner);
+    if (rows <= 64) {
+        const fo::TokensArgs p{(const char*)a, (const uint8_t*)a_scales, (const char*)b, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)inner, (int)blocks, 0, false, dtype};
+        return launch_tokens<fo::DT_BF16, false>(p, stream);
+    }
+    const bool aligned = ((uintptr_t)out & 15) == 0 && cols * width % 16 == 0;
+    const fo::ProductArgs p{(const char*)a, (const char*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)blocks, dtype, aligned};
+    const int cus = compute_units();
+    if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
+    const char* what = "fo_mxfp4_product";
+    if (tiles(rows, cols, 256) >= cus)
+        return launch(fo::mx_product_kernel<128>, tiles(rows, cols, 256), 256, fo::GemmTile<fo::Mx4Product, 128>::kLds, stream, what, p);
+    if (tiles(rows, cols, 128) >= cus)
+        return launch(fo::mx_product_kernel<64>, tiles(rows, cols, 128), 256, fo::GemmTile<fo::Mx4Product, 64>::kLds, stream, what, p);
+    return launch(fo::mx_product_kernel<32>, tiles(rows, cols, 64), 256, fo::GemmTile<fo::Mx4Product, 32>::kLds, stream, what, p);
+}
+
+int fo_mxfp4_tokens(const void* x, int x_dtype, int64_t tokens, int64_t row_stride, const void* weight, const void* weight_scales, int64_t cols,
+                    int64_t inner, void* out, int dtype, void* stream) {
+    if (int rc = validate_matrix("fo_mxfp4_tokens", tokens, cols, dtype)) return rc;
+    if (int rc = validate_matrix("fo_mxfp4_tokens", tokens, inner, x_dtype)) return rc;
+    if (tokens > FO_MXFP4_MOST_TOKENS) return fail(FO_ERR_UNSUPPORTED, "fo_mxfp4_tokens takes at most %d rows, not %lld", FO_MXFP4_MOST_TOKENS, (long long)tokens);
+    if (tokens == 0 || cols == 0) return 0;
+    if (int rc = validate_inner("fo_mxfp4_tokens", inner)) return rc;
+    if (!x || !weight || !weight_scales || !out) return fail(FO_ERR_INVALID_ARGUMENT, "operands and out must not be NULL");
+    if ((uintptr_t)weight & 15) return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes");
+    const int width = x_dtype == FO_F32 ? 4 : 2;
+    const bool aligned = (((uintptr_t)x | (uintptr_t)(row_stride * width)) & 15) == 0;
+    const fo::TokensArgs p{(const char*)x, nullptr, (const char*)weight, (const uint8_t*)weight_scales, (char*)out, (int)tokens, (int)cols, (int)inner, (int)blocks_of(inner), row_stride, aligned, dtype};
+    switch (x_dtype) {
+        case FO_F32: return launch_tokens<fo::DT_F32, true>(p, stream);
+        case FO_BF16: return launch_tokens<fo::DT_BF16, true>(p, stream);
+        default: return launch_tokens<fo::DT_F16, true>(p, stream);
+    }
+}
+}  // extern "C"

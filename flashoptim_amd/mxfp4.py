@@ -1,0 +1,266 @@
+"""Microscaled 4-bit floating point (MXFP4): quantiser, products, and a linear layer that trains and serves in it.
+
+32 values share one power of two and are E2M1 codes each: 17/32 bytes a value, and the matrix cores multiply them at four times
+the bfloat16 rate.  The reference package has nothing of the kind; the format is that of the OCP microscaling specification.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Union
+
+import torch
+
+from . import _native, kernels
+from ._native import DTYPE_CODE
+
+GROUP_SIZE = 32
+BLOCK = 128  # rows are filled up to multiples of it
+_MOST_TOKENS = 16  # FO_MXFP4_MOST_TOKENS
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+class MXFP4Tensor:
+    """A ``rows x cols`` matrix in MXFP4, its rows cut into groups of 32.
+
+    Args:
+        codes: uint8 ``(rows, 64 * ceil(cols / 128))``, contiguous: two E2M1 codes a byte (sign, two exponent bits, one
+            mantissa bit), the first in the low half; zero beyond `cols`.
+        scales: uint8 ``(rows, 4 * ceil(cols / 128))``, contiguous: the power of two of 32 values, plus 127; 255 for a group
+            that held an infinity or a NaN.
+        shape: ``(rows, cols)``.
+    """
+
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape):
+        rows, cols = shape
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise ValueError(f"codes and scales must be uint8, got {codes.dtype} and {scales.dtype}.")
+        if rows < 0 or cols < 0 or tuple(codes.shape) != (rows, 64 * _blocks(cols)) or tuple(scales.shape) != (rows, 4 * _blocks(cols)):
+            raise ValueError(
+                f"a {rows} x {cols} matrix has codes of shape {(rows, 64 * _blocks(cols))} and scales of shape "
+                f"{(rows, 4 * _blocks(cols))}, got {tuple(codes.shape)} and {tuple(scales.shape)}.")
+        if not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError("codes and scales must be contiguous")
+        kernels._require_same_device(codes, scales, "scales")
+        self.codes, self.scales, self.shape = codes, scales, (int(rows), int(cols))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def to(self, device) -> "MXFP4Tensor":
+        return MXFP4Tensor(self.codes.to(device), self.scales.to(device), self.shape)
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        return mxfp4_dequantize(self, dtype)
+
+    def __repr__(self) -> str:
+        return f"MXFP4Tensor(shape={self.shape}, device={self.device})"
+
+
+def _check_matrix(x: torch.Tensor, what: str) -> torch.Tensor:
+    kernels._require_device(x, what)
+    if x.dtype not in DTYPE_CODE:
+        raise ValueError(f"{what} expects fp32, bf16 or fp16 input, got {x.dtype}.")
+    if x.dim() != 2:
+        raise ValueError(f"{what} expects a matrix, got shape {tuple(x.shape)}.")
+    x = x.detach()
+    return x.resolve_neg() if x.is_neg() else x
+
+
+def _empty(rows: int, cols: int, device: torch.device) -> MXFP4Tensor:
+    codes = torch.empty((rows, 64 * _blocks(cols)), dtype=torch.uint8, device=device)
+    scales = torch.empty((rows, 4 * _blocks(cols)), dtype=torch.uint8, device=device)
+    return MXFP4Tensor(codes, scales, (rows, cols))
+
+
+def _quantize(x: torch.Tensor, rows: bool, columns: bool) -> tuple[Optional[MXFP4Tensor], Optional[MXFP4Tensor]]:
+    """The row forms of `x` and of its transpose, as asked for, from one read."""
+    r, c = x.shape
+    if x.stride(1) != 1 and c > 1:
+        if x.stride(0) == 1 or r == 1:  # the transpose's rows are what is contiguous
+            columns_out, rows_out = _quantize(x.t(), columns, rows)
+            return rows_out, columns_out
+        x = x.contiguous()
+    by_row = _empty(r, c, x.device) if rows else None
+    by_column = _empty(c, r, x.device) if columns else None
+    if x.numel() > 0:
+        ptr = [None if t is None else getattr(t, k).data_ptr() for t in (by_row, by_column) for k in ("codes", "scales")]
+        with _native.device_guard(x.device):
+            rc = _native.lib().fo_mxfp4_quantize(x.data_ptr(), DTYPE_CODE[x.dtype], r, c, x.stride(0), *ptr,
+                                                 _native.current_stream_ptr(x.device))
+        _native.check(rc, "fo_mxfp4_quantize")
+    return by_row, by_column
+
+
+def mxfp4_quantize(x: torch.Tensor, transpose: bool = False) -> MXFP4Tensor:
+    """The matrix `x` (fp32, bf16 or fp16, any strides), or its transpose, in MXFP4.
+
+    The scale of a group is the power of two of its largest magnitude, over 4; values are rounded to the nearest code,
+    ties to the even one, and cut off at 6 times the scale.  A group with an infinity or a NaN comes back as NaNs.
+    """
+    rows, columns = _quantize(_check_matrix(x, "mxfp4_quantize"), not transpose, transpose)
+    return columns if transpose else rows
+
+
+def mxfp4_quantize_both(x: torch.Tensor) -> tuple[MXFP4Tensor, MXFP4Tensor]:
+    """``(mxfp4_quantize(x), mxfp4_quantize(x, transpose=True))`` from one read of `x`."""
+    return _quantize(_check_matrix(x, "mxfp4_quantize_both"), True, True)
+
+
+def mxfp4_dequantize(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that `q` stands for, as a matrix of `dtype` (fp32, bf16 or fp16).  bf16 and fp32 hold them exactly."""
+    if not isinstance(q, MXFP4Tensor):
+        raise ValueError(f"mxfp4_dequantize expects an MXFP4Tensor, got {type(q)}.")
+    if dtype not in DTYPE_CODE:
+        raise ValueError(f"Unsupported dtype {dtype}.")
+    kernels._require_device(q.codes, "mxfp4_dequantize")
+    rows, cols = q.shape
+    out = torch.empty((rows, cols), dtype=dtype, device=q.device)
+    if out.numel() > 0:
+        with _native.device_guard(q.device):
+            rc = _native.lib().fo_mxfp4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, out.data_ptr(),
+                                                   DTYPE_CODE[dtype], _native.current_stream_ptr(q.device))
+        _native.check(rc, "fo_mxfp4_dequantize")
+    return out
+
+
+def mxfp4_matmul(a: Union[MXFP4Tensor, torch.Tensor], b: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``a @ b.T`` of an ``m x k`` and an ``n x k`` matrix in MXFP4, summed in fp32, as an ``m x n`` matrix of `dtype`.
+
+    `a` may be a plain matrix: it is quantised on the way, for up to 16 rows within the product's own kernel.
+    """
+    if not isinstance(b, MXFP4Tensor):
+        raise ValueError(f"mxfp4_matmul expects its second operand as an MXFP4Tensor, got {type(b)}.")
+    if dtype not in DTYPE_CODE:
+        raise ValueError(f"Unsupported dtype {dtype}.")
+    plain = not isinstance(a, MXFP4Tensor)
+    if plain:
+        a = _check_matrix(a, "mxfp4_matmul")
+    kernels._require_device(b.codes, "mxfp4_matmul")
+    if a.device != b.device:
+        raise ValueError(f"b is on {b.device}, expected {a.device}.")
+    (m, k), n = a.shape, b.shape[0]
+    if b.shape[1] != k:
+        raise ValueError(f"operands of shapes {tuple(a.shape)} and {tuple(b.shape)} do not contract over one length")
+    if k == 0:
+        return torch.zeros((m, n), dtype=dtype, device=b.device)
+    out = torch.empty((m, n), dtype=dtype, device=b.device)
+    if out.numel() == 0:
+        return out
+    tokens = plain and m <= _MOST_TOKENS
+    if tokens and a.stride(1) != 1 and k > 1:
+        a = a.contiguous()
+    elif plain and not tokens:
+        a = _quantize(a, True, False)[0]
+    with _native.device_guard(b.device):
+        stream = _native.current_stream_ptr(b.device)
+        if tokens:
+            rc = _native.lib().fo_mxfp4_tokens(a.data_ptr(), DTYPE_CODE[a.dtype], m, a.stride(0), b.codes.data_ptr(), b.scales.data_ptr(),
+                                               n, k, out.data_ptr(), DTYPE_CODE[dtype], stream)
+        else:
+            rc = _native.lib().fo_mxfp4_product(a.codes.data_ptr(), a.scales.data_ptr(), m, b.codes.data_ptr(), b.scales.data_ptr(),
+                                                n, k, out.data_ptr(), DTYPE_CODE[dtype], stream)
+    _native.check(rc, "fo_mxfp4_tokens" if tokens else "fo_mxfp4_product")
+    return out
+
+
+class _Linear(torch.autograd.Function):
+    """x (tokens, in) and weight (out, in) to x weight', every product on MXFP4 forms of its operands along the contracted axis.
+
+    What the backward pass needs of x and of the weight is their column forms, 17/32 bytes a value, made in the same read
+    as the row forms; x itself is not kept.
+    """
+
+    @staticmethod
+    def forward(ctx, x, weight):
+        need_dx, need_dw = ctx.needs_input_grad
+        ctx.dtypes, ctx.shapes = (x.dtype, weight.dtype), (x.shape, weight.shape)
+        x, weight = _check_matrix(x, "mxfp4_linear"), _check_matrix(weight, "mxfp4_linear")
+        if need_dw or x.shape[0] > _MOST_TOKENS:
+            xr, xc = _quantize(x, True, need_dw)
+        else:
+            xr, xc = x, None
+        wr, wc = _quantize(weight, True, need_dx)
+        saved = [t for q in (xc, wc) if q is not None for t in (q.codes, q.scales)]
+        ctx.save_for_backward(*saved)
+        return mxfp4_matmul(xr, wr, x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        need_dx, need_dw = ctx.needs_input_grad
+        (tokens, inner), (outer, _) = ctx.shapes
+        saved = list(ctx.saved_tensors)
+        xc = MXFP4Tensor(saved.pop(0), saved.pop(0), (inner, tokens)) if need_dw else None
+        wc = MXFP4Tensor(saved.pop(0), saved.pop(0), (inner, outer)) if need_dx else None
+        dy = _check_matrix(dy, "mxfp4_linear backward")
+        by_row, by_column = _quantize(dy, need_dx, need_dw)
+        dx = mxfp4_matmul(by_row, wc, ctx.dtypes[0]) if need_dx else None
+        dw = mxfp4_matmul(by_column, xc, ctx.dtypes[1]) if need_dw else None
+        return dx, dw
+
+
+class _FrozenLinear(torch.autograd.Function):
+    """The same with a weight that is held in MXFP4 and not trained."""
+
+    @staticmethod
+    def forward(ctx, x, codes, scales, shape):
+        ctx.dtype, ctx.shape = x.dtype, shape
+        ctx.save_for_backward(codes, scales)
+        return mxfp4_matmul(x, MXFP4Tensor(codes, scales, shape), x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        weight = MXFP4Tensor(*ctx.saved_tensors, ctx.shape)
+        # the scales have to run along the other axis now; bf16 holds the weight's values
+        columns = mxfp4_quantize(mxfp4_dequantize(weight), transpose=True)
+        return mxfp4_matmul(dy, columns, ctx.dtype), None, None, None
+
+
+def mxfp4_linear(x: torch.Tensor, weight: Union[torch.Tensor, MXFP4Tensor]) -> torch.Tensor:
+    """``x @ weight.T`` in MXFP4, with gradients.
+
+    Args:
+        x: ``(..., in)`` in fp32, bf16 or fp16.
+        weight: ``(out, in)``; a tensor is quantised in the call and receives a gradient, an :class:`MXFP4Tensor` is frozen.
+
+    Returns:
+        ``(..., out)`` in the type of `x`.
+
+    Each of the three products of a training step contracts over another axis, so each operand is quantised along two:
+
+        y = Q(x) Q(w)',    dx = Q(dy) Q(w')',    dw = Q(dy') Q(x')'
+
+    with Q along rows; the quantisation itself counts as the identity in the backward pass.
+    """
+    inner = weight.shape[-1]
+    if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] != inner:
+        raise ValueError(f"mxfp4_linear: input of shape {tuple(x.shape)} does not fit a weight of shape {tuple(weight.shape)}")
+    if weight.device != x.device:
+        raise ValueError(f"weight is on {weight.device}, expected {x.device}.")
+    tokens = x.reshape(-1, inner) if inner else x.reshape(x.shape[:-1].numel(), 0)
+    if isinstance(weight, MXFP4Tensor):
+        if torch.is_grad_enabled() and x.requires_grad:
+            y = _FrozenLinear.apply(tokens, weight.codes, weight.scales, weight.shape)
+        else:
+            y = mxfp4_matmul(tokens, weight, x.dtype)
+    else:
+        if weight.dim() != 2:
+            raise ValueError(f"mxfp4_linear expects a matrix as weight, got shape {tuple(weight.shape)}.")
+        y = _Linear.apply(tokens, weight)
+    return y.reshape(*x.shape[:-1], weight.shape[0])
+
+
+class MXFP4Linear(torch.nn.Linear):
+    """``torch.nn.Linear`` whose three products run in MXFP4 (:func:`mxfp4_linear`); the weight keeps its type, so the optimizers of
+    this package hold masters and correction bits for it as for any other.  A bias is added in the output's type."""
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        y = mxfp4_linear(input, self.weight)
+        return y if self.bias is None else y + self.bias

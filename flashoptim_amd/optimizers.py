@@ -20,6 +20,15 @@ from .kernels import (
 )
 from .lion import FlashLion
 from .muon import FlashMuon, newton_schulz
+from .mxfp4 import (
+    MXFP4Linear,
+    MXFP4Tensor,
+    mxfp4_dequantize,
+    mxfp4_linear,
+    mxfp4_matmul,
+    mxfp4_quantize,
+    mxfp4_quantize_both,
+)
 from .release import GradientReleaseHandle, enable_gradient_release
 from .sgd import FlashSGD, FlashSGDW
 from .state import QuantizedTensorSpec, _MaybeQuantizedTensor
@@ -34,9 +43,16 @@ __all__ = [
     "FlashAdam",
     "FlashAdamW",
     "GradientReleaseHandle",
+    "MXFP4Linear",
+    "MXFP4Tensor",
     "cast_model",
     "compute_ecc_bits",
     "enable_gradient_release",
+    "mxfp4_dequantize",
+    "mxfp4_linear",
+    "mxfp4_matmul",
+    "mxfp4_quantize",
+    "mxfp4_quantize_both",
     "newton_schulz",
     "reconstruct_fp32_param",
 ]

@@ -264,6 +264,30 @@ int fo_muon_step(const fo_tensor_desc *matrices, const fo_matrix_shape *shapes, 
                  int quantized, float keep, float momentum_coef, int nesterov, int steps, const float *coefficients, float eps,
                  void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * Microscaled 4-bit floating point (MXFP4, no counterpart in the reference).  A row of `cols` values is stored as
+ * 64 * ceil(cols / 128) bytes of E2M1 codes, two to a byte, the first in the low half, and 4 * ceil(cols / 128) E8M0 scale
+ * bytes, one per 32 values; zeros fill it up.  Scale: floor(log2(largest magnitude)) - 2, codes rounded to nearest even, magnitudes
+ * above 6 become 6; a group with an infinity or a NaN has scale byte 255.  Codes are aligned to 16 bytes, scales of a product to 4.
+ */
+
+/* x: rows x cols of `dtype`, rows `row_stride` elements apart, columns adjacent.  codes, scales: of the rows; column_codes,
+ * column_scales: of the transpose (cols rows of `rows` values).  Either pair may be NULL. */
+int fo_mxfp4_quantize(const void *x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void *codes, void *scales,
+                      void *column_codes, void *column_scales, void *stream);
+
+/* out: rows x cols of `dtype`, contiguous */
+int fo_mxfp4_dequantize(const void *codes, const void *scales, int64_t rows, int64_t cols, void *out, int dtype, void *stream);
+
+/* out[i][j] = sum over `inner` values of a[i] * b[j], summed in fp32; out: rows x cols of `dtype`, contiguous */
+int fo_mxfp4_product(const void *a, const void *a_scales, int64_t rows, const void *b, const void *b_scales, int64_t cols, int64_t inner,
+                     void *out, int dtype, void *stream);
+
+/* The same for up to FO_MXFP4_MOST_TOKENS rows that are not quantised yet: one launch quantises and multiplies them */
+#define FO_MXFP4_MOST_TOKENS 16
+int fo_mxfp4_tokens(const void *x, int x_dtype, int64_t tokens, int64_t row_stride, const void *weight, const void *weight_scales,
+                    int64_t cols, int64_t inner, void *out, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
