@@ -4,8 +4,8 @@
 // instruction only: either way a lane's operand of one 16x16 instruction is 16 bytes of one row, so a tile is rows of
 // bytes and the same staging serves both.
 //
-// Shape.  A workgroup is four wavefronts in a 2x2 arrangement; a wavefront owns a WT x WT piece of the tile (WT = 128, 64
-// or 32) and keeps it in its accumulators.  The operands pass through LDS in stages of 128 bytes of every row (64 fp16
+// Shape.  A workgroup is four wavefronts in a 2x2 arrangement; a wavefront owns a WT x WT piece of the tile (WT = 128, 96,
+// 64 or 32) and keeps it in its accumulators.  The operands pass through LDS in stages of 128 bytes of every row (64 fp16
 // values, 256 codes), two stages in turn.  With WT = 128 the workgroup holds 128 KiB of LDS, a wavefront 256 accumulator
 // registers and both halves of a stage's operands in registers, and one wavefront runs on each SIMD: every LDS byte read is
 // used for eight instructions, which is what keeps LDS (128 bytes a clock) behind the matrix cores.
@@ -248,29 +248,43 @@ template <class Product, int WT> struct GemmTile {
     }
 
     // ------------------------------------------------------------------------------------------- epilogue
-    // Hands the tile to `out` row by row: out.row(i, j, v) gets v[0..7] = C[i][j .. j+7] (i, j counted in the whole result, j
-    // a multiple of 8) and, with out.kColumns, leaves in v what out.column(i, j, w) then gets column by column: w[0..7] =
-    // rows i .. i+7 of column j.  Consecutive lanes get consecutive pieces of a row (of eight rows of a column).
+    // Hands the tile to `out` row by row: out.row(i, j, in, v) gets v[0..7] = C[i][j .. j+7] (i, j counted in the whole result, j
+    // a multiple of 8 and the same for all rows that a lane gets, said before by out.begin(j)) and, with out.kColumns,
+    // leaves in v what out.column(i, j, w) then gets column by column: w[0..7] = rows i .. i+7 of column j.  Consecutive lanes get
+    // consecutive pieces of a row (of eight rows of a column).  What out reads from memory for a row it reads in
+    // out.load(i, j, in), called a strip ahead.
     template <class Out> __device__ __forceinline__ void finish(int row0, int col0, Out& out) {
         float* strip = reinterpret_cast<float*>(smem + wave * kStripBytes);
         constexpr int kPieces = WT / 8;              // 8-value pieces of a row
-        constexpr int kRowsAtOnce = 64 / kPieces;
+        constexpr int kRowsAtOnce = 64 / kPieces;    // WT = 96: five rows, four lanes sit out
+        constexpr int kPasses = (32 + kRowsAtOnce - 1) / kRowsAtOnce;
+        constexpr int kStrips = WT / 32;
         const int r0 = row0 + (wave >> 1) * WT, c0 = col0 + (wave & 1) * WT;
+        const int first = lane / kPieces, piece = lane % kPieces * 8;
+        const bool idle = first >= kRowsAtOnce;
+        typename Out::In in[kPasses];
+        out.begin(c0 + piece);
 #pragma unroll
-        for (int s = 0; s < WT / 32; ++s) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < kFrags; ++j)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        strip[(h * 16 + (lane >> 4) * 4 + k) * kStripStride + j * 16 + (lane & 15)] = acc[2 * s + h][j][k];
+        for (int k = 0; k < kPasses; ++k)
+            if (!idle && first + k * kRowsAtOnce < 32) out.load(r0 + first + k * kRowsAtOnce, c0 + piece, in[k]);
+#pragma unroll 1
+        for (int s = 0; s < kStrips; ++s) {
+            // the accumulators are named registers: one copy of this part for each strip, one of the rest
+            if (s == 0) lay_out<0>(strip);
+            else if (s == 1) lay_out<1>(strip);
+            else if (s == 2) lay_out<2>(strip);
+            else lay_out<3>(strip);
             same_wave();
-            for (int r = lane / kPieces; r < 32; r += kRowsAtOnce) {
-                f32x4* p = reinterpret_cast<f32x4*>(strip + r * kStripStride + (lane % kPieces) * 8);
+#pragma unroll
+            for (int k = 0; k < kPasses; ++k) {
+                const int r = first + k * kRowsAtOnce;
+                if (idle || r >= 32) continue;
+                f32x4* p = reinterpret_cast<f32x4*>(strip + r * kStripStride + piece);
                 const f32x4 lo = p[0], hi = p[1];
                 float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                out.row(r0 + s * 32 + r, c0 + (lane % kPieces) * 8, v);
+                const typename Out::In now = in[k];
+                if (s + 1 < kStrips) out.load(r0 + (s + 1) * 32 + r, c0 + piece, in[k]);
+                out.row(r0 + s * 32 + r, c0 + piece, now, v);
                 if constexpr (Out::kColumns) {
                     p[0] = f32x4{v[0], v[1], v[2], v[3]};
                     p[1] = f32x4{v[4], v[5], v[6], v[7]};
@@ -278,15 +292,28 @@ template <class Product, int WT> struct GemmTile {
             }
             if constexpr (Out::kColumns) {
                 same_wave();
-                for (int k = lane; k < WT * 4; k += 64) {
-                    const int col = k >> 2, rows = (k & 3) * 8;
-                    float w[8];
+                if (out.columns()) {
+                    for (int k = lane; k < WT * 4; k += 64) {
+                        const int col = k >> 2, rows = (k & 3) * 8;
+                        float w[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = strip[(rows + e) * kStripStride + col];
-                    out.column(r0 + s * 32 + rows, c0 + col, w);
+                        for (int e = 0; e < 8; ++e) w[e] = strip[(rows + e) * kStripStride + col];
+                        out.column(r0 + s * 32 + rows, c0 + col, w);
+                    }
                 }
             }
             same_wave();
+        }
+    }
+    template <int S> __device__ __forceinline__ void lay_out(float* strip) const {
+        if constexpr (S < WT / 32) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < kFrags; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        strip[(h * 16 + (lane >> 4) * 4 + k) * kStripStride + j * 16 + (lane & 15)] = acc[2 * S + h][j][k];
         }
     }
     // A wavefront's LDS accesses take effect in order; this keeps the compiler from reordering them.
@@ -298,9 +325,13 @@ template <class Product, int WT> struct GemmTile {
 
 // ------------------------------------------------------------------------------------------- which tile a workgroup takes
 // Workgroup b runs on accelerator die b % 8, each with an L2 of its own: every die takes a contiguous run of the tiles.
-__device__ __forceinline__ int64_t tile_of_workgroup(int64_t b, int64_t tiles) {
-    const int64_t per = tiles >> 3, rest = tiles & 7, die = b & 7;
-    return die * per + (die < rest ? die : rest) + (b >> 3);
+// `seat` is the workgroup's place among its die's; a grid has 8 * seats_of(tiles) workgroups, up to seven of them without a
+// tile (negative).
+__host__ __device__ __forceinline__ int64_t seats_of(int64_t tiles) { return (tiles + 7) >> 3; }
+__device__ __forceinline__ int64_t tile_of_seat(int die, int64_t seat, int64_t tiles) {
+    const int64_t per = tiles >> 3, rest = tiles & 7;
+    if (seat >= per + (die < rest ? 1 : 0)) return -1;
+    return die * per + (die < rest ? die : rest) + seat;
 }
 // Tile t of a result of `rows` x `cols` tiles, in bands of four rows, column by column: 32 consecutive tiles (a die's
 // compute units) share twelve operand panels.

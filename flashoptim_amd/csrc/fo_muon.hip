@@ -25,6 +25,9 @@
 #include "fo_host.h"
 #include "fo_step.h"
 
+#include <algorithm>
+#include <cmath>
+
 namespace fo {
 
 constexpr int kMaxShapes = 16;    // of one launch
@@ -61,7 +64,8 @@ struct MatrixGroup {
     __device__ double* squares(int k) const { return (double*)((char*)factor(k) + 256); }
 };
 
-// A launch over all groups; workgroups first[g] .. first[g + 1] belong to group g.
+// A launch over all groups.  Workgroups begin[g] .. begin[g + 1] belong to group g; in the products' launches these are seats,
+// of which each of the eight dies has all (fo_gemm.h), so that every die gets its share of every shape.
 struct Groups {
     MatrixGroup group[kMaxShapes];
     int64_t begin[kMaxShapes + 1];
@@ -297,45 +301,50 @@ __device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
 }
 
 // S, and B without its diagonal: rows of a symmetric matrix, each tile off the diagonal twice.
-struct SymmetricOut {
+template <bool GRAM> struct SymmetricOut {
     static constexpr bool kColumns = true;
-    const _Float16* s;      // B: the matrix that it is made of; S: null
+    const _Float16* s;      // what B is made of
     _Float16* out;
     float* diagonal;
     int side;
     float scale, b, c;
     bool mirror;
 
-    __device__ __forceinline__ void row(int i, int j, float (&v)[8]) const {
+    struct In { f16x8 s; };
+    __device__ __forceinline__ void begin(int) const {}
+    __device__ __forceinline__ void load(int i, int j, In& in) const {
+        if constexpr (!GRAM) { if (i < side && j < side) in.s = *reinterpret_cast<const f16x8*>(s + (int64_t)i * side + j); }
+    }
+    __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
         if (i >= side || j >= side) return;
-        const int64_t at = (int64_t)i * side + j;
-        if (s) {
-            const f16x8 old = *reinterpret_cast<const f16x8*>(s + at);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] = fmaf(c, v[e], b * (float)old[e]);
-                if (i == j + e) { diagonal[i] = v[e]; v[e] = 0.0f; }
-            }
-        } else {
+        if constexpr (GRAM) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= scale;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = fmaf(c, v[e], b * (float)in.s[e]);
+                if (i == j + e) { diagonal[i] = v[e]; v[e] = 0.0f; }
+            }
         }
-        *reinterpret_cast<f16x8*>(out + at) = half8(v);
+        *reinterpret_cast<f16x8*>(out + (int64_t)i * side + j) = half8(v);
     }
+    __device__ __forceinline__ bool columns() const { return mirror; }
     __device__ __forceinline__ void column(int i, int j, const float (&v)[8]) const {
-        if (!mirror || i >= side || j >= side) return;
+        if (i >= side || j >= side) return;
         *reinterpret_cast<f16x8*>(out + (int64_t)j * side + i) = half8(v);
     }
 };
 
-template <int WT, bool GRAM> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2) void symmetric_kernel(Groups a, StepArgs h) {
+template <int WT, bool GRAM> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void symmetric_kernel(Groups a, StepArgs h) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef GemmTile<F16Product, WT> Tile;
-    const int64_t b = tile_of_workgroup(blockIdx.x, a.begin[a.n]);
-    const int g = group_of(a, b);
+    const int64_t seat = blockIdx.x >> 3;
+    const int g = group_of(a, seat);
     const MatrixGroup& m = a.group[g];
     const int side = m.side(), n = (side + Tile::kTile - 1) / Tile::kTile, tiles = n * (n + 1) / 2;
-    const int64_t local = b - a.begin[g];
+    const int64_t local = tile_of_seat(blockIdx.x & 7, seat - a.begin[g], (int64_t)tiles * m.count);
+    if (local < 0) return;
     const int k = (int)(local / tiles);
     int i, j;
     tile_at_symmetric((int)(local % tiles), n, i, j);
@@ -345,7 +354,7 @@ template <int WT, bool GRAM> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2
     const Operand op{(const char*)x, length, nullptr, 0, side};
     Tile tile(lds);
     tile.multiply(op, op, i * Tile::kTile, j * Tile::kTile, (int)length);
-    SymmetricOut out{GRAM ? nullptr : m.s(k), GRAM ? m.s(k) : m.b(k), m.diagonal(k), side, h.first ? 1.0f / (m.unit * m.unit) : 1.0f, h.b, h.c, i != j};
+    SymmetricOut<GRAM> out{m.s(k), GRAM ? m.s(k) : m.b(k), m.diagonal(k), side, h.first ? 1.0f / (m.unit * m.unit) : 1.0f, h.b, h.c, i != j};
     tile.finish(i * Tile::kTile, j * Tile::kTile, out);
 }
 
@@ -357,25 +366,27 @@ struct ApplyIn {
     int rows, cols;     // padded
     float a, scale;
     bool tall;
+    float d[8];         // of the lane's columns
 
-    __device__ __forceinline__ void x(int i, int j, float (&v)[8], u32x4& low) const {
-        const int64_t at = (int64_t)i * cols + j;
-        const f16x8 h = *reinterpret_cast<const f16x8*>(hi + at);
-        low = *reinterpret_cast<const u32x4*>(lo + at / 2);
-        float d[8];
-        if (tall) {
-            const f32x4 d0 = *reinterpret_cast<const f32x4*>(diagonal + j), d1 = *reinterpret_cast<const f32x4*>(diagonal + j + 4);
+    struct In { f16x8 hi; u32x4 lo; float d; };
+    __device__ __forceinline__ void begin(int j) {
+        if (tall && j < cols) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { d[e] = a + d0[e]; d[4 + e] = a + d1[e]; }
-        } else {
-            const float one = a + diagonal[i];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] = one;
+            for (int e = 0; e < 8; ++e) d[e] = a + diagonal[j + e];
         }
+    }
+    __device__ __forceinline__ void load(int i, int j, In& in) const {
+        if (i >= rows || j >= cols) return;
+        const int64_t at = (int64_t)i * cols + j;
+        in.hi = *reinterpret_cast<const f16x8*>(hi + at);
+        in.lo = *reinterpret_cast<const u32x4*>(lo + at / 2);
+        if (!tall) in.d = a + diagonal[i];
+    }
+    __device__ __forceinline__ void x(const In& in, float (&v)[8]) const {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float rest = as_f32(e & 1 ? low[e / 2] & 0xffff0000u : low[e / 2] << 16);
-            v[e] = fmaf(d[e], (float)h[e] + rest, v[e]) * scale;
+            const float rest = as_f32(e & 1 ? in.lo[e / 2] & 0xffff0000u : in.lo[e / 2] << 16);
+            v[e] = fmaf(tall ? d[e] : in.d, (float)in.hi[e] + rest, v[e]) * scale;
         }
     }
 };
@@ -383,11 +394,11 @@ struct ApplyIn {
 struct ApplyOut : ApplyIn {
     static constexpr bool kColumns = true;
     _Float16 *next_hi, *next_t;
-    __device__ __forceinline__ void row(int i, int j, float (&v)[8]) const {
+    __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
         if (i >= rows || j >= cols) return;
-        u32x4 low;
-        x(i, j, v, low);
+        x(in, v);
         const f16x8 h = half8(v);
+        u32x4 low;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const f32x2 rest = {v[2 * e] - (float)h[2 * e], v[2 * e + 1] - (float)h[2 * e + 1]};
@@ -397,87 +408,99 @@ struct ApplyOut : ApplyIn {
         *reinterpret_cast<f16x8*>(next_hi + at) = h;
         *reinterpret_cast<u32x4*>(lo + at / 2) = low;
     }
+    __device__ __forceinline__ bool columns() const { return true; }
     __device__ __forceinline__ void column(int i, int j, const float (&v)[8]) const {
         if (i >= rows || j >= cols) return;
         *reinterpret_cast<f16x8*>(next_t + (int64_t)j * rows + i) = half8(v);
     }
 };
 
-// The last step: the result as bfloat16, or the weights moved along it.
+// What the last step does with the result: hands it out as bfloat16, or moves the weights along it.
 struct LastArgs {
-    uint16_t* result;               // rows x cols matrices one after the other; null: update the weights
+    uint16_t* result;               // rows x cols matrices one after the other
     const fo_tensor_desc* matrices;
-    int dtype, ecc_bytes;
     float keep;                     // 1 - lr * weight decay
 };
 
-// 8 weights of a row (the first `valid` of them): p <- p * keep - lr * x at master precision.
-template <int DT, int ECCB> __device__ __forceinline__ void update8(const fo_tensor_desc& d, int64_t at, int valid, bool aligned, const float (&x)[8], float keep, float lr) {
-    constexpr int PB = DTypeInfo<DT>::bytes, EPL = DTypeInfo<DT>::epl;
-#pragma unroll
-    for (int part = 0; part < 8; part += EPL) {
-        Pack<PB, EPL> p;
-        Pack<ECCB, EPL> e;
-        const int64_t first = at + part, end = at + valid;
-        if (aligned) { load_lane<PB, EPL, kLane>(p, d.param, first, end); load_lane<ECCB, EPL, kLane>(e, d.ecc, first, end); }
-        else { load_lane<PB, EPL, kGuarded>(p, d.param, first, end); load_lane<ECCB, EPL, kGuarded>(e, d.ecc, first, end); }
-        float w[EPL];
-#pragma unroll
-        for (int k = 0; k < EPL; ++k) {
-            float master = widen<DT, EPL>(p, k);
-            if constexpr (ECCB > 0) master = ecc_join<DT, ECCB>(master, ecc_to_float<ECCB, EPL>(e, k));
-            w[k] = master * keep - x[part + k] * lr;
-        }
-        write_master<DT, ECCB, EPL>(w, p, e);
-        if (aligned) { store_lane<PB, EPL, kLane>(p, d.param, first, end); store_lane<ECCB, EPL, kLane>(e, d.ecc, first, end); }
-        else { store_lane<PB, EPL, kGuarded>(p, d.param, first, end); store_lane<ECCB, EPL, kGuarded>(e, d.ecc, first, end); }
-    }
-}
-
-struct LastOut : ApplyIn {
+struct ResultOut : ApplyIn {
     static constexpr bool kColumns = false;
-    LastArgs last;
-    fo_tensor_desc matrix;
     uint16_t* result;
     int true_rows, true_cols;
-    float lr;
     bool aligned;
-
-    __device__ __forceinline__ void row(int i, int j, float (&v)[8]) const {
+    __device__ __forceinline__ ResultOut(const ApplyIn& in, const LastArgs& last, const MatrixGroup& m, int k)
+        : ApplyIn(in), result(last.result + (int64_t)(m.first + k) * m.rows * m.cols), true_rows(m.rows), true_cols(m.cols), aligned(m.cols % 8 == 0) {}
+    __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
         if (i >= true_rows || j >= true_cols) return;
-        u32x4 low;
-        x(i, j, v, low);
+        x(in, v);
+        Pack<2, 8> p;
+        narrow_all<DT_BF16, 8>(v, p);
         const int64_t at = (int64_t)i * true_cols + j;
-        const int valid = true_cols - j;
-        if (result) {
-            Pack<2, 8> p;
-            narrow_all<DT_BF16, 8>(v, p);
-            if (aligned && valid >= 8) *reinterpret_cast<u32x4*>(result + at) = u32x4{p.w[0], p.w[1], p.w[2], p.w[3]};
-            else store_guarded<2, 8>(p, result, at, at + valid);
-            return;
-        }
-        const int v8 = valid < 8 ? valid : 8;
-        switch (last.dtype * 4 + last.ecc_bytes) {
-            case DT_BF16 * 4 + 0: update8<DT_BF16, 0>(matrix, at, v8, aligned, v, last.keep, lr); break;
-            case DT_BF16 * 4 + 1: update8<DT_BF16, 1>(matrix, at, v8, aligned, v, last.keep, lr); break;
-            case DT_BF16 * 4 + 2: update8<DT_BF16, 2>(matrix, at, v8, aligned, v, last.keep, lr); break;
-            case DT_F16 * 4 + 0: update8<DT_F16, 0>(matrix, at, v8, aligned, v, last.keep, lr); break;
-            case DT_F16 * 4 + 1: update8<DT_F16, 1>(matrix, at, v8, aligned, v, last.keep, lr); break;
-            case DT_F16 * 4 + 2: update8<DT_F16, 2>(matrix, at, v8, aligned, v, last.keep, lr); break;
-            default: update8<DT_F32, 0>(matrix, at, v8, aligned, v, last.keep, lr);
-        }
+        if (aligned) *reinterpret_cast<u32x4*>(result + at) = u32x4{p.w[0], p.w[1], p.w[2], p.w[3]};
+        else store_guarded<2, 8>(p, result, at, (int64_t)(i + 1) * true_cols);
     }
-    __device__ __forceinline__ void column(int, int, const float (&)[8]) const {}
 };
 
-template <int WT, bool LAST> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2) void apply_kernel(Groups a, StepArgs h, LastArgs last) {
+// p <- p * keep - lr * x at master precision.
+template <int DT, int ECCB> struct UpdateOut : ApplyIn {
+    static constexpr bool kColumns = false;
+    static constexpr int PB = DTypeInfo<DT>::bytes, EPL = DTypeInfo<DT>::epl, kParts = 8 / EPL;
+    void *param, *ecc;
+    int true_rows, true_cols;
+    float keep, lr;
+    bool aligned;      // rows are whole 16-byte pieces
+    struct In : ApplyIn::In {
+        Pack<PB, EPL> p[kParts];
+        Pack<ECCB, EPL> e[kParts];
+    };
+    __device__ __forceinline__ UpdateOut(const ApplyIn& in, const LastArgs& last, const MatrixGroup& m, int k)
+        : ApplyIn(in), true_rows(m.rows), true_cols(m.cols), keep(last.keep), lr(m.lr) {
+        const fo_tensor_desc& d = last.matrices[m.first + k];
+        param = d.param;
+        ecc = d.ecc;
+        aligned = m.cols % 8 == 0 && (((uintptr_t)param | (uintptr_t)ecc) & 15) == 0;
+    }
+    __device__ __forceinline__ void load(int i, int j, In& in) const {
+        if (i >= true_rows || j >= true_cols) return;
+        ApplyIn::load(i, j, in);
+        const int64_t at = (int64_t)i * true_cols + j, end = (int64_t)(i + 1) * true_cols;
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            if (aligned) { load_lane<PB, EPL, kVector>(in.p[k], param, at + k * EPL, end); load_lane<ECCB, EPL, kVector>(in.e[k], ecc, at + k * EPL, end); }
+            else { load_lane<PB, EPL, kGuarded>(in.p[k], param, at + k * EPL, end); load_lane<ECCB, EPL, kGuarded>(in.e[k], ecc, at + k * EPL, end); }
+        }
+    }
+    __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
+        if (i >= true_rows || j >= true_cols) return;
+        x(in, v);
+        const int64_t at = (int64_t)i * true_cols + j, end = (int64_t)(i + 1) * true_cols;
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            Pack<PB, EPL> p;
+            Pack<ECCB, EPL> e;
+            float w[EPL];
+#pragma unroll
+            for (int q = 0; q < EPL; ++q) {
+                float master = widen<DT, EPL>(in.p[k], q);
+                if constexpr (ECCB > 0) master = ecc_join<DT, ECCB>(master, ecc_to_float<ECCB, EPL>(in.e[k], q));
+                w[q] = master * keep - v[k * EPL + q] * lr;
+            }
+            write_master<DT, ECCB, EPL>(w, p, e);
+            if (aligned) { store_lane<PB, EPL, kVector>(p, param, at + k * EPL, end); store_lane<ECCB, EPL, kVector>(e, ecc, at + k * EPL, end); }
+            else { store_lane<PB, EPL, kGuarded>(p, param, at + k * EPL, end); store_lane<ECCB, EPL, kGuarded>(e, ecc, at + k * EPL, end); }
+        }
+    }
+};
+
+// Out: ApplyOut, or what the last step does.
+template <int WT, class Out> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void apply_kernel(Groups a, StepArgs h, LastArgs last) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef GemmTile<F16Product, WT> Tile;
-    const int64_t b = tile_of_workgroup(blockIdx.x, a.begin[a.n]);
-    const int g = group_of(a, b);
+    const int64_t seat = blockIdx.x >> 3;
+    const int g = group_of(a, seat);
     const MatrixGroup& m = a.group[g];
     const int rows = (m.padded_rows + Tile::kTile - 1) / Tile::kTile, cols = (m.padded_cols + Tile::kTile - 1) / Tile::kTile;
-    const int64_t local = b - a.begin[g];
+    const int64_t local = tile_of_seat(blockIdx.x & 7, seat - a.begin[g], (int64_t)rows * cols * m.count);
+    if (local < 0) return;
     const int k = (int)(local / (rows * cols));
     int i, j;
     tile_at((int)(local % (rows * cols)), rows, cols, i, j);
@@ -488,19 +511,12 @@ template <int WT, bool LAST> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2
     const Operand turned{(const char*)m.t(k, h.generation), side * 2, nullptr, 0, m.padded_cols};
     Tile tile(lds);
     tile.multiply(tall ? main : poly, tall ? poly : turned, i * Tile::kTile, j * Tile::kTile, side * 2);
-    const ApplyIn in{m.hi(k, h.generation), m.lo(k), m.diagonal(k), m.padded_rows, m.padded_cols, h.a, h.first ? 1.0f / m.unit : 1.0f, tall};
-    if constexpr (LAST) {
-        LastOut out{in, last, {}, nullptr, m.rows, m.cols, m.lr, true};
-        if (last.result) {
-            out.result = last.result + (int64_t)(m.first + k) * m.rows * m.cols;
-            out.aligned = m.cols % 8 == 0;
-        } else {
-            out.matrix = last.matrices[m.first + k];
-            out.aligned = m.cols % 8 == 0 && (((uintptr_t)out.matrix.param | (uintptr_t)out.matrix.ecc) & 15) == 0;
-        }
+    const ApplyIn in{m.hi(k, h.generation), m.lo(k), m.diagonal(k), m.padded_rows, m.padded_cols, h.a, h.first ? 1.0f / m.unit : 1.0f, tall, {}};
+    if constexpr (Out::kColumns) {
+        Out out{in, m.hi(k, h.generation ^ 1), m.t(k, h.generation ^ 1)};
         tile.finish(i * Tile::kTile, j * Tile::kTile, out);
     } else {
-        ApplyOut out{in, m.hi(k, h.generation ^ 1), m.t(k, h.generation ^ 1)};
+        Out out(in, last, m, k);
         tile.finish(i * Tile::kTile, j * Tile::kTile, out);
     }
 }
@@ -550,7 +566,13 @@ int64_t plan(const fo_matrix_shape* shapes, int64_t n, char* workspace, fo::Grou
         }
         first += s.count;
     }
-    if (out) out->n = used;
+    if (out) {
+        out->n = used;
+        // the longest contractions first: what is left at the end of a launch is short
+        std::stable_sort(out->group, out->group + used, [](const fo::MatrixGroup& x, const fo::MatrixGroup& y) {
+            return std::max(x.rows, x.cols) > std::max(y.rows, y.cols);
+        });
+    }
     return at;
 }
 
@@ -563,13 +585,6 @@ template <class F> int64_t spread(fo::Groups& a, F each) {
 
 int64_t tiles_across(int n, int tile) { return (n + tile - 1) / tile; }
 
-template <int WT> int64_t symmetric_tiles(fo::Groups& a) {
-    return spread(a, [](const fo::MatrixGroup& m) { const int64_t n = tiles_across(m.side(), 2 * WT); return n * (n + 1) / 2; });
-}
-template <int WT> int64_t apply_tiles(fo::Groups& a) {
-    return spread(a, [](const fo::MatrixGroup& m) { return tiles_across(m.padded_rows, 2 * WT) * tiles_across(m.padded_cols, 2 * WT); });
-}
-
 template <class K, class... Args> int launch(K kernel, int64_t grid, int lds, hipStream_t stream, const char* what, Args... args) {
     if (grid > kMostWorkgroups) return fail(FO_ERR_UNSUPPORTED, "%s: %lld workgroups are more than one launch takes", what, (long long)grid);
     if (lds > 65536) {
@@ -579,27 +594,73 @@ template <class K, class... Args> int launch(K kernel, int64_t grid, int lds, hi
     return check_hip(hipGetLastError(), what);
 }
 
-// The largest tile that still gives every compute unit one.
-int choose(int64_t large, int64_t middle, int cus) {
-    if (large >= cus) return 128;
-    return middle >= cus ? 64 : 32;
+// Which tile a product takes: the one whose rounds over the compute units cost least.  A round is one workgroup's tile with
+// `resident` of them on a compute unit; it takes `start` plus `each` per value contracted, in us, fitted to steps of 4096 x
+// 14336, 4096 x 4096, 1024 x 4096 and 1000 x 2730 matrices: 131 us for a 256 x 256 tile over 4096 values, 86 for 192 x 192,
+// 75 for two 128 x 128, 52 for five 64 x 64 (the smaller ones read more of LDS per multiplication), 43 to 17 us over 1000.
+struct TileCost { int wt, resident; double start, each; };
+constexpr TileCost kTileCosts[] = {{128, 1, 14.0, 0.0286}, {96, 1, 16.0, 0.0170}, {64, 2, 8.0, 0.0165}, {32, 5, 7.0, 0.0110}};
+
+// tiles(group, wt) of a matrix, length(group) contracted.
+template <class T, class L> int choose(const fo::Groups& a, int cus, T tiles, L length) {
+    int best = 0;
+    double least = 0.0;
+    for (const TileCost& t : kTileCosts) {
+        double all = 0.0, time = 0.0;
+        for (int g = 0; g < a.n; ++g) {
+            const double n = (double)tiles(a.group[g], t.wt) * a.group[g].count;
+            all += n;
+            time += n * (t.start + t.each * length(a.group[g]));
+        }
+        const double rounds = ceil(all / ((double)cus * t.resident));
+        const double cost = rounds * time / all;
+        if (!best || cost < least) { best = t.wt; least = cost; }
+    }
+    return best;
 }
 
+int64_t symmetric_tiles(const fo::MatrixGroup& m, int wt) { const int64_t n = tiles_across(m.side(), 2 * wt); return n * (n + 1) / 2; }
+int64_t apply_tiles(const fo::MatrixGroup& m, int wt) { return tiles_across(m.padded_rows, 2 * wt) * tiles_across(m.padded_cols, 2 * wt); }
+
+// Seats per die, and the grid.
+template <class F> int64_t seat(fo::Groups& a, F tiles) {
+    a.begin[0] = 0;
+    for (int g = 0; g < a.n; ++g) a.begin[g + 1] = a.begin[g] + fo::seats_of(tiles(a.group[g]) * a.group[g].count);
+    return a.begin[a.n] * 8;
+}
+
+template <int WT, bool GRAM> int launch_symmetric(fo::Groups& a, const fo::StepArgs& h, hipStream_t stream) {
+    const int64_t grid = seat(a, [](const fo::MatrixGroup& m) { return symmetric_tiles(m, WT); });
+    return launch(fo::symmetric_kernel<WT, GRAM>, grid, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz product", a, h);
+}
 template <bool GRAM> int launch_symmetric(fo::Groups& a, const fo::StepArgs& h, int cus, hipStream_t stream) {
-    const char* what = "Newton-Schulz product";
-    switch (choose(symmetric_tiles<128>(a), symmetric_tiles<64>(a), cus)) {
-        case 128: return launch(fo::symmetric_kernel<128, GRAM>, symmetric_tiles<128>(a), fo::GemmTile<fo::F16Product, 128>::kLds, stream, what, a, h);
-        case 64: return launch(fo::symmetric_kernel<64, GRAM>, symmetric_tiles<64>(a), fo::GemmTile<fo::F16Product, 64>::kLds, stream, what, a, h);
-        default: return launch(fo::symmetric_kernel<32, GRAM>, symmetric_tiles<32>(a), fo::GemmTile<fo::F16Product, 32>::kLds, stream, what, a, h);
+    switch (choose(a, cus, symmetric_tiles, [](const fo::MatrixGroup& m) { return !GRAM ? m.side() : m.tall() ? m.padded_rows : m.padded_cols; })) {
+        case 128: return launch_symmetric<128, GRAM>(a, h, stream);
+        case 96: return launch_symmetric<96, GRAM>(a, h, stream);
+        case 64: return launch_symmetric<64, GRAM>(a, h, stream);
+        default: return launch_symmetric<32, GRAM>(a, h, stream);
     }
 }
-template <bool LAST> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, int cus, hipStream_t stream) {
-    const char* what = "Newton-Schulz step";
-    switch (choose(apply_tiles<128>(a), apply_tiles<64>(a), cus)) {
-        case 128: return launch(fo::apply_kernel<128, LAST>, apply_tiles<128>(a), fo::GemmTile<fo::F16Product, 128>::kLds, stream, what, a, h, last);
-        case 64: return launch(fo::apply_kernel<64, LAST>, apply_tiles<64>(a), fo::GemmTile<fo::F16Product, 64>::kLds, stream, what, a, h, last);
-        default: return launch(fo::apply_kernel<32, LAST>, apply_tiles<32>(a), fo::GemmTile<fo::F16Product, 32>::kLds, stream, what, a, h, last);
+template <int WT, class Out> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, hipStream_t stream) {
+    const int64_t grid = seat(a, [](const fo::MatrixGroup& m) { return apply_tiles(m, WT); });
+    return launch(fo::apply_kernel<WT, Out>, grid, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz step", a, h, last);
+}
+template <class Out> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, int cus, hipStream_t stream) {
+    switch (choose(a, cus, apply_tiles, [](const fo::MatrixGroup& m) { return m.side(); })) {
+        case 128: return launch_apply<128, Out>(a, h, last, stream);
+        case 96: return launch_apply<96, Out>(a, h, last, stream);
+        case 64: return launch_apply<64, Out>(a, h, last, stream);
+        default: return launch_apply<32, Out>(a, h, last, stream);
     }
+}
+int launch_update(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, int dtype, int ecc_bytes, int cus, hipStream_t stream) {
+    if (dtype == FO_F32) return launch_apply<fo::UpdateOut<fo::DT_F32, 0>>(a, h, last, cus, stream);
+    if (dtype == FO_BF16) return ecc_bytes == 0 ? launch_apply<fo::UpdateOut<fo::DT_BF16, 0>>(a, h, last, cus, stream)
+                               : ecc_bytes == 1 ? launch_apply<fo::UpdateOut<fo::DT_BF16, 1>>(a, h, last, cus, stream)
+                                                : launch_apply<fo::UpdateOut<fo::DT_BF16, 2>>(a, h, last, cus, stream);
+    return ecc_bytes == 0 ? launch_apply<fo::UpdateOut<fo::DT_F16, 0>>(a, h, last, cus, stream)
+         : ecc_bytes == 1 ? launch_apply<fo::UpdateOut<fo::DT_F16, 1>>(a, h, last, cus, stream)
+                          : launch_apply<fo::UpdateOut<fo::DT_F16, 2>>(a, h, last, cus, stream);
 }
 
 struct Iteration { int steps; float a, b, c, eps; };
@@ -612,7 +673,8 @@ int validate_iteration(int steps, const float* coefficients, float eps) {
 }
 
 // From the sums of squares on.
-template <int DT> int iterate(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, const fo::LastArgs& last, hipStream_t stream) {
+// finish(h) launches the last step.
+template <int DT, class F> int iterate(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, hipStream_t stream, F finish) {
     const int cus = compute_units();
     if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
     int64_t grid = spread(a, [](const fo::MatrixGroup&) { return (int64_t)1; });
@@ -623,7 +685,7 @@ template <int DT> int iterate(fo::Groups& a, const fo::MatrixSource& source, con
         const fo::StepArgs h{it.a, it.b, it.c, k & 1, k == 0};
         if (int rc = launch_symmetric<true>(a, h, cus, stream)) return rc;
         if (int rc = launch_symmetric<false>(a, h, cus, stream)) return rc;
-        if (int rc = k + 1 < it.steps ? launch_apply<false>(a, h, last, cus, stream) : launch_apply<true>(a, h, last, cus, stream)) return rc;
+        if (int rc = k + 1 < it.steps ? launch_apply<fo::ApplyOut>(a, h, fo::LastArgs{}, cus, stream) : finish(h, cus)) return rc;
     }
     return 0;
 }
@@ -631,7 +693,7 @@ template <int DT> int iterate(fo::Groups& a, const fo::MatrixSource& source, con
 template <int DT> int orthogonalise(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, const fo::LastArgs& last, hipStream_t stream) {
     const int64_t grid = spread(a, [](const fo::MatrixGroup& m) { return (int64_t)m.chunks; });
     if (int rc = launch(fo::squares_kernel<DT>, grid, 0, stream, "sum of squares", a, source)) return rc;
-    return iterate<DT>(a, source, it, last, stream);
+    return iterate<DT>(a, source, it, stream, [&](const fo::StepArgs& h, int cus) { return launch_apply<fo::ResultOut>(a, h, last, cus, stream); });
 }
 
 template <int DT> int momentum(fo::Groups& a, const fo::MomentumArgs& h, int quantized, hipStream_t stream) {
@@ -673,7 +735,7 @@ int fo_newton_schulz(const void* x, int dtype, int64_t count, int64_t rows, int6
     const bool aligned = (((uintptr_t)x | (uintptr_t)(stride * width) | (uintptr_t)(row_stride * width)) & 15) == 0;
     const fo::MatrixSource source{x, stride, row_stride, aligned};
     const Iteration it{steps, coefficients[0], coefficients[1], coefficients[2], eps};
-    const fo::LastArgs last{(uint16_t*)result, nullptr, 0, 0, 0.0f};
+    const fo::LastArgs last{(uint16_t*)result, nullptr, 0.0f};
     switch (dtype) {
         case FO_F32: return orthogonalise<fo::DT_F32>(a, source, it, last, (hipStream_t)stream);
         case FO_BF16: return orthogonalise<fo::DT_BF16>(a, source, it, last, (hipStream_t)stream);
@@ -701,11 +763,13 @@ int fo_muon_step(const fo_tensor_desc* matrices, const fo_matrix_shape* shapes, 
         plan(shapes + i, n, (char*)workspace, &a);
         if (a.n > 0) {
             const fo::MomentumArgs h{matrices, momentum_coef, 1.0f - momentum_coef, nesterov};
-            const fo::LastArgs last{nullptr, matrices, dtype, ecc_bytes, keep};
+            const fo::LastArgs last{nullptr, matrices, keep};
             hipStream_t s = (hipStream_t)stream;
             if (int rc = dtype == FO_F32 ? momentum<fo::DT_F32>(a, h, quantized, s) : dtype == FO_BF16 ? momentum<fo::DT_BF16>(a, h, quantized, s)
                                                                                                 : momentum<fo::DT_F16>(a, h, quantized, s)) return rc;
-            if (int rc = iterate<fo::DT_F32>(a, fo::MatrixSource{nullptr, 0, 0, false}, it, last, s)) return rc;
+            if (int rc = iterate<fo::DT_F32>(a, fo::MatrixSource{nullptr, 0, 0, false}, it, s, [&](const fo::StepArgs& step, int cus) {
+                    return launch_update(a, step, last, dtype, ecc_bytes, cus, s);
+                })) return rc;
         }
         for (int64_t k = 0; k < n; ++k) matrices += shapes[i + k].count;
     }

@@ -234,21 +234,25 @@ struct ProductOut {
             else store_guarded<B, EPL>(d, p, part * EPL, valid);
         }
     }
-    __device__ __forceinline__ void row(int i, int j, float (&v)[8]) const {
+    struct In {};
+    __device__ __forceinline__ void begin(int) const {}
+    __device__ __forceinline__ void load(int, int, In&) const {}
+    __device__ __forceinline__ void row(int i, int j, In, float (&v)[8]) const {
         if (i >= rows || j >= cols) return;
         if (dtype == DT_BF16) put<DT_BF16>(i, j, v);
         else if (dtype == DT_F16) put<DT_F16>(i, j, v);
         else put<DT_F32>(i, j, v);
     }
-    __device__ __forceinline__ void column(int, int, const float (&)[8]) const {}
 };
 
 template <int WT> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2) void mx_product_kernel(ProductArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmTile<Mx4Product, WT> Tile;
     const int rows = (p.rows + Tile::kTile - 1) / Tile::kTile, cols = (p.cols + Tile::kTile - 1) / Tile::kTile;
+    const int64_t t = tile_of_seat(blockIdx.x & 7, blockIdx.x >> 3, (int64_t)rows * cols);
+    if (t < 0) return;
     int i, j;
-    tile_at((int)tile_of_workgroup(blockIdx.x, (int64_t)rows * cols), rows, cols, i, j);
+    tile_at((int)t, rows, cols, i, j);
     const int64_t row_bytes = (int64_t)p.blocks * (kBlock / 2);
     const Operand a{p.a, row_bytes, p.a_scales, row_bytes / 16, p.rows}, b{p.b, row_bytes, p.b_scales, row_bytes / 16, p.cols};
     Tile tile(smem);
@@ -456,10 +460,10 @@ int fo_mxfp4_product(const void* a, const void* a_scales, int64_t rows, const vo
     if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
     const char* what = "fo_mxfp4_product";
     if (tiles(rows, cols, 256) >= cus)
-        return launch(fo::mx_product_kernel<128>, tiles(rows, cols, 256), 256, fo::GemmTile<fo::Mx4Product, 128>::kLds, stream, what, p);
+        return launch(fo::mx_product_kernel<128>, 8 * fo::seats_of(tiles(rows, cols, 256)), 256, fo::GemmTile<fo::Mx4Product, 128>::kLds, stream, what, p);
     if (tiles(rows, cols, 128) >= cus)
-        return launch(fo::mx_product_kernel<64>, tiles(rows, cols, 128), 256, fo::GemmTile<fo::Mx4Product, 64>::kLds, stream, what, p);
-    return launch(fo::mx_product_kernel<32>, tiles(rows, cols, 64), 256, fo::GemmTile<fo::Mx4Product, 32>::kLds, stream, what, p);
+        return launch(fo::mx_product_kernel<64>, 8 * fo::seats_of(tiles(rows, cols, 128)), 256, fo::GemmTile<fo::Mx4Product, 64>::kLds, stream, what, p);
+    return launch(fo::mx_product_kernel<32>, 8 * fo::seats_of(tiles(rows, cols, 64)), 256, fo::GemmTile<fo::Mx4Product, 32>::kLds, stream, what, p);
 }
 
 int fo_mxfp4_tokens(const void* x, int x_dtype, int64_t tokens, int64_t row_stride, const void* weight, const void* weight_scales, int64_t cols,
