@@ -31,7 +31,48 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kGemmThreads = 256;
+// Pieces of rows that begin at any element: global memory takes vector accesses at any address (the compiler emits them as
+// such for its default unaligned access mode), so rows of odd lengths need no path of their own.
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+typedef u32x2 u32x2_any __attribute__((aligned(1)));
+
+// EPL elements of EB bytes at p, `valid` of them there; the rest reads as zero and is not written.
+template <int EB, int EPL> __device__ __forceinline__ void load_piece(Pack<EB, EPL>& d, const void* p, int valid) {
+    if constexpr (EB > 0) {
+        if (valid < EPL) { load_guarded<EB, EPL>(d, p, 0, valid); return; }
+        if constexpr (EB * EPL == 16) {
+            const u32x4 v = *reinterpret_cast<const FO_GLOBAL u32x4_any*>((const FO_GLOBAL char*)p);
+            d.w[0] = v.x; d.w[1] = v.y; d.w[2] = v.z; d.w[3] = v.w;
+        } else {
+            static_assert(EB * EPL == 8, "8 or 16 bytes");
+            const u32x2 v = *reinterpret_cast<const FO_GLOBAL u32x2_any*>((const FO_GLOBAL char*)p);
+            d.w[0] = v.x; d.w[1] = v.y;
+        }
+    }
+}
+template <int EB, int EPL> __device__ __forceinline__ void store_piece(const Pack<EB, EPL>& d, void* p, int valid) {
+    if constexpr (EB > 0) {
+        if (valid < EPL) { store_guarded<EB, EPL>(d, p, 0, valid); return; }
+        if constexpr (EB * EPL == 16) {
+            *reinterpret_cast<FO_GLOBAL u32x4_any*>((FO_GLOBAL char*)p) = u32x4{d.w[0], d.w[1], d.w[2], d.w[3]};
+        } else {
+            static_assert(EB * EPL == 8, "8 or 16 bytes");
+            *reinterpret_cast<FO_GLOBAL u32x2_any*>((FO_GLOBAL char*)p) = u32x2{d.w[0], d.w[1]};
+        }
+    }
+}
+// Eight values as a piece of a row of type DT.
+template <int DT> __device__ __forceinline__ void store_values(const float (&v)[8], void* p, int valid) {
+    constexpr int B = DTypeInfo<DT>::bytes, EPL = 16 / B;
+#pragma unroll
+    for (int part = 0; part < 8 / EPL; ++part) {
+        Pack<B, EPL> d;
+#pragma unroll
+        for (int k = 0; k < EPL; k += 2) { float x, y; narrow_pair<DT, EPL>(d, k, v[part * EPL + k], v[part * EPL + k + 1], x, y); }
+        store_piece<B, EPL>(d, (char*)p + part * 16, valid - part * EPL);
+    }
+}
+
 constexpr int kStageBytes = 128;   // of each row
 constexpr int kHalfBytes = 64;     // what one phase multiplies; rows are whole multiples of it
 
@@ -172,25 +213,29 @@ template <class Product, int WT> struct GemmTile {
             out.scale = *reinterpret_cast<const uint8_t*>(buffer + kScaleOffset + row * 8 + half * 4 + (lane >> 4));
     }
 
-    // Multiplies (a, b) while reading the operands of the next phase into (na, nb) and, with LOAD, issuing a stage's loads.
-    // One row of instructions at a time, fenced off from the next, so that the reads and loads stay spread among them; the
-    // reads are over well before the last row, the next phase finds its operands there.
+    // Multiplies (a, b) while reading the operands of the next phase into (na, nb) and, with LOAD, issuing a stage's loads: at
+    // most one of each between two matrix instructions, fenced so that they stay there (in clumps they hold the wavefront up: 5 %
+    // of the rate at 4096 x 4096 x 8192).  The reads end a quarter before the phase does, so the next finds its operands.
     template <bool LOAD>
     __device__ __forceinline__ void phase(const Frag (&a)[kFrags], const Frag (&b)[kFrags], Frag (&na)[kFrags], Frag (&nb)[kFrags],
                                           int read_stage, int read_half, const Loader& l, int load_stage, bool load_half) {
-        constexpr int kReads = 2 * kFrags;
-        constexpr int kReadsPerRow = kFrags >= 4 ? (kReads + kFrags - 3) / (kFrags - 2) : kReads;
-        constexpr int kLoadsPerRow = (kLoads + kFrags - 1) / kFrags;
+        constexpr int kReads = 2 * kFrags, kAll = kFrags * kFrags;
+        constexpr int kReadWithin = kAll >= 16 ? kAll - kAll / 4 : kAll;
 #pragma unroll
-        for (int i = 0; i < kFrags; ++i) {
+        for (int q = 0; q < kAll; ++q) {
             if constexpr (LOAD) {
 #pragma unroll
-                for (int k = i * kLoadsPerRow; k < (i + 1) * kLoadsPerRow && k < kLoads; ++k) load(l, k, load_stage, load_half);
+                for (int k = q * kLoads / kAll; k < (q + 1) * kLoads / kAll; ++k) {
+                    load(l, k, load_stage, load_half);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
 #pragma unroll
-            for (int k = i * kReadsPerRow; k < (i + 1) * kReadsPerRow && k < kReads; ++k) read(na, nb, k, read_stage, read_half);
-#pragma unroll
-            for (int j = 0; j < kFrags; ++j) Product::multiply(a[i], b[j], acc[i][j]);
+            for (int k = q * kReads / kReadWithin; k < (q + 1) * kReads / kReadWithin && k < kReads; ++k) {
+                read(na, nb, k, read_stage, read_half);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            Product::multiply(a[q / kFrags], b[q % kFrags], acc[q / kFrags][q % kFrags]);
             __builtin_amdgcn_sched_barrier(0);
         }
     }

@@ -87,25 +87,15 @@ __device__ __forceinline__ int group_of(const Groups& a, int64_t b) {
 struct MatrixSource {
     const void* data;
     int64_t stride, row_stride;
-    bool aligned;   // 16-byte pieces of eight values may be read
 };
 
-template <int DT> __device__ __forceinline__ void read8(const char* p, bool aligned, int valid, float (&v)[8]) {
-    constexpr int B = DTypeInfo<DT>::bytes;
-    Pack<B, 16 / B> raw[B / 2];
-    if (aligned && valid >= 8) {
-        const u32x4* q = reinterpret_cast<const u32x4*>(p);
+template <int DT> __device__ __forceinline__ void read8(const char* p, int valid, float (&v)[8]) {
+    constexpr int B = DTypeInfo<DT>::bytes, EPL = 16 / B;
+    Pack<B, EPL> raw[B / 2];
 #pragma unroll
-        for (int i = 0; i < B / 2; ++i) {
-            const u32x4 w = q[i];
-            raw[i].w[0] = w.x; raw[i].w[1] = w.y; raw[i].w[2] = w.z; raw[i].w[3] = w.w;
-        }
-    } else {
+    for (int i = 0; i < B / 2; ++i) load_piece<B, EPL>(raw[i], p + i * 16, valid - i * EPL);
 #pragma unroll
-        for (int i = 0; i < B / 2; ++i) load_guarded<B, 16 / B>(raw[i], p, i * (16 / B), valid);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = widen<DT, 16 / B>(raw[k / (16 / B)], k % (16 / B));
+    for (int k = 0; k < 8; ++k) v[k] = widen<DT, EPL>(raw[k / EPL], k % EPL);
 }
 
 __device__ __forceinline__ double workgroup_sum(double x, double* lds) {
@@ -131,7 +121,7 @@ template <int DT> __global__ __launch_bounds__(256) void squares_kernel(Groups a
         const int64_t row = i / pieces;
         const int col = (int)(i - row * pieces) * 8;
         float v[8];
-        read8<DT>((const char*)source.data + (source.stride * k + source.row_stride * row + col) * DTypeInfo<DT>::bytes, source.aligned, m.cols - col, v);
+        read8<DT>((const char*)source.data + (source.stride * k + source.row_stride * row + col) * DTypeInfo<DT>::bytes, m.cols - col, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
     }
@@ -163,13 +153,12 @@ template <int DT> __global__ __launch_bounds__(256) void split_kernel(Groups a, 
     const float factor = *m.factor(k);
     const char* base = source.data ? (const char*)source.data + source.stride * k * DTypeInfo<DT>::bytes : (const char*)m.update(k);
     const int64_t row_stride = source.data ? source.row_stride : m.cols;
-    const bool aligned = source.data ? source.aligned : m.cols % 4 == 0;
     const int piece = (threadIdx.x & 7) * 8;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
         const int r = (threadIdx.x >> 3) + 32 * p, row = row0 + r, col = col0 + piece;
         float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (row < m.rows && col < m.cols) read8<DT>(base + (row_stride * row + col) * DTypeInfo<DT>::bytes, aligned, m.cols - col, v);
+        if (row < m.rows && col < m.cols) read8<DT>(base + (row_stride * row + col) * DTypeInfo<DT>::bytes, m.cols - col, v);
         f16x8 hi;
         u32x4 lo;
 #pragma unroll
@@ -426,17 +415,12 @@ struct ResultOut : ApplyIn {
     static constexpr bool kColumns = false;
     uint16_t* result;
     int true_rows, true_cols;
-    bool aligned;
     __device__ __forceinline__ ResultOut(const ApplyIn& in, const LastArgs& last, const MatrixGroup& m, int k)
-        : ApplyIn(in), result(last.result + (int64_t)(m.first + k) * m.rows * m.cols), true_rows(m.rows), true_cols(m.cols), aligned(m.cols % 8 == 0) {}
+        : ApplyIn(in), result(last.result + (int64_t)(m.first + k) * m.rows * m.cols), true_rows(m.rows), true_cols(m.cols) {}
     __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
         if (i >= true_rows || j >= true_cols) return;
         x(in, v);
-        Pack<2, 8> p;
-        narrow_all<DT_BF16, 8>(v, p);
-        const int64_t at = (int64_t)i * true_cols + j;
-        if (aligned) *reinterpret_cast<u32x4*>(result + at) = u32x4{p.w[0], p.w[1], p.w[2], p.w[3]};
-        else store_guarded<2, 8>(p, result, at, (int64_t)(i + 1) * true_cols);
+        store_values<DT_BF16>(v, result + (int64_t)i * true_cols + j, true_cols - j);
     }
 };
 
@@ -447,7 +431,6 @@ template <int DT, int ECCB> struct UpdateOut : ApplyIn {
     void *param, *ecc;
     int true_rows, true_cols;
     float keep, lr;
-    bool aligned;      // rows are whole 16-byte pieces
     struct In : ApplyIn::In {
         Pack<PB, EPL> p[kParts];
         Pack<ECCB, EPL> e[kParts];
@@ -457,22 +440,21 @@ template <int DT, int ECCB> struct UpdateOut : ApplyIn {
         const fo_tensor_desc& d = last.matrices[m.first + k];
         param = d.param;
         ecc = d.ecc;
-        aligned = m.cols % 8 == 0 && (((uintptr_t)param | (uintptr_t)ecc) & 15) == 0;
     }
     __device__ __forceinline__ void load(int i, int j, In& in) const {
         if (i >= true_rows || j >= true_cols) return;
         ApplyIn::load(i, j, in);
-        const int64_t at = (int64_t)i * true_cols + j, end = (int64_t)(i + 1) * true_cols;
+        const int64_t at = (int64_t)i * true_cols + j;
 #pragma unroll
         for (int k = 0; k < kParts; ++k) {
-            if (aligned) { load_lane<PB, EPL, kVector>(in.p[k], param, at + k * EPL, end); load_lane<ECCB, EPL, kVector>(in.e[k], ecc, at + k * EPL, end); }
-            else { load_lane<PB, EPL, kGuarded>(in.p[k], param, at + k * EPL, end); load_lane<ECCB, EPL, kGuarded>(in.e[k], ecc, at + k * EPL, end); }
+            load_piece<PB, EPL>(in.p[k], (char*)param + (at + k * EPL) * PB, true_cols - j - k * EPL);
+            load_piece<ECCB, EPL>(in.e[k], (char*)ecc + (at + k * EPL) * ECCB, true_cols - j - k * EPL);
         }
     }
     __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
         if (i >= true_rows || j >= true_cols) return;
         x(in, v);
-        const int64_t at = (int64_t)i * true_cols + j, end = (int64_t)(i + 1) * true_cols;
+        const int64_t at = (int64_t)i * true_cols + j;
 #pragma unroll
         for (int k = 0; k < kParts; ++k) {
             Pack<PB, EPL> p;
@@ -485,8 +467,8 @@ template <int DT, int ECCB> struct UpdateOut : ApplyIn {
                 w[q] = master * keep - v[k * EPL + q] * lr;
             }
             write_master<DT, ECCB, EPL>(w, p, e);
-            if (aligned) { store_lane<PB, EPL, kVector>(p, param, at + k * EPL, end); store_lane<ECCB, EPL, kVector>(e, ecc, at + k * EPL, end); }
-            else { store_lane<PB, EPL, kGuarded>(p, param, at + k * EPL, end); store_lane<ECCB, EPL, kGuarded>(e, ecc, at + k * EPL, end); }
+            store_piece<PB, EPL>(p, (char*)param + (at + k * EPL) * PB, true_cols - j - k * EPL);
+            store_piece<ECCB, EPL>(e, (char*)ecc + (at + k * EPL) * ECCB, true_cols - j - k * EPL);
         }
     }
 };
@@ -728,12 +710,10 @@ int fo_newton_schulz(const void* x, int dtype, int64_t count, int64_t rows, int6
     if (int rc = validate_shapes(&shape, 1)) return rc;
     if (count == 0 || rows == 0 || cols == 0) return 0;
     if (!x || !result || !workspace) return fail(FO_ERR_INVALID_ARGUMENT, "x, result and workspace must not be NULL");
-    if ((uintptr_t)workspace & 255 || (uintptr_t)result & 15) return fail(FO_ERR_INVALID_ARGUMENT, "workspace must be aligned to 256 bytes, result to 16");
+    if ((uintptr_t)workspace & 255) return fail(FO_ERR_INVALID_ARGUMENT, "workspace must be aligned to 256 bytes");
     fo::Groups a{};
     if (workspace_bytes < plan(&shape, 1, (char*)workspace, &a)) return fail(FO_ERR_INVALID_ARGUMENT, "workspace too small");
-    const int width = dtype == FO_F32 ? 4 : 2;
-    const bool aligned = (((uintptr_t)x | (uintptr_t)(stride * width) | (uintptr_t)(row_stride * width)) & 15) == 0;
-    const fo::MatrixSource source{x, stride, row_stride, aligned};
+    const fo::MatrixSource source{x, stride, row_stride};
     const Iteration it{steps, coefficients[0], coefficients[1], coefficients[2], eps};
     const fo::LastArgs last{(uint16_t*)result, nullptr, 0.0f};
     switch (dtype) {
@@ -767,7 +747,7 @@ int fo_muon_step(const fo_tensor_desc* matrices, const fo_matrix_shape* shapes, 
             hipStream_t s = (hipStream_t)stream;
             if (int rc = dtype == FO_F32 ? momentum<fo::DT_F32>(a, h, quantized, s) : dtype == FO_BF16 ? momentum<fo::DT_BF16>(a, h, quantized, s)
                                                                                                 : momentum<fo::DT_F16>(a, h, quantized, s)) return rc;
-            if (int rc = iterate<fo::DT_F32>(a, fo::MatrixSource{nullptr, 0, 0, false}, it, s, [&](const fo::StepArgs& step, int cus) {
+            if (int rc = iterate<fo::DT_F32>(a, fo::MatrixSource{nullptr, 0, 0}, it, s, [&](const fo::StepArgs& step, int cus) {
                     return launch_update(a, step, last, dtype, ecc_bytes, cus, s);
                 })) return rc;
         }

@@ -73,29 +73,15 @@ template <int DT> __device__ __forceinline__ u32 encode8(const Pair<DT>* p, floa
 }
 
 // Four pairs from memory, the first `valid` values of them, zeros after.
-template <int DT> __device__ __forceinline__ void load_pairs(const char* p, bool aligned, int valid, Pair<DT> (&out)[4]) {
-    constexpr int B = DTypeInfo<DT>::bytes;
-    u32 w[2 * B];
-    if (aligned && valid >= 8) {
+template <int DT> __device__ __forceinline__ void load_pairs(const char* p, int valid, Pair<DT> (&out)[4]) {
+    constexpr int B = DTypeInfo<DT>::bytes, EPL = 16 / B;
+    Pack<B, EPL> raw[B / 2];
 #pragma unroll
-        for (int i = 0; i < B / 2; ++i) {
-            const u32x4 q = reinterpret_cast<const u32x4*>(p)[i];
-            w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if constexpr (B == 2) {
-                const u32 x = k < valid ? reinterpret_cast<const uint16_t*>(p)[k] : 0u;
-                w[k / 2] = k & 1 ? w[k / 2] | x << 16 : x;
-            } else {
-                w[k] = k < valid ? reinterpret_cast<const u32*>(p)[k] : 0u;
-            }
-        }
-    }
+    for (int i = 0; i < B / 2; ++i) load_piece<B, EPL>(raw[i], p + i * 16, valid - i * EPL);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if constexpr (B == 2) out[i].v = w[i]; else { out[i].a = as_f32(w[2 * i]); out[i].b = as_f32(w[2 * i + 1]); }
+        if constexpr (B == 2) out[i].v = raw[0].w[i];
+        else { out[i].a = as_f32(raw[i / 2].w[i % 2 * 2]); out[i].b = as_f32(raw[i / 2].w[i % 2 * 2 + 1]); }
     }
 }
 
@@ -103,7 +89,6 @@ struct QuantizeArgs {
     const char* x;
     int64_t row_stride;   // in elements
     int rows, cols;
-    bool aligned;
     uint8_t *codes, *scales;                  // of the rows, or null
     uint8_t *column_codes, *column_scales;    // of the columns, or null
 };
@@ -123,7 +108,7 @@ template <int DT> __global__ __launch_bounds__(256) void mx_quantize_kernel(Quan
     for (int pass = 0; pass < 8; ++pass) {
         const int r = pass * 16 + (threadIdx.x >> 4), row = row0 + r;
         Pair<DT> p[4] = {};
-        if (row < a.rows && col < a.cols) load_pairs<DT>(a.x + (a.row_stride * row + col) * B, a.aligned, a.cols - col, p);
+        if (row < a.rows && col < a.cols) load_pairs<DT>(a.x + (a.row_stride * row + col) * B, a.cols - col, p);
         if (a.codes) {
             u32 m = 0;
 #pragma unroll
@@ -176,7 +161,7 @@ template <int DT> __global__ __launch_bounds__(256) void mx_quantize_kernel(Quan
 }
 
 // Eight values per thread.
-template <int DT> __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, char* out, int rows, int cols, bool aligned) {
+template <int DT> __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, char* out, int rows, int cols) {
     const int blocks = (cols + kBlock - 1) / kBlock, pieces = (cols + 7) / 8;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t row = i / pieces;
@@ -191,17 +176,7 @@ template <int DT> __global__ __launch_bounds__(256) void mx_dequantize_kernel(co
     const f32x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
     v[0] = v0.x * scale; v[1] = v0.y * scale; v[2] = v1.x * scale; v[3] = v1.y * scale;
     v[4] = v2.x * scale; v[5] = v2.y * scale; v[6] = v3.x * scale; v[7] = v3.y * scale;
-    constexpr int B = DTypeInfo<DT>::bytes, EPL = 16 / B;
-    const int valid = cols - piece * 8;
-    char* p = out + (row * cols + piece * 8) * B;
-#pragma unroll
-    for (int part = 0; part < 8 / EPL; ++part) {
-        Pack<B, EPL> d;
-#pragma unroll
-        for (int k = 0; k < EPL; k += 2) { float x, y; narrow_pair<DT, EPL>(d, k, v[part * EPL + k], v[part * EPL + k + 1], x, y); }
-        if (aligned && valid >= 8) *reinterpret_cast<u32x4*>(p + part * 16) = u32x4{d.w[0], d.w[1], d.w[2], d.w[3]};
-        else store_guarded<B, EPL>(d, p, part * EPL, valid);
-    }
+    store_values<DT>(v, out + (row * cols + piece * 8) * DTypeInfo<DT>::bytes, cols - piece * 8);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -213,35 +188,21 @@ struct ProductArgs {
     char* out;
     int rows, cols, blocks;             // of the result; 128-value blocks of the contracted axis
     int dtype;
-    bool aligned;                       // 16-byte pieces of the result may be written
 };
 
 struct ProductOut {
     static constexpr bool kColumns = false;
     char* out;
     int rows, cols, dtype;
-    bool aligned;
-    template <int DT> __device__ __forceinline__ void put(int i, int j, const float (&v)[8]) const {
-        constexpr int B = DTypeInfo<DT>::bytes, EPL = 16 / B;
-        char* p = out + ((int64_t)i * cols + j) * B;
-        const int valid = cols - j;
-#pragma unroll
-        for (int part = 0; part < 8 / EPL; ++part) {
-            Pack<B, EPL> d;
-#pragma unroll
-            for (int k = 0; k < EPL; k += 2) { float x, y; narrow_pair<DT, EPL>(d, k, v[part * EPL + k], v[part * EPL + k + 1], x, y); }
-            if (aligned && valid >= 8) *reinterpret_cast<u32x4*>(p + part * 16) = u32x4{d.w[0], d.w[1], d.w[2], d.w[3]};
-            else store_guarded<B, EPL>(d, p, part * EPL, valid);
-        }
-    }
     struct In {};
     __device__ __forceinline__ void begin(int) const {}
     __device__ __forceinline__ void load(int, int, In&) const {}
     __device__ __forceinline__ void row(int i, int j, In, float (&v)[8]) const {
         if (i >= rows || j >= cols) return;
-        if (dtype == DT_BF16) put<DT_BF16>(i, j, v);
-        else if (dtype == DT_F16) put<DT_F16>(i, j, v);
-        else put<DT_F32>(i, j, v);
+        const int64_t at = (int64_t)i * cols + j;
+        if (dtype == DT_BF16) store_values<DT_BF16>(v, out + at * 2, cols - j);
+        else if (dtype == DT_F16) store_values<DT_F16>(v, out + at * 2, cols - j);
+        else store_values<DT_F32>(v, out + at * 4, cols - j);
     }
 };
 
@@ -257,7 +218,7 @@ template <int WT> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2) void mx_p
     const Operand a{p.a, row_bytes, p.a_scales, row_bytes / 16, p.rows}, b{p.b, row_bytes, p.b_scales, row_bytes / 16, p.cols};
     Tile tile(smem);
     tile.multiply(a, b, i * Tile::kTile, j * Tile::kTile, (int)row_bytes);
-    ProductOut out{p.out, p.rows, p.cols, p.dtype, p.aligned};
+    ProductOut out{p.out, p.rows, p.cols, p.dtype};
     tile.finish(i * Tile::kTile, j * Tile::kTile, out);
 }
 
@@ -274,7 +235,6 @@ struct TokensArgs {
     char* out;
     int tokens, cols, inner, blocks;
     int64_t x_stride;              // RAW: elements between rows
-    bool x_aligned;
     int dtype;                     // of the result
 };
 constexpr int kTokenWaves = 8;
@@ -310,7 +270,7 @@ template <int DT, bool RAW, int TILES> __global__ __launch_bounds__(64 * kTokenW
                         for (int i = 0; i < 4; ++i) {
                             Pair<DT> q[4] = {};
                             if (at + i * 8 < p.inner)
-                                load_pairs<DT>(p.x + (p.x_stride * token + at + i * 8) * DTypeInfo<DT>::bytes, p.x_aligned, p.inner - at - i * 8, q);
+                                load_pairs<DT>(p.x + (p.x_stride * token + at + i * 8) * DTypeInfo<DT>::bytes, p.inner - at - i * 8, q);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) { v[i * 4 + e] = q[e]; const u32 k = q[e].magnitude(); m = m > k ? m : k; }
                         }
@@ -412,9 +372,7 @@ int fo_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int6
     if (rows == 0 || cols == 0) return 0;
     if (!x) return fail(FO_ERR_INVALID_ARGUMENT, "x must not be NULL");
     if (((uintptr_t)codes | (uintptr_t)column_codes) & 15) return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes");
-    const int width = dtype == FO_F32 ? 4 : 2;
-    const bool aligned = (((uintptr_t)x | (uintptr_t)(row_stride * width)) & 15) == 0;
-    const fo::QuantizeArgs a{(const char*)x, row_stride, (int)rows, (int)cols, aligned, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)column_codes, (uint8_t*)column_scales};
+    const fo::QuantizeArgs a{(const char*)x, row_stride, (int)rows, (int)cols, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)column_codes, (uint8_t*)column_scales};
     const int64_t grid = blocks_of(rows) * blocks_of(cols);
     switch (dtype) {
         case FO_F32: return launch_quantize<fo::DT_F32>(a, grid, stream);
@@ -428,14 +386,12 @@ int fo_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int
     if (rows == 0 || cols == 0) return 0;
     if (!codes || !scales || !out) return fail(FO_ERR_INVALID_ARGUMENT, "codes, scales and out must not be NULL");
     if ((uintptr_t)codes & 3) return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 4 bytes");
-    const int width = dtype == FO_F32 ? 4 : 2;
-    const bool aligned = ((uintptr_t)out & 15) == 0 && cols * width % 16 == 0;
     const int64_t grid = (rows * ((cols + 7) / 8) + 255) / 256;
     const char* what = "fo_mxfp4_dequantize";
     switch (dtype) {
-        case FO_F32: return launch(fo::mx_dequantize_kernel<fo::DT_F32>, grid, 256, 0, stream, what, (const uint8_t*)codes, (const uint8_t*)scales, (char*)out, (int)rows, (int)cols, aligned);
-        case FO_BF16: return launch(fo::mx_dequantize_kernel<fo::DT_BF16>, grid, 256, 0, stream, what, (const uint8_t*)codes, (const uint8_t*)scales, (char*)out, (int)rows, (int)cols, aligned);
-        default: return launch(fo::mx_dequantize_kernel<fo::DT_F16>, grid, 256, 0, stream, what, (const uint8_t*)codes, (const uint8_t*)scales, (char*)out, (int)rows, (int)cols, aligned);
+        case FO_F32: return launch(fo::mx_dequantize_kernel<fo::DT_F32>, grid, 256, 0, stream, what, (const uint8_t*)codes, (const uint8_t*)scales, (char*)out, (int)rows, (int)cols);
+        case FO_BF16: return launch(fo::mx_dequantize_kernel<fo::DT_BF16>, grid, 256, 0, stream, what, (const uint8_t*)codes, (const uint8_t*)scales, (char*)out, (int)rows, (int)cols);
+        default: return launch(fo::mx_dequantize_kernel<fo::DT_F16>, grid, 256, 0, stream, what, (const uint8_t*)codes, (const uint8_t*)scales, (char*)out, (int)rows, (int)cols);
     }
 }
 
@@ -448,14 +404,12 @@ int fo_mxfp4_product(const void* a, const void* a_scales, int64_t rows, const vo
     if (!a || !a_scales || !b || !b_scales || !out) return fail(FO_ERR_INVALID_ARGUMENT, "operands and out must not be NULL");
     if (((uintptr_t)a | (uintptr_t)b) & 15 || ((uintptr_t)a_scales | (uintptr_t)b_scales) & 3)
         return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes, scales to 4");
-    const int width = dtype == FO_F32 ? 4 : 2;
     const int64_t blocks = blocks_of(inner);
     if (rows <= 64) {
-        const fo::TokensArgs p{(const char*)a, (const uint8_t*)a_scales, (const char*)b, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)inner, (int)blocks, 0, false, dtype};
+        const fo::TokensArgs p{(const char*)a, (const uint8_t*)a_scales, (const char*)b, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)inner, (int)blocks, 0, dtype};
         return launch_tokens<fo::DT_BF16, false>(p, stream);
     }
-    const bool aligned = ((uintptr_t)out & 15) == 0 && cols * width % 16 == 0;
-    const fo::ProductArgs p{(const char*)a, (const char*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)blocks, dtype, aligned};
+    const fo::ProductArgs p{(const char*)a, (const char*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)blocks, dtype};
     const int cus = compute_units();
     if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
     const char* what = "fo_mxfp4_product";
@@ -475,9 +429,7 @@ int fo_mxfp4_tokens(const void* x, int x_dtype, int64_t tokens, int64_t row_stri
     if (int rc = validate_inner("fo_mxfp4_tokens", inner)) return rc;
     if (!x || !weight || !weight_scales || !out) return fail(FO_ERR_INVALID_ARGUMENT, "operands and out must not be NULL");
     if ((uintptr_t)weight & 15) return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes");
-    const int width = x_dtype == FO_F32 ? 4 : 2;
-    const bool aligned = (((uintptr_t)x | (uintptr_t)(row_stride * width)) & 15) == 0;
-    const fo::TokensArgs p{(const char*)x, nullptr, (const char*)weight, (const uint8_t*)weight_scales, (char*)out, (int)tokens, (int)cols, (int)inner, (int)blocks_of(inner), row_stride, aligned, dtype};
+    const fo::TokensArgs p{(const char*)x, nullptr, (const char*)weight, (const uint8_t*)weight_scales, (char*)out, (int)tokens, (int)cols, (int)inner, (int)blocks_of(inner), row_stride, dtype};
     switch (x_dtype) {
         case FO_F32: return launch_tokens<fo::DT_F32, true>(p, stream);
         case FO_BF16: return launch_tokens<fo::DT_BF16, true>(p, stream);

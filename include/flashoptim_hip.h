@@ -248,8 +248,8 @@ typedef struct fo_matrix_shape {
 /* Bytes of device memory, aligned to 256, that the calls below need for these shapes; negative: FO_ERR_* */
 int64_t fo_newton_schulz_workspace(const fo_matrix_shape *shapes, int64_t n_shapes);
 
-/* `count` matrices of `dtype`, `stride` elements apart, rows `row_stride` apart, columns adjacent; result: bfloat16, contiguous,
- * aligned to 16 bytes.  The workspace is free again when the call's work on `stream` is done. */
+/* `count` matrices of `dtype`, `stride` elements apart, rows `row_stride` apart, columns adjacent; result: bfloat16, contiguous.
+ * The workspace is free again when the call's work on `stream` is done. */
 int fo_newton_schulz(const void *x, int dtype, int64_t count, int64_t rows, int64_t cols, int64_t stride, int64_t row_stride,
                      void *result, int steps, const float *coefficients, float eps, void *workspace, int64_t workspace_bytes,
                      void *stream);
