@@ -222,11 +222,12 @@ template <int WT> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2) void mx_p
     tile.finish(i * Tile::kTile, j * Tile::kTile, out);
 }
 
-// Few rows against many: `tokens` <= 16 TILES rows of x, a weight of `cols` rows.  Bound by the weight's bytes.  A workgroup takes 16
-// weight rows, its eight wavefronts take turns along the contracted axis, 256 values at a time, straight from memory into
-// the operand registers of 16x16x128 instructions (weight rows as their rows, tokens as their columns), and add up through
-// LDS at the end.  x comes as codes, or, with RAW, as values of type DT that every wavefront quantises as it needs them: a
-// lane's operand is one group, so the scale never leaves the lane.
+// Few rows against many: `tokens` <= 16 TILES rows of x, a weight of `cols` rows.  Bound by the weight's bytes, so what counts is
+// how many of them are under way: a workgroup takes 16 ROWS weight rows, each of its eight wavefronts a run of blocks along the
+// contracted axis, and asks for BATCH blocks (1 KiB of codes for 16 rows) before it looks at x.  The codes go straight from memory
+// into the operand registers of 16x16x128 instructions (weight rows as their rows, tokens as their columns); the wavefronts add up
+// through LDS at the end.  x comes as codes; or, with RAW, as values of type DT, which the workgroup quantises into LDS first, a
+// group per thread: free beside the weight as long as it is a pass or two (kRawBlocks).
 struct TokensArgs {
     const char* x;                 // codes, or values
     const uint8_t* x_scales;
@@ -237,67 +238,124 @@ struct TokensArgs {
     int64_t x_stride;              // RAW: elements between rows
     int dtype;                     // of the result
 };
-constexpr int kTokenWaves = 8;
+constexpr int kTokenWaves = 8, kTokenThreads = 64 * kTokenWaves;
+constexpr int kRawBlocks = 256;    // most blocks of x that are quantised within the product: two groups per thread
 
-template <int DT, bool RAW, int TILES> __global__ __launch_bounds__(64 * kTokenWaves) void mx_tokens_kernel(TokensArgs p) {
-    __shared__ f32x4 sums[kTokenWaves][TILES][64];
+template <int DT> __device__ __forceinline__ void quantise_tokens(const TokensArgs& p, char* codes, uint8_t* scales) {
+    constexpr int B = DTypeInfo<DT>::bytes;
+    for (int i = threadIdx.x; i < p.tokens * p.blocks * 4; i += kTokenThreads) {
+        const int token = i / (p.blocks * 4), group = i - token * p.blocks * 4, at = group * kMxGroup;
+        const char* x = p.x + (p.x_stride * token + at) * B;
+        Pair<DT> q[4][4];
+        u32 m = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) load_pairs<DT>(x + k * 8 * B, p.inner - at - k * 8, q[k]);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) { const u32 e = q[k / 4][k % 4].magnitude(); m = m > e ? m : e; }
+        const u32 byte = scale_byte(m);
+        i32x4 v = {0, 0, 0, 0};
+        if (byte != 255u) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = (int)encode8<DT>(q[k], scale_value(byte));
+        }
+        *reinterpret_cast<i32x4*>(codes + i * 16) = v;
+        scales[i] = (uint8_t)byte;
+    }
+}
+
+template <int DT, bool RAW, int TILES, int ROWS, int BATCH> __global__ __launch_bounds__(kTokenThreads) void mx_tokens_kernel(TokensArgs p) {
+    constexpr int kAtOnce = TILES == 4 ? 2 : 4;   // blocks of x under way
+    __shared__ f32x4 sums[kTokenWaves][ROWS * TILES][64];
+    __shared__ __attribute__((aligned(16))) char raw_codes[RAW ? kRawBlocks * 64 : 16];
+    __shared__ uint8_t raw_scales[RAW ? kRawBlocks * 4 : 1];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int line = lane & 15, group = lane >> 4;
-    const int row = blockIdx.x * 16 + line < p.cols ? blockIdx.x * 16 + line : p.cols - 1;   // past the last: copies, not stored
-    const char* w = p.weight + (int64_t)row * p.blocks * 64 + group * 16;
-    const uint8_t* ws = p.weight_scales + (int64_t)row * p.blocks * 4 + group;
-    f32x4 acc[TILES];
+    // rows past the last, of the weight and of x, are read as copies of it: they make results that are not stored
+    const char* w[ROWS];
+    const uint8_t* ws[ROWS];
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int first = wave * 2; first < p.blocks; first += kTokenWaves * 2) {
+    for (int r = 0; r < ROWS; ++r) {
+        const int64_t want = ((int64_t)blockIdx.x * ROWS + r) * 16 + line, row = want < p.cols ? want : p.cols - 1;
+        w[r] = p.weight + row * p.blocks * 64 + group * 16;
+        ws[r] = p.weight_scales + row * p.blocks * 4 + group;
+    }
+    const char* x[TILES];
+    const uint8_t* xs[TILES];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int block = first + u;
-            if (block >= p.blocks) break;
-            const i32x4 wv = *reinterpret_cast<const i32x4*>(w + block * 64);
-            const int wscale = ws[block * 4];
+    for (int t = 0; t < TILES; ++t) {
+        const int token = t * 16 + line < p.tokens ? t * 16 + line : p.tokens - 1;
+        x[t] = (RAW ? raw_codes : p.x) + (int64_t)token * p.blocks * 64 + group * 16;
+        xs[t] = (RAW ? raw_scales : p.x_scales) + (int64_t)token * p.blocks * 4 + group;
+    }
+    const int per = (p.blocks + kTokenWaves - 1) / kTokenWaves;
+    const int end = (wave + 1) * per < p.blocks ? (wave + 1) * per : p.blocks;
+    f32x4 acc[ROWS][TILES];
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                const int token = t * 16 + line;
-                i32x4 xv = {0, 0, 0, 0};
-                int xscale = 127;
-                if (token < p.tokens) {
-                    if constexpr (RAW) {
-                        const int at = block * kBlock + group * kMxGroup;
-                        Pair<DT> v[16];
-                        u32 m = 0;
+    for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            Pair<DT> q[4] = {};
-                            if (at + i * 8 < p.inner)
-                                load_pairs<DT>(p.x + (p.x_stride * token + at + i * 8) * DTypeInfo<DT>::bytes, p.inner - at - i * 8, q);
+        for (int t = 0; t < TILES; ++t) acc[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    bool ready = !RAW;
+    for (int first = wave * per; first < end || !ready; first += BATCH) {
+        i32x4 wv[BATCH][ROWS];
+        int wscale[BATCH][ROWS];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) { v[i * 4 + e] = q[e]; const u32 k = q[e].magnitude(); m = m > k ? m : k; }
-                        }
-                        const u32 byte = scale_byte(m);
-                        xscale = (int)byte;
-                        if (byte != 255u) {
+        for (int u = 0; u < BATCH; ++u) {
+            if (first + u < end) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) xv[i] = (int)encode8<DT>(v + 4 * i, scale_value(byte));
-                        }
-                    } else {
-                        xv = *reinterpret_cast<const i32x4*>(p.x + ((int64_t)token * p.blocks + block) * 64 + group * 16);
-                        xscale = p.x_scales[((int64_t)token * p.blocks + block) * 4 + group];
+                for (int r = 0; r < ROWS; ++r) {
+                    wv[u][r] = *reinterpret_cast<const i32x4*>(w[r] + (first + u) * 64);
+                    wscale[u][r] = ws[r][(first + u) * 4];
+                }
+            }
+        }
+        if constexpr (RAW) {
+            if (!ready) {   // every wavefront comes here once, in its first turn
+                quantise_tokens<DT>(p, raw_codes, raw_scales);
+                __syncthreads();
+                ready = true;
+            }
+        }
+#pragma unroll
+        for (int part = 0; part < BATCH; part += kAtOnce) {
+            i32x4 xv[kAtOnce][TILES];
+            int xscale[kAtOnce][TILES];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (first + part + u < end) {
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) {
+                        xv[u][t] = *reinterpret_cast<const i32x4*>(x[t] + (first + part + u) * 64);
+                        xscale[u][t] = xs[t][(first + part + u) * 4];
                     }
                 }
-                const i32x8 va = {wv.x, wv.y, wv.z, wv.w, 0, 0, 0, 0}, vb = {xv.x, xv.y, xv.z, xv.w, 0, 0, 0, 0};
-                acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, acc[t], 4, 4, 0, wscale, 0, xscale);
-            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (first + part + u < end) {
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) {
+                        const i32x8 vb = {xv[u][t].x, xv[u][t].y, xv[u][t].z, xv[u][t].w, 0, 0, 0, 0};
+#pragma unroll
+                        for (int r = 0; r < ROWS; ++r) {
+                            const i32x4 c = wv[part + u][r];
+                            const i32x8 va = {c.x, c.y, c.z, c.w, 0, 0, 0, 0};
+                            acc[r][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, acc[r][t], 4, 4, 0, wscale[part + u][r], 0, xscale[u][t]);
+                        }
+                    }
+                }
         }
     }
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) sums[wave][t][lane] = acc[t];
-    __syncthreads();
-    for (int k = threadIdx.x; k < TILES * 64; k += 64 * kTokenWaves) {
-        f32x4 v = sums[0][k >> 6][k & 63];
+    for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-        for (int s = 1; s < kTokenWaves; ++s) v += sums[s][k >> 6][k & 63];
-        const int token = (k >> 6) * 16 + (k & 15), col = blockIdx.x * 16 + (k >> 4 & 3) * 4;
+        for (int t = 0; t < TILES; ++t) sums[wave][r * TILES + t][lane] = acc[r][t];
+    __syncthreads();
+    for (int k = threadIdx.x; k < ROWS * TILES * 64; k += kTokenThreads) {
+        const int piece = k >> 6, from = k & 63;
+        f32x4 v = sums[0][piece][from];
+#pragma unroll
+        for (int s = 1; s < kTokenWaves; ++s) v += sums[s][piece][from];
+        const int token = piece % TILES * 16 + (from & 15);
+        const int64_t col = ((int64_t)blockIdx.x * ROWS + piece / TILES) * 16 + (from >> 4) * 4;
         if (token >= p.tokens) continue;
         const int64_t at = (int64_t)token * p.cols + col;
 #pragma unroll
@@ -320,6 +378,7 @@ using namespace fo_host;
 
 constexpr int64_t kMostWorkgroups = 1 << 22;
 constexpr int64_t kMostLines = INT32_MAX - 255;
+static_assert(FO_MXFP4_MOST_TOKENS == 64, "four tiles of 16");
 
 int validate_matrix(const char* what, int64_t rows, int64_t cols, int dtype) {
     if (rows < 0 || cols < 0) return fail(FO_ERR_INVALID_ARGUMENT, "%s: negative size", what);
@@ -351,12 +410,27 @@ template <int DT> int launch_quantize(const fo::QuantizeArgs& a, int64_t grid, v
     return launch(fo::mx_quantize_kernel<DT>, grid, 256, lds, stream, "fo_mxfp4_quantize", a);
 }
 
-template <int DT, bool RAW> int launch_tokens(const fo::TokensArgs& p, void* stream) {
-    const int64_t grid = (p.cols + 15) / 16;
-    const char* what = "fo_mxfp4_product";
-    if (RAW || p.tokens <= 16) return launch(fo::mx_tokens_kernel<DT, RAW, 1>, grid, 64 * fo::kTokenWaves, 0, stream, what, p);
-    if (p.tokens <= 32) return launch(fo::mx_tokens_kernel<DT, RAW, RAW ? 1 : 2>, grid, 64 * fo::kTokenWaves, 0, stream, what, p);
-    return launch(fo::mx_tokens_kernel<DT, RAW, RAW ? 1 : 4>, grid, 64 * fo::kTokenWaves, 0, stream, what, p);
+template <int DT, bool RAW, int TILES, int ROWS> int launch_tokens(const fo::TokensArgs& p, void* stream) {
+    const int64_t grid = (p.cols + 16 * ROWS - 1) / (16 * ROWS);
+    const char* what = RAW ? "fo_mxfp4_tokens" : "fo_mxfp4_product";
+    // a wavefront's run in one batch where it fits
+    if (p.blocks <= 4 * fo::kTokenWaves) return launch(fo::mx_tokens_kernel<DT, RAW, TILES, ROWS, 4>, grid, fo::kTokenThreads, 0, stream, what, p);
+    return launch(fo::mx_tokens_kernel<DT, RAW, TILES, ROWS, 16 / ROWS>, grid, fo::kTokenThreads, 0, stream, what, p);
+}
+// Two pieces of 16 weight rows to a workgroup read x half as often, where that leaves every compute unit a workgroup: 13.2 us
+// for 16 tokens by 14336 x 4096 against 16.1, 26.2 against 37.6 for 64; with 4096 rows (half the compute units) 38.8 against 32.8.
+bool by_two(const fo::TokensArgs& p) { return p.cols >= 32 * compute_units(); }
+
+template <int DT> int launch_raw_tokens(const fo::TokensArgs& p, void* stream) {
+    if (p.tokens <= 16) return by_two(p) ? launch_tokens<DT, true, 1, 2>(p, stream) : launch_tokens<DT, true, 1, 1>(p, stream);
+    return p.tokens <= 32 ? launch_tokens<DT, true, 2, 1>(p, stream) : launch_tokens<DT, true, 4, 1>(p, stream);
+}
+template <int TILES> int launch_coded_tokens(const fo::TokensArgs& p, void* stream) {
+    return by_two(p) ? launch_tokens<fo::DT_BF16, false, TILES, 2>(p, stream) : launch_tokens<fo::DT_BF16, false, TILES, 1>(p, stream);
+}
+int launch_coded_tokens(const fo::TokensArgs& p, void* stream) {
+    if (p.tokens <= 16) return launch_coded_tokens<1>(p, stream);
+    return p.tokens <= 32 ? launch_coded_tokens<2>(p, stream) : launch_coded_tokens<4>(p, stream);
 }
 
 int64_t tiles(int64_t rows, int64_t cols, int tile) { return ((rows + tile - 1) / tile) * ((cols + tile - 1) / tile); }
@@ -405,9 +479,9 @@ int fo_mxfp4_product(const void* a, const void* a_scales, int64_t rows, const vo
     if (((uintptr_t)a | (uintptr_t)b) & 15 || ((uintptr_t)a_scales | (uintptr_t)b_scales) & 3)
         return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes, scales to 4");
     const int64_t blocks = blocks_of(inner);
-    if (rows <= 64) {
+    if (rows <= FO_MXFP4_MOST_TOKENS) {
         const fo::TokensArgs p{(const char*)a, (const uint8_t*)a_scales, (const char*)b, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)inner, (int)blocks, 0, dtype};
-        return launch_tokens<fo::DT_BF16, false>(p, stream);
+        return launch_coded_tokens(p, stream);
     }
     const fo::ProductArgs p{(const char*)a, (const char*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)blocks, dtype};
     const int cus = compute_units();
@@ -420,8 +494,14 @@ int fo_mxfp4_product(const void* a, const void* a_scales, int64_t rows, const vo
     return launch(fo::mx_product_kernel<32>, 8 * fo::seats_of(tiles(rows, cols, 64)), 256, fo::GemmTile<fo::Mx4Product, 32>::kLds, stream, what, p);
 }
 
+int64_t fo_mxfp4_tokens_workspace(int64_t tokens, int64_t inner) {
+    if (int rc = validate_matrix("fo_mxfp4_tokens", tokens, inner, FO_F32)) return rc;
+    const int64_t blocks = tokens * blocks_of(inner);
+    return blocks <= fo::kRawBlocks ? 0 : blocks * 68;
+}
+
 int fo_mxfp4_tokens(const void* x, int x_dtype, int64_t tokens, int64_t row_stride, const void* weight, const void* weight_scales, int64_t cols,
-                    int64_t inner, void* out, int dtype, void* stream) {
+                    int64_t inner, void* out, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
     if (int rc = validate_matrix("fo_mxfp4_tokens", tokens, cols, dtype)) return rc;
     if (int rc = validate_matrix("fo_mxfp4_tokens", tokens, inner, x_dtype)) return rc;
     if (tokens > FO_MXFP4_MOST_TOKENS) return fail(FO_ERR_UNSUPPORTED, "fo_mxfp4_tokens takes at most %d rows, not %lld", FO_MXFP4_MOST_TOKENS, (long long)tokens);
@@ -429,11 +509,20 @@ int fo_mxfp4_tokens(const void* x, int x_dtype, int64_t tokens, int64_t row_stri
     if (int rc = validate_inner("fo_mxfp4_tokens", inner)) return rc;
     if (!x || !weight || !weight_scales || !out) return fail(FO_ERR_INVALID_ARGUMENT, "operands and out must not be NULL");
     if ((uintptr_t)weight & 15) return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes");
-    const fo::TokensArgs p{(const char*)x, nullptr, (const char*)weight, (const uint8_t*)weight_scales, (char*)out, (int)tokens, (int)cols, (int)inner, (int)blocks_of(inner), row_stride, dtype};
+    const int64_t need = fo_mxfp4_tokens_workspace(tokens, inner), blocks = blocks_of(inner);
+    fo::TokensArgs p{(const char*)x, nullptr, (const char*)weight, (const uint8_t*)weight_scales, (char*)out, (int)tokens, (int)cols, (int)inner, (int)blocks, row_stride, dtype};
+    if (need > 0) {
+        if (!workspace || workspace_bytes < need || (uintptr_t)workspace & 15)
+            return fail(FO_ERR_INVALID_ARGUMENT, "a workspace of %lld bytes, aligned to 16, is needed", (long long)need);
+        p.x = (const char*)workspace;
+        p.x_scales = (const uint8_t*)workspace + tokens * blocks * 64;
+        if (int rc = fo_mxfp4_quantize(x, x_dtype, tokens, inner, row_stride, workspace, (uint8_t*)workspace + tokens * blocks * 64, nullptr, nullptr, stream)) return rc;
+        return launch_coded_tokens(p, stream);
+    }
     switch (x_dtype) {
-        case FO_F32: return launch_tokens<fo::DT_F32, true>(p, stream);
-        case FO_BF16: return launch_tokens<fo::DT_BF16, true>(p, stream);
-        default: return launch_tokens<fo::DT_F16, true>(p, stream);
+        case FO_F32: return launch_raw_tokens<fo::DT_F32>(p, stream);
+        case FO_BF16: return launch_raw_tokens<fo::DT_BF16>(p, stream);
+        default: return launch_raw_tokens<fo::DT_F16>(p, stream);
     }
 }
 }  // extern "C"

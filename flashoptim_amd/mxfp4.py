@@ -15,7 +15,8 @@ from ._native import DTYPE_CODE
 
 GROUP_SIZE = 32
 BLOCK = 128  # rows are filled up to multiples of it
-_MOST_TOKENS = 16  # FO_MXFP4_MOST_TOKENS
+_MOST_TOKENS = 64  # FO_MXFP4_MOST_TOKENS
+_RAW_BLOCKS = 256  # blocks of the input that the product for few rows quantises itself (fo_mxfp4_tokens_workspace)
 
 
 def _blocks(n: int) -> int:
@@ -129,10 +130,27 @@ def mxfp4_dequantize(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> tor
     return out
 
 
+def _tokens(x: torch.Tensor, weight: MXFP4Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The product for a few rows of plain values; every argument is checked, x's columns are adjacent."""
+    m, (n, k) = x.shape[0], weight.shape
+    out = torch.empty((m, n), dtype=dtype, device=x.device)
+    blocks = m * _blocks(k)
+    size, workspace = 0, None
+    if blocks > _RAW_BLOCKS:
+        size = blocks * 68
+        workspace = torch.empty(size, dtype=torch.uint8, device=x.device).data_ptr()
+    with _native.device_guard(x.device):
+        rc = _native.lib().fo_mxfp4_tokens(x.data_ptr(), DTYPE_CODE[x.dtype], m, x.stride(0), weight.codes.data_ptr(), weight.scales.data_ptr(),
+                                           n, k, out.data_ptr(), DTYPE_CODE[dtype], workspace, size, _native.current_stream_ptr(x.device))
+    if rc:
+        _native.check(rc, "fo_mxfp4_tokens")
+    return out
+
+
 def mxfp4_matmul(a: Union[MXFP4Tensor, torch.Tensor], b: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``a @ b.T`` of an ``m x k`` and an ``n x k`` matrix in MXFP4, summed in fp32, as an ``m x n`` matrix of `dtype`.
 
-    `a` may be a plain matrix: it is quantised on the way, for up to 16 rows within the product's own kernel.
+    `a` may be a plain matrix: it is quantised on the way, in the product's own kernel where it is a few short rows.
     """
     if not isinstance(b, MXFP4Tensor):
         raise ValueError(f"mxfp4_matmul expects its second operand as an MXFP4Tensor, got {type(b)}.")
@@ -149,23 +167,17 @@ def mxfp4_matmul(a: Union[MXFP4Tensor, torch.Tensor], b: MXFP4Tensor, dtype: tor
         raise ValueError(f"operands of shapes {tuple(a.shape)} and {tuple(b.shape)} do not contract over one length")
     if k == 0:
         return torch.zeros((m, n), dtype=dtype, device=b.device)
-    out = torch.empty((m, n), dtype=dtype, device=b.device)
-    if out.numel() == 0:
-        return out
-    tokens = plain and m <= _MOST_TOKENS
-    if tokens and a.stride(1) != 1 and k > 1:
-        a = a.contiguous()
-    elif plain and not tokens:
+    if m == 0 or n == 0:
+        return torch.empty((m, n), dtype=dtype, device=b.device)
+    if plain and m <= _MOST_TOKENS:
+        return _tokens(a if a.stride(1) == 1 or k == 1 else a.contiguous(), b, dtype)
+    if plain:
         a = _quantize(a, True, False)[0]
+    out = torch.empty((m, n), dtype=dtype, device=b.device)
     with _native.device_guard(b.device):
-        stream = _native.current_stream_ptr(b.device)
-        if tokens:
-            rc = _native.lib().fo_mxfp4_tokens(a.data_ptr(), DTYPE_CODE[a.dtype], m, a.stride(0), b.codes.data_ptr(), b.scales.data_ptr(),
-                                               n, k, out.data_ptr(), DTYPE_CODE[dtype], stream)
-        else:
-            rc = _native.lib().fo_mxfp4_product(a.codes.data_ptr(), a.scales.data_ptr(), m, b.codes.data_ptr(), b.scales.data_ptr(),
-                                                n, k, out.data_ptr(), DTYPE_CODE[dtype], stream)
-    _native.check(rc, "fo_mxfp4_tokens" if tokens else "fo_mxfp4_product")
+        rc = _native.lib().fo_mxfp4_product(a.codes.data_ptr(), a.scales.data_ptr(), m, b.codes.data_ptr(), b.scales.data_ptr(),
+                                            n, k, out.data_ptr(), DTYPE_CODE[dtype], _native.current_stream_ptr(b.device))
+    _native.check(rc, "fo_mxfp4_product")
     return out
 
 
@@ -240,6 +252,10 @@ def mxfp4_linear(x: torch.Tensor, weight: Union[torch.Tensor, MXFP4Tensor]) -> t
     with Q along rows; the quantisation itself counts as the identity in the backward pass.
     """
     inner = weight.shape[-1]
+    if (type(weight) is MXFP4Tensor and type(x) is torch.Tensor and x.dim() == 2 and x.shape[1] == inner and x.is_cuda
+            and 0 < x.shape[0] <= _MOST_TOKENS and x.stride(1) == 1 and inner and weight.shape[0] and x.dtype in DTYPE_CODE
+            and x.device == weight.codes.device and not x.is_neg() and not (x.requires_grad and torch.is_grad_enabled())):
+        return _tokens(x, weight, x.dtype)  # the call of a decoding step, without the ways round
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] != inner:
         raise ValueError(f"mxfp4_linear: input of shape {tuple(x.shape)} does not fit a weight of shape {tuple(weight.shape)}")
     if weight.device != x.device:

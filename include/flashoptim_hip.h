@@ -283,10 +283,12 @@ int fo_mxfp4_dequantize(const void *codes, const void *scales, int64_t rows, int
 int fo_mxfp4_product(const void *a, const void *a_scales, int64_t rows, const void *b, const void *b_scales, int64_t cols, int64_t inner,
                      void *out, int dtype, void *stream);
 
-/* The same for up to FO_MXFP4_MOST_TOKENS rows that are not quantised yet: one launch quantises and multiplies them */
-#define FO_MXFP4_MOST_TOKENS 16
+/* The same for up to FO_MXFP4_MOST_TOKENS rows that are not quantised yet.  Where fo_mxfp4_tokens_workspace is 0 one launch
+ * quantises and multiplies them; else they are quantised into a workspace of so many bytes of device memory, aligned to 16. */
+#define FO_MXFP4_MOST_TOKENS 64
+int64_t fo_mxfp4_tokens_workspace(int64_t tokens, int64_t inner);
 int fo_mxfp4_tokens(const void *x, int x_dtype, int64_t tokens, int64_t row_stride, const void *weight, const void *weight_scales,
-                    int64_t cols, int64_t inner, void *out, int dtype, void *stream);
+                    int64_t cols, int64_t inner, void *out, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
