@@ -93,69 +93,80 @@ struct QuantizeArgs {
     uint8_t *column_codes, *column_scales;    // of the columns, or null
 };
 
-// A 128 x 128 piece per workgroup: read once, the row form out of registers (a group is four lanes), the column form through LDS
-// (a thread takes 32 rows of a column; two neighbouring columns at once for 2-byte types).  Bound by memory: 2 bytes in, 17/32
-// out per value and form.
-template <int DT> __global__ __launch_bounds__(256) void mx_quantize_kernel(QuantizeArgs a) {
+// A 128 x 128 piece per workgroup: read once, all of it asked for before any of it is used; the row form out of registers (a
+// group is four lanes), the column form through LDS (a thread takes 32 rows of a column, two neighbouring columns one after the
+// other; four neighbouring threads write 64 adjacent bytes).  Bound by memory: 2 bytes in, 17/32 out per value and form.
+template <int DT, bool ROWS, bool COLUMNS> __global__ __launch_bounds__(256) void mx_quantize_kernel(QuantizeArgs a) {
     constexpr int B = DTypeInfo<DT>::bytes, kStride = kBlock * B / 4 + 1;   // dwords, odd: rows begin in different banks
     extern __shared__ u32 lds[];
     const int tile_cols = (a.cols + kBlock - 1) / kBlock;
     const int row0 = blockIdx.x / tile_cols * kBlock, col0 = blockIdx.x % tile_cols * kBlock;
     const int64_t row_bytes = (int64_t)tile_cols * (kBlock / 2);
-    const int piece = threadIdx.x & 15;
+    const int piece = threadIdx.x & 15, line = threadIdx.x >> 4;
     const int col = col0 + piece * 8;
+    Pair<DT> p[8][4];
+    const char* x = a.x + (a.row_stride * (row0 + line) + col) * B;
+    if (row0 + kBlock <= a.rows && col0 + kBlock <= a.cols) {
 #pragma unroll
-    for (int pass = 0; pass < 8; ++pass) {
-        const int r = pass * 16 + (threadIdx.x >> 4), row = row0 + r;
-        Pair<DT> p[4] = {};
-        if (row < a.rows && col < a.cols) load_pairs<DT>(a.x + (a.row_stride * row + col) * B, a.cols - col, p);
-        if (a.codes) {
+        for (int k = 0; k < 8; ++k) load_pairs<DT>(x + a.row_stride * k * 16 * B, 8, p[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) load_pairs<DT>(x + a.row_stride * k * 16 * B, row0 + line + k * 16 < a.rows ? a.cols - col : 0, p[k]);
+    }
+    if constexpr (COLUMNS) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            u32* out = lds + (k * 16 + line) * kStride + piece * 2 * B;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (B == 2) out[i] = p[k][i].v; else { out[2 * i] = as_u32(p[k][i].a); out[2 * i + 1] = as_u32(p[k][i].b); }
+            }
+        }
+    }
+    if constexpr (ROWS) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int row = row0 + line + k * 16;
             u32 m = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { const u32 k = p[i].magnitude(); m = m > k ? m : k; }
+            for (int i = 0; i < 4; ++i) { const u32 e = p[k][i].magnitude(); m = m > e ? m : e; }
             const u32 byte = scale_byte(largest_of_quad(m));
-            const u32 w = byte == 255u ? 0u : encode8<DT>(p, scale_value(byte));
+            const u32 w = byte == 255u ? 0u : encode8<DT>(p[k], scale_value(byte));
             if (row < a.rows) {
                 *reinterpret_cast<u32*>(a.codes + row * row_bytes + col0 / 2 + piece * 4) = w;
                 if ((piece & 3) == 0) a.scales[row * (row_bytes / 16) + col0 / kMxGroup + piece / 4] = (uint8_t)byte;
             }
         }
-        if (a.column_codes) {
-            u32* out = lds + r * kStride + piece * 2 * B;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (B == 2) out[i] = p[i].v; else { out[2 * i] = as_u32(p[i].a); out[2 * i + 1] = as_u32(p[i].b); }
-            }
-        }
     }
-    if (!a.column_codes) return;
-    __syncthreads();
-    const int64_t column_bytes = (int64_t)((a.rows + kBlock - 1) / kBlock) * (kBlock / 2);
-    const int group = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if constexpr (COLUMNS) {
+        __syncthreads();
+        const int64_t column_bytes = (int64_t)((a.rows + kBlock - 1) / kBlock) * (kBlock / 2);
+        const int group = threadIdx.x & 3, pair = threadIdx.x >> 2;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {   // of the wavefront's columns: even and odd ones, or left and right
-        Pair<DT> p[16];
-        const u32* in = lds + group * 32 * kStride + (B == 2 ? lane : lane + half * 64);
-        u32 m = 0;
+        for (int half = 0; half < 2; ++half) {
+            Pair<DT> q[16];
+            const u32* in = lds + group * 32 * kStride + (B == 2 ? pair : pair * 2 + half);
+            u32 m = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const u32 x = in[2 * i * kStride], y = in[(2 * i + 1) * kStride];
-            if constexpr (B == 2) p[i].v = half ? __builtin_amdgcn_perm(y, x, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
-            else { p[i].a = as_f32(x); p[i].b = as_f32(y); }
-            const u32 k = p[i].magnitude();
-            m = m > k ? m : k;
-        }
-        const u32 byte = scale_byte(m);
-        u32x4 w = {0, 0, 0, 0};
-        if (byte != 255u) {
-            const float scale = scale_value(byte);
+            for (int i = 0; i < 16; ++i) {
+                const u32 x = in[2 * i * kStride], y = in[(2 * i + 1) * kStride];
+                if constexpr (B == 2) q[i].v = half ? __builtin_amdgcn_perm(y, x, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
+                else { q[i].a = as_f32(x); q[i].b = as_f32(y); }
+                const u32 e = q[i].magnitude();
+                m = m > e ? m : e;
+            }
+            const u32 byte = scale_byte(m);
+            u32x4 w = {0, 0, 0, 0};
+            if (byte != 255u) {
+                const float scale = scale_value(byte);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = encode8<DT>(p + 4 * i, scale);
-        }
-        const int c = col0 + (B == 2 ? lane * 2 + half : lane + half * 64);
-        if (c < a.cols) {
-            *reinterpret_cast<u32x4*>(a.column_codes + c * column_bytes + row0 / 2 + group * 16) = w;
-            a.column_scales[c * (column_bytes / 16) + row0 / kMxGroup + group] = (uint8_t)byte;
+                for (int i = 0; i < 4; ++i) w[i] = encode8<DT>(q + 4 * i, scale);
+            }
+            const int c = col0 + pair * 2 + half;
+            if (c < a.cols) {
+                *reinterpret_cast<u32x4*>(a.column_codes + c * column_bytes + row0 / 2 + group * 16) = w;
+                a.column_scales[c * (column_bytes / 16) + row0 / kMxGroup + group] = (uint8_t)byte;
+            }
         }
     }
 }
@@ -406,8 +417,11 @@ template <class K, class... Args> int launch(K kernel, int64_t grid, int threads
 }
 
 template <int DT> int launch_quantize(const fo::QuantizeArgs& a, int64_t grid, void* stream) {
-    const int lds = a.column_codes ? fo::kBlock * (fo::kBlock * fo::DTypeInfo<DT>::bytes / 4 + 1) * 4 : 0;
-    return launch(fo::mx_quantize_kernel<DT>, grid, 256, lds, stream, "fo_mxfp4_quantize", a);
+    constexpr int kLds = fo::kBlock * (fo::kBlock * fo::DTypeInfo<DT>::bytes / 4 + 1) * 4;
+    const char* what = "fo_mxfp4_quantize";
+    if (!a.column_codes) return launch(fo::mx_quantize_kernel<DT, true, false>, grid, 256, 0, stream, what, a);
+    if (!a.codes) return launch(fo::mx_quantize_kernel<DT, false, true>, grid, 256, kLds, stream, what, a);
+    return launch(fo::mx_quantize_kernel<DT, true, true>, grid, 256, kLds, stream, what, a);
 }
 
 template <int DT, bool RAW, int TILES, int ROWS> int launch_tokens(const fo::TokensArgs& p, void* stream) {
