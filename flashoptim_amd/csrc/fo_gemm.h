@@ -92,18 +92,23 @@ struct Operand {
 // multiply().  Results feed the next instruction on the same accumulator without a wait, at least three others lie between.
 struct F16Product {
     static constexpr bool kScaled = false;
-    struct Frag { f16x8 v; };
-    __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c) {
-        asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a.v), "v"(b.v));
+    typedef f16x8 Frag;
+    template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int, int) {
+        asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     }
 };
 
+// HALF: which byte of the two scales is meant.
 struct Mx4Product {
     static constexpr bool kScaled = true;
-    struct Frag { i32x4 v; int scale; };
-    __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c) {
-        asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
-            : "+a"(c) : "v"(a.v), "v"(b.v), "v"(a.scale), "v"(b.scale));
+    typedef i32x4 Frag;
+    template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int a_scales, int b_scales) {
+        if constexpr (HALF == 0)
+            asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                : "+a"(c) : "v"(a), "v"(b), "v"(a_scales), "v"(b_scales));
+        else
+            asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                : "+a"(c) : "v"(a), "v"(b), "v"(a_scales), "v"(b_scales));
     }
 };
 
@@ -201,25 +206,47 @@ template <class Product, int WT> struct GemmTile {
         }
     }
 
-    // Operand piece f of the wavefront (0..kFrags-1: B's, then A's) from half `half` of a stage.
-    __device__ __forceinline__ void read(Frag (&fa)[kFrags], Frag (&fb)[kFrags], int f, int stage, int half) const {
+    // What a wavefront multiplies in one phase; of a scaled product also its scales, as read and as the instructions take them.
+    struct Operands { Frag a[kFrags], b[kFrags]; };
+    struct Scales { int a[Product::kScaled ? kFrags : 1], b[Product::kScaled ? kFrags : 1]; };
+
+    // Operand piece f of the wavefront (0..kFrags-1: B's, then A's) for phase `half` of a stage.  Each of the four groups of 16
+    // lanes takes 16-byte piece `group` of eight; the phases of a whole stage take pieces 2 group and 2 group + 1, in any
+    // order the sum is the same and a lane's two scales are neighbours.  short_stage: the stage has four pieces, phase 0 takes them.
+    __device__ __forceinline__ void read(Operands& to, int f, int stage, int half, bool short_stage) const {
         const bool is_b = f < kFrags;
-        const int i = is_b ? f : f - kFrags;
+        const int i = is_b ? f : f - kFrags, group = lane >> 4;
         const int row = (is_b ? kTile + (wave & 1) * WT : (wave >> 1) * WT) + i * 16 + (lane & 15);
-        const char* buffer = smem + (stage & 1) * kBuffer;
-        Frag& out = is_b ? fb[i] : fa[i];
-        out.v = *reinterpret_cast<const decltype(out.v)*>(buffer + row * kStageBytes + (((half * 4 + (lane >> 4)) ^ (row & 7)) * 16));
-        if constexpr (Product::kScaled)
-            out.scale = *reinterpret_cast<const uint8_t*>(buffer + kScaleOffset + row * 8 + half * 4 + (lane >> 4));
+        const int piece = short_stage ? group : 2 * group + half;
+        (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const Frag*>(smem + (stage & 1) * kBuffer + row * kStageBytes + ((piece ^ (row & 7)) * 16));
+    }
+    // The four scale bytes among which the lane's two are.
+    __device__ __forceinline__ void read_scales(Scales& to, int f, int stage, bool short_stage) const {
+        const bool is_b = f < kFrags;
+        const int i = is_b ? f : f - kFrags, group = lane >> 4;
+        const int row = (is_b ? kTile + (wave & 1) * WT : (wave >> 1) * WT) + i * 16 + (lane & 15);
+        (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const int*>(smem + (stage & 1) * kBuffer + kScaleOffset + row * 8 + (short_stage ? 0 : (group >> 1) * 4));
+    }
+    __device__ __forceinline__ void settle(Scales& now, const Scales& raw, bool short_stage) const {
+        if constexpr (Product::kScaled) {
+            const int group = lane >> 4, shift = short_stage ? group * 8 : (group & 1) * 16;
+#pragma unroll
+            for (int i = 0; i < kFrags; ++i) {
+                now.a[i] = (int)((u32)raw.a[i] >> shift);
+                now.b[i] = (int)((u32)raw.b[i] >> shift);
+            }
+        }
     }
 
-    // Multiplies (a, b) while reading the operands of the next phase into (na, nb) and, with LOAD, issuing a stage's loads: at
-    // most one of each between two matrix instructions, fenced so that they stay there (in clumps they hold the wavefront up: 5 %
-    // of the rate at 4096 x 4096 x 8192).  The reads end a quarter before the phase does, so the next finds its operands.
-    template <bool LOAD>
-    __device__ __forceinline__ void phase(const Frag (&a)[kFrags], const Frag (&b)[kFrags], Frag (&na)[kFrags], Frag (&nb)[kFrags],
-                                          int read_stage, int read_half, const Loader& l, int load_stage, bool load_half) {
-        constexpr int kReads = 2 * kFrags, kAll = kFrags * kFrags;
+    // Phase HALF of a stage: multiplies `now` while reading the operands of the next phase and, with LOAD, issuing a stage's loads:
+    // at most one of each between two matrix instructions, fenced so that they stay there (in clumps they hold the wavefront
+    // up: 5 % of the rate at 4096 x 4096 x 8192).  The reads end a quarter before the phase does, so the next finds its operands.
+    template <int HALF, bool LOAD>
+    __device__ __forceinline__ void phase(const Operands& now, const Scales& scales, Operands& next, Scales& next_scales, int read_stage,
+                                          bool read_short, const Loader& l, int load_stage, bool load_half) {
+        constexpr int kAll = kFrags * kFrags;
+        constexpr int kScaleReads = Product::kScaled && HALF == 1 ? kFrags : 0;   // two at a time
+        constexpr int kReads = 2 * kFrags + kScaleReads;
         constexpr int kReadWithin = kAll >= 16 ? kAll - kAll / 4 : kAll;
 #pragma unroll
         for (int q = 0; q < kAll; ++q) {
@@ -232,10 +259,16 @@ template <class Product, int WT> struct GemmTile {
             }
 #pragma unroll
             for (int k = q * kReads / kReadWithin; k < (q + 1) * kReads / kReadWithin && k < kReads; ++k) {
-                read(na, nb, k, read_stage, read_half);
+                if (k < kScaleReads) {
+                    read_scales(next_scales, 2 * k, read_stage, read_short);
+                    read_scales(next_scales, 2 * k + 1, read_stage, read_short);
+                } else {
+                    read(next, k - kScaleReads, read_stage, 1 - HALF, read_short);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            Product::multiply(a[q / kFrags], b[q % kFrags], acc[q / kFrags][q % kFrags]);
+            constexpr int kOnly = Product::kScaled ? 1 : 0;
+            Product::template multiply<HALF>(now.a[q / kFrags], now.b[q % kFrags], acc[q / kFrags][q % kFrags], scales.a[q / kFrags * kOnly], scales.b[q % kFrags * kOnly]);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -253,7 +286,7 @@ template <class Product, int WT> struct GemmTile {
                 keep(acc[i][j]);
             }
         const int stages = (row_bytes + kStageBytes - 1) / kStageBytes;
-        const bool odd = (row_bytes / kHalfBytes) & 1;
+        const bool odd = (row_bytes / kHalfBytes) & 1;   // the last stage is a short one
         Loader l;
         start(l, a, b, row0, col0);
 #pragma unroll
@@ -266,23 +299,31 @@ template <class Product, int WT> struct GemmTile {
             wait_loads<0>();
         }
         meet();
-        Frag a0[kFrags], b0[kFrags], a1[kFrags], b1[kFrags];
+        Operands even, uneven;
+        Scales raw, scales;
+        const bool first_short = odd && stages == 1;
 #pragma unroll
-        for (int f = 0; f < 2 * kFrags; ++f) read(a0, b0, f, 0, 0);
+        for (int f = 0; f < 2 * kFrags; ++f) {
+            read(even, f, 0, 0, first_short);
+            if constexpr (Product::kScaled) read_scales(raw, f, 0, first_short);
+        }
         int s = 0;
         for (; s + 2 < stages; ++s) {
-            phase<false>(a0, b0, a1, b1, s, 1, l, 0, false);
+            settle(scales, raw, false);
+            phase<0, false>(even, scales, uneven, raw, s, false, l, 0, false);
             wait_loads_and_lds();  // stage s is in registers, stage s + 1 in LDS
             meet();
-            phase<true>(a1, b1, a0, b0, s + 1, 0, l, s + 2, odd && s + 3 == stages);
+            phase<1, true>(uneven, scales, even, raw, s + 1, odd && s + 2 == stages, l, s + 2, odd && s + 3 == stages);
         }
         for (;; ++s) {
-            phase<false>(a0, b0, a1, b1, s, 1, l, 0, false);
+            const bool last = s + 1 == stages;
+            settle(scales, raw, odd && last);
+            phase<0, false>(even, scales, uneven, raw, s, false, l, 0, false);
             wait_loads_and_lds();
             meet();
-            if (s + 1 == stages && odd) break;
-            phase<false>(a1, b1, a0, b0, s + 1, 0, l, 0, false);
-            if (s + 1 == stages) break;
+            if (last && odd) break;
+            phase<1, false>(uneven, scales, even, raw, s + 1, odd && s + 2 == stages, l, 0, false);
+            if (last) break;
         }
         asm volatile("s_nop 15\n\ts_nop 3" : : : "memory");  // the last results are written
 #pragma unroll
