@@ -105,6 +105,9 @@ SIGNATURES = {
     "fo_mxfp4_product": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp]),
     "fo_mxfp4_tokens_workspace": (_i64, [_i64, _i64]),
     "fo_mxfp4_tokens": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _vp]),
+    "fo_mxfp4_form_bytes": (_i64, [_i64, _i64]),
+    "fo_mxfp4_linear_forward": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _i64, _i64, _i64] + [_vp] * 4 + [_i64, _vp]),
+    "fo_mxfp4_linear_backward": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _i64, _vp]),
     "fo_muon_step": (_i32, [_vp, _vp, _i64, _i32, _i32, _i32, _f32, _f32, _i32, _i32, _vp, _f32, _vp, _i64, _vp]),
 }
 # include/flashoptim_hip_diag.h: exported by the diagnostics build only (libflashoptim_hip_diag.so, which also

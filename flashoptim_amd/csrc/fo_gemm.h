@@ -451,4 +451,18 @@ __device__ __forceinline__ void tile_at_symmetric(int t, int n, int& i, int& j) 
     }
 }
 
+// ------------------------------------------------------------------------------------------- which tile a launch uses
+// Measured times of tiles, in us: a workgroup alone on its compute unit, and with the unit full of them; `each` per value
+// contracted.
+struct TileCost { int wt, resident; double start, each, start_full, each_full; };
+
+// What `tiles` of them take on `cus` compute units, `length` values contracted: full rounds, then what is left.
+inline double tiles_time(const TileCost& c, double tiles, double length, int cus) {
+    const double seats = (double)cus * c.resident, rounds = __builtin_floor(tiles / seats);
+    const double full = c.start_full + c.each_full * length, alone = c.start + c.each * length;
+    const double left = __builtin_ceil((tiles - rounds * seats) / cus);   // on the fullest unit
+    const double last = left == 0 ? 0.0 : c.resident == 1 ? full : alone + (full - alone) * (left - 1) / (c.resident - 1);
+    return rounds * full + last;
+}
+
 }  // namespace fo

@@ -576,27 +576,25 @@ template <class K, class... Args> int launch(K kernel, int64_t grid, int lds, hi
     return check_hip(hipGetLastError(), what);
 }
 
-// Which tile a product takes: the one whose rounds over the compute units cost least.  A round is one workgroup's tile with
-// `resident` of them on a compute unit; it takes `start` plus `each` per value contracted, in us, fitted to steps of 4096 x
-// 14336, 4096 x 4096, 1024 x 4096 and 1000 x 2730 matrices: 131 us for a 256 x 256 tile over 4096 values, 86 for 192 x 192,
-// 75 for two 128 x 128, 52 for five 64 x 64 (the smaller ones read more of LDS per multiplication), 43 to 17 us over 1000.
-struct TileCost { int wt, resident; double start, each; };
-constexpr TileCost kTileCosts[] = {{128, 1, 14.0, 0.0286}, {96, 1, 16.0, 0.0170}, {64, 2, 8.0, 0.0165}, {32, 5, 7.0, 0.0110}};
+// Which tile a launch takes: the one whose rounds over the compute units take least, by times fitted to steps of 4096 x 14336, 4096 x
+// 4096, 1024 x 4096 and 1000 x 2730 matrices: 131 us for a 256 x 256 tile over 4096 values, 86 for 192 x 192, 75 for two
+// 128 x 128, 52 for five 64 x 64 (the smaller ones read more of LDS per multiplication); 43, 33, 24 (21 alone) and 18 (11) over 1024.
+constexpr fo::TileCost kTileCosts[] = {
+    {128, 1, 14.0, 0.0286, 14.0, 0.0286}, {96, 1, 16.0, 0.0170, 16.0, 0.0170}, {64, 2, 9.5, 0.0115, 8.0, 0.0165}, {32, 5, 4.2, 0.0063, 7.0, 0.0110}};
 
 // tiles(group, wt) of a matrix, length(group) contracted.
 template <class T, class L> int choose(const fo::Groups& a, int cus, T tiles, L length) {
     int best = 0;
     double least = 0.0;
-    for (const TileCost& t : kTileCosts) {
-        double all = 0.0, time = 0.0;
+    for (const fo::TileCost& t : kTileCosts) {
+        double all = 0.0, values = 0.0;
         for (int g = 0; g < a.n; ++g) {
             const double n = (double)tiles(a.group[g], t.wt) * a.group[g].count;
             all += n;
-            time += n * (t.start + t.each * length(a.group[g]));
+            values += n * length(a.group[g]);
         }
-        const double rounds = ceil(all / ((double)cus * t.resident));
-        const double cost = rounds * time / all;
-        if (!best || cost < least) { best = t.wt; least = cost; }
+        const double time = fo::tiles_time(t, all, values / all, cus);
+        if (!best || time < least) { best = t.wt; least = time; }
     }
     return best;
 }

@@ -85,22 +85,29 @@ template <int DT> __device__ __forceinline__ void load_pairs(const char* p, int 
     }
 }
 
-struct QuantizeArgs {
+struct QuantizeJob {
     const char* x;
     int64_t row_stride;   // in elements
     int rows, cols;
     uint8_t *codes, *scales;                  // of the rows, or null
     uint8_t *column_codes, *column_scales;    // of the columns, or null
 };
+struct QuantizeArgs {
+    QuantizeJob job[2];
+    int first_of_second;    // its first workgroup
+};
 
 // A 128 x 128 piece per workgroup: read once, all of it asked for before any of it is used; the row form out of registers (a
 // group is four lanes), the column form through LDS (a thread takes 32 rows of a column, two neighbouring columns one after the
 // other; four neighbouring threads write 64 adjacent bytes).  Bound by memory: 2 bytes in, 17/32 out per value and form.
-template <int DT, bool ROWS, bool COLUMNS> __global__ __launch_bounds__(256) void mx_quantize_kernel(QuantizeArgs a) {
+template <int DT, bool ROWS, bool COLUMNS> __global__ __launch_bounds__(256) void mx_quantize_kernel(QuantizeArgs args) {
+    const bool second = (int)blockIdx.x >= args.first_of_second;
+    const QuantizeJob& a = args.job[second];
+    const int tile = (int)blockIdx.x - (second ? args.first_of_second : 0);
     constexpr int B = DTypeInfo<DT>::bytes, kStride = kBlock * B / 4 + 1;   // dwords, odd: rows begin in different banks
     extern __shared__ u32 lds[];
     const int tile_cols = (a.cols + kBlock - 1) / kBlock;
-    const int row0 = blockIdx.x / tile_cols * kBlock, col0 = blockIdx.x % tile_cols * kBlock;
+    const int row0 = tile / tile_cols * kBlock, col0 = tile % tile_cols * kBlock;
     const int64_t row_bytes = (int64_t)tile_cols * (kBlock / 2);
     const int piece = threadIdx.x & 15, line = threadIdx.x >> 4;
     const int col = col0 + piece * 8;
@@ -123,7 +130,7 @@ template <int DT, bool ROWS, bool COLUMNS> __global__ __launch_bounds__(256) voi
             }
         }
     }
-    if constexpr (ROWS) {
+    if (ROWS && a.codes) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int row = row0 + line + k * 16;
@@ -139,6 +146,7 @@ template <int DT, bool ROWS, bool COLUMNS> __global__ __launch_bounds__(256) voi
         }
     }
     if constexpr (COLUMNS) {
+        if (!a.column_codes) return;
         __syncthreads();
         const int64_t column_bytes = (int64_t)((a.rows + kBlock - 1) / kBlock) * (kBlock / 2);
         const int group = threadIdx.x & 3, pair = threadIdx.x >> 2;
@@ -193,12 +201,16 @@ template <int DT> __global__ __launch_bounds__(256) void mx_dequantize_kernel(co
 // ------------------------------------------------------------------------------------------------
 // products
 // ------------------------------------------------------------------------------------------------
-struct ProductArgs {
+struct ProductJob {
     const char *a, *b;                  // codes
     const uint8_t *a_scales, *b_scales;
     char* out;
     int rows, cols, blocks;             // of the result; 128-value blocks of the contracted axis
     int dtype;
+};
+struct ProductArgs {
+    ProductJob job[2];
+    int seats_of_first;                 // of each die (fo_gemm.h)
 };
 
 struct ProductOut {
@@ -217,11 +229,14 @@ struct ProductOut {
     }
 };
 
-template <int WT> __global__ __launch_bounds__(256, WT == 128 ? 1 : 2) void mx_product_kernel(ProductArgs p) {
+template <int WT> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void mx_product_kernel(ProductArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmTile<Mx4Product, WT> Tile;
+    const int seat = (int)(blockIdx.x >> 3);
+    const bool second = seat >= args.seats_of_first;
+    const ProductJob& p = args.job[second];
     const int rows = (p.rows + Tile::kTile - 1) / Tile::kTile, cols = (p.cols + Tile::kTile - 1) / Tile::kTile;
-    const int64_t t = tile_of_seat(blockIdx.x & 7, blockIdx.x >> 3, (int64_t)rows * cols);
+    const int64_t t = tile_of_seat(blockIdx.x & 7, seat - (second ? args.seats_of_first : 0), (int64_t)rows * cols);
     if (t < 0) return;
     int i, j;
     tile_at((int)t, rows, cols, i, j);
@@ -416,12 +431,35 @@ template <class K, class... Args> int launch(K kernel, int64_t grid, int threads
     return check_hip(hipGetLastError(), what);
 }
 
-template <int DT> int launch_quantize(const fo::QuantizeArgs& a, int64_t grid, void* stream) {
+// One matrix and where its forms go: codes, then scales.
+fo::QuantizeJob quantize_job(const void* x, int64_t rows, int64_t cols, int64_t row_stride, void* codes, void* scales, void* column_codes, void* column_scales) {
+    return {(const char*)x, row_stride, (int)rows, (int)cols, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)column_codes, (uint8_t*)column_scales};
+}
+int64_t form_codes(int64_t rows, int64_t cols) { return rows * blocks_of(cols) * 64; }
+int64_t form_bytes(int64_t rows, int64_t cols) { return (rows * blocks_of(cols) * 68 + 255) / 256 * 256; }
+
+template <int DT> int launch_quantize(const fo::QuantizeJob* jobs, int n, void* stream) {
     constexpr int kLds = fo::kBlock * (fo::kBlock * fo::DTypeInfo<DT>::bytes / 4 + 1) * 4;
     const char* what = "fo_mxfp4_quantize";
-    if (!a.column_codes) return launch(fo::mx_quantize_kernel<DT, true, false>, grid, 256, 0, stream, what, a);
-    if (!a.codes) return launch(fo::mx_quantize_kernel<DT, false, true>, grid, 256, kLds, stream, what, a);
+    fo::QuantizeArgs a{};
+    int64_t grid = 0;
+    bool rows = false, columns = false;
+    for (int i = 0; i < n; ++i) {
+        a.job[i] = jobs[i];
+        if (i == 1) a.first_of_second = (int)grid;
+        grid += blocks_of(jobs[i].rows) * blocks_of(jobs[i].cols);
+        if (grid > kMostWorkgroups) return fail(FO_ERR_UNSUPPORTED, "%s: too many values for one launch", what);
+        rows |= jobs[i].codes != nullptr;
+        columns |= jobs[i].column_codes != nullptr;
+    }
+    if (n == 1) a.first_of_second = (int)grid;
+    if (!columns) return launch(fo::mx_quantize_kernel<DT, true, false>, grid, 256, 0, stream, what, a);
+    if (!rows) return launch(fo::mx_quantize_kernel<DT, false, true>, grid, 256, kLds, stream, what, a);
     return launch(fo::mx_quantize_kernel<DT, true, true>, grid, 256, kLds, stream, what, a);
+}
+int launch_quantize(int dtype, const fo::QuantizeJob* jobs, int n, void* stream) {
+    if (dtype == FO_F32) return launch_quantize<fo::DT_F32>(jobs, n, stream);
+    return dtype == FO_BF16 ? launch_quantize<fo::DT_BF16>(jobs, n, stream) : launch_quantize<fo::DT_F16>(jobs, n, stream);
 }
 
 template <int DT, bool RAW, int TILES, int ROWS> int launch_tokens(const fo::TokensArgs& p, void* stream) {
@@ -447,7 +485,71 @@ int launch_coded_tokens(const fo::TokensArgs& p, void* stream) {
     return p.tokens <= 32 ? launch_coded_tokens<2>(p, stream) : launch_coded_tokens<4>(p, stream);
 }
 
-int64_t tiles(int64_t rows, int64_t cols, int tile) { return ((rows + tile - 1) / tile) * ((cols + tile - 1) / tile); }
+// Times of 4096 x 4096 products (3840 x 3840 for 192 x 192 tiles) over 1024 to 16384 values: a 256 x 256 tile takes 40 us over 4096 and
+// 130 over 16384, two 128 x 128 tiles on a compute unit 26 and 90 (alone 18 and 62), five 64 x 64 21 and 75 (two of them 13 and 44).
+constexpr fo::TileCost kTileCosts[] = {
+    {128, 1, 11.5, 0.0073, 11.5, 0.0073}, {96, 1, 8.0, 0.0046, 8.0, 0.0046}, {64, 2, 3.5, 0.0036, 5.0, 0.0052}, {32, 5, 2.0, 0.0022, 5.0, 0.0043}};
+
+int64_t tiles(const fo::ProductJob& p, int wt) { return (int64_t)((p.rows + 2 * wt - 1) / (2 * wt)) * ((p.cols + 2 * wt - 1) / (2 * wt)); }
+
+template <int WT> int launch_products(const fo::ProductJob* jobs, int n, void* stream) {
+    fo::ProductArgs a{};
+    int64_t seats = 0;
+    for (int i = 0; i < n; ++i) {
+        a.job[i] = jobs[i];
+        if (i == 1) a.seats_of_first = (int)seats;
+        seats += fo::seats_of(tiles(jobs[i], WT));
+        if (seats > kMostWorkgroups) return fail(FO_ERR_UNSUPPORTED, "fo_mxfp4_product: too large a result for one launch");
+    }
+    if (n == 1) a.seats_of_first = (int)seats;
+    return launch(fo::mx_product_kernel<WT>, 8 * seats, 256, fo::GemmTile<fo::Mx4Product, WT>::kLds, stream, "fo_mxfp4_product", a);
+}
+
+// Up to two products in one launch, the longer contraction first.
+int launch_products(fo::ProductJob* jobs, int n, void* stream) {
+    const int cus = compute_units();
+    if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
+    if (n == 2 && jobs[0].blocks < jobs[1].blocks) { const fo::ProductJob t = jobs[0]; jobs[0] = jobs[1]; jobs[1] = t; }
+    int best = 0;
+    double least = 0.0;
+    for (const fo::TileCost& c : kTileCosts) {
+        double all = 0.0, values = 0.0;
+        for (int i = 0; i < n; ++i) { all += (double)tiles(jobs[i], c.wt); values += (double)tiles(jobs[i], c.wt) * jobs[i].blocks * fo::kBlock; }
+        const double time = fo::tiles_time(c, all, values / all, cus);
+        if (!best || time < least) { best = c.wt; least = time; }
+    }
+    switch (best) {
+        case 128: return launch_products<128>(jobs, n, stream);
+        case 96: return launch_products<96>(jobs, n, stream);
+        case 64: return launch_products<64>(jobs, n, stream);
+        default: return launch_products<32>(jobs, n, stream);
+    }
+}
+
+fo::TokensArgs tokens_of(const fo::ProductJob& p) {
+    return {p.a, p.a_scales, p.b, p.b_scales, p.out, p.rows, p.cols, p.blocks * fo::kBlock, p.blocks, 0, p.dtype};
+}
+// The kernel for few rows for those that have few, one launch for the others.
+int run_products(const fo::ProductJob* jobs, int n, void* stream) {
+    fo::ProductJob large[2];
+    int k = 0;
+    for (int i = 0; i < n; ++i) {
+        if (jobs[i].rows > FO_MXFP4_MOST_TOKENS) { large[k++] = jobs[i]; continue; }
+        if (int rc = launch_coded_tokens(tokens_of(jobs[i]), stream)) return rc;
+    }
+    return k ? launch_products(large, k, stream) : 0;
+}
+
+// A product of two forms: codes, then scales.
+fo::ProductJob product_of(const void* a, int64_t rows, const void* b, int64_t cols, int64_t inner, void* out, int dtype) {
+    return {(const char*)a, (const char*)b, (const uint8_t*)a + form_codes(rows, inner), (const uint8_t*)b + form_codes(cols, inner), (char*)out,
+            (int)rows, (int)cols, (int)blocks_of(inner), dtype};
+}
+
+int check_forms(const void* a, const void* b, const void* c) {
+    if (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15) return fail(FO_ERR_INVALID_ARGUMENT, "forms and workspace must be aligned to 16 bytes");
+    return 0;
+}
 
 }  // namespace
 
@@ -460,13 +562,8 @@ int fo_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int6
     if (rows == 0 || cols == 0) return 0;
     if (!x) return fail(FO_ERR_INVALID_ARGUMENT, "x must not be NULL");
     if (((uintptr_t)codes | (uintptr_t)column_codes) & 15) return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes");
-    const fo::QuantizeArgs a{(const char*)x, row_stride, (int)rows, (int)cols, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)column_codes, (uint8_t*)column_scales};
-    const int64_t grid = blocks_of(rows) * blocks_of(cols);
-    switch (dtype) {
-        case FO_F32: return launch_quantize<fo::DT_F32>(a, grid, stream);
-        case FO_BF16: return launch_quantize<fo::DT_BF16>(a, grid, stream);
-        default: return launch_quantize<fo::DT_F16>(a, grid, stream);
-    }
+    const fo::QuantizeJob job = quantize_job(x, rows, cols, row_stride, codes, scales, column_codes, column_scales);
+    return launch_quantize(dtype, &job, 1, stream);
 }
 
 int fo_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype, void* stream) {
@@ -492,20 +589,8 @@ int fo_mxfp4_product(const void* a, const void* a_scales, int64_t rows, const vo
     if (!a || !a_scales || !b || !b_scales || !out) return fail(FO_ERR_INVALID_ARGUMENT, "operands and out must not be NULL");
     if (((uintptr_t)a | (uintptr_t)b) & 15 || ((uintptr_t)a_scales | (uintptr_t)b_scales) & 3)
         return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes, scales to 4");
-    const int64_t blocks = blocks_of(inner);
-    if (rows <= FO_MXFP4_MOST_TOKENS) {
-        const fo::TokensArgs p{(const char*)a, (const uint8_t*)a_scales, (const char*)b, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)inner, (int)blocks, 0, dtype};
-        return launch_coded_tokens(p, stream);
-    }
-    const fo::ProductArgs p{(const char*)a, (const char*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)blocks, dtype};
-    const int cus = compute_units();
-    if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
-    const char* what = "fo_mxfp4_product";
-    if (tiles(rows, cols, 256) >= cus)
-        return launch(fo::mx_product_kernel<128>, 8 * fo::seats_of(tiles(rows, cols, 256)), 256, fo::GemmTile<fo::Mx4Product, 128>::kLds, stream, what, p);
-    if (tiles(rows, cols, 128) >= cus)
-        return launch(fo::mx_product_kernel<64>, 8 * fo::seats_of(tiles(rows, cols, 128)), 256, fo::GemmTile<fo::Mx4Product, 64>::kLds, stream, what, p);
-    return launch(fo::mx_product_kernel<32>, 8 * fo::seats_of(tiles(rows, cols, 64)), 256, fo::GemmTile<fo::Mx4Product, 32>::kLds, stream, what, p);
+    const fo::ProductJob job{(const char*)a, (const char*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)blocks_of(inner), dtype};
+    return run_products(&job, 1, stream);
 }
 
 int64_t fo_mxfp4_tokens_workspace(int64_t tokens, int64_t inner) {
@@ -538,5 +623,63 @@ int fo_mxfp4_tokens(const void* x, int x_dtype, int64_t tokens, int64_t row_stri
         case FO_BF16: return launch_raw_tokens<fo::DT_BF16>(p, stream);
         default: return launch_raw_tokens<fo::DT_F16>(p, stream);
     }
+}
+
+int64_t fo_mxfp4_form_bytes(int64_t rows, int64_t cols) {
+    if (int rc = validate_matrix("fo_mxfp4_form_bytes", rows, cols, FO_F32)) return rc;
+    return form_bytes(rows, cols);
+}
+
+int fo_mxfp4_linear_forward(const void* x, int x_dtype, int64_t tokens, int64_t x_stride, const void* weight, int weight_dtype, int64_t outer,
+                            int64_t weight_stride, int64_t inner, void* x_columns, void* weight_columns, void* out, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+    const char* what = "fo_mxfp4_linear_forward";
+    if (int rc = validate_matrix(what, tokens, inner, x_dtype)) return rc;
+    if (int rc = validate_matrix(what, outer, inner, weight_dtype)) return rc;
+    if (tokens == 0 || outer == 0) return fail(FO_ERR_UNSUPPORTED, "%s: an empty product", what);
+    if (int rc = validate_inner(what, inner)) return rc;
+    if (!x || !weight || !out || !workspace) return fail(FO_ERR_INVALID_ARGUMENT, "x, weight, out and workspace must not be NULL");
+    if (int rc = check_forms(x_columns, weight_columns, workspace)) return rc;
+    const int64_t x_form = form_bytes(tokens, inner);
+    if (workspace_bytes < x_form + form_bytes(outer, inner)) return fail(FO_ERR_INVALID_ARGUMENT, "workspace too small");
+    char *xr = (char*)workspace, *wr = xr + x_form;
+    const fo::QuantizeJob jobs[2] = {
+        quantize_job(x, tokens, inner, x_stride, xr, xr + form_codes(tokens, inner), x_columns, x_columns ? (char*)x_columns + form_codes(inner, tokens) : nullptr),
+        quantize_job(weight, outer, inner, weight_stride, wr, wr + form_codes(outer, inner), weight_columns, weight_columns ? (char*)weight_columns + form_codes(inner, outer) : nullptr)};
+    if (x_dtype == weight_dtype) {
+        if (int rc = launch_quantize(x_dtype, jobs, 2, stream)) return rc;
+    } else {
+        if (int rc = launch_quantize(x_dtype, jobs, 1, stream)) return rc;
+        if (int rc = launch_quantize(weight_dtype, jobs + 1, 1, stream)) return rc;
+    }
+    const fo::ProductJob y = product_of(xr, tokens, wr, outer, inner, out, x_dtype);
+    return run_products(&y, 1, stream);
+}
+
+int fo_mxfp4_linear_backward(const void* dy, int dy_dtype, int64_t tokens, int64_t dy_stride, int64_t outer, int64_t inner, const void* x_columns,
+                             const void* weight_columns, void* dx, int dx_dtype, void* dw, int dw_dtype, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+    const char* what = "fo_mxfp4_linear_backward";
+    if (int rc = validate_matrix(what, tokens, outer, dy_dtype)) return rc;
+    if (int rc = validate_matrix(what, outer, inner, dx_dtype)) return rc;
+    if (int rc = validate_matrix(what, tokens, inner, dw_dtype)) return rc;
+    if (tokens == 0 || inner == 0) return fail(FO_ERR_UNSUPPORTED, "%s: an empty product", what);
+    if (int rc = validate_inner(what, outer)) return rc;
+    if (int rc = validate_inner(what, tokens)) return rc;
+    if (!dy || !workspace || !dx != !weight_columns || !dw != !x_columns || (!dx && !dw))
+        return fail(FO_ERR_INVALID_ARGUMENT, "dy, workspace, and dx with weight_columns or dw with x_columns or both must be given");
+    if (int rc = check_forms(x_columns, weight_columns, workspace)) return rc;
+    const int64_t row_form = dx ? form_bytes(tokens, outer) : 0;
+    if (workspace_bytes < row_form + (dw ? form_bytes(outer, tokens) : 0)) return fail(FO_ERR_INVALID_ARGUMENT, "workspace too small");
+    char* rows = dx ? (char*)workspace : nullptr;
+    char* columns = dw ? (char*)workspace + row_form : nullptr;
+    const fo::QuantizeJob job = quantize_job(dy, tokens, outer, dy_stride, rows, rows ? rows + form_codes(tokens, outer) : nullptr, columns,
+                                             columns ? columns + form_codes(outer, tokens) : nullptr);
+    if (int rc = launch_quantize(dy_dtype, &job, 1, stream)) return rc;
+    fo::ProductJob products[2];
+    int n = 0;
+    if (dx) products[n++] = product_of(rows, tokens, weight_columns, inner, outer, dx, dx_dtype);
+    if (dw) products[n++] = product_of(columns, outer, x_columns, inner, tokens, dw, dw_dtype);
+    return run_products(products, n, stream);
 }
 }  // extern "C"

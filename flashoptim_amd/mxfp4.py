@@ -69,14 +69,17 @@ def _check_matrix(x: torch.Tensor, what: str) -> torch.Tensor:
         raise ValueError(f"{what} expects fp32, bf16 or fp16 input, got {x.dtype}.")
     if x.dim() != 2:
         raise ValueError(f"{what} expects a matrix, got shape {tuple(x.shape)}.")
-    x = x.detach()
+    if x.requires_grad:
+        x = x.detach()
     return x.resolve_neg() if x.is_neg() else x
 
 
 def _empty(rows: int, cols: int, device: torch.device) -> MXFP4Tensor:
-    codes = torch.empty((rows, 64 * _blocks(cols)), dtype=torch.uint8, device=device)
-    scales = torch.empty((rows, 4 * _blocks(cols)), dtype=torch.uint8, device=device)
-    return MXFP4Tensor(codes, scales, (rows, cols))
+    q = MXFP4Tensor.__new__(MXFP4Tensor)  # what is made here needs no check
+    q.codes = torch.empty((rows, 64 * _blocks(cols)), dtype=torch.uint8, device=device)
+    q.scales = torch.empty((rows, 4 * _blocks(cols)), dtype=torch.uint8, device=device)
+    q.shape = (rows, cols)
+    return q
 
 
 def _quantize(x: torch.Tensor, rows: bool, columns: bool) -> tuple[Optional[MXFP4Tensor], Optional[MXFP4Tensor]]:
@@ -90,7 +93,8 @@ def _quantize(x: torch.Tensor, rows: bool, columns: bool) -> tuple[Optional[MXFP
     by_row = _empty(r, c, x.device) if rows else None
     by_column = _empty(c, r, x.device) if columns else None
     if x.numel() > 0:
-        ptr = [None if t is None else getattr(t, k).data_ptr() for t in (by_row, by_column) for k in ("codes", "scales")]
+        ptr = [None if t is None else p for t in (by_row, by_column)
+               for p in ((None, None) if t is None else (t.codes.data_ptr(), t.scales.data_ptr()))]
         with _native.device_guard(x.device):
             rc = _native.lib().fo_mxfp4_quantize(x.data_ptr(), DTYPE_CODE[x.dtype], r, c, x.stride(0), *ptr,
                                                  _native.current_stream_ptr(x.device))
@@ -181,6 +185,14 @@ def mxfp4_matmul(a: Union[MXFP4Tensor, torch.Tensor], b: MXFP4Tensor, dtype: tor
     return out
 
 
+def _form_bytes(rows: int, cols: int) -> int:
+    return (rows * _blocks(cols) * 68 + 255) // 256 * 256  # fo_mxfp4_form_bytes
+
+
+def _adjacent(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+
+
 class _Linear(torch.autograd.Function):
     """x (tokens, in) and weight (out, in) to x weight', every product on MXFP4 forms of its operands along the contracted axis.
 
@@ -193,27 +205,54 @@ class _Linear(torch.autograd.Function):
         need_dx, need_dw = ctx.needs_input_grad
         ctx.dtypes, ctx.shapes = (x.dtype, weight.dtype), (x.shape, weight.shape)
         x, weight = _check_matrix(x, "mxfp4_linear"), _check_matrix(weight, "mxfp4_linear")
-        if need_dw or x.shape[0] > _MOST_TOKENS:
-            xr, xc = _quantize(x, True, need_dw)
-        else:
-            xr, xc = x, None
-        wr, wc = _quantize(weight, True, need_dx)
-        saved = [t for q in (xc, wc) if q is not None for t in (q.codes, q.scales)]
-        ctx.save_for_backward(*saved)
-        return mxfp4_matmul(xr, wr, x.dtype)
+        (tokens, inner), outer = x.shape, weight.shape[0]
+        if not (tokens and inner and outer):
+            ctx.save_for_backward()
+            return torch.zeros((tokens, outer), dtype=x.dtype, device=x.device)
+        x, weight = _adjacent(x), _adjacent(weight)
+        device = x.device
+        # the column forms of x and of the weight, kept; the row forms, used here
+        x_bytes, w_bytes = _form_bytes(inner, tokens) if need_dw else 0, _form_bytes(inner, outer) if need_dx else 0
+        kept = torch.empty(x_bytes + w_bytes, dtype=torch.uint8, device=device)
+        used = _form_bytes(tokens, inner) + _form_bytes(outer, inner)
+        workspace = torch.empty(used, dtype=torch.uint8, device=device)
+        y = torch.empty((tokens, outer), dtype=x.dtype, device=device)
+        at = kept.data_ptr()
+        with _native.device_guard(device):
+            rc = _native.lib().fo_mxfp4_linear_forward(
+                x.data_ptr(), DTYPE_CODE[x.dtype], tokens, x.stride(0), weight.data_ptr(), DTYPE_CODE[weight.dtype], outer, weight.stride(0),
+                inner, at if need_dw else None, at + x_bytes if need_dx else None, y.data_ptr(), workspace.data_ptr(), used,
+                _native.current_stream_ptr(device))
+        if rc:
+            _native.check(rc, "fo_mxfp4_linear_forward")
+        ctx.save_for_backward(kept)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         need_dx, need_dw = ctx.needs_input_grad
         (tokens, inner), (outer, _) = ctx.shapes
-        saved = list(ctx.saved_tensors)
-        xc = MXFP4Tensor(saved.pop(0), saved.pop(0), (inner, tokens)) if need_dw else None
-        wc = MXFP4Tensor(saved.pop(0), saved.pop(0), (inner, outer)) if need_dx else None
-        dy = _check_matrix(dy, "mxfp4_linear backward")
-        by_row, by_column = _quantize(dy, need_dx, need_dw)
-        dx = mxfp4_matmul(by_row, wc, ctx.dtypes[0]) if need_dx else None
-        dw = mxfp4_matmul(by_column, xc, ctx.dtypes[1]) if need_dw else None
+        device = dy.device
+        empty = not (tokens and inner and outer)
+        make = torch.zeros if empty else torch.empty
+        dx = make((tokens, inner), dtype=ctx.dtypes[0], device=device) if need_dx else None
+        dw = make((outer, inner), dtype=ctx.dtypes[1], device=device) if need_dw else None
+        if empty:
+            return dx, dw
+        (kept,) = ctx.saved_tensors
+        dy = _adjacent(_check_matrix(dy, "mxfp4_linear backward"))
+        at = kept.data_ptr()
+        x_bytes = _form_bytes(inner, tokens) if need_dw else 0
+        used = (_form_bytes(tokens, outer) if need_dx else 0) + (_form_bytes(outer, tokens) if need_dw else 0)
+        workspace = torch.empty(used, dtype=torch.uint8, device=device)
+        with _native.device_guard(device):
+            rc = _native.lib().fo_mxfp4_linear_backward(
+                dy.data_ptr(), DTYPE_CODE[dy.dtype], tokens, dy.stride(0), outer, inner, at if need_dw else None, at + x_bytes if need_dx else None,
+                _native.ptr(dx), DTYPE_CODE[ctx.dtypes[0]], _native.ptr(dw), DTYPE_CODE[ctx.dtypes[1]], workspace.data_ptr(), used,
+                _native.current_stream_ptr(device))
+        if rc:
+            _native.check(rc, "fo_mxfp4_linear_backward")
         return dx, dw
 
 
@@ -260,7 +299,7 @@ def mxfp4_linear(x: torch.Tensor, weight: Union[torch.Tensor, MXFP4Tensor]) -> t
         raise ValueError(f"mxfp4_linear: input of shape {tuple(x.shape)} does not fit a weight of shape {tuple(weight.shape)}")
     if weight.device != x.device:
         raise ValueError(f"weight is on {weight.device}, expected {x.device}.")
-    tokens = x.reshape(-1, inner) if inner else x.reshape(x.shape[:-1].numel(), 0)
+    tokens = x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), inner)
     if isinstance(weight, MXFP4Tensor):
         if torch.is_grad_enabled() and x.requires_grad:
             y = _FrozenLinear.apply(tokens, weight.codes, weight.scales, weight.shape)
@@ -270,6 +309,8 @@ def mxfp4_linear(x: torch.Tensor, weight: Union[torch.Tensor, MXFP4Tensor]) -> t
         if weight.dim() != 2:
             raise ValueError(f"mxfp4_linear expects a matrix as weight, got shape {tuple(weight.shape)}.")
         y = _Linear.apply(tokens, weight)
+        if x.dim() == 2:
+            return y
     return y.reshape(*x.shape[:-1], weight.shape[0])
 
 

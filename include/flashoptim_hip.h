@@ -290,6 +290,23 @@ int64_t fo_mxfp4_tokens_workspace(int64_t tokens, int64_t inner);
 int fo_mxfp4_tokens(const void *x, int x_dtype, int64_t tokens, int64_t row_stride, const void *weight, const void *weight_scales,
                     int64_t cols, int64_t inner, void *out, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * A linear layer, y = x weight', its products in this format.  A form here is a matrix's codes followed by its scales,
+ * fo_mxfp4_form_bytes(rows, cols) bytes of it, aligned to 16 bytes.
+ * Forward: x is tokens x inner, weight outer x inner, out tokens x outer of x's type.  x_columns (inner x tokens) and
+ * weight_columns (inner x outer), the forms of the transposes, are what the backward pass needs; either may be NULL.
+ *   workspace: the forms of x and of weight.
+ * Backward: dy is tokens x outer; dx = dy weight (tokens x inner) needs weight_columns, dw = dy' x (outer x inner) x_columns; either
+ * may be left out (NULL).  workspace: the form of dy for dx, of its transpose for dw.
+ */
+int64_t fo_mxfp4_form_bytes(int64_t rows, int64_t cols);
+int fo_mxfp4_linear_forward(const void *x, int x_dtype, int64_t tokens, int64_t x_stride, const void *weight, int weight_dtype, int64_t outer,
+                            int64_t weight_stride, int64_t inner, void *x_columns, void *weight_columns, void *out, void *workspace,
+                            int64_t workspace_bytes, void *stream);
+int fo_mxfp4_linear_backward(const void *dy, int dy_dtype, int64_t tokens, int64_t dy_stride, int64_t outer, int64_t inner, const void *x_columns,
+                             const void *weight_columns, void *dx, int dx_dtype, void *dw, int dw_dtype, void *workspace,
+                             int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
