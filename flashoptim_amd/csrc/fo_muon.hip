@@ -7,8 +7,8 @@
 // Precision.  The products run on the matrix cores in fp16 with fp32 sums.  Rounding X itself to fp16 in every step would
 // cost up to 1e-2 of the result: an error among the small singular directions is multiplied like the signal there (3.4 per
 // step).  So X is held in two parts, hi (fp16, the operand of the products) and lo (bf16, the rest, 19 bits or more together); lo
-// enters where X is multiplied by a.  The diagonal of B, by far its largest entries on a flat spectrum, is kept apart in
-// fp32 and added to a; the products see B without it.  What is left (S and B off the diagonal in fp16) costs 1e-4 .. 8e-4
+// enters where X is multiplied by a.  The diagonals of S and B, by far their largest entries on a flat spectrum, are kept apart
+// in fp32; the products see the matrices without them: S S = O O + O D + D O + D D for S = O + D, and B's is added to a.  What is left (S and B off the diagonal in fp16) costs 1e-4 .. 8e-4
 // of the result, below the bfloat16 rounding it is handed out with.  X starts at |X|_F = 1, entries as small as 1e-4, so
 // the first X is kept times a power of two near sqrt(n), in fp16's normal range.
 //
@@ -47,10 +47,10 @@ struct MatrixGroup {
     __host__ __device__ int side() const { return tall() ? padded_cols : padded_rows; }
     __host__ __device__ int64_t area() const { return (int64_t)padded_rows * padded_cols; }
     __host__ __device__ int64_t gram_area() const { return (int64_t)side() * side(); }
-    // per matrix: two generations of hi and of T, lo, S, B, the diagonal of B, the factor that normalises, sums of squares.
+    // per matrix: two generations of hi and of T, lo, S, B, their diagonals, the factor that normalises, sums of squares.
     // The update before its normalisation (fp32) lies over the second generation, which is written later.
     __host__ __device__ int64_t bytes_each() const {
-        return area() * 10 + gram_area() * 4 + side() * 4 + 256 + ((int64_t)chunks * 8 + 255) / 256 * 256;
+        return area() * 10 + gram_area() * 4 + side() * 8 + 256 + ((int64_t)chunks * 8 + 255) / 256 * 256;
     }
     __device__ char* of(int k) const { return workspace + bytes_each() * k; }
     __device__ _Float16* hi(int k, int generation) const { return (_Float16*)(of(k) + generation * area() * 4); }
@@ -59,7 +59,8 @@ struct MatrixGroup {
     __device__ u32* lo(int k) const { return (u32*)(of(k) + area() * 8); }   // pairs of bf16
     __device__ _Float16* s(int k) const { return (_Float16*)(of(k) + area() * 10); }
     __device__ _Float16* b(int k) const { return (_Float16*)(of(k) + area() * 10 + gram_area() * 2); }
-    __device__ float* diagonal(int k) const { return (float*)(of(k) + area() * 10 + gram_area() * 4); }
+    __device__ float* s_diagonal(int k) const { return (float*)(of(k) + area() * 10 + gram_area() * 4); }
+    __device__ float* diagonal(int k) const { return s_diagonal(k) + side(); }   // of B
     __device__ float* factor(int k) const { return diagonal(k) + side(); }
     __device__ double* squares(int k) const { return (double*)((char*)factor(k) + 256); }
 };
@@ -289,31 +290,44 @@ __device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
     return h;
 }
 
-// S, and B without its diagonal: rows of a symmetric matrix, each tile off the diagonal twice.
+// S and B without their diagonals: rows of a symmetric matrix, each tile off the diagonal twice.
 template <bool GRAM> struct SymmetricOut {
     static constexpr bool kColumns = true;
-    const _Float16* s;      // what B is made of
+    const _Float16* s;            // what B is made of,
+    const float* s_diagonal;      // with its diagonal
     _Float16* out;
     float* diagonal;
     int side;
     float scale, b, c;
     bool mirror;
+    float d[8];                   // of the lane's columns
 
-    struct In { f16x8 s; };
-    __device__ __forceinline__ void begin(int) const {}
+    struct In { f16x8 s; float d; };
+    __device__ __forceinline__ void begin(int j) {
+        if constexpr (!GRAM) {
+            if (j < side) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[e] = s_diagonal[j + e];
+            }
+        }
+    }
     __device__ __forceinline__ void load(int i, int j, In& in) const {
-        if constexpr (!GRAM) { if (i < side && j < side) in.s = *reinterpret_cast<const f16x8*>(s + (int64_t)i * side + j); }
+        if constexpr (!GRAM) {
+            if (i < side && j < side) {
+                in.s = *reinterpret_cast<const f16x8*>(s + (int64_t)i * side + j);
+                in.d = s_diagonal[i];
+            }
+        }
     }
     __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
         if (i >= side || j >= side) return;
-        if constexpr (GRAM) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= scale;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] = fmaf(c, v[e], b * (float)in.s[e]);
-                if (i == j + e) { diagonal[i] = v[e]; v[e] = 0.0f; }
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (GRAM) v[e] *= scale;
+            else v[e] = fmaf(c, fmaf(in.d + d[e], (float)in.s[e], v[e]), b * (float)in.s[e]);
+            if (i == j + e) {   // B: v is c O O here, S's entry is not in it
+                diagonal[i] = GRAM ? v[e] : fmaf(in.d, fmaf(c, in.d, b), v[e]);
+                v[e] = 0.0f;
             }
         }
         *reinterpret_cast<f16x8*>(out + (int64_t)i * side + j) = half8(v);
@@ -343,7 +357,8 @@ template <int WT, bool GRAM> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2)
     const Operand op{(const char*)x, length, nullptr, 0, side};
     Tile tile(lds);
     tile.multiply(op, op, i * Tile::kTile, j * Tile::kTile, (int)length);
-    SymmetricOut<GRAM> out{m.s(k), GRAM ? m.s(k) : m.b(k), m.diagonal(k), side, h.first ? 1.0f / (m.unit * m.unit) : 1.0f, h.b, h.c, i != j};
+    SymmetricOut<GRAM> out{m.s(k), m.s_diagonal(k), GRAM ? m.s(k) : m.b(k), GRAM ? m.s_diagonal(k) : m.diagonal(k), side,
+                           h.first ? 1.0f / (m.unit * m.unit) : 1.0f, h.b, h.c, i != j, {}};
     tile.finish(i * Tile::kTile, j * Tile::kTile, out);
 }
 
@@ -424,17 +439,43 @@ struct ResultOut : ApplyIn {
     }
 };
 
-// p <- p * keep - lr * x at master precision.
+// Eight weights of a row, the first `valid` of them there:  p <- p * keep - lr * x  at master precision.
+template <int DT, int ECCB> struct Weights {
+    static constexpr int PB = DTypeInfo<DT>::bytes, EPL = DTypeInfo<DT>::epl, kParts = 8 / EPL;
+    Pack<PB, EPL> p[kParts];
+    Pack<ECCB, EPL> e[kParts];
+    __device__ __forceinline__ void load(const void* param, const void* ecc, int64_t at, int valid) {
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            load_piece<PB, EPL>(p[k], (const char*)param + (at + k * EPL) * PB, valid - k * EPL);
+            load_piece<ECCB, EPL>(e[k], (const char*)ecc + (at + k * EPL) * ECCB, valid - k * EPL);
+        }
+    }
+    __device__ __forceinline__ void move(const float (&x)[8], float keep, float lr, void* param, void* ecc, int64_t at, int valid) const {
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            Pack<PB, EPL> narrow;
+            Pack<ECCB, EPL> rest;
+            float w[EPL];
+#pragma unroll
+            for (int q = 0; q < EPL; ++q) {
+                float master = widen<DT, EPL>(p[k], q);
+                if constexpr (ECCB > 0) master = ecc_join<DT, ECCB>(master, ecc_to_float<ECCB, EPL>(e[k], q));
+                w[q] = master * keep - x[k * EPL + q] * lr;
+            }
+            write_master<DT, ECCB, EPL>(w, narrow, rest);
+            store_piece<PB, EPL>(narrow, (char*)param + (at + k * EPL) * PB, valid - k * EPL);
+            store_piece<ECCB, EPL>(rest, (char*)ecc + (at + k * EPL) * ECCB, valid - k * EPL);
+        }
+    }
+};
+
 template <int DT, int ECCB> struct UpdateOut : ApplyIn {
     static constexpr bool kColumns = false;
-    static constexpr int PB = DTypeInfo<DT>::bytes, EPL = DTypeInfo<DT>::epl, kParts = 8 / EPL;
     void *param, *ecc;
     int true_rows, true_cols;
     float keep, lr;
-    struct In : ApplyIn::In {
-        Pack<PB, EPL> p[kParts];
-        Pack<ECCB, EPL> e[kParts];
-    };
+    struct In : ApplyIn::In { Weights<DT, ECCB> w; };
     __device__ __forceinline__ UpdateOut(const ApplyIn& in, const LastArgs& last, const MatrixGroup& m, int k)
         : ApplyIn(in), true_rows(m.rows), true_cols(m.cols), keep(last.keep), lr(m.lr) {
         const fo_tensor_desc& d = last.matrices[m.first + k];
@@ -444,32 +485,12 @@ template <int DT, int ECCB> struct UpdateOut : ApplyIn {
     __device__ __forceinline__ void load(int i, int j, In& in) const {
         if (i >= true_rows || j >= true_cols) return;
         ApplyIn::load(i, j, in);
-        const int64_t at = (int64_t)i * true_cols + j;
-#pragma unroll
-        for (int k = 0; k < kParts; ++k) {
-            load_piece<PB, EPL>(in.p[k], (char*)param + (at + k * EPL) * PB, true_cols - j - k * EPL);
-            load_piece<ECCB, EPL>(in.e[k], (char*)ecc + (at + k * EPL) * ECCB, true_cols - j - k * EPL);
-        }
+        in.w.load(param, ecc, (int64_t)i * true_cols + j, true_cols - j);
     }
     __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
         if (i >= true_rows || j >= true_cols) return;
         x(in, v);
-        const int64_t at = (int64_t)i * true_cols + j;
-#pragma unroll
-        for (int k = 0; k < kParts; ++k) {
-            Pack<PB, EPL> p;
-            Pack<ECCB, EPL> e;
-            float w[EPL];
-#pragma unroll
-            for (int q = 0; q < EPL; ++q) {
-                float master = widen<DT, EPL>(in.p[k], q);
-                if constexpr (ECCB > 0) master = ecc_join<DT, ECCB>(master, ecc_to_float<ECCB, EPL>(in.e[k], q));
-                w[q] = master * keep - v[k * EPL + q] * lr;
-            }
-            write_master<DT, ECCB, EPL>(w, p, e);
-            store_piece<PB, EPL>(p, (char*)param + (at + k * EPL) * PB, true_cols - j - k * EPL);
-            store_piece<ECCB, EPL>(e, (char*)ecc + (at + k * EPL) * ECCB, true_cols - j - k * EPL);
-        }
+        in.w.move(v, keep, lr, param, ecc, (int64_t)i * true_cols + j, true_cols - j);
     }
 };
 
@@ -503,6 +524,314 @@ template <int WT, class Out> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2)
     }
 }
 
+// ------------------------------------------------------------------------------------------------
+// matrices that one workgroup holds
+// ------------------------------------------------------------------------------------------------
+// The whole iteration in one launch, a workgroup of 16 wavefronts per matrix: the fp32 X stays in registers in the layout the
+// matrix instructions leave it in; LDS holds X's columns (T), S and B.  S is made of T through transposing LDS reads.  What bounds
+// it is the chain of four phases per step with a barrier between them; 64 matrices of 128 x 256 take hardly longer than one.
+constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
+constexpr int kSmallUnits = 4;                  // pieces of 32 x 16 of X per wavefront, side by side
+constexpr int kSmallLds = 163840;
+constexpr int kSmallPieces = 4;                 // 8-value pieces of G's rows per thread
+
+// X is side x length, padded to multiples of 32.
+struct SmallShape {
+    int side, length;
+    __host__ __device__ explicit SmallShape(const MatrixGroup& m) {
+        side = ((m.tall() ? m.cols : m.rows) + 31) / 32 * 32;
+        length = ((m.tall() ? m.rows : m.cols) + 31) / 32 * 32;
+    }
+    __host__ __device__ int pitch() const { return side * 2 + 16; }   // bytes; 16 rows' 16-byte pieces lie in different banks
+    __host__ __device__ int gram() const { return length * pitch(); }   // where S begins; then B, then their diagonals
+    __host__ __device__ int lds() const { return gram() + 2 * side * pitch() + 8 * side; }
+    __host__ __device__ int waves_across() const { return (length + 16 * kSmallUnits - 1) / (16 * kSmallUnits); }
+    // one 32 x 32 block of S per wavefront
+    __host__ __device__ bool fits() const {
+        const int blocks = side / 32;
+        // (G itself, in fp32, takes 135168 bytes at most and four pieces per thread)
+        return lds() <= kSmallLds && blocks * waves_across() <= kSmallWaves && blocks * (blocks + 1) / 2 <= kSmallWaves;
+    }
+};
+
+// A lane's places in a matrix in LDS: byte offsets that depend on the lane, to which the place of a block is added, the same
+// for all lanes.
+struct SmallPlaces {
+    int pitch;
+    int read_from;      // row `lane & 15`, columns (lane >> 4) * 8 on: an operand
+    int turn_from;      // an operand of the transpose: in each 16 lanes, the columns of four rows, see read_turned
+    int put_from[4];    // rows (lane >> 4) * 4 + e, column `lane & 15`: a result
+    int put4_from;      // row `lane & 15`, columns (lane >> 4) * 4 on: a result transposed
+    __device__ __forceinline__ SmallPlaces(int pitch, int lane) : pitch(pitch) {
+        const int line = lane & 15, quad = (lane >> 4) * 4;
+        read_from = line * pitch + quad * 4;
+        turn_from = (quad * 2 + (line >> 2)) * pitch + (line & 3) * 8;
+        put4_from = line * pitch + quad * 2;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) put_from[e] = (quad + e) * pitch + line * 2;
+    }
+    __device__ __forceinline__ int block(int row, int col) const { return row * pitch + col * 2; }
+};
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f16x8 read_piece(const char* lds, int at) { return *reinterpret_cast<const f16x8*>(lds + at); }
+// Rows of the transpose: lane i of each 16 gives the address of four values and gets value i of what lanes 0..3, 4..7, 8..11 and
+// 12..15 point at (16 values each).  Two such reads make an operand's eight values along k.
+__device__ __forceinline__ f16x8 read_turned(char* lds, int at, int pitch) {
+    typedef __attribute__((address_space(3))) s16x4* place;
+    const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(lds + at)));
+    const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(lds + at + 4 * pitch)));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ void put_half(char* lds, int at, _Float16 v) { *reinterpret_cast<_Float16*>(lds + at) = v; }
+__device__ __forceinline__ void put_halves(char* lds, int at, f16x4 v) { *reinterpret_cast<f16x4*>(lds + at) = v; }
+__device__ __forceinline__ f16x4 halves(f32x4 v) { return f16x4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w}; }
+
+// What becomes of eight values of the result; what that needs from memory is loaded before the result is there.
+struct SmallResult {
+    uint16_t* result;
+    struct In {};
+    __device__ __forceinline__ SmallResult(const LastArgs& last, const MatrixGroup& m, int k) : result(last.result + (int64_t)(m.first + k) * m.rows * m.cols) {}
+    __device__ __forceinline__ void load(int64_t, int, In&) const {}
+    __device__ __forceinline__ void take(int64_t at, int valid, const float (&x)[8], const In&) const { store_values<DT_BF16>(x, result + at, valid); }
+};
+template <int DT, int ECCB> struct SmallUpdate {
+    void *param, *ecc;
+    float keep, lr;
+    typedef Weights<DT, ECCB> In;
+    __device__ __forceinline__ SmallUpdate(const LastArgs& last, const MatrixGroup& m, int k)
+        : param(last.matrices[m.first + k].param), ecc(last.matrices[m.first + k].ecc), keep(last.keep), lr(m.lr) {}
+    __device__ __forceinline__ void load(int64_t at, int valid, In& in) const { in.load(param, ecc, at, valid); }
+    __device__ __forceinline__ void take(int64_t at, int valid, const float (&x)[8], const In& in) const { in.move(x, keep, lr, param, ecc, at, valid); }
+};
+
+// 32 x 32 block (bi, bj) of rows times rows over `length` values; TURNED: the rows are columns of what LDS holds.
+template <bool TURNED> __device__ __forceinline__ void small_block(char* rows, const SmallPlaces& p, int bi, int bj, int length, f32x4 (&acc)[2][2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    int a_from = TURNED ? p.turn_from + bi * 64 : p.read_from + p.block(bi * 32, 0);
+    int b_from = TURNED ? p.turn_from + bj * 64 : p.read_from + p.block(bj * 32, 0);
+    const int next_rows = TURNED ? 32 : p.block(16, 0), next_values = TURNED ? p.block(32, 0) : 64;
+    for (int at = 0; at < length; at += 32) {
+        f16x8 a[2], b[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            a[i] = TURNED ? read_turned(rows, a_from + i * next_rows, p.pitch) : read_piece(rows, a_from + i * next_rows);
+            b[i] = TURNED ? read_turned(rows, b_from + i * next_rows, p.pitch) : read_piece(rows, b_from + i * next_rows);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], b[j], acc[i][j], 0, 0, 0);
+        a_from += next_values;
+        b_from += next_values;
+    }
+}
+// Puts block (bi, bj) of a symmetric matrix and its mirror image.
+__device__ __forceinline__ void put_block(char* to, const SmallPlaces& p, int bi, int bj, const f16x4 (&v)[2][2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int row = bi * 32 + i * 16, col = bj * 32 + j * 16;
+            put_halves(to, p.put4_from + p.block(col, row), v[i][j]);
+            if (bi != bj) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) put_half(to, p.put_from[e] + p.block(row, col), v[i][j][e]);
+            }
+        }
+}
+
+struct SmallArgs {
+    float a, b, c, eps;
+    int steps;
+};
+
+template <int DT, class Out> __global__ __launch_bounds__(kSmallThreads) void small_kernel(Groups groups, MatrixSource source, SmallArgs h, LastArgs last) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int g = group_of(groups, blockIdx.x);
+    const MatrixGroup& m = groups.group[g];
+    const int k = (int)(blockIdx.x - groups.begin[g]);
+    const SmallShape shape(m);
+    const int side = shape.side, length = shape.length;
+    char *const t = lds, *const gram_rows = lds + shape.gram(), *const poly_rows = gram_rows + side * shape.pitch();
+    float *const s_diagonal = reinterpret_cast<float*>(poly_rows + side * shape.pitch()), *const diagonal = s_diagonal + side;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int line = lane & 15, quad = (lane >> 4) * 4;
+
+    // The wavefront's pieces of X.  Where there are fewer than places for them, places share a piece: they work out and
+    // write the same values, and nothing below asks.
+    const int across = shape.waves_across(), whole_waves = side / 32 * across, mine = wave < whole_waves ? wave : whole_waves - 1;
+    const int row_of = mine / across * 32;
+    int col_of[kSmallUnits];
+#pragma unroll
+    for (int u = 0; u < kSmallUnits; ++u) {
+        const int col = mine % across * 16 * kSmallUnits + u * 16;
+        col_of[u] = col < length ? col : length - 16;
+    }
+    const bool tall = m.tall();
+    const char* in = source.data ? (const char*)source.data + source.stride * k * DTypeInfo<DT>::bytes : (const char*)m.update(k);
+    const int64_t row_stride = source.data ? source.row_stride : m.cols;
+    // G passes through LDS in fp32, row by row in 8-value pieces here, as the instructions lay X out there
+    float* const whole = reinterpret_cast<float*>(lds);
+    const int pitch = m.cols | 1, row_step = tall ? 1 : pitch, col_step = tall ? pitch : 1;
+    const int pieces = (m.cols + 7) / 8, all = pieces * m.rows;
+    float sum = 0.0f;
+    {
+        float v[kSmallPieces][8];
+#pragma unroll
+        for (int i = 0; i < kSmallPieces; ++i) {
+            const int at = threadIdx.x + i * kSmallThreads, row = at / pieces, col = (at - row * pieces) * 8;
+            if (at < all) read8<DT>(in + (row_stride * row + col) * DTypeInfo<DT>::bytes, m.cols - col, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kSmallPieces; ++i) {
+            const int at = threadIdx.x + i * kSmallThreads, row = at / pieces, col = (at - row * pieces) * 8;
+            if (at < all) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (col + e < m.cols) whole[row * pitch + col + e] = v[i][e];
+                    sum = fmaf(v[i][e], v[i][e], sum);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int true_side = tall ? m.cols : m.rows, true_length = tall ? m.rows : m.cols;
+    f32x4 x[kSmallUnits][2];
+#pragma unroll
+    for (int u = 0; u < kSmallUnits; ++u) {
+        const int row = row_of + quad, col = col_of[u] + line;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool there = row + half * 16 + e < true_side && col < true_length;
+                const float v = whole[there ? (row + half * 16 + e) * row_step + col * col_step : 0];
+                x[u][half][e] = there ? v : 0.0f;
+            }
+    }
+    __syncthreads();
+    double* sums = reinterpret_cast<double*>(lds);
+    double total = sum;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) total += __shfl_down(total, d);
+    if (lane == 0) sums[wave] = total;
+    __syncthreads();
+    total = 0.0;
+#pragma unroll
+    for (int w = 0; w < kSmallWaves; ++w) total += sums[w];
+    const float factor = (float)(1.0 / (sqrt(total) + (double)h.eps));
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kSmallUnits; ++u) { x[u][0] *= factor; x[u][1] *= factor; }
+
+    // the wavefront's block of S and B, on or above the diagonal, column by column
+    int bi = wave, bj = 0;
+    while (bi > bj) { ++bj; bi -= bj; }
+    const bool has_block = bj < side / 32;
+    const SmallPlaces at(shape.pitch(), lane);
+    for (int step = 0; step < h.steps; ++step) {
+#pragma unroll
+        for (int u = 0; u < kSmallUnits; ++u)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) put_halves(t, at.put4_from + at.block(col_of[u], row_of + half * 16), halves(x[u][half]));
+        __syncthreads();
+        f32x4 gram[2][2];
+        if (has_block) {
+            f16x4 v[2][2];
+            small_block<true>(t, at, bi, bj, length, gram);
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (bi == bj && p == q && quad + e == line) { s_diagonal[bi * 32 + p * 16 + line] = gram[p][q][e]; gram[p][q][e] = 0.0f; }
+                    v[p][q] = halves(gram[p][q]);
+                    // B is made of S as the products see it: its two terms nearly cancel near the end of the iteration
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) gram[p][q][e] = (float)v[p][q][e];
+                }
+            put_block(gram_rows, at, bi, bj, v);
+        }
+        __syncthreads();
+        if (has_block) {
+            f32x4 squared[2][2];
+            f16x4 w[2][2];
+            small_block<false>(gram_rows, at, bi, bj, side, squared);
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const f32x4 di = *reinterpret_cast<const f32x4*>(s_diagonal + bi * 32 + p * 16 + quad);
+                    const float dj = s_diagonal[bj * 32 + q * 16 + line];
+                    f32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[e] = fmaf(h.c, fmaf(di[e] + dj, gram[p][q][e], squared[p][q][e]), h.b * gram[p][q][e]);
+                        if (bi == bj && p == q && quad + e == line) { diagonal[bi * 32 + p * 16 + line] = fmaf(dj, fmaf(h.c, dj, h.b), v[e]); v[e] = 0.0f; }
+                    }
+                    w[p][q] = halves(v);
+                }
+            put_block(poly_rows, at, bi, bj, w);
+        }
+        __syncthreads();
+        f32x4 acc[kSmallUnits][2];
+#pragma unroll
+        for (int u = 0; u < kSmallUnits; ++u) acc[u][0] = acc[u][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int from = 0; from < side; from += 32) {
+            const f16x8 poly0 = read_piece(poly_rows, at.read_from + at.block(row_of, from)), poly1 = read_piece(poly_rows, at.read_from + at.block(row_of + 16, from));
+#pragma unroll
+            for (int u = 0; u < kSmallUnits; ++u) {
+                const f16x8 column = read_piece(t, at.read_from + at.block(col_of[u], from));
+                acc[u][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(poly0, column, acc[u][0], 0, 0, 0);
+                acc[u][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(poly1, column, acc[u][1], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const f32x4 d = *reinterpret_cast<const f32x4*>(diagonal + row_of + quad + half * 16);
+#pragma unroll
+            for (int u = 0; u < kSmallUnits; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[u][half][e] = fmaf(h.a + d[e], x[u][half][e], acc[u][half][e]);
+        }
+        __syncthreads();
+    }
+    // places worked out again, not kept from the beginning
+    int thread = threadIdx.x, last_line = line, last_quad = quad;
+    asm volatile("" : "+v"(thread), "+v"(last_line), "+v"(last_quad));
+    const Out out(last, m, k);
+    typename Out::In with[kSmallPieces];
+#pragma unroll
+    for (int i = 0; i < kSmallPieces; ++i) {
+        const int at = thread + i * kSmallThreads, row = at / pieces, col = (at - row * pieces) * 8;
+        if (at < all) out.load((int64_t)row * m.cols + col, m.cols - col, with[i]);
+    }
+#pragma unroll
+    for (int u = 0; u < kSmallUnits; ++u) {
+        const int row = row_of + last_quad, col = col_of[u] + last_line;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (row + half * 16 + e < true_side && col < true_length) whole[(row + half * 16 + e) * row_step + col * col_step] = x[u][half][e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSmallPieces; ++i) {
+        const int at = thread + i * kSmallThreads, row = at / pieces, col = (at - row * pieces) * 8;
+        if (at >= all) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = whole[row * pitch + (col + e < m.cols ? col + e : 0)];
+        out.take((int64_t)row * m.cols + col, m.cols - col, v, with[i]);
+    }
+}
+
 }  // namespace fo
 
 // ------------------------------------------------------------------------------------------------
@@ -511,7 +840,7 @@ template <int WT, class Out> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2)
 namespace {
 using namespace fo_host;
 
-constexpr int64_t kMostWorkgroups = 1 << 23;   // of 256 threads: below 2^32 work-items
+constexpr int64_t kMostWorkgroups = 1 << 21;   // of up to 1024 threads: below 2^32 work-items
 
 int64_t padded(int64_t n) { return (n + fo::kPad - 1) / fo::kPad * fo::kPad; }
 
@@ -567,12 +896,12 @@ template <class F> int64_t spread(fo::Groups& a, F each) {
 
 int64_t tiles_across(int n, int tile) { return (n + tile - 1) / tile; }
 
-template <class K, class... Args> int launch(K kernel, int64_t grid, int lds, hipStream_t stream, const char* what, Args... args) {
+template <class K, class... Args> int launch(K kernel, int64_t grid, int threads, int lds, hipStream_t stream, const char* what, Args... args) {
     if (grid > kMostWorkgroups) return fail(FO_ERR_UNSUPPORTED, "%s: %lld workgroups are more than one launch takes", what, (long long)grid);
     if (lds > 65536) {
         if (int rc = check_hip(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds), what)) return rc;
     }
-    kernel<<<dim3((unsigned)grid), dim3(256), lds, stream>>>(args...);
+    kernel<<<dim3((unsigned)grid), dim3(threads), lds, stream>>>(args...);
     return check_hip(hipGetLastError(), what);
 }
 
@@ -611,7 +940,7 @@ template <class F> int64_t seat(fo::Groups& a, F tiles) {
 
 template <int WT, bool GRAM> int launch_symmetric(fo::Groups& a, const fo::StepArgs& h, hipStream_t stream) {
     const int64_t grid = seat(a, [](const fo::MatrixGroup& m) { return symmetric_tiles(m, WT); });
-    return launch(fo::symmetric_kernel<WT, GRAM>, grid, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz product", a, h);
+    return launch(fo::symmetric_kernel<WT, GRAM>, grid, 256, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz product", a, h);
 }
 template <bool GRAM> int launch_symmetric(fo::Groups& a, const fo::StepArgs& h, int cus, hipStream_t stream) {
     switch (choose(a, cus, symmetric_tiles, [](const fo::MatrixGroup& m) { return !GRAM ? m.side() : m.tall() ? m.padded_rows : m.padded_cols; })) {
@@ -623,7 +952,7 @@ template <bool GRAM> int launch_symmetric(fo::Groups& a, const fo::StepArgs& h, 
 }
 template <int WT, class Out> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, hipStream_t stream) {
     const int64_t grid = seat(a, [](const fo::MatrixGroup& m) { return apply_tiles(m, WT); });
-    return launch(fo::apply_kernel<WT, Out>, grid, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz step", a, h, last);
+    return launch(fo::apply_kernel<WT, Out>, grid, 256, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz step", a, h, last);
 }
 template <class Out> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, int cus, hipStream_t stream) {
     switch (choose(a, cus, apply_tiles, [](const fo::MatrixGroup& m) { return m.side(); })) {
@@ -653,14 +982,40 @@ int validate_iteration(int steps, const float* coefficients, float eps) {
 }
 
 // From the sums of squares on.
+// The shapes that one workgroup holds leave `a` and are done in a launch of their own.
+template <int DT, class Out> int launch_small(const fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, const fo::LastArgs& last, hipStream_t stream) {
+    return launch(fo::small_kernel<DT, Out>, a.begin[a.n], fo::kSmallThreads, fo::kSmallLds, stream, "Newton-Schulz of small matrices", a, source,
+                  fo::SmallArgs{it.a, it.b, it.c, it.eps, it.steps}, last);
+}
+fo::Groups take_small(fo::Groups& a) {
+    fo::Groups small{}, large{};
+    for (int g = 0; g < a.n; ++g) {
+        fo::Groups& to = fo::SmallShape(a.group[g]).fits() ? small : large;
+        to.group[to.n++] = a.group[g];
+    }
+    a = large;
+    spread(small, [](const fo::MatrixGroup&) { return (int64_t)1; });
+    return small;
+}
+int launch_small_update(const fo::Groups& a, const Iteration& it, const fo::LastArgs& last, int dtype, int ecc_bytes, hipStream_t stream) {
+    const fo::MatrixSource s{nullptr, 0, 0};
+    if (dtype == FO_F32) return launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_F32, 0>>(a, s, it, last, stream);
+    if (dtype == FO_BF16) return ecc_bytes == 0 ? launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_BF16, 0>>(a, s, it, last, stream)
+                               : ecc_bytes == 1 ? launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_BF16, 1>>(a, s, it, last, stream)
+                                                : launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_BF16, 2>>(a, s, it, last, stream);
+    return ecc_bytes == 0 ? launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_F16, 0>>(a, s, it, last, stream)
+         : ecc_bytes == 1 ? launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_F16, 1>>(a, s, it, last, stream)
+                          : launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_F16, 2>>(a, s, it, last, stream);
+}
+
 // finish(h) launches the last step.
 template <int DT, class F> int iterate(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, hipStream_t stream, F finish) {
     const int cus = compute_units();
     if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
     int64_t grid = spread(a, [](const fo::MatrixGroup&) { return (int64_t)1; });
-    if (int rc = launch(fo::norm_kernel, grid, 0, stream, "norm", a, it.eps)) return rc;
+    if (int rc = launch(fo::norm_kernel, grid, 256, 0, stream, "norm", a, it.eps)) return rc;
     grid = spread(a, [](const fo::MatrixGroup& m) { return m.area() / 4096; });
-    if (int rc = launch(fo::split_kernel<DT>, grid, 0, stream, "normalisation", a, source)) return rc;
+    if (int rc = launch(fo::split_kernel<DT>, grid, 256, 0, stream, "normalisation", a, source)) return rc;
     for (int k = 0; k < it.steps; ++k) {
         const fo::StepArgs h{it.a, it.b, it.c, k & 1, k == 0};
         if (int rc = launch_symmetric<true>(a, h, cus, stream)) return rc;
@@ -671,15 +1026,17 @@ template <int DT, class F> int iterate(fo::Groups& a, const fo::MatrixSource& so
 }
 
 template <int DT> int orthogonalise(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, const fo::LastArgs& last, hipStream_t stream) {
+    const fo::Groups small = take_small(a);
+    if (small.n > 0) return launch_small<DT, fo::SmallResult>(small, source, it, last, stream);
     const int64_t grid = spread(a, [](const fo::MatrixGroup& m) { return (int64_t)m.chunks; });
-    if (int rc = launch(fo::squares_kernel<DT>, grid, 0, stream, "sum of squares", a, source)) return rc;
+    if (int rc = launch(fo::squares_kernel<DT>, grid, 256, 0, stream, "sum of squares", a, source)) return rc;
     return iterate<DT>(a, source, it, stream, [&](const fo::StepArgs& h, int cus) { return launch_apply<fo::ResultOut>(a, h, last, cus, stream); });
 }
 
 template <int DT> int momentum(fo::Groups& a, const fo::MomentumArgs& h, int quantized, hipStream_t stream) {
     const int64_t grid = spread(a, [](const fo::MatrixGroup& m) { return (int64_t)m.chunks; });
-    return quantized ? launch(fo::momentum_kernel<DT, true>, grid, 0, stream, "momentum", a, h)
-                     : launch(fo::momentum_kernel<DT, false>, grid, 0, stream, "momentum", a, h);
+    return quantized ? launch(fo::momentum_kernel<DT, true>, grid, 256, 0, stream, "momentum", a, h)
+                     : launch(fo::momentum_kernel<DT, false>, grid, 256, 0, stream, "momentum", a, h);
 }
 
 }  // namespace
@@ -745,6 +1102,14 @@ int fo_muon_step(const fo_tensor_desc* matrices, const fo_matrix_shape* shapes, 
             hipStream_t s = (hipStream_t)stream;
             if (int rc = dtype == FO_F32 ? momentum<fo::DT_F32>(a, h, quantized, s) : dtype == FO_BF16 ? momentum<fo::DT_BF16>(a, h, quantized, s)
                                                                                                 : momentum<fo::DT_F16>(a, h, quantized, s)) return rc;
+            const fo::Groups small = take_small(a);
+            if (small.n > 0) {
+                if (int rc = launch_small_update(small, it, last, dtype, ecc_bytes, s)) return rc;
+            }
+            if (a.n == 0) {
+                for (int64_t k = 0; k < n; ++k) matrices += shapes[i + k].count;
+                continue;
+            }
             if (int rc = iterate<fo::DT_F32>(a, fo::MatrixSource{nullptr, 0, 0}, it, s, [&](const fo::StepArgs& step, int cus) {
                     return launch_update(a, step, last, dtype, ecc_bytes, cus, s);
                 })) return rc;
