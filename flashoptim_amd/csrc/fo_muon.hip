@@ -17,6 +17,11 @@
 //     S = rows of X by rows of X          (X = hi where rows <= cols, else T); the tiles on and above the diagonal, written twice
 //     B = rows of S by rows of S          (S is symmetric); likewise
 //     X = rows of B by rows of T          (rows <= cols), or rows of hi by rows of B: main orientation either way
+// The first two steps of a matrix that is longer than wide are merged: with P = a + B its second S is P S P, so both B's come of
+// side x side products and X is read and written once for  X <- P2 P1 X.  That costs three such products more and saves an S
+// and a step, 2 longer / shorter times as much arithmetic each; and it costs no accuracy, unlike merging later steps (there an
+// error of S is no longer small against the small singular values: 2 to 3 times the error, measured on flat, low-rank, peaked
+// and decaying spectra).
 // so the result comes out in G's orientation and the last product's epilogue writes it, or updates the weights with it.
 //
 // One launch covers matrices of many shapes: the shapes travel as kernel arguments, matrices of one shape lie one after the
@@ -38,6 +43,7 @@ constexpr int kChunk = 8192;      // elements of a matrix whose squares one work
 struct MatrixGroup {
     int rows, cols, padded_rows, padded_cols, count;
     int first;            // matrix number of the first of them
+    int generation;       // of hi and T that X is in
     int chunks;           // sums of squares of each
     float unit;           // the power of two that the first X is kept times
     float lr;             // optimizer step: learning rate with the shape's factor
@@ -47,21 +53,19 @@ struct MatrixGroup {
     __host__ __device__ int side() const { return tall() ? padded_cols : padded_rows; }
     __host__ __device__ int64_t area() const { return (int64_t)padded_rows * padded_cols; }
     __host__ __device__ int64_t gram_area() const { return (int64_t)side() * side(); }
-    // per matrix: two generations of hi and of T, lo, S, B, their diagonals, the factor that normalises, sums of squares.
+    // per matrix: two generations of hi and of T, lo, three square matrices, their diagonals, the factor that normalises, sums of squares.
     // The update before its normalisation (fp32) lies over the second generation, which is written later.
     __host__ __device__ int64_t bytes_each() const {
-        return area() * 10 + gram_area() * 4 + side() * 8 + 256 + ((int64_t)chunks * 8 + 255) / 256 * 256;
+        return area() * 10 + gram_area() * 6 + side() * 12 + 256 + ((int64_t)chunks * 8 + 255) / 256 * 256;
     }
     __device__ char* of(int k) const { return workspace + bytes_each() * k; }
     __device__ _Float16* hi(int k, int generation) const { return (_Float16*)(of(k) + generation * area() * 4); }
     __device__ _Float16* t(int k, int generation) const { return (_Float16*)(of(k) + generation * area() * 4 + area() * 2); }
     __device__ float* update(int k) const { return (float*)(of(k) + area() * 4); }
     __device__ u32* lo(int k) const { return (u32*)(of(k) + area() * 8); }   // pairs of bf16
-    __device__ _Float16* s(int k) const { return (_Float16*)(of(k) + area() * 10); }
-    __device__ _Float16* b(int k) const { return (_Float16*)(of(k) + area() * 10 + gram_area() * 2); }
-    __device__ float* s_diagonal(int k) const { return (float*)(of(k) + area() * 10 + gram_area() * 4); }
-    __device__ float* diagonal(int k) const { return s_diagonal(k) + side(); }   // of B
-    __device__ float* factor(int k) const { return diagonal(k) + side(); }
+    __device__ _Float16* square(int k, int which) const { return (_Float16*)(of(k) + area() * 10 + gram_area() * 2 * which); }
+    __device__ float* diagonal(int k, int which) const { return (float*)(of(k) + area() * 10 + gram_area() * 6) + side() * which; }
+    __device__ float* factor(int k) const { return diagonal(k, 3); }
     __device__ double* squares(int k) const { return (double*)((char*)factor(k) + 256); }
 };
 
@@ -277,10 +281,18 @@ template <int DT, bool QUANT> __global__ __launch_bounds__(256) void momentum_ke
 // the products
 // ------------------------------------------------------------------------------------------------
 
+// One of a matrix's three square matrices from two others: out = gamma U V + alpha U + beta V; or S (GRAM), of which `first` says that X
+// still carries the unit.
+enum { kSlots = 3 };
+struct SquareArgs {
+    int u, v, out;
+    float alpha, beta, gamma;
+    int first;
+};
+// X <- a X + (square matrix `poly`) X.
 struct StepArgs {
-    float a, b, c;
-    int generation;    // of hi and T that the step starts from
-    int first;         // the parts still carry the unit
+    float a;
+    int poly, first;
 };
 
 __device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
@@ -290,56 +302,62 @@ __device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
     return h;
 }
 
-// S and B without their diagonals: rows of a symmetric matrix, each tile off the diagonal twice.
+// Square matrices without their diagonals: all are symmetric, so each tile off the diagonal is written twice.
 template <bool GRAM> struct SymmetricOut {
     static constexpr bool kColumns = true;
-    const _Float16* s;            // what B is made of,
-    const float* s_diagonal;      // with its diagonal
+    const _Float16 *u, *v;
+    const float *u_diagonal, *v_diagonal;
     _Float16* out;
     float* diagonal;
     int side;
-    float scale, b, c;
+    float scale, alpha, beta, gamma;
     bool mirror;
-    float d[8];                   // of the lane's columns
+    float d[8];                   // V's diagonal at the lane's columns
 
-    struct In { f16x8 s; float d; };
+    struct In { f16x8 u, v; float d; };
     __device__ __forceinline__ void begin(int j) {
         if constexpr (!GRAM) {
             if (j < side) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) d[e] = s_diagonal[j + e];
+                for (int e = 0; e < 8; ++e) d[e] = v_diagonal[j + e];
             }
         }
     }
     __device__ __forceinline__ void load(int i, int j, In& in) const {
         if constexpr (!GRAM) {
             if (i < side && j < side) {
-                in.s = *reinterpret_cast<const f16x8*>(s + (int64_t)i * side + j);
-                in.d = s_diagonal[i];
+                in.u = *reinterpret_cast<const f16x8*>(u + (int64_t)i * side + j);
+                in.v = u == v ? in.u : *reinterpret_cast<const f16x8*>(v + (int64_t)i * side + j);
+                in.d = u_diagonal[i];
             }
         }
     }
-    __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
+    __device__ __forceinline__ void row(int i, int j, const In& in, float (&x)[8]) const {
         if (i >= side || j >= side) return;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if constexpr (GRAM) v[e] *= scale;
-            else v[e] = fmaf(c, fmaf(in.d + d[e], (float)in.s[e], v[e]), b * (float)in.s[e]);
-            if (i == j + e) {   // B: v is c O O here, S's entry is not in it
-                diagonal[i] = GRAM ? v[e] : fmaf(in.d, fmaf(c, in.d, b), v[e]);
-                v[e] = 0.0f;
+            if constexpr (GRAM) {
+                x[e] *= scale;
+                if (i == j + e) { diagonal[i] = x[e]; x[e] = 0.0f; }
+            } else {
+                const float a = (float)in.u[e], b = (float)in.v[e], product = fmaf(in.d, b, fmaf(a, d[e], x[e]));   // a = b = 0 on the diagonal
+                x[e] = fmaf(gamma, product, fmaf(alpha, a, beta * b));
+                if (i == j + e) {
+                    diagonal[i] = fmaf(gamma, fmaf(in.d, d[e], product), fmaf(alpha, in.d, beta * d[e]));
+                    x[e] = 0.0f;
+                }
             }
         }
-        *reinterpret_cast<f16x8*>(out + (int64_t)i * side + j) = half8(v);
+        *reinterpret_cast<f16x8*>(out + (int64_t)i * side + j) = half8(x);
     }
     __device__ __forceinline__ bool columns() const { return mirror; }
-    __device__ __forceinline__ void column(int i, int j, const float (&v)[8]) const {
+    __device__ __forceinline__ void column(int i, int j, const float (&x)[8]) const {
         if (i >= side || j >= side) return;
-        *reinterpret_cast<f16x8*>(out + (int64_t)j * side + i) = half8(v);
+        *reinterpret_cast<f16x8*>(out + (int64_t)j * side + i) = half8(x);
     }
 };
 
-template <int WT, bool GRAM> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void symmetric_kernel(Groups a, StepArgs h) {
+template <int WT, bool GRAM> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void symmetric_kernel(Groups a, SquareArgs h) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef GemmTile<F16Product, WT> Tile;
     const int64_t seat = blockIdx.x >> 3;
@@ -352,13 +370,14 @@ template <int WT, bool GRAM> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2)
     int i, j;
     tile_at_symmetric((int)(local % tiles), n, i, j);
     const bool tall = m.tall();
-    const _Float16* x = GRAM ? (tall ? m.t(k, h.generation) : m.hi(k, h.generation)) : m.s(k);
+    const _Float16* x = tall ? m.t(k, m.generation) : m.hi(k, m.generation);
     const int64_t length = (GRAM ? (tall ? m.padded_rows : m.padded_cols) : side) * 2;
-    const Operand op{(const char*)x, length, nullptr, 0, side};
+    const Operand left{(const char*)(GRAM ? x : m.square(k, h.u)), length, nullptr, 0, side};
+    const Operand right{(const char*)(GRAM ? x : m.square(k, h.v)), length, nullptr, 0, side};
     Tile tile(lds);
-    tile.multiply(op, op, i * Tile::kTile, j * Tile::kTile, (int)length);
-    SymmetricOut<GRAM> out{m.s(k), m.s_diagonal(k), GRAM ? m.s(k) : m.b(k), GRAM ? m.s_diagonal(k) : m.diagonal(k), side,
-                           h.first ? 1.0f / (m.unit * m.unit) : 1.0f, h.b, h.c, i != j, {}};
+    tile.multiply(left, right, i * Tile::kTile, j * Tile::kTile, (int)length);
+    SymmetricOut<GRAM> out{m.square(k, h.u), m.square(k, h.v), m.diagonal(k, h.u), m.diagonal(k, h.v), m.square(k, h.out), m.diagonal(k, h.out), side,
+                           h.first ? 1.0f / (m.unit * m.unit) : 1.0f, h.alpha, h.beta, h.gamma, i != j, {}};
     tile.finish(i * Tile::kTile, j * Tile::kTile, out);
 }
 
@@ -509,14 +528,14 @@ template <int WT, class Out> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2)
     tile_at((int)(local % (rows * cols)), rows, cols, i, j);
     const bool tall = m.tall();
     const int side = m.side();
-    const Operand poly{(const char*)m.b(k), side * 2, nullptr, 0, side};
-    const Operand main{(const char*)m.hi(k, h.generation), side * 2, nullptr, 0, m.padded_rows};
-    const Operand turned{(const char*)m.t(k, h.generation), side * 2, nullptr, 0, m.padded_cols};
+    const Operand poly{(const char*)m.square(k, h.poly), side * 2, nullptr, 0, side};
+    const Operand main{(const char*)m.hi(k, m.generation), side * 2, nullptr, 0, m.padded_rows};
+    const Operand turned{(const char*)m.t(k, m.generation), side * 2, nullptr, 0, m.padded_cols};
     Tile tile(lds);
     tile.multiply(tall ? main : poly, tall ? poly : turned, i * Tile::kTile, j * Tile::kTile, side * 2);
-    const ApplyIn in{m.hi(k, h.generation), m.lo(k), m.diagonal(k), m.padded_rows, m.padded_cols, h.a, h.first ? 1.0f / m.unit : 1.0f, tall, {}};
+    const ApplyIn in{m.hi(k, m.generation), m.lo(k), m.diagonal(k, h.poly), m.padded_rows, m.padded_cols, h.a, h.first ? 1.0f / m.unit : 1.0f, tall, {}};
     if constexpr (Out::kColumns) {
-        Out out{in, m.hi(k, h.generation ^ 1), m.t(k, h.generation ^ 1)};
+        Out out{in, m.hi(k, m.generation ^ 1), m.t(k, m.generation ^ 1)};
         tile.finish(i * Tile::kTile, j * Tile::kTile, out);
     } else {
         Out out(in, last, m, k);
@@ -938,11 +957,11 @@ template <class F> int64_t seat(fo::Groups& a, F tiles) {
     return a.begin[a.n] * 8;
 }
 
-template <int WT, bool GRAM> int launch_symmetric(fo::Groups& a, const fo::StepArgs& h, hipStream_t stream) {
+template <int WT, bool GRAM> int launch_symmetric(fo::Groups& a, const fo::SquareArgs& h, hipStream_t stream) {
     const int64_t grid = seat(a, [](const fo::MatrixGroup& m) { return symmetric_tiles(m, WT); });
     return launch(fo::symmetric_kernel<WT, GRAM>, grid, 256, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz product", a, h);
 }
-template <bool GRAM> int launch_symmetric(fo::Groups& a, const fo::StepArgs& h, int cus, hipStream_t stream) {
+template <bool GRAM> int launch_symmetric(fo::Groups& a, const fo::SquareArgs& h, int cus, hipStream_t stream) {
     switch (choose(a, cus, symmetric_tiles, [](const fo::MatrixGroup& m) { return !GRAM ? m.side() : m.tall() ? m.padded_rows : m.padded_cols; })) {
         case 128: return launch_symmetric<128, GRAM>(a, h, stream);
         case 96: return launch_symmetric<96, GRAM>(a, h, stream);
@@ -1008,7 +1027,53 @@ int launch_small_update(const fo::Groups& a, const Iteration& it, const fo::Last
                           : launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_F16, 2>>(a, s, it, last, stream);
 }
 
-// finish(h) launches the last step.
+// The products of one or two steps over the matrices of `a`.
+struct Steps {
+    const Iteration& it;
+    int cus;
+    hipStream_t stream;
+
+    int gram(fo::Groups& a, int out, int first) const { return launch_symmetric<true>(a, fo::SquareArgs{0, 0, out, 0.0f, 0.0f, 0.0f, first}, cus, stream); }
+    int square(fo::Groups& a, int u, int v, int out, float alpha, float beta, float gamma) const {
+        return launch_symmetric<false>(a, fo::SquareArgs{u, v, out, alpha, beta, gamma, 0}, cus, stream);
+    }
+    // B of S
+    int poly(fo::Groups& a, int s, int out) const { return square(a, s, s, out, it.b, 0.0f, it.c); }
+
+    // Up to X's own product.
+    int one(fo::Groups& a, int first, fo::StepArgs& then) const {
+        if (int rc = gram(a, 0, first)) return rc;
+        if (int rc = poly(a, 0, 1)) return rc;
+        then = fo::StepArgs{it.a, 1, first};
+        return 0;
+    }
+    // The first two: B1 of S, T = (a + B1) S, S2 = T (a + B1), B2 of it, and (a + B2) (a + B1) = a a + B2 B1 + a B2 + a B1.
+    int two(fo::Groups& a, fo::StepArgs& then) const {
+        if (int rc = gram(a, 0, 1)) return rc;
+        if (int rc = poly(a, 0, 1)) return rc;
+        if (int rc = square(a, 1, 0, 2, 0.0f, it.a, 1.0f)) return rc;
+        if (int rc = square(a, 2, 1, 0, it.a, 0.0f, 1.0f)) return rc;
+        if (int rc = poly(a, 0, 2)) return rc;
+        if (int rc = square(a, 2, 1, 0, it.a, it.a, 1.0f)) return rc;
+        then = fo::StepArgs{it.a * it.a, 0, 1};
+        return 0;
+    }
+    // X's own product; finish(a, then) where it is the last.
+    template <class F> int apply(fo::Groups& a, const fo::StepArgs& then, bool last, F finish) const {
+        if (int rc = last ? finish(a, then, cus) : launch_apply<fo::ApplyOut>(a, then, fo::LastArgs{}, cus, stream)) return rc;
+        for (int g = 0; g < a.n; ++g) a.group[g].generation ^= 1;
+        return 0;
+    }
+};
+
+// Whether the first two steps are merged.  14336 x 4096: 4.2 ms in all become 3.7, 4096 x 1024 and 2730 x 1000 gain too; square
+// matrices gain nothing, and small ones lose by the launch more that it takes (8 of 250 x 1000: 121 us become 127).
+bool merges(const fo::MatrixGroup& m) {
+    const int longer = std::max(m.rows, m.cols), shorter = std::min(m.rows, m.cols);
+    return shorter > 512 && 2 * longer >= 3 * shorter;
+}
+
+// From the sums of squares on.  finish(a, step, cus) launches the last step.
 template <int DT, class F> int iterate(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, hipStream_t stream, F finish) {
     const int cus = compute_units();
     if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
@@ -1016,11 +1081,30 @@ template <int DT, class F> int iterate(fo::Groups& a, const fo::MatrixSource& so
     if (int rc = launch(fo::norm_kernel, grid, 256, 0, stream, "norm", a, it.eps)) return rc;
     grid = spread(a, [](const fo::MatrixGroup& m) { return m.area() / 4096; });
     if (int rc = launch(fo::split_kernel<DT>, grid, 256, 0, stream, "normalisation", a, source)) return rc;
-    for (int k = 0; k < it.steps; ++k) {
-        const fo::StepArgs h{it.a, it.b, it.c, k & 1, k == 0};
-        if (int rc = launch_symmetric<true>(a, h, cus, stream)) return rc;
-        if (int rc = launch_symmetric<false>(a, h, cus, stream)) return rc;
-        if (int rc = k + 1 < it.steps ? launch_apply<fo::ApplyOut>(a, h, fo::LastArgs{}, cus, stream) : finish(h, cus)) return rc;
+    const Steps steps{it, cus, stream};
+    fo::StepArgs then{};
+    int done = 0;
+    if (it.steps >= 2) {
+        fo::Groups merged{}, single{};
+        for (int g = 0; g < a.n; ++g) {
+            fo::Groups& to = merges(a.group[g]) ? merged : single;
+            to.group[to.n++] = a.group[g];
+        }
+        if (merged.n > 0) {
+            const bool last = it.steps == 2;
+            if (int rc = steps.two(merged, then)) return rc;
+            if (int rc = steps.apply(merged, then, last, finish)) return rc;
+            for (int k = 0; k < 2 && single.n > 0; ++k) {
+                if (int rc = steps.one(single, k == 0, then)) return rc;
+                if (int rc = steps.apply(single, then, last && k == 1, finish)) return rc;
+            }
+            for (int g = 0, i = 0, j = 0; g < a.n; ++g) a.group[g] = merges(a.group[g]) ? merged.group[i++] : single.group[j++];
+            done = 2;
+        }
+    }
+    for (int k = done; k < it.steps; ++k) {
+        if (int rc = steps.one(a, k == 0, then)) return rc;
+        if (int rc = steps.apply(a, then, k + 1 == it.steps, finish)) return rc;
     }
     return 0;
 }
@@ -1030,7 +1114,7 @@ template <int DT> int orthogonalise(fo::Groups& a, const fo::MatrixSource& sourc
     if (small.n > 0) return launch_small<DT, fo::SmallResult>(small, source, it, last, stream);
     const int64_t grid = spread(a, [](const fo::MatrixGroup& m) { return (int64_t)m.chunks; });
     if (int rc = launch(fo::squares_kernel<DT>, grid, 256, 0, stream, "sum of squares", a, source)) return rc;
-    return iterate<DT>(a, source, it, stream, [&](const fo::StepArgs& h, int cus) { return launch_apply<fo::ResultOut>(a, h, last, cus, stream); });
+    return iterate<DT>(a, source, it, stream, [&](fo::Groups& some, const fo::StepArgs& h, int cus) { return launch_apply<fo::ResultOut>(some, h, last, cus, stream); });
 }
 
 template <int DT> int momentum(fo::Groups& a, const fo::MomentumArgs& h, int quantized, hipStream_t stream) {
@@ -1110,8 +1194,8 @@ int fo_muon_step(const fo_tensor_desc* matrices, const fo_matrix_shape* shapes, 
                 for (int64_t k = 0; k < n; ++k) matrices += shapes[i + k].count;
                 continue;
             }
-            if (int rc = iterate<fo::DT_F32>(a, fo::MatrixSource{nullptr, 0, 0}, it, s, [&](const fo::StepArgs& step, int cus) {
-                    return launch_update(a, step, last, dtype, ecc_bytes, cus, s);
+            if (int rc = iterate<fo::DT_F32>(a, fo::MatrixSource{nullptr, 0, 0}, it, s, [&](fo::Groups& some, const fo::StepArgs& step, int cus) {
+                    return launch_update(some, step, last, dtype, ecc_bytes, cus, s);
                 })) return rc;
         }
         for (int64_t k = 0; k < n; ++k) matrices += shapes[i + k].count;
