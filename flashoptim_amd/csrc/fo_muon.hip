@@ -8,8 +8,8 @@
 // cost up to 1e-2 of the result: an error among the small singular directions is multiplied like the signal there (3.4 per
 // step).  So X is held in two parts, hi (fp16, the operand of the products) and lo (bf16, the rest, 19 bits or more together); lo
 // enters where X is multiplied by a.  The diagonals of S and B, by far their largest entries on a flat spectrum, are kept apart
-// in fp32; the products see the matrices without them: S S = O O + O D + D O + D D for S = O + D, and B's is added to a.  What is left (S and B off the diagonal in fp16) costs 1e-4 .. 8e-4
-// of the result, below the bfloat16 rounding it is handed out with.  X starts at |X|_F = 1, entries as small as 1e-4, so
+// in fp32; the products see the matrices without them: S S = O O + O D + D O + D D for S = O + D, and B's is added to a.  What is left (S and B off the diagonal and the products' X
+// in fp16) costs 1e-4 .. 1e-3 of the result, below the bfloat16 rounding it is handed out with; the smallest matrices are done in fp32.  X starts at |X|_F = 1, entries as small as 1e-4, so
 // the first X is kept times a power of two near sqrt(n), in fp16's normal range.
 //
 // Layout.  "Main" arrays have G's own orientation, padded with zeros to multiples of 64 (Rp x Cp), so that the products need no
@@ -17,12 +17,13 @@
 //     S = rows of X by rows of X          (X = hi where rows <= cols, else T); the tiles on and above the diagonal, written twice
 //     B = rows of S by rows of S          (S is symmetric); likewise
 //     X = rows of B by rows of T          (rows <= cols), or rows of hi by rows of B: main orientation either way
+// so the result comes out in G's orientation and the last product's epilogue writes it, or updates the weights with it.
+//
 // The first two steps of a matrix that is longer than wide are merged: with P = a + B its second S is P S P, so both B's come of
 // side x side products and X is read and written once for  X <- P2 P1 X.  That costs three such products more and saves an S
 // and a step, 2 longer / shorter times as much arithmetic each; and it costs no accuracy, unlike merging later steps (there an
 // error of S is no longer small against the small singular values: 2 to 3 times the error, measured on flat, low-rank, peaked
 // and decaying spectra).
-// so the result comes out in G's orientation and the last product's epilogue writes it, or updates the weights with it.
 //
 // One launch covers matrices of many shapes: the shapes travel as kernel arguments, matrices of one shape lie one after the
 // other in the workspace.
@@ -851,6 +852,102 @@ template <int DT, class Out> __global__ __launch_bounds__(kSmallThreads) void sm
     }
 }
 
+// ------------------------------------------------------------------------------------------------
+// matrices that one wavefront holds
+// ------------------------------------------------------------------------------------------------
+// Sixteen rows of up to 64 values at most: a lane has a column of X in registers, S and B lie in LDS, and all of it is fp32 on the
+// vector units.  Not for speed: where the sides are this short a matrix is often nearly singular, and then the roundings to
+// fp16 above, which longer sides average out, reach 1e-2 of the result (4000 random matrices of each shape: 4e-2 at 2 x 2, 7e-3 at 8 x 8,
+// 1.8e-3 at 8 x 32; above these sizes 1.3e-3 at most).
+constexpr int kTinySide = 16, kTinyLength = 64, kTinyPieces = 2;   // 8-value pieces of G's rows per lane
+
+template <int DT, class Out> __global__ __launch_bounds__(64) void tiny_kernel(Groups groups, MatrixSource source, SmallArgs h, LastArgs last) {
+    __shared__ float xs[kTinySide][kTinyLength + 1];
+    __shared__ __attribute__((aligned(16))) float s[kTinySide][kTinySide + 4], b[kTinySide][kTinySide + 4];
+    const int g = group_of(groups, blockIdx.x);
+    const MatrixGroup& m = groups.group[g];
+    const int k = (int)(blockIdx.x - groups.begin[g]), lane = threadIdx.x;
+    const bool tall = m.tall();
+    const int length = tall ? m.rows : m.cols, pieces = (m.cols + 7) / 8, all = pieces * m.rows;
+    const char* in = source.data ? (const char*)source.data + source.stride * k * DTypeInfo<DT>::bytes : (const char*)m.update(k);
+    const int64_t row_stride = source.data ? source.row_stride : m.cols;
+    const Out out(last, m, k);
+    typename Out::In with[kTinyPieces];
+    float x[kTinySide];
+#pragma unroll
+    for (int i = 0; i < kTinySide; ++i) xs[i][lane] = 0.0f;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTinyPieces; ++i) {
+        const int at = lane + i * 64, row = at / pieces, col = (at - row * pieces) * 8;
+        if (at >= all) continue;
+        float v[8];
+        read8<DT>(in + (row_stride * row + col) * DTypeInfo<DT>::bytes, m.cols - col, v);
+        out.load((int64_t)row * m.cols + col, m.cols - col, with[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + e < m.cols) xs[tall ? col + e : row][tall ? row : col + e] = v[e];
+    }
+    __syncthreads();
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kTinySide; ++i) {
+        x[i] = xs[i][lane];
+        sum = fmaf(x[i], x[i], sum);
+    }
+    double total = sum;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
+    const float factor = (float)(1.0 / (sqrt(total) + (double)h.eps));
+#pragma unroll
+    for (int i = 0; i < kTinySide; ++i) x[i] *= factor;
+    const int row = lane >> 2, first = (lane & 3) * 4;   // the lane's four entries of S and B
+    for (int step = 0; step < h.steps; ++step) {
+#pragma unroll
+        for (int i = 0; i < kTinySide; ++i) xs[i][lane] = x[i];
+        __syncthreads();
+        float gram[4] = {0.0f, 0.0f, 0.0f, 0.0f}, squared[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < length; ++c) {
+            const float v = xs[row][c];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) gram[e] = fmaf(v, xs[first + e][c], gram[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[row][first + e] = gram[e];
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < kTinySide; ++c) {
+            const float v = s[row][c];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) squared[e] = fmaf(v, s[c][first + e], squared[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[row][first + e] = fmaf(h.c, squared[e], h.b * gram[e]);
+        __syncthreads();
+        float next[kTinySide];
+#pragma unroll
+        for (int i = 0; i < kTinySide; ++i) {
+            next[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kTinySide; ++j) next[i] = fmaf(b[i][j], x[j], next[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kTinySide; ++i) x[i] = fmaf(h.a, x[i], next[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kTinySide; ++i) xs[i][lane] = x[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTinyPieces; ++i) {
+        const int at = lane + i * 64, row = at / pieces, col = (at - row * pieces) * 8;
+        if (at >= all) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = col + e < m.cols ? xs[tall ? col + e : row][tall ? row : col + e] : 0.0f;
+        out.take((int64_t)row * m.cols + col, m.cols - col, v, with[i]);
+    }
+}
+
 }  // namespace fo
 
 // ------------------------------------------------------------------------------------------------
@@ -1000,31 +1097,39 @@ int validate_iteration(int steps, const float* coefficients, float eps) {
     return 0;
 }
 
-// From the sums of squares on.
-// The shapes that one workgroup holds leave `a` and are done in a launch of their own.
-template <int DT, class Out> int launch_small(const fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, const fo::LastArgs& last, hipStream_t stream) {
-    return launch(fo::small_kernel<DT, Out>, a.begin[a.n], fo::kSmallThreads, fo::kSmallLds, stream, "Newton-Schulz of small matrices", a, source,
-                  fo::SmallArgs{it.a, it.b, it.c, it.eps, it.steps}, last);
-}
-fo::Groups take_small(fo::Groups& a) {
-    fo::Groups small{}, large{};
+// The shapes that one wavefront or one workgroup holds leave `a` and are done in a launch of their own.
+bool is_tiny(const fo::MatrixGroup& m) { return std::min(m.rows, m.cols) <= fo::kTinySide && std::max(m.rows, m.cols) <= fo::kTinyLength; }
+bool is_small(const fo::MatrixGroup& m) { return fo::SmallShape(m).fits(); }
+
+fo::Groups take(fo::Groups& a, bool (*which)(const fo::MatrixGroup&)) {
+    fo::Groups taken{}, left{};
     for (int g = 0; g < a.n; ++g) {
-        fo::Groups& to = fo::SmallShape(a.group[g]).fits() ? small : large;
+        fo::Groups& to = which(a.group[g]) ? taken : left;
         to.group[to.n++] = a.group[g];
     }
-    a = large;
-    spread(small, [](const fo::MatrixGroup&) { return (int64_t)1; });
-    return small;
+    a = left;
+    spread(taken, [](const fo::MatrixGroup&) { return (int64_t)1; });
+    return taken;
 }
-int launch_small_update(const fo::Groups& a, const Iteration& it, const fo::LastArgs& last, int dtype, int ecc_bytes, hipStream_t stream) {
+template <int DT, class Out> int launch_held(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, const fo::LastArgs& last, hipStream_t stream) {
+    const fo::SmallArgs h{it.a, it.b, it.c, it.eps, it.steps};
+    const fo::Groups tiny = take(a, is_tiny);
+    if (tiny.n > 0) {
+        if (int rc = launch(fo::tiny_kernel<DT, Out>, tiny.begin[tiny.n], 64, 0, stream, "Newton-Schulz of the smallest matrices", tiny, source, h, last)) return rc;
+    }
+    const fo::Groups small = take(a, is_small);
+    if (small.n == 0) return 0;
+    return launch(fo::small_kernel<DT, Out>, small.begin[small.n], fo::kSmallThreads, fo::kSmallLds, stream, "Newton-Schulz of small matrices", small, source, h, last);
+}
+int launch_held_update(fo::Groups& a, const Iteration& it, const fo::LastArgs& last, int dtype, int ecc_bytes, hipStream_t stream) {
     const fo::MatrixSource s{nullptr, 0, 0};
-    if (dtype == FO_F32) return launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_F32, 0>>(a, s, it, last, stream);
-    if (dtype == FO_BF16) return ecc_bytes == 0 ? launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_BF16, 0>>(a, s, it, last, stream)
-                               : ecc_bytes == 1 ? launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_BF16, 1>>(a, s, it, last, stream)
-                                                : launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_BF16, 2>>(a, s, it, last, stream);
-    return ecc_bytes == 0 ? launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_F16, 0>>(a, s, it, last, stream)
-         : ecc_bytes == 1 ? launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_F16, 1>>(a, s, it, last, stream)
-                          : launch_small<fo::DT_F32, fo::SmallUpdate<fo::DT_F16, 2>>(a, s, it, last, stream);
+    if (dtype == FO_F32) return launch_held<fo::DT_F32, fo::SmallUpdate<fo::DT_F32, 0>>(a, s, it, last, stream);
+    if (dtype == FO_BF16) return ecc_bytes == 0 ? launch_held<fo::DT_F32, fo::SmallUpdate<fo::DT_BF16, 0>>(a, s, it, last, stream)
+                               : ecc_bytes == 1 ? launch_held<fo::DT_F32, fo::SmallUpdate<fo::DT_BF16, 1>>(a, s, it, last, stream)
+                                                : launch_held<fo::DT_F32, fo::SmallUpdate<fo::DT_BF16, 2>>(a, s, it, last, stream);
+    return ecc_bytes == 0 ? launch_held<fo::DT_F32, fo::SmallUpdate<fo::DT_F16, 0>>(a, s, it, last, stream)
+         : ecc_bytes == 1 ? launch_held<fo::DT_F32, fo::SmallUpdate<fo::DT_F16, 1>>(a, s, it, last, stream)
+                          : launch_held<fo::DT_F32, fo::SmallUpdate<fo::DT_F16, 2>>(a, s, it, last, stream);
 }
 
 // The products of one or two steps over the matrices of `a`.
@@ -1110,8 +1215,8 @@ template <int DT, class F> int iterate(fo::Groups& a, const fo::MatrixSource& so
 }
 
 template <int DT> int orthogonalise(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, const fo::LastArgs& last, hipStream_t stream) {
-    const fo::Groups small = take_small(a);
-    if (small.n > 0) return launch_small<DT, fo::SmallResult>(small, source, it, last, stream);
+    if (int rc = launch_held<DT, fo::SmallResult>(a, source, it, last, stream)) return rc;
+    if (a.n == 0) return 0;
     const int64_t grid = spread(a, [](const fo::MatrixGroup& m) { return (int64_t)m.chunks; });
     if (int rc = launch(fo::squares_kernel<DT>, grid, 256, 0, stream, "sum of squares", a, source)) return rc;
     return iterate<DT>(a, source, it, stream, [&](fo::Groups& some, const fo::StepArgs& h, int cus) { return launch_apply<fo::ResultOut>(some, h, last, cus, stream); });
@@ -1186,10 +1291,7 @@ int fo_muon_step(const fo_tensor_desc* matrices, const fo_matrix_shape* shapes, 
             hipStream_t s = (hipStream_t)stream;
             if (int rc = dtype == FO_F32 ? momentum<fo::DT_F32>(a, h, quantized, s) : dtype == FO_BF16 ? momentum<fo::DT_BF16>(a, h, quantized, s)
                                                                                                 : momentum<fo::DT_F16>(a, h, quantized, s)) return rc;
-            const fo::Groups small = take_small(a);
-            if (small.n > 0) {
-                if (int rc = launch_small_update(small, it, last, dtype, ecc_bytes, s)) return rc;
-            }
+            if (int rc = launch_held_update(a, it, last, dtype, ecc_bytes, s)) return rc;
             if (a.n == 0) {
                 for (int64_t k = 0; k < n; ++k) matrices += shapes[i + k].count;
                 continue;

@@ -74,8 +74,9 @@ def newton_schulz(
         eps: added to the norm; a matrix of zeros stays one.
 
     Returns:
-        bfloat16, whatever the type of `x` (the products run on fp16 parts and come within 1e-3 of the result), in the shape of
-        `x`; contiguous, or laid out like `x` where its columns and not its rows are contiguous.
+        bfloat16, whatever the type of `x` (the products run on fp16 parts and come within 1e-3 of the result's norm), in the shape of
+        `x`; contiguous, or laid out like `x` where its columns and not its rows are contiguous.  A matrix with an infinity or
+        a NaN comes back as NaNs.  No gradient flows through.
     """
     kernels._require_device(x, "newton_schulz")
     if x.dtype not in DTYPE_CODE:
@@ -288,6 +289,6 @@ class FlashMuon(FlashOptimizer):
         return MuonPlan(key.kind, key.dtype, key.ecc_bytes, key.quantized, tensors)
 
     def _launch_single(self, kind: str, quantized: bool, scalars: dict[str, Any], t: StepTensors) -> None:
-        # one matrix on its own (gradient release): its table is small, and kept with the parameter's other transient state
+        # one matrix on its own (gradient release): the gradient was made just now, and its table with it
         plan = MuonPlan(kind, t.param.dtype, kernels._ecc_bytes(t.ecc), quantized, [t])
         plan.launch(**scalars)
