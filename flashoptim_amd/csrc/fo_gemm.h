@@ -465,4 +465,37 @@ inline double tiles_time(const TileCost& c, double tiles, double length, int cus
     return rounds * full + last;
 }
 
+// A result of rows x cols in two launches: its first `lines` tile rows (columns) in tiles of `wt`, which fill whole rounds, what is left in
+// tiles of `rest`, two or more on a compute unit.  `wt` alone (rest = 0) where that takes no longer.  4096 x 14336 over 4096 values
+// is three and a half rounds of 256 x 256 tiles: with the last half
+// in one round of 128 x 128 tiles an fp16 step takes 492 us, in one launch 528; a scaled product's 155 us become 146.
+struct Cut { int wt, rest; bool columns; int lines; double time; };
+constexpr double kLaunchTime = 6.0;   // us that a second launch costs
+
+inline int64_t tiles_of(int64_t rows, int64_t cols, int wt) { return ((rows + 2 * wt - 1) / (2 * wt)) * ((cols + 2 * wt - 1) / (2 * wt)); }
+
+// `before` tiles over before_length values(wt) are in the launch already, ahead of this result.
+template <int N, class F> Cut best_cut(const TileCost (&costs)[N], int64_t rows, int64_t cols, double length, F before, double before_length, int cus) {
+    Cut best{};
+    for (const TileCost& c : costs) {
+        const double ahead = before(c.wt);
+        const auto time = [&](double tiles) { return tiles_time(c, ahead + tiles, (ahead * before_length + tiles * length) / (ahead + tiles), cus); };
+        const int64_t across[2] = {(cols + 2 * c.wt - 1) / (2 * c.wt), (rows + 2 * c.wt - 1) / (2 * c.wt)};   // tiles in a row, in a column
+        const double whole = time((double)(across[0] * across[1]));
+        if (!best.wt || whole < best.time) best = Cut{c.wt, 0, false, 0, whole};
+        const double seats = (double)cus * c.resident, full = __builtin_floor((ahead + (double)(across[0] * across[1])) / seats) * seats - ahead;
+        for (int columns = 0; columns < 2; ++columns) {
+            const int64_t lines = (int64_t)(full / (double)across[columns]);
+            if (full <= 0.0 || lines <= 0 || lines >= across[1 - columns]) continue;
+            const double first = time((double)(lines * across[columns])) + kLaunchTime;
+            const int64_t left_rows = columns ? rows : rows - lines * 2 * c.wt, left_cols = columns ? cols - lines * 2 * c.wt : cols;
+            for (const TileCost& r : costs) {
+                const double both = first + tiles_time(r, (double)tiles_of(left_rows, left_cols, r.wt), length, cus);
+                if (both < best.time) best = Cut{c.wt, r.wt, columns != 0, (int)lines, both};
+            }
+        }
+    }
+    return best;
+}
+
 }  // namespace fo

@@ -46,6 +46,7 @@ struct MatrixGroup {
     int first;            // matrix number of the first of them
     int generation;       // of hi and T that X is in
     int chunks;           // sums of squares of each
+    int parts;            // S: runs of the long axis that are summed apart
     float unit;           // the power of two that the first X is kept times
     float lr;             // optimizer step: learning rate with the shape's factor
     char* workspace;      // their arrays, see the functions below
@@ -63,6 +64,9 @@ struct MatrixGroup {
     __device__ _Float16* hi(int k, int generation) const { return (_Float16*)(of(k) + generation * area() * 4); }
     __device__ _Float16* t(int k, int generation) const { return (_Float16*)(of(k) + generation * area() * 4 + area() * 2); }
     __device__ float* update(int k) const { return (float*)(of(k) + area() * 4); }
+    // Sums over the parts, side x side each: over the generation that the step writes next.
+    __host__ __device__ int most_parts() const { return (tall() ? padded_rows : padded_cols) / side(); }
+    __device__ float* partial(int k, int part) const { return (float*)(of(k) + (generation ^ 1) * area() * 4) + gram_area() * part; }
     __device__ u32* lo(int k) const { return (u32*)(of(k) + area() * 8); }   // pairs of bf16
     __device__ _Float16* square(int k, int which) const { return (_Float16*)(of(k) + area() * 10 + gram_area() * 2 * which); }
     __device__ float* diagonal(int k, int which) const { return (float*)(of(k) + area() * 10 + gram_area() * 6) + side() * which; }
@@ -142,6 +146,7 @@ __global__ __launch_bounds__(256) void norm_kernel(Groups a, float eps) {
     const MatrixGroup& m = a.group[g];
     const int k = (int)(blockIdx.x - a.begin[g]);
     double sum = 0.0;
+#pragma unroll 8
     for (int i = threadIdx.x; i < m.chunks; i += 256) sum += m.squares(k)[i];
     const double total = workgroup_sum(sum, lds);
     if (threadIdx.x == 0) *m.factor(k) = (float)((double)m.unit / (sqrt(total) + (double)eps));
@@ -282,18 +287,20 @@ template <int DT, bool QUANT> __global__ __launch_bounds__(256) void momentum_ke
 // the products
 // ------------------------------------------------------------------------------------------------
 
-// One of a matrix's three square matrices from two others: out = gamma U V + alpha U + beta V; or S (GRAM), of which `first` says that X
-// still carries the unit.
-enum { kSlots = 3 };
+// One of a matrix's three square matrices: S, of which `first` says that X still carries the unit (kGram); from two others, out = gamma U V +
+// alpha U + beta V (kMixed); or, where U = V and beta = 0, the same with half of the epilogue's reads (kPoly).
+// kPartial: S over one part of the long axis, added up by gather_kernel.
+enum { kGram, kPoly, kMixed, kPartial };
 struct SquareArgs {
     int u, v, out;
     float alpha, beta, gamma;
     int first;
 };
-// X <- a X + (square matrix `poly`) X.
+// X <- a X + (square matrix `poly`) X, between the given rows and columns of the padded matrices (to their ends at most).
 struct StepArgs {
     float a;
     int poly, first;
+    int row_begin = 0, col_begin = 0, row_end = INT32_MAX, col_end = INT32_MAX;
 };
 
 __device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
@@ -304,7 +311,7 @@ __device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
 }
 
 // Square matrices without their diagonals: all are symmetric, so each tile off the diagonal is written twice.
-template <bool GRAM> struct SymmetricOut {
+template <int KIND> struct SymmetricOut {
     static constexpr bool kColumns = true;
     const _Float16 *u, *v;
     const float *u_diagonal, *v_diagonal;
@@ -317,7 +324,7 @@ template <bool GRAM> struct SymmetricOut {
 
     struct In { f16x8 u, v; float d; };
     __device__ __forceinline__ void begin(int j) {
-        if constexpr (!GRAM) {
+        if constexpr (KIND != kGram) {
             if (j < side) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[e] = v_diagonal[j + e];
@@ -325,10 +332,10 @@ template <bool GRAM> struct SymmetricOut {
         }
     }
     __device__ __forceinline__ void load(int i, int j, In& in) const {
-        if constexpr (!GRAM) {
+        if constexpr (KIND != kGram) {
             if (i < side && j < side) {
                 in.u = *reinterpret_cast<const f16x8*>(u + (int64_t)i * side + j);
-                in.v = u == v ? in.u : *reinterpret_cast<const f16x8*>(v + (int64_t)i * side + j);
+                if constexpr (KIND == kMixed) in.v = *reinterpret_cast<const f16x8*>(v + (int64_t)i * side + j);
                 in.d = u_diagonal[i];
             }
         }
@@ -337,9 +344,16 @@ template <bool GRAM> struct SymmetricOut {
         if (i >= side || j >= side) return;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if constexpr (GRAM) {
+            if constexpr (KIND == kGram) {
                 x[e] *= scale;
                 if (i == j + e) { diagonal[i] = x[e]; x[e] = 0.0f; }
+            } else if constexpr (KIND == kPoly) {
+                const float a = (float)in.u[e];   // 0 on the diagonal
+                x[e] = fmaf(gamma, fmaf(in.d + d[e], a, x[e]), alpha * a);
+                if (i == j + e) {
+                    diagonal[i] = fmaf(in.d, fmaf(gamma, in.d, alpha), x[e]);
+                    x[e] = 0.0f;
+                }
             } else {
                 const float a = (float)in.u[e], b = (float)in.v[e], product = fmaf(in.d, b, fmaf(a, d[e], x[e]));   // a = b = 0 on the diagonal
                 x[e] = fmaf(gamma, product, fmaf(alpha, a, beta * b));
@@ -358,28 +372,75 @@ template <bool GRAM> struct SymmetricOut {
     }
 };
 
-template <int WT, bool GRAM> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void symmetric_kernel(Groups a, SquareArgs h) {
+struct PartialOut {
+    static constexpr bool kColumns = false;
+    float* out;
+    int side;
+    struct In {};
+    __device__ __forceinline__ void begin(int) const {}
+    __device__ __forceinline__ void load(int, int, In&) const {}
+    __device__ __forceinline__ void row(int i, int j, In, const float (&x)[8]) const {
+        if (i >= side || j >= side) return;
+        f32x4* to = reinterpret_cast<f32x4*>(out + (int64_t)i * side + j);
+        to[0] = f32x4{x[0], x[1], x[2], x[3]};
+        to[1] = f32x4{x[4], x[5], x[6], x[7]};
+    }
+};
+
+template <int WT, int KIND> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void symmetric_kernel(Groups a, SquareArgs h) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef GemmTile<F16Product, WT> Tile;
     const int64_t seat = blockIdx.x >> 3;
     const int g = group_of(a, seat);
     const MatrixGroup& m = a.group[g];
     const int side = m.side(), n = (side + Tile::kTile - 1) / Tile::kTile, tiles = n * (n + 1) / 2;
-    const int64_t local = tile_of_seat(blockIdx.x & 7, seat - a.begin[g], (int64_t)tiles * m.count);
+    const int parts = KIND == kPartial ? m.parts : 1, each = tiles * parts;
+    const int64_t local = tile_of_seat(blockIdx.x & 7, seat - a.begin[g], (int64_t)each * m.count);
     if (local < 0) return;
-    const int k = (int)(local / tiles);
+    const int k = (int)(local / each), part = (int)(local % each) / tiles;
     int i, j;
     tile_at_symmetric((int)(local % tiles), n, i, j);
     const bool tall = m.tall();
     const _Float16* x = tall ? m.t(k, m.generation) : m.hi(k, m.generation);
-    const int64_t length = (GRAM ? (tall ? m.padded_rows : m.padded_cols) : side) * 2;
-    const Operand left{(const char*)(GRAM ? x : m.square(k, h.u)), length, nullptr, 0, side};
-    const Operand right{(const char*)(GRAM ? x : m.square(k, h.v)), length, nullptr, 0, side};
+    constexpr bool kOfX = KIND == kGram || KIND == kPartial;
+    const int64_t length = (kOfX ? (tall ? m.padded_rows : m.padded_cols) : side) * 2;
+    // whole stages of 64 values for each part
+    const int64_t run = KIND == kPartial ? ((length / kStageBytes + parts - 1) / parts) * kStageBytes : length, from = part * run;
+    const Operand left{(const char*)(kOfX ? x : m.square(k, h.u)) + from, length, nullptr, 0, side};
+    const Operand right{(const char*)(kOfX ? x : m.square(k, h.v)) + from, length, nullptr, 0, side};
     Tile tile(lds);
-    tile.multiply(left, right, i * Tile::kTile, j * Tile::kTile, (int)length);
-    SymmetricOut<GRAM> out{m.square(k, h.u), m.square(k, h.v), m.diagonal(k, h.u), m.diagonal(k, h.v), m.square(k, h.out), m.diagonal(k, h.out), side,
-                           h.first ? 1.0f / (m.unit * m.unit) : 1.0f, h.alpha, h.beta, h.gamma, i != j, {}};
-    tile.finish(i * Tile::kTile, j * Tile::kTile, out);
+    tile.multiply(left, right, i * Tile::kTile, j * Tile::kTile, (int)(run < length - from ? run : length - from));
+    if constexpr (KIND == kPartial) {
+        PartialOut out{m.partial(k, part), side};
+        tile.finish(i * Tile::kTile, j * Tile::kTile, out);
+    } else {
+        SymmetricOut<KIND> out{m.square(k, h.u), m.square(k, h.v), m.diagonal(k, h.u), m.diagonal(k, h.v), m.square(k, h.out), m.diagonal(k, h.out), side,
+                               h.first ? 1.0f / (m.unit * m.unit) : 1.0f, h.alpha, h.beta, h.gamma, i != j, {}};
+        tile.finish(i * Tile::kTile, j * Tile::kTile, out);
+    }
+}
+
+// S of its parts, in order; a workgroup takes four rows of a 64 x 64 tile on or above the diagonal.
+__global__ __launch_bounds__(256) void gather_kernel(Groups a, SquareArgs h) {
+    const int g = group_of(a, blockIdx.x);
+    const MatrixGroup& m = a.group[g];
+    const int side = m.side(), n = side / 64, each = n * (n + 1) / 2 * 16;
+    const int64_t local = blockIdx.x - a.begin[g];
+    const int k = (int)(local / each), piece = (int)(local % each);
+    int i, j;
+    tile_at_symmetric(piece / 16, n, i, j);
+    i = i * 64 + piece % 16 * 4 + (threadIdx.x >> 6);
+    j = j * 64 + (threadIdx.x & 63);
+    if (i > j) return;
+    const float* in = m.partial(k, 0) + (int64_t)i * side + j;
+    float x = 0.0f;
+#pragma unroll 8
+    for (int part = 0; part < m.parts; ++part) x += in[m.gram_area() * part];
+    if (h.first) x *= 1.0f / (m.unit * m.unit);
+    if (i == j) { m.diagonal(k, h.out)[i] = x; x = 0.0f; }
+    _Float16* s = m.square(k, h.out);
+    s[(int64_t)i * side + j] = (_Float16)x;
+    s[(int64_t)j * side + i] = (_Float16)x;
 }
 
 // X <- a X + B X, common to the steps: x = (acc + (a + d) (hi + lo)) / unit, d the diagonal entry of B.
@@ -521,7 +582,8 @@ template <int WT, class Out> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2)
     const int64_t seat = blockIdx.x >> 3;
     const int g = group_of(a, seat);
     const MatrixGroup& m = a.group[g];
-    const int rows = (m.padded_rows + Tile::kTile - 1) / Tile::kTile, cols = (m.padded_cols + Tile::kTile - 1) / Tile::kTile;
+    const int row_end = m.padded_rows < h.row_end ? m.padded_rows : h.row_end, col_end = m.padded_cols < h.col_end ? m.padded_cols : h.col_end;
+    const int rows = (row_end - h.row_begin + Tile::kTile - 1) / Tile::kTile, cols = (col_end - h.col_begin + Tile::kTile - 1) / Tile::kTile;
     const int64_t local = tile_of_seat(blockIdx.x & 7, seat - a.begin[g], (int64_t)rows * cols * m.count);
     if (local < 0) return;
     const int k = (int)(local / (rows * cols));
@@ -533,14 +595,15 @@ template <int WT, class Out> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2)
     const Operand main{(const char*)m.hi(k, m.generation), side * 2, nullptr, 0, m.padded_rows};
     const Operand turned{(const char*)m.t(k, m.generation), side * 2, nullptr, 0, m.padded_cols};
     Tile tile(lds);
-    tile.multiply(tall ? main : poly, tall ? poly : turned, i * Tile::kTile, j * Tile::kTile, side * 2);
+    const int row0 = h.row_begin + i * Tile::kTile, col0 = h.col_begin + j * Tile::kTile;
+    tile.multiply(tall ? main : poly, tall ? poly : turned, row0, col0, side * 2);
     const ApplyIn in{m.hi(k, m.generation), m.lo(k), m.diagonal(k, h.poly), m.padded_rows, m.padded_cols, h.a, h.first ? 1.0f / m.unit : 1.0f, tall, {}};
     if constexpr (Out::kColumns) {
         Out out{in, m.hi(k, m.generation ^ 1), m.t(k, m.generation ^ 1)};
-        tile.finish(i * Tile::kTile, j * Tile::kTile, out);
+        tile.finish(row0, col0, out);
     } else {
         Out out(in, last, m, k);
-        tile.finish(i * Tile::kTile, j * Tile::kTile, out);
+        tile.finish(row0, col0, out);
     }
 }
 
@@ -984,6 +1047,7 @@ int64_t plan(const fo_matrix_shape* shapes, int64_t n, char* workspace, fo::Grou
             m.padded_rows = (int)padded(s.rows); m.padded_cols = (int)padded(s.cols);
             m.chunks = (int)(((int64_t)s.rows * s.cols + fo::kChunk - 1) / fo::kChunk);
             m.unit = 1.0f;
+            m.parts = 1;
             const int longer = s.rows > s.cols ? s.rows : s.cols;
             while (m.unit * m.unit * 4.0f <= (float)longer) m.unit *= 2.0f;
             m.workspace = workspace + at;
@@ -1010,6 +1074,18 @@ template <class F> int64_t spread(fo::Groups& a, F each) {
     return a.begin[a.n];
 }
 
+// The groups that `which` picks, a workgroup to a matrix; with `leave` they are gone from `a`.
+fo::Groups take(fo::Groups& a, bool (*which)(const fo::MatrixGroup&), bool leave) {
+    fo::Groups taken{}, left{};
+    for (int g = 0; g < a.n; ++g) {
+        fo::Groups& to = which(a.group[g]) ? taken : left;
+        to.group[to.n++] = a.group[g];
+    }
+    if (leave) a = left;
+    spread(taken, [](const fo::MatrixGroup&) { return (int64_t)1; });
+    return taken;
+}
+
 int64_t tiles_across(int n, int tile) { return (n + tile - 1) / tile; }
 
 template <class K, class... Args> int launch(K kernel, int64_t grid, int threads, int lds, hipStream_t stream, const char* what, Args... args) {
@@ -1028,9 +1104,9 @@ constexpr fo::TileCost kTileCosts[] = {
     {128, 1, 14.0, 0.0286, 14.0, 0.0286}, {96, 1, 16.0, 0.0170, 16.0, 0.0170}, {64, 2, 9.5, 0.0115, 8.0, 0.0165}, {32, 5, 4.2, 0.0063, 7.0, 0.0110}};
 
 // tiles(group, wt) of a matrix, length(group) contracted.
-template <class T, class L> int choose(const fo::Groups& a, int cus, T tiles, L length) {
+template <class T, class L> int choose(const fo::Groups& a, int cus, T tiles, L length, double& least) {
     int best = 0;
-    double least = 0.0;
+    least = 0.0;
     for (const fo::TileCost& t : kTileCosts) {
         double all = 0.0, values = 0.0;
         for (int g = 0; g < a.n; ++g) {
@@ -1045,7 +1121,7 @@ template <class T, class L> int choose(const fo::Groups& a, int cus, T tiles, L 
 }
 
 int64_t symmetric_tiles(const fo::MatrixGroup& m, int wt) { const int64_t n = tiles_across(m.side(), 2 * wt); return n * (n + 1) / 2; }
-int64_t apply_tiles(const fo::MatrixGroup& m, int wt) { return tiles_across(m.padded_rows, 2 * wt) * tiles_across(m.padded_cols, 2 * wt); }
+int64_t apply_tiles(const fo::MatrixGroup& m, int wt) { return fo::tiles_of(m.padded_rows, m.padded_cols, wt); }
 
 // Seats per die, and the grid.
 template <class F> int64_t seat(fo::Groups& a, F tiles) {
@@ -1054,29 +1130,93 @@ template <class F> int64_t seat(fo::Groups& a, F tiles) {
     return a.begin[a.n] * 8;
 }
 
-template <int WT, bool GRAM> int launch_symmetric(fo::Groups& a, const fo::SquareArgs& h, hipStream_t stream) {
-    const int64_t grid = seat(a, [](const fo::MatrixGroup& m) { return symmetric_tiles(m, WT); });
-    return launch(fo::symmetric_kernel<WT, GRAM>, grid, 256, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz product", a, h);
+template <int WT, int KIND> int launch_symmetric(fo::Groups& a, const fo::SquareArgs& h, hipStream_t stream) {
+    const int64_t grid = seat(a, [](const fo::MatrixGroup& m) { return symmetric_tiles(m, WT) * (KIND == fo::kPartial ? m.parts : 1); });
+    return launch(fo::symmetric_kernel<WT, KIND>, grid, 256, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz product", a, h);
 }
-template <bool GRAM> int launch_symmetric(fo::Groups& a, const fo::SquareArgs& h, int cus, hipStream_t stream) {
-    switch (choose(a, cus, symmetric_tiles, [](const fo::MatrixGroup& m) { return !GRAM ? m.side() : m.tall() ? m.padded_rows : m.padded_cols; })) {
-        case 128: return launch_symmetric<128, GRAM>(a, h, stream);
-        case 96: return launch_symmetric<96, GRAM>(a, h, stream);
-        case 64: return launch_symmetric<64, GRAM>(a, h, stream);
-        default: return launch_symmetric<32, GRAM>(a, h, stream);
+template <int KIND> int launch_symmetric(int wt, fo::Groups& a, const fo::SquareArgs& h, hipStream_t stream) {
+    switch (wt) {
+        case 128: return launch_symmetric<128, KIND>(a, h, stream);
+        case 96: return launch_symmetric<96, KIND>(a, h, stream);
+        case 64: return launch_symmetric<64, KIND>(a, h, stream);
+        default: return launch_symmetric<32, KIND>(a, h, stream);
     }
 }
+template <int KIND> int launch_square(fo::Groups& a, const fo::SquareArgs& h, int cus, hipStream_t stream) {
+    double least;
+    return launch_symmetric<KIND>(choose(a, cus, symmetric_tiles, [](const fo::MatrixGroup& m) { return m.side(); }, least), a, h, stream);
+}
+
+int long_axis(const fo::MatrixGroup& m) { return m.tall() ? m.padded_rows : m.padded_cols; }
+constexpr int kPartialMost = 64;   // few and short parts are what small tiles are for
+// At most `most`, of whole stages of 64 values, none of them empty.
+int parts_of(const fo::MatrixGroup& m, int most) {
+    const int stages = long_axis(m) / 64, parts = std::max(1, std::min({most, m.most_parts(), stages / 2})), run = (stages + parts - 1) / parts;
+    return (stages + run - 1) / run;
+}
+
+// S has few tiles where one side is short, each contracted over the whole other side.  Then the long axis is cut into parts that
+// are contracted at the same time and added up: 64 x 14336 takes 115 instead of 518 us in all, 1024 x 14336 493 instead of 733.
+// How many parts goes by the shape alone, so that a matrix's result does not depend on what shares the launch; a quarter of the time has
+// to be gained by it.
+int gram_parts(const fo::MatrixGroup& m, int cus) {
+    double least = 0.0;
+    int best = 1;
+    for (const fo::TileCost& t : kTileCosts) {
+        const double time = 0.75 * fo::tiles_time(t, (double)symmetric_tiles(m, t.wt), long_axis(m), cus);
+        if (least == 0.0 || time < least) least = time;
+    }
+    for (int most = 2; most <= 128; most *= 2) {
+        for (const fo::TileCost& t : kTileCosts) {
+            if (t.wt > kPartialMost) continue;
+            const int parts = parts_of(m, most);
+            const double time = fo::tiles_time(t, (double)symmetric_tiles(m, t.wt) * parts, (double)long_axis(m) / parts, cus) + fo::kLaunchTime
+                              + (double)m.gram_area() * parts * 4e-6;   // sums written and read at 2 TB/s
+            if (time < least) { least = time; best = parts; }
+        }
+    }
+    return best;
+}
+int launch_gram(fo::Groups& a, const fo::SquareArgs& h, int cus, hipStream_t stream) {
+    fo::Groups parted = take(a, [](const fo::MatrixGroup& m) { return m.parts > 1; }, false), whole = take(a, [](const fo::MatrixGroup& m) { return m.parts == 1; }, false);
+    double least;
+    if (whole.n > 0) {
+        const int wt = choose(whole, cus, symmetric_tiles, long_axis, least);
+        if (int rc = launch_symmetric<fo::kGram>(wt, whole, h, stream)) return rc;
+    }
+    if (parted.n == 0) return 0;
+    const int wt = choose(parted, cus, [](const fo::MatrixGroup& m, int wt) { return symmetric_tiles(m, wt) * m.parts; },
+                          [](const fo::MatrixGroup& m) { return long_axis(m) / m.parts; }, least);
+    if (int rc = wt >= kPartialMost ? launch_symmetric<kPartialMost, fo::kPartial>(parted, h, stream) : launch_symmetric<32, fo::kPartial>(parted, h, stream)) return rc;
+    const int64_t grid = spread(parted, [](const fo::MatrixGroup& m) { return symmetric_tiles(m, 32) * 16; });
+    return launch(fo::gather_kernel, grid, 256, 0, stream, "Newton-Schulz sums", parted, h);
+}
 template <int WT, class Out> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, hipStream_t stream) {
-    const int64_t grid = seat(a, [](const fo::MatrixGroup& m) { return apply_tiles(m, WT); });
+    const int64_t grid = seat(a, [&](const fo::MatrixGroup& m) {
+        return fo::tiles_of(std::min(m.padded_rows, h.row_end) - h.row_begin, std::min(m.padded_cols, h.col_end) - h.col_begin, WT);
+    });
     return launch(fo::apply_kernel<WT, Out>, grid, 256, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz step", a, h, last);
 }
-template <class Out> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, int cus, hipStream_t stream) {
-    switch (choose(a, cus, apply_tiles, [](const fo::MatrixGroup& m) { return m.side(); })) {
+template <class Out> int launch_apply(int wt, fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, hipStream_t stream) {
+    switch (wt) {
         case 128: return launch_apply<128, Out>(a, h, last, stream);
         case 96: return launch_apply<96, Out>(a, h, last, stream);
         case 64: return launch_apply<64, Out>(a, h, last, stream);
         default: return launch_apply<32, Out>(a, h, last, stream);
     }
+}
+// One matrix may be cut (fo_gemm.h); of several the rounds run on from one to the next.
+template <class Out> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, int cus, hipStream_t stream) {
+    const fo::MatrixGroup& m = a.group[0];
+    double least;
+    if (a.n > 1 || m.count > 1) return launch_apply<Out>(choose(a, cus, apply_tiles, [](const fo::MatrixGroup& m) { return m.side(); }, least), a, h, last, stream);
+    const fo::Cut cut = fo::best_cut(kTileCosts, m.padded_rows, m.padded_cols, m.side(), [](int) { return 0.0; }, 0.0, cus);
+    if (!cut.rest) return launch_apply<Out>(cut.wt, a, h, last, stream);
+    fo::StepArgs first = h, rest = h;
+    if (cut.columns) first.col_end = rest.col_begin = cut.lines * 2 * cut.wt;
+    else first.row_end = rest.row_begin = cut.lines * 2 * cut.wt;
+    if (int rc = launch_apply<Out>(cut.wt, a, first, last, stream)) return rc;
+    return launch_apply<Out>(cut.rest, a, rest, last, stream);
 }
 int launch_update(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, int dtype, int ecc_bytes, int cus, hipStream_t stream) {
     if (dtype == FO_F32) return launch_apply<fo::UpdateOut<fo::DT_F32, 0>>(a, h, last, cus, stream);
@@ -1101,23 +1241,13 @@ int validate_iteration(int steps, const float* coefficients, float eps) {
 bool is_tiny(const fo::MatrixGroup& m) { return std::min(m.rows, m.cols) <= fo::kTinySide && std::max(m.rows, m.cols) <= fo::kTinyLength; }
 bool is_small(const fo::MatrixGroup& m) { return fo::SmallShape(m).fits(); }
 
-fo::Groups take(fo::Groups& a, bool (*which)(const fo::MatrixGroup&)) {
-    fo::Groups taken{}, left{};
-    for (int g = 0; g < a.n; ++g) {
-        fo::Groups& to = which(a.group[g]) ? taken : left;
-        to.group[to.n++] = a.group[g];
-    }
-    a = left;
-    spread(taken, [](const fo::MatrixGroup&) { return (int64_t)1; });
-    return taken;
-}
 template <int DT, class Out> int launch_held(fo::Groups& a, const fo::MatrixSource& source, const Iteration& it, const fo::LastArgs& last, hipStream_t stream) {
     const fo::SmallArgs h{it.a, it.b, it.c, it.eps, it.steps};
-    const fo::Groups tiny = take(a, is_tiny);
+    const fo::Groups tiny = take(a, is_tiny, true);
     if (tiny.n > 0) {
         if (int rc = launch(fo::tiny_kernel<DT, Out>, tiny.begin[tiny.n], 64, 0, stream, "Newton-Schulz of the smallest matrices", tiny, source, h, last)) return rc;
     }
-    const fo::Groups small = take(a, is_small);
+    const fo::Groups small = take(a, is_small, true);
     if (small.n == 0) return 0;
     return launch(fo::small_kernel<DT, Out>, small.begin[small.n], fo::kSmallThreads, fo::kSmallLds, stream, "Newton-Schulz of small matrices", small, source, h, last);
 }
@@ -1138,12 +1268,12 @@ struct Steps {
     int cus;
     hipStream_t stream;
 
-    int gram(fo::Groups& a, int out, int first) const { return launch_symmetric<true>(a, fo::SquareArgs{0, 0, out, 0.0f, 0.0f, 0.0f, first}, cus, stream); }
+    int gram(fo::Groups& a, int out, int first) const { return launch_gram(a, fo::SquareArgs{0, 0, out, 0.0f, 0.0f, 0.0f, first}, cus, stream); }
     int square(fo::Groups& a, int u, int v, int out, float alpha, float beta, float gamma) const {
-        return launch_symmetric<false>(a, fo::SquareArgs{u, v, out, alpha, beta, gamma, 0}, cus, stream);
+        return launch_square<fo::kMixed>(a, fo::SquareArgs{u, v, out, alpha, beta, gamma, 0}, cus, stream);
     }
     // B of S
-    int poly(fo::Groups& a, int s, int out) const { return square(a, s, s, out, it.b, 0.0f, it.c); }
+    int poly(fo::Groups& a, int s, int out) const { return launch_square<fo::kPoly>(a, fo::SquareArgs{s, s, out, it.b, 0.0f, it.c, 0}, cus, stream); }
 
     // Up to X's own product.
     int one(fo::Groups& a, int first, fo::StepArgs& then) const {
@@ -1186,6 +1316,7 @@ template <int DT, class F> int iterate(fo::Groups& a, const fo::MatrixSource& so
     if (int rc = launch(fo::norm_kernel, grid, 256, 0, stream, "norm", a, it.eps)) return rc;
     grid = spread(a, [](const fo::MatrixGroup& m) { return m.area() / 4096; });
     if (int rc = launch(fo::split_kernel<DT>, grid, 256, 0, stream, "normalisation", a, source)) return rc;
+    for (int g = 0; g < a.n; ++g) a.group[g].parts = gram_parts(a.group[g], cus);
     const Steps steps{it, cus, stream};
     fo::StepArgs then{};
     int done = 0;

@@ -207,6 +207,7 @@ struct ProductJob {
     char* out;
     int rows, cols, blocks;             // of the result; 128-value blocks of the contracted axis
     int dtype;
+    int64_t out_stride;                 // values between the result's rows
 };
 struct ProductArgs {
     ProductJob job[2];
@@ -217,12 +218,13 @@ struct ProductOut {
     static constexpr bool kColumns = false;
     char* out;
     int rows, cols, dtype;
+    int64_t stride;
     struct In {};
     __device__ __forceinline__ void begin(int) const {}
     __device__ __forceinline__ void load(int, int, In&) const {}
     __device__ __forceinline__ void row(int i, int j, In, float (&v)[8]) const {
         if (i >= rows || j >= cols) return;
-        const int64_t at = (int64_t)i * cols + j;
+        const int64_t at = i * stride + j;
         if (dtype == DT_BF16) store_values<DT_BF16>(v, out + at * 2, cols - j);
         else if (dtype == DT_F16) store_values<DT_F16>(v, out + at * 2, cols - j);
         else store_values<DT_F32>(v, out + at * 4, cols - j);
@@ -244,7 +246,7 @@ template <int WT> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void mx_pr
     const Operand a{p.a, row_bytes, p.a_scales, row_bytes / 16, p.rows}, b{p.b, row_bytes, p.b_scales, row_bytes / 16, p.cols};
     Tile tile(smem);
     tile.multiply(a, b, i * Tile::kTile, j * Tile::kTile, (int)row_bytes);
-    ProductOut out{p.out, p.rows, p.cols, p.dtype};
+    ProductOut out{p.out, p.rows, p.cols, p.dtype, p.out_stride};
     tile.finish(i * Tile::kTile, j * Tile::kTile, out);
 }
 
@@ -490,7 +492,7 @@ int launch_coded_tokens(const fo::TokensArgs& p, void* stream) {
 constexpr fo::TileCost kTileCosts[] = {
     {128, 1, 11.5, 0.0073, 11.5, 0.0073}, {96, 1, 8.0, 0.0046, 8.0, 0.0046}, {64, 2, 3.5, 0.0036, 5.0, 0.0052}, {32, 5, 2.0, 0.0022, 5.0, 0.0043}};
 
-int64_t tiles(const fo::ProductJob& p, int wt) { return (int64_t)((p.rows + 2 * wt - 1) / (2 * wt)) * ((p.cols + 2 * wt - 1) / (2 * wt)); }
+int64_t tiles(const fo::ProductJob& p, int wt) { return fo::tiles_of(p.rows, p.cols, wt); }
 
 template <int WT> int launch_products(const fo::ProductJob* jobs, int n, void* stream) {
     fo::ProductArgs a{};
@@ -505,25 +507,38 @@ template <int WT> int launch_products(const fo::ProductJob* jobs, int n, void* s
     return launch(fo::mx_product_kernel<WT>, 8 * seats, 256, fo::GemmTile<fo::Mx4Product, WT>::kLds, stream, "fo_mxfp4_product", a);
 }
 
-// Up to two products in one launch, the longer contraction first.
-int launch_products(fo::ProductJob* jobs, int n, void* stream) {
-    const int cus = compute_units();
-    if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
-    if (n == 2 && jobs[0].blocks < jobs[1].blocks) { const fo::ProductJob t = jobs[0]; jobs[0] = jobs[1]; jobs[1] = t; }
-    int best = 0;
-    double least = 0.0;
-    for (const fo::TileCost& c : kTileCosts) {
-        double all = 0.0, values = 0.0;
-        for (int i = 0; i < n; ++i) { all += (double)tiles(jobs[i], c.wt); values += (double)tiles(jobs[i], c.wt) * jobs[i].blocks * fo::kBlock; }
-        const double time = fo::tiles_time(c, all, values / all, cus);
-        if (!best || time < least) { best = c.wt; least = time; }
-    }
-    switch (best) {
+int launch_products(int wt, const fo::ProductJob* jobs, int n, void* stream) {
+    switch (wt) {
         case 128: return launch_products<128>(jobs, n, stream);
         case 96: return launch_products<96>(jobs, n, stream);
         case 64: return launch_products<64>(jobs, n, stream);
         default: return launch_products<32>(jobs, n, stream);
     }
+}
+// The first `at` rows (columns) of a product, and the others.  Codes of rows are multiples of 64 bytes, so all stays aligned.
+void divide(const fo::ProductJob& p, bool columns, int at, fo::ProductJob& first, fo::ProductJob& rest) {
+    const int64_t row_bytes = (int64_t)p.blocks * (fo::kBlock / 2);
+    first = rest = p;
+    (columns ? first.cols : first.rows) = at;
+    (columns ? rest.cols : rest.rows) -= at;
+    (columns ? rest.b : rest.a) += at * row_bytes;
+    (columns ? rest.b_scales : rest.a_scales) += at * (row_bytes / 16);
+    rest.out += (columns ? (int64_t)at : (int64_t)at * p.out_stride) * (p.dtype == fo::DT_F32 ? 4 : 2);
+}
+
+// Up to two products in one launch, the longer contraction first; the last one may be cut (fo_gemm.h).
+int launch_products(fo::ProductJob* jobs, int n, void* stream) {
+    const int cus = compute_units();
+    if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
+    if (n == 2 && jobs[0].blocks < jobs[1].blocks) { const fo::ProductJob t = jobs[0]; jobs[0] = jobs[1]; jobs[1] = t; }
+    const fo::ProductJob last = jobs[n - 1];
+    const fo::Cut cut = fo::best_cut(kTileCosts, last.rows, last.cols, (double)last.blocks * fo::kBlock,
+                                     [&](int wt) { return n == 2 ? (double)tiles(jobs[0], wt) : 0.0; }, (double)jobs[0].blocks * fo::kBlock, cus);
+    if (!cut.rest) return launch_products(cut.wt, jobs, n, stream);
+    fo::ProductJob rest;
+    divide(last, cut.columns, cut.lines * 2 * cut.wt, jobs[n - 1], rest);
+    if (int rc = launch_products(cut.wt, jobs, n, stream)) return rc;
+    return launch_products(cut.rest, &rest, 1, stream);
 }
 
 fo::TokensArgs tokens_of(const fo::ProductJob& p) {
@@ -543,7 +558,7 @@ int run_products(const fo::ProductJob* jobs, int n, void* stream) {
 // A product of two forms: codes, then scales.
 fo::ProductJob product_of(const void* a, int64_t rows, const void* b, int64_t cols, int64_t inner, void* out, int dtype) {
     return {(const char*)a, (const char*)b, (const uint8_t*)a + form_codes(rows, inner), (const uint8_t*)b + form_codes(cols, inner), (char*)out,
-            (int)rows, (int)cols, (int)blocks_of(inner), dtype};
+            (int)rows, (int)cols, (int)blocks_of(inner), dtype, cols};
 }
 
 int check_forms(const void* a, const void* b, const void* c) {
@@ -589,7 +604,7 @@ int fo_mxfp4_product(const void* a, const void* a_scales, int64_t rows, const vo
     if (!a || !a_scales || !b || !b_scales || !out) return fail(FO_ERR_INVALID_ARGUMENT, "operands and out must not be NULL");
     if (((uintptr_t)a | (uintptr_t)b) & 15 || ((uintptr_t)a_scales | (uintptr_t)b_scales) & 3)
         return fail(FO_ERR_INVALID_ARGUMENT, "codes must be aligned to 16 bytes, scales to 4");
-    const fo::ProductJob job{(const char*)a, (const char*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)blocks_of(inner), dtype};
+    const fo::ProductJob job{(const char*)a, (const char*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, (char*)out, (int)rows, (int)cols, (int)blocks_of(inner), dtype, cols};
     return run_products(&job, 1, stream);
 }
 

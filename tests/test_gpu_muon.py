@@ -83,6 +83,15 @@ def test_iteration_against_float64(shape, dtype):
     _check(_fo().newton_schulz(x), _iterate(x), (shape, dtype))
 
 
+@pytest.mark.parametrize("shape", [(1, 40, 9000), (1, 9000, 40), (3, 130, 5000), (1, 600, 8000), (1, 8000, 600), (2, 64, 20011), (1, 16, 65536), (1, 65536, 3),
+                                   (40, 65, 4097), (1, 330, 14336)])
+def test_long_matrices_against_float64(shape):
+    """S comes as a sum over parts of the long axis."""
+    for steps in (1, 5):
+        x = _matrices(*shape, seed=sum(shape), dtype=torch.bfloat16)
+        _check(_fo().newton_schulz(x, steps=steps), _iterate(x, steps), (shape, steps))
+
+
 @pytest.mark.parametrize("steps,coefficients", [(1, COEFFICIENTS), (2, COEFFICIENTS), (3, COEFFICIENTS), (4, (2.0, -1.5, 0.5)),
                                                 (2, (1.5, -0.5, 0.0)), (6, (1.875, -1.25, 0.375))])
 @pytest.mark.parametrize("shape", [(2, 60, 90), (2, 300, 310), (1, 600, 1300), (1, 1300, 600)])
@@ -334,7 +343,7 @@ def test_step_against_float64(dtype, bits, quantize, hyper):
 
 def test_equal_gradients_take_equal_steps_whatever_shares_the_launch():
     """A matrix moves alike on its own, among others, in any order, and one parameter at a time."""
-    shapes = [(250, 300), (64, 40), (700, 500), (250, 300), (40, 64), (1, 9)]
+    shapes = [(250, 300), (64, 40), (700, 500), (250, 300), (40, 64), (1, 9), (70, 5000), (600, 4000), (5000, 70)]
     together = _make(shapes, torch.bfloat16, 2)
     alone = [nn.Parameter(p.detach().clone()) for p in together]
     one_by_one = [nn.Parameter(p.detach().clone()) for p in together]
