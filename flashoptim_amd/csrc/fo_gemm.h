@@ -6,14 +6,16 @@
 //
 // Shape.  A workgroup is four wavefronts in a 2x2 arrangement; a wavefront owns a WT x WT piece of the tile (WT = 128, 96,
 // 64 or 32) and keeps it in its accumulators.  The operands pass through LDS in stages of 128 bytes of every row (64 fp16
-// values, 256 codes), two stages in turn.  With WT = 128 the workgroup holds 128 KiB of LDS, a wavefront 256 accumulator
+// values, 256 codes), two stages in turn (or four, see below).  With WT = 128 the workgroup holds 128 KiB of LDS, a wavefront 256 accumulator
 // registers and both halves of a stage's operands in registers, and one wavefront runs on each SIMD: every LDS byte read is
 // used for eight instructions, which is what keeps LDS (128 bytes a clock) behind the matrix cores.
 //
 // Flow.  Per stage two phases of (WT/16)^2 matrix instructions.  Phase 1 multiplies the first half of the stage out of
 // registers while the second half is read from LDS; then the workgroup meets (nobody reads this stage any more, and the next
 // one has arrived); phase 2 multiplies the second half while the next stage's first half is read and the loads of the
-// stage after it are issued into the buffer that has become free.  A load has one whole stage of multiplications to arrive.
+// stage after it are issued into the buffer that has become free.  A load has one whole stage of multiplications to arrive; of
+// 64 x 64 tiles, whose stages are short, that covers it where four or five workgroups share a compute unit.  Where one has it alone, four
+// stages in LDS give a load three: 1000 x 1000 through five Newton-Schulz steps takes 154 instead of 190 us.
 //
 // Loads go from memory straight into LDS (16 bytes a lane, no registers).  They are inline asm: the compiler would wait for
 // all of them before every LDS read.  They have no register result, and every wait for them is written out below.
@@ -120,8 +122,7 @@ __device__ __forceinline__ void load_to_lds16(unsigned lds, unsigned offset, con
 __device__ __forceinline__ void load_to_lds4(unsigned lds, unsigned offset, const char* base) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory");
 }
-template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
-__device__ __forceinline__ void wait_loads_and_lds() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory"); }
+template <int N> __device__ __forceinline__ void wait_loads_and_lds() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory"); }
 __device__ __forceinline__ void meet() {
     asm volatile("" : : : "memory");
     __builtin_amdgcn_s_barrier();
@@ -136,7 +137,8 @@ __device__ __forceinline__ const char* uniform(const char* p) {
     return (const char*)(((uint64_t)hi << 32) | lo);
 }
 
-template <class Product, int WT> struct GemmTile {
+template <class Product, int WT, int STAGES> struct GemmTile {
+    static constexpr int kStages = STAGES;        // in LDS, 2 or 4
     static constexpr int kTile = 2 * WT;          // rows and columns of a workgroup's tile
     static constexpr int kFrags = WT / 16;        // 16-row pieces of a wavefront's operands
     static constexpr int kRows = 2 * kTile;       // rows of a stage, A's then B's
@@ -148,7 +150,7 @@ template <class Product, int WT> struct GemmTile {
     // the epilogue moves the tile through LDS in strips of 32 rows of a wavefront, 4 floats of padding per row
     static constexpr int kStripStride = WT + 4;
     static constexpr int kStripBytes = 32 * kStripStride * 4;
-    static constexpr int kLds = 2 * kBuffer > 4 * kStripBytes ? 2 * kBuffer : 4 * kStripBytes;
+    static constexpr int kLds = kStages * kBuffer > 4 * kStripBytes ? kStages * kBuffer : 4 * kStripBytes;
 
     typedef typename Product::Frag Frag;
 
@@ -196,7 +198,7 @@ template <class Product, int WT> struct GemmTile {
     }
     // The i-th load of a stage.  half: the rows end in the middle of the stage, its second half repeats the first.
     __device__ __forceinline__ void load(const Loader& l, int i, int stage, bool half) const {
-        const unsigned buffer = smem_address + (stage & 1) * kBuffer;
+        const unsigned buffer = smem_address + (stage & (kStages - 1)) * kBuffer;
         if (i < kRowLoads) {
             load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, l.row[i] - (half ? l.past_half : 0), l.base + (int64_t)stage * kStageBytes);
         } else if constexpr (Product::kScaled) {
@@ -218,14 +220,14 @@ template <class Product, int WT> struct GemmTile {
         const int i = is_b ? f : f - kFrags, group = lane >> 4;
         const int row = (is_b ? kTile + (wave & 1) * WT : (wave >> 1) * WT) + i * 16 + (lane & 15);
         const int piece = short_stage ? group : 2 * group + half;
-        (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const Frag*>(smem + (stage & 1) * kBuffer + row * kStageBytes + ((piece ^ (row & 7)) * 16));
+        (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const Frag*>(smem + (stage & (kStages - 1)) * kBuffer + row * kStageBytes + ((piece ^ (row & 7)) * 16));
     }
     // The four scale bytes among which the lane's two are.
     __device__ __forceinline__ void read_scales(Scales& to, int f, int stage, bool short_stage) const {
         const bool is_b = f < kFrags;
         const int i = is_b ? f : f - kFrags, group = lane >> 4;
         const int row = (is_b ? kTile + (wave & 1) * WT : (wave >> 1) * WT) + i * 16 + (lane & 15);
-        (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const int*>(smem + (stage & 1) * kBuffer + kScaleOffset + row * 8 + (short_stage ? 0 : (group >> 1) * 4));
+        (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const int*>(smem + (stage & (kStages - 1)) * kBuffer + kScaleOffset + row * 8 + (short_stage ? 0 : (group >> 1) * 4));
     }
     __device__ __forceinline__ void settle(Scales& now, const Scales& raw, bool short_stage) const {
         if constexpr (Product::kScaled) {
@@ -276,6 +278,16 @@ template <class Product, int WT> struct GemmTile {
     // Says that an accumulator lives in accumulator registers here.
     __device__ __forceinline__ static void keep(f32x4& c) { asm volatile("" : "+a"(c)); }
 
+    // Waits for LDS reads and for all loads but those of the last `later` stages (of kStages at most).
+    __device__ __forceinline__ static void wait_behind(int later) {
+        if constexpr (kStages > 2) {
+            if (later >= 3) { wait_loads_and_lds<3 * kLoads>(); return; }
+            if (later == 2) { wait_loads_and_lds<2 * kLoads>(); return; }
+        }
+        if (later >= 1) wait_loads_and_lds<kLoads>();
+        else wait_loads_and_lds<0>();
+    }
+
     // acc = the product's tile at (row0, col0) over rows of `row_bytes` > 0.
     __device__ __forceinline__ void multiply(const Operand& a, const Operand& b, int row0, int col0, int row_bytes) {
 #pragma unroll
@@ -290,14 +302,12 @@ template <class Product, int WT> struct GemmTile {
         Loader l;
         start(l, a, b, row0, col0);
 #pragma unroll
-        for (int k = 0; k < kLoads; ++k) load(l, k, 0, odd && stages == 1);
-        if (stages > 1) {
+        for (int stage = 0; stage < kStages; ++stage) {
+            if (stage >= stages) break;
 #pragma unroll
-            for (int k = 0; k < kLoads; ++k) load(l, k, 1, odd && stages == 2);
-            wait_loads<kLoads>();
-        } else {
-            wait_loads<0>();
+            for (int k = 0; k < kLoads; ++k) load(l, k, stage, odd && stages == stage + 1);
         }
+        wait_behind(stages - 1);
         meet();
         Operands even, uneven;
         Scales raw, scales;
@@ -308,18 +318,18 @@ template <class Product, int WT> struct GemmTile {
             if constexpr (Product::kScaled) read_scales(raw, f, 0, first_short);
         }
         int s = 0;
-        for (; s + 2 < stages; ++s) {
+        for (; s + kStages < stages; ++s) {
             settle(scales, raw, false);
             phase<0, false>(even, scales, uneven, raw, s, false, l, 0, false);
-            wait_loads_and_lds();  // stage s is in registers, stage s + 1 in LDS
+            wait_loads_and_lds<(kStages - 2) * kLoads>();  // stage s is in registers, stage s + 1 in LDS
             meet();
-            phase<1, true>(uneven, scales, even, raw, s + 1, odd && s + 2 == stages, l, s + 2, odd && s + 3 == stages);
+            phase<1, true>(uneven, scales, even, raw, s + 1, odd && s + 2 == stages, l, s + kStages, odd && s + kStages + 1 == stages);
         }
         for (;; ++s) {
             const bool last = s + 1 == stages;
             settle(scales, raw, odd && last);
             phase<0, false>(even, scales, uneven, raw, s, false, l, 0, false);
-            wait_loads_and_lds();
+            wait_behind(stages - s - 2);
             meet();
             if (last && odd) break;
             phase<1, false>(uneven, scales, even, raw, s + 1, odd && s + 2 == stages, l, 0, false);
@@ -454,7 +464,7 @@ __device__ __forceinline__ void tile_at_symmetric(int t, int n, int& i, int& j) 
 // ------------------------------------------------------------------------------------------- which tile a launch uses
 // Measured times of tiles, in us: a workgroup alone on its compute unit, and with the unit full of them; `each` per value
 // contracted.
-struct TileCost { int wt, resident; double start, each, start_full, each_full; };
+struct TileCost { int wt, stages, resident; double start, each, start_full, each_full; };
 
 // What `tiles` of them take on `cus` compute units, `length` values contracted: full rounds, then what is left.
 inline double tiles_time(const TileCost& c, double tiles, double length, int cus) {
@@ -465,11 +475,11 @@ inline double tiles_time(const TileCost& c, double tiles, double length, int cus
     return rounds * full + last;
 }
 
-// A result of rows x cols in two launches: its first `lines` tile rows (columns) in tiles of `wt`, which fill whole rounds, what is left in
-// tiles of `rest`, two or more on a compute unit.  `wt` alone (rest = 0) where that takes no longer.  4096 x 14336 over 4096 values
+// A result of rows x cols in two launches: its first `lines` tile rows (columns) in one kind of tile, which fill whole rounds, what is left in
+// another, two or more on a compute unit.  One kind alone (rest.wt = 0) where that takes no longer.  4096 x 14336 over 4096 values
 // is three and a half rounds of 256 x 256 tiles: with the last half
 // in one round of 128 x 128 tiles an fp16 step takes 492 us, in one launch 528; a scaled product's 155 us become 151.
-struct Cut { int wt, rest; bool columns; int lines; double time; };
+struct Cut { TileCost tile, rest; bool columns; int lines; double time; };
 constexpr double kLaunchTime = 6.0;   // us that a second launch costs
 
 inline int64_t tiles_of(int64_t rows, int64_t cols, int wt) { return ((rows + 2 * wt - 1) / (2 * wt)) * ((cols + 2 * wt - 1) / (2 * wt)); }
@@ -482,7 +492,7 @@ template <int N, class F> Cut best_cut(const TileCost (&costs)[N], int64_t rows,
         const auto time = [&](double tiles) { return tiles_time(c, ahead + tiles, (ahead * before_length + tiles * length) / (ahead + tiles), cus); };
         const int64_t across[2] = {(cols + 2 * c.wt - 1) / (2 * c.wt), (rows + 2 * c.wt - 1) / (2 * c.wt)};   // tiles in a row, in a column
         const double whole = time((double)(across[0] * across[1]));
-        if (!best.wt || whole < best.time) best = Cut{c.wt, 0, false, 0, whole};
+        if (!best.tile.wt || whole < best.time) best = Cut{c, TileCost{}, false, 0, whole};
         const double seats = (double)cus * c.resident, full = __builtin_floor((ahead + (double)(across[0] * across[1])) / seats) * seats - ahead;
         for (int columns = 0; columns < 2; ++columns) {
             const int64_t lines = (int64_t)(full / (double)across[columns]);
@@ -491,7 +501,7 @@ template <int N, class F> Cut best_cut(const TileCost (&costs)[N], int64_t rows,
             const int64_t left_rows = columns ? rows : rows - lines * 2 * c.wt, left_cols = columns ? cols - lines * 2 * c.wt : cols;
             for (const TileCost& r : costs) {
                 const double both = first + tiles_time(r, (double)tiles_of(left_rows, left_cols, r.wt), length, cus);
-                if (both < best.time) best = Cut{c.wt, r.wt, columns != 0, (int)lines, both};
+                if (both < best.time) best = Cut{c, r, columns != 0, (int)lines, both};
             }
         }
     }

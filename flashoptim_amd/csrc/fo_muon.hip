@@ -390,9 +390,9 @@ struct PartialOut {
 
 // Bound by the matrix cores, with 192 x 192 tiles as much by LDS: S of 14336 x 4096 in 260 us (925 TFLOP/s of the half that is computed), a
 // square of 4096 x 4096 in 80 (one round of 253 tiles either way; 256 x 256 tiles would fill 136 of 256 compute units).
-template <int WT, int KIND> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void symmetric_kernel(Groups a, SquareArgs h) {
+template <int WT, int STAGES, int KIND> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void symmetric_kernel(Groups a, SquareArgs h) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef GemmTile<F16Product, WT> Tile;
+    typedef GemmTile<F16Product, WT, STAGES> Tile;
     const int64_t seat = blockIdx.x >> 3;
     const int g = group_of(a, seat);
     const MatrixGroup& m = a.group[g];
@@ -581,9 +581,9 @@ template <int DT, int ECCB> struct UpdateOut : ApplyIn {
 
 // Out: ApplyOut, or what the last step does.  14336 x 4096 in 492 us, 980 TFLOP/s: a round of 256 x 256 tiles takes 135 us, 35 of which
 // its epilogues' 10 bytes an element would take alone, and the card's clock falls under such products.
-template <int WT, class Out> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void apply_kernel(Groups a, StepArgs h, LastArgs last) {
+template <int WT, int STAGES, class Out> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void apply_kernel(Groups a, StepArgs h, LastArgs last) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    typedef GemmTile<F16Product, WT> Tile;
+    typedef GemmTile<F16Product, WT, STAGES> Tile;
     const int64_t seat = blockIdx.x >> 3;
     const int g = group_of(a, seat);
     const MatrixGroup& m = a.group[g];
@@ -1107,11 +1107,12 @@ template <class K, class... Args> int launch(K kernel, int64_t grid, int threads
 // 4096, 1024 x 4096 and 1000 x 2730 matrices: 131 us for a 256 x 256 tile over 4096 values, 86 for 192 x 192, 75 for two
 // 128 x 128, 52 for five 64 x 64 (the smaller ones read more of LDS per multiplication); 43, 33, 24 (21 alone) and 18 (11) over 1024.
 constexpr fo::TileCost kTileCosts[] = {
-    {128, 1, 14.0, 0.0286, 14.0, 0.0286}, {96, 1, 16.0, 0.0170, 16.0, 0.0170}, {64, 2, 9.5, 0.0115, 8.0, 0.0165}, {32, 5, 4.2, 0.0063, 7.0, 0.0110}};
+    {128, 2, 1, 14.0, 0.0286, 14.0, 0.0286}, {96, 2, 1, 16.0, 0.0170, 16.0, 0.0170}, {64, 2, 2, 9.5, 0.0115, 8.0, 0.0165},
+    {32, 2, 5, 4.2, 0.0063, 7.0, 0.0110}, {32, 4, 2, 4.2, 0.0036, 7.0, 0.0058}};
 
 // tiles(group, wt) of a matrix, length(group) contracted.
-template <class T, class L> int choose(const fo::Groups& a, int cus, T tiles, L length, double& least) {
-    int best = 0;
+template <class T, class L> fo::TileCost choose(const fo::Groups& a, int cus, T tiles, L length, double& least) {
+    fo::TileCost best{};
     least = 0.0;
     for (const fo::TileCost& t : kTileCosts) {
         double all = 0.0, values = 0.0;
@@ -1121,7 +1122,7 @@ template <class T, class L> int choose(const fo::Groups& a, int cus, T tiles, L 
             values += n * length(a.group[g]);
         }
         const double time = fo::tiles_time(t, all, values / all, cus);
-        if (!best || time < least) { best = t.wt; least = time; }
+        if (!best.wt || time < least) { best = t; least = time; }
     }
     return best;
 }
@@ -1136,16 +1137,16 @@ template <class F> int64_t seat(fo::Groups& a, F tiles) {
     return a.begin[a.n] * 8;
 }
 
-template <int WT, int KIND> int launch_symmetric(fo::Groups& a, const fo::SquareArgs& h, hipStream_t stream) {
+template <int WT, int STAGES, int KIND> int launch_symmetric(fo::Groups& a, const fo::SquareArgs& h, hipStream_t stream) {
     const int64_t grid = seat(a, [](const fo::MatrixGroup& m) { return symmetric_tiles(m, WT) * (KIND == fo::kPartial ? m.parts : 1); });
-    return launch(fo::symmetric_kernel<WT, KIND>, grid, 256, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz product", a, h);
+    return launch(fo::symmetric_kernel<WT, STAGES, KIND>, grid, 256, fo::GemmTile<fo::F16Product, WT, STAGES>::kLds, stream, "Newton-Schulz product", a, h);
 }
-template <int KIND> int launch_symmetric(int wt, fo::Groups& a, const fo::SquareArgs& h, hipStream_t stream) {
-    switch (wt) {
-        case 128: return launch_symmetric<128, KIND>(a, h, stream);
-        case 96: return launch_symmetric<96, KIND>(a, h, stream);
-        case 64: return launch_symmetric<64, KIND>(a, h, stream);
-        default: return launch_symmetric<32, KIND>(a, h, stream);
+template <int KIND> int launch_symmetric(const fo::TileCost& t, fo::Groups& a, const fo::SquareArgs& h, hipStream_t stream) {
+    switch (t.wt) {
+        case 128: return launch_symmetric<128, 2, KIND>(a, h, stream);
+        case 96: return launch_symmetric<96, 2, KIND>(a, h, stream);
+        case 64: return launch_symmetric<64, 2, KIND>(a, h, stream);
+        default: return t.stages == 4 ? launch_symmetric<32, 4, KIND>(a, h, stream) : launch_symmetric<32, 2, KIND>(a, h, stream);
     }
 }
 template <int KIND> int launch_square(fo::Groups& a, const fo::SquareArgs& h, int cus, hipStream_t stream) {
@@ -1162,14 +1163,14 @@ int parts_of(const fo::MatrixGroup& m, int most) {
 }
 
 // S has few tiles where one side is short, each contracted over the whole other side.  Then the long axis is cut into parts that
-// are contracted at the same time and added up: 64 x 14336 takes 115 instead of 518 us in all, 1024 x 14336 493 instead of 733.
-// How many parts goes by the shape alone, so that a matrix's result does not depend on what shares the launch; a quarter of the time has
+// are contracted at the same time and added up: 64 x 14336 takes 109 instead of 518 us in all, 1024 x 14336 480 instead of 520.
+// How many parts goes by the shape alone, so that a matrix's result does not depend on what shares the launch; a tenth of the time has
 // to be gained by it.
 int gram_parts(const fo::MatrixGroup& m, int cus) {
     double least = 0.0;
     int best = 1;
     for (const fo::TileCost& t : kTileCosts) {
-        const double time = 0.75 * fo::tiles_time(t, (double)symmetric_tiles(m, t.wt), long_axis(m), cus);
+        const double time = 0.9 * fo::tiles_time(t, (double)symmetric_tiles(m, t.wt), long_axis(m), cus);
         if (least == 0.0 || time < least) least = time;
     }
     for (int most = 2; most <= 128; most *= 2) {
@@ -1177,7 +1178,7 @@ int gram_parts(const fo::MatrixGroup& m, int cus) {
             if (t.wt > kPartialMost) continue;
             const int parts = parts_of(m, most);
             const double time = fo::tiles_time(t, (double)symmetric_tiles(m, t.wt) * parts, (double)long_axis(m) / parts, cus) + fo::kLaunchTime
-                              + (double)m.gram_area() * parts * 4e-6;   // sums written and read at 2 TB/s
+                              + (double)m.gram_area() * parts * 1e-6 + 0.06 * parts;   // sums written and read, a row of loads of each
             if (time < least) { least = time; best = parts; }
         }
     }
@@ -1187,28 +1188,29 @@ int launch_gram(fo::Groups& a, const fo::SquareArgs& h, int cus, hipStream_t str
     fo::Groups parted = take(a, [](const fo::MatrixGroup& m) { return m.parts > 1; }, false), whole = take(a, [](const fo::MatrixGroup& m) { return m.parts == 1; }, false);
     double least;
     if (whole.n > 0) {
-        const int wt = choose(whole, cus, symmetric_tiles, long_axis, least);
-        if (int rc = launch_symmetric<fo::kGram>(wt, whole, h, stream)) return rc;
+        const fo::TileCost t = choose(whole, cus, symmetric_tiles, long_axis, least);
+        if (int rc = launch_symmetric<fo::kGram>(t, whole, h, stream)) return rc;
     }
     if (parted.n == 0) return 0;
-    const int wt = choose(parted, cus, [](const fo::MatrixGroup& m, int wt) { return symmetric_tiles(m, wt) * m.parts; },
-                          [](const fo::MatrixGroup& m) { return long_axis(m) / m.parts; }, least);
-    if (int rc = wt >= kPartialMost ? launch_symmetric<kPartialMost, fo::kPartial>(parted, h, stream) : launch_symmetric<32, fo::kPartial>(parted, h, stream)) return rc;
+    const fo::TileCost t = choose(parted, cus, [](const fo::MatrixGroup& m, int wt) { return symmetric_tiles(m, wt) * m.parts; },
+                                  [](const fo::MatrixGroup& m) { return long_axis(m) / m.parts; }, least);
+    if (int rc = t.wt >= kPartialMost ? launch_symmetric<kPartialMost, 2, fo::kPartial>(parted, h, stream)
+               : t.stages == 4 ? launch_symmetric<32, 4, fo::kPartial>(parted, h, stream) : launch_symmetric<32, 2, fo::kPartial>(parted, h, stream)) return rc;
     const int64_t grid = spread(parted, [](const fo::MatrixGroup& m) { return symmetric_tiles(m, 32) * 16; });
     return launch(fo::gather_kernel, grid, 256, 0, stream, "Newton-Schulz sums", parted, h);
 }
-template <int WT, class Out> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, hipStream_t stream) {
+template <int WT, int STAGES, class Out> int launch_apply(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, hipStream_t stream) {
     const int64_t grid = seat(a, [&](const fo::MatrixGroup& m) {
         return fo::tiles_of(std::min(m.padded_rows, h.row_end) - h.row_begin, std::min(m.padded_cols, h.col_end) - h.col_begin, WT);
     });
-    return launch(fo::apply_kernel<WT, Out>, grid, 256, fo::GemmTile<fo::F16Product, WT>::kLds, stream, "Newton-Schulz step", a, h, last);
+    return launch(fo::apply_kernel<WT, STAGES, Out>, grid, 256, fo::GemmTile<fo::F16Product, WT, STAGES>::kLds, stream, "Newton-Schulz step", a, h, last);
 }
-template <class Out> int launch_apply(int wt, fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, hipStream_t stream) {
-    switch (wt) {
-        case 128: return launch_apply<128, Out>(a, h, last, stream);
-        case 96: return launch_apply<96, Out>(a, h, last, stream);
-        case 64: return launch_apply<64, Out>(a, h, last, stream);
-        default: return launch_apply<32, Out>(a, h, last, stream);
+template <class Out> int launch_apply(const fo::TileCost& t, fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, hipStream_t stream) {
+    switch (t.wt) {
+        case 128: return launch_apply<128, 2, Out>(a, h, last, stream);
+        case 96: return launch_apply<96, 2, Out>(a, h, last, stream);
+        case 64: return launch_apply<64, 2, Out>(a, h, last, stream);
+        default: return t.stages == 4 ? launch_apply<32, 4, Out>(a, h, last, stream) : launch_apply<32, 2, Out>(a, h, last, stream);
     }
 }
 // One matrix may be cut (fo_gemm.h); of several the rounds run on from one to the next.
@@ -1217,11 +1219,11 @@ template <class Out> int launch_apply(fo::Groups& a, const fo::StepArgs& h, cons
     double least;
     if (a.n > 1 || m.count > 1) return launch_apply<Out>(choose(a, cus, apply_tiles, [](const fo::MatrixGroup& m) { return m.side(); }, least), a, h, last, stream);
     const fo::Cut cut = fo::best_cut(kTileCosts, m.padded_rows, m.padded_cols, m.side(), [](int) { return 0.0; }, 0.0, cus);
-    if (!cut.rest) return launch_apply<Out>(cut.wt, a, h, last, stream);
+    if (!cut.rest.wt) return launch_apply<Out>(cut.tile, a, h, last, stream);
     fo::StepArgs first = h, rest = h;
-    if (cut.columns) first.col_end = rest.col_begin = cut.lines * 2 * cut.wt;
-    else first.row_end = rest.row_begin = cut.lines * 2 * cut.wt;
-    if (int rc = launch_apply<Out>(cut.wt, a, first, last, stream)) return rc;
+    if (cut.columns) first.col_end = rest.col_begin = cut.lines * 2 * cut.tile.wt;
+    else first.row_end = rest.row_begin = cut.lines * 2 * cut.tile.wt;
+    if (int rc = launch_apply<Out>(cut.tile, a, first, last, stream)) return rc;
     return launch_apply<Out>(cut.rest, a, rest, last, stream);
 }
 int launch_update(fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, int dtype, int ecc_bytes, int cus, hipStream_t stream) {

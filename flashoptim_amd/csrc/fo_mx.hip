@@ -100,12 +100,19 @@ struct QuantizeArgs {
 // A 128 x 128 piece per workgroup: read once, all of it asked for before any of it is used; the row form out of registers (a
 // group is four lanes), the column form through LDS (a thread takes 32 rows of a column, two neighbouring columns one after the
 // other; four neighbouring threads write 64 adjacent bytes).  Bound by memory: 2 bytes in, 17/32 out per value and form; 14336 x 4096
-// bf16 both ways in 47 us, 3.8 TB/s.
+// bf16 both ways in 39 us, 4.6 TB/s, one way in 30 to 33.
+// The piece in LDS: rows an odd number of dwords apart, the lower half shifted so that the four groups of 32 rows that a wavefront reads
+// at a time lie in different banks.
+template <int B> struct QuantizePlaces {
+    static constexpr int kStride = kBlock * B / 4 + 1, kShift = B == 2 ? 16 : 1, kDwords = kBlock * kStride + kShift;
+    __device__ __forceinline__ static int of(int row) { return row * kStride + (row >> 6) * kShift; }
+};
 template <int DT, bool ROWS, bool COLUMNS> __global__ __launch_bounds__(256) void mx_quantize_kernel(QuantizeArgs args) {
     const bool second = (int)blockIdx.x >= args.first_of_second;
     const QuantizeJob& a = args.job[second];
     const int tile = (int)blockIdx.x - (second ? args.first_of_second : 0);
-    constexpr int B = DTypeInfo<DT>::bytes, kStride = kBlock * B / 4 + 1;   // dwords, odd: rows begin in different banks
+    constexpr int B = DTypeInfo<DT>::bytes;
+    typedef QuantizePlaces<B> Places;
     extern __shared__ u32 lds[];
     const int tile_cols = (a.cols + kBlock - 1) / kBlock;
     const int row0 = tile / tile_cols * kBlock, col0 = tile % tile_cols * kBlock;
@@ -124,7 +131,7 @@ template <int DT, bool ROWS, bool COLUMNS> __global__ __launch_bounds__(256) voi
     if constexpr (COLUMNS) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            u32* out = lds + (k * 16 + line) * kStride + piece * 2 * B;
+            u32* out = lds + Places::of(k * 16 + line) + piece * 2 * B;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (B == 2) out[i] = p[k][i].v; else { out[2 * i] = as_u32(p[k][i].a); out[2 * i + 1] = as_u32(p[k][i].b); }
@@ -151,18 +158,27 @@ template <int DT, bool ROWS, bool COLUMNS> __global__ __launch_bounds__(256) voi
         __syncthreads();
         const int64_t column_bytes = (int64_t)((a.rows + kBlock - 1) / kBlock) * (kBlock / 2);
         const int group = threadIdx.x & 3, pair = threadIdx.x >> 2;
+        const u32* in = lds + Places::of(group * 32) + pair * (B / 2);
+        u32 raw[32];   // both columns of a 16-bit type, the first of fp32
+#pragma unroll
+        for (int i = 0; i < 32; ++i) raw[i] = in[i * Places::kStride];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             Pair<DT> q[16];
-            const u32* in = lds + group * 32 * kStride + (B == 2 ? pair : pair * 2 + half);
             u32 m = 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const u32 x = in[2 * i * kStride], y = in[(2 * i + 1) * kStride];
+                const u32 x = raw[2 * i], y = raw[2 * i + 1];
                 if constexpr (B == 2) q[i].v = half ? __builtin_amdgcn_perm(y, x, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
                 else { q[i].a = as_f32(x); q[i].b = as_f32(y); }
                 const u32 e = q[i].magnitude();
                 m = m > e ? m : e;
+            }
+            if constexpr (B == 4) {
+                if (half == 0) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) raw[i] = in[i * Places::kStride + 1];
+                }
             }
             const u32 byte = scale_byte(m);
             u32x4 w = {0, 0, 0, 0};
@@ -234,9 +250,9 @@ struct ProductOut {
 
 // Bound by the matrix cores: 4096 x 4096 over 32768 values in 231 us, 4750 TFLOP/s; over 4096 values a round of 256 x 256 tiles takes 40 us,
 // a quarter of it the start and the writing of the result.
-template <int WT> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void mx_product_kernel(ProductArgs args) {
+template <int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void mx_product_kernel(ProductArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    typedef GemmTile<Mx4Product, WT> Tile;
+    typedef GemmTile<Mx4Product, WT, STAGES> Tile;
     const int seat = (int)(blockIdx.x >> 3);
     const bool second = seat >= args.seats_of_first;
     const ProductJob& p = args.job[second];
@@ -445,7 +461,7 @@ int64_t form_codes(int64_t rows, int64_t cols) { return rows * blocks_of(cols) *
 int64_t form_bytes(int64_t rows, int64_t cols) { return (rows * blocks_of(cols) * 68 + 255) / 256 * 256; }
 
 template <int DT> int launch_quantize(const fo::QuantizeJob* jobs, int n, void* stream) {
-    constexpr int kLds = fo::kBlock * (fo::kBlock * fo::DTypeInfo<DT>::bytes / 4 + 1) * 4;
+    constexpr int kLds = fo::QuantizePlaces<fo::DTypeInfo<DT>::bytes>::kDwords * 4;
     const char* what = "fo_mxfp4_quantize";
     fo::QuantizeArgs a{};
     int64_t grid = 0;
@@ -494,11 +510,12 @@ int launch_coded_tokens(const fo::TokensArgs& p, void* stream) {
 // Times of 4096 x 4096 products (3840 x 3840 for 192 x 192 tiles) over 1024 to 16384 values: a 256 x 256 tile takes 40 us over 4096 and
 // 130 over 16384, two 128 x 128 tiles on a compute unit 26 and 90 (alone 18 and 62), five 64 x 64 21 and 75 (two of them 13 and 44).
 constexpr fo::TileCost kTileCosts[] = {
-    {128, 1, 11.5, 0.0073, 11.5, 0.0073}, {96, 1, 8.0, 0.0046, 8.0, 0.0046}, {64, 2, 3.5, 0.0036, 5.0, 0.0052}, {32, 5, 2.0, 0.0022, 5.0, 0.0043}};
+    {128, 2, 1, 11.5, 0.0073, 11.5, 0.0073}, {96, 2, 1, 8.0, 0.0046, 8.0, 0.0046}, {64, 2, 2, 3.5, 0.0036, 5.0, 0.0052},
+    {32, 2, 5, 2.0, 0.0022, 5.0, 0.0043}, {32, 4, 2, 2.0, 0.0012, 2.2, 0.0024}};
 
 int64_t tiles(const fo::ProductJob& p, int wt) { return fo::tiles_of(p.rows, p.cols, wt); }
 
-template <int WT> int launch_products(const fo::ProductJob* jobs, int n, void* stream) {
+template <int WT, int STAGES> int launch_products(const fo::ProductJob* jobs, int n, void* stream) {
     fo::ProductArgs a{};
     int64_t seats = 0;
     for (int i = 0; i < n; ++i) {
@@ -508,15 +525,15 @@ template <int WT> int launch_products(const fo::ProductJob* jobs, int n, void* s
         if (seats > kMostWorkgroups) return fail(FO_ERR_UNSUPPORTED, "fo_mxfp4_product: too large a result for one launch");
     }
     if (n == 1) a.seats_of_first = (int)seats;
-    return launch(fo::mx_product_kernel<WT>, 8 * seats, 256, fo::GemmTile<fo::Mx4Product, WT>::kLds, stream, "fo_mxfp4_product", a);
+    return launch(fo::mx_product_kernel<WT, STAGES>, 8 * seats, 256, fo::GemmTile<fo::Mx4Product, WT, STAGES>::kLds, stream, "fo_mxfp4_product", a);
 }
 
-int launch_products(int wt, const fo::ProductJob* jobs, int n, void* stream) {
-    switch (wt) {
-        case 128: return launch_products<128>(jobs, n, stream);
-        case 96: return launch_products<96>(jobs, n, stream);
-        case 64: return launch_products<64>(jobs, n, stream);
-        default: return launch_products<32>(jobs, n, stream);
+int launch_products(const fo::TileCost& t, const fo::ProductJob* jobs, int n, void* stream) {
+    switch (t.wt) {
+        case 128: return launch_products<128, 2>(jobs, n, stream);
+        case 96: return launch_products<96, 2>(jobs, n, stream);
+        case 64: return launch_products<64, 2>(jobs, n, stream);
+        default: return t.stages == 4 ? launch_products<32, 4>(jobs, n, stream) : launch_products<32, 2>(jobs, n, stream);
     }
 }
 // The first `at` rows (columns) of a product, and the others.  Codes of rows are multiples of 64 bytes, so all stays aligned.
@@ -538,10 +555,10 @@ int launch_products(fo::ProductJob* jobs, int n, void* stream) {
     const fo::ProductJob last = jobs[n - 1];
     const fo::Cut cut = fo::best_cut(kTileCosts, last.rows, last.cols, (double)last.blocks * fo::kBlock,
                                      [&](int wt) { return n == 2 ? (double)tiles(jobs[0], wt) : 0.0; }, (double)jobs[0].blocks * fo::kBlock, cus);
-    if (!cut.rest) return launch_products(cut.wt, jobs, n, stream);
+    if (!cut.rest.wt) return launch_products(cut.tile, jobs, n, stream);
     fo::ProductJob rest;
-    divide(last, cut.columns, cut.lines * 2 * cut.wt, jobs[n - 1], rest);
-    if (int rc = launch_products(cut.wt, jobs, n, stream)) return rc;
+    divide(last, cut.columns, cut.lines * 2 * cut.tile.wt, jobs[n - 1], rest);
+    if (int rc = launch_products(cut.tile, jobs, n, stream)) return rc;
     return launch_products(cut.rest, &rest, 1, stream);
 }
 
