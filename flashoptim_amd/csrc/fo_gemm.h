@@ -6,7 +6,7 @@
 //
 // Shape.  A workgroup is four wavefronts in a 2x2 arrangement; a wavefront owns a WT x WT piece of the tile (WT = 128, 96,
 // 64 or 32) and keeps it in its accumulators.  The operands pass through LDS in stages of 128 bytes of every row (64 fp16
-// values, 256 codes), two stages in turn (or four, see below).  With WT = 128 the workgroup holds 128 KiB of LDS, a wavefront 256 accumulator
+// values, 256 codes), two stages in turn (or three or four, see below).  With WT = 128 the workgroup holds 128 KiB of LDS, a wavefront 256 accumulator
 // registers and both halves of a stage's operands in registers, and one wavefront runs on each SIMD: every LDS byte read is
 // used for eight instructions, which is what keeps LDS (128 bytes a clock) behind the matrix cores.
 //
@@ -15,13 +15,18 @@
 // one has arrived); phase 2 multiplies the second half while the next stage's first half is read and the loads of the
 // stage after it are issued into the buffer that has become free.  A load has one whole stage of multiplications to arrive; of
 // 64 x 64 tiles, whose stages are short, that covers it where four or five workgroups share a compute unit.  Where one has it alone, four
-// stages in LDS give a load three: 1000 x 1000 through five Newton-Schulz steps takes 154 instead of 190 us.
+// stages in LDS give a load three: 1000 x 1000 through five Newton-Schulz steps takes 154 instead of 190 us.  192 x 192 tiles have room for
+// three: S of 14336 x 4096 takes 233 us, 260 with two.
 //
 // Loads go from memory straight into LDS (16 bytes a lane, no registers).  They are inline asm: the compiler would wait for
 // all of them before every LDS read.  They have no register result, and every wait for them is written out below.
 //
-// LDS layout: rows of 128 bytes, the eight 16-byte pieces of row r stored in the order piece ^ (r & 7), so that the 16 rows
-// that an instruction's operand needs lie in different banks.  The order is applied to the address that a lane loads from.
+// LDS layout: rows of 128 bytes, the eight 16-byte pieces of row r stored in the order piece ^ (r / 2 & 7).  The hardware serves a
+// 16-byte read in four turns over all 64 banks, and what it takes together are not the 16 rows of one piece but eight of one and
+// eight of the next: the order keeps those apart where the two pieces are neighbours, so a lane's group takes piece `group` in one phase
+// and `group` + 4 in the other (bank conflicts of S of 14336 x 4096: 1.1e6 cycles; 22.9e6 with pieces 2 group and 2 group + 1, or with
+// r & 7; 1000 x 1000 in all 144 us against 152).  Scaled operands keep 2 group and 2 group + 1, a lane's two scales are neighbours then.
+// The order is applied to the address that a lane loads from.
 #pragma once
 
 #include "fo_device.h"
@@ -138,7 +143,7 @@ __device__ __forceinline__ const char* uniform(const char* p) {
 }
 
 template <class Product, int WT, int STAGES> struct GemmTile {
-    static constexpr int kStages = STAGES;        // in LDS, 2 or 4
+    static constexpr int kStages = STAGES;        // in LDS, 2 to 4
     static constexpr int kTile = 2 * WT;          // rows and columns of a workgroup's tile
     static constexpr int kFrags = WT / 16;        // 16-row pieces of a wavefront's operands
     static constexpr int kRows = 2 * kTile;       // rows of a stage, A's then B's
@@ -150,6 +155,7 @@ template <class Product, int WT, int STAGES> struct GemmTile {
     // the epilogue moves the tile through LDS in strips of 32 rows of a wavefront, 4 floats of padding per row
     static constexpr int kStripStride = WT + 4;
     static constexpr int kStripBytes = 32 * kStripStride * 4;
+    static_assert(kStages * kBuffer <= 163840 && (kStages - 1) * kLoads <= 63, "what LDS holds, what the counter of loads under way counts to");
     static constexpr int kLds = kStages * kBuffer > 4 * kStripBytes ? kStages * kBuffer : 4 * kStripBytes;
 
     typedef typename Product::Frag Frag;
@@ -163,6 +169,8 @@ template <class Product, int WT, int STAGES> struct GemmTile {
         : smem(lds), smem_address(lds_address(lds)), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), lane(threadIdx.x & 63) {}
 
     // ------------------------------------------------------------------------------------------- staging
+    __device__ __forceinline__ static int buffer_of(int stage) { return (kStages == 3 ? stage % 3 : stage & (kStages - 1)) * kBuffer; }
+    __device__ __forceinline__ static int place_of(int row) { return (row >> 1) & 7; }
     struct Loader {
         unsigned row[kRowLoads];
         unsigned scale[kScaleLoads > 0 ? kScaleLoads : 1];
@@ -176,11 +184,11 @@ template <class Product, int WT, int STAGES> struct GemmTile {
         const int64_t stride = first ? a.stride : b.stride;
         const int at = first ? row0 : col0, left = (first ? a.rows : b.rows) - at;
         l.base = uniform(data + at * stride);
-        const int row = lane >> 3, piece = (lane & 7) ^ (row & 7);
-        l.past_half = piece >= 4 ? kHalfBytes : 0;
+        l.past_half = ((lane & 7) ^ place_of(lane >> 3)) >= 4 ? kHalfBytes : 0;
 #pragma unroll
         for (int i = 0; i < kRowLoads; ++i) {
-            int r = (wave & 1) * (kRowLoads * 8) + i * 8 + row;
+            const int row = i * 8 + (lane >> 3), piece = (lane & 7) ^ place_of(row);   // the other wavefronts' rows are multiples of 16 away
+            int r = (wave & 1) * (kRowLoads * 8) + row;
             r = r < left ? r : left - 1;
             l.row[i] = (unsigned)(r * stride) + piece * 16;
         }
@@ -198,9 +206,10 @@ template <class Product, int WT, int STAGES> struct GemmTile {
     }
     // The i-th load of a stage.  half: the rows end in the middle of the stage, its second half repeats the first.
     __device__ __forceinline__ void load(const Loader& l, int i, int stage, bool half) const {
-        const unsigned buffer = smem_address + (stage & (kStages - 1)) * kBuffer;
+        const unsigned buffer = smem_address + buffer_of(stage);
         if (i < kRowLoads) {
-            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, l.row[i] - (half ? l.past_half : 0), l.base + (int64_t)stage * kStageBytes);
+            const unsigned past = i & 1 ? kHalfBytes - l.past_half : l.past_half;   // eight rows on the halves change places
+            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, l.row[i] - (half ? past : 0), l.base + (int64_t)stage * kStageBytes);
         } else if constexpr (Product::kScaled) {
             const int k = i - kRowLoads;
             load_to_lds4(buffer + kScaleOffset + (wave * kScaleLoads + k) * 256, l.scale[k] - (half ? l.past_half_scale : 0),
@@ -213,21 +222,21 @@ template <class Product, int WT, int STAGES> struct GemmTile {
     struct Scales { int a[Product::kScaled ? kFrags : 1], b[Product::kScaled ? kFrags : 1]; };
 
     // Operand piece f of the wavefront (0..kFrags-1: B's, then A's) for phase `half` of a stage.  Each of the four groups of 16
-    // lanes takes 16-byte piece `group` of eight; the phases of a whole stage take pieces 2 group and 2 group + 1, in any
-    // order the sum is the same and a lane's two scales are neighbours.  short_stage: the stage has four pieces, phase 0 takes them.
+    // lanes takes a 16-byte piece of eight (which ones in which phase: see the layout above; any order gives the same sum).
+    // short_stage: the stage has four pieces, phase 0 takes them.
     __device__ __forceinline__ void read(Operands& to, int f, int stage, int half, bool short_stage) const {
         const bool is_b = f < kFrags;
         const int i = is_b ? f : f - kFrags, group = lane >> 4;
         const int row = (is_b ? kTile + (wave & 1) * WT : (wave >> 1) * WT) + i * 16 + (lane & 15);
-        const int piece = short_stage ? group : 2 * group + half;
-        (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const Frag*>(smem + (stage & (kStages - 1)) * kBuffer + row * kStageBytes + ((piece ^ (row & 7)) * 16));
+        const int piece = short_stage ? group : Product::kScaled ? 2 * group + half : group + 4 * half;
+        (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const Frag*>(smem + buffer_of(stage) + row * kStageBytes + ((piece ^ place_of(row)) * 16));
     }
     // The four scale bytes among which the lane's two are.
     __device__ __forceinline__ void read_scales(Scales& to, int f, int stage, bool short_stage) const {
         const bool is_b = f < kFrags;
         const int i = is_b ? f : f - kFrags, group = lane >> 4;
         const int row = (is_b ? kTile + (wave & 1) * WT : (wave >> 1) * WT) + i * 16 + (lane & 15);
-        (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const int*>(smem + (stage & (kStages - 1)) * kBuffer + kScaleOffset + row * 8 + (short_stage ? 0 : (group >> 1) * 4));
+        (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const int*>(smem + buffer_of(stage) + kScaleOffset + row * 8 + (short_stage ? 0 : (group >> 1) * 4));
     }
     __device__ __forceinline__ void settle(Scales& now, const Scales& raw, bool short_stage) const {
         if constexpr (Product::kScaled) {
@@ -280,9 +289,11 @@ template <class Product, int WT, int STAGES> struct GemmTile {
 
     // Waits for LDS reads and for all loads but those of the last `later` stages (of kStages at most).
     __device__ __forceinline__ static void wait_behind(int later) {
-        if constexpr (kStages > 2) {
+        if constexpr (kStages > 3) {
             if (later >= 3) { wait_loads_and_lds<3 * kLoads>(); return; }
-            if (later == 2) { wait_loads_and_lds<2 * kLoads>(); return; }
+        }
+        if constexpr (kStages > 2) {
+            if (later >= 2) { wait_loads_and_lds<2 * kLoads>(); return; }
         }
         if (later >= 1) wait_loads_and_lds<kLoads>();
         else wait_loads_and_lds<0>();

@@ -390,7 +390,7 @@ struct PartialOut {
     }
 };
 
-// Bound by the matrix cores, with 192 x 192 tiles as much by LDS: S of 14336 x 4096 in 260 us (925 TFLOP/s of the half that is computed), a
+// Bound by the matrix cores, with 192 x 192 tiles as much by LDS: S of 14336 x 4096 in 233 us (1030 TFLOP/s of the half that is computed), a
 // square of 4096 x 4096 in 80 (one round of 253 tiles either way; 256 x 256 tiles would fill 136 of 256 compute units).
 template <int WT, int STAGES, int KIND> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void symmetric_kernel(Groups a, SquareArgs h) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -1106,10 +1106,10 @@ template <class K, class... Args> int launch(K kernel, int64_t grid, int threads
 }
 
 // Which tile a launch takes: the one whose rounds over the compute units take least, by times fitted to steps of 4096 x 14336, 4096 x
-// 4096, 1024 x 4096 and 1000 x 2730 matrices: 131 us for a 256 x 256 tile over 4096 values, 86 for 192 x 192, 75 for two
+// 4096, 1024 x 4096 and 1000 x 2730 matrices: 131 us for a 256 x 256 tile over 4096 values, 80 for 192 x 192, 75 for two
 // 128 x 128, 52 for five 64 x 64 (the smaller ones read more of LDS per multiplication); 43, 33, 24 (21 alone) and 18 (11) over 1024.
 constexpr fo::TileCost kTileCosts[] = {
-    {128, 2, 1, 14.0, 0.0286, 14.0, 0.0286}, {96, 2, 1, 16.0, 0.0170, 16.0, 0.0170}, {64, 2, 2, 9.5, 0.0115, 8.0, 0.0165},
+    {128, 2, 1, 14.0, 0.0286, 14.0, 0.0286}, {96, 3, 1, 19.0, 0.0150, 19.0, 0.0150}, {64, 2, 2, 9.5, 0.0115, 8.0, 0.0165},
     {32, 2, 5, 4.2, 0.0063, 7.0, 0.0110}, {32, 4, 2, 4.2, 0.0036, 7.0, 0.0058}};
 
 // tiles(group, wt) of a matrix, length(group) contracted.
@@ -1146,7 +1146,7 @@ template <int WT, int STAGES, int KIND> int launch_symmetric(fo::Groups& a, cons
 template <int KIND> int launch_symmetric(const fo::TileCost& t, fo::Groups& a, const fo::SquareArgs& h, hipStream_t stream) {
     switch (t.wt) {
         case 128: return launch_symmetric<128, 2, KIND>(a, h, stream);
-        case 96: return launch_symmetric<96, 2, KIND>(a, h, stream);
+        case 96: return launch_symmetric<96, 3, KIND>(a, h, stream);
         case 64: return launch_symmetric<64, 2, KIND>(a, h, stream);
         default: return t.stages == 4 ? launch_symmetric<32, 4, KIND>(a, h, stream) : launch_symmetric<32, 2, KIND>(a, h, stream);
     }
@@ -1210,7 +1210,7 @@ template <int WT, int STAGES, class Out> int launch_apply(fo::Groups& a, const f
 template <class Out> int launch_apply(const fo::TileCost& t, fo::Groups& a, const fo::StepArgs& h, const fo::LastArgs& last, hipStream_t stream) {
     switch (t.wt) {
         case 128: return launch_apply<128, 2, Out>(a, h, last, stream);
-        case 96: return launch_apply<96, 2, Out>(a, h, last, stream);
+        case 96: return launch_apply<96, 3, Out>(a, h, last, stream);
         case 64: return launch_apply<64, 2, Out>(a, h, last, stream);
         default: return t.stages == 4 ? launch_apply<32, 4, Out>(a, h, last, stream) : launch_apply<32, 2, Out>(a, h, last, stream);
     }

@@ -510,7 +510,7 @@ int launch_coded_tokens(const fo::TokensArgs& p, void* stream) {
 // Times of 4096 x 4096 products (3840 x 3840 for 192 x 192 tiles) over 1024 to 16384 values: a 256 x 256 tile takes 40 us over 4096 and
 // 130 over 16384, two 128 x 128 tiles on a compute unit 26 and 90 (alone 18 and 62), five 64 x 64 21 and 75 (two of them 13 and 44).
 constexpr fo::TileCost kTileCosts[] = {
-    {128, 2, 1, 11.5, 0.0073, 11.5, 0.0073}, {96, 2, 1, 8.0, 0.0046, 8.0, 0.0046}, {64, 2, 2, 3.5, 0.0036, 5.0, 0.0052},
+    {128, 2, 1, 11.5, 0.0073, 11.5, 0.0073}, {96, 3, 1, 8.0, 0.0046, 8.0, 0.0046}, {64, 2, 2, 3.5, 0.0036, 5.0, 0.0052},
     {32, 2, 5, 2.0, 0.0022, 5.0, 0.0043}, {32, 4, 2, 2.0, 0.0012, 2.2, 0.0024}};
 
 int64_t tiles(const fo::ProductJob& p, int wt) { return fo::tiles_of(p.rows, p.cols, wt); }
@@ -531,7 +531,7 @@ template <int WT, int STAGES> int launch_products(const fo::ProductJob* jobs, in
 int launch_products(const fo::TileCost& t, const fo::ProductJob* jobs, int n, void* stream) {
     switch (t.wt) {
         case 128: return launch_products<128, 2>(jobs, n, stream);
-        case 96: return launch_products<96, 2>(jobs, n, stream);
+        case 96: return launch_products<96, 3>(jobs, n, stream);
         case 64: return launch_products<64, 2>(jobs, n, stream);
         default: return t.stages == 4 ? launch_products<32, 4>(jobs, n, stream) : launch_products<32, 2>(jobs, n, stream);
     }
