@@ -142,10 +142,10 @@ def _tokens(x: torch.Tensor, weight: MXFP4Tensor, dtype: torch.dtype) -> torch.T
     size, workspace = 0, None
     if blocks > _RAW_BLOCKS:
         size = blocks * 68
-        workspace = torch.empty(size, dtype=torch.uint8, device=x.device).data_ptr()
+        workspace = torch.empty(size, dtype=torch.uint8, device=x.device)  # held until the launches are in the stream
     with _native.device_guard(x.device):
         rc = _native.lib().fo_mxfp4_tokens(x.data_ptr(), DTYPE_CODE[x.dtype], m, x.stride(0), weight.codes.data_ptr(), weight.scales.data_ptr(),
-                                           n, k, out.data_ptr(), DTYPE_CODE[dtype], workspace, size, _native.current_stream_ptr(x.device))
+                                           n, k, out.data_ptr(), DTYPE_CODE[dtype], _native.ptr(workspace), size, _native.current_stream_ptr(x.device))
     if rc:
         _native.check(rc, "fo_mxfp4_tokens")
     return out
