@@ -313,8 +313,12 @@ __device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
     return h;
 }
 
-// Square matrices without their diagonals: all are symmetric, so each tile off the diagonal is written twice.
+// Square matrices without their diagonals: all are symmetric, so each tile off the diagonal is written twice.  Of a tile on the diagonal
+// both halves are computed.  Those of S and of its polynomial agree to the bit; those of U V do only as far as U and V commute, and which entries
+// lie in such tiles goes by the tile's size: there too what is below the diagonal is copied from above it, so that no result depends on the
+// tile, which is chosen by all that shares the launch.
 template <int KIND> struct SymmetricOut {
+    static constexpr bool kCopied = KIND == kMixed;   // below the diagonal, in tiles on it
     static constexpr bool kColumns = true;
     const _Float16 *u, *v;
     const float *u_diagonal, *v_diagonal;
@@ -366,12 +370,26 @@ template <int KIND> struct SymmetricOut {
                 }
             }
         }
-        *reinterpret_cast<f16x8*>(out + (int64_t)i * side + j) = half8(x);
+        _Float16* to = out + (int64_t)i * side + j;
+        if (kCopied && !mirror && j < i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (j + e >= i) to[e] = (_Float16)x[e];
+        } else {
+            *reinterpret_cast<f16x8*>(to) = half8(x);
+        }
     }
-    __device__ __forceinline__ bool columns() const { return mirror; }
+    __device__ __forceinline__ bool columns() const { return kCopied || mirror; }
     __device__ __forceinline__ void column(int i, int j, const float (&x)[8]) const {
         if (i >= side || j >= side) return;
-        *reinterpret_cast<f16x8*>(out + (int64_t)j * side + i) = half8(x);
+        _Float16* to = out + (int64_t)j * side + i;
+        if (kCopied && !mirror && j < i + 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i + e < j) to[e] = (_Float16)x[e];
+        } else {
+            *reinterpret_cast<f16x8*>(to) = half8(x);
+        }
     }
 };
 
