@@ -152,6 +152,20 @@ __global__ __launch_bounds__(256) void norm_kernel(Groups a, float eps) {
     if (threadIdx.x == 0) *m.factor(k) = (float)((double)m.unit / (sqrt(total) + (double)eps));
 }
 
+// fp16 of a value that has been rounded to fp32 before.  The empty statement keeps the two roundings apart: the compiler joins a product or a sum
+// and its conversion into one instruction, which rounds once, for some uses of a value and in some kernels only.  In the polynomial's 256 x 256
+// tiles an entry and its mirror image then differed by a unit of fp16 at one place in 1e5, and both from what other tiles make.
+__device__ __forceinline__ _Float16 to_half(float x) {
+    asm("" : "+v"(x));
+    return (_Float16)x;
+}
+__device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
+    f16x8 h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = to_half(v[e]);
+    return h;
+}
+
 // 64 x 64 pieces of G, normalised, as hi and lo in G's orientation and hi transposed (through LDS), zeros in the padding.  Bound by
 // memory, 6 bytes written per element: 14336 x 4096 bf16 in 86 us, 5.5 TB/s.
 template <int DT> __global__ __launch_bounds__(256) void split_kernel(Groups a, MatrixSource source) {
@@ -176,7 +190,7 @@ template <int DT> __global__ __launch_bounds__(256) void split_kernel(Groups a, 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             v[e] *= factor;
-            hi[e] = (_Float16)v[e];
+            hi[e] = to_half(v[e]);
             v[e] -= (float)hi[e];
             lds[r][piece + e] = hi[e];
         }
@@ -306,12 +320,6 @@ struct StepArgs {
     int row_begin = 0, col_begin = 0, row_end = INT32_MAX, col_end = INT32_MAX;
 };
 
-__device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
-    f16x8 h;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = (_Float16)v[e];
-    return h;
-}
 
 // Square matrices without their diagonals: all are symmetric, so each tile off the diagonal is written twice.  Of a tile on the diagonal
 // both halves are computed.  Those of S and of its polynomial agree to the bit; those of U V do only as far as U and V commute, and which entries
@@ -374,7 +382,7 @@ template <int KIND> struct SymmetricOut {
         if (kCopied && !mirror && j < i) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (j + e >= i) to[e] = (_Float16)x[e];
+                if (j + e >= i) to[e] = to_half(x[e]);
         } else {
             *reinterpret_cast<f16x8*>(to) = half8(x);
         }
@@ -386,7 +394,7 @@ template <int KIND> struct SymmetricOut {
         if (kCopied && !mirror && j < i + 8) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (i + e < j) to[e] = (_Float16)x[e];
+                if (i + e < j) to[e] = to_half(x[e]);
         } else {
             *reinterpret_cast<f16x8*>(to) = half8(x);
         }
@@ -463,8 +471,7 @@ __global__ __launch_bounds__(256) void gather_kernel(Groups a, SquareArgs h) {
     if (h.first) x *= 1.0f / (m.unit * m.unit);
     if (i == j) { m.diagonal(k, h.out)[i] = x; x = 0.0f; }
     _Float16* s = m.square(k, h.out);
-    s[(int64_t)i * side + j] = (_Float16)x;
-    s[(int64_t)j * side + i] = (_Float16)x;
+    s[(int64_t)i * side + j] = s[(int64_t)j * side + i] = to_half(x);
 }
 
 // X <- a X + B X, common to the steps: x = (acc + (a + d) (hi + lo)) / unit, d the diagonal entry of B.
@@ -694,7 +701,7 @@ __device__ __forceinline__ f16x8 read_turned(char* lds, int at, int pitch) {
 }
 __device__ __forceinline__ void put_half(char* lds, int at, _Float16 v) { *reinterpret_cast<_Float16*>(lds + at) = v; }
 __device__ __forceinline__ void put_halves(char* lds, int at, f16x4 v) { *reinterpret_cast<f16x4*>(lds + at) = v; }
-__device__ __forceinline__ f16x4 halves(f32x4 v) { return f16x4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w}; }
+__device__ __forceinline__ f16x4 halves(f32x4 v) { return f16x4{to_half(v.x), to_half(v.y), to_half(v.z), to_half(v.w)}; }
 
 // What becomes of eight values of the result; what that needs from memory is loaded before the result is there.
 struct SmallResult {
