@@ -280,9 +280,8 @@ template <int DT, bool QUANT> __global__ __launch_bounds__(256) void momentum_ke
     const int k = (int)(local / m.chunks), chunk = (int)(local % m.chunks);
     const fo_tensor_desc d = h.matrices[m.first + k];
     if constexpr (QUANT) {
-        // (q / 127) / (2 - |q / 127|) with q times 1/127 for the first quotient: a value in the last place of the step kernels'
-        // table, without reading one.  About one code in 1e5 comes out one step apart for it.
-        const float y = (float)(int8_t)threadIdx.x * (1.0f / 127.0f);
+        // what a code stands for, as the step kernels' table and the dequantiser have it: both quotients correctly rounded
+        const float y = (float)(int8_t)threadIdx.x / 127.0f;
         lut[threadIdx.x] = y / (2.0f - fabsf(y));
         __syncthreads();
     }
