@@ -9,6 +9,7 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native, kernels
 from ._native import DTYPE_CODE
@@ -274,6 +275,10 @@ class _FrozenLinear(torch.autograd.Function):
         return mxfp4_matmul(dy, columns, ctx.dtype), None, None, None
 
 
+def _has_tangent(x: torch.Tensor) -> bool:
+    return forward_ad.unpack_dual(x).tangent is not None
+
+
 def mxfp4_linear(x: torch.Tensor, weight: Union[torch.Tensor, MXFP4Tensor]) -> torch.Tensor:
     """``x @ weight.T`` in MXFP4, with gradients.
 
@@ -289,16 +294,21 @@ def mxfp4_linear(x: torch.Tensor, weight: Union[torch.Tensor, MXFP4Tensor]) -> t
         y = Q(x) Q(w)',    dx = Q(dy) Q(w')',    dw = Q(dy') Q(x')'
 
     with Q along rows; the quantisation itself counts as the identity in the backward pass.
+
+    Raises:
+        NotImplementedError: no ROCm device, or an operand with a forward-mode tangent (there is no such derivative here).
     """
     inner = weight.shape[-1]
     if (type(weight) is MXFP4Tensor and type(x) is torch.Tensor and x.dim() == 2 and x.shape[1] == inner and x.is_cuda
             and 0 < x.shape[0] <= _MOST_TOKENS and x.stride(1) == 1 and inner and weight.shape[0] and x.dtype in DTYPE_CODE
-            and x.device == weight.codes.device and not x.is_neg() and not (x.requires_grad and torch.is_grad_enabled())):
+            and x.device == weight.codes.device and not x.is_neg() and not (x.requires_grad and torch.is_grad_enabled()) and not _has_tangent(x)):
         return _tokens(x, weight, x.dtype)  # the call of a decoding step, without the ways round
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] != inner:
         raise ValueError(f"mxfp4_linear: input of shape {tuple(x.shape)} does not fit a weight of shape {tuple(weight.shape)}")
     if weight.device != x.device:
         raise ValueError(f"weight is on {weight.device}, expected {x.device}.")
+    if _has_tangent(x) or (isinstance(weight, torch.Tensor) and _has_tangent(weight)):
+        raise NotImplementedError("mxfp4_linear has no forward-mode derivative")
     tokens = x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), inner)
     if isinstance(weight, MXFP4Tensor):
         if torch.is_grad_enabled() and x.requires_grad:

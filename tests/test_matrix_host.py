@@ -5,6 +5,7 @@ import weakref
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import flashoptim_amd as fo
 from flashoptim_amd import mxfp4
@@ -57,3 +58,24 @@ def test_memory_of_the_product_for_few_rows_is_held_over_the_call(monkeypatch, t
     needs = tokens * inner // 128 > mxfp4._RAW_BLOCKS
     assert name == "fo_mxfp4_tokens" and alive == [True] * (2 if needs else 1)
     assert (args[-3] is not None) == needs and args[-2] == (tokens * inner // 128 * 68 if needs else 0)
+
+
+def _held(rows, cols):
+    return fo.MXFP4Tensor(torch.zeros((rows, cols // 2), dtype=torch.uint8), torch.zeros((rows, cols // 32), dtype=torch.uint8), (rows, cols))
+
+
+@pytest.mark.parametrize("shape", [(3, 128), (100, 128), (2, 3, 128)])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused_and_not_answered_with_nothing(monkeypatch, shape, grad):
+    """A tangent is neither carried on nor lost without a word, whatever the weight and also where no gradients are recorded."""
+    library, _ = _without_device(monkeypatch)
+    x, weight = torch.zeros(shape), torch.zeros(5, 128)
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        dual = fwd.make_dual(x, torch.ones(shape))
+        for call in (lambda: fo.mxfp4_linear(dual, _held(5, 128)), lambda: fo.mxfp4_linear(dual, weight),
+                     lambda: fo.mxfp4_linear(x, fwd.make_dual(weight, torch.ones(5, 128)))):
+            with pytest.raises(NotImplementedError, match="forward"):
+                call()
+        assert not library.seen
+        fo.mxfp4_linear(x, _held(5, 128))    # without a tangent a level means nothing
+        assert library.seen
