@@ -194,6 +194,32 @@ def _adjacent(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
+def _linear(x: torch.Tensor, weight: torch.Tensor, need_dx: bool, need_dw: bool) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The layer's output, and the column forms that its gradients need: of x for dw, then of the weight for dx."""
+    x, weight = _check_matrix(x, "mxfp4_linear"), _check_matrix(weight, "mxfp4_linear")
+    (tokens, inner), outer = x.shape, weight.shape[0]
+    if not (tokens and inner and outer):
+        return torch.zeros((tokens, outer), dtype=x.dtype, device=x.device), None
+    x, weight = _adjacent(x), _adjacent(weight)
+    device = x.device
+    x_bytes, w_bytes = _form_bytes(inner, tokens) if need_dw else 0, _form_bytes(inner, outer) if need_dx else 0
+    kept, at = None, 0
+    if need_dx or need_dw:
+        kept = torch.empty(x_bytes + w_bytes, dtype=torch.uint8, device=device)
+        at = kept.data_ptr()
+    used = _form_bytes(tokens, inner) + _form_bytes(outer, inner)  # the row forms
+    workspace = torch.empty(used, dtype=torch.uint8, device=device)
+    y = torch.empty((tokens, outer), dtype=x.dtype, device=device)
+    with _native.device_guard(device):
+        rc = _native.lib().fo_mxfp4_linear_forward(
+            x.data_ptr(), DTYPE_CODE[x.dtype], tokens, x.stride(0), weight.data_ptr(), DTYPE_CODE[weight.dtype], outer, weight.stride(0),
+            inner, at if need_dw else None, at + x_bytes if need_dx else None, y.data_ptr(), workspace.data_ptr(), used,
+            _native.current_stream_ptr(device))
+    if rc:
+        _native.check(rc, "fo_mxfp4_linear_forward")
+    return y, kept
+
+
 class _Linear(torch.autograd.Function):
     """x (tokens, in) and weight (out, in) to x weight', every product on MXFP4 forms of its operands along the contracted axis.
 
@@ -203,29 +229,8 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight):
-        need_dx, need_dw = ctx.needs_input_grad
         ctx.dtypes, ctx.shapes = (x.dtype, weight.dtype), (x.shape, weight.shape)
-        x, weight = _check_matrix(x, "mxfp4_linear"), _check_matrix(weight, "mxfp4_linear")
-        (tokens, inner), outer = x.shape, weight.shape[0]
-        if not (tokens and inner and outer):
-            ctx.save_for_backward()
-            return torch.zeros((tokens, outer), dtype=x.dtype, device=x.device)
-        x, weight = _adjacent(x), _adjacent(weight)
-        device = x.device
-        # the column forms of x and of the weight, kept; the row forms, used here
-        x_bytes, w_bytes = _form_bytes(inner, tokens) if need_dw else 0, _form_bytes(inner, outer) if need_dx else 0
-        kept = torch.empty(x_bytes + w_bytes, dtype=torch.uint8, device=device)
-        used = _form_bytes(tokens, inner) + _form_bytes(outer, inner)
-        workspace = torch.empty(used, dtype=torch.uint8, device=device)
-        y = torch.empty((tokens, outer), dtype=x.dtype, device=device)
-        at = kept.data_ptr()
-        with _native.device_guard(device):
-            rc = _native.lib().fo_mxfp4_linear_forward(
-                x.data_ptr(), DTYPE_CODE[x.dtype], tokens, x.stride(0), weight.data_ptr(), DTYPE_CODE[weight.dtype], outer, weight.stride(0),
-                inner, at if need_dw else None, at + x_bytes if need_dx else None, y.data_ptr(), workspace.data_ptr(), used,
-                _native.current_stream_ptr(device))
-        if rc:
-            _native.check(rc, "fo_mxfp4_linear_forward")
+        y, kept = _linear(x, weight, *ctx.needs_input_grad)
         ctx.save_for_backward(kept)
         return y
 
@@ -318,7 +323,10 @@ def mxfp4_linear(x: torch.Tensor, weight: Union[torch.Tensor, MXFP4Tensor]) -> t
     else:
         if weight.dim() != 2:
             raise ValueError(f"mxfp4_linear expects a matrix as weight, got shape {tuple(weight.shape)}.")
-        y = _Linear.apply(tokens, weight)
+        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+            y = _Linear.apply(tokens, weight)
+        else:
+            y, _ = _linear(tokens, weight, False, False)
         if x.dim() == 2:
             return y
     return y.reshape(*x.shape[:-1], weight.shape[0])

@@ -79,3 +79,33 @@ def test_forward_mode_is_refused_and_not_answered_with_nothing(monkeypatch, shap
         assert not library.seen
         fo.mxfp4_linear(x, _held(5, 128))    # without a tangent a level means nothing
         assert library.seen
+
+
+@pytest.mark.parametrize("way", ["no_grad", "inference", "detached", "frozen"])
+def test_calls_without_gradients_ask_for_no_column_forms(monkeypatch, way):
+    """What the backward pass would need is neither allocated nor made where none can follow, whatever the operands say of themselves."""
+    library, made = _without_device(monkeypatch)
+    layer = fo.MXFP4Linear(128, 256, bias=False)
+    x = torch.zeros(100, 128)
+    if way == "frozen":
+        layer.weight.requires_grad_(False)
+    with {"no_grad": torch.no_grad, "inference": torch.inference_mode}.get(way, contextlib.nullcontext)():
+        if way in ("no_grad", "inference"):
+            y = layer(x.requires_grad_())
+        else:
+            y = fo.mxfp4_linear(x, layer.weight.detach() if way == "detached" else layer.weight)
+    (name, _, args), = library.seen
+    assert name == "fo_mxfp4_linear_forward" and not y.requires_grad
+    assert args[9:11] == (None, None)
+    assert len(made) == 2    # the output and the workspace
+
+
+def test_calls_with_gradients_ask_for_the_forms_that_they_need(monkeypatch):
+    library, _ = _without_device(monkeypatch)
+    for dx in (True, False):
+        for dw in (True, False):
+            if dx or dw:
+                y = fo.mxfp4_linear(torch.zeros(100, 128, requires_grad=dx), torch.zeros(256, 128, requires_grad=dw))
+                name, _, args = library.seen[-1]
+                assert name == "fo_mxfp4_linear_forward" and y.requires_grad
+                assert (args[9] is not None, args[10] is not None) == (dw, dx)
