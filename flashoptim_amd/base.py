@@ -16,7 +16,7 @@ import math
 import os
 import warnings
 from collections.abc import Iterable
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Any, Callable, Literal, Optional, cast
 
 import torch
@@ -86,8 +86,9 @@ class _GroupCache:
     buckets: list
     idle: list                        # non-empty parameters that had no gradient (or are frozen) when the cache was built
     state_len: int                    # len(optimizer.state) then: a cleared or pruned state dict invalidates the cache
-    # check_numerics: log2 of the coarsest weight resolution over the group's parameters (None: nothing to check)
-    numerics_needed: Optional[float] = None
+    # check_numerics: log2 of the coarsest weight resolution over the group's parameters, by the size of their smallest steps
+    # relative to the learning rate (one size for all but Muon's matrices)
+    numerics_needed: dict[float, float] = field(default_factory=dict)
 
 
 class FlashOptimizer(torch.optim.Optimizer, abc.ABC):
@@ -227,6 +228,11 @@ class FlashOptimizer(torch.optim.Optimizer, abc.ABC):
     def _min_step_size_relative_to_lr(self) -> float:
         return 1.0  # sign-based updates (Lion) move every weight by exactly lr
 
+    def _min_step_of(self, p: torch.Tensor, group: dict[str, Any]) -> float:
+        """The same for one parameter, where it depends on that."""
+        del p, group
+        return self._min_step_size_relative_to_lr()
+
     def _order_bucket(self, items: list) -> list:
         """The (parameter, tensors) pairs of one launch in the order its tables hold them."""
         return items
@@ -276,14 +282,14 @@ class FlashOptimizer(torch.optim.Optimizer, abc.ABC):
             return None
         return _log2_min_expressible_step_size(dtype=p.dtype, maxabs=maxabs, master_bytewidth=master_bytewidth)
 
-    def _check_param_numerics(self, p: torch.Tensor, lr: float, master_bytewidth: int) -> None:
+    def _check_param_numerics(self, p: torch.Tensor, lr: float, master_bytewidth: int, min_step: float) -> None:
         if lr == 0.0:
             return
         maxabs = self._transient_state.get(id(p), {}).get("maxabs", 0)
         if maxabs <= 0 or not math.isfinite(maxabs):
             return
         needed = _log2_min_expressible_step_size(dtype=p.dtype, maxabs=maxabs, master_bytewidth=master_bytewidth)
-        guaranteed = math.log2(lr * self._min_step_size_relative_to_lr())
+        guaranteed = math.log2(lr * min_step)
         if needed > guaranteed:
             bits = max(_DTYPE_WIDTHS[p.dtype], master_bytewidth) * 8
             raise NumericsError(
@@ -367,7 +373,7 @@ class FlashOptimizer(torch.optim.Optimizer, abc.ABC):
         if not p.requires_grad or p.grad is None:
             return None
         if self._check_numerics:
-            self._check_param_numerics(p, lr=group["lr"], master_bytewidth=group["master_bytewidth"])
+            self._check_param_numerics(p, lr=group["lr"], master_bytewidth=group["master_bytewidth"], min_step=self._min_step_of(p, group))
         p_local = self._get_local_tensor(p)
         grad_local = self._get_local_tensor(p.grad)
         if not p_local.is_cuda:
@@ -468,10 +474,13 @@ class FlashOptimizer(torch.optim.Optimizer, abc.ABC):
                                    plan, step_pool, scalars.get("step"), step_views,
                                    None if step_views is None else list(map(id, step_views))))
         if cacheable and buckets:
-            needed = None
+            needed: dict[float, float] = {}
             if self._check_numerics:
-                each = [self._numerics_needed(p, group["master_bytewidth"]) for b in buckets for p in b.params]
-                needed = max((x for x in each if x is not None), default=None)
+                for p in (p for b in buckets for p in b.params):
+                    bits = self._numerics_needed(p, group["master_bytewidth"])
+                    if bits is not None:
+                        step = self._min_step_of(p, group)
+                        needed[step] = max(bits, needed.get(step, bits))
             self._group_cache[index] = _GroupCache(self._plan_epoch, list(group["params"]), list(map(id, group["params"])),
                                                    self._plan_signature(group), buckets, idle, len(self.state), needed)
         else:
@@ -549,9 +558,9 @@ class FlashOptimizer(torch.optim.Optimizer, abc.ABC):
     def _cached_numerics_ok(self, cache: _GroupCache, group: dict[str, Any]) -> bool:
         """check_numerics for a cached group: the weights' resolution is cached, only lr can have moved.  False
         sends the group through the full path, which raises the NumericsError naming the parameter."""
-        if not self._check_numerics or cache.numerics_needed is None or group["lr"] == 0.0:
+        if not self._check_numerics or group["lr"] == 0.0:
             return True
-        return cache.numerics_needed <= math.log2(group["lr"] * self._min_step_size_relative_to_lr())
+        return all(bits <= math.log2(group["lr"] * step) for step, bits in cache.numerics_needed.items())
 
     @torch.no_grad()
     def step(self, closure: Optional[Callable] = None) -> Optional[torch.Tensor]:

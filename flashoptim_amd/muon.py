@@ -271,11 +271,13 @@ class FlashMuon(FlashOptimizer):
                     steps=hparams["ns_steps"], coefficients=tuple(hparams["ns_coefficients"]), eps=hparams["eps"],
                     adjust_lr_fn=hparams["adjust_lr_fn"])
 
-    def _min_step_size_relative_to_lr(self) -> float:
+    def _min_step_of(self, p: torch.Tensor, group: dict[str, Any]) -> float:
         # an orthogonalised rows x cols matrix has entries of about 1 / sqrt(the longer side); as with Adam's ratio, updates
         # routinely shrink to a tenth of that
-        return 0.1 * min((_update_factor(g["adjust_lr_fn"], *p.shape) / math.sqrt(max(p.shape))
-                          for g in self.param_groups for p in g["params"] if p.numel()), default=1.0)
+        return 0.1 * _update_factor(group["adjust_lr_fn"], *p.shape) / math.sqrt(max(p.shape))
+
+    def _plan_signature(self, hparams: dict[str, Any]) -> Any:
+        return super()._plan_signature(hparams), hparams["adjust_lr_fn"]
 
     def _prepare_param(self, p: torch.Tensor, group: dict[str, Any]):
         if hasattr(p, "to_local"):

@@ -4,7 +4,7 @@ import pytest
 import torch
 import torch.nn as nn
 
-from tests.test_gpu_muon import DEV, _muon
+from tests.test_gpu_muon import DEV, _fo, _grads, _muon
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,49 @@ def test_momentum_codes_stand_for_what_dequantize_reads():
         moved.append(weight.detach().clone())
     assert moved[1].count_nonzero() >= 250
     assert torch.equal(moved[0], moved[1]), (moved[0] != moved[1]).sum().item()
+
+
+def _numerics(shapes, lr, bits=24):
+    fo = _fo()
+    params = [nn.Parameter(torch.full(s, 100.0, device=DEV, dtype=torch.bfloat16)) for s in shapes]
+    opt = fo.FlashMuon(params, lr=lr, master_weight_bits=bits, check_numerics=True)
+    _grads(params, 1)
+    return opt, params
+
+
+def test_check_numerics_judges_each_matrix_by_its_own_step():
+    """A square matrix beside a long one, whose steps are 32 times smaller: a learning rate that moves either alone is taken for the two of them
+    where each is fine, and refused, by the long one, where only that is not."""
+    fo = _fo()
+    square, long = (64, 64), (64, 65536)
+
+    def refused(shapes, lr):
+        opt, params = _numerics(shapes, lr)
+        try:
+            for _ in range(2):      # the second step goes by what the first one kept
+                _grads(params, 1)
+                opt.step()
+        except fo.NumericsError as e:
+            return str(e)
+        return ""
+
+    rates = [2.0 ** -k for k in range(-8, 24)]
+    alone = {s: min(lr for lr in rates if not refused([s], lr)) for s in (square, long)}
+    assert alone[long] == 32 * alone[square]
+    assert not refused([square, long], alone[long])
+    assert refused([square, long], alone[long] / 2)
+    # the long one sits out: nothing about it matters
+    opt, params = _numerics([square, long], alone[square])
+    params[1].grad = None
+    opt.step()
+    params[0].grad = params[0].grad.clone()
+    opt.step()
+    # a group of its own, with its own learning rate
+    params = [nn.Parameter(torch.full(s, 100.0, device=DEV, dtype=torch.bfloat16)) for s in (square, long)]
+    opt = fo.FlashMuon([dict(params=params[:1], lr=alone[square]), dict(params=params[1:], lr=alone[long])], check_numerics=True)
+    for _ in range(2):
+        _grads(params, 1)
+        opt.step()
+    opt.param_groups[0]["lr"] /= 2
+    with pytest.raises(fo.NumericsError):
+        opt.step()
