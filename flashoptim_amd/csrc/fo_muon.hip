@@ -40,6 +40,9 @@ constexpr int kMaxShapes = 16;    // of one launch
 constexpr int kPad = 64, kNarrow = 32;
 constexpr int kChunk = 8192;      // elements of a matrix whose squares one workgroup sums
 
+// What a matrix is multiplied by for its norm, the power of two first: fp32 holds both for every norm that fp32 values have.
+struct Scaling { float power, factor; };
+
 // The matrices of one shape.
 struct MatrixGroup {
     int rows, cols, padded_rows, padded_cols, count;
@@ -55,7 +58,7 @@ struct MatrixGroup {
     __host__ __device__ int side() const { return tall() ? padded_cols : padded_rows; }
     __host__ __device__ int64_t area() const { return (int64_t)padded_rows * padded_cols; }
     __host__ __device__ int64_t gram_area() const { return (int64_t)side() * side(); }
-    // per matrix: two generations of hi and of T, lo, three square matrices, their diagonals, the factor that normalises, sums of squares.
+    // per matrix: two generations of hi and of T, lo, three square matrices, their diagonals, what normalises, sums of squares.
     // The update before its normalisation (fp32) lies over the second generation, which is written later.
     __host__ __device__ int64_t bytes_each() const {
         return area() * 10 + gram_area() * 6 + (side() * 12 + 255) / 256 * 256 + 256 + ((int64_t)chunks * 8 + 255) / 256 * 256;
@@ -70,8 +73,8 @@ struct MatrixGroup {
     __device__ u32* lo(int k) const { return (u32*)(of(k) + area() * 8); }   // pairs of bf16
     __device__ _Float16* square(int k, int which) const { return (_Float16*)(of(k) + area() * 10 + gram_area() * 2 * which); }
     __device__ float* diagonal(int k, int which) const { return (float*)(of(k) + area() * 10 + gram_area() * 6) + side() * which; }
-    __device__ float* factor(int k) const { return diagonal(k, 3); }
-    __device__ double* squares(int k) const { return (double*)((char*)factor(k) + 256); }
+    __device__ Scaling* scaling(int k) const { return (Scaling*)diagonal(k, 3); }
+    __device__ double* squares(int k) const { return (double*)((char*)scaling(k) + 256); }
 };
 
 // A launch over all groups.  Workgroups begin[g] .. begin[g + 1] belong to group g; in the products' launches these are seats,
@@ -116,6 +119,14 @@ __device__ __forceinline__ double workgroup_sum(double x, double* lds) {
     return lds[0] + lds[1] + lds[2] + lds[3];
 }
 
+// The squares of what fp32 holds are summed in fp64, which holds them.
+__device__ __forceinline__ double add_square(float x, double sum) { return fma((double)x, (double)x, sum); }
+
+__device__ __forceinline__ Scaling scaling_of(double norm, float unit) {
+    const float power = norm > 0x1p64 ? 0x1p-64f : norm < 0x1p-64 ? 0x1p64f : 1.0f;
+    return {power, (float)((double)unit / (norm * (double)power))};
+}
+
 // Sum of the squares of a run of 8-value pieces of the matrix, one number per workgroup (in order, so a step repeats to
 // the bit).  One read of the matrix, bound by memory: 14336 x 4096 bf16 in 25 us, 4.7 TB/s.
 template <int DT> __global__ __launch_bounds__(256) void squares_kernel(Groups a, MatrixSource source) {
@@ -126,16 +137,16 @@ template <int DT> __global__ __launch_bounds__(256) void squares_kernel(Groups a
     const int k = (int)(local / m.chunks), chunk = (int)(local % m.chunks);
     const int64_t pieces = (m.cols + 7) / 8, all = pieces * m.rows, each = (all + m.chunks - 1) / m.chunks;
     const int64_t last = (chunk + 1) * each < all ? (chunk + 1) * each : all;
-    float sum = 0.0f;
+    double sum = 0.0;
     for (int64_t i = chunk * each + threadIdx.x; i < last; i += 256) {
         const int64_t row = i / pieces;
         const int col = (int)(i - row * pieces) * 8;
         float v[8];
         read8<DT>((const char*)source.data + (source.stride * k + source.row_stride * row + col) * DTypeInfo<DT>::bytes, m.cols - col, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
+        for (int e = 0; e < 8; ++e) sum = add_square(v[e], sum);
     }
-    const double total = workgroup_sum((double)sum, lds);
+    const double total = workgroup_sum(sum, lds);
     if (threadIdx.x == 0) m.squares(k)[chunk] = total;
 }
 
@@ -149,7 +160,7 @@ __global__ __launch_bounds__(256) void norm_kernel(Groups a, float eps) {
 #pragma unroll 8
     for (int i = threadIdx.x; i < m.chunks; i += 256) sum += m.squares(k)[i];
     const double total = workgroup_sum(sum, lds);
-    if (threadIdx.x == 0) *m.factor(k) = (float)((double)m.unit / (sqrt(total) + (double)eps));
+    if (threadIdx.x == 0) *m.scaling(k) = scaling_of(sqrt(total) + (double)eps, m.unit);
 }
 
 // fp16 of a value that has been rounded to fp32 before.  The empty statement keeps the two roundings apart: the compiler joins a product or a sum
@@ -176,7 +187,7 @@ template <int DT> __global__ __launch_bounds__(256) void split_kernel(Groups a, 
     const int64_t local = blockIdx.x - a.begin[g];
     const int k = (int)(local / tiles), tile = (int)(local % tiles);
     const int row0 = tile / tile_cols * 64, col0 = tile % tile_cols * 64;
-    const float factor = *m.factor(k);
+    const Scaling scale = *m.scaling(k);
     const char* base = source.data ? (const char*)source.data + source.stride * k * DTypeInfo<DT>::bytes : (const char*)m.update(k);
     const int64_t row_stride = source.data ? source.row_stride : m.cols;
     const int piece = (threadIdx.x & 7) * 8;
@@ -189,7 +200,7 @@ template <int DT> __global__ __launch_bounds__(256) void split_kernel(Groups a, 
         u32x4 lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            v[e] *= factor;
+            v[e] = v[e] * scale.power * scale.factor;
             hi[e] = to_half(v[e]);
             v[e] -= (float)hi[e];
             lds[r][piece + e] = hi[e];
@@ -227,7 +238,7 @@ struct MomentumArgs {
 };
 
 template <int DT, bool QUANT, int MODE>
-__device__ __forceinline__ float momentum_span(const fo_tensor_desc& d, float* update, Where w, int64_t n, const MomentumArgs& h, const float* lut) {
+__device__ __forceinline__ double momentum_span(const fo_tensor_desc& d, float* update, Where w, int64_t n, const MomentumArgs& h, const float* lut) {
     constexpr int EPL = DTypeInfo<DT>::epl, PB = DTypeInfo<DT>::bytes, SB = QUANT ? 1 : PB;
     Pack<PB, EPL> g;
     Pack<SB, EPL> raw;
@@ -236,7 +247,8 @@ __device__ __forceinline__ float momentum_span(const fo_tensor_desc& d, float* u
     const bool live = MODE == kVector || w.first() < n;
     float scale = 1.0f;
     if constexpr (QUANT) { if (live) scale = f16_bits_to_f32(load_scale((const uint16_t*)d.mom_scales, w)); }
-    float m[EPL], u[EPL], am = 0.0f, sum = 0.0f;
+    float m[EPL], u[EPL], am = 0.0f;
+    double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < EPL; ++k) {
         const float gk = widen<DT, EPL>(g, k) * h.one_minus_mu;
@@ -245,7 +257,7 @@ __device__ __forceinline__ float momentum_span(const fo_tensor_desc& d, float* u
         m[k] = old * h.mu + gk;
         u[k] = h.nesterov ? gk + m[k] * h.mu : m[k];
         am = fmaxf(am, fabsf(m[k]));
-        sum = fmaf(u[k], u[k], sum);
+        sum = add_square(u[k], sum);
     }
     if constexpr (QUANT) {
         am = fmaxf(group_max<EPL>(am), 1e-12f);
@@ -262,10 +274,10 @@ __device__ __forceinline__ float momentum_span(const fo_tensor_desc& d, float* u
 #pragma unroll
         for (int k = 0; k < EPL; k += 4) *reinterpret_cast<f32x4*>(out + k) = f32x4{u[k], u[k + 1], u[k + 2], u[k + 3]};
     } else {
-        sum = 0.0f;
+        sum = 0.0;
 #pragma unroll
         for (int k = 0; k < EPL; ++k)
-            if (w.first() + k < n) { out[k] = u[k]; sum = fmaf(u[k], u[k], sum); }
+            if (w.first() + k < n) { out[k] = u[k]; sum = add_square(u[k], sum); }
     }
     return sum;
 }
@@ -287,7 +299,7 @@ template <int DT, bool QUANT> __global__ __launch_bounds__(256) void momentum_ke
     }
     const bool aligned = (((uintptr_t)d.grad | (uintptr_t)d.mom) & 15) == 0;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    float sum = 0.0f;
+    double sum = 0.0;
     for (int i = wave; i < kChunk / (64 * EPL); i += 4) {
         const Where w{(int64_t)chunk * kChunk + i * 64 * EPL, (int)(threadIdx.x & 63) * EPL};
         if (w.span >= n) break;
@@ -295,7 +307,7 @@ template <int DT, bool QUANT> __global__ __launch_bounds__(256) void momentum_ke
         else if (aligned) sum += momentum_span<DT, QUANT, kLane>(d, m.update(k), w, n, h, lut);
         else sum += momentum_span<DT, QUANT, kGuarded>(d, m.update(k), w, n, h, lut);
     }
-    const double total = workgroup_sum((double)sum, lds);
+    const double total = workgroup_sum(sum, lds);
     if (threadIdx.x == 0) m.squares(k)[chunk] = total;
 }
 
@@ -793,7 +805,7 @@ template <int DT, class Out> __global__ __launch_bounds__(kSmallThreads) void sm
     float* const whole = reinterpret_cast<float*>(lds);
     const int pitch = m.cols | 1, row_step = tall ? 1 : pitch, col_step = tall ? pitch : 1;
     const int pieces = (m.cols + 7) / 8, all = pieces * m.rows;
-    float sum = 0.0f;
+    double total = 0.0;
     {
         float v[kSmallPieces][8];
 #pragma unroll
@@ -808,7 +820,7 @@ template <int DT, class Out> __global__ __launch_bounds__(kSmallThreads) void sm
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     if (col + e < m.cols) whole[row * pitch + col + e] = v[i][e];
-                    sum = fmaf(v[i][e], v[i][e], sum);
+                    total = add_square(v[i][e], total);
                 }
             }
         }
@@ -830,7 +842,6 @@ template <int DT, class Out> __global__ __launch_bounds__(kSmallThreads) void sm
     }
     __syncthreads();
     double* sums = reinterpret_cast<double*>(lds);
-    double total = sum;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) total += __shfl_down(total, d);
     if (lane == 0) sums[wave] = total;
@@ -838,10 +849,10 @@ template <int DT, class Out> __global__ __launch_bounds__(kSmallThreads) void sm
     total = 0.0;
 #pragma unroll
     for (int w = 0; w < kSmallWaves; ++w) total += sums[w];
-    const float factor = (float)(1.0 / (sqrt(total) + (double)h.eps));
+    const Scaling scale = scaling_of(sqrt(total) + (double)h.eps, 1.0f);
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kSmallUnits; ++u) { x[u][0] *= factor; x[u][1] *= factor; }
+    for (int u = 0; u < kSmallUnits; ++u) { x[u][0] = x[u][0] * scale.power * scale.factor; x[u][1] = x[u][1] * scale.power * scale.factor; }
 
     // the wavefront's block of S and B, on or above the diagonal, column by column
     int bi = wave, bj = 0;
@@ -984,18 +995,17 @@ template <int DT, class Out> __global__ __launch_bounds__(64) void tiny_kernel(G
             if (col + e < m.cols) xs[tall ? col + e : row][tall ? row : col + e] = v[e];
     }
     __syncthreads();
-    float sum = 0.0f;
+    double total = 0.0;
 #pragma unroll
     for (int i = 0; i < kTinySide; ++i) {
         x[i] = xs[i][lane];
-        sum = fmaf(x[i], x[i], sum);
+        total = add_square(x[i], total);
     }
-    double total = sum;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
-    const float factor = (float)(1.0 / (sqrt(total) + (double)h.eps));
+    const Scaling scale = scaling_of(sqrt(total) + (double)h.eps, 1.0f);
 #pragma unroll
-    for (int i = 0; i < kTinySide; ++i) x[i] *= factor;
+    for (int i = 0; i < kTinySide; ++i) x[i] = x[i] * scale.power * scale.factor;
     const int row = lane >> 2, first = (lane & 3) * 4;   // the lane's four entries of S and B
     for (int step = 0; step < h.steps; ++step) {
 #pragma unroll

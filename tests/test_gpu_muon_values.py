@@ -1,10 +1,10 @@
-"""GPU tests of single values on their way through the Muon step."""
+"""GPU tests of single values on their way through the Muon step and the iteration."""
 
 import pytest
 import torch
 import torch.nn as nn
 
-from tests.test_gpu_muon import DEV, _fo, _grads, _muon
+from tests.test_gpu_muon import DEV, _check, _fo, _grads, _iterate, _matrices, _muon
 
 pytestmark = pytest.mark.gpu
 
@@ -35,6 +35,26 @@ def test_momentum_codes_stand_for_what_dequantize_reads():
         moved.append(weight.detach().clone())
     assert moved[1].count_nonzero() >= 250
     assert torch.equal(moved[0], moved[1]), (moved[0] != moved[1]).sum().item()
+
+
+@pytest.mark.parametrize("size", [1e-36, 1e-30, 1e-22, 1e19, 1e25, 1e33])
+@pytest.mark.parametrize("shape", [(10, 12), (60, 90), (300, 700), (700, 300)])
+def test_matrices_whose_squares_fp32_does_not_hold(shape, size):
+    x = _matrices(*shape, seed=3, size=size)
+    assert x.isfinite().all() and float(x.abs().max()) > 2.0 ** -126
+    _check(_fo().newton_schulz(x, eps=0.0), _iterate(x, eps=0.0), (shape, size))
+
+
+@pytest.mark.parametrize("size", [1e-22, 1e19, 1e25, 1e33])
+@pytest.mark.parametrize("shape", [(10, 12), (60, 90), (300, 700)])
+@pytest.mark.parametrize("dtype,quantize", [(torch.float32, False), (torch.bfloat16, False)])
+def test_steps_along_gradients_whose_squares_fp32_does_not_hold(shape, size, dtype, quantize):
+    weight = nn.Parameter(torch.zeros(shape, device=DEV, dtype=dtype))
+    opt = _muon([weight], lr=1.0, weight_decay=0.0, momentum=0.0, master_weight_bits=None, eps=0.0, quantize=quantize)
+    weight.grad = _matrices(*shape, seed=4, size=size, dtype=dtype)
+    opt.step()
+    factor = max(1.0, shape[0] / shape[1]) ** 0.5
+    _check((-weight.detach() / factor).to(torch.bfloat16), _iterate(weight.grad, eps=0.0), (shape, size, dtype))
 
 
 def _numerics(shapes, lr, bits=24):
