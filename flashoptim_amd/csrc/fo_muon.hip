@@ -119,12 +119,24 @@ __device__ __forceinline__ double workgroup_sum(double x, double* lds) {
     return lds[0] + lds[1] + lds[2] + lds[3];
 }
 
-// The squares of what fp32 holds are summed in fp64, which holds them.
-__device__ __forceinline__ double add_square(float x, double sum) { return fma((double)x, (double)x, sum); }
+// Whether a sum of a few squares in fp32 will do: it is not beyond that, nor so small that some of the squares are (what is lost among them is 2^-46
+// of a sum of 2^-80).  fp64 holds the square of every fp32 value.
+__device__ __forceinline__ bool holds_squares(float sum) { return sum > 0x1p-80f && sum < __builtin_inff(); }
+template <int N> __device__ __forceinline__ double sum_of_squares(const float (&v)[N]) {
+    float quick = 0.0f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) quick = fmaf(v[e], v[e], quick);
+    if (holds_squares(quick)) return (double)quick;
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum = fma((double)v[e], (double)v[e], sum);
+    return sum;
+}
 
-__device__ __forceinline__ Scaling scaling_of(double norm, float unit) {
-    const float power = norm > 0x1p64 ? 0x1p-64f : norm < 0x1p-64 ? 0x1p64f : 1.0f;
-    return {power, (float)((double)unit / (norm * (double)power))};
+// The first of what a matrix of this norm is multiplied by.
+__device__ __forceinline__ float power_for(double norm) {
+    const float near = (float)norm;
+    return near > 0x1p64f ? 0x1p-64f : near < 0x1p-64f ? 0x1p64f : 1.0f;
 }
 
 // Sum of the squares of a run of 8-value pieces of the matrix, one number per workgroup (in order, so a step repeats to
@@ -143,8 +155,7 @@ template <int DT> __global__ __launch_bounds__(256) void squares_kernel(Groups a
         const int col = (int)(i - row * pieces) * 8;
         float v[8];
         read8<DT>((const char*)source.data + (source.stride * k + source.row_stride * row + col) * DTypeInfo<DT>::bytes, m.cols - col, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = add_square(v[e], sum);
+        sum += sum_of_squares(v);
     }
     const double total = workgroup_sum(sum, lds);
     if (threadIdx.x == 0) m.squares(k)[chunk] = total;
@@ -160,20 +171,21 @@ __global__ __launch_bounds__(256) void norm_kernel(Groups a, float eps) {
 #pragma unroll 8
     for (int i = threadIdx.x; i < m.chunks; i += 256) sum += m.squares(k)[i];
     const double total = workgroup_sum(sum, lds);
-    if (threadIdx.x == 0) *m.scaling(k) = scaling_of(sqrt(total) + (double)eps, m.unit);
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(total) + (double)eps;
+        const float power = power_for(norm);
+        *m.scaling(k) = {power, (float)((double)m.unit / (norm * (double)power))};
+    }
 }
 
-// fp16 of a value that has been rounded to fp32 before.  The empty statement keeps the two roundings apart: the compiler joins a product or a sum
-// and its conversion into one instruction, which rounds once, for some uses of a value and in some kernels only.  In the polynomial's 256 x 256
-// tiles an entry and its mirror image then differed by a unit of fp16 at one place in 1e5, and both from what other tiles make.
-__device__ __forceinline__ _Float16 to_half(float x) {
-    asm("" : "+v"(x));
-    return (_Float16)x;
-}
+// Says that a value is rounded to fp32 here.  Left to itself the compiler joins the product or sum that makes it and its conversion to fp16 into one
+// instruction, which rounds once, for some uses of a value and in some kernels only.  In the polynomial's 256 x 256 tiles an entry and
+// its mirror image then differed by a unit of fp16 at one place in 1e5, and both from what other tiles make.
+__device__ __forceinline__ void rounded(float& x) { asm("" : "+v"(x)); }
 __device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
     f16x8 h;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = to_half(v[e]);
+    for (int e = 0; e < 8; ++e) h[e] = (_Float16)v[e];
     return h;
 }
 
@@ -201,7 +213,8 @@ template <int DT> __global__ __launch_bounds__(256) void split_kernel(Groups a, 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             v[e] = v[e] * scale.power * scale.factor;
-            hi[e] = to_half(v[e]);
+            rounded(v[e]);
+            hi[e] = (_Float16)v[e];
             v[e] -= (float)hi[e];
             lds[r][piece + e] = hi[e];
         }
@@ -248,7 +261,6 @@ __device__ __forceinline__ double momentum_span(const fo_tensor_desc& d, float* 
     float scale = 1.0f;
     if constexpr (QUANT) { if (live) scale = f16_bits_to_f32(load_scale((const uint16_t*)d.mom_scales, w)); }
     float m[EPL], u[EPL], am = 0.0f;
-    double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < EPL; ++k) {
         const float gk = widen<DT, EPL>(g, k) * h.one_minus_mu;
@@ -257,7 +269,6 @@ __device__ __forceinline__ double momentum_span(const fo_tensor_desc& d, float* 
         m[k] = old * h.mu + gk;
         u[k] = h.nesterov ? gk + m[k] * h.mu : m[k];
         am = fmaxf(am, fabsf(m[k]));
-        sum = add_square(u[k], sum);
     }
     if constexpr (QUANT) {
         am = fmaxf(group_max<EPL>(am), 1e-12f);
@@ -274,12 +285,12 @@ __device__ __forceinline__ double momentum_span(const fo_tensor_desc& d, float* 
 #pragma unroll
         for (int k = 0; k < EPL; k += 4) *reinterpret_cast<f32x4*>(out + k) = f32x4{u[k], u[k + 1], u[k + 2], u[k + 3]};
     } else {
-        sum = 0.0;
 #pragma unroll
-        for (int k = 0; k < EPL; ++k)
-            if (w.first() + k < n) { out[k] = u[k]; sum = add_square(u[k], sum); }
+        for (int k = 0; k < EPL; ++k) {
+            if (w.first() + k < n) out[k] = u[k]; else u[k] = 0.0f;
+        }
     }
-    return sum;
+    return sum_of_squares(u);
 }
 
 template <int DT, bool QUANT> __global__ __launch_bounds__(256) void momentum_kernel(Groups a, MomentumArgs h) {
@@ -332,13 +343,14 @@ struct StepArgs {
 };
 
 
-// Square matrices without their diagonals: all are symmetric, so each tile off the diagonal is written twice.  Of a tile on the diagonal
-// both halves are computed.  Those of S and of its polynomial agree to the bit; those of U V do only as far as U and V commute, and which entries
-// lie in such tiles goes by the tile's size: there too what is below the diagonal is copied from above it, so that no result depends on the
-// tile, which is chosen by all that shares the launch.
-template <int KIND> struct SymmetricOut {
-    static constexpr bool kCopied = KIND == kMixed;   // below the diagonal, in tiles on it
+// Square matrices without their diagonals: all are symmetric, so each tile off the diagonal is written twice.  Of what lies on it both halves are computed.
+// Those of S and of its polynomial agree to the bit; those of U V do only as far as U and V commute.  So that no result goes by the tile, which
+// all that shares the launch has a say in, it is blocks of 64 x 64 on the diagonal of which both halves are kept, and in larger tiles what is
+// below these is copied as well.
+template <int KIND, int TILE> struct SymmetricOut {
     static constexpr bool kColumns = true;
+    static constexpr bool kCopied = KIND == kMixed && TILE > kPad;
+    __device__ __forceinline__ static bool below(int i, int j) { return i / kPad > j / kPad; }
     const _Float16 *u, *v;
     const float *u_diagonal, *v_diagonal;
     _Float16* out;
@@ -367,7 +379,7 @@ template <int KIND> struct SymmetricOut {
         }
     }
     __device__ __forceinline__ void row(int i, int j, const In& in, float (&x)[8]) const {
-        if (i >= side || j >= side) return;
+        if (i >= side || j >= side || (kCopied && !mirror && below(i, j))) return;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if constexpr (KIND == kGram) {
@@ -388,27 +400,14 @@ template <int KIND> struct SymmetricOut {
                     x[e] = 0.0f;
                 }
             }
+            rounded(x[e]);
         }
-        _Float16* to = out + (int64_t)i * side + j;
-        if (kCopied && !mirror && j < i) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (j + e >= i) to[e] = to_half(x[e]);
-        } else {
-            *reinterpret_cast<f16x8*>(to) = half8(x);
-        }
+        *reinterpret_cast<f16x8*>(out + (int64_t)i * side + j) = half8(x);
     }
     __device__ __forceinline__ bool columns() const { return kCopied || mirror; }
     __device__ __forceinline__ void column(int i, int j, const float (&x)[8]) const {
-        if (i >= side || j >= side) return;
-        _Float16* to = out + (int64_t)j * side + i;
-        if (kCopied && !mirror && j < i + 8) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (i + e < j) to[e] = to_half(x[e]);
-        } else {
-            *reinterpret_cast<f16x8*>(to) = half8(x);
-        }
+        if (i >= side || j >= side || (kCopied && !mirror && !below(j, i))) return;
+        *reinterpret_cast<f16x8*>(out + (int64_t)j * side + i) = half8(x);
     }
 };
 
@@ -456,7 +455,7 @@ template <int WT, int STAGES, int KIND> __global__ __launch_bounds__(256, WT >= 
         PartialOut out{m.partial(k, part), side};
         tile.finish(i * Tile::kTile, j * Tile::kTile, out);
     } else {
-        SymmetricOut<KIND> out{m.square(k, h.u), m.square(k, h.v), m.diagonal(k, h.u), m.diagonal(k, h.v), m.square(k, h.out), m.diagonal(k, h.out), side,
+        SymmetricOut<KIND, Tile::kTile> out{m.square(k, h.u), m.square(k, h.v), m.diagonal(k, h.u), m.diagonal(k, h.v), m.square(k, h.out), m.diagonal(k, h.out), side,
                                h.first ? 1.0f / (m.unit * m.unit) : 1.0f, h.alpha, h.beta, h.gamma, i != j, {}};
         tile.finish(i * Tile::kTile, j * Tile::kTile, out);
     }
@@ -482,7 +481,8 @@ __global__ __launch_bounds__(256) void gather_kernel(Groups a, SquareArgs h) {
     if (h.first) x *= 1.0f / (m.unit * m.unit);
     if (i == j) { m.diagonal(k, h.out)[i] = x; x = 0.0f; }
     _Float16* s = m.square(k, h.out);
-    s[(int64_t)i * side + j] = s[(int64_t)j * side + i] = to_half(x);
+    rounded(x);
+    s[(int64_t)i * side + j] = s[(int64_t)j * side + i] = (_Float16)x;
 }
 
 // X <- a X + B X, common to the steps: x = (acc + (a + d) (hi + lo)) / unit, d the diagonal entry of B.
@@ -514,6 +514,7 @@ struct ApplyIn {
         for (int e = 0; e < 8; ++e) {
             const float rest = as_f32(e & 1 ? in.lo[e / 2] & 0xffff0000u : in.lo[e / 2] << 16);
             v[e] = fmaf(tall ? d[e] : in.d, (float)in.hi[e] + rest, v[e]) * scale;
+            rounded(v[e]);
         }
     }
 };
@@ -712,7 +713,7 @@ __device__ __forceinline__ f16x8 read_turned(char* lds, int at, int pitch) {
 }
 __device__ __forceinline__ void put_half(char* lds, int at, _Float16 v) { *reinterpret_cast<_Float16*>(lds + at) = v; }
 __device__ __forceinline__ void put_halves(char* lds, int at, f16x4 v) { *reinterpret_cast<f16x4*>(lds + at) = v; }
-__device__ __forceinline__ f16x4 halves(f32x4 v) { return f16x4{to_half(v.x), to_half(v.y), to_half(v.z), to_half(v.w)}; }
+__device__ __forceinline__ f16x4 halves(f32x4 v) { return f16x4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w}; }
 
 // What becomes of eight values of the result; what that needs from memory is loaded before the result is there.
 struct SmallResult {
@@ -805,9 +806,9 @@ template <int DT, class Out> __global__ __launch_bounds__(kSmallThreads) void sm
     float* const whole = reinterpret_cast<float*>(lds);
     const int pitch = m.cols | 1, row_step = tall ? 1 : pitch, col_step = tall ? pitch : 1;
     const int pieces = (m.cols + 7) / 8, all = pieces * m.rows;
-    double total = 0.0;
+    double total;
     {
-        float v[kSmallPieces][8];
+        float v[kSmallPieces][8], quick = 0.0f;
 #pragma unroll
         for (int i = 0; i < kSmallPieces; ++i) {
             const int at = threadIdx.x + i * kSmallThreads, row = at / pieces, col = (at - row * pieces) * 8;
@@ -820,9 +821,16 @@ template <int DT, class Out> __global__ __launch_bounds__(kSmallThreads) void sm
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     if (col + e < m.cols) whole[row * pitch + col + e] = v[i][e];
-                    total = add_square(v[i][e], total);
+                    quick = fmaf(v[i][e], v[i][e], quick);
                 }
             }
+        }
+        total = (double)quick;
+        if (!holds_squares(quick)) {
+            total = 0.0;
+#pragma unroll
+            for (int i = 0; i < kSmallPieces; ++i)
+                if ((int)threadIdx.x + i * kSmallThreads < all) total += sum_of_squares(v[i]);
         }
     }
     __syncthreads();
@@ -849,10 +857,17 @@ template <int DT, class Out> __global__ __launch_bounds__(kSmallThreads) void sm
     total = 0.0;
 #pragma unroll
     for (int w = 0; w < kSmallWaves; ++w) total += sums[w];
-    const Scaling scale = scaling_of(sqrt(total) + (double)h.eps, 1.0f);
+    double norm = sqrt(total) + (double)h.eps;
     __syncthreads();
+    const float power = power_for(norm);
+    if (power != 1.0f) {   // seldom
+        norm *= (double)power;
 #pragma unroll
-    for (int u = 0; u < kSmallUnits; ++u) { x[u][0] = x[u][0] * scale.power * scale.factor; x[u][1] = x[u][1] * scale.power * scale.factor; }
+        for (int u = 0; u < kSmallUnits; ++u) { x[u][0] *= power; x[u][1] *= power; }
+    }
+    const float factor = (float)(1.0 / norm);
+#pragma unroll
+    for (int u = 0; u < kSmallUnits; ++u) { x[u][0] *= factor; x[u][1] *= factor; }
 
     // the wavefront's block of S and B, on or above the diagonal, column by column
     int bi = wave, bj = 0;
@@ -995,17 +1010,15 @@ template <int DT, class Out> __global__ __launch_bounds__(64) void tiny_kernel(G
             if (col + e < m.cols) xs[tall ? col + e : row][tall ? row : col + e] = v[e];
     }
     __syncthreads();
-    double total = 0.0;
 #pragma unroll
-    for (int i = 0; i < kTinySide; ++i) {
-        x[i] = xs[i][lane];
-        total = add_square(x[i], total);
-    }
+    for (int i = 0; i < kTinySide; ++i) x[i] = xs[i][lane];
+    double total = sum_of_squares(x);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
-    const Scaling scale = scaling_of(sqrt(total) + (double)h.eps, 1.0f);
+    const double norm = sqrt(total) + (double)h.eps;
+    const float power = power_for(norm), factor = (float)(1.0 / (norm * (double)power));
 #pragma unroll
-    for (int i = 0; i < kTinySide; ++i) x[i] = x[i] * scale.power * scale.factor;
+    for (int i = 0; i < kTinySide; ++i) x[i] = x[i] * power * factor;
     const int row = lane >> 2, first = (lane & 3) * 4;   // the lane's four entries of S and B
     for (int step = 0; step < h.steps; ++step) {
 #pragma unroll
