@@ -229,32 +229,39 @@ class FlashMuon(FlashOptimizer):
         check_numerics: bool = False,
         fused: bool = True,
     ):
-        if not 0.0 <= momentum < 1.0:
-            raise ValueError(f"Invalid momentum value: {momentum}")
-        if not 0.0 <= weight_decay:
-            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
-        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
-            raise ValueError(f'adjust_lr_fn must be "original" or "match_rms_adamw", got {adjust_lr_fn!r}')
-        _check_iteration(ns_steps, ns_coefficients, eps)
+        defaults = {"momentum": momentum, "weight_decay": weight_decay, "nesterov": bool(nesterov), "ns_coefficients": ns_coefficients, "eps": eps,
+                    "ns_steps": ns_steps, "adjust_lr_fn": adjust_lr_fn}
+        self._check_hyperparameters(defaults)
         super().__init__(
-            params, lr=lr,
-            defaults={"momentum": momentum, "weight_decay": weight_decay, "nesterov": bool(nesterov),
-                      "ns_coefficients": tuple(ns_coefficients), "eps": eps, "ns_steps": int(ns_steps), "adjust_lr_fn": adjust_lr_fn},
+            params, lr=lr, defaults={**defaults, "ns_coefficients": tuple(ns_coefficients), "ns_steps": int(ns_steps)},
             quantize=quantize, compress_state_dict=compress_state_dict, master_weight_bits=master_weight_bits,
             check_numerics=check_numerics, fused=fused,
         )
 
+    @staticmethod
+    def _check_hyperparameters(hparams: dict[str, Any]) -> None:
+        if not 0.0 <= hparams["momentum"] < 1.0:
+            raise ValueError(f"Invalid momentum value: {hparams['momentum']}")
+        if not 0.0 <= hparams["weight_decay"]:
+            raise ValueError(f"Invalid weight_decay value: {hparams['weight_decay']}")
+        if hparams["adjust_lr_fn"] not in (None, "original", "match_rms_adamw"):
+            raise ValueError(f'adjust_lr_fn must be "original" or "match_rms_adamw", got {hparams["adjust_lr_fn"]!r}')
+        _check_iteration(hparams["ns_steps"], hparams["ns_coefficients"], hparams["eps"])
+
     def add_param_group(self, param_group: dict[str, Any]) -> None:
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
-            problem = None
-            if p.dim() != 2:
-                problem = f"FlashMuon steps matrices only, got a parameter of shape {tuple(p.shape)}."
-            elif max(p.shape, default=0) > MATRIX_MOST_LINES:
-                problem = f"FlashMuon steps matrices of at most {MATRIX_MOST_LINES} rows and columns, got {tuple(p.shape)}."
-            if problem:
-                self.param_groups.pop()
-                raise ValueError(problem)
+        group = self.param_groups[-1]
+        try:
+            self._check_hyperparameters(group)
+            for p in group["params"]:
+                if p.dim() != 2:
+                    raise ValueError(f"FlashMuon steps matrices only, got a parameter of shape {tuple(p.shape)}.")
+                if max(p.shape) > MATRIX_MOST_LINES:
+                    raise ValueError(f"FlashMuon steps matrices of at most {MATRIX_MOST_LINES} rows and columns, got {tuple(p.shape)}.")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+        group.update(ns_coefficients=tuple(group["ns_coefficients"]), ns_steps=int(group["ns_steps"]))
 
     def _quantized_state_spec(self) -> dict[str, QuantizedTensorSpec]:
         return {"momentum_buffer": QuantizedTensorSpec(signed=True)}

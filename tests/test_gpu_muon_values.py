@@ -101,3 +101,20 @@ def test_check_numerics_judges_each_matrix_by_its_own_step():
     opt.param_groups[0]["lr"] /= 2
     with pytest.raises(fo.NumericsError):
         opt.step()
+
+
+@pytest.mark.parametrize("bad", [dict(ns_coefficients=(1.5, -0.5)), dict(ns_coefficients=(1.0, float("inf"), 0.0)), dict(ns_steps=0), dict(ns_steps=2.5), dict(eps=-1.0),
+                                 dict(momentum=1.0), dict(weight_decay=-0.1), dict(adjust_lr_fn="spectral")])
+def test_groups_are_checked_like_the_constructor(bad):
+    """What a group says for itself, in the constructor's list or added later."""
+    fo = _fo()
+    first, second = (nn.Parameter(torch.zeros(8, 8, device=DEV, dtype=torch.bfloat16)) for _ in range(2))
+    with pytest.raises(ValueError):
+        fo.FlashMuon([dict(params=[first], **bad)])
+    opt = fo.FlashMuon([dict(params=[first], ns_steps=3.0, ns_coefficients=[1.5, -0.5, 0.0], adjust_lr_fn="match_rms_adamw")])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[second], **bad))
+    assert len(opt.param_groups) == 1
+    first.grad = torch.ones_like(first)
+    opt.step()
+    assert first.any()
