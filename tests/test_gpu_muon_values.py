@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 
 def test_momentum_codes_stand_for_what_dequantize_reads():
     """Every code, through one step that moves weights of zero along momentum codes, and through the same step with the momentum held in fp32 as
-    `dequantize` gives it: to the bit.  (16 x 16 runs in fp32, and with coefficients (1, 0, 0) the step is the normalised momentum.)"""
+    `dequantize` gives it.  (16 x 16 runs in fp32, and with coefficients (1, 0, 0) the step is the normalised momentum.)  The quotient by 127 is off by
+    2^-23 at most, y / (2 - |y|) makes 2^-22 of it, the norm can shift by as much, and the roundings of fp32 add less than that again: 2^-20."""
     from flashoptim_amd.kernels import dequantize
 
     codes = torch.arange(256, device=DEV).to(torch.uint8).view(torch.int8).view(16, 16)
@@ -34,7 +35,7 @@ def test_momentum_codes_stand_for_what_dequantize_reads():
         opt.step()
         moved.append(weight.detach().clone())
     assert moved[1].count_nonzero() >= 250
-    assert torch.equal(moved[0], moved[1]), (moved[0] != moved[1]).sum().item()
+    assert bool(((moved[0] - moved[1]).abs() <= 2.0 ** -20 * moved[1].abs()).all())
 
 
 @pytest.mark.parametrize("size", [1e-36, 1e-30, 1e-22, 1e19, 1e25, 1e33])
