@@ -680,7 +680,8 @@ struct SmallShape {
     __host__ __device__ bool fits() const {
         const int blocks = side / 32;
         // (G itself, in fp32, takes 135168 bytes at most and four pieces per thread)
-        return lds() <= kSmallLds && blocks * waves_across() <= kSmallWaves && blocks * (blocks + 1) / 2 <= kSmallWaves;
+        // the counts first: beyond them lds() can pass 32 bits
+        return blocks * waves_across() <= kSmallWaves && blocks * (blocks + 1) / 2 <= kSmallWaves && lds() <= kSmallLds;
     }
 };
 
