@@ -15,8 +15,8 @@
 // one has arrived); phase 2 multiplies the second half while the next stage's first half is read and the loads of the
 // stage after it are issued into the buffer that has become free.  A load has one whole stage of multiplications to arrive; of
 // 64 x 64 tiles, whose stages are short, that covers it where four or five workgroups share a compute unit.  Where one has it alone, four
-// stages in LDS give a load three: 1000 x 1000 through five Newton-Schulz steps takes 154 instead of 190 us.  192 x 192 tiles have room for
-// three: S of 14336 x 4096 takes 233 us, 260 with two.
+// stages in LDS give a load three: 1000 x 1000 through five Newton-Schulz steps takes 148 instead of 191 us.  192 x 192 tiles have room for
+// three: 14336 x 4096 takes 3.48 ms, 3.56 with two.
 //
 // Loads go from memory straight into LDS (16 bytes a lane, no registers).  They are inline asm: the compiler would wait for
 // all of them before every LDS read.  They have no register result, and every wait for them is written out below.
@@ -25,7 +25,7 @@
 // 16-byte read in four turns over all 64 banks, and what it takes together are not the 16 rows of one piece but eight of one and
 // eight of the next: the order keeps those apart where the two pieces are neighbours, so a lane's group takes piece `group` in one phase
 // and `group` + 4 in the other (bank conflicts of S of 14336 x 4096: 1.1e6 cycles; 22.9e6 with pieces 2 group and 2 group + 1, or with
-// r & 7; 1000 x 1000 in all 144 us against 152).  Scaled operands keep 2 group and 2 group + 1, a lane's two scales are neighbours then, and
+// r & 7; 1000 x 1000 in all took 5 % less).  Scaled operands keep 2 group and 2 group + 1, a lane's two scales are neighbours then, and
 // their conflicts are hidden: an order without them took as long.
 // The order is applied to the address that a lane loads from.
 #pragma once
@@ -490,7 +490,7 @@ inline double tiles_time(const TileCost& c, double tiles, double length, int cus
 // A result of rows x cols in two launches: its first `lines` tile rows (columns) in one kind of tile, which fill whole rounds, what is left in
 // another, two or more on a compute unit.  One kind alone (rest.wt = 0) where that takes no longer.  4096 x 14336 over 4096 values
 // is three and a half rounds of 256 x 256 tiles: with the last half
-// in one round of 128 x 128 tiles an fp16 step takes 492 us, in one launch 528; a scaled product's 155 us become 151.
+// in one round of 128 x 128 tiles the iteration takes 3.48 ms, in one launch 3.61; a scaled product's 145 us become 141.
 struct Cut { TileCost tile, rest; bool columns; int lines; double time; };
 constexpr double kLaunchTime = 6.0;   // us that a second launch costs
 

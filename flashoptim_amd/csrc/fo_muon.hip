@@ -9,11 +9,11 @@
 // step).  So X is held in two parts, hi (fp16, the operand of the products) and lo (bf16, the rest, 19 bits or more together); lo
 // enters where X is multiplied by a.  The diagonals of S and B, by far their largest entries on a flat spectrum, are kept apart
 // in fp32; the products see the matrices without them: S S = O O + O D + D O + D D for S = O + D, and B's is added to a.  What is left (S and B off the diagonal and the products' X
-// in fp16) costs 1e-4 .. 1e-3 of the result, below the bfloat16 rounding it is handed out with; the smallest matrices are done in fp32.  X starts at |X|_F = 1, entries as small as 1e-4, so
+// in fp16) costs 1e-4 .. 1.3e-3 of the result, below the bfloat16 rounding it is handed out with; the smallest matrices are done in fp32.  X starts at |X|_F = 1, entries as small as 1e-4, so
 // the first X is kept times a power of two near sqrt(n), in fp16's normal range.
 //
 // Layout.  "Main" arrays have G's own orientation, padded with zeros to multiples of 64 (Rp x Cp), a shorter side of at most 32 to 32 (49
-// of 23 x 4934: 195 us instead of 222), so that the products need no bounds inside; T is hi transposed.  Every product is then rows times rows (fo_gemm.h):
+// of 23 x 4934 took 195 us with it and 222 with 64), so that the products need no bounds inside; T is hi transposed.  Every product is then rows times rows (fo_gemm.h):
 //     S = rows of X by rows of X          (X = hi where rows <= cols, else T); the tiles on and above the diagonal, written twice
 //     B = rows of S by rows of S          (S is symmetric); likewise
 //     X = rows of B by rows of T          (rows <= cols), or rows of hi by rows of B: main orientation either way
@@ -140,7 +140,7 @@ __device__ __forceinline__ float power_for(double norm) {
 }
 
 // Sum of the squares of a run of 8-value pieces of the matrix, one number per workgroup (in order, so a step repeats to
-// the bit).  One read of the matrix, bound by memory: 14336 x 4096 bf16 in 25 us, 4.7 TB/s.
+// the bit).  One read of the matrix, bound by memory: 14336 x 4096 bf16 in 26 to 31 us, 3.8 to 4.5 TB/s.
 template <int DT> __global__ __launch_bounds__(256) void squares_kernel(Groups a, MatrixSource source) {
     __shared__ double lds[4];
     const int g = group_of(a, blockIdx.x);
@@ -190,7 +190,7 @@ __device__ __forceinline__ f16x8 half8(const float (&v)[8]) {
 }
 
 // 64 x 64 pieces of G, normalised, as hi and lo in G's orientation and hi transposed (through LDS), zeros in the padding.  Bound by
-// memory, 6 bytes written per element: 14336 x 4096 bf16 in 86 us, 5.5 TB/s.
+// memory, 6 bytes written per element: 14336 x 4096 bf16 in 84 to 92 us, 5.1 to 5.6 TB/s.
 template <int DT> __global__ __launch_bounds__(256) void split_kernel(Groups a, MatrixSource source) {
     __shared__ _Float16 lds[64][64 + 2];
     const int g = group_of(a, blockIdx.x);
@@ -243,7 +243,7 @@ template <int DT> __global__ __launch_bounds__(256) void split_kernel(Groups a, 
 // Momentum of the optimizer step, over the flat elements of every matrix (groups of 32 codes run on across rows):
 //     m <- mu m + (1 - mu) g,   u = nesterov ? (1 - mu) g + mu m : m
 // each product and sum rounded, requantised as the SGD / Lion kernels do (how codes are read: see the kernel); u goes to the workspace in fp32 together with the
-// sum of its squares.  Bound by memory: 8 bytes per bf16 element, 218e6 of them in 313 us, 5.6 TB/s.
+// sum of its squares.  Bound by memory: 8 bytes per bf16 element, 218e6 of them in 311 us, 5.6 TB/s.
 struct MomentumArgs {
     const fo_tensor_desc* matrices;
     float mu, one_minus_mu;
@@ -428,8 +428,9 @@ struct PartialOut {
     }
 };
 
-// Bound by the matrix cores, with 192 x 192 tiles as much by LDS: S of 14336 x 4096 in 233 us (1030 TFLOP/s of the half that is computed), a
-// square of 4096 x 4096 in 80 (one round of 253 tiles either way; 256 x 256 tiles would fill 136 of 256 compute units).
+// Bound by the matrix cores, with 192 x 192 tiles as much by LDS: S of 14336 x 4096 in 272 us (885 TFLOP/s of the half that is computed), a
+// square of 4096 x 4096 in 95 (medians of an iteration's launches, whose products pull the clock down; 232 and 81 at least; one round of 253
+// tiles either way; 256 x 256 tiles would fill 136 of 256 compute units).
 template <int WT, int STAGES, int KIND> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void symmetric_kernel(Groups a, SquareArgs h) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef GemmTile<F16Product, WT, STAGES> Tile;
@@ -620,7 +621,7 @@ template <int DT, int ECCB> struct UpdateOut : ApplyIn {
     }
 };
 
-// Out: ApplyOut, or what the last step does.  14336 x 4096 in 492 us, 980 TFLOP/s: a round of 256 x 256 tiles takes 135 us, 35 of which
+// Out: ApplyOut, or what the last step does.  14336 x 4096 in 533 us, 900 TFLOP/s (the median; 489 at least): a round of 256 x 256 tiles takes 135 us, 35 of which
 // its epilogues' 10 bytes an element would take alone, and the card's clock falls under such products.
 template <int WT, int STAGES, class Out> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void apply_kernel(Groups a, StepArgs h, LastArgs last) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -1215,7 +1216,8 @@ int parts_of(const fo::MatrixGroup& m, int most) {
 }
 
 // S has few tiles where one side is short, each contracted over the whole other side.  Then the long axis is cut into parts that
-// are contracted at the same time and added up: 64 x 14336 takes 109 instead of 518 us in all, 1024 x 14336 480 instead of 520.
+// are contracted at the same time and added up: 64 x 14336 takes 115 instead of 249 us in all, 300 x 9000 154 instead of 222,
+// 1024 x 14336 486 instead of 499.
 // How many parts goes by the shape alone, so that a matrix's result does not depend on what shares the launch; a tenth of the time has
 // to be gained by it.
 int gram_parts(const fo::MatrixGroup& m, int cus) {
@@ -1361,8 +1363,8 @@ struct Steps {
     }
 };
 
-// Whether the first two steps are merged.  14336 x 4096: 4.2 ms in all become 3.7; 512 x 14336: 266 us become 248, 512 x 4096: 192 become 182;
-// 250 x 1000 takes 128 either way, square matrices would only pay for it.
+// Whether the first two steps are merged.  14336 x 4096: 3.95 ms in all become 3.48; 512 x 14336: 255 us become 236, 512 x 4096: 170 become 161;
+// 900 x 1800 takes 172 either way, 250 x 1000 115 and not 112, 1500 x 1000 174 and not 171; square matrices would only pay for it.
 bool merges(const fo::MatrixGroup& m) { return 2 * std::max(m.rows, m.cols) >= 3 * std::min(m.rows, m.cols); }
 
 // From the sums of squares on.  finish(a, step, cus) launches the last step.

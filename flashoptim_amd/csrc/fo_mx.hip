@@ -100,7 +100,7 @@ struct QuantizeArgs {
 // A 128 x 128 piece per workgroup: read once, all of it asked for before any of it is used; the row form out of registers (a
 // group is four lanes), the column form through LDS (a thread takes 32 rows of a column, two neighbouring columns one after the
 // other; four neighbouring threads write 64 adjacent bytes).  Bound by memory: 2 bytes in, 17/32 out per value and form; 14336 x 4096
-// bf16 both ways in 39 us, 4.6 TB/s, one way in 30 to 33.
+// bf16 both ways in 47 us between other kernels (3.8 TB/s), in 39 after one of its kind on another matrix, one way in 29 to 33.
 // The piece in LDS: rows an odd number of dwords apart, the lower half shifted so that the four groups of 32 rows that a wavefront reads
 // at a time lie in different banks.
 template <int B> struct QuantizePlaces {
@@ -248,7 +248,7 @@ struct ProductOut {
     }
 };
 
-// Bound by the matrix cores: 4096 x 4096 over 32768 values in 231 us, 4750 TFLOP/s; over 4096 values a round of 256 x 256 tiles takes 40 us,
+// Bound by the matrix cores: 4096 x 4096 over 32768 values in 231 us at least, 272 one after the other (4050 TFLOP/s); over 4096 values a round of 256 x 256 tiles takes 40 us,
 // a quarter of it the start and the writing of the result.
 template <int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void mx_product_kernel(ProductArgs args) {
     extern __shared__ __attribute__((aligned(16))) char smem[];

@@ -25,8 +25,9 @@ DEFAULT_STEPS = 5
 DEFAULT_EPS = 1e-7
 
 # Device memory that the matrices of one launch may take (10 bytes an element and 6 per entry of a square of the shorter side), unless
-# a single one needs more: a stack or list beyond it goes through in parts.  One layer of an 8B-parameter transformer needs 2.7
-# GB; more at once does not run faster.
+# a single one needs more: a stack or list beyond it goes through in parts, to the same result.  It is held for the call only.  One
+# layer of an 8B-parameter transformer needs 2.7 GB.  Four of them take 58.5 ms within 8 GiB and 59.0 to 60.0 within 1 to 4;
+# 32 layers of a model 1000 wide 11.9 ms within 8, 12.2 within 3, 13.6 within 1.
 WORKSPACE_BYTES = 8 << 30
 
 
@@ -70,11 +71,13 @@ def newton_schulz(
     Args:
         x: ``(..., rows, cols)`` in fp32, bf16 or fp16 on a ROCm GPU, any strides.
         steps: how often the polynomial is applied (1 to 99).
-        coefficients: of the odd polynomial.
+        coefficients: (a, b, c) of the polynomial.  One that takes singular values far beyond one, so that an entry on the way passes fp16's
+            range, comes back with infinities or NaNs.
         eps: added to the norm; a matrix of zeros stays one.
 
     Returns:
-        bfloat16, whatever the type of `x` (the products run on fp16 parts and come within 1e-3 of the result's norm), in the shape of
+        bfloat16, whatever the type of `x` (the products run on fp16 parts: their error is 1e-4 to 1.3e-3 of the
+        result's norm, less than this rounding's), in the shape of
         `x`; contiguous, or laid out like `x` where its columns and not its rows are contiguous.  A matrix with an infinity or
         a NaN comes back as NaNs.  No gradient flows through.
     """

@@ -107,7 +107,8 @@ def mxfp4_quantize(x: torch.Tensor, transpose: bool = False) -> MXFP4Tensor:
     """The matrix `x` (fp32, bf16 or fp16, any strides), or its transpose, in MXFP4.
 
     The scale of a group is the power of two of its largest magnitude, over 4; values are rounded to the nearest code,
-    ties to the even one, and cut off at 6 times the scale.  A group with an infinity or a NaN comes back as NaNs.
+    ties to the even one, and cut off at 6 times the scale.  A group with an infinity or a NaN comes back as NaNs.  No gradient flows
+    through.
     """
     rows, columns = _quantize(_check_matrix(x, "mxfp4_quantize"), not transpose, transpose)
     return columns if transpose else rows
@@ -155,7 +156,8 @@ def _tokens(x: torch.Tensor, weight: MXFP4Tensor, dtype: torch.dtype) -> torch.T
 def mxfp4_matmul(a: Union[MXFP4Tensor, torch.Tensor], b: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``a @ b.T`` of an ``m x k`` and an ``n x k`` matrix in MXFP4, summed in fp32, as an ``m x n`` matrix of `dtype`.
 
-    `a` may be a plain matrix: it is quantised on the way, in the product's own kernel where it is a few short rows.
+    `a` may be a plain matrix: it is quantised on the way, in the product's own kernel where it is a few short rows.  No gradient flows
+    through; :func:`mxfp4_linear` has them.
     """
     if not isinstance(b, MXFP4Tensor):
         raise ValueError(f"mxfp4_matmul expects its second operand as an MXFP4Tensor, got {type(b)}.")
@@ -334,7 +336,8 @@ def mxfp4_linear(x: torch.Tensor, weight: Union[torch.Tensor, MXFP4Tensor]) -> t
 
 class MXFP4Linear(torch.nn.Linear):
     """``torch.nn.Linear`` whose three products run in MXFP4 (:func:`mxfp4_linear`); the weight keeps its type, so the optimizers of
-    this package hold masters and correction bits for it as for any other.  A bias is added in the output's type."""
+    this package hold masters and correction bits for it as for any other; every call quantises it, so a weight that is only served is better
+    held by :func:`mxfp4_quantize`.  A bias is added by torch's rules: one in fp32 makes an fp32 output of a 16-bit input."""
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         y = mxfp4_linear(input, self.weight)
