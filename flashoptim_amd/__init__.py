@@ -8,9 +8,11 @@ numerical work runs in hand-written HIP kernels (``flashoptim_amd/csrc``) reache
 from .optimizers import (
     FlashAdam,
     FlashAdamW,
+    FlashEmbedding,
     FlashLion,
     FlashMuon,
     FlashOptimizer,
+    FlashRMSNorm,
     FlashSGD,
     FlashSGDW,
     GradientReleaseHandle,
@@ -19,7 +21,9 @@ from .optimizers import (
     NumericsError,
     cast_model,
     compute_ecc_bits,
+    embedding,
     enable_gradient_release,
+    linear_cross_entropy,
     mxfp4_dequantize,
     mxfp4_linear,
     mxfp4_matmul,
@@ -27,6 +31,8 @@ from .optimizers import (
     mxfp4_quantize_both,
     newton_schulz,
     reconstruct_fp32_param,
+    rms_norm,
+    rms_norm_mxfp4,
 )
 
 __version__ = "0.1.0"
@@ -34,9 +40,11 @@ __version__ = "0.1.0"
 __all__ = [
     "FlashAdam",
     "FlashAdamW",
+    "FlashEmbedding",
     "FlashLion",
     "FlashMuon",
     "FlashOptimizer",
+    "FlashRMSNorm",
     "FlashSGD",
     "FlashSGDW",
     "GradientReleaseHandle",
@@ -45,7 +53,9 @@ __all__ = [
     "NumericsError",
     "cast_model",
     "compute_ecc_bits",
+    "embedding",
     "enable_gradient_release",
+    "linear_cross_entropy",
     "mxfp4_dequantize",
     "mxfp4_linear",
     "mxfp4_matmul",
@@ -53,4 +63,6 @@ __all__ = [
     "mxfp4_quantize_both",
     "newton_schulz",
     "reconstruct_fp32_param",
+    "rms_norm",
+    "rms_norm_mxfp4",
 ]

@@ -108,6 +108,17 @@ SIGNATURES = {
     "fo_mxfp4_form_bytes": (_i64, [_i64, _i64]),
     "fo_mxfp4_linear_forward": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _i64, _i64, _i64] + [_vp] * 4 + [_i64, _vp]),
     "fo_mxfp4_linear_backward": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _i64, _vp]),
+    "fo_rms_norm": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _i32, _f32] + [_vp] * 4),
+    "fo_rms_norm_mxfp4": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _i32, _f32] + [_vp] * 4),
+    "fo_rms_norm_backward_workspace": (_i64, [_i64, _i64]),
+    "fo_rms_norm_backward": (_i32, [_vp, _i32, _i64, _vp, _i32, _vp, _vp, _i32, _i64, _vp] + [_i64] * 3 + [_vp] * 4 + [_i64, _vp]),
+    "fo_embedding": (_i32, [_vp, _i32, _i64, _vp, _i32] + [_i64] * 3 + [_f32, _vp, _vp]),
+    "fo_embedding_backward_workspace": (_i64, [_i64] * 3),
+    "fo_embedding_backward": (_i32, [_vp, _i32, _i64, _vp, _i32] + [_i64] * 3 + [_f32, _i64, _vp, _vp, _i64, _vp]),
+    "fo_linear_cross_entropy_workspace": (_i64, [_i32] + [_i64] * 3),
+    "fo_linear_cross_entropy": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _i64, _i32, _f32, _vp, _vp, _vp, _i64, _vp]),
+    "fo_linear_cross_entropy_backward_workspace": (_i64, [_i32] + [_i64] * 3 + [_i32, _i32]),
+    "fo_linear_cross_entropy_backward": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _i64, _i32, _f32, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp]),
     "fo_muon_step": (_i32, [_vp, _vp, _i64, _i32, _i32, _i32, _f32, _f32, _i32, _i32, _vp, _f32, _vp, _i64, _vp]),
 }
 # include/flashoptim_hip_diag.h: exported by the diagnostics build only (libflashoptim_hip_diag.so, which also

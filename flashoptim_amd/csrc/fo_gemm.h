@@ -35,6 +35,7 @@
 namespace fo {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -67,6 +68,17 @@ template <int EB, int EPL> __device__ __forceinline__ void store_piece(const Pac
             static_assert(EB * EPL == 8, "8 or 16 bytes");
             *reinterpret_cast<FO_GLOBAL u32x2_any*>((FO_GLOBAL char*)p) = u32x2{d.w[0], d.w[1]};
         }
+    }
+}
+// Eight values from a row of type DT, the first `valid` of them there (the others read as zero).
+template <int DT> __device__ __forceinline__ void load_values(float (&v)[8], const void* p, int valid) {
+    constexpr int B = DTypeInfo<DT>::bytes, EPL = 16 / B;
+#pragma unroll
+    for (int part = 0; part < 8 / EPL; ++part) {
+        Pack<B, EPL> d;
+        load_piece<B, EPL>(d, (const char*)p + part * 16, valid - part * EPL);
+#pragma unroll
+        for (int k = 0; k < EPL; ++k) v[part * EPL + k] = widen<DT, EPL>(d, k);
     }
 }
 // Eight values as a piece of a row of type DT.
@@ -103,6 +115,14 @@ struct F16Product {
     typedef f16x8 Frag;
     template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int, int) {
         asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    }
+};
+
+struct Bf16Product {
+    static constexpr bool kScaled = false;
+    typedef bf16x8 Frag;
+    template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int, int) {
+        asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     }
 };
 

@@ -1,0 +1,705 @@
+// Cross entropy over a vocabulary straight from hidden states, without the logits in memory, and its gradients.
+//
+//   z = x W'      lse[i] = log sum_v exp(z[i][v])      loss[i] = lse[i] - (1 - e) z[i][t_i] - e mean_v z[i][v]      (0 for ignored targets)
+//   G[i][v] = f_i (exp(z[i][v] - lse[i]) - e / V - (1 - e) [v = t_i])        dx = G W        dW = G' x
+//
+// with f_i what the loss of row i is multiplied by on its way back, over the number of targets where the loss is a mean.
+//
+// Forward: a tile of z stays in a workgroup's accumulators; out go each row's maximum, its sum of exponentials relative to that, and the
+// target's logit where the tile holds it: 8 bytes for a row of a wavefront's part of the tile.  Another launch joins the parts.
+// Backward: a piece of the vocabulary at a time.  The piece's logits are computed again (a product more, and nothing of tokens x vocabulary size kept
+// from the forward pass), turned into G in the same accumulators and written as rows and as columns, 16 bits a value; then one product adds
+// G's share to dx (fp32 sums between pieces), another makes the piece's rows of dW, complete.
+//
+// Types.  bf16 and fp16 operands go into the matrix cores as they are, sums are fp32.  G is rounded to the operands' type once, as the
+// other operand of its products is; the factors f_i are first scaled by a power of two to at most 1 (fp16: 2^15, so that probabilities down to 2^-39
+// survive), which the products' results are freed of at the end.  fp32 operands are cut into three bf16 parts of 8 bits each, a = a1 + a2 + a3
+// exactly, and the six products a1 b1, a1 b2, a1 b3, a2 b1, a2 b2, a3 b1 are one contraction over six times the length: what is left
+// out is below 2^-23 of a product.
+//
+// Rows of operands are whole multiples of 32 values, filled up with zeros: matrices that are so already are read in place, others are laid out
+// first.  Rows of ignored targets are left out of dW by zeros on both sides, so that what stands in them (infinities, NaN) does not matter.
+#include "fo_gemm.h"
+#include "fo_host.h"
+
+namespace fo {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kMinusInf = -__builtin_inff();
+constexpr int kIgnored = -1, kNone = -2;    // labels
+
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// ------------------------------------------------------------------------------------------- operands
+// Where eight neighbouring values of a row go, as the matrix instructions' operands have them.  PARTS = 1: the values; 6: the three parts of
+// each, in the order that this side of the product needs, `length` values apart.
+template <int DT> struct OperandOf {
+    static constexpr int kParts = 1;
+    template <bool RIGHT> __device__ __forceinline__ static void store(const float (&v)[8], char* p, int64_t) { store_values<DT>(v, p, 8); }
+};
+template <> struct OperandOf<DT_F32> {
+    static constexpr int kParts = 6;
+    template <bool RIGHT> __device__ __forceinline__ static void store(const float (&v)[8], char* p, int64_t length) {
+        u32x4 part[3];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            u32 lo[3], hi[3];
+            cut(v[2 * k], lo);
+            cut(v[2 * k + 1], hi);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) part[i][k] = __builtin_amdgcn_perm(hi[i], lo[i], 0x07060302u);
+        }
+        constexpr int kLeft[6] = {0, 0, 0, 1, 1, 2}, kRight[6] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+        for (int i = 0; i < 6; ++i) *reinterpret_cast<FO_GLOBAL u32x4*>((FO_GLOBAL char*)p + i * length * 2) = part[RIGHT ? kRight[i] : kLeft[i]];
+    }
+    // Eight bits of the significand at a time, cut off: nothing overflows, and the rest is exact.
+    __device__ __forceinline__ static void cut(float x, u32 (&part)[3]) {
+        part[0] = as_u32(x) & 0xffff0000u;
+        const bool finite = (as_u32(x) & 0x7f800000u) != 0x7f800000u;
+        if (!finite && x != x) part[0] |= 0x00400000u;
+        const float rest = finite ? x - as_f32(part[0]) : 0.0f;
+        part[1] = as_u32(rest) & 0xffff0000u;
+        part[2] = as_u32(rest - as_f32(part[1])) & 0xffff0000u;
+    }
+};
+
+struct FormArgs {
+    const char* x;
+    char* out;
+    const int* labels;        // rows of x whose label is kIgnored count as zeros; or null
+    int64_t stride;           // of x, in values
+    int rows, cols;           // of x
+    int length;               // of a part of an operand's row: what is contracted, filled up to a multiple of 32
+};
+// The rows of x, or (TURN) its columns, as operand rows.  64 x 64 values a workgroup.
+template <int DT, bool TURN, bool RIGHT> __global__ __launch_bounds__(256) void form_kernel(FormArgs a) {
+    constexpr int B = DTypeInfo<DT>::bytes;
+    const int across = (a.cols + 63) / 64;
+    const int row0 = (int)(blockIdx.x / across) * 64, col0 = (int)(blockIdx.x % across) * 64;
+    const int piece = threadIdx.x & 7, line = threadIdx.x >> 3;
+    float v[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = row0 + line + h * 32, c = col0 + piece * 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[h][k] = 0.0f;
+        if (r < a.rows && c < a.cols && !(a.labels && a.labels[r] == kIgnored)) load_values<DT>(v[h], a.x + (r * a.stride + c) * B, a.cols - c);
+    }
+    const int64_t row_bytes = (int64_t)a.length * OperandOf<DT>::kParts * 2;
+    if constexpr (!TURN) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = row0 + line + h * 32, c = col0 + piece * 8;
+            if (r < a.rows && c < a.length) OperandOf<DT>::template store<RIGHT>(v[h], a.out + r * row_bytes + c * 2, a.length);
+        }
+    } else {
+        __shared__ float tile[64][65];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) tile[line + h * 32][piece * 8 + k] = v[h][k];
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            // a wavefront takes eight columns, its lanes' pieces of one column are neighbours in memory
+            const int c = line + h * 32;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[h][k] = tile[piece * 8 + k][c];
+            if (col0 + c < a.cols && row0 + piece * 8 < a.length)
+                OperandOf<DT>::template store<RIGHT>(v[h], a.out + (col0 + c) * row_bytes + (row0 + piece * 8) * 2, a.length);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------- forward
+__global__ __launch_bounds__(256) void loss_labels_kernel(const void* targets, int bytes, int64_t n, int64_t vocabulary, int64_t ignore, int* labels) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int64_t t = bytes == 8 ? ((const int64_t*)targets)[i] : (int64_t)((const int32_t*)targets)[i];
+    labels[i] = t == ignore ? kIgnored : t >= 0 && t < vocabulary ? (int)t : kNone;
+}
+
+template <int CTRL> __device__ __forceinline__ float of_lane(float x) {
+    return as_f32((u32)__builtin_amdgcn_mov_dpp((int)as_u32(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float max_of_16(float x) {
+    x = fmaxf(x, of_lane<0xb1>(x));
+    x = fmaxf(x, of_lane<0x4e>(x));
+    x = fmaxf(x, of_lane<0x141>(x));
+    return fmaxf(x, of_lane<0x140>(x));
+}
+__device__ __forceinline__ float sum_of_16(float x) {
+    x += of_lane<0xb1>(x);
+    x += of_lane<0x4e>(x);
+    x += of_lane<0x141>(x);
+    return x + of_lane<0x140>(x);
+}
+
+struct LogitsArgs {
+    Operand x, weight;
+    int row_bytes;
+    const int* labels;
+    f32x2* stats;       // [part][row]: maximum, and sum of exponentials relative to it
+    float* sums;        // [part][row]: sum of logits, or null
+    float* picked;      // the target's logit
+};
+
+// What a grid of result tiles does first: which one is mine.
+template <class Tile> __device__ __forceinline__ bool my_tile(int rows, int cols, int& row0, int& col0) {
+    const int down = (rows + Tile::kTile - 1) / Tile::kTile, across = (cols + Tile::kTile - 1) / Tile::kTile;
+    const int64_t t = tile_of_seat(blockIdx.x & 7, blockIdx.x >> 3, (int64_t)down * across);
+    if (t < 0) return false;
+    int i, j;
+    tile_at((int)t, down, across, i, j);
+    row0 = i * Tile::kTile;
+    col0 = j * Tile::kTile;
+    return true;
+}
+
+template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void logits_kernel(LogitsArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typedef GemmTile<Product, WT, STAGES> Tile;
+    int row0, col0;
+    if (!my_tile<Tile>(a.x.rows, a.weight.rows, row0, col0)) return;
+    Tile tile(smem);
+    tile.multiply(a.x, a.weight, row0, col0, a.row_bytes);
+    const int rows = a.x.rows, cols = a.weight.rows;
+    const int r0 = row0 + (tile.wave >> 1) * WT + (tile.lane >> 4) * 4, part0 = col0 + (tile.wave & 1) * WT, mine = tile.lane & 15;
+    if (part0 >= cols) return;
+    const int64_t part = part0 / WT;
+#pragma unroll
+    for (int i = 0; i < Tile::kFrags; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = r0 + i * 16 + k;
+            float v[Tile::kFrags], most = kMinusInf;
+#pragma unroll
+            for (int j = 0; j < Tile::kFrags; ++j) {
+                v[j] = part0 + j * 16 + mine < cols ? tile.acc[i][j][k] : kMinusInf;
+                most = fmaxf(most, v[j]);
+            }
+            most = max_of_16(most);
+            const float base = most == kMinusInf ? 0.0f : most;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < Tile::kFrags; ++j) sum += exp_of(v[j] - base);
+            sum = sum_of_16(sum);
+            if (r < rows) {
+                const int at = a.labels[r] - part0;
+                if (at >= 0 && at < WT && (at & 15) == mine) {
+#pragma unroll
+                    for (int j = 0; j < Tile::kFrags; ++j)
+                        if (j == at >> 4) a.picked[r] = v[j];
+                }
+                if (mine == 0) a.stats[part * rows + r] = f32x2{most, sum};
+            }
+            if (a.sums) {
+                float all = 0.0f;
+#pragma unroll
+                for (int j = 0; j < Tile::kFrags; ++j) all += part0 + j * 16 + mine < cols ? v[j] : 0.0f;
+                all = sum_of_16(all);
+                if (mine == 0 && r < rows) a.sums[part * rows + r] = all;
+            }
+        }
+}
+
+struct JoinArgs {
+    const f32x2* stats;
+    const float *sums, *picked;
+    const int* labels;
+    float *lse, *loss;
+    int rows, parts;
+    float smoothing, vocabulary;
+};
+struct Exps {
+    float most, sum;
+    __device__ __forceinline__ void add(float m, float s) {
+        const float top = fmaxf(most, m), base = top == kMinusInf ? 0.0f : top;
+        sum = sum * exp_of(most - base) + s * exp_of(m - base);
+        most = top;
+    }
+};
+// Rows' parts joined: 64 rows a workgroup, each of 16 wavefronts every 16th part.
+__global__ __launch_bounds__(1024) void loss_join_kernel(JoinArgs a) {
+    __shared__ float most[16][64], sum[16][64], all[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x * 64 + lane;
+    Exps e{kMinusInf, 0.0f};
+    float logits = 0.0f;
+    if (row < a.rows) {
+#pragma unroll 4
+        for (int p = wave; p < a.parts; p += 16) {
+            const f32x2 v = a.stats[(int64_t)p * a.rows + row];
+            e.add(v.x, v.y);
+            if (a.sums) logits += a.sums[(int64_t)p * a.rows + row];
+        }
+    }
+    most[wave][lane] = e.most;
+    sum[wave][lane] = e.sum;
+    all[wave][lane] = logits;
+    __syncthreads();
+    if (wave != 0 || row >= a.rows) return;
+    for (int w = 1; w < 16; ++w) {
+        e.add(most[w][lane], sum[w][lane]);
+        logits += all[w][lane];
+    }
+    const float lse = e.most + __builtin_logf(e.sum);
+    const int label = a.labels[row];
+    float loss = 0.0f;
+    if (label == kNone) loss = __builtin_nanf("");
+    else if (label != kIgnored) {
+        loss = lse - (a.smoothing > 0.0f ? (1.0f - a.smoothing) * a.picked[row] + a.smoothing * (logits / a.vocabulary) : a.picked[row]);
+    }
+    a.lse[row] = lse;
+    a.loss[row] = loss;
+}
+
+// The losses' sum, over their number where a mean is wanted; count: that number.
+__global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* losses, const int* labels, int64_t n, int reduction, float* loss, float* count) {
+    __shared__ double sums[16];
+    __shared__ int counts[16];
+    double sum = 0.0;
+    int kept = 0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        if (reduction != FO_REDUCE_NONE) sum += losses[i];
+        kept += labels[i] != kIgnored;
+    }
+    for (int d = 1; d < 64; d <<= 1) { sum += __shfl_xor(sum, d); kept += __shfl_xor(kept, d); }
+    if ((threadIdx.x & 63) == 0) { sums[threadIdx.x >> 6] = sum; counts[threadIdx.x >> 6] = kept; }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < 16; ++w) { sum += sums[w]; kept += counts[w]; }
+    if (reduction == FO_REDUCE_MEAN) loss[0] = (float)(sum / (double)kept);
+    if (reduction == FO_REDUCE_SUM) loss[0] = (float)sum;
+    count[0] = (float)kept;
+}
+
+// ------------------------------------------------------------------------------------------- backward
+// factors[i]: f_i times a power of two that brings the largest to `top` at most; scale[0]: that power's inverse.
+__global__ __launch_bounds__(1024) void loss_factors_kernel(const float* upstream, int64_t stride, const int* labels, int64_t n, int reduction, const float* count,
+                                                            float top, float* factors, float* scale) {
+    __shared__ float mosts[16];
+    const float share = reduction == FO_REDUCE_MEAN ? 1.0f / count[0] : 1.0f;
+    float most = 0.0f;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        const float f = fabsf(upstream[i * stride] * share);
+        if (labels[i] >= 0 && f < __builtin_inff()) most = fmaxf(most, f);
+    }
+    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+    if ((threadIdx.x & 63) == 0) mosts[threadIdx.x >> 6] = most;
+    __syncthreads();
+    most = mosts[0];
+    for (int w = 1; w < 16; ++w) most = fmaxf(most, mosts[w]);
+    // most <= 2^exponent
+    int exponent;
+    (void)__builtin_frexpf(most, &exponent);
+    if (most == 0.0f) exponent = 0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        const float f = __builtin_ldexpf(upstream[i * stride] * share, -exponent) * top;
+        factors[i] = labels[i] == kIgnored ? 0.0f : labels[i] == kNone ? __builtin_nanf("") : f;
+    }
+    if (threadIdx.x == 0) scale[0] = __builtin_ldexpf(1.0f / top, exponent);
+}
+
+struct GradArgs {
+    Operand x, weight;     // of a piece of the vocabulary
+    int row_bytes;
+    const int* labels;
+    const float *lse, *factors;
+    char *grad, *turned;   // G as operand rows over the piece, its transpose as operand rows over the tokens; either may be null
+    int grad_length, turned_length;    // of a part of their rows
+    int first;             // the piece's first token of the vocabulary
+    float kept, even;      // 1 - e, e / V
+};
+template <int DT> struct GradOut {
+    static constexpr bool kColumns = true;
+    const GradArgs& a;
+    struct In { float lse, factor; int label; };
+    __device__ __forceinline__ void begin(int) const {}
+    __device__ __forceinline__ void load(int i, int, In& in) const {
+        if (i < a.x.rows) in = {a.lse[i], a.factors[i], a.labels[i]};
+    }
+    __device__ __forceinline__ bool columns() const { return a.turned != nullptr; }
+    __device__ __forceinline__ void row(int i, int j, In in, float (&v)[8]) const {
+        const bool zero = i >= a.x.rows || in.label == kIgnored;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float g = exp_of(v[k] - in.lse) - a.even;
+            if (a.first + j + k == in.label) g -= a.kept;
+            v[k] = zero || j + k >= a.weight.rows ? 0.0f : g * in.factor;
+        }
+        if (a.grad && i < a.x.rows && j < a.grad_length)
+            OperandOf<DT>::template store<false>(v, a.grad + ((int64_t)i * a.grad_length * OperandOf<DT>::kParts + j) * 2, a.grad_length);
+    }
+    __device__ __forceinline__ void column(int i, int j, const float (&w)[8]) const {
+        if (j < a.weight.rows && i < a.turned_length)
+            OperandOf<DT>::template store<false>(w, a.turned + ((int64_t)j * a.turned_length * OperandOf<DT>::kParts + i) * 2, a.turned_length);
+    }
+};
+template <int DT, class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void grad_kernel(GradArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typedef GemmTile<Product, WT, STAGES> Tile;
+    int row0, col0;
+    if (!my_tile<Tile>(a.x.rows, a.weight.rows, row0, col0)) return;
+    Tile tile(smem);
+    tile.multiply(a.x, a.weight, row0, col0, a.row_bytes);
+    GradOut<DT> out{a};
+    tile.finish(row0, col0, out);
+}
+
+struct GradProductArgs {
+    Operand left, right;
+    int row_bytes;
+    const float* more;     // what is added, fp32, as far apart as out's rows; or null
+    float* sums;           // fp32 result that goes on; or
+    char* out;             // the last one, of type `dtype`, times scale[0]
+    const float* scale;
+    int64_t stride;
+    int dtype;
+};
+struct GradProductOut {
+    static constexpr bool kColumns = false;
+    const GradProductArgs& a;
+    float scale;
+    struct In { f32x4 lo, hi; };
+    __device__ __forceinline__ void begin(int) { scale = a.out ? a.scale[0] : 1.0f; }
+    __device__ __forceinline__ void load(int i, int j, In& in) const {
+        in.lo = in.hi = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (!a.more || i >= a.left.rows || j >= a.right.rows) return;
+        float v[8];
+        load_values<DT_F32>(v, a.more + i * a.stride + j, a.right.rows - j);
+        in.lo = f32x4{v[0], v[1], v[2], v[3]};
+        in.hi = f32x4{v[4], v[5], v[6], v[7]};
+    }
+    __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
+        if (i >= a.left.rows || j >= a.right.rows) return;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { v[k] += in.lo[k]; v[4 + k] += in.hi[k]; }
+        const int64_t at = i * a.stride + j;
+        const int valid = a.right.rows - j;
+        if (!a.out) { store_values<DT_F32>(v, a.sums + at, valid); return; }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= scale;
+        if (a.dtype == DT_BF16) store_values<DT_BF16>(v, a.out + at * 2, valid);
+        else if (a.dtype == DT_F16) store_values<DT_F16>(v, a.out + at * 2, valid);
+        else store_values<DT_F32>(v, a.out + at * 4, valid);
+    }
+};
+template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void grad_product_kernel(GradProductArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typedef GemmTile<Product, WT, STAGES> Tile;
+    int row0, col0;
+    if (!my_tile<Tile>(a.left.rows, a.right.rows, row0, col0)) return;
+    Tile tile(smem);
+    tile.multiply(a.left, a.right, row0, col0, a.row_bytes);
+    GradProductOut out{a, 1.0f};
+    tile.finish(row0, col0, out);
+}
+
+}  // namespace fo
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+namespace {
+using namespace fo_host;
+
+constexpr int64_t kMostWorkgroups = 1 << 22;
+constexpr int64_t kMostTokens = 1 << 20, kMostCols = 1 << 16, kMostVocabulary = 1 << 24;    // 32-bit offsets into a tile's rows
+constexpr int64_t kBlockTokens = 16384;          // rows of one forward launch: bounds the parts' memory
+constexpr int64_t kPieceValues = 1 << 27;        // of G, as rows and as columns: 256 MiB each in 16 bits
+
+// Times of tiles as measured for the iteration's products (fo_muon.hip), which are of the same kind.
+constexpr fo::TileCost kTileCosts[] = {
+    {128, 2, 1, 14.0, 0.0286, 14.0, 0.0286}, {96, 3, 1, 19.0, 0.0150, 19.0, 0.0150}, {64, 2, 2, 9.5, 0.0115, 8.0, 0.0165},
+    {32, 2, 5, 4.2, 0.0063, 7.0, 0.0110}, {32, 4, 2, 4.2, 0.0036, 7.0, 0.0058}};
+
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+int64_t aligned(int64_t bytes) { return round_up(bytes, 256); }
+int64_t length_of(int64_t n) { return round_up(n, 32); }
+int parts_of(int dtype) { return dtype == FO_F32 ? 6 : 1; }
+int64_t form_bytes(int dtype, int64_t rows, int64_t inner) { return aligned(rows * length_of(inner) * parts_of(dtype) * 2); }
+
+int validate(const char* what, int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
+    if (tokens < 0 || cols < 0 || vocabulary < 0) return fail(FO_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+    if (dtype < FO_F32 || dtype > FO_F16) return fail(FO_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+    if (tokens > kMostTokens || cols > kMostCols || vocabulary > kMostVocabulary)
+        return fail(FO_ERR_UNSUPPORTED, "%s: %lld tokens of %lld values over a vocabulary of %lld are too many", what, (long long)tokens, (long long)cols, (long long)vocabulary);
+    if (tokens == 0 || cols == 0 || vocabulary == 0) return fail(FO_ERR_UNSUPPORTED, "%s: an empty product", what);
+    return 0;
+}
+
+template <class K, class A> int launch(K kernel, int64_t grid, int threads, int lds, hipStream_t stream, const char* what, const A& args) {
+    if (grid > kMostWorkgroups) return fail(FO_ERR_UNSUPPORTED, "%s: %lld workgroups are more than one launch takes", what, (long long)grid);
+    if (lds > 65536) {
+        if (int rc = check_hip(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds), what)) return rc;
+    }
+    kernel<<<dim3((unsigned)grid), dim3(threads), lds, stream>>>(args);
+    return check_hip(hipGetLastError(), what);
+}
+
+// ---- products in tiles of a size that suits the result
+fo::TileCost tile_for(int64_t rows, int64_t cols, double inner, int cus) {
+    fo::TileCost best{};
+    double least = 0.0;
+    for (const fo::TileCost& t : kTileCosts) {
+        const double time = fo::tiles_time(t, (double)fo::tiles_of(rows, cols, t.wt), inner, cus);
+        if (!best.wt || time < least) { best = t; least = time; }
+    }
+    return best;
+}
+
+template <class Product> struct LogitsLaunch {
+    typedef fo::LogitsArgs Args;
+    template <int WT, int STAGES> static auto kernel() { return fo::logits_kernel<Product, WT, STAGES>; }
+    template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES>::kLds; }
+    static int64_t rows(const Args& a) { return a.x.rows; }
+    static int64_t cols(const Args& a) { return a.weight.rows; }
+};
+template <int DT, class Product> struct GradLaunch {
+    typedef fo::GradArgs Args;
+    template <int WT, int STAGES> static auto kernel() { return fo::grad_kernel<DT, Product, WT, STAGES>; }
+    template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES>::kLds; }
+    static int64_t rows(const Args& a) { return a.x.rows; }
+    static int64_t cols(const Args& a) { return a.weight.rows; }
+};
+template <class Product> struct ProductLaunch {
+    typedef fo::GradProductArgs Args;
+    template <int WT, int STAGES> static auto kernel() { return fo::grad_product_kernel<Product, WT, STAGES>; }
+    template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES>::kLds; }
+    static int64_t rows(const Args& a) { return a.left.rows; }
+    static int64_t cols(const Args& a) { return a.right.rows; }
+};
+
+template <class L, int WT, int STAGES> int launch_tiles(const typename L::Args& a, hipStream_t s, const char* what) {
+    const int64_t tiles = fo::tiles_of(L::rows(a), L::cols(a), WT);
+    return launch(L::template kernel<WT, STAGES>(), 8 * fo::seats_of(tiles), 256, L::template lds<WT, STAGES>(), s, what, a);
+}
+template <class L> int launch_tiles(const fo::TileCost& t, const typename L::Args& a, hipStream_t s, const char* what) {
+    switch (t.wt) {
+        case 128: return launch_tiles<L, 128, 2>(a, s, what);
+        case 96: return launch_tiles<L, 96, 3>(a, s, what);
+        case 64: return launch_tiles<L, 64, 2>(a, s, what);
+        default: return t.stages == 4 ? launch_tiles<L, 32, 4>(a, s, what) : launch_tiles<L, 32, 2>(a, s, what);
+    }
+}
+
+// ---- operands
+struct Matrix {
+    const char* p;
+    int64_t stride, rows, cols;
+    int dtype;
+    int64_t width() const { return dtype == FO_F32 ? 4 : 2; }
+    Matrix part(int64_t first, int64_t n) const { return {p + first * stride * width(), stride, n, cols, dtype}; }
+    // Whether the rows are operand rows as they are.
+    bool ready() const { return dtype != FO_F32 && cols % 32 == 0 && stride % 8 == 0 && stride >= 0 && stride < (1 << 22) && ((uintptr_t)p & 15) == 0; }
+};
+fo::Operand operand(const void* p, int64_t row_bytes, int64_t rows) { return {(const char*)p, row_bytes, nullptr, 0, (int)rows}; }
+
+template <bool TURN, bool RIGHT> int form(const Matrix& m, const int* labels, void* out, hipStream_t s, const char* what) {
+    const fo::FormArgs a{m.p, (char*)out, labels, m.stride, (int)m.rows, (int)m.cols, (int)length_of(TURN ? m.rows : m.cols)};
+    const int64_t grid = ((m.rows + 63) / 64) * ((m.cols + 63) / 64);
+    switch (m.dtype) {
+        case FO_F32: return launch(fo::form_kernel<fo::DT_F32, TURN, RIGHT>, grid, 256, 0, s, what, a);
+        case FO_BF16: return launch(fo::form_kernel<fo::DT_BF16, TURN, RIGHT>, grid, 256, 0, s, what, a);
+        default: return launch(fo::form_kernel<fo::DT_F16, TURN, RIGHT>, grid, 256, 0, s, what, a);
+    }
+}
+// The rows of m as an operand, in place where they are one, else laid out at `space`.
+template <bool RIGHT> int rows_of(const Matrix& m, char* space, fo::Operand& to, hipStream_t s, const char* what) {
+    if (m.ready()) { to = operand(m.p, m.stride * 2, m.rows); return 0; }
+    to = operand(space, length_of(m.cols) * parts_of(m.dtype) * 2, m.rows);
+    return form<false, RIGHT>(m, nullptr, space, s, what);
+}
+
+template <class F> int by_product(int dtype, const F& f) {
+    if (dtype == FO_F32) return f.template run<fo::DT_F32, fo::Bf16Product>();
+    return dtype == FO_BF16 ? f.template run<fo::DT_BF16, fo::Bf16Product>() : f.template run<fo::DT_F16, fo::F16Product>();
+}
+
+int check_common(const char* what, const void* x, const void* weight, const void* targets, int index_bytes, int reduction, float smoothing, const void* workspace) {
+    if (!x || !weight || !targets) return fail(FO_ERR_INVALID_ARGUMENT, "%s: x, weight and targets must not be NULL", what);
+    if (index_bytes != 4 && index_bytes != 8) return fail(FO_ERR_INVALID_ARGUMENT, "%s: targets of %d bytes", what, index_bytes);
+    if (reduction < FO_REDUCE_NONE || reduction > FO_REDUCE_MEAN) return fail(FO_ERR_INVALID_ARGUMENT, "%s: unknown reduction %d", what, reduction);
+    if (!(smoothing >= 0.0f && smoothing <= 1.0f)) return fail(FO_ERR_INVALID_ARGUMENT, "%s: smoothing is between 0 and 1", what);
+    if (!workspace || (uintptr_t)workspace & 255) return fail(FO_ERR_INVALID_ARGUMENT, "%s: a workspace, aligned to 256 bytes, is needed", what);
+    return 0;
+}
+
+// ---- what a call keeps in its workspace.  Matrices that are operands in place leave their space unused.
+constexpr int kLeastPart = 32;    // columns of the smallest tile's wavefront
+struct ForwardSpace {
+    int64_t labels, picked, losses, stats, sums, x, weight, total;
+    ForwardSpace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
+        const int64_t rows = tokens < kBlockTokens ? tokens : kBlockTokens, parts = (vocabulary + kLeastPart - 1) / kLeastPart;
+        labels = 0;
+        picked = labels + aligned(tokens * 4);
+        losses = picked + aligned(tokens * 4);
+        stats = losses + aligned(tokens * 4);
+        sums = stats + aligned(rows * parts * 8);
+        x = sums + aligned(rows * parts * 4);
+        weight = x + form_bytes(dtype, rows, cols);
+        total = weight + form_bytes(dtype, vocabulary, cols);
+    }
+};
+
+struct BackwardSpace {
+    int64_t piece;    // tokens of the vocabulary at a time
+    int64_t labels, factors, scale, x, turned_x, weight, turned_weight, grad, turned_grad, sums, total;
+    BackwardSpace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, bool dx, bool dw) {
+        const int64_t most = round_up(kPieceValues / parts_of(dtype) / tokens + 1, 256);
+        const int64_t pieces = (vocabulary + most - 1) / most;
+        piece = round_up((vocabulary + pieces - 1) / pieces, 256);
+        if (piece > vocabulary) piece = vocabulary;
+        labels = 0;
+        factors = labels + aligned(tokens * 4);
+        scale = factors + aligned(tokens * 4);
+        x = scale + 256;
+        turned_x = x + form_bytes(dtype, tokens, cols);
+        weight = turned_x + (dw ? form_bytes(dtype, cols, tokens) : 0);
+        turned_weight = weight + form_bytes(dtype, piece, cols);
+        grad = turned_weight + (dx ? form_bytes(dtype, cols, piece) : 0);
+        turned_grad = grad + (dx ? form_bytes(dtype, tokens, piece) : 0);
+        sums = turned_grad + (dw ? form_bytes(dtype, piece, tokens) : 0);
+        total = sums + (dx && piece < vocabulary ? aligned(tokens * cols * 4) : 0);
+    }
+};
+
+struct Forward {
+    Matrix x, weight;
+    const void* targets;
+    int index_bytes, reduction;
+    int64_t ignore;
+    float smoothing;
+    float *loss, *kept;
+    char* base;
+    hipStream_t s;
+
+    template <int DT, class Product> int run() const {
+        const char* what = "fo_linear_cross_entropy";
+        const int cus = compute_units();
+        if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
+        const ForwardSpace at(x.dtype, x.rows, x.cols, weight.rows);
+        int* labels = (int*)(base + at.labels);
+        float* losses = reduction == FO_REDUCE_NONE ? loss : (float*)(base + at.losses);
+        fo::loss_labels_kernel<<<dim3((unsigned)((x.rows + 255) / 256)), dim3(256), 0, s>>>(targets, index_bytes, x.rows, weight.rows, ignore, labels);
+        if (int rc = check_hip(hipGetLastError(), what)) return rc;
+        fo::Operand w;
+        if (int rc = rows_of<true>(weight, base + at.weight, w, s, what)) return rc;
+        const int row_bytes = (int)(length_of(x.cols) * parts_of(x.dtype) * 2);
+        for (int64_t first = 0; first < x.rows; first += kBlockTokens) {
+            const Matrix some = x.part(first, x.rows - first < kBlockTokens ? x.rows - first : kBlockTokens);
+            fo::Operand rows;
+            if (int rc = rows_of<false>(some, base + at.x, rows, s, what)) return rc;
+            const fo::TileCost tile = tile_for(some.rows, weight.rows, row_bytes / 2, cus);
+            const fo::LogitsArgs a{rows, w, row_bytes, labels + first, (fo::f32x2*)(base + at.stats), smoothing > 0.0f ? (float*)(base + at.sums) : nullptr,
+                                   (float*)(base + at.picked) + first};
+            if (int rc = launch_tiles<LogitsLaunch<Product>>(tile, a, s, what)) return rc;
+            const fo::JoinArgs join{a.stats, a.sums, a.picked, a.labels, kept + first, losses + first, (int)some.rows, (int)((weight.rows + tile.wt - 1) / tile.wt),
+                                    smoothing, (float)weight.rows};
+            if (int rc = launch(fo::loss_join_kernel, (some.rows + 63) / 64, 1024, 0, s, what, join)) return rc;
+        }
+        fo::loss_reduce_kernel<<<dim3(1), dim3(1024), 0, s>>>(losses, labels, x.rows, reduction, loss, kept + x.rows);
+        return check_hip(hipGetLastError(), what);
+    }
+};
+
+struct Backward {
+    Matrix x, weight;
+    const void* targets;
+    int index_bytes, reduction;
+    int64_t ignore;
+    float smoothing;
+    const float *kept, *upstream;
+    int64_t upstream_stride;
+    char *dx, *dw, *base;
+    hipStream_t s;
+
+    template <int DT, class Product> int run() const {
+        const char* what = "fo_linear_cross_entropy_backward";
+        const int cus = compute_units();
+        if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
+        const BackwardSpace at(x.dtype, x.rows, x.cols, weight.rows, dx != nullptr, dw != nullptr);
+        const int parts = parts_of(x.dtype);
+        int* labels = (int*)(base + at.labels);
+        float *factors = (float*)(base + at.factors), *scale = (float*)(base + at.scale), *sums = (float*)(base + at.sums);
+        fo::loss_labels_kernel<<<dim3((unsigned)((x.rows + 255) / 256)), dim3(256), 0, s>>>(targets, index_bytes, x.rows, weight.rows, ignore, labels);
+        if (int rc = check_hip(hipGetLastError(), what)) return rc;
+        fo::loss_factors_kernel<<<dim3(1), dim3(1024), 0, s>>>(upstream, upstream_stride, labels, x.rows, reduction, kept + x.rows, x.dtype == FO_F16 ? 32768.0f : 1.0f,
+                                                               factors, scale);
+        if (int rc = check_hip(hipGetLastError(), what)) return rc;
+        fo::Operand rows;
+        if (int rc = rows_of<false>(x, base + at.x, rows, s, what)) return rc;
+        if (dw) {
+            if (int rc = form<true, true>(x, labels, base + at.turned_x, s, what)) return rc;
+        }
+        const int64_t tokens_length = length_of(x.rows);
+        for (int64_t first = 0; first < weight.rows; first += at.piece) {
+            const int64_t n = weight.rows - first < at.piece ? weight.rows - first : at.piece, length = length_of(n);
+            const bool last = first + n == weight.rows;
+            const Matrix some = weight.part(first, n);
+            fo::Operand w;
+            if (int rc = rows_of<true>(some, base + at.weight, w, s, what)) return rc;
+            const int row_bytes = (int)(length_of(x.cols) * parts * 2);
+            const fo::GradArgs grad{rows, w, row_bytes, labels, kept, factors, dx ? base + at.grad : nullptr, dw ? base + at.turned_grad : nullptr, (int)length,
+                                    (int)tokens_length, (int)first, 1.0f - smoothing, smoothing / (float)weight.rows};
+            if (int rc = launch_tiles<GradLaunch<DT, Product>>(tile_for(x.rows, n, row_bytes / 2, cus), grad, s, what)) return rc;
+            if (dx) {
+                if (int rc = form<true, true>(some, nullptr, base + at.turned_weight, s, what)) return rc;
+                const int64_t bytes = length * parts * 2;
+                const fo::GradProductArgs p{operand(base + at.grad, bytes, x.rows), operand(base + at.turned_weight, bytes, x.cols), (int)bytes, first ? sums : nullptr,
+                                            last ? nullptr : sums, last ? dx : nullptr, scale, x.cols, x.dtype};
+                if (int rc = launch_tiles<ProductLaunch<Product>>(tile_for(x.rows, x.cols, bytes / 2, cus), p, s, what)) return rc;
+            }
+            if (dw) {
+                const int64_t bytes = tokens_length * parts * 2;
+                const fo::GradProductArgs p{operand(base + at.turned_grad, bytes, n), operand(base + at.turned_x, bytes, x.cols), (int)bytes, nullptr, nullptr,
+                                            dw + first * x.cols * x.width(), scale, x.cols, x.dtype};
+                if (int rc = launch_tiles<ProductLaunch<Product>>(tile_for(n, x.cols, bytes / 2, cus), p, s, what)) return rc;
+            }
+        }
+        return 0;
+    }
+};
+
+}  // namespace
+
+extern "C" {
+
+int64_t fo_linear_cross_entropy_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
+    if (int rc = validate("fo_linear_cross_entropy", dtype, tokens, cols, vocabulary)) return rc;
+    return ForwardSpace(dtype, tokens, cols, vocabulary).total;
+}
+
+int fo_linear_cross_entropy(const void* x, int dtype, int64_t tokens, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t vocabulary, int64_t cols,
+                            const void* targets, int index_bytes, int64_t ignore, int reduction, float smoothing, float* loss, float* kept, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+    const char* what = "fo_linear_cross_entropy";
+    if (int rc = validate(what, dtype, tokens, cols, vocabulary)) return rc;
+    if (int rc = check_common(what, x, weight, targets, index_bytes, reduction, smoothing, workspace)) return rc;
+    if (!loss || !kept) return fail(FO_ERR_INVALID_ARGUMENT, "%s: loss and kept must not be NULL", what);
+    if (workspace_bytes < ForwardSpace(dtype, tokens, cols, vocabulary).total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+    const Forward f{{(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, targets, index_bytes, reduction,
+                    ignore, smoothing, loss, kept, (char*)workspace, (hipStream_t)stream};
+    return by_product(dtype, f);
+}
+
+int64_t fo_linear_cross_entropy_backward_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int want_dx, int want_dw) {
+    if (int rc = validate("fo_linear_cross_entropy_backward", dtype, tokens, cols, vocabulary)) return rc;
+    return BackwardSpace(dtype, tokens, cols, vocabulary, want_dx != 0, want_dw != 0).total;
+}
+
+int fo_linear_cross_entropy_backward(const void* x, int dtype, int64_t tokens, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t vocabulary,
+                                     int64_t cols, const void* targets, int index_bytes, int64_t ignore, int reduction, float smoothing, const float* kept,
+                                     const float* upstream, int64_t upstream_stride, void* dx, void* dw, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* what = "fo_linear_cross_entropy_backward";
+    if (int rc = validate(what, dtype, tokens, cols, vocabulary)) return rc;
+    if (int rc = check_common(what, x, weight, targets, index_bytes, reduction, smoothing, workspace)) return rc;
+    if (!kept || !upstream || (!dx && !dw)) return fail(FO_ERR_INVALID_ARGUMENT, "%s: kept, upstream and a result must be given", what);
+    if (workspace_bytes < BackwardSpace(dtype, tokens, cols, vocabulary, dx != nullptr, dw != nullptr).total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+    const Backward b{{(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, targets, index_bytes, reduction,
+                     ignore, smoothing, kept, upstream, upstream_stride, (char*)dx, (char*)dw, (char*)workspace, (hipStream_t)stream};
+    return by_product(dtype, b);
+}
+
+}  // extern "C"

@@ -10,6 +10,7 @@ from .base import (
     _log2_min_expressible_step_size,
 )
 from .cast import cast_model
+from .embed import FlashEmbedding, embedding
 from .kernels import (
     _fused_adam_step,
     _fused_momentum_step,
@@ -19,6 +20,7 @@ from .kernels import (
     reconstruct_fp32_param,
 )
 from .lion import FlashLion
+from .loss import linear_cross_entropy
 from .muon import FlashMuon, newton_schulz
 from .mxfp4 import (
     MXFP4Linear,
@@ -29,6 +31,7 @@ from .mxfp4 import (
     mxfp4_quantize,
     mxfp4_quantize_both,
 )
+from .norm import FlashRMSNorm, rms_norm, rms_norm_mxfp4
 from .release import GradientReleaseHandle, enable_gradient_release
 from .sgd import FlashSGD, FlashSGDW
 from .state import QuantizedTensorSpec, _MaybeQuantizedTensor
@@ -55,4 +58,10 @@ __all__ = [
     "mxfp4_quantize_both",
     "newton_schulz",
     "reconstruct_fp32_param",
+    "FlashEmbedding",
+    "FlashRMSNorm",
+    "embedding",
+    "linear_cross_entropy",
+    "rms_norm",
+    "rms_norm_mxfp4",
 ]

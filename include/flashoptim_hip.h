@@ -307,6 +307,67 @@ int fo_mxfp4_linear_backward(const void *dy, int dy_dtype, int64_t tokens, int64
                              const void *weight_columns, void *dx, int dx_dtype, void *dw, int dw_dtype, void *workspace,
                              int64_t workspace_bytes, void *stream);
 
+/*
+ * What stands between the linear layers of a language model and at its two ends (no counterpart in the reference).  Rows may lie any
+ * distance apart (strides in elements), their values are adjacent.
+ *
+ * Root-mean-square norm of the rows of s = x + residual (rounded to the residual's type and written to out_stream; s = x where
+ * residual is NULL):  y = s / sqrt(mean(s^2) + eps) * weight.  x and y are of x_dtype, residual and out_stream of stream_dtype (x_dtype or
+ * fp32), weight of any type or NULL (ones); y and out_stream are contiguous.  inverse (NULL, or `rows` fp32 numbers) gets
+ * 1 / sqrt(mean(s^2) + eps), which the backward pass takes.  The second form writes y in MXFP4, unrounded before, as fo_mxfp4_quantize
+ * lays it out.
+ */
+#define FO_RMS_NORM_MOST_COLS 32768
+int fo_rms_norm(const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t x_stride, const void *residual, int stream_dtype,
+                int64_t residual_stride, const void *weight, int weight_dtype, float eps, void *out_stream, void *y, float *inverse,
+                void *stream);
+int fo_rms_norm_mxfp4(const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t x_stride, const void *residual, int stream_dtype,
+                      int64_t residual_stride, const void *weight, int weight_dtype, float eps, void *out_stream, void *codes, void *scales,
+                      void *stream);
+
+/* Gradients.  s: the stream (x where there was no residual, stream_dtype = x_dtype then); dy of x_dtype; dstream: the gradient that the stream itself
+ * has, or NULL.  dx (x_dtype) and dresidual (stream_dtype), contiguous, get the same values, dw those of weight; any may be NULL.
+ * dw needs a workspace of fo_rms_norm_backward_workspace bytes of device memory, aligned to 16. */
+int64_t fo_rms_norm_backward_workspace(int64_t rows, int64_t cols);
+int fo_rms_norm_backward(const void *s, int stream_dtype, int64_t s_stride, const void *weight, int weight_dtype, const float *inverse,
+                         const void *dy, int x_dtype, int64_t dy_stride, const void *dstream, int64_t dstream_stride, int64_t rows,
+                         int64_t cols, void *dx, void *dresidual, void *dw, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Rows of an embedding matrix:  y[i] = scale * weight[tokens[i]], rounded once.  tokens: index_bytes 4 or 8 each, contiguous; weight:
+ * vocabulary x cols of `dtype`; y contiguous.  A token outside 0 .. vocabulary - 1 makes a row of NaNs.
+ * The gradient of the matrix (vocabulary x cols, contiguous):  dw[v] = scale * sum of dy[i] over the i with tokens[i] = v, in the order of i, in fp32,
+ * rounded once; rows of no token are zero, and so is row `padding` (-1: none); tokens outside the vocabulary are left out.
+ * workspace: fo_embedding_backward_workspace bytes of device memory, aligned to 256.
+ */
+#define FO_EMBEDDING_MOST 33554432 /* tokens, and rows of the matrix */
+int fo_embedding(const void *tokens, int index_bytes, int64_t n_tokens, const void *weight, int dtype, int64_t vocabulary, int64_t cols,
+                 int64_t weight_stride, float scale, void *y, void *stream);
+int64_t fo_embedding_backward_workspace(int64_t n_tokens, int64_t vocabulary, int64_t cols);
+int fo_embedding_backward(const void *tokens, int index_bytes, int64_t n_tokens, const void *dy, int dtype, int64_t dy_stride, int64_t vocabulary,
+                          int64_t cols, float scale, int64_t padding, void *dw, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Cross entropy of the logits x weight' (tokens x vocabulary, never in memory) against target tokens:
+ *     loss[i] = log sum exp(logits[i]) - (1 - smoothing) logits[i][target[i]] - smoothing mean(logits[i]),     0 where target[i] = ignore
+ * x: tokens x cols, weight: vocabulary x cols, both of `dtype`; targets: index_bytes 4 or 8 each, contiguous.  A target outside the
+ * vocabulary makes a NaN.
+ *   loss: fp32, `tokens` of them, or one: their sum or their sum over the number of targets that are not ignored
+ *   kept: tokens + 1 fp32 numbers that the backward pass takes: log sum exp of each row, and that number
+ * Backward: upstream: the loss's gradient, fp32, upstream_stride elements apart (0: one for all); dx (tokens x cols) and dw (vocabulary
+ * x cols) of `dtype`, contiguous, either may be NULL.  workspace: device memory, aligned to 256.
+ */
+enum fo_reduction { FO_REDUCE_NONE = 0, FO_REDUCE_SUM = 1, FO_REDUCE_MEAN = 2 };
+int64_t fo_linear_cross_entropy_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary);
+int fo_linear_cross_entropy(const void *x, int dtype, int64_t tokens, int64_t x_stride, const void *weight, int64_t weight_stride,
+                            int64_t vocabulary, int64_t cols, const void *targets, int index_bytes, int64_t ignore, int reduction,
+                            float smoothing, float *loss, float *kept, void *workspace, int64_t workspace_bytes, void *stream);
+int64_t fo_linear_cross_entropy_backward_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int want_dx, int want_dw);
+int fo_linear_cross_entropy_backward(const void *x, int dtype, int64_t tokens, int64_t x_stride, const void *weight, int64_t weight_stride,
+                                     int64_t vocabulary, int64_t cols, const void *targets, int index_bytes, int64_t ignore, int reduction,
+                                     float smoothing, const float *kept, const float *upstream, int64_t upstream_stride, void *dx, void *dw,
+                                     void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,101 @@
+"""What the embedding, the norm and the loss refuse before any device work, through their C entry points and through Python."""
+
+import pytest
+import torch
+
+import flashoptim_amd as fo
+from flashoptim_amd import _native
+
+INVALID, UNSUPPORTED = -1, -2
+SOME = 1 << 20    # an address that no call here gets to use
+NAN = float("nan")
+
+
+def test_norm_checks_its_arguments():
+    lib = _native.lib()
+
+    def call(x=SOME, x_dtype=1, rows=3, cols=5, residual=SOME, stream_dtype=1, weight=SOME, weight_dtype=0, eps=1e-6, out=SOME, y=SOME):
+        return lib.fo_rms_norm(x, x_dtype, rows, cols, cols, residual, stream_dtype, cols, weight, weight_dtype, eps, out, y, None, None)
+
+    def packed(scales=SOME, codes=SOME, **kw):
+        a = {**dict(x=SOME, x_dtype=1, rows=3, cols=5, eps=1e-6), **kw}
+        return lib.fo_rms_norm_mxfp4(a["x"], a["x_dtype"], a["rows"], a["cols"], a["cols"], None, 0, 0, None, 0, a["eps"], None, codes, scales, None)
+
+    for bad in (dict(rows=-1), dict(cols=-1), dict(x_dtype=3), dict(x_dtype=-1), dict(stream_dtype=7), dict(weight_dtype=3), dict(eps=-1.0), dict(eps=NAN), dict(x=None), dict(y=None),
+                dict(out=None)):
+        assert call(**bad) == INVALID, bad
+        assert lib.fo_last_error()
+    assert call(stream_dtype=2) == UNSUPPORTED and call(cols=32769) == UNSUPPORTED and call(rows=1 << 31) == UNSUPPORTED
+    assert call(rows=0, x=None, y=None) == 0 and call(cols=0, x=None, y=None) == 0
+    for bad in (dict(scales=None), dict(codes=None), dict(codes=SOME + 8), dict(x=None), dict(x_dtype=4)):
+        assert packed(**bad) == INVALID, bad
+
+
+def test_norm_gradient_checks_its_arguments():
+    lib = _native.lib()
+
+    def call(s=SOME, stream_dtype=1, weight=SOME, weight_dtype=1, inverse=SOME, dy=SOME, x_dtype=1, rows=3, cols=5, dx=SOME, dresidual=None, dw=None):
+        return lib.fo_rms_norm_backward(s, stream_dtype, cols, weight, weight_dtype, inverse, dy, x_dtype, cols, None, 0, rows, cols, dx, dresidual, dw, None, 0, None)
+
+    for bad in (dict(s=None), dict(inverse=None), dict(dy=None), dict(dx=None), dict(rows=-1), dict(x_dtype=3), dict(weight=None, dw=SOME)):
+        assert call(**bad) == INVALID, bad
+    assert call(stream_dtype=2) == UNSUPPORTED and call(rows=0, s=None) == 0
+    assert lib.fo_rms_norm_backward_workspace(-1, 5) == INVALID and lib.fo_rms_norm_backward_workspace(1, 32769) == UNSUPPORTED
+    assert lib.fo_rms_norm_backward_workspace(0, 5) == 0
+
+
+def test_embedding_checks_its_arguments():
+    lib = _native.lib()
+
+    def call(tokens=SOME, index=8, n=3, weight=SOME, dtype=1, vocabulary=7, cols=5, y=SOME):
+        return lib.fo_embedding(tokens, index, n, weight, dtype, vocabulary, cols, cols, 1.0, y, None)
+
+    def back(tokens=SOME, index=8, n=3, dy=SOME, dtype=1, vocabulary=7, cols=5, dw=SOME, workspace=SOME, size=1 << 30):
+        return lib.fo_embedding_backward(tokens, index, n, dy, dtype, cols, vocabulary, cols, 1.0, -1, dw, workspace, size, None)
+
+    for bad in (dict(index=2), dict(n=-1), dict(dtype=3), dict(vocabulary=-1), dict(cols=-1), dict(tokens=None)):
+        assert call(**bad) == INVALID and back(**bad) == INVALID, bad
+    assert call(weight=None) == INVALID and call(y=None) == INVALID
+    for bad in (dict(dy=None), dict(dw=None), dict(workspace=None), dict(workspace=SOME + 128), dict(size=10)):
+        assert back(**bad) == INVALID, bad
+    for large in (dict(n=(1 << 25) + 1), dict(vocabulary=(1 << 25) + 1), dict(cols=1 << 26)):
+        assert call(**large) == UNSUPPORTED and back(**large) == UNSUPPORTED, large
+    assert call(n=0, tokens=None) == 0 and back(vocabulary=0, dw=None) == 0
+    size = lib.fo_embedding_backward_workspace
+    assert size(-1, 1, 1) == INVALID and size(0, 1000, 8) == 4096
+    # keys, a second array of them from the second run on, starts, two rows a window once there are two windows
+    assert size(64, 10, 8) == 512 + 256 and size(512, 10, 8) == 4096 + 256 + 8 * 2 * 8 * 4 and size(513, 10, 8) == 2 * 4352 + 256 + 9 * 2 * 8 * 4 // 256 * 256 + 256
+
+
+def test_loss_checks_its_arguments():
+    lib = _native.lib()
+
+    def call(x=SOME, dtype=1, tokens=3, weight=SOME, vocabulary=7, cols=5, targets=SOME, index=8, reduction=2, smoothing=0.0, loss=SOME, kept=SOME, workspace=SOME, size=1 << 40):
+        return lib.fo_linear_cross_entropy(x, dtype, tokens, cols, weight, cols, vocabulary, cols, targets, index, -100, reduction, smoothing, loss, kept, workspace, size, None)
+
+    def back(x=SOME, dtype=1, tokens=3, weight=SOME, vocabulary=7, cols=5, targets=SOME, index=8, reduction=2, smoothing=0.0, kept=SOME, upstream=SOME, dx=SOME, workspace=SOME,
+             size=1 << 40):
+        return lib.fo_linear_cross_entropy_backward(x, dtype, tokens, cols, weight, cols, vocabulary, cols, targets, index, -100, reduction, smoothing, kept, upstream, 0, dx, None,
+                                                    workspace, size, None)
+
+    for bad in (dict(x=None), dict(dtype=3), dict(dtype=-1), dict(tokens=-1), dict(weight=None), dict(vocabulary=-1), dict(cols=-1), dict(targets=None), dict(index=1), dict(reduction=3),
+                dict(reduction=-1), dict(smoothing=-0.5), dict(smoothing=1.5), dict(smoothing=NAN), dict(kept=None), dict(workspace=None), dict(workspace=SOME + 64), dict(size=100)):
+        assert call(**bad) == INVALID and back(**bad) == INVALID, bad
+    assert call(loss=None) == INVALID and back(upstream=None) == INVALID and back(dx=None) == INVALID
+    for other in (dict(tokens=0), dict(cols=0), dict(vocabulary=0), dict(tokens=(1 << 20) + 1), dict(cols=65537), dict(vocabulary=(1 << 24) + 1)):
+        assert call(**other) == UNSUPPORTED and back(**other) == UNSUPPORTED, other
+    forward, backward = lib.fo_linear_cross_entropy_workspace, lib.fo_linear_cross_entropy_backward_workspace
+    assert forward(1, -1, 5, 7) == INVALID and forward(1, 0, 5, 7) == UNSUPPORTED and backward(5, 3, 5, 7, 1, 1) == INVALID
+    # a piece's gradient as rows and as columns, 2^27 values each, not the logits
+    logits = 8192 * 128256 * 2
+    assert backward(1, 8192, 4096, 128256, 1, 1) < logits and forward(1, 8192, 4096, 128256) < 2 * logits
+    assert backward(1, 8192, 4096, 128256, 1, 0) < backward(1, 8192, 4096, 128256, 1, 1) > backward(1, 8192, 4096, 128256, 0, 1)
+
+
+def test_without_a_gpu():
+    x = torch.zeros(3, 8)
+    for call in (lambda: fo.rms_norm(x), lambda: fo.rms_norm_mxfp4(x), lambda: fo.embedding(torch.zeros(2, dtype=torch.int64), x),
+                 lambda: fo.linear_cross_entropy(x, x, torch.zeros(3, dtype=torch.int64)), lambda: fo.FlashRMSNorm(8)(x),
+                 lambda: fo.FlashEmbedding(4, 8)(torch.zeros(2, dtype=torch.int64))):
+        with pytest.raises(NotImplementedError):
+            call()
