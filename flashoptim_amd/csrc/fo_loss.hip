@@ -12,10 +12,11 @@
 // G's share to dx (fp32 sums between pieces), another makes the piece's rows of dW, complete.
 //
 // Types.  bf16 and fp16 operands go into the matrix cores as they are, sums are fp32.  G is rounded to the operands' type once, as the
-// other operand of its products is; the factors f_i are first scaled by a power of two to at most 1 (fp16: 2^15, so that probabilities down to 2^-39
-// survive), which the products' results are freed of at the end.  fp32 operands are cut into three bf16 parts of 8 bits each, a = a1 + a2 + a3
-// exactly, and the six products a1 b1, a1 b2, a1 b3, a2 b1, a2 b2, a3 b1 are one contraction over six times the length: what is left
-// out is below 2^-23 of a product.
+// other operand of its products is; the factors f_i are first divided by the largest of them (and multiplied by 2^15 for fp16, so that probabilities down to 2^-39
+// survive), which the products' results are multiplied by at the end: where all are equal, as in a mean, they are 1, and the entry p - 1 of an unlikely
+// target rounds to almost itself.  fp32 operands are cut into three bf16 parts of 8 bits each, a = a1 + a2 + a3
+// exactly, and the six products a3 b1, a2 b2, a1 b3, a2 b1, a1 b2, a1 b1 are one contraction over six times the length: what is left
+// out is below 2^-23 of a product.  The small ones come first, so that the sums are small while most of the additions round.
 //
 // Rows of operands are whole multiples of 32 values, filled up with zeros: matrices that are so already are read in place, others are laid out
 // first.  Rows of ignored targets are left out of dW by zeros on both sides, so that what stands in them (infinities, NaN) does not matter.
@@ -49,7 +50,7 @@ template <> struct OperandOf<DT_F32> {
 #pragma unroll
             for (int i = 0; i < 3; ++i) part[i][k] = __builtin_amdgcn_perm(hi[i], lo[i], 0x07060302u);
         }
-        constexpr int kLeft[6] = {0, 0, 0, 1, 1, 2}, kRight[6] = {0, 1, 2, 0, 1, 0};
+        constexpr int kLeft[6] = {2, 1, 0, 1, 0, 0}, kRight[6] = {0, 1, 2, 0, 1, 0};
 #pragma unroll
         for (int i = 0; i < 6; ++i) *reinterpret_cast<FO_GLOBAL u32x4*>((FO_GLOBAL char*)p + i * length * 2) = part[RIGHT ? kRight[i] : kLeft[i]];
     }
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* losses, 
 }
 
 // ------------------------------------------------------------------------------------------- backward
-// factors[i]: f_i times a power of two that brings the largest to `top` at most; scale[0]: that power's inverse.
+// factors[i]: f_i over the largest magnitude among them, times `top` (a power of two); scale[0]: what that is to be multiplied by.
 __global__ __launch_bounds__(1024) void loss_factors_kernel(const float* upstream, int64_t stride, const int* labels, int64_t n, int reduction, const float* count,
                                                             float top, float* factors, float* scale) {
     __shared__ float mosts[16];
@@ -290,15 +291,12 @@ __global__ __launch_bounds__(1024) void loss_factors_kernel(const float* upstrea
     __syncthreads();
     most = mosts[0];
     for (int w = 1; w < 16; ++w) most = fmaxf(most, mosts[w]);
-    // most <= 2^exponent
-    int exponent;
-    (void)__builtin_frexpf(most, &exponent);
-    if (most == 0.0f) exponent = 0;
+    if (most == 0.0f) most = 1.0f;
     for (int64_t i = threadIdx.x; i < n; i += 1024) {
-        const float f = __builtin_ldexpf(upstream[i * stride] * share, -exponent) * top;
+        const float f = upstream[i * stride] * share / most * top;
         factors[i] = labels[i] == kIgnored ? 0.0f : labels[i] == kNone ? __builtin_nanf("") : f;
     }
-    if (threadIdx.x == 0) scale[0] = __builtin_ldexpf(1.0f / top, exponent);
+    if (threadIdx.x == 0) scale[0] = most / top;
 }
 
 struct GradArgs {

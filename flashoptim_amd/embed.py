@@ -5,13 +5,14 @@ The reference package has nothing of the kind.  ``torch.nn.Embedding``'s meaning
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
 import torch
 from torch.autograd import forward_ad
 
-from . import _native, kernels
+from . import _autograd, _native, kernels
 from ._native import DTYPE_CODE
 
 _INDEX_BYTES = {torch.int64: 8, torch.int32: 4}
@@ -46,6 +47,21 @@ def _plain(x: torch.Tensor) -> torch.Tensor:
     return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
 
 
+def _differentiable_once(backward):
+    """A backward pass without a derivative of its own: in a graph that records it, its results lead to an error."""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        error = torch._C._functions.DelayedError(b"trying to differentiate twice a function that has one derivative only", 1)
+        return tuple(o if o is None else error(o.detach().requires_grad_()) for o in out)
+
+    return wrapper
+
+
 def _lookup(tokens: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
     """tokens: flat.  Every argument is checked."""
     weight = _plain(weight)
@@ -69,7 +85,7 @@ class _Embedding(torch.autograd.Function):
         return _lookup(tokens, weight, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dy):
         (tokens,) = ctx.saved_tensors
         vocabulary, width = ctx.shape
@@ -107,6 +123,11 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
     Raises:
         NotImplementedError: no ROCm device, or a weight with a forward-mode tangent (there is no such derivative here).
     """
+    if _autograd.embedding is not None and (padding_idx is None or (isinstance(weight, torch.Tensor) and weight.dim() == 2 and 0 <= padding_idx < weight.shape[0])):
+        y = _autograd.embedding(tokens, weight, scale, -1 if padding_idx is None else padding_idx)
+        if y is not None:
+            return y
+    _autograd.bind()
     _check_values(weight, "embedding", "weight")
     if weight.dim() != 2:
         raise ValueError(f"embedding expects a matrix as weight, got shape {tuple(weight.shape)}.")

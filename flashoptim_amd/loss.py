@@ -8,9 +8,9 @@ from __future__ import annotations
 
 import torch
 
-from . import _native
+from . import _autograd, _native
 from ._native import DTYPE_CODE
-from .embed import _INDEX_BYTES, _check_tokens, _check_values, _plain
+from .embed import _INDEX_BYTES, _check_tokens, _check_values, _differentiable_once, _plain
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}  # fo_reduction
 
@@ -48,7 +48,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, upstream):
         x, weight, target, kept = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[:2]
@@ -95,6 +95,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     Raises:
         NotImplementedError: no ROCm device, or an operand with a forward-mode tangent (there is no such derivative here).
     """
+    if _autograd.linear_cross_entropy is not None and reduction in _REDUCTIONS:
+        loss = _autograd.linear_cross_entropy(x, weight, target, ignore_index, _REDUCTIONS[reduction], label_smoothing)
+        if loss is not None:
+            return loss
+    _autograd.bind()
     _check_values(x, "linear_cross_entropy", "x")
     _check_values(weight, "linear_cross_entropy", "weight")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:

@@ -10,9 +10,9 @@ from typing import Optional, Union
 
 import torch
 
-from . import _native
+from . import _autograd, _native
 from ._native import DTYPE_CODE
-from .embed import _check_values, _plain
+from .embed import _check_values, _differentiable_once, _plain
 from .mxfp4 import MXFP4Tensor, _empty
 
 
@@ -54,7 +54,7 @@ class _RMSNorm(torch.autograd.Function):
         return y if residual is None else (y, stream.view(x.shape))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dy, dstream=None):
         s, weight, inverse = ctx.saved_tensors
         need_dx, need_dw, need_dresidual, _ = ctx.needs_input_grad
@@ -133,6 +133,11 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
     Raises:
         NotImplementedError: no ROCm device, or an operand with a forward-mode tangent (there is no such derivative here).
     """
+    if _autograd.rms_norm is not None:
+        got = _autograd.rms_norm(x, weight, residual, eps)
+        if got is not None:
+            return got
+    _autograd.bind()
     eps = _check(x, weight, residual, eps, "rms_norm")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (residual is not None and residual.requires_grad)):
         return _RMSNorm.apply(x, weight, residual, eps)
@@ -147,6 +152,13 @@ def rms_norm_mxfp4(x: torch.Tensor, weight: Optional[torch.Tensor] = None, resid
     """:func:`rms_norm` of a matrix's rows with the output in MXFP4, as :func:`mxfp4_matmul` reads it: one launch in place of the norm and
     the quantiser, the output quantised from fp32.  No gradient flows through.
     """
+    if _autograd.rms_norm_mxfp4 is not None:
+        got = _autograd.rms_norm_mxfp4(x, weight, residual, eps)
+        if got is not None:
+            y = MXFP4Tensor.__new__(MXFP4Tensor)  # what is made here needs no check
+            y.codes, y.scales, y.shape = got[0], got[1], tuple(x.shape)
+            return y if residual is None else (y, got[2])
+    _autograd.bind()
     eps = _check(x, weight, residual, eps, "rms_norm_mxfp4")
     if x.dim() != 2:
         raise ValueError(f"rms_norm_mxfp4 expects a matrix, got shape {tuple(x.shape)}.")

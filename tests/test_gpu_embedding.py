@@ -17,6 +17,19 @@ HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16
 SMALLEST = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
 
 
+@pytest.fixture(params=["nodes", "python"], autouse=True)
+def host(request, monkeypatch):
+    """Every test through the C++ calls and nodes, and through the Python ones that stand in for them."""
+    from flashoptim_amd import _autograd
+
+    _autograd.bind()
+    assert _autograd.rms_norm and _autograd.rms_norm_mxfp4 and _autograd.embedding and _autograd.linear_cross_entropy
+    if request.param == "python":
+        for name in ("rms_norm", "rms_norm_mxfp4", "embedding", "linear_cross_entropy"):
+            monkeypatch.setattr(_autograd, name, None)
+    return request.param
+
+
 def _fo():
     import flashoptim_amd
 
@@ -220,3 +233,13 @@ def test_refusals():
     (dw,) = torch.autograd.grad(fo.embedding(tokens, weight).square().sum(), weight, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dw.sum(), weight)
+
+def test_one_derivative_only(host):
+    """A second one is refused, also where it is only a part of what is asked for, and whatever came in does not require a gradient."""
+    fo = _fo()
+    leaf = torch.randn(9, 40, device=DEV, requires_grad=True)
+    out = fo.embedding(torch.tensor([1, 2], device=DEV), leaf)
+    first = torch.autograd.grad(out, leaf, torch.ones_like(out), create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        (first.sum() + (leaf * leaf).sum()).backward()
+    assert (out.grad_fn.name() == "EmbeddingBackward") == (host == "nodes")

@@ -23,6 +23,19 @@ SMALLEST = {F32: 2.0 ** -149, BF16: 2.0 ** -133, F16: 2.0 ** -24}
 IGNORE = -100
 
 
+@pytest.fixture(params=["nodes", "python"], autouse=True)
+def host(request, monkeypatch):
+    """Every test through the C++ calls and nodes, and through the Python ones that stand in for them."""
+    from flashoptim_amd import _autograd
+
+    _autograd.bind()
+    assert _autograd.rms_norm and _autograd.rms_norm_mxfp4 and _autograd.embedding and _autograd.linear_cross_entropy
+    if request.param == "python":
+        for name in ("rms_norm", "rms_norm_mxfp4", "embedding", "linear_cross_entropy"):
+            monkeypatch.setattr(_autograd, name, None)
+    return request.param
+
+
 def _fo():
     import flashoptim_amd
 
@@ -331,3 +344,13 @@ def test_refusals():
     (dx,) = torch.autograd.grad(fo.linear_cross_entropy(leaf, w + 1.0, t), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dx.sum(), leaf)
+
+def test_one_derivative_only(host):
+    """A second one is refused, also where it is only a part of what is asked for, and whatever came in does not require a gradient."""
+    fo = _fo()
+    leaf = torch.randn(3, 40, device=DEV, requires_grad=True)
+    out = fo.linear_cross_entropy(leaf, torch.randn(9, 40, device=DEV), torch.tensor([1, 2, 8], device=DEV))
+    first = torch.autograd.grad(out, leaf, torch.ones_like(out), create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        (first.sum() + (leaf * leaf).sum()).backward()
+    assert (out.grad_fn.name() == "LinearCrossEntropyBackward") == (host == "nodes")

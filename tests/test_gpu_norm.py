@@ -22,6 +22,19 @@ SMALLEST = {F32: 2.0 ** -149, BF16: 2.0 ** -133, F16: 2.0 ** -24}
 WIDTHS = [1, 7, 8, 31, 128, 250, 512, 513, 2048, 2730, 4096, 4100, 8192, 8200, 16384, 16400, 32768]
 
 
+@pytest.fixture(params=["nodes", "python"], autouse=True)
+def host(request, monkeypatch):
+    """Every test through the C++ calls and nodes, and through the Python ones that stand in for them."""
+    from flashoptim_amd import _autograd
+
+    _autograd.bind()
+    assert _autograd.rms_norm and _autograd.rms_norm_mxfp4 and _autograd.embedding and _autograd.linear_cross_entropy
+    if request.param == "python":
+        for name in ("rms_norm", "rms_norm_mxfp4", "embedding", "linear_cross_entropy"):
+            monkeypatch.setattr(_autograd, name, None)
+    return request.param
+
+
 def _fo():
     import flashoptim_amd
 
@@ -275,3 +288,13 @@ def test_refusals():
     (dx,) = torch.autograd.grad(fo.rms_norm(leaf).square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dx.sum(), leaf)
+
+def test_one_derivative_only(host):
+    """A second one is refused, also where it is only a part of what is asked for, and whatever came in does not require a gradient."""
+    fo = _fo()
+    leaf, w = torch.randn(3, 40, device=DEV, requires_grad=True), torch.ones(40, device=DEV)
+    out = fo.rms_norm(leaf, w)
+    first = torch.autograd.grad(out, leaf, torch.ones_like(out), create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        (first.sum() + (leaf * leaf).sum()).backward()
+    assert (out.grad_fn.name() == "RMSNormBackward") == (host == "nodes")
