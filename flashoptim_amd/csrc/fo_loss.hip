@@ -67,15 +67,16 @@ template <> struct OperandOf<DT_F32> {
 
 struct FormArgs {
     const char* x;
-    char* out;
-    const int* labels;        // rows of x whose label is kIgnored count as zeros; or null
-    int64_t stride;           // of x, in values
-    int rows, cols;           // of x
-    int length;               // of a part of an operand's row: what is contracted, filled up to a multiple of 32
+    char *rows_out, *turned_out;          // the rows of x, and its columns, as operand rows; either may be null
+    const int* labels;                    // rows of x whose label is kIgnored count as zeros; or null
+    int64_t stride;                       // of x, in values
+    int rows, cols;                       // of x
+    int rows_length, turned_length;       // of a part of an operand's row: what is contracted, filled up to a multiple of 32
 };
-// The rows of x, or (TURN) its columns, as operand rows.  64 x 64 values a workgroup.
-template <int DT, bool TURN, bool RIGHT> __global__ __launch_bounds__(256) void form_kernel(FormArgs a) {
+// 64 x 64 values a workgroup, read once.  Bound by memory: the 16384 x 4096 bf16 rows of a piece of a weight turned in 64 us (4.2 TB/s).
+template <int DT, bool RIGHT> __global__ __launch_bounds__(256) void form_kernel(FormArgs a) {
     constexpr int B = DTypeInfo<DT>::bytes;
+    __shared__ float tile[64][65];
     const int across = (a.cols + 63) / 64;
     const int row0 = (int)(blockIdx.x / across) * 64, col0 = (int)(blockIdx.x % across) * 64;
     const int piece = threadIdx.x & 7, line = threadIdx.x >> 3;
@@ -87,39 +88,40 @@ template <int DT, bool TURN, bool RIGHT> __global__ __launch_bounds__(256) void 
         for (int k = 0; k < 8; ++k) v[h][k] = 0.0f;
         if (r < a.rows && c < a.cols && !(a.labels && a.labels[r] == kIgnored)) load_values<DT>(v[h], a.x + (r * a.stride + c) * B, a.cols - c);
     }
-    const int64_t row_bytes = (int64_t)a.length * OperandOf<DT>::kParts * 2;
-    if constexpr (!TURN) {
+    if (a.rows_out) {
+        const int64_t row_bytes = (int64_t)a.rows_length * OperandOf<DT>::kParts * 2;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int r = row0 + line + h * 32, c = col0 + piece * 8;
-            if (r < a.rows && c < a.length) OperandOf<DT>::template store<RIGHT>(v[h], a.out + r * row_bytes + c * 2, a.length);
+            if (r < a.rows && c < a.rows_length) OperandOf<DT>::template store<RIGHT>(v[h], a.rows_out + r * row_bytes + c * 2, a.rows_length);
         }
-    } else {
-        __shared__ float tile[64][65];
+    }
+    if (!a.turned_out) return;
+    const int64_t row_bytes = (int64_t)a.turned_length * OperandOf<DT>::kParts * 2;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) tile[line + h * 32][piece * 8 + k] = v[h][k];
-        __syncthreads();
+        for (int k = 0; k < 8; ++k) tile[line + h * 32][piece * 8 + k] = v[h][k];
+    __syncthreads();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            // a wavefront takes eight columns, its lanes' pieces of one column are neighbours in memory
-            const int c = line + h * 32;
+    for (int h = 0; h < 2; ++h) {
+        // a wavefront takes eight columns, its lanes' pieces of one column are neighbours in memory
+        const int c = line + h * 32;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[h][k] = tile[piece * 8 + k][c];
-            if (col0 + c < a.cols && row0 + piece * 8 < a.length)
-                OperandOf<DT>::template store<RIGHT>(v[h], a.out + (col0 + c) * row_bytes + (row0 + piece * 8) * 2, a.length);
-        }
+        for (int k = 0; k < 8; ++k) v[h][k] = tile[piece * 8 + k][c];
+        if (col0 + c < a.cols && row0 + piece * 8 < a.turned_length)
+            OperandOf<DT>::template store<true>(v[h], a.turned_out + (col0 + c) * row_bytes + (row0 + piece * 8) * 2, a.turned_length);
     }
 }
 
 // ------------------------------------------------------------------------------------------- forward
-__global__ __launch_bounds__(256) void loss_labels_kernel(const void* targets, int bytes, int64_t n, int64_t vocabulary, int64_t ignore, int* labels) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const int64_t t = bytes == 8 ? ((const int64_t*)targets)[i] : (int64_t)((const int32_t*)targets)[i];
-    labels[i] = t == ignore ? kIgnored : t >= 0 && t < vocabulary ? (int)t : kNone;
-}
+struct Targets {
+    const void* p;
+    int bytes;
+    __device__ __forceinline__ int64_t operator[](int64_t i) const {
+        return bytes == 8 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+    }
+};
 
 template <int CTRL> __device__ __forceinline__ float of_lane(float x) {
     return as_f32((u32)__builtin_amdgcn_mov_dpp((int)as_u32(x), CTRL, 0xf, 0xf, true));
@@ -140,7 +142,8 @@ __device__ __forceinline__ float sum_of_16(float x) {
 struct LogitsArgs {
     Operand x, weight;
     int row_bytes;
-    const int* labels;
+    Targets targets;    // of row `first` on
+    int64_t first;
     f32x2* stats;       // [part][row]: maximum, and sum of exponentials relative to it
     float* sums;        // [part][row]: sum of logits, or null
     float* picked;      // the target's logit
@@ -187,7 +190,7 @@ template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, W
             for (int j = 0; j < Tile::kFrags; ++j) sum += exp_of(v[j] - base);
             sum = sum_of_16(sum);
             if (r < rows) {
-                const int at = a.labels[r] - part0;
+                const int64_t at = a.targets[a.first + r] - part0;    // one that is ignored, or none, may be found too: nobody asks for it
                 if (at >= 0 && at < WT && (at & 15) == mine) {
 #pragma unroll
                     for (int j = 0; j < Tile::kFrags; ++j)
@@ -208,10 +211,12 @@ template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, W
 struct JoinArgs {
     const f32x2* stats;
     const float *sums, *picked;
-    const int* labels;
+    Targets targets;
+    int64_t first, ignore, vocabulary;
     float *lse, *loss;
+    int* labels;
     int rows, parts;
-    float smoothing, vocabulary;
+    float smoothing;
 };
 struct Exps {
     float most, sum;
@@ -221,38 +226,46 @@ struct Exps {
         most = top;
     }
 };
-// Rows' parts joined: 64 rows a workgroup, each of 16 wavefronts every 16th part.
-__global__ __launch_bounds__(1024) void loss_join_kernel(JoinArgs a) {
-    __shared__ float most[16][64], sum[16][64], all[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x * 64 + lane;
+// Rows' parts joined: ROWS rows a workgroup, each by 1024 / ROWS threads.  Few rows have many parts: five rows of 4008 parts take 44 us with 64 rows to a
+// workgroup, 6 with one.
+template <int ROWS> __global__ __launch_bounds__(1024) void loss_join_kernel(JoinArgs a) {
+    constexpr int kSlices = 1024 / ROWS;
+    __shared__ float most[1024], sum[1024], all[1024];
+    const int slice = threadIdx.x / ROWS, row = blockIdx.x * ROWS + threadIdx.x % ROWS;
     Exps e{kMinusInf, 0.0f};
     float logits = 0.0f;
     if (row < a.rows) {
 #pragma unroll 4
-        for (int p = wave; p < a.parts; p += 16) {
+        for (int p = slice; p < a.parts; p += kSlices) {
             const f32x2 v = a.stats[(int64_t)p * a.rows + row];
             e.add(v.x, v.y);
             if (a.sums) logits += a.sums[(int64_t)p * a.rows + row];
         }
     }
-    most[wave][lane] = e.most;
-    sum[wave][lane] = e.sum;
-    all[wave][lane] = logits;
-    __syncthreads();
-    if (wave != 0 || row >= a.rows) return;
-    for (int w = 1; w < 16; ++w) {
-        e.add(most[w][lane], sum[w][lane]);
-        logits += all[w][lane];
+#pragma unroll 1
+    for (int half = kSlices / 2; half > 0; half >>= 1) {    // the upper half of the slices that are left hands over to the lower
+        most[threadIdx.x] = e.most;
+        sum[threadIdx.x] = e.sum;
+        all[threadIdx.x] = logits;
+        __syncthreads();
+        if (slice < half) {
+            e.add(most[threadIdx.x + half * ROWS], sum[threadIdx.x + half * ROWS]);
+            logits += all[threadIdx.x + half * ROWS];
+        }
+        __syncthreads();
     }
+    if (slice != 0 || row >= a.rows) return;
     const float lse = e.most + __builtin_logf(e.sum);
-    const int label = a.labels[row];
+    const int64_t target = a.targets[a.first + row];
+    const int label = target == a.ignore ? kIgnored : target >= 0 && target < a.vocabulary ? (int)target : kNone;
     float loss = 0.0f;
     if (label == kNone) loss = __builtin_nanf("");
     else if (label != kIgnored) {
-        loss = lse - (a.smoothing > 0.0f ? (1.0f - a.smoothing) * a.picked[row] + a.smoothing * (logits / a.vocabulary) : a.picked[row]);
+        loss = lse - (a.smoothing > 0.0f ? (1.0f - a.smoothing) * a.picked[row] + a.smoothing * (logits / (float)a.vocabulary) : a.picked[row]);
     }
     a.lse[row] = lse;
     a.loss[row] = loss;
+    a.labels[row] = label;
 }
 
 // The losses' sum, over their number where a mean is wanted; count: that number.
@@ -262,7 +275,7 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* losses, 
     double sum = 0.0;
     int kept = 0;
     for (int64_t i = threadIdx.x; i < n; i += 1024) {
-        if (reduction != FO_REDUCE_NONE) sum += losses[i];
+        sum += losses[i];
         kept += labels[i] != kIgnored;
     }
     for (int d = 1; d < 64; d <<= 1) { sum += __shfl_xor(sum, d); kept += __shfl_xor(kept, d); }
@@ -270,8 +283,7 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* losses, 
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int w = 1; w < 16; ++w) { sum += sums[w]; kept += counts[w]; }
-    if (reduction == FO_REDUCE_MEAN) loss[0] = (float)(sum / (double)kept);
-    if (reduction == FO_REDUCE_SUM) loss[0] = (float)sum;
+    loss[0] = (float)(reduction == FO_REDUCE_MEAN ? sum / (double)kept : sum);
     count[0] = (float)kept;
 }
 
@@ -345,22 +357,31 @@ template <int DT, class Product, int WT, int STAGES> __global__ __launch_bounds_
     tile.finish(row0, col0, out);
 }
 
+// A product of operand rows; `parts` of the contraction may go to workgroups of their own, each with a result of its own in `sums`.
 struct GradProductArgs {
     Operand left, right;
-    int row_bytes;
+    int row_bytes, part_bytes, parts;
     const float* more;     // what is added, fp32, as far apart as out's rows; or null
-    float* sums;           // fp32 result that goes on; or
+    float* sums;           // fp32 results that go on; or
     char* out;             // the last one, of type `dtype`, times scale[0]
     const float* scale;
     int64_t stride;
     int dtype;
 };
+__device__ __forceinline__ void store_result(float (&v)[8], const GradProductArgs& a, int64_t at, int valid) {
+    const float scale = a.scale[0];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= scale;
+    if (a.dtype == DT_BF16) store_values<DT_BF16>(v, a.out + at * 2, valid);
+    else if (a.dtype == DT_F16) store_values<DT_F16>(v, a.out + at * 2, valid);
+    else store_values<DT_F32>(v, a.out + at * 4, valid);
+}
 struct GradProductOut {
     static constexpr bool kColumns = false;
     const GradProductArgs& a;
-    float scale;
+    int64_t part;
     struct In { f32x4 lo, hi; };
-    __device__ __forceinline__ void begin(int) { scale = a.out ? a.scale[0] : 1.0f; }
+    __device__ __forceinline__ void begin(int) const {}
     __device__ __forceinline__ void load(int i, int j, In& in) const {
         in.lo = in.hi = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (!a.more || i >= a.left.rows || j >= a.right.rows) return;
@@ -374,24 +395,52 @@ struct GradProductOut {
 #pragma unroll
         for (int k = 0; k < 4; ++k) { v[k] += in.lo[k]; v[4 + k] += in.hi[k]; }
         const int64_t at = i * a.stride + j;
-        const int valid = a.right.rows - j;
-        if (!a.out) { store_values<DT_F32>(v, a.sums + at, valid); return; }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] *= scale;
-        if (a.dtype == DT_BF16) store_values<DT_BF16>(v, a.out + at * 2, valid);
-        else if (a.dtype == DT_F16) store_values<DT_F16>(v, a.out + at * 2, valid);
-        else store_values<DT_F32>(v, a.out + at * 4, valid);
+        if (a.out) store_result(v, a, at, a.right.rows - j);
+        else store_values<DT_F32>(v, a.sums + part * a.left.rows * a.stride + at, a.right.rows - j);
     }
 };
 template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void grad_product_kernel(GradProductArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmTile<Product, WT, STAGES> Tile;
-    int row0, col0;
-    if (!my_tile<Tile>(a.left.rows, a.right.rows, row0, col0)) return;
+    const int down = (a.left.rows + Tile::kTile - 1) / Tile::kTile, across = (a.right.rows + Tile::kTile - 1) / Tile::kTile;
+    const int64_t t = tile_of_seat(blockIdx.x & 7, blockIdx.x >> 3, (int64_t)down * across * a.parts);
+    if (t < 0) return;
+    const int part = (int)(t / (down * across));
+    int i, j;
+    tile_at((int)(t - (int64_t)part * down * across), down, across, i, j);
+    const int64_t from = (int64_t)part * a.part_bytes;
+    Operand left = a.left, right = a.right;
+    left.data += from;
+    right.data += from;
     Tile tile(smem);
-    tile.multiply(a.left, a.right, row0, col0, a.row_bytes);
-    GradProductOut out{a, 1.0f};
-    tile.finish(row0, col0, out);
+    tile.multiply(left, right, i * Tile::kTile, j * Tile::kTile, part + 1 < a.parts ? a.part_bytes : (int)(a.row_bytes - from));
+    GradProductOut out{a, part};
+    tile.finish(i * Tile::kTile, j * Tile::kTile, out);
+}
+// The parts' results and `more`, added up in their order.  A thread takes eight values of a row.
+__global__ __launch_bounds__(256) void grad_join_kernel(GradProductArgs a, const float* partial) {
+    const int pieces = (a.right.rows + 7) / 8;
+    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, i = k / pieces;
+    const int j = (int)(k - i * pieces) * 8, valid = a.right.rows - j;
+    if (i >= a.left.rows) return;
+    const int64_t at = i * a.stride + j;
+    float sum[8];
+    load_values<DT_F32>(sum, partial + at, valid);
+#pragma unroll 8
+    for (int p = 1; p < a.parts; ++p) {
+        float v[8];
+        load_values<DT_F32>(v, partial + (int64_t)p * a.left.rows * a.stride + at, valid);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += v[e];
+    }
+    if (a.more) {
+        float v[8];
+        load_values<DT_F32>(v, a.more + at, valid);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += v[e];
+    }
+    if (a.out) store_result(sum, a, at, valid);
+    else store_values<DT_F32>(sum, a.sums + at, valid);
 }
 
 }  // namespace fo
@@ -402,15 +451,17 @@ template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, W
 namespace {
 using namespace fo_host;
 
-constexpr int64_t kMostWorkgroups = 1 << 22;
+constexpr int64_t kMostWorkgroups = (1 << 24) - 1;    // of 256 threads: a launch has less than 2^32 threads
 constexpr int64_t kMostTokens = 1 << 20, kMostCols = 1 << 16, kMostVocabulary = 1 << 24;    // 32-bit offsets into a tile's rows
 constexpr int64_t kBlockTokens = 16384;          // rows of one forward launch: bounds the parts' memory
 constexpr int64_t kPieceValues = 1 << 27;        // of G, as rows and as columns: 256 MiB each in 16 bits
 
-// Times of tiles as measured for the iteration's products (fo_muon.hip), which are of the same kind.
+// Times of bf16 tiles in logits_kernel and grad_product_kernel, which differ by a tenth, over 1024 and 4096 values: a 256 x 256 tile takes 42 and 109 us, 192 x 192
+// 29 and 72, two 128 x 128 on a compute unit 23 and 63 (alone 17 and 48), five 64 x 64 24 and 74 (alone 10 and 32; in four stages 9 and 19, two of
+// those 11 and 27).
 constexpr fo::TileCost kTileCosts[] = {
-    {128, 2, 1, 14.0, 0.0286, 14.0, 0.0286}, {96, 3, 1, 19.0, 0.0150, 19.0, 0.0150}, {64, 2, 2, 9.5, 0.0115, 8.0, 0.0165},
-    {32, 2, 5, 4.2, 0.0063, 7.0, 0.0110}, {32, 4, 2, 4.2, 0.0036, 7.0, 0.0058}};
+    {128, 2, 1, 20.0, 0.0216, 20.0, 0.0216}, {96, 3, 1, 15.0, 0.0137, 15.0, 0.0137}, {64, 2, 2, 6.8, 0.0099, 9.9, 0.0130},
+    {32, 2, 5, 3.2, 0.0071, 7.4, 0.0161}, {32, 4, 2, 4.6, 0.0034, 5.5, 0.0054}};
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t aligned(int64_t bytes) { return round_up(bytes, 256); }
@@ -447,12 +498,34 @@ fo::TileCost tile_for(int64_t rows, int64_t cols, double inner, int cus) {
     return best;
 }
 
+// A product of few tiles over a long contraction is cut along it: parts of whole stages, their fp32 results joined by another launch.  1003 x 1000 over
+// 32003 values: 157 us in 64 x 64 tiles, TODO in parts.
+struct Cut { fo::TileCost tile; int parts; int64_t part; double time; };
+constexpr int kMostParts = 32;
+constexpr int64_t kLeastPartValues = 512;
+Cut cut_for(int64_t rows, int64_t cols, int64_t inner, int cus) {
+    Cut best{};
+    for (const fo::TileCost& t : kTileCosts) {
+        const double tiles = (double)fo::tiles_of(rows, cols, t.wt);
+        for (int parts = 1; parts <= kMostParts; parts = parts < 4 ? parts + 1 : parts + parts / 2) {
+            if (parts > 1 && inner < parts * kLeastPartValues) break;
+            const int64_t part = round_up((inner + parts - 1) / parts, 64), used = (inner + part - 1) / part;
+            // the join reads and writes 4 bytes a value and part, at 4 TB/s, and is a launch
+            const double join = used > 1 ? 5.0 + (double)used * (double)(rows * cols) * 8e-6 / 4.0 : 0.0;
+            const double time = fo::tiles_time(t, tiles * (double)used, (double)part, cus) + join;
+            if (!best.parts || time < best.time) best = Cut{t, (int)used, part, time};
+        }
+    }
+    return best;
+}
+
 template <class Product> struct LogitsLaunch {
     typedef fo::LogitsArgs Args;
     template <int WT, int STAGES> static auto kernel() { return fo::logits_kernel<Product, WT, STAGES>; }
     template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES>::kLds; }
     static int64_t rows(const Args& a) { return a.x.rows; }
     static int64_t cols(const Args& a) { return a.weight.rows; }
+    static int64_t parts(const Args&) { return 1; }
 };
 template <int DT, class Product> struct GradLaunch {
     typedef fo::GradArgs Args;
@@ -460,6 +533,7 @@ template <int DT, class Product> struct GradLaunch {
     template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES>::kLds; }
     static int64_t rows(const Args& a) { return a.x.rows; }
     static int64_t cols(const Args& a) { return a.weight.rows; }
+    static int64_t parts(const Args&) { return 1; }
 };
 template <class Product> struct ProductLaunch {
     typedef fo::GradProductArgs Args;
@@ -467,10 +541,11 @@ template <class Product> struct ProductLaunch {
     template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES>::kLds; }
     static int64_t rows(const Args& a) { return a.left.rows; }
     static int64_t cols(const Args& a) { return a.right.rows; }
+    static int64_t parts(const Args& a) { return a.parts; }
 };
 
 template <class L, int WT, int STAGES> int launch_tiles(const typename L::Args& a, hipStream_t s, const char* what) {
-    const int64_t tiles = fo::tiles_of(L::rows(a), L::cols(a), WT);
+    const int64_t tiles = fo::tiles_of(L::rows(a), L::cols(a), WT) * L::parts(a);
     return launch(L::template kernel<WT, STAGES>(), 8 * fo::seats_of(tiles), 256, L::template lds<WT, STAGES>(), s, what, a);
 }
 template <class L> int launch_tiles(const fo::TileCost& t, const typename L::Args& a, hipStream_t s, const char* what) {
@@ -494,20 +569,33 @@ struct Matrix {
 };
 fo::Operand operand(const void* p, int64_t row_bytes, int64_t rows) { return {(const char*)p, row_bytes, nullptr, 0, (int)rows}; }
 
-template <bool TURN, bool RIGHT> int form(const Matrix& m, const int* labels, void* out, hipStream_t s, const char* what) {
-    const fo::FormArgs a{m.p, (char*)out, labels, m.stride, (int)m.rows, (int)m.cols, (int)length_of(TURN ? m.rows : m.cols)};
+// The rows of m as an operand: in place where they are one, else laid out at `space`; and its columns at `turned`, if that is given.  labels: see FormArgs.
+template <bool RIGHT> int operand_of(const Matrix& m, const int* labels, char* space, char* turned, fo::Operand& to, hipStream_t s, const char* what) {
+    const bool ready = m.ready();
+    to = ready ? operand(m.p, m.stride * 2, m.rows) : operand(space, length_of(m.cols) * parts_of(m.dtype) * 2, m.rows);
+    if (ready && !turned) return 0;
+    const fo::FormArgs a{m.p, ready ? nullptr : space, turned, labels, m.stride, (int)m.rows, (int)m.cols, (int)length_of(m.cols), (int)length_of(m.rows)};
     const int64_t grid = ((m.rows + 63) / 64) * ((m.cols + 63) / 64);
     switch (m.dtype) {
-        case FO_F32: return launch(fo::form_kernel<fo::DT_F32, TURN, RIGHT>, grid, 256, 0, s, what, a);
-        case FO_BF16: return launch(fo::form_kernel<fo::DT_BF16, TURN, RIGHT>, grid, 256, 0, s, what, a);
-        default: return launch(fo::form_kernel<fo::DT_F16, TURN, RIGHT>, grid, 256, 0, s, what, a);
+        case FO_F32: return launch(fo::form_kernel<fo::DT_F32, RIGHT>, grid, 256, 0, s, what, a);
+        case FO_BF16: return launch(fo::form_kernel<fo::DT_BF16, RIGHT>, grid, 256, 0, s, what, a);
+        default: return launch(fo::form_kernel<fo::DT_F16, RIGHT>, grid, 256, 0, s, what, a);
     }
 }
-// The rows of m as an operand, in place where they are one, else laid out at `space`.
-template <bool RIGHT> int rows_of(const Matrix& m, char* space, fo::Operand& to, hipStream_t s, const char* what) {
-    if (m.ready()) { to = operand(m.p, m.stride * 2, m.rows); return 0; }
-    to = operand(space, length_of(m.cols) * parts_of(m.dtype) * 2, m.rows);
-    return form<false, RIGHT>(m, nullptr, space, s, what);
+
+template <class Product> int product(fo::GradProductArgs a, const Cut& cut, float* partial, hipStream_t s, const char* what) {
+    a.parts = cut.parts;
+    a.part_bytes = (int)(cut.part * 2);
+    if (cut.parts == 1) return launch_tiles<ProductLaunch<Product>>(cut.tile, a, s, what);
+    fo::GradProductArgs some = a;
+    some.more = nullptr;
+    some.out = nullptr;
+    some.sums = partial;
+    if (int rc = launch_tiles<ProductLaunch<Product>>(cut.tile, some, s, what)) return rc;
+    const int64_t grid = ((int64_t)a.left.rows * ((a.right.rows + 7) / 8) + 255) / 256;
+    if (grid > kMostWorkgroups) return fail(FO_ERR_UNSUPPORTED, "%s: too large a result for one launch", what);
+    fo::grad_join_kernel<<<dim3((unsigned)grid), dim3(256), 0, s>>>(a, partial);
+    return check_hip(hipGetLastError(), what);
 }
 
 template <class F> int by_product(int dtype, const F& f) {
@@ -515,9 +603,14 @@ template <class F> int by_product(int dtype, const F& f) {
     return dtype == FO_BF16 ? f.template run<fo::DT_BF16, fo::Bf16Product>() : f.template run<fo::DT_F16, fo::F16Product>();
 }
 
-int check_common(const char* what, const void* x, const void* weight, const void* targets, int index_bytes, int reduction, float smoothing, const void* workspace) {
-    if (!x || !weight || !targets) return fail(FO_ERR_INVALID_ARGUMENT, "%s: x, weight and targets must not be NULL", what);
-    if (index_bytes != 4 && index_bytes != 8) return fail(FO_ERR_INVALID_ARGUMENT, "%s: targets of %d bytes", what, index_bytes);
+// Compute units to plan for; without a device those of this part, so that sizes can be asked for anywhere.
+int units() {
+    const int cus = compute_units();
+    return cus > 0 ? cus : 256;
+}
+
+int check_common(const char* what, const void* x, const void* weight, int reduction, float smoothing, const void* workspace) {
+    if (!x || !weight) return fail(FO_ERR_INVALID_ARGUMENT, "%s: x and weight must not be NULL", what);
     if (reduction < FO_REDUCE_NONE || reduction > FO_REDUCE_MEAN) return fail(FO_ERR_INVALID_ARGUMENT, "%s: unknown reduction %d", what, reduction);
     if (!(smoothing >= 0.0f && smoothing <= 1.0f)) return fail(FO_ERR_INVALID_ARGUMENT, "%s: smoothing is between 0 and 1", what);
     if (!workspace || (uintptr_t)workspace & 255) return fail(FO_ERR_INVALID_ARGUMENT, "%s: a workspace, aligned to 256 bytes, is needed", what);
@@ -527,12 +620,11 @@ int check_common(const char* what, const void* x, const void* weight, const void
 // ---- what a call keeps in its workspace.  Matrices that are operands in place leave their space unused.
 constexpr int kLeastPart = 32;    // columns of the smallest tile's wavefront
 struct ForwardSpace {
-    int64_t labels, picked, losses, stats, sums, x, weight, total;
+    int64_t picked, losses, stats, sums, x, weight, total;
     ForwardSpace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
         const int64_t rows = tokens < kBlockTokens ? tokens : kBlockTokens, parts = (vocabulary + kLeastPart - 1) / kLeastPart;
-        labels = 0;
-        picked = labels + aligned(tokens * 4);
-        losses = picked + aligned(tokens * 4);
+        picked = 0;
+        losses = picked + aligned(rows * 4);
         stats = losses + aligned(tokens * 4);
         sums = stats + aligned(rows * parts * 8);
         x = sums + aligned(rows * parts * 4);
@@ -543,14 +635,17 @@ struct ForwardSpace {
 
 struct BackwardSpace {
     int64_t piece;    // tokens of the vocabulary at a time
-    int64_t labels, factors, scale, x, turned_x, weight, turned_weight, grad, turned_grad, sums, total;
-    BackwardSpace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, bool dx, bool dw) {
+    int64_t factors, scale, x, turned_x, weight, turned_weight, grad, turned_grad, sums, partial, total;
+    Cut dx_cut, dw_cut;
+    BackwardSpace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, bool dx, bool dw, int cus) {
         const int64_t most = round_up(kPieceValues / parts_of(dtype) / tokens + 1, 256);
         const int64_t pieces = (vocabulary + most - 1) / most;
         piece = round_up((vocabulary + pieces - 1) / pieces, 256);
         if (piece > vocabulary) piece = vocabulary;
-        labels = 0;
-        factors = labels + aligned(tokens * 4);
+        // a last piece that is shorter goes by the same cuts: its parts are fewer
+        dx_cut = dx ? cut_for(tokens, cols, length_of(piece) * parts_of(dtype), cus) : Cut{};
+        dw_cut = dw ? cut_for(piece, cols, length_of(tokens) * parts_of(dtype), cus) : Cut{};
+        factors = 0;
         scale = factors + aligned(tokens * 4);
         x = scale + 256;
         turned_x = x + form_bytes(dtype, tokens, cols);
@@ -559,7 +654,9 @@ struct BackwardSpace {
         grad = turned_weight + (dx ? form_bytes(dtype, cols, piece) : 0);
         turned_grad = grad + (dx ? form_bytes(dtype, tokens, piece) : 0);
         sums = turned_grad + (dw ? form_bytes(dtype, piece, tokens) : 0);
-        total = sums + (dx && piece < vocabulary ? aligned(tokens * cols * 4) : 0);
+        partial = sums + (dx && piece < vocabulary ? aligned(tokens * cols * 4) : 0);
+        const int64_t of_dx = dx_cut.parts > 1 ? dx_cut.parts * tokens * cols : 0, of_dw = dw_cut.parts > 1 ? dw_cut.parts * piece * cols : 0;
+        total = partial + aligned((of_dx > of_dw ? of_dx : of_dw) * 4);
     }
 };
 
@@ -578,25 +675,28 @@ struct Forward {
         const int cus = compute_units();
         if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
         const ForwardSpace at(x.dtype, x.rows, x.cols, weight.rows);
-        int* labels = (int*)(base + at.labels);
+        int* labels = (int*)(kept + x.rows + 1);
+        const fo::Targets t{targets, index_bytes};
         float* losses = reduction == FO_REDUCE_NONE ? loss : (float*)(base + at.losses);
-        fo::loss_labels_kernel<<<dim3((unsigned)((x.rows + 255) / 256)), dim3(256), 0, s>>>(targets, index_bytes, x.rows, weight.rows, ignore, labels);
-        if (int rc = check_hip(hipGetLastError(), what)) return rc;
         fo::Operand w;
-        if (int rc = rows_of<true>(weight, base + at.weight, w, s, what)) return rc;
+        if (int rc = operand_of<true>(weight, nullptr, base + at.weight, nullptr, w, s, what)) return rc;
         const int row_bytes = (int)(length_of(x.cols) * parts_of(x.dtype) * 2);
         for (int64_t first = 0; first < x.rows; first += kBlockTokens) {
             const Matrix some = x.part(first, x.rows - first < kBlockTokens ? x.rows - first : kBlockTokens);
             fo::Operand rows;
-            if (int rc = rows_of<false>(some, base + at.x, rows, s, what)) return rc;
+            if (int rc = operand_of<false>(some, nullptr, base + at.x, nullptr, rows, s, what)) return rc;
             const fo::TileCost tile = tile_for(some.rows, weight.rows, row_bytes / 2, cus);
-            const fo::LogitsArgs a{rows, w, row_bytes, labels + first, (fo::f32x2*)(base + at.stats), smoothing > 0.0f ? (float*)(base + at.sums) : nullptr,
-                                   (float*)(base + at.picked) + first};
+            const fo::LogitsArgs a{rows, w, row_bytes, t, first, (fo::f32x2*)(base + at.stats), smoothing > 0.0f ? (float*)(base + at.sums) : nullptr, (float*)(base + at.picked)};
             if (int rc = launch_tiles<LogitsLaunch<Product>>(tile, a, s, what)) return rc;
-            const fo::JoinArgs join{a.stats, a.sums, a.picked, a.labels, kept + first, losses + first, (int)some.rows, (int)((weight.rows + tile.wt - 1) / tile.wt),
-                                    smoothing, (float)weight.rows};
-            if (int rc = launch(fo::loss_join_kernel, (some.rows + 63) / 64, 1024, 0, s, what, join)) return rc;
+            const fo::JoinArgs join{a.stats, a.sums, a.picked, t, first, ignore, weight.rows, kept + first, losses + first, labels + first, (int)some.rows,
+                                    (int)((weight.rows + tile.wt - 1) / tile.wt), smoothing};
+            int rc;
+            if (some.rows >= 64 * 128) rc = launch(fo::loss_join_kernel<64>, (some.rows + 63) / 64, 1024, 0, s, what, join);
+            else if (some.rows >= 64) rc = launch(fo::loss_join_kernel<8>, (some.rows + 7) / 8, 1024, 0, s, what, join);
+            else rc = launch(fo::loss_join_kernel<1>, some.rows, 1024, 0, s, what, join);
+            if (rc) return rc;
         }
+        if (reduction == FO_REDUCE_NONE) return 0;
         fo::loss_reduce_kernel<<<dim3(1), dim3(1024), 0, s>>>(losses, labels, x.rows, reduction, loss, kept + x.rows);
         return check_hip(hipGetLastError(), what);
     }
@@ -604,56 +704,48 @@ struct Forward {
 
 struct Backward {
     Matrix x, weight;
-    const void* targets;
-    int index_bytes, reduction;
-    int64_t ignore;
+    int reduction;
     float smoothing;
     const float *kept, *upstream;
     int64_t upstream_stride;
     char *dx, *dw, *base;
+    const BackwardSpace& at;
+    int cus;
     hipStream_t s;
 
     template <int DT, class Product> int run() const {
         const char* what = "fo_linear_cross_entropy_backward";
-        const int cus = compute_units();
-        if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
-        const BackwardSpace at(x.dtype, x.rows, x.cols, weight.rows, dx != nullptr, dw != nullptr);
         const int parts = parts_of(x.dtype);
-        int* labels = (int*)(base + at.labels);
-        float *factors = (float*)(base + at.factors), *scale = (float*)(base + at.scale), *sums = (float*)(base + at.sums);
-        fo::loss_labels_kernel<<<dim3((unsigned)((x.rows + 255) / 256)), dim3(256), 0, s>>>(targets, index_bytes, x.rows, weight.rows, ignore, labels);
-        if (int rc = check_hip(hipGetLastError(), what)) return rc;
+        const int* labels = (const int*)(kept + x.rows + 1);
+        float *factors = (float*)(base + at.factors), *scale = (float*)(base + at.scale), *sums = (float*)(base + at.sums), *partial = (float*)(base + at.partial);
         fo::loss_factors_kernel<<<dim3(1), dim3(1024), 0, s>>>(upstream, upstream_stride, labels, x.rows, reduction, kept + x.rows, x.dtype == FO_F16 ? 32768.0f : 1.0f,
                                                                factors, scale);
         if (int rc = check_hip(hipGetLastError(), what)) return rc;
         fo::Operand rows;
-        if (int rc = rows_of<false>(x, base + at.x, rows, s, what)) return rc;
-        if (dw) {
-            if (int rc = form<true, true>(x, labels, base + at.turned_x, s, what)) return rc;
-        }
+        if (int rc = operand_of<false>(x, labels, base + at.x, dw ? base + at.turned_x : nullptr, rows, s, what)) return rc;
         const int64_t tokens_length = length_of(x.rows);
+        const int row_bytes = (int)(length_of(x.cols) * parts * 2);
         for (int64_t first = 0; first < weight.rows; first += at.piece) {
             const int64_t n = weight.rows - first < at.piece ? weight.rows - first : at.piece, length = length_of(n);
             const bool last = first + n == weight.rows;
-            const Matrix some = weight.part(first, n);
             fo::Operand w;
-            if (int rc = rows_of<true>(some, base + at.weight, w, s, what)) return rc;
-            const int row_bytes = (int)(length_of(x.cols) * parts * 2);
+            if (int rc = operand_of<true>(weight.part(first, n), nullptr, base + at.weight, dx ? base + at.turned_weight : nullptr, w, s, what)) return rc;
             const fo::GradArgs grad{rows, w, row_bytes, labels, kept, factors, dx ? base + at.grad : nullptr, dw ? base + at.turned_grad : nullptr, (int)length,
                                     (int)tokens_length, (int)first, 1.0f - smoothing, smoothing / (float)weight.rows};
             if (int rc = launch_tiles<GradLaunch<DT, Product>>(tile_for(x.rows, n, row_bytes / 2, cus), grad, s, what)) return rc;
             if (dx) {
-                if (int rc = form<true, true>(some, nullptr, base + at.turned_weight, s, what)) return rc;
                 const int64_t bytes = length * parts * 2;
-                const fo::GradProductArgs p{operand(base + at.grad, bytes, x.rows), operand(base + at.turned_weight, bytes, x.cols), (int)bytes, first ? sums : nullptr,
+                Cut cut = at.dx_cut;
+                cut.parts = (int)((bytes / 2 + cut.part - 1) / cut.part);
+                const fo::GradProductArgs p{operand(base + at.grad, bytes, x.rows), operand(base + at.turned_weight, bytes, x.cols), (int)bytes, 0, 0, first ? sums : nullptr,
                                             last ? nullptr : sums, last ? dx : nullptr, scale, x.cols, x.dtype};
-                if (int rc = launch_tiles<ProductLaunch<Product>>(tile_for(x.rows, x.cols, bytes / 2, cus), p, s, what)) return rc;
+                if (int rc = product<Product>(p, cut, partial, s, what)) return rc;
             }
             if (dw) {
                 const int64_t bytes = tokens_length * parts * 2;
-                const fo::GradProductArgs p{operand(base + at.turned_grad, bytes, n), operand(base + at.turned_x, bytes, x.cols), (int)bytes, nullptr, nullptr,
+                const fo::GradProductArgs p{operand(base + at.turned_grad, bytes, n), operand(base + at.turned_x, bytes, x.cols), (int)bytes, 0, 0, nullptr, nullptr,
                                             dw + first * x.cols * x.width(), scale, x.cols, x.dtype};
-                if (int rc = launch_tiles<ProductLaunch<Product>>(tile_for(n, x.cols, bytes / 2, cus), p, s, what)) return rc;
+                if (int rc = product<Product>(p, at.dw_cut, partial, s, what)) return rc;
             }
         }
         return 0;
@@ -674,8 +766,9 @@ int fo_linear_cross_entropy(const void* x, int dtype, int64_t tokens, int64_t x_
                             int64_t workspace_bytes, void* stream) {
     const char* what = "fo_linear_cross_entropy";
     if (int rc = validate(what, dtype, tokens, cols, vocabulary)) return rc;
-    if (int rc = check_common(what, x, weight, targets, index_bytes, reduction, smoothing, workspace)) return rc;
-    if (!loss || !kept) return fail(FO_ERR_INVALID_ARGUMENT, "%s: loss and kept must not be NULL", what);
+    if (int rc = check_common(what, x, weight, reduction, smoothing, workspace)) return rc;
+    if (!targets || !loss || !kept) return fail(FO_ERR_INVALID_ARGUMENT, "%s: targets, loss and kept must not be NULL", what);
+    if (index_bytes != 4 && index_bytes != 8) return fail(FO_ERR_INVALID_ARGUMENT, "%s: targets of %d bytes", what, index_bytes);
     if (workspace_bytes < ForwardSpace(dtype, tokens, cols, vocabulary).total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
     const Forward f{{(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, targets, index_bytes, reduction,
                     ignore, smoothing, loss, kept, (char*)workspace, (hipStream_t)stream};
@@ -684,19 +777,22 @@ int fo_linear_cross_entropy(const void* x, int dtype, int64_t tokens, int64_t x_
 
 int64_t fo_linear_cross_entropy_backward_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int want_dx, int want_dw) {
     if (int rc = validate("fo_linear_cross_entropy_backward", dtype, tokens, cols, vocabulary)) return rc;
-    return BackwardSpace(dtype, tokens, cols, vocabulary, want_dx != 0, want_dw != 0).total;
+    const int cus = units();
+    return BackwardSpace(dtype, tokens, cols, vocabulary, want_dx != 0, want_dw != 0, cus).total;
 }
 
 int fo_linear_cross_entropy_backward(const void* x, int dtype, int64_t tokens, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t vocabulary,
-                                     int64_t cols, const void* targets, int index_bytes, int64_t ignore, int reduction, float smoothing, const float* kept,
-                                     const float* upstream, int64_t upstream_stride, void* dx, void* dw, void* workspace, int64_t workspace_bytes, void* stream) {
+                                     int64_t cols, int reduction, float smoothing, const float* kept, const float* upstream, int64_t upstream_stride, void* dx, void* dw,
+                                     void* workspace, int64_t workspace_bytes, void* stream) {
     const char* what = "fo_linear_cross_entropy_backward";
     if (int rc = validate(what, dtype, tokens, cols, vocabulary)) return rc;
-    if (int rc = check_common(what, x, weight, targets, index_bytes, reduction, smoothing, workspace)) return rc;
+    if (int rc = check_common(what, x, weight, reduction, smoothing, workspace)) return rc;
     if (!kept || !upstream || (!dx && !dw)) return fail(FO_ERR_INVALID_ARGUMENT, "%s: kept, upstream and a result must be given", what);
-    if (workspace_bytes < BackwardSpace(dtype, tokens, cols, vocabulary, dx != nullptr, dw != nullptr).total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
-    const Backward b{{(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, targets, index_bytes, reduction,
-                     ignore, smoothing, kept, upstream, upstream_stride, (char*)dx, (char*)dw, (char*)workspace, (hipStream_t)stream};
+    const int cus = units();
+    const BackwardSpace at(dtype, tokens, cols, vocabulary, dx != nullptr, dw != nullptr, cus);
+    if (workspace_bytes < at.total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+    const Backward b{{(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, reduction, smoothing, kept, upstream,
+                     upstream_stride, (char*)dx, (char*)dw, (char*)workspace, at, cus, (hipStream_t)stream};
     return by_product(dtype, b);
 }
 

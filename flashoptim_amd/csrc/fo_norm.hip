@@ -65,9 +65,19 @@ template <int RT> __device__ __forceinline__ void store_rounded(float (&v)[8], c
 template <int CTRL> __device__ __forceinline__ float from_lane(float x) {
     return as_f32((u32)__builtin_amdgcn_mov_dpp((int)as_u32(x), CTRL, 0xf, 0xf, true));
 }
+template <int CTRL> __device__ __forceinline__ double from_lane(double x) {
+    const u32x2 v = __builtin_bit_cast(u32x2, x);
+    const u32x2 w = {(u32)__builtin_amdgcn_mov_dpp((int)v.x, CTRL, 0xf, 0xf, true), (u32)__builtin_amdgcn_mov_dpp((int)v.y, CTRL, 0xf, 0xf, true)};
+    return __builtin_bit_cast(double, w);
+}
 __device__ __forceinline__ float read_lane(float x, int lane) { return as_f32((u32)__builtin_amdgcn_readlane((int)as_u32(x), lane)); }
+__device__ __forceinline__ double read_lane(double x, int lane) {
+    const u32x2 v = __builtin_bit_cast(u32x2, x);
+    const u32x2 w = {(u32)__builtin_amdgcn_readlane((int)v.x, lane), (u32)__builtin_amdgcn_readlane((int)v.y, lane)};
+    return __builtin_bit_cast(double, w);
+}
 // The sum over a wavefront, the same in every lane.
-__device__ __forceinline__ float wave_sum(float x) {
+template <class T> __device__ __forceinline__ T wave_sum(T x) {
     x += from_lane<0xb1>(x);     // lanes 1 0 3 2
     x += from_lane<0x4e>(x);     // lanes 2 3 0 1
     x += from_lane<0x141>(x);    // eight lanes mirrored
@@ -76,88 +86,90 @@ __device__ __forceinline__ float wave_sum(float x) {
 }
 
 // The sum over a workgroup, the same in every thread.  `places` takes turns between two arrays, so one barrier is enough.
-template <int THREADS> __device__ __forceinline__ float group_sum(float x, float (&places)[2][16], int& turn) {
+template <int THREADS, class T> __device__ __forceinline__ T group_sum(T x, T (&places)[2][16], int& turn) {
     x = wave_sum(x);
     if constexpr (THREADS == 64) return x;
-    float(&mine)[16] = places[turn];
+    T(&mine)[16] = places[turn];
     turn ^= 1;
     if ((threadIdx.x & 63) == 0) mine[threadIdx.x >> 6] = x;
     __syncthreads();
-    float all = mine[0];
+    T all = mine[0];
 #pragma unroll
     for (int w = 1; w < THREADS / 64; ++w) all += mine[w];
     return all;
 }
-// The same in fp64, for the rare rows that fp32 cannot hold the squares of.
-template <int THREADS> __device__ __attribute__((noinline)) double group_sum_wide(double x) {
-    __shared__ double places[16];
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) places[threadIdx.x >> 6] = x;
-    __syncthreads();
-    double all = places[0];
-    for (int w = 1; w < THREADS / 64; ++w) all += places[w];
-    return all;
-}
 
-template <int THREADS, int V> __device__ __forceinline__ float inverse_root(const float (&s)[V][8], int cols, float eps, float (&places)[2][16], int& turn) {
-    float sum = 0.0f;
+// 1 / sqrt(mean(s^2) + eps).  Squares are added in fp64, which costs nothing beside the loads and holds the squares of every fp32 number, and rounded to fp32 as a
+// mean; only where that is no normal number is the root taken in fp64 too.
+template <int THREADS, int V> __device__ __forceinline__ float inverse_root(const float (&s)[V][8], int cols, float eps, double (&places)[2][16], int& turn) {
+    double sum = 0.0;
 #pragma unroll
     for (int p = 0; p < V; ++p)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum = fmaf(s[p][k], s[p][k], sum);
-    sum = group_sum<THREADS>(sum, places, turn);
-    if (sum >= 0x1p-90f && sum <= 0x1p120f) return 1.0f / __builtin_sqrtf(sum / (float)cols + eps);
-    // squares beyond what fp32 holds (or a row of zeros): the same for every thread of the workgroup
-    double wide = 0.0;
-#pragma unroll
-    for (int p = 0; p < V; ++p)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) wide += (double)s[p][k] * (double)s[p][k];
-    return (float)(1.0 / __builtin_sqrt(group_sum_wide<THREADS>(wide) / cols + (double)eps));
+        for (int k = 0; k < 8; ++k) sum = __builtin_fma((double)s[p][k], (double)s[p][k], sum);
+    sum = group_sum<THREADS>(sum, places, turn) / cols;
+    const float mean = (float)sum + eps;
+    if (mean >= 0x1p-120f && mean <= 0x1p126f) return rsqrtf(mean);
+    return (float)(1.0 / __builtin_sqrt(sum + (double)eps));
 }
 
-// XT: type of x and y, RT: of the residual and the stream.  THREADS hold V pieces of eight values each, THREADS * V * 8 >= cols.
-template <int XT, int RT, int THREADS, int V, bool MX> __global__ __launch_bounds__(THREADS) void norm_kernel(NormArgs a) {
+// What a thread holds of a row as it came from memory: V pieces of eight values.  WHOLE: rows are whole multiples of eight, so a piece is there or it is not.
+template <int DT, int THREADS, int V, bool WHOLE> struct Raw {
+    static constexpr int B = DTypeInfo<DT>::bytes, EPL = 16 / B;
+    Pack<B, EPL> d[V][8 / EPL];
+    __device__ __forceinline__ void load(const char* row, int cols) {
+#pragma unroll
+        for (int p = 0; p < V; ++p) {
+            const int c = (threadIdx.x + p * THREADS) * 8;
+#pragma unroll
+            for (int part = 0; part < 8 / EPL; ++part) {
+#pragma unroll
+                for (int k = 0; k < Pack<B, EPL>::kDwords; ++k) d[p][part].w[k] = 0;
+                if (c < cols) load_piece<B, EPL>(d[p][part], row + ((int64_t)c + part * EPL) * B, WHOLE ? EPL : cols - c - part * EPL);
+            }
+        }
+    }
+    __device__ __forceinline__ float value(int p, int k) const { return widen<DT, EPL>(d[p][k / EPL], k % EPL); }
+};
+
+// XT: type of x and y, RT: of the residual and the stream.  THREADS hold V pieces of eight values each, THREADS * V * 8 >= cols.  A workgroup takes every
+// gridDim.x-th row and asks for the next one before it adds up the squares of this one (rows of up to 8192 values; longer ones leave no registers
+// for that).
+template <int XT, int RT, int THREADS, int V, bool MX, bool WHOLE> __global__ __launch_bounds__(THREADS) void norm_kernel(NormArgs a) {
     constexpr int XB = DTypeInfo<XT>::bytes, RB = DTypeInfo<RT>::bytes;
-    __shared__ float places[2][16];
+    constexpr bool kAhead = THREADS <= 256;
+    __shared__ double places[2][16];
     int turn = 0;
     const int cols = a.cols, first = threadIdx.x * 8;
+    Raw<XT, THREADS, V, WHOLE> x;
+    Raw<RT, THREADS, V, WHOLE> r;
+    x.load(a.x + blockIdx.x * a.x_stride * XB, cols);
+    if (a.residual) r.load(a.residual + blockIdx.x * a.residual_stride * RB, cols);
     float w[V][8];
 #pragma unroll
     for (int p = 0; p < V; ++p) {
         const int c = first + p * THREADS * 8;
 #pragma unroll
         for (int k = 0; k < 8; ++k) w[p][k] = 1.0f;
-        if (a.weight && c < cols) load_any(w[p], a.weight, a.weight_dtype, c, cols - c);
+        if (a.weight && c < cols) load_any(w[p], a.weight, a.weight_dtype, c, WHOLE ? 8 : cols - c);
     }
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float s[V][8];
-        const char* x = a.x + row * a.x_stride * XB;
 #pragma unroll
         for (int p = 0; p < V; ++p) {
             const int c = first + p * THREADS * 8;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s[p][k] = 0.0f;
-            if (c < cols) load_values<XT>(s[p], x + (int64_t)c * XB, cols - c);
+            for (int k = 0; k < 8; ++k) s[p][k] = x.value(p, k);
+            if (a.residual) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) s[p][k] += r.value(p, k);
+                if (c < cols) store_rounded<RT>(s[p], a.stream + (row * cols + c) * RB, WHOLE ? 8 : cols - c);
+            }
         }
-        if (a.residual) {
-            const char* residual = a.residual + row * a.residual_stride * RB;
-            char* stream = a.stream + row * cols * RB;
-            float r[V][8];
-#pragma unroll
-            for (int p = 0; p < V; ++p) {
-                const int c = first + p * THREADS * 8;
-                if (c < cols) load_values<RT>(r[p], residual + (int64_t)c * RB, cols - c);
-            }
-#pragma unroll
-            for (int p = 0; p < V; ++p) {
-                const int c = first + p * THREADS * 8;
-                if (c >= cols) continue;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) s[p][k] += r[p][k];
-                store_rounded<RT>(s[p], stream + (int64_t)c * RB, cols - c);
-            }
+        const int64_t next = row + gridDim.x;
+        if (kAhead && next < a.rows) {
+            x.load(a.x + next * a.x_stride * XB, cols);
+            if (a.residual) r.load(a.residual + next * a.residual_stride * RB, cols);
         }
         const float inverse = inverse_root<THREADS, V>(s, cols, a.eps, places, turn);
         if (a.inverse && threadIdx.x == 0) a.inverse[row] = inverse;
@@ -184,72 +196,78 @@ template <int XT, int RT, int THREADS, int V, bool MX> __global__ __launch_bound
                 *reinterpret_cast<u32*>(a.y + row * blocks * (kBlock / 2) + c / 2) = codes;
                 if ((threadIdx.x & 3) == 0) a.scales[row * blocks * 4 + c / kMxGroup] = (uint8_t)byte;
             } else {
-                if (c < cols) store_values<XT>(y, a.y + (row * cols + c) * XB, cols - c);
+                if (c < cols) store_values<XT>(y, a.y + (row * cols + c) * XB, WHOLE ? 8 : cols - c);
             }
+        }
+        if (!kAhead && next < a.rows) {
+            x.load(a.x + next * a.x_stride * XB, cols);
+            if (a.residual) r.load(a.residual + next * a.residual_stride * RB, cols);
         }
     }
 }
 
-template <int XT, int RT, int THREADS, int V> __global__ __launch_bounds__(THREADS) void norm_grad_kernel(NormGradArgs a) {
+template <int XT, int RT, int THREADS, int V, bool WHOLE> __global__ __launch_bounds__(THREADS) void norm_grad_kernel(NormGradArgs a) {
     constexpr int XB = DTypeInfo<XT>::bytes, RB = DTypeInfo<RT>::bytes;
+    constexpr bool kAhead = THREADS <= 256;
     __shared__ float places[2][16];
     int turn = 0;
     const int cols = a.cols, first = threadIdx.x * 8;
+    Raw<RT, THREADS, V, WHOLE> s, more;
+    Raw<XT, THREADS, V, WHOLE> dy;
+    float inverse = 0.0f;
+    const auto load = [&](int64_t row) {
+        s.load(a.s + row * a.s_stride * RB, cols);
+        dy.load(a.dy + row * a.dy_stride * XB, cols);
+        inverse = a.inverse[row];
+        if (a.dstream) more.load(a.dstream + row * a.dstream_stride * RB, cols);
+    };
+    load(blockIdx.x);
     float dw[V][8];
 #pragma unroll
     for (int p = 0; p < V; ++p)
 #pragma unroll
         for (int k = 0; k < 8; ++k) dw[p][k] = 0.0f;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        float n[V][8], dn[V][8];
-        const char *s = a.s + row * a.s_stride * RB, *dy = a.dy + row * a.dy_stride * XB;
+        const float root = inverse;
+        float n[V][8], dn[V][8], along = 0.0f;
 #pragma unroll
         for (int p = 0; p < V; ++p) {
             const int c = first + p * THREADS * 8;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) n[p][k] = dn[p][k] = 0.0f;
-            if (c < cols) {
-                load_values<RT>(n[p], s + (int64_t)c * RB, cols - c);
-                load_values<XT>(dn[p], dy + (int64_t)c * XB, cols - c);
-            }
-        }
-        const float inverse = a.inverse[row];
-        float along = 0.0f;
-#pragma unroll
-        for (int p = 0; p < V; ++p) {
-            const int c = first + p * THREADS * 8;
-            if (c >= cols) continue;
             float w[8];
-            if (a.weight) load_any(w, a.weight, a.weight_dtype, c, cols - c);
+            if (a.weight && c < cols) load_any(w, a.weight, a.weight_dtype, c, WHOLE ? 8 : cols - c);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                n[p][k] *= inverse;
+                n[p][k] = s.value(p, k) * root;
+                dn[p][k] = dy.value(p, k);
                 dw[p][k] = fmaf(dn[p][k], n[p][k], dw[p][k]);
                 if (a.weight) dn[p][k] *= w[k];
-                if (c + k < cols) along = fmaf(dn[p][k], n[p][k], along);
+                if (WHOLE ? c < cols : c + k < cols) along = fmaf(dn[p][k], n[p][k], along);
             }
         }
-        if (!a.dx && !a.dresidual) continue;
-        along = group_sum<THREADS>(along, places, turn) / (float)cols;
-        const char* dstream = a.dstream + row * a.dstream_stride * RB;
+        const int64_t next = row + gridDim.x;
+        Raw<RT, THREADS, V, WHOLE> ds_in = more;
+        if (kAhead && next < a.rows) load(next);
+        if (a.dx || a.dresidual) {
+            along = group_sum<THREADS>(along, places, turn) / (float)cols;
 #pragma unroll
-        for (int p = 0; p < V; ++p) {
-            const int c = first + p * THREADS * 8;
-            if (c >= cols) continue;
-            float more[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, ds[8];
-            if (a.dstream) load_values<RT>(more, dstream + (int64_t)c * RB, cols - c);
+            for (int p = 0; p < V; ++p) {
+                const int c = first + p * THREADS * 8;
+                if (c >= cols) continue;
+                float ds[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) ds[k] = fmaf(inverse, fmaf(-n[p][k], along, dn[p][k]), more[k]);
-            if (a.dresidual) store_values<RT>(ds, a.dresidual + (row * cols + c) * RB, cols - c);
-            if (a.dx) store_values<XT>(ds, a.dx + (row * cols + c) * XB, cols - c);
+                for (int k = 0; k < 8; ++k) ds[k] = fmaf(root, fmaf(-n[p][k], along, dn[p][k]), a.dstream ? ds_in.value(p, k) : 0.0f);
+                if (a.dresidual) store_values<RT>(ds, a.dresidual + (row * cols + c) * RB, WHOLE ? 8 : cols - c);
+                if (a.dx) store_values<XT>(ds, a.dx + (row * cols + c) * XB, WHOLE ? 8 : cols - c);
+            }
         }
+        if (!kAhead && next < a.rows) load(next);
     }
     if (a.partial) {
         float* out = a.partial + (int64_t)blockIdx.x * cols;
 #pragma unroll
         for (int p = 0; p < V; ++p) {
             const int c = first + p * THREADS * 8;
-            if (c < cols) store_values<DT_F32>(dw[p], out + c, cols - c);
+            if (c < cols) store_values<DT_F32>(dw[p], out + c, WHOLE ? 8 : cols - c);
         }
     }
 }
@@ -306,8 +324,7 @@ template <class L> int by_width(int cols, const L& launch) {
     if (cols <= 2048) return launch.template with<256, 1>();
     if (cols <= 4096) return launch.template with<256, 2>();
     if (cols <= 8192) return launch.template with<256, 4>();
-    if (cols <= 16384) return launch.template with<1024, 2>();
-    return launch.template with<1024, 4>();
+    return launch.template with<1024, 2>();
 }
 
 struct Forward {
@@ -319,9 +336,12 @@ struct Forward {
         template <int THREADS, int V> int with() const {
             const int64_t most = (int64_t)compute_units() * (2048 / THREADS);
             if (most <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
-            const unsigned grid = (unsigned)(f.a.rows < most ? f.a.rows : most);
-            if (f.mx) fo::norm_kernel<XT, RT, THREADS, V, true><<<dim3(grid), dim3(THREADS), 0, f.stream>>>(f.a);
-            else fo::norm_kernel<XT, RT, THREADS, V, false><<<dim3(grid), dim3(THREADS), 0, f.stream>>>(f.a);
+            const dim3 grid((unsigned)(f.a.rows < most ? f.a.rows : most)), threads(THREADS);
+            const bool whole = f.a.cols % 8 == 0;
+            if (f.mx && whole) fo::norm_kernel<XT, RT, THREADS, V, true, true><<<grid, threads, 0, f.stream>>>(f.a);
+            else if (f.mx) fo::norm_kernel<XT, RT, THREADS, V, true, false><<<grid, threads, 0, f.stream>>>(f.a);
+            else if (whole) fo::norm_kernel<XT, RT, THREADS, V, false, true><<<grid, threads, 0, f.stream>>>(f.a);
+            else fo::norm_kernel<XT, RT, THREADS, V, false, false><<<grid, threads, 0, f.stream>>>(f.a);
             return check_hip(hipGetLastError(), "fo_rms_norm");
         }
     };
@@ -338,7 +358,8 @@ struct Backward {
     template <int XT, int RT> struct Width {
         const Backward& b;
         template <int THREADS, int V> int with() const {
-            fo::norm_grad_kernel<XT, RT, THREADS, V><<<dim3(b.grid), dim3(THREADS), 0, b.stream>>>(b.a);
+            if (b.a.cols % 8 == 0) fo::norm_grad_kernel<XT, RT, THREADS, V, true><<<dim3(b.grid), dim3(THREADS), 0, b.stream>>>(b.a);
+            else fo::norm_grad_kernel<XT, RT, THREADS, V, false><<<dim3(b.grid), dim3(THREADS), 0, b.stream>>>(b.a);
             return check_hip(hipGetLastError(), "fo_rms_norm_backward");
         }
     };

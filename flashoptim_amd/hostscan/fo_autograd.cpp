@@ -312,15 +312,13 @@ PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // ---------------------------------------------------------------------------------------------------- loss
 struct LossNode : Node {
-    SavedVariable x, weight, target, kept;
-    int64_t ignore = 0;
+    SavedVariable x, weight, kept;
     int reduction = 0;
     float smoothing = 0.0f;
 
     void release_variables() override {
         x.reset_data();
         weight.reset_data();
-        target.reset_data();
         kept.reset_data();
     }
     std::string name() const override { return "LinearCrossEntropyBackward"; }
@@ -328,13 +326,13 @@ struct LossNode : Node {
     variable_list apply(variable_list&& grads) override {
         variable_list out(2);
         if (!grads[0].defined()) return out;
-        const Tensor x = this->x.unpack(), weight = this->weight.unpack(), target = this->target.unpack(), kept = this->kept.unpack();
+        const Tensor x = this->x.unpack(), weight = this->weight.unpack(), kept = this->kept.unpack();
         const bool need_dx = task_should_compute_output(0), need_dw = task_should_compute_output(1);
         if (!need_dx && !need_dw) return out;
         {
             at::NoGradGuard none;
             const c10::DeviceGuard guard(x.device());
-            const int64_t width = x.size(-1), tokens = target.numel(), vocabulary = weight.size(0);
+            const int64_t width = x.size(-1), tokens = leading(x), vocabulary = weight.size(0);
             Tensor upstream = grads[0].is_neg() ? grads[0].resolve_neg() : grads[0];
             if (upstream.dim() > 1) upstream = upstream.reshape({tokens});
             const int64_t size = api.fo_linear_cross_entropy_backward_workspace(code_of(x), tokens, width, vocabulary, need_dx, need_dw);
@@ -342,8 +340,8 @@ struct LossNode : Node {
             const Tensor workspace = bytes(size, x);
             if (need_dx) out[0] = at::empty(x.sizes(), x.options());
             if (need_dw) out[1] = at::empty({vocabulary, width}, weight.options());
-            check(api.fo_linear_cross_entropy_backward(x.data_ptr(), code_of(x), tokens, row_stride(x), weight.data_ptr(), weight.stride(0), vocabulary, width, target.data_ptr(),
-                                                       index_bytes(target), ignore, reduction, smoothing, (const float*)kept.data_ptr(), (const float*)upstream.data_ptr(),
+            check(api.fo_linear_cross_entropy_backward(x.data_ptr(), code_of(x), tokens, row_stride(x), weight.data_ptr(), weight.stride(0), vocabulary, width, reduction,
+                                                       smoothing, (const float*)kept.data_ptr(), (const float*)upstream.data_ptr(),
                                                        upstream.dim() ? upstream.stride(0) : 0, ptr(out[0]), ptr(out[1]), workspace.data_ptr(), size, stream_of(x)),
                   "fo_linear_cross_entropy_backward");
         }
@@ -371,7 +369,7 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
             at::NoGradGuard none;
             const auto numbers = x->options().dtype(at::kFloat);
             loss = reduction == FO_REDUCE_NONE ? at::empty(target->sizes(), numbers) : at::empty({}, numbers);
-            kept = at::empty({tokens + 1}, numbers);
+            kept = at::empty({2 * tokens + 1}, numbers);
             const int64_t size = api.fo_linear_cross_entropy_workspace(code_of(*x), tokens, width, vocabulary);
             check_size(size, "fo_linear_cross_entropy");
             const Tensor workspace = bytes(size, *x);
@@ -385,9 +383,7 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
             node->set_next_edges(torch::autograd::collect_next_edges(*x, *weight));
             node->x = SavedVariable(*x, false);
             node->weight = SavedVariable(*weight, false);
-            node->target = SavedVariable(*target, false);
             node->kept = SavedVariable(kept, false);
-            node->ignore = ignore;
             node->reduction = (int)reduction;
             node->smoothing = (float)smoothing;
             torch::autograd::set_history(loss, node);

@@ -21,12 +21,12 @@ def _forward(x, weight, target, how):
     device, lib = x.device, _native.lib()
     ignore, reduction, smoothing = how
     loss = torch.empty(tokens if reduction == 0 else (), dtype=torch.float32, device=device)
-    kept = torch.empty(tokens + 1, dtype=torch.float32, device=device)
-    size = lib.fo_linear_cross_entropy_workspace(DTYPE_CODE[x.dtype], tokens, width, vocabulary)
-    if size < 0:
-        _native.check(size, "fo_linear_cross_entropy")
-    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    kept = torch.empty(2 * tokens + 1, dtype=torch.float32, device=device)
     with _native.device_guard(device):
+        size = lib.fo_linear_cross_entropy_workspace(DTYPE_CODE[x.dtype], tokens, width, vocabulary)
+        if size < 0:
+            _native.check(size, "fo_linear_cross_entropy")
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
         rc = lib.fo_linear_cross_entropy(
             x.data_ptr(), DTYPE_CODE[x.dtype], tokens, x.stride(0), weight.data_ptr(), weight.stride(0), vocabulary, width, target.data_ptr(),
             _INDEX_BYTES[target.dtype], ignore, reduction, smoothing, loss.data_ptr(), kept.data_ptr(), workspace.data_ptr(), size,
@@ -37,36 +37,34 @@ def _forward(x, weight, target, how):
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
-    """Keeps its operands and one number a row."""
+    """Keeps its operands and two numbers a row."""
 
     @staticmethod
     def forward(ctx, x, weight, target, how):
         x, weight = _plain(x), _plain(weight)
         loss, kept = _forward(x, weight, target, how)
-        ctx.save_for_backward(x, weight, target, kept)
-        ctx.how = how
+        ctx.save_for_backward(x, weight, kept)
+        _, ctx.reduction, ctx.smoothing = how
         return loss
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, upstream):
-        x, weight, target, kept = ctx.saved_tensors
+        x, weight, kept = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[:2]
-        ignore, reduction, smoothing = ctx.how
         (tokens, width), vocabulary = x.shape, weight.shape[0]
         device, lib = x.device, _native.lib()
         upstream = upstream.resolve_neg() if upstream.is_neg() else upstream
         dx = torch.empty((tokens, width), dtype=x.dtype, device=device) if need_dx else None
         dw = torch.empty((vocabulary, width), dtype=x.dtype, device=device) if need_dw else None
-        size = lib.fo_linear_cross_entropy_backward_workspace(DTYPE_CODE[x.dtype], tokens, width, vocabulary, need_dx, need_dw)
-        if size < 0:
-            _native.check(size, "fo_linear_cross_entropy_backward")
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
         with _native.device_guard(device):
+            size = lib.fo_linear_cross_entropy_backward_workspace(DTYPE_CODE[x.dtype], tokens, width, vocabulary, need_dx, need_dw)
+            if size < 0:
+                _native.check(size, "fo_linear_cross_entropy_backward")
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
             rc = lib.fo_linear_cross_entropy_backward(
-                x.data_ptr(), DTYPE_CODE[x.dtype], tokens, x.stride(0), weight.data_ptr(), weight.stride(0), vocabulary, width, target.data_ptr(),
-                _INDEX_BYTES[target.dtype], ignore, reduction, smoothing, kept.data_ptr(), upstream.data_ptr(), upstream.stride(0) if upstream.dim() else 0,
-                _native.ptr(dx), _native.ptr(dw), workspace.data_ptr(), size, _native.current_stream_ptr(device))
+                x.data_ptr(), DTYPE_CODE[x.dtype], tokens, x.stride(0), weight.data_ptr(), weight.stride(0), vocabulary, width, ctx.reduction,
+                ctx.smoothing, kept.data_ptr(), upstream.data_ptr(), upstream.stride(0) if upstream.dim() else 0, _native.ptr(dx), _native.ptr(dw), workspace.data_ptr(), size, _native.current_stream_ptr(device))
         if rc:
             _native.check(rc, "fo_linear_cross_entropy_backward")
         return dx, dw, None, None
@@ -89,7 +87,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 
     Logits are summed in fp32 and not rounded.  The backward pass computes them again, a piece of the vocabulary at a time, so that of size tokens
     x vocabulary there is only a piece of their gradient; the sums have a fixed order, so results repeat to the bit.  Between the passes
-    `x`, `weight` and one number a row are kept.  A target outside the vocabulary makes a NaN (the call does not wait for
+    `x`, `weight` and two numbers a row are kept.  A target outside the vocabulary makes a NaN (the call does not wait for
     the GPU to look at the targets).
 
     Raises:

@@ -317,7 +317,7 @@ int fo_mxfp4_linear_backward(const void *dy, int dy_dtype, int64_t tokens, int64
  * 1 / sqrt(mean(s^2) + eps), which the backward pass takes.  The second form writes y in MXFP4, unrounded before, as fo_mxfp4_quantize
  * lays it out.
  */
-#define FO_RMS_NORM_MOST_COLS 32768
+#define FO_RMS_NORM_MOST_COLS 16384
 int fo_rms_norm(const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t x_stride, const void *residual, int stream_dtype,
                 int64_t residual_stride, const void *weight, int weight_dtype, float eps, void *out_stream, void *y, float *inverse,
                 void *stream);
@@ -340,7 +340,8 @@ int fo_rms_norm_backward(const void *s, int stream_dtype, int64_t s_stride, cons
  * rounded once; rows of no token are zero, and so is row `padding` (-1: none); tokens outside the vocabulary are left out.
  * workspace: fo_embedding_backward_workspace bytes of device memory, aligned to 256.
  */
-#define FO_EMBEDDING_MOST 33554432 /* tokens, and rows of the matrix */
+#define FO_EMBEDDING_MOST_TOKENS 33554432
+#define FO_EMBEDDING_MOST_ROWS 8388607 /* of the matrix */
 int fo_embedding(const void *tokens, int index_bytes, int64_t n_tokens, const void *weight, int dtype, int64_t vocabulary, int64_t cols,
                  int64_t weight_stride, float scale, void *y, void *stream);
 int64_t fo_embedding_backward_workspace(int64_t n_tokens, int64_t vocabulary, int64_t cols);
@@ -353,7 +354,8 @@ int fo_embedding_backward(const void *tokens, int index_bytes, int64_t n_tokens,
  * x: tokens x cols, weight: vocabulary x cols, both of `dtype`; targets: index_bytes 4 or 8 each, contiguous.  A target outside the
  * vocabulary makes a NaN.
  *   loss: fp32, `tokens` of them, or one: their sum or their sum over the number of targets that are not ignored
- *   kept: tokens + 1 fp32 numbers that the backward pass takes: log sum exp of each row, and that number
+ *   kept: 2 * tokens + 1 fp32 numbers that the backward pass takes: log sum exp of each row, that number, and the rows' targets as int32 (-1: ignored,
+ *   -2: none of the vocabulary)
  * Backward: upstream: the loss's gradient, fp32, upstream_stride elements apart (0: one for all); dx (tokens x cols) and dw (vocabulary
  * x cols) of `dtype`, contiguous, either may be NULL.  workspace: device memory, aligned to 256.
  */
@@ -364,9 +366,9 @@ int fo_linear_cross_entropy(const void *x, int dtype, int64_t tokens, int64_t x_
                             float smoothing, float *loss, float *kept, void *workspace, int64_t workspace_bytes, void *stream);
 int64_t fo_linear_cross_entropy_backward_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int want_dx, int want_dw);
 int fo_linear_cross_entropy_backward(const void *x, int dtype, int64_t tokens, int64_t x_stride, const void *weight, int64_t weight_stride,
-                                     int64_t vocabulary, int64_t cols, const void *targets, int index_bytes, int64_t ignore, int reduction,
-                                     float smoothing, const float *kept, const float *upstream, int64_t upstream_stride, void *dx, void *dw,
-                                     void *workspace, int64_t workspace_bytes, void *stream);
+                                     int64_t vocabulary, int64_t cols, int reduction, float smoothing, const float *kept,
+                                     const float *upstream, int64_t upstream_stride, void *dx, void *dw, void *workspace,
+                                     int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -2,9 +2,9 @@
 
 What they allow, with u = 2^-24:
 * the stream is one fp32 addition and one rounding, as in torch: exact;
-* the mean of squares is a sum in which a value passes at most 32 + 14 additions, so 46 u of it, 23 u of its root, and 5 u for the root, its
-  inverse, the eps and the two products: 2^-19 of the result in all, and half a step of its type;
-* in the gradient the mean of dn n is off by at most 46 u of the mean of the magnitudes besides; a term has 2^-18 of its magnitude, the result
+* the mean of squares is summed in fp64, so u of it for its rounding and u for the eps, half of both in its root; that is off by a unit (2 u), and the two
+  products by u each: 5 u, and half a step of the type; 2^-19 is allowed;
+* in the gradient the mean of dn n, where a value passes at most 32 + 14 additions, is off by at most 46 u of the mean of the magnitudes besides; a term has 2^-18 of its magnitude, the result
   half a step;
 * a sum over rows is made of at most 1 + rows / 512 + 72 additions: that many u of the magnitudes' sum, and 2^-19 for n.
 """
@@ -19,7 +19,7 @@ F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 TYPES = [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)]
 HALF_STEP = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}
 SMALLEST = {F32: 2.0 ** -149, BF16: 2.0 ** -133, F16: 2.0 ** -24}
-WIDTHS = [1, 7, 8, 31, 128, 250, 512, 513, 2048, 2730, 4096, 4100, 8192, 8200, 16384, 16400, 32768]
+WIDTHS = [1, 7, 8, 31, 128, 250, 512, 513, 2048, 2730, 4096, 4100, 8192, 8200, 16379, 16384]
 
 
 @pytest.fixture(params=["nodes", "python"], autouse=True)
@@ -102,7 +102,7 @@ def test_norm_and_gradients(width, types):
             assert torch.equal(plain[0], y) and torch.equal(plain[1], s) if with_residual else torch.equal(plain, y), what
 
 
-@pytest.mark.parametrize("width", [1, 31, 33, 128, 129, 250, 512, 520, 2730, 4096, 5000, 16400])
+@pytest.mark.parametrize("width", [1, 31, 33, 128, 129, 250, 512, 520, 2730, 4096, 5000, 16300])
 @pytest.mark.parametrize("types", TYPES, ids=str)
 def test_mxfp4_output_is_the_quantised_norm(width, types):
     """Bit for bit what the quantiser makes of the norm in fp32 of the same stream."""
@@ -276,7 +276,7 @@ def test_refusals():
         with pytest.raises(NotImplementedError):
             call(x.cpu())
         with pytest.raises(RuntimeError, match="too long"):
-            call(torch.zeros(1, 32769, device=DEV))
+            call(torch.zeros(1, 16385, device=DEV))
         with torch.autograd.forward_ad.dual_level():
             with pytest.raises(NotImplementedError):
                 call(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
