@@ -2,29 +2,29 @@
 //
 //   y[i] = scale weight[tokens[i]]          dw[v] = scale (sum of dy[i] over the i with tokens[i] = v)
 //
-// The gradient is a sum over lists of positions, one list per row.  Positions are sorted by token, in their own order within a token, so a
-// list is a run of the sorted array, and every row of dw is written once, by a sum whose order is fixed: no atomics, the
-// same bits every time.
+// The gradient is a sum over lists of positions, one list per row.  dw is filled with zeros, positions are sorted by token, in their own order within a
+// token, so a list is a run of the sorted array, and every row that has a list is written once more, by a sum whose order is fixed: no atomics,
+// the same bits every time.
 //
-// Sorting.  A key is token << 32 | position, so no two are equal and a sort of keys is a stable sort of tokens.  Workgroups of 256
-// threads sort runs of 512 keys, each key's place being the number of smaller ones (512 comparisons against LDS, no exchanges);
-// then sixteen runs at a time are merged, again by counting: a key's place in the merged run is its place in its own plus
-// the numbers of smaller keys in the fifteen others, binary searches that do not wait for one another (the first merge's in LDS).  8192 tokens take
-// two launches, where the lists begin included, 131072 four.
+// Sorting.  A key is token << 32 | position, so no two are equal and a sort of keys is a stable sort of tokens.  A key's place is the
+// number of keys below it, counted: in the 64 of its wavefront by comparing with each, in the workgroup's eight such runs by binary searches
+// in LDS, that makes runs of 512; then in sixteen of those at a time, again by binary searches, the first time in LDS, from 131072 tokens on in
+// memory.  None of these launches has work for a fill's memory bandwidth, so the first two carry the fill with them.
 //
-// Summing.  A wavefront adds up a row's list, up to `window` positions of it.  Longer lists (padding, the most
-// frequent words) are cut at multiples of that in the sorted array and their parts summed by wavefronts of their own first, in fp32, and the row's
-// wavefront adds up those sums.
+// Summing.  The sorted array is cut into windows of the same length whatever the lists, a wavefront takes a window (and 512 columns), so the
+// padding token or the most frequent word keeps nobody longer than the others.  A list that ends where its window does not is complete;
+// lists that go on over a border leave fp32 sums, which another launch adds up.
 #include "fo_gemm.h"
 #include "fo_host.h"
 
 namespace fo {
 
 typedef uint64_t u64;
-constexpr int kRun = 512, kSortThreads = 256;    // keys a workgroup sorts
+constexpr int kRun = 512;                        // keys, and threads, of a workgroup that sorts
 constexpr int kWays = 16;                        // runs that one merge takes
-constexpr int kMergeThreads = 256;
-constexpr u32 kNoToken = (1u << 23) - 1;         // sorts last; tokens are below FO_EMBEDDING_MOST_ROWS
+constexpr int kMergeKeys = kRun * kWays, kMergeThreads = 256;
+constexpr u32 kNoToken = (1u << 23) - 1;         // sorts last; tokens are below it, FO_EMBEDDING_MOST_ROWS
+constexpr int kFillBytes = 65536;                // a workgroup's share of a fill
 
 struct Tokens {
     const void* p;
@@ -34,38 +34,49 @@ struct Tokens {
     }
 };
 
-// Runs of kRun keys, sorted.  Within a run token << 9 | place is a key of 32 bits, so a 16-byte read from LDS brings four to compare with.
-__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(Tokens tokens, int n, int64_t vocabulary, int64_t skip, u64* keys) {
-    __shared__ __attribute__((aligned(16))) u32 run[kRun];
-    const int first = (int)blockIdx.x * kRun;
-    u32 mine[2];
+// Zeros from `first` of kFillBytes on.
+template <int THREADS> __device__ __forceinline__ void fill(char* to, int64_t bytes, int64_t first) {
+    const int64_t from = first * kFillBytes;
+    const u32x4 zero = {0, 0, 0, 0};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int at = threadIdx.x + k * kSortThreads;
-        u32 t = kNoToken;
-        if (first + at < n) {
-            const int64_t token = tokens[first + at];
-            if (token >= 0 && token < vocabulary && token != skip) t = (u32)token;
-        }
-        mine[k] = t << 9 | (u32)at;    // what lies behind the last token sorts behind it
-        run[at] = mine[k];
+    for (int k = 0; k < kFillBytes / 16 / THREADS; ++k) {
+        const int64_t at = from + ((int64_t)k * THREADS + threadIdx.x) * 16;
+        if (at + 16 <= bytes) *reinterpret_cast<FO_GLOBAL u32x4_any*>((FO_GLOBAL char*)to + at) = zero;
+        else for (int64_t i = at; i < bytes; ++i) to[i] = 0;
     }
+}
+
+// The number of the run's 2^log keys below `limit`; LDS holds kNoToken << 9 and more behind the last key.  `key(i)` is its i-th.
+template <int LOG, class F> __device__ __forceinline__ int below(u32 limit, const F& key) {
+    int pos = 0;
+#pragma unroll
+    for (int step = 1 << (LOG - 1); step > 0; step >>= 1) pos += key(pos + step - 1) < limit ? step : 0;
+    return pos + (key(pos) < limit ? 1 : 0);
+}
+
+// Runs of kRun keys, sorted; workgroups from `sorting` on fill.  Within a run token << 9 | place is a key of 32 bits.
+__global__ __launch_bounds__(kRun) void embed_sort_kernel(Tokens tokens, int n, int64_t vocabulary, int64_t skip, u64* keys, int sorting, char* filled, int64_t fill_bytes) {
+    if ((int)blockIdx.x >= sorting) { fill<kRun>(filled, fill_bytes, (int64_t)blockIdx.x - sorting); return; }
+    __shared__ u32 run[kRun];
+    const int first = (int)blockIdx.x * kRun, at = threadIdx.x, lane = at & 63, wave = at >> 6;
+    u32 t = kNoToken;
+    if (first + at < n) {
+        const int64_t token = tokens[first + at];
+        if (token >= 0 && token < vocabulary && token != skip) t = (u32)token;
+    }
+    const u32 mine = t << 9 | (u32)at;    // what lies behind the last token sorts behind it
+    int place = 0;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) place += (u32)__builtin_amdgcn_readlane((int)mine, i) < mine;
+    run[wave * 64 + place] = mine;
+    (void)lane;
     __syncthreads();
-    int place[2] = {0, 0};
-#pragma unroll 8
-    for (int i = 0; i < kRun; i += 4) {
-        const u32x4 other = *reinterpret_cast<const u32x4*>(run + i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            place[0] += other[e] < mine[0];
-            place[1] += other[e] < mine[1];
-        }
+    for (int w = 0; w < kRun / 64; ++w) {
+        const int there = below<6>(mine, [&](int i) { return run[w * 64 + i]; });
+        place += w == wave ? 0 : there;
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int at = threadIdx.x + k * kSortThreads;
-        if (first + at < n) keys[first + place[k]] = (u64)(mine[k] >> 9) << 32 | (u32)(first + at);
-    }
+    if (first + at < n) keys[first + place] = (u64)t << 32 | (u32)(first + at);
 }
 
 // How many of the sorted keys[0 .. size) are below `limit`: kWays searches at a time, each run's in its own registers, so that a step waits for memory
@@ -112,153 +123,127 @@ __global__ __launch_bounds__(kMergeThreads) void embed_merge_kernel(const u64* _
     to[group + place] = key;
 }
 
-// The first merge, of runs of kRun keys, whose tokens a workgroup brings into LDS; kPer keys a thread.  Where that is all there is to merge, the workgroups
-// from `merging` on write starts[v], the number of tokens below v, for v = 0 .. vocabulary.
-constexpr int kMergeKeys = kRun * kWays, kPer = 2;
-__global__ __launch_bounds__(kMergeThreads) void embed_first_merge_kernel(const u64* __restrict__ from, u64* __restrict__ to, int n, int merging, int64_t vocabulary, int* starts) {
+// The first merge, of runs of kRun keys, whose tokens a workgroup brings into LDS; workgroups from `merging` on fill, beginning with `first_fill`.
+__global__ __launch_bounds__(kMergeThreads) void embed_first_merge_kernel(const u64* __restrict__ from, u64* __restrict__ to, int n, int merging, char* filled, int64_t fill_bytes,
+                                                                          int64_t first_fill) {
+    if ((int)blockIdx.x >= merging) { fill<kMergeThreads>(filled, fill_bytes, first_fill + (int64_t)blockIdx.x - merging); return; }
     __shared__ u32 tokens[kMergeKeys];
-    const bool merges = (int)blockIdx.x < merging;
-    const int i0 = merges ? (int)blockIdx.x * kMergeThreads * kPer : 0, group = i0 / kMergeKeys * kMergeKeys;
-    const int here = n - group < kMergeKeys ? n - group : kMergeKeys;
-    for (int k = threadIdx.x; k < here; k += kMergeThreads) tokens[k] = (u32)(from[group + k] >> 32);
+    const int i = (int)blockIdx.x * kMergeThreads + threadIdx.x, group = i / kMergeKeys * kMergeKeys;
+    const int here = n - group < kMergeKeys ? n - group : kMergeKeys, runs = (here + kRun - 1) / kRun;
+#pragma unroll 4
+    for (int k = threadIdx.x; k < runs * kRun; k += kMergeThreads) tokens[k] = k < here ? (u32)(from[group + k] >> 32) : ~0u;
     __syncthreads();
-    int start[kWays], size[kWays], below[kWays];
+    if (i >= n) return;
+    const int own = (i - group) / kRun;
+    const u32 token = tokens[i - group];
+    int place = i - group - own * kRun;
 #pragma unroll
     for (int r = 0; r < kWays; ++r) {
-        start[r] = r * kRun;
-        size[r] = start[r] >= here ? 0 : here - start[r] < kRun ? here - start[r] : kRun;
+        if (r >= runs) break;
+        // equal tokens keep the order of their runs: those of runs before its own count as below it
+        const int there = below<9>(token + (r < own ? 1u : 0u), [&](int k) { return tokens[r * kRun + k]; });
+        place += r == own ? 0 : there;
     }
-    if (!merges) {
-        const int64_t v = (int64_t)((int)blockIdx.x - merging) * kMergeThreads + threadIdx.x;
-        if (v > vocabulary) return;
-        search_runs<u32>(tokens, start, size, here - 1, 10, (u32)v, below);
-        int all = 0;
-#pragma unroll
-        for (int r = 0; r < kWays; ++r) all += below[r];
-        starts[v] = all;
-        return;
-    }
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const int i = i0 + k * kMergeThreads + threadIdx.x;
-        if (i >= n) return;
-        const int own = (i - group) / kRun;
-        const u32 token = tokens[i - group];
-        // equal tokens keep the order of their runs: in those before its own they count as smaller
-        int low[kWays], left[kWays];
-#pragma unroll
-        for (int r = 0; r < kWays; ++r) { low[r] = start[r]; left[r] = r == own ? 0 : size[r]; }
-        for (int s = 0; s < 10; ++s) {
-#pragma unroll
-            for (int r = 0; r < kWays; ++r) {
-                const int half = left[r] >> 1, at = low[r] + half;
-                const u32 other = tokens[at < here ? at : here - 1];
-                const bool more = left[r] > 0 && other < token + (r < own ? 1u : 0u);
-                low[r] += more ? half + 1 : 0;
-                left[r] = more ? left[r] - half - 1 : half;
-            }
-        }
-        int place = i - group - own * kRun;
-#pragma unroll
-        for (int r = 0; r < kWays; ++r) place += r == own ? 0 : low[r] - start[r];
-        to[group + place] = from[i];
-    }
-}
-
-// starts[v]: the first sorted key of a token of v or more, for v = 0 .. vocabulary.
-__global__ __launch_bounds__(256) void embed_starts_kernel(const u64* keys, int n, int64_t vocabulary, int* starts) {
-    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v > vocabulary) return;
-    const u64 want = (u64)v << 32;
-    int low = 0, high = n;
-    while (low < high) {
-        const int mid = (low + high) >> 1;
-        if (keys[mid] < want) low = mid + 1; else high = mid;
-    }
-    starts[v] = low;
+    to[group + place] = from[i];
 }
 
 struct EmbedGrad {
-    const u64* keys;
-    const int* starts;
+    const u64* keys;         // sorted
     const char* dy;
     char* dw;
-    float* partial;          // two rows per window
-    int64_t dy_stride, n;
-    int cols, vocabulary, window;
+    float* partial;          // two rows per window: of the list that comes into it, of the one that begins in it and goes on
+    int64_t dy_stride;
+    int n, cols, window;
     float scale;
+    __device__ __forceinline__ u32 token(int i) const { return (u32)(keys[i] >> 32); }
+    __device__ __forceinline__ float* part(int w, int which, int c) const { return partial + (2 * (int64_t)w + which) * cols + c; }
 };
 
 // Lanes take eight neighbouring values each; blockIdx.y says which 512 columns.
 constexpr int kEmbedColumns = 512;
 
-// The rows of dy that keys[first .. end) name, added up; N of them under way.
-template <int DT, int N> __device__ __forceinline__ void add_rows(float (&sum)[8], const EmbedGrad& a, int64_t first, int64_t end, int c) {
-    constexpr int B = DTypeInfo<DT>::bytes;
-    int64_t i = first;
-    for (; i + N <= end; i += N) {
-        float v[N][8];
+template <int DT> __device__ __forceinline__ void store_row(const EmbedGrad& a, u32 token, int c, const float (&sum)[8]) {
+    float v[8];
 #pragma unroll
-        for (int k = 0; k < N; ++k) load_values<DT>(v[k], a.dy + ((int64_t)(u32)a.keys[i + k] * a.dy_stride + c) * B, a.cols - c);
+    for (int e = 0; e < 8; ++e) v[e] = sum[e] * a.scale;
+    store_values<DT>(v, a.dw + ((int64_t)token * a.cols + c) * DTypeInfo<DT>::bytes, a.cols - c);
+}
+
+// A wavefront adds up the lists, and parts of lists, of its window, kAtOnce rows of dy under way.  Bound by the latency of those: 8192 rows of 4096 bf16 values
+// in TODO us.
+template <int DT> __global__ __launch_bounds__(256) void embed_windows_kernel(EmbedGrad a) {
+    constexpr int B = DTypeInfo<DT>::bytes, kAtOnce = 8;
+    const int w = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = (int)blockIdx.y * kEmbedColumns + (threadIdx.x & 63) * 8;
+    const int first = w * a.window, end = first + a.window < a.n ? first + a.window : a.n;
+    if (first >= a.n || c >= a.cols) return;
+    float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    u32 token = a.token(first);
+    bool came_in = first > 0 && a.token(first - 1) == token;
+    for (int i = first; i < end; i += kAtOnce) {
+        float v[kAtOnce][8];
 #pragma unroll
-        for (int k = 0; k < N; ++k)
+        for (int k = 0; k < kAtOnce; ++k)
+            if (i + k < end) load_values<DT>(v[k], a.dy + ((int64_t)(u32)a.keys[i + k] * a.dy_stride + c) * B, a.cols - c);
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (i + k >= end) break;
+            if (token == kNoToken) return;    // there are none behind
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] += v[k][e];
-    }
-#pragma unroll 1
-    for (; i < end; ++i) {
-        float v[8];
-        load_values<DT>(v, a.dy + ((int64_t)(u32)a.keys[i] * a.dy_stride + c) * B, a.cols - c);
+            const u32 next = i + k + 1 < a.n ? a.token(i + k + 1) : kNoToken;
+            if (next != token) {
+                if (came_in) store_values<DT_F32>(sum, a.part(w, 0, c), a.cols - c);
+                else store_row<DT>(a, token, c, sum);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += v[e];
+                for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
+                came_in = false;
+                token = next;
+            } else if (i + k + 1 == end) {
+                store_values<DT_F32>(sum, a.part(w, came_in ? 0 : 1, c), a.cols - c);
+            }
+        }
     }
 }
 
-// Sums of the long lists' parts.  At most two lists longer than a window reach into one: the one that began before it (its part goes to row
-// 2 w) and the last one that begins in it (2 w + 1).
-template <int DT> __global__ __launch_bounds__(64) void embed_parts_kernel(EmbedGrad a) {
-    const int64_t w = blockIdx.x, first = w * a.window, end = first + a.window < a.n ? first + a.window : a.n;
-    const int c = (int)blockIdx.y * kEmbedColumns + threadIdx.x * 8;
-    if (c >= a.cols) return;
-#pragma unroll 1
-    for (int which = 0; which < 2; ++which) {
-        const u32 token = (u32)(a.keys[which ? end - 1 : first] >> 32);
-        if (token >= (u32)a.vocabulary) continue;
-        const int64_t start = a.starts[token], stop = a.starts[token + 1];
-        if (stop - start <= a.window || (which ? start < first : start >= first)) continue;
-        float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        add_rows<DT, 16>(sum, a, start > first ? start : first, stop < end ? stop : end, c);
-        store_values<DT_F32>(sum, a.partial + (2 * w + which) * a.cols + c, a.cols - c);
+// The list that begins in window blockIdx.x and goes on: its parts are added up, every fourth by a wavefront, and the four sums then.
+template <int DT> __global__ __launch_bounds__(256) void embed_borders_kernel(EmbedGrad a) {
+    __shared__ float sums[3][64][9];
+    const int w = blockIdx.x, first = w * a.window, end = first + a.window;
+    if (end >= a.n) return;
+    const u32 token = a.token(end - 1);
+    if (token == kNoToken || a.token(end) != token || (first > 0 && a.token(first) == token && a.token(first - 1) == token)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = (int)blockIdx.y * kEmbedColumns + lane * 8;
+    int last = w;    // the last window that the list reaches into
+    for (;;) {
+        const int64_t at = (int64_t)(last + 1 + lane) * a.window;
+        const uint64_t in = __builtin_amdgcn_ballot_w64(at < a.n && a.token(at < a.n ? (int)at : 0) == token);
+        const int more = in == ~0ull ? 64 : __builtin_ctzll(~in);
+        last += more;
+        if (more < 64) break;
     }
-}
-
-// A wavefront writes 512 columns of a row of dw.
-template <int DT> __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedGrad a) {
-    constexpr int B = DTypeInfo<DT>::bytes;
-    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = (int)blockIdx.y * kEmbedColumns + (threadIdx.x & 63) * 8;
-    if (row >= a.vocabulary || c >= a.cols) return;
-    const int start = a.starts[row], stop = a.starts[row + 1];
-    char* out = a.dw + (row * a.cols + c) * B;
     float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (stop - start > a.window) {
-        const int64_t last = (stop - 1) / a.window;
-        int64_t w = start / a.window;
-        // the window in which the list begins, then those that it goes on into
-        load_values<DT_F32>(sum, a.partial + (2 * w + 1) * a.cols + c, a.cols - c);
+    if (c < a.cols) {
+        if (wave == 0) load_values<DT_F32>(sum, a.part(w, 1, c), a.cols - c);
 #pragma unroll 8
-        for (++w; w <= last; ++w) {
+        for (int j = w + 1 + wave; j <= last; j += 4) {
             float v[8];
-            load_values<DT_F32>(v, a.partial + 2 * w * a.cols + c, a.cols - c);
+            load_values<DT_F32>(v, a.part(j, 0, c), a.cols - c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] += v[e];
         }
-    } else if (stop > start) {
-        add_rows<DT, 4>(sum, a, start, stop, c);
     }
+    if (wave > 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] *= a.scale;
-    store_values<DT>(sum, out, a.cols - c);
+        for (int e = 0; e < 8; ++e) sums[wave - 1][lane][e] = sum[e];
+    }
+    __syncthreads();
+    if (wave > 0 || c >= a.cols) return;
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += sums[q][lane][e];
+    store_row<DT>(a, token, c, sum);
 }
 
 // A wavefront writes 512 columns of y's rows.
@@ -295,24 +280,24 @@ int validate(const char* what, int index_bytes, int64_t n, int dtype, int64_t vo
     if (n < 0 || vocabulary < 0 || cols < 0) return fail(FO_ERR_INVALID_ARGUMENT, "%s: negative size", what);
     if (index_bytes != 4 && index_bytes != 8) return fail(FO_ERR_INVALID_ARGUMENT, "%s: tokens of %d bytes", what, index_bytes);
     if (dtype < FO_F32 || dtype > FO_F16) return fail(FO_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
-    if (n > FO_EMBEDDING_MOST_TOKENS || vocabulary > FO_EMBEDDING_MOST_ROWS || cols > kMostCols) return fail(FO_ERR_UNSUPPORTED, "%s: too many tokens, rows or columns", what);
+    // fewer than 2^32 threads fill
+    if (n > FO_EMBEDDING_MOST_TOKENS || vocabulary > FO_EMBEDDING_MOST_ROWS || cols > kMostCols || vocabulary * cols > (int64_t)1 << 37) return fail(FO_ERR_UNSUPPORTED, "%s: too many tokens, rows or columns", what);
     return 0;
 }
 
-// At most twice as many windows as a window has positions, so that neither a list's parts nor their sums keep one wavefront long.
+// At most 1024 windows of at least 16 positions, so that neither a window nor the parts of one list keep a workgroup long; at most 4096 positions.
 int window_of(int64_t n) {
-    int w = 64;
-    while (2 * (int64_t)w * w < n && w < 4096) w *= 2;
+    int w = 16;
+    while ((int64_t)w * 1024 < n && w < 4096) w *= 2;
     return w;
 }
 
-struct Layout { int64_t keys, more, starts, partial, total; };
-Layout layout(int64_t n, int64_t vocabulary, int64_t cols) {
+struct Layout { int64_t keys, more, partial, total; };
+Layout layout(int64_t n, int64_t cols) {
     const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
     Layout l{};
     l.more = up(n * 8);
-    l.starts = l.more + up(n * 8);
-    l.partial = l.starts + up((vocabulary + 1) * 4);
+    l.partial = l.more + (n > fo::kRun ? up(n * 8) : 0);
     const int64_t w = window_of(n);
     l.total = l.partial + (n > w ? up((n + w - 1) / w * 2 * cols * 4) : 0);
     return l;
@@ -327,12 +312,11 @@ template <int DT> int forward(const fo::Tokens& t, int64_t n, const void* weight
 }
 
 template <int DT> int sums(const fo::EmbedGrad& a, hipStream_t s) {
-    const unsigned across = blocks(a.cols, fo::kEmbedColumns);
-    if (a.n > a.window) {
-        fo::embed_parts_kernel<DT><<<dim3(blocks(a.n, a.window), across), dim3(64), 0, s>>>(a);
-        if (int rc = check_hip(hipGetLastError(), "fo_embedding_backward")) return rc;
-    }
-    fo::embed_rows_kernel<DT><<<dim3(blocks(a.vocabulary, 4), across), dim3(256), 0, s>>>(a);
+    const unsigned across = blocks(a.cols, fo::kEmbedColumns), windows = blocks(a.n, a.window);
+    fo::embed_windows_kernel<DT><<<dim3((windows + 3) / 4, across), dim3(256), 0, s>>>(a);
+    if (int rc = check_hip(hipGetLastError(), "fo_embedding_backward")) return rc;
+    if (windows == 1) return 0;
+    fo::embed_borders_kernel<DT><<<dim3(windows - 1, across), dim3(256), 0, s>>>(a);
     return check_hip(hipGetLastError(), "fo_embedding_backward");
 }
 
@@ -355,7 +339,7 @@ int fo_embedding(const void* tokens, int index_bytes, int64_t n_tokens, const vo
 
 int64_t fo_embedding_backward_workspace(int64_t n_tokens, int64_t vocabulary, int64_t cols) {
     if (int rc = validate("fo_embedding_backward", 8, n_tokens, FO_F32, vocabulary, cols)) return rc;
-    return layout(n_tokens, vocabulary, cols).total;
+    return layout(n_tokens, cols).total;
 }
 
 int fo_embedding_backward(const void* tokens, int index_bytes, int64_t n_tokens, const void* dy, int dtype, int64_t dy_stride, int64_t vocabulary, int64_t cols,
@@ -363,42 +347,33 @@ int fo_embedding_backward(const void* tokens, int index_bytes, int64_t n_tokens,
     const char* what = "fo_embedding_backward";
     if (int rc = validate(what, index_bytes, n_tokens, dtype, vocabulary, cols)) return rc;
     if (vocabulary == 0 || cols == 0) return 0;
-    const Layout l = layout(n_tokens, vocabulary, cols);
+    const Layout l = layout(n_tokens, cols);
     if (!dw || (n_tokens > 0 && (!tokens || !dy))) return fail(FO_ERR_INVALID_ARGUMENT, "%s: tokens, dy and dw must not be NULL", what);
-    if (!workspace || workspace_bytes < l.total || (uintptr_t)workspace & 255)
+    if (n_tokens > 0 && (!workspace || workspace_bytes < l.total || (uintptr_t)workspace & 255))
         return fail(FO_ERR_INVALID_ARGUMENT, "a workspace of %lld bytes, aligned to 256, is needed", (long long)l.total);
     const hipStream_t s = (hipStream_t)stream;
     char* base = (char*)workspace;
     fo::u64 *keys = (fo::u64*)base, *other = (fo::u64*)(base + l.more);
-    int* starts = (int*)(base + l.starts);
     const int n = (int)n_tokens;
-    const unsigned starting = blocks(vocabulary + 1, 256);
-    if (n <= fo::kMergeKeys && n > 0) {
-        fo::embed_sort_kernel<<<dim3(blocks(n, fo::kRun)), dim3(fo::kSortThreads), 0, s>>>(fo::Tokens{tokens, index_bytes}, n, vocabulary, padding, other);
+    // an odd number of merges ends in the other array
+    int merges = 0;
+    for (int64_t length = fo::kRun; length < n; length *= fo::kWays) ++merges;
+    fo::u64 *from = merges & 1 ? other : keys, *to = merges & 1 ? keys : other;
+    const int64_t bytes = vocabulary * cols * (dtype == FO_F32 ? 4 : 2), fills = (bytes + fo::kFillBytes - 1) / fo::kFillBytes, fills_first = merges > 0 ? fills / 2 : fills;
+    const unsigned sorting = blocks(n, fo::kRun), merging = blocks(n, fo::kMergeThreads);
+    fo::embed_sort_kernel<<<dim3(sorting + (unsigned)fills_first), dim3(fo::kRun), 0, s>>>(fo::Tokens{tokens, index_bytes}, n, vocabulary, padding, from, (int)sorting, (char*)dw, bytes);
+    if (int rc = check_hip(hipGetLastError(), what)) return rc;
+    if (n == 0) return 0;
+    int steps = 10;    // of a search among `length` keys
+    for (int64_t length = fo::kRun; length < n; length *= fo::kWays, steps += 4) {
+        if (length == fo::kRun)
+            fo::embed_first_merge_kernel<<<dim3(merging + (unsigned)(fills - fills_first)), dim3(fo::kMergeThreads), 0, s>>>(from, to, n, (int)merging, (char*)dw, bytes, fills_first);
+        else
+            fo::embed_merge_kernel<<<dim3(merging), dim3(fo::kMergeThreads), 0, s>>>(from, to, n, (int)length, steps);
         if (int rc = check_hip(hipGetLastError(), what)) return rc;
-        const unsigned merging = blocks(n, fo::kMergeThreads * fo::kPer);
-        fo::embed_first_merge_kernel<<<dim3(merging + starting), dim3(fo::kMergeThreads), 0, s>>>(other, keys, n, (int)merging, vocabulary, starts);
-        if (int rc = check_hip(hipGetLastError(), what)) return rc;
-    } else {
-        // where the keys are to end up decides where they begin
-        int merges = 0;
-        for (int64_t length = fo::kRun; length < n; length *= fo::kWays) ++merges;
-        fo::u64 *from = merges & 1 ? other : keys, *to = merges & 1 ? keys : other;
-        if (n > 0) {
-            fo::embed_sort_kernel<<<dim3(blocks(n, fo::kRun)), dim3(fo::kSortThreads), 0, s>>>(fo::Tokens{tokens, index_bytes}, n, vocabulary, padding, from);
-            if (int rc = check_hip(hipGetLastError(), what)) return rc;
-        }
-        int steps = 10;    // of a search among `length` keys
-        for (int64_t length = fo::kRun; length < n; length *= fo::kWays, steps += 4) {
-            if (length == fo::kRun) fo::embed_first_merge_kernel<<<dim3(blocks(n, fo::kMergeThreads * fo::kPer)), dim3(fo::kMergeThreads), 0, s>>>(from, to, n, INT32_MAX, 0, nullptr);
-            else fo::embed_merge_kernel<<<dim3(blocks(n, fo::kMergeThreads)), dim3(fo::kMergeThreads), 0, s>>>(from, to, n, (int)length, steps);
-            if (int rc = check_hip(hipGetLastError(), what)) return rc;
-            fo::u64* t = from; from = to; to = t;
-        }
-        fo::embed_starts_kernel<<<dim3(starting), dim3(256), 0, s>>>(keys, n, vocabulary, starts);
-        if (int rc = check_hip(hipGetLastError(), what)) return rc;
+        fo::u64* t = from; from = to; to = t;
     }
-    const fo::EmbedGrad a{keys, starts, (const char*)dy, (char*)dw, (float*)(base + l.partial), dy_stride, n_tokens, (int)cols, (int)vocabulary, window_of(n_tokens), scale};
+    const fo::EmbedGrad a{keys, (const char*)dy, (char*)dw, (float*)(base + l.partial), dy_stride, n, (int)cols, window_of(n), scale};
     switch (dtype) {
         case FO_F32: return sums<fo::DT_F32>(a, s);
         case FO_BF16: return sums<fo::DT_BF16>(a, s);

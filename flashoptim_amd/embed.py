@@ -117,7 +117,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
     Returns:
         ``(*tokens.shape, width)`` in the type of `weight`.
 
-    The gradient is dense, summed in fp32 in the order of the tokens and rounded once, so it repeats to the bit.  A token outside the
+    The gradient is dense, summed in fp32 in a fixed order and rounded once, so it repeats to the bit.  A token outside the
     vocabulary makes a row of NaNs and gives no gradient (the call does not wait for the GPU to look at the tokens).
 
     Raises:

@@ -336,8 +336,8 @@ int fo_rms_norm_backward(const void *s, int stream_dtype, int64_t s_stride, cons
 /*
  * Rows of an embedding matrix:  y[i] = scale * weight[tokens[i]], rounded once.  tokens: index_bytes 4 or 8 each, contiguous; weight:
  * vocabulary x cols of `dtype`; y contiguous.  A token outside 0 .. vocabulary - 1 makes a row of NaNs.
- * The gradient of the matrix (vocabulary x cols, contiguous):  dw[v] = scale * sum of dy[i] over the i with tokens[i] = v, in the order of i, in fp32,
- * rounded once; rows of no token are zero, and so is row `padding` (-1: none); tokens outside the vocabulary are left out.
+ * The gradient of the matrix (vocabulary x cols, contiguous):  dw[v] = scale * sum of dy[i] over the i with tokens[i] = v, in fp32 and a fixed
+ * order, rounded once; rows of no token are zero, and so is row `padding` (-1: none); tokens outside the vocabulary are left out.
  * workspace: fo_embedding_backward_workspace bytes of device memory, aligned to 256.
  */
 #define FO_EMBEDDING_MOST_TOKENS 33554432

@@ -99,11 +99,13 @@ def test_many_tokens(n, kind):
 
 
 def test_the_order_of_summing_is_that_of_the_tokens():
-    """A list within one window is a plain sum from the first position to the last: it equals that sum in fp32 to the bit."""
+    """A list within one window (sixteen neighbours of the sorted tokens, counted from their first) is a plain sum in fp32 from the first position to the
+    last; here every list is one window."""
     fo = _fo()
-    n, vocabulary, width = 3000, 200, 16
-    tokens = _tokens(n, vocabulary, "any")
-    dy = torch.randn(n, width) * torch.exp2(torch.randint(-12, 12, (n, 1)).float())
+    vocabulary, width = 200, 16
+    g = torch.Generator().manual_seed(3)
+    tokens = torch.arange(vocabulary).repeat_interleave(16)[torch.randperm(16 * vocabulary, generator=g)]
+    dy = torch.randn(16 * vocabulary, width, generator=g) * torch.exp2(torch.randint(-12, 12, (16 * vocabulary, 1), generator=g).float())
     want = torch.zeros(vocabulary, width)
     for i, t in enumerate(tokens.tolist()):
         want[t] += dy[i]

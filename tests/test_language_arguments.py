@@ -58,13 +58,14 @@ def test_embedding_checks_its_arguments():
     assert call(weight=None) == INVALID and call(y=None) == INVALID
     for bad in (dict(dy=None), dict(dw=None), dict(workspace=None), dict(workspace=SOME + 128), dict(size=10)):
         assert back(**bad) == INVALID, bad
-    for large in (dict(n=(1 << 25) + 1), dict(vocabulary=1 << 23), dict(cols=1 << 26)):
+    for large in (dict(n=(1 << 25) + 1), dict(vocabulary=1 << 23), dict(cols=1 << 26), dict(vocabulary=(1 << 23) - 1, cols=1 << 15)):
         assert call(**large) == UNSUPPORTED and back(**large) == UNSUPPORTED, large
     assert call(n=0, tokens=None) == 0 and back(vocabulary=0, dw=None) == 0
     size = lib.fo_embedding_backward_workspace
-    assert size(-1, 1, 1) == INVALID and size(0, 1000, 8) == 4096
-    # keys twice, starts, two rows a window once there are two windows
-    assert size(64, 10, 8) == 2 * 512 + 256 and size(512, 10, 8) == 2 * 4096 + 256 + 8 * 2 * 8 * 4 and size(513, 10, 8) == 2 * 4352 + 256 + 9 * 2 * 8 * 4 // 256 * 256 + 256
+    assert size(-1, 1, 1) == INVALID and size(0, 1000, 8) == 0
+    # keys, a second array of them from the second run on, two rows a window of 16 from the second on
+    assert size(16, 10, 8) == 256 and size(17, 10, 8) == 256 + 2 * 2 * 8 * 4 * 2 and size(512, 10, 8) == 4096 + 32 * 2 * 8 * 4
+    assert size(513, 10, 8) == 2 * 4352 + -(-33 * 2 * 8 * 4 // 256) * 256
 
 
 def test_loss_checks_its_arguments():
