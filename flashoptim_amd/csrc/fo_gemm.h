@@ -28,6 +28,12 @@
 // r & 7; 1000 x 1000 in all took 5 % less).  Scaled operands keep 2 group and 2 group + 1, a lane's two scales are neighbours then, and
 // their conflicts are hidden: an order without them took as long.
 // The order is applied to the address that a lane loads from.
+//
+// Either operand of 16-bit values may lie the other way round in memory, the contracted axis down the rows: A[k][i], B[k][j] with i and j adjacent (KA, KB).  Its stage
+// is then 64 rows of a tile's width, of the same number of bytes, and the operand of an instruction comes out of LDS through two transposing reads: sixteen lanes
+// read four rows of sixteen values and get four values of a column each.  A 32-byte piece of a row is what one such read takes; row k keeps its pieces shifted by
+// turned_shift(k), so that the sixteen rows that a wavefront reads at a time lie in all banks.  Rows need not be filled up to whole stages: those behind the last are read as
+// copies of it, the other operand holds zeros for them.
 #pragma once
 
 #include "fo_device.h"
@@ -37,6 +43,8 @@ namespace fo {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -104,6 +112,9 @@ struct Operand {
     const uint8_t* scales;
     int64_t scale_stride;
     int rows;
+    int depth;              // turned operands: how many rows there are along the contracted axis; `rows`, a multiple of 8, is how long they are
+    int64_t part_stride;    // products in parts: bytes from a part of the values to the next
+    u32 order;              // and which part each segment of the contraction takes, two bits each
 };
 
 // The matrix instructions are inline asm so that an accumulator stays in the registers it is in (the compiler's own form lets
@@ -111,7 +122,7 @@ struct Operand {
 // not see: an accumulator may be read by other instructions 18 wait states after the last instruction that wrote it, see
 // multiply().  Results feed the next instruction on the same accumulator without a wait, at least three others lie between.
 struct F16Product {
-    static constexpr bool kScaled = false;
+    static constexpr bool kScaled = false, kParts = false;
     typedef f16x8 Frag;
     template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int, int) {
         asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
@@ -119,16 +130,22 @@ struct F16Product {
 };
 
 struct Bf16Product {
-    static constexpr bool kScaled = false;
+    static constexpr bool kScaled = false, kParts = false;
     typedef bf16x8 Frag;
     template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int, int) {
         asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     }
 };
 
+// Values in three bf16 parts each, part after part in memory: the contraction is kSegments products of parts one after the other, each over whole stages.
+struct Bf16PartsProduct : Bf16Product {
+    static constexpr bool kParts = true;
+};
+constexpr int kSegments = 6;
+
 // HALF: which byte of the two scales is meant.
 struct Mx4Product {
-    static constexpr bool kScaled = true;
+    static constexpr bool kScaled = true, kParts = false;
     typedef i32x4 Frag;
     template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int a_scales, int b_scales) {
         if constexpr (HALF == 0)
@@ -163,7 +180,7 @@ __device__ __forceinline__ const char* uniform(const char* p) {
     return (const char*)(((uint64_t)hi << 32) | lo);
 }
 
-template <class Product, int WT, int STAGES> struct GemmTile {
+template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> struct GemmTile {
     static constexpr int kStages = STAGES;        // in LDS, 2 to 4
     static constexpr int kTile = 2 * WT;          // rows and columns of a workgroup's tile
     static constexpr int kFrags = WT / 16;        // 16-row pieces of a wavefront's operands
@@ -179,9 +196,14 @@ template <class Product, int WT, int STAGES> struct GemmTile {
     static_assert(kStages * kBuffer <= 163840 && (kStages - 1) * kLoads <= 63, "what LDS holds, what the counter of loads under way counts to");
     static constexpr int kLds = kStages * kBuffer > 4 * kStripBytes ? kStages * kBuffer : 4 * kStripBytes;
 
+    static constexpr int kPieces32 = WT / 8;      // of 32 bytes, in a stage row of a turned operand
+    static_assert(!Product::kScaled || (!KA && !KB), "codes have no transposing read");
+
     typedef typename Product::Frag Frag;
 
     f32x4 acc[kFrags][kFrags];
+    int first_stage = 0;       // where along the contraction this product begins
+    int segment_stages = 0;    // products in parts: stages of a segment
     char* smem;
     unsigned smem_address;
     int wave, lane;
@@ -192,8 +214,28 @@ template <class Product, int WT, int STAGES> struct GemmTile {
     // ------------------------------------------------------------------------------------------- staging
     __device__ __forceinline__ static int buffer_of(int stage) { return (kStages == 3 ? stage % 3 : stage & (kStages - 1)) * kBuffer; }
     __device__ __forceinline__ static int place_of(int row) { return (row >> 1) & 7; }
+    __device__ __forceinline__ static int turned_shift(int k) {
+        return kPieces32 % 8 == 0 ? (k & 3) | (k >> 3 & 1) << 2 : (k >> 1 & 1) | (k >> 3 & 1) << 1;
+    }
+    // Where piece `at` of stage row k lies in that row.
+    __device__ __forceinline__ static int turned_place(int at, int k) {
+        if constexpr (kPieces32 % 8 == 0) return at ^ turned_shift(k);
+        const int place = at + turned_shift(k);
+        return place < kPieces32 ? place : place - kPieces32;
+    }
+    __device__ __forceinline__ static int turned_piece(int place, int k) {    // and back
+        if constexpr (kPieces32 % 8 == 0) return place ^ turned_shift(k);
+        const int at = place - turned_shift(k);
+        return at < 0 ? at + kPieces32 : at;
+    }
     struct Loader {
         unsigned row[kRowLoads];
+        bool turned;
+        int64_t part_stride;
+        u32 order;
+        int64_t step;            // bytes from a stage to the next
+        unsigned line;           // turned: bytes from a row to the next, and the rows that there are
+        int depth;
         unsigned scale[kScaleLoads > 0 ? kScaleLoads : 1];
         unsigned past_half, past_half_scale;   // what a lane steps back by when the last stage is half of one
         const char* base;
@@ -204,6 +246,22 @@ template <class Product, int WT, int STAGES> struct GemmTile {
         const char* data = first ? a.data : b.data;
         const int64_t stride = first ? a.stride : b.stride;
         const int at = first ? row0 : col0, left = (first ? a.rows : b.rows) - at;
+        l.turned = first ? KA : KB;
+        l.step = l.turned ? 64 * stride : kStageBytes;
+        l.line = (unsigned)stride;
+        l.depth = first ? a.depth : b.depth;
+        l.part_stride = first ? a.part_stride : b.part_stride;
+        l.order = first ? a.order : b.order;
+        if ((KA || KB) && l.turned) {
+            l.base = uniform(data + at * 2);
+#pragma unroll
+            for (int i = 0; i < kRowLoads; ++i) {
+                const int k = turned_row(i), byte = turned_byte(i) % (2 * kTile);
+                const int chunk = turned_piece(byte >> 5, k) * 2 + (byte >> 4 & 1), last = left / 8 - 1;    // of 16 bytes
+                l.row[i] = (unsigned)(k * stride) + (chunk < last ? chunk : last) * 16;
+            }
+            return;
+        }
         l.base = uniform(data + at * stride);
         l.past_half = ((lane & 7) ^ place_of(lane >> 3)) >= 4 ? kHalfBytes : 0;
 #pragma unroll
@@ -225,17 +283,44 @@ template <class Product, int WT, int STAGES> struct GemmTile {
             }
         }
     }
+    // Turned operands: which byte of the wavefront's operand in a stage the lane's part of load i is, and in which row that is.
+    __device__ __forceinline__ int turned_byte(int i) const { return (wave & 1) * (kRowLoads * 1024) + i * 1024 + lane * 16; }
+    __device__ __forceinline__ int turned_row(int i) const { return turned_byte(i) / (2 * kTile); }
+
     // The i-th load of a stage.  half: the rows end in the middle of the stage, its second half repeats the first.
     __device__ __forceinline__ void load(const Loader& l, int i, int stage, bool half) const {
         const unsigned buffer = smem_address + buffer_of(stage);
+        const char* base = l.base;
+        stage += first_stage;
+        if constexpr (Product::kParts) {
+            int segment = 0;
+#pragma unroll
+            for (int k = 1; k < kSegments; ++k) segment += stage >= k * segment_stages ? 1 : 0;
+            stage -= segment * segment_stages;
+            base += (int64_t)(l.order >> 2 * segment & 3) * l.part_stride;
+        }
+        if ((KA || KB) && l.turned) {
+            const int last = l.depth - 1 - stage * 64;    // row of the stage
+            unsigned at = l.row[i];
+            if (last < 63) {
+                const int k = turned_row(i);
+                at -= k > last ? (unsigned)(k - last) * l.line : 0u;
+            }
+            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, at, base + stage * l.step);
+            return;
+        }
         if (i < kRowLoads) {
             const unsigned past = i & 1 ? kHalfBytes - l.past_half : l.past_half;   // eight rows on the halves change places
-            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, l.row[i] - (half ? past : 0), l.base + (int64_t)stage * kStageBytes);
+            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, l.row[i] - (half ? past : 0), base + (int64_t)stage * kStageBytes);
         } else if constexpr (Product::kScaled) {
             const int k = i - kRowLoads;
             load_to_lds4(buffer + kScaleOffset + (wave * kScaleLoads + k) * 256, l.scale[k] - (half ? l.past_half_scale : 0),
                          l.scale_base + (int64_t)stage * (kStageBytes / 16));
         }
+    }
+
+    __device__ __forceinline__ static i16x4 transposed(const char* p) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)p);
     }
 
     // What a wavefront multiplies in one phase; of a scaled product also its scales, as read and as the instructions take them.
@@ -248,6 +333,15 @@ template <class Product, int WT, int STAGES> struct GemmTile {
     __device__ __forceinline__ void read(Operands& to, int f, int stage, int half, bool short_stage) const {
         const bool is_b = f < kFrags;
         const int i = is_b ? f : f - kFrags, group = lane >> 4;
+        if ((KA && !is_b) || (KB && is_b)) {
+            const int k = half * 32 + group * 8 + (lane >> 2 & 3), piece = (is_b ? wave & 1 : wave >> 1) * kFrags + i;
+            const char* from = smem + buffer_of(stage) + (is_b ? kTile * kStageBytes : 0) + (lane & 3) * 8;
+            const i16x4 lo = transposed(from + k * (2 * kTile) + turned_place(piece, k) * 32);
+            const i16x4 hi = transposed(from + (k + 4) * (2 * kTile) + turned_place(piece, k + 4) * 32);
+            const i16x8 all = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            (is_b ? to.b[i] : to.a[i]) = __builtin_bit_cast(Frag, all);
+            return;
+        }
         const int row = (is_b ? kTile + (wave & 1) * WT : (wave >> 1) * WT) + i * 16 + (lane & 15);
         const int piece = short_stage ? group : Product::kScaled ? 2 * group + half : group + 4 * half;
         (is_b ? to.b[i] : to.a[i]) = *reinterpret_cast<const Frag*>(smem + buffer_of(stage) + row * kStageBytes + ((piece ^ place_of(row)) * 16));

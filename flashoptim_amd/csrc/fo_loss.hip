@@ -8,18 +8,20 @@
 // Forward: a tile of z stays in a workgroup's accumulators; out go each row's maximum, its sum of exponentials relative to that, and the
 // target's logit where the tile holds it: 8 bytes for a row of a wavefront's part of the tile.  Another launch joins the parts.
 // Backward: a piece of the vocabulary at a time.  The piece's logits are computed again (a product more, and nothing of tokens x vocabulary size kept
-// from the forward pass), turned into G in the same accumulators and written as rows and as columns, 16 bits a value; then one product adds
+// from the forward pass), turned into G in the same accumulators and written, 16 bits a value; then one product adds
 // G's share to dx (fp32 sums between pieces), another makes the piece's rows of dW, complete.
 //
 // Types.  bf16 and fp16 operands go into the matrix cores as they are, sums are fp32.  G is rounded to the operands' type once, as the
 // other operand of its products is; the factors f_i are first divided by the largest of them (and multiplied by 2^15 for fp16, so that probabilities down to 2^-39
 // survive), which the products' results are multiplied by at the end: where all are equal, as in a mean, they are 1, and the entry p - 1 of an unlikely
-// target rounds to almost itself.  fp32 operands are cut into three bf16 parts of 8 bits each, a = a1 + a2 + a3
+// target rounds to almost itself.  What the target's entry, by far the largest of most rows, loses in its rounding goes into dx all the same: that times the
+// target's row of W is added in fp32.  fp32 operands are cut into three bf16 parts of 8 bits each, a = a1 + a2 + a3
 // exactly, and the six products a3 b1, a2 b2, a1 b3, a2 b1, a1 b2, a1 b1 are one contraction over six times the length: what is left
 // out is below 2^-23 of a product.  The small ones come first, so that the sums are small while most of the additions round.
 //
-// Rows of operands are whole multiples of 32 values, filled up with zeros: matrices that are so already are read in place, others are laid out
-// first.  Rows of ignored targets are left out of dW by zeros on both sides, so that what stands in them (infinities, NaN) does not matter.
+// Rows of operands are whole multiples of 32 values (64 in parts), filled up with zeros: matrices that are so already are read in place, others are laid out
+// first.  G = f (p - ...) is written once, by rows, and read by rows for dx and by columns for dW, W by rows for the logits and by columns for dx: the product core reads
+// either way.  Rows of ignored targets are left out of dW by zeros on both sides, so that what stands in them (infinities, NaN) does not matter: x is copied for that.
 #include "fo_gemm.h"
 #include "fo_host.h"
 
@@ -32,15 +34,27 @@ constexpr int kIgnored = -1, kNone = -2;    // labels
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // ------------------------------------------------------------------------------------------- operands
-// Where eight neighbouring values of a row go, as the matrix instructions' operands have them.  PARTS = 1: the values; 6: the three parts of
-// each, in the order that this side of the product needs, `length` values apart.
+// Eight neighbouring values of a row as the matrix instructions' operands have them: rounded to a 16-bit type, or the three parts of each, `part_stride` bytes apart.
+// Returned is what was lost of v[at] by that (0 where at is none of them).
 template <int DT> struct OperandOf {
     static constexpr int kParts = 1;
-    template <bool RIGHT> __device__ __forceinline__ static void store(const float (&v)[8], char* p, int64_t) { store_values<DT>(v, p, 8); }
+    __device__ __forceinline__ static float store(const float (&v)[8], char* p, int64_t, int at) {
+        Pack<2, 8> d;
+        float lost = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+            float a, b;
+            narrow_pair<DT, 8>(d, k, v[k], v[k + 1], a, b);
+            if (at == k) lost = v[k] - a;
+            if (at == k + 1) lost = v[k + 1] - b;
+        }
+        store_piece<2, 8>(d, p, 8);
+        return lost;
+    }
 };
 template <> struct OperandOf<DT_F32> {
-    static constexpr int kParts = 6;
-    template <bool RIGHT> __device__ __forceinline__ static void store(const float (&v)[8], char* p, int64_t length) {
+    static constexpr int kParts = 3;
+    __device__ __forceinline__ static float store(const float (&v)[8], char* p, int64_t part_stride, int) {
         u32x4 part[3];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -50,9 +64,9 @@ template <> struct OperandOf<DT_F32> {
 #pragma unroll
             for (int i = 0; i < 3; ++i) part[i][k] = __builtin_amdgcn_perm(hi[i], lo[i], 0x07060302u);
         }
-        constexpr int kLeft[6] = {2, 1, 0, 1, 0, 0}, kRight[6] = {0, 1, 2, 0, 1, 0};
 #pragma unroll
-        for (int i = 0; i < 6; ++i) *reinterpret_cast<FO_GLOBAL u32x4*>((FO_GLOBAL char*)p + i * length * 2) = part[RIGHT ? kRight[i] : kLeft[i]];
+        for (int i = 0; i < 3; ++i) *reinterpret_cast<FO_GLOBAL u32x4*>((FO_GLOBAL char*)p + i * part_stride) = part[i];
+        return 0.0f;
     }
     // Eight bits of the significand at a time, cut off: nothing overflows, and the rest is exact.
     __device__ __forceinline__ static void cut(float x, u32 (&part)[3]) {
@@ -64,54 +78,27 @@ template <> struct OperandOf<DT_F32> {
         part[2] = as_u32(rest - as_f32(part[1])) & 0xffff0000u;
     }
 };
+// Which part each segment of a product in parts takes, of its left and of its right operand: 2 1 0 1 0 0 and 0 1 2 0 1 0, the first in the low bits.
+constexpr u32 kLeftOrder = 2u | 1u << 2 | 0u << 4 | 1u << 6, kRightOrder = 0u | 1u << 2 | 2u << 4 | 0u << 6 | 1u << 8;
 
 struct FormArgs {
     const char* x;
-    char *rows_out, *turned_out;          // the rows of x, and its columns, as operand rows; either may be null
-    const int* labels;                    // rows of x whose label is kIgnored count as zeros; or null
-    int64_t stride;                       // of x, in values
-    int rows, cols;                       // of x
-    int rows_length, turned_length;       // of a part of an operand's row: what is contracted, filled up to a multiple of 32
+    char* out;
+    const int* labels;        // rows of x whose label is kIgnored count as zeros; or null
+    int64_t stride;           // of x, in values
+    int64_t part_stride;      // of out, in bytes
+    int rows, cols;           // of x
+    int out_rows, length;     // of out: filled up with zeros
 };
-// 64 x 64 values a workgroup, read once.  Bound by memory: the 16384 x 4096 bf16 rows of a piece of a weight turned in 64 us (4.2 TB/s).
-template <int DT, bool RIGHT> __global__ __launch_bounds__(256) void form_kernel(FormArgs a) {
-    constexpr int B = DTypeInfo<DT>::bytes;
-    __shared__ float tile[64][65];
-    const int across = (a.cols + 63) / 64;
-    const int row0 = (int)(blockIdx.x / across) * 64, col0 = (int)(blockIdx.x % across) * 64;
-    const int piece = threadIdx.x & 7, line = threadIdx.x >> 3;
-    float v[2][8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = row0 + line + h * 32, c = col0 + piece * 8;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[h][k] = 0.0f;
-        if (r < a.rows && c < a.cols && !(a.labels && a.labels[r] == kIgnored)) load_values<DT>(v[h], a.x + (r * a.stride + c) * B, a.cols - c);
-    }
-    if (a.rows_out) {
-        const int64_t row_bytes = (int64_t)a.rows_length * OperandOf<DT>::kParts * 2;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = row0 + line + h * 32, c = col0 + piece * 8;
-            if (r < a.rows && c < a.rows_length) OperandOf<DT>::template store<RIGHT>(v[h], a.rows_out + r * row_bytes + c * 2, a.rows_length);
-        }
-    }
-    if (!a.turned_out) return;
-    const int64_t row_bytes = (int64_t)a.turned_length * OperandOf<DT>::kParts * 2;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) tile[line + h * 32][piece * 8 + k] = v[h][k];
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        // a wavefront takes eight columns, its lanes' pieces of one column are neighbours in memory
-        const int c = line + h * 32;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[h][k] = tile[piece * 8 + k][c];
-        if (col0 + c < a.cols && row0 + piece * 8 < a.turned_length)
-            OperandOf<DT>::template store<true>(v[h], a.turned_out + (col0 + c) * row_bytes + (row0 + piece * 8) * 2, a.turned_length);
-    }
+// Rows as operand rows, eight values a thread.  Bound by memory: 8192 x 4096 bf16 in TODO us.
+template <int DT> __global__ __launch_bounds__(256) void form_kernel(FormArgs a) {
+    const int pieces = a.length / 8;
+    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, r = k / pieces;
+    const int c = (int)(k - r * pieces) * 8;
+    if (r >= a.out_rows) return;
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (r < a.rows && c < a.cols && !(a.labels && a.labels[r] == kIgnored)) load_values<DT>(v, a.x + (r * a.stride + c) * DTypeInfo<DT>::bytes, a.cols - c);
+    OperandOf<DT>::store(v, a.out + (r * a.length + c) * 2, a.part_stride, -1);
 }
 
 // ------------------------------------------------------------------------------------------- forward
@@ -141,7 +128,7 @@ __device__ __forceinline__ float sum_of_16(float x) {
 
 struct LogitsArgs {
     Operand x, weight;
-    int row_bytes;
+    int row_bytes, segment_stages;
     Targets targets;    // of row `first` on
     int64_t first;
     f32x2* stats;       // [part][row]: maximum, and sum of exponentials relative to it
@@ -167,6 +154,7 @@ template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, W
     int row0, col0;
     if (!my_tile<Tile>(a.x.rows, a.weight.rows, row0, col0)) return;
     Tile tile(smem);
+    tile.segment_stages = a.segment_stages;
     tile.multiply(a.x, a.weight, row0, col0, a.row_bytes);
     const int rows = a.x.rows, cols = a.weight.rows;
     const int r0 = row0 + (tile.wave >> 1) * WT + (tile.lane >> 4) * 4, part0 = col0 + (tile.wave & 1) * WT, mine = tile.lane & 15;
@@ -290,7 +278,7 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* losses, 
 // ------------------------------------------------------------------------------------------- backward
 // factors[i]: f_i over the largest magnitude among them, times `top` (a power of two); scale[0]: what that is to be multiplied by.
 __global__ __launch_bounds__(1024) void loss_factors_kernel(const float* upstream, int64_t stride, const int* labels, int64_t n, int reduction, const float* count,
-                                                            float top, float* factors, float* scale) {
+                                                            float top, float* factors, float* lost, float* scale) {
     __shared__ float mosts[16];
     const float share = reduction == FO_REDUCE_MEAN ? 1.0f / count[0] : 1.0f;
     float most = 0.0f;
@@ -307,43 +295,42 @@ __global__ __launch_bounds__(1024) void loss_factors_kernel(const float* upstrea
     for (int64_t i = threadIdx.x; i < n; i += 1024) {
         const float f = upstream[i * stride] * share / most * top;
         factors[i] = labels[i] == kIgnored ? 0.0f : labels[i] == kNone ? __builtin_nanf("") : f;
+        lost[i] = 0.0f;
     }
     if (threadIdx.x == 0) scale[0] = most / top;
 }
 
 struct GradArgs {
     Operand x, weight;     // of a piece of the vocabulary
-    int row_bytes;
+    int row_bytes, segment_stages;
     const int* labels;
     const float *lse, *factors;
-    char *grad, *turned;   // G as operand rows over the piece, its transpose as operand rows over the tokens; either may be null
-    int grad_length, turned_length;    // of a part of their rows
+    char* grad;            // G as operand rows over the piece
+    float* lost;           // of each row: what its target's entry lost in its rounding
+    int64_t part_stride;
+    int length;            // of G's rows
     int first;             // the piece's first token of the vocabulary
     float kept, even;      // 1 - e, e / V
 };
 template <int DT> struct GradOut {
-    static constexpr bool kColumns = true;
+    static constexpr bool kColumns = false;
     const GradArgs& a;
     struct In { float lse, factor; int label; };
     __device__ __forceinline__ void begin(int) const {}
     __device__ __forceinline__ void load(int i, int, In& in) const {
         if (i < a.x.rows) in = {a.lse[i], a.factors[i], a.labels[i]};
     }
-    __device__ __forceinline__ bool columns() const { return a.turned != nullptr; }
     __device__ __forceinline__ void row(int i, int j, In in, float (&v)[8]) const {
-        const bool zero = i >= a.x.rows || in.label == kIgnored;
+        if (i >= a.x.rows || j >= a.length) return;
+        const int at = in.label - a.first - j;    // among the eight, if the target is
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             float g = exp_of(v[k] - in.lse) - a.even;
-            if (a.first + j + k == in.label) g -= a.kept;
-            v[k] = zero || j + k >= a.weight.rows ? 0.0f : g * in.factor;
+            if (at == k) g -= a.kept;
+            v[k] = in.label == kIgnored || j + k >= a.weight.rows ? 0.0f : g * in.factor;
         }
-        if (a.grad && i < a.x.rows && j < a.grad_length)
-            OperandOf<DT>::template store<false>(v, a.grad + ((int64_t)i * a.grad_length * OperandOf<DT>::kParts + j) * 2, a.grad_length);
-    }
-    __device__ __forceinline__ void column(int i, int j, const float (&w)[8]) const {
-        if (j < a.weight.rows && i < a.turned_length)
-            OperandOf<DT>::template store<false>(w, a.turned + ((int64_t)j * a.turned_length * OperandOf<DT>::kParts + i) * 2, a.turned_length);
+        const float lost = OperandOf<DT>::store(v, a.grad + ((int64_t)i * a.length + j) * 2, a.part_stride, at);
+        if (at >= 0 && at < 8) a.lost[i] = lost;
     }
 };
 template <int DT, class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void grad_kernel(GradArgs a) {
@@ -352,26 +339,44 @@ template <int DT, class Product, int WT, int STAGES> __global__ __launch_bounds_
     int row0, col0;
     if (!my_tile<Tile>(a.x.rows, a.weight.rows, row0, col0)) return;
     Tile tile(smem);
+    tile.segment_stages = a.segment_stages;
     tile.multiply(a.x, a.weight, row0, col0, a.row_bytes);
     GradOut<DT> out{a};
     tile.finish(row0, col0, out);
 }
 
-// A product of operand rows; `parts` of the contraction may go to workgroups of their own, each with a result of its own in `sums`.
+// rows x cols of a product; `parts` of the contraction, part_stages each, may go to workgroups of their own, each with a result of its own in `sums`.
 struct GradProductArgs {
     Operand left, right;
-    int row_bytes, part_bytes, parts;
+    int rows, cols;
+    int row_bytes, segment_stages, part_stages, parts;
     const float* more;     // what is added, fp32, as far apart as out's rows; or null
     float* sums;           // fp32 results that go on; or
     char* out;             // the last one, of type `dtype`, times scale[0]
     const float* scale;
+    const float* lost;     // dx: what the rows' targets lost, times their rows of the weight, is added before that; or null
+    const int* labels;
+    const char* weight;
+    int64_t weight_stride;
     int64_t stride;
     int dtype;
 };
-__device__ __forceinline__ void store_result(float (&v)[8], const GradProductArgs& a, int64_t at, int valid) {
+__device__ __forceinline__ void store_result(float (&v)[8], const GradProductArgs& a, int i, int j, int valid) {
     const float scale = a.scale[0];
+    if (a.lost) {
+        const int label = a.labels[i];
+        if (label >= 0) {
+            const float lost = a.lost[i];
+            const char* row = a.weight + (label * a.weight_stride + j) * 2;
+            float w[8];
+            if (a.dtype == DT_BF16) load_values<DT_BF16>(w, row, valid); else load_values<DT_F16>(w, row, valid);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = fmaf(lost, w[k], v[k]);
+        }
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] *= scale;
+    const int64_t at = i * a.stride + j;
     if (a.dtype == DT_BF16) store_values<DT_BF16>(v, a.out + at * 2, valid);
     else if (a.dtype == DT_F16) store_values<DT_F16>(v, a.out + at * 2, valid);
     else store_values<DT_F32>(v, a.out + at * 4, valid);
@@ -384,52 +389,50 @@ struct GradProductOut {
     __device__ __forceinline__ void begin(int) const {}
     __device__ __forceinline__ void load(int i, int j, In& in) const {
         in.lo = in.hi = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (!a.more || i >= a.left.rows || j >= a.right.rows) return;
+        if (!a.more || i >= a.rows || j >= a.cols) return;
         float v[8];
-        load_values<DT_F32>(v, a.more + i * a.stride + j, a.right.rows - j);
+        load_values<DT_F32>(v, a.more + i * a.stride + j, a.cols - j);
         in.lo = f32x4{v[0], v[1], v[2], v[3]};
         in.hi = f32x4{v[4], v[5], v[6], v[7]};
     }
     __device__ __forceinline__ void row(int i, int j, const In& in, float (&v)[8]) const {
-        if (i >= a.left.rows || j >= a.right.rows) return;
+        if (i >= a.rows || j >= a.cols) return;
 #pragma unroll
         for (int k = 0; k < 4; ++k) { v[k] += in.lo[k]; v[4 + k] += in.hi[k]; }
-        const int64_t at = i * a.stride + j;
-        if (a.out) store_result(v, a, at, a.right.rows - j);
-        else store_values<DT_F32>(v, a.sums + part * a.left.rows * a.stride + at, a.right.rows - j);
+        if (a.out) store_result(v, a, i, j, a.cols - j);
+        else store_values<DT_F32>(v, a.sums + part * a.rows * a.stride + i * a.stride + j, a.cols - j);
     }
 };
-template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void grad_product_kernel(GradProductArgs a) {
+// TURNED: the left operand comes by columns too (dW = G' x).
+template <class Product, bool TURNED, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void grad_product_kernel(GradProductArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    typedef GemmTile<Product, WT, STAGES> Tile;
-    const int down = (a.left.rows + Tile::kTile - 1) / Tile::kTile, across = (a.right.rows + Tile::kTile - 1) / Tile::kTile;
+    typedef GemmTile<Product, WT, STAGES, TURNED, true> Tile;
+    const int down = (a.rows + Tile::kTile - 1) / Tile::kTile, across = (a.cols + Tile::kTile - 1) / Tile::kTile;
     const int64_t t = tile_of_seat(blockIdx.x & 7, blockIdx.x >> 3, (int64_t)down * across * a.parts);
     if (t < 0) return;
     const int part = (int)(t / (down * across));
     int i, j;
     tile_at((int)(t - (int64_t)part * down * across), down, across, i, j);
-    const int64_t from = (int64_t)part * a.part_bytes;
-    Operand left = a.left, right = a.right;
-    left.data += from;
-    right.data += from;
     Tile tile(smem);
-    tile.multiply(left, right, i * Tile::kTile, j * Tile::kTile, part + 1 < a.parts ? a.part_bytes : (int)(a.row_bytes - from));
+    tile.segment_stages = a.segment_stages;
+    tile.first_stage = part * a.part_stages;
+    tile.multiply(a.left, a.right, i * Tile::kTile, j * Tile::kTile, part + 1 < a.parts ? a.part_stages * kStageBytes : a.row_bytes - tile.first_stage * kStageBytes);
     GradProductOut out{a, part};
     tile.finish(i * Tile::kTile, j * Tile::kTile, out);
 }
 // The parts' results and `more`, added up in their order.  A thread takes eight values of a row.
 __global__ __launch_bounds__(256) void grad_join_kernel(GradProductArgs a, const float* partial) {
-    const int pieces = (a.right.rows + 7) / 8;
+    const int pieces = (a.cols + 7) / 8;
     const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, i = k / pieces;
-    const int j = (int)(k - i * pieces) * 8, valid = a.right.rows - j;
-    if (i >= a.left.rows) return;
+    const int j = (int)(k - i * pieces) * 8, valid = a.cols - j;
+    if (i >= a.rows) return;
     const int64_t at = i * a.stride + j;
     float sum[8];
     load_values<DT_F32>(sum, partial + at, valid);
 #pragma unroll 8
     for (int p = 1; p < a.parts; ++p) {
         float v[8];
-        load_values<DT_F32>(v, partial + (int64_t)p * a.left.rows * a.stride + at, valid);
+        load_values<DT_F32>(v, partial + (int64_t)p * a.rows * a.stride + at, valid);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] += v[e];
     }
@@ -439,7 +442,7 @@ __global__ __launch_bounds__(256) void grad_join_kernel(GradProductArgs a, const
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] += v[e];
     }
-    if (a.out) store_result(sum, a, at, valid);
+    if (a.out) store_result(sum, a, (int)i, j, valid);
     else store_values<DT_F32>(sum, a.sums + at, valid);
 }
 
@@ -450,6 +453,7 @@ __global__ __launch_bounds__(256) void grad_join_kernel(GradProductArgs a, const
 // ------------------------------------------------------------------------------------------------
 namespace {
 using namespace fo_host;
+using fo::u32;
 
 constexpr int64_t kMostWorkgroups = (1 << 24) - 1;    // of 256 threads: a launch has less than 2^32 threads
 constexpr int64_t kMostTokens = 1 << 20, kMostCols = 1 << 16, kMostVocabulary = 1 << 24;    // 32-bit offsets into a tile's rows
@@ -465,9 +469,11 @@ constexpr fo::TileCost kTileCosts[] = {
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t aligned(int64_t bytes) { return round_up(bytes, 256); }
-int64_t length_of(int64_t n) { return round_up(n, 32); }
-int parts_of(int dtype) { return dtype == FO_F32 ? 6 : 1; }
-int64_t form_bytes(int dtype, int64_t rows, int64_t inner) { return aligned(rows * length_of(inner) * parts_of(dtype) * 2); }
+// An operand's rows; those in parts are contracted segment after segment, each of whole stages.
+int64_t length_of(int dtype, int64_t n) { return round_up(n, dtype == FO_F32 ? 64 : 32); }
+int parts_of(int dtype) { return dtype == FO_F32 ? 3 : 1; }
+int64_t segments_of(int dtype) { return dtype == FO_F32 ? fo::kSegments : 1; }
+int64_t form_bytes(int dtype, int64_t rows, int64_t inner) { return aligned(rows * length_of(dtype, inner) * parts_of(dtype) * 2); }
 
 int validate(const char* what, int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
     if (tokens < 0 || cols < 0 || vocabulary < 0) return fail(FO_ERR_INVALID_ARGUMENT, "%s: negative size", what);
@@ -535,12 +541,12 @@ template <int DT, class Product> struct GradLaunch {
     static int64_t cols(const Args& a) { return a.weight.rows; }
     static int64_t parts(const Args&) { return 1; }
 };
-template <class Product> struct ProductLaunch {
+template <class Product, bool TURNED> struct ProductLaunch {
     typedef fo::GradProductArgs Args;
-    template <int WT, int STAGES> static auto kernel() { return fo::grad_product_kernel<Product, WT, STAGES>; }
-    template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES>::kLds; }
-    static int64_t rows(const Args& a) { return a.left.rows; }
-    static int64_t cols(const Args& a) { return a.right.rows; }
+    template <int WT, int STAGES> static auto kernel() { return fo::grad_product_kernel<Product, TURNED, WT, STAGES>; }
+    template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES, TURNED, true>::kLds; }
+    static int64_t rows(const Args& a) { return a.rows; }
+    static int64_t cols(const Args& a) { return a.cols; }
     static int64_t parts(const Args& a) { return a.parts; }
 };
 
@@ -567,39 +573,45 @@ struct Matrix {
     // Whether the rows are operand rows as they are.
     bool ready() const { return dtype != FO_F32 && cols % 32 == 0 && stride % 8 == 0 && stride >= 0 && stride < (1 << 22) && ((uintptr_t)p & 15) == 0; }
 };
-fo::Operand operand(const void* p, int64_t row_bytes, int64_t rows) { return {(const char*)p, row_bytes, nullptr, 0, (int)rows}; }
+// The rows of an operand, or (turned) `depth` rows whose columns are it.  part_stride: see fo_gemm.h.
+fo::Operand operand(const void* p, int64_t length, int64_t rows, int64_t part_stride, u32 order) { return {(const char*)p, length * 2, nullptr, 0, (int)rows, 0, part_stride, order}; }
+fo::Operand turned(fo::Operand o, int64_t length, int64_t depth) {
+    o.rows = (int)length;
+    o.depth = (int)depth;
+    return o;
+}
 
-// The rows of m as an operand: in place where they are one, else laid out at `space`; and its columns at `turned`, if that is given.  labels: see FormArgs.
-template <bool RIGHT> int operand_of(const Matrix& m, const int* labels, char* space, char* turned, fo::Operand& to, hipStream_t s, const char* what) {
-    const bool ready = m.ready();
-    to = ready ? operand(m.p, m.stride * 2, m.rows) : operand(space, length_of(m.cols) * parts_of(m.dtype) * 2, m.rows);
-    if (ready && !turned) return 0;
-    const fo::FormArgs a{m.p, ready ? nullptr : space, turned, labels, m.stride, (int)m.rows, (int)m.cols, (int)length_of(m.cols), (int)length_of(m.rows)};
-    const int64_t grid = ((m.rows + 63) / 64) * ((m.cols + 63) / 64);
+// The rows of m as an operand: in place where they are one and `copy` does not ask for more, else laid out at `space`, filled up to out_rows rows.  labels: see FormArgs.
+int operand_of(const Matrix& m, bool copy, const int* labels, int64_t out_rows, char* space, u32 order, fo::Operand& to, hipStream_t s, const char* what) {
+    if (m.ready() && !copy) { to = operand(m.p, m.stride, m.rows, 0, order); return 0; }
+    const int64_t length = length_of(m.dtype, m.cols), part_stride = out_rows * length * 2;
+    to = operand(space, length, m.rows, part_stride, order);
+    const fo::FormArgs a{m.p, space, labels, m.stride, part_stride, (int)m.rows, (int)m.cols, (int)out_rows, (int)length};
+    const int64_t grid = (out_rows * (length / 8) + 255) / 256;
     switch (m.dtype) {
-        case FO_F32: return launch(fo::form_kernel<fo::DT_F32, RIGHT>, grid, 256, 0, s, what, a);
-        case FO_BF16: return launch(fo::form_kernel<fo::DT_BF16, RIGHT>, grid, 256, 0, s, what, a);
-        default: return launch(fo::form_kernel<fo::DT_F16, RIGHT>, grid, 256, 0, s, what, a);
+        case FO_F32: return launch(fo::form_kernel<fo::DT_F32>, grid, 256, 0, s, what, a);
+        case FO_BF16: return launch(fo::form_kernel<fo::DT_BF16>, grid, 256, 0, s, what, a);
+        default: return launch(fo::form_kernel<fo::DT_F16>, grid, 256, 0, s, what, a);
     }
 }
 
-template <class Product> int product(fo::GradProductArgs a, const Cut& cut, float* partial, hipStream_t s, const char* what) {
+template <class Product, bool TURNED> int product(fo::GradProductArgs a, const Cut& cut, float* partial, hipStream_t s, const char* what) {
     a.parts = cut.parts;
-    a.part_bytes = (int)(cut.part * 2);
-    if (cut.parts == 1) return launch_tiles<ProductLaunch<Product>>(cut.tile, a, s, what);
+    a.part_stages = (int)(cut.part / 64);
+    if (cut.parts == 1) return launch_tiles<ProductLaunch<Product, TURNED>>(cut.tile, a, s, what);
     fo::GradProductArgs some = a;
     some.more = nullptr;
     some.out = nullptr;
     some.sums = partial;
-    if (int rc = launch_tiles<ProductLaunch<Product>>(cut.tile, some, s, what)) return rc;
-    const int64_t grid = ((int64_t)a.left.rows * ((a.right.rows + 7) / 8) + 255) / 256;
+    if (int rc = launch_tiles<ProductLaunch<Product, TURNED>>(cut.tile, some, s, what)) return rc;
+    const int64_t grid = ((int64_t)a.rows * ((a.cols + 7) / 8) + 255) / 256;
     if (grid > kMostWorkgroups) return fail(FO_ERR_UNSUPPORTED, "%s: too large a result for one launch", what);
     fo::grad_join_kernel<<<dim3((unsigned)grid), dim3(256), 0, s>>>(a, partial);
     return check_hip(hipGetLastError(), what);
 }
 
 template <class F> int by_product(int dtype, const F& f) {
-    if (dtype == FO_F32) return f.template run<fo::DT_F32, fo::Bf16Product>();
+    if (dtype == FO_F32) return f.template run<fo::DT_F32, fo::Bf16PartsProduct>();
     return dtype == FO_BF16 ? f.template run<fo::DT_BF16, fo::Bf16Product>() : f.template run<fo::DT_F16, fo::F16Product>();
 }
 
@@ -635,7 +647,7 @@ struct ForwardSpace {
 
 struct BackwardSpace {
     int64_t piece;    // tokens of the vocabulary at a time
-    int64_t factors, scale, x, turned_x, weight, turned_weight, grad, turned_grad, sums, partial, total;
+    int64_t factors, lost, scale, x, weight, grad, sums, partial, total;
     Cut dx_cut, dw_cut;
     BackwardSpace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, bool dx, bool dw, int cus) {
         const int64_t most = round_up(kPieceValues / parts_of(dtype) / tokens + 1, 256);
@@ -643,17 +655,15 @@ struct BackwardSpace {
         piece = round_up((vocabulary + pieces - 1) / pieces, 256);
         if (piece > vocabulary) piece = vocabulary;
         // a last piece that is shorter goes by the same cuts: its parts are fewer
-        dx_cut = dx ? cut_for(tokens, cols, length_of(piece) * parts_of(dtype), cus) : Cut{};
-        dw_cut = dw ? cut_for(piece, cols, length_of(tokens) * parts_of(dtype), cus) : Cut{};
+        dx_cut = dx ? cut_for(tokens, cols, length_of(dtype, piece) * segments_of(dtype), cus) : Cut{};
+        dw_cut = dw ? cut_for(piece, cols, length_of(dtype, tokens) * segments_of(dtype), cus) : Cut{};
         factors = 0;
-        scale = factors + aligned(tokens * 4);
+        lost = factors + aligned(tokens * 4);
+        scale = lost + aligned(tokens * 4);
         x = scale + 256;
-        turned_x = x + form_bytes(dtype, tokens, cols);
-        weight = turned_x + (dw ? form_bytes(dtype, cols, tokens) : 0);
-        turned_weight = weight + form_bytes(dtype, piece, cols);
-        grad = turned_weight + (dx ? form_bytes(dtype, cols, piece) : 0);
-        turned_grad = grad + (dx ? form_bytes(dtype, tokens, piece) : 0);
-        sums = turned_grad + (dw ? form_bytes(dtype, piece, tokens) : 0);
+        weight = x + form_bytes(dtype, length_of(dtype, tokens), cols);
+        grad = weight + form_bytes(dtype, piece, cols);
+        sums = grad + form_bytes(dtype, tokens, piece);
         partial = sums + (dx && piece < vocabulary ? aligned(tokens * cols * 4) : 0);
         const int64_t of_dx = dx_cut.parts > 1 ? dx_cut.parts * tokens * cols : 0, of_dw = dw_cut.parts > 1 ? dw_cut.parts * piece * cols : 0;
         total = partial + aligned((of_dx > of_dw ? of_dx : of_dw) * 4);
@@ -679,14 +689,15 @@ struct Forward {
         const fo::Targets t{targets, index_bytes};
         float* losses = reduction == FO_REDUCE_NONE ? loss : (float*)(base + at.losses);
         fo::Operand w;
-        if (int rc = operand_of<true>(weight, nullptr, base + at.weight, nullptr, w, s, what)) return rc;
-        const int row_bytes = (int)(length_of(x.cols) * parts_of(x.dtype) * 2);
+        if (int rc = operand_of(weight, false, nullptr, weight.rows, base + at.weight, fo::kRightOrder, w, s, what)) return rc;
+        const int64_t length = length_of(x.dtype, x.cols);
+        const int row_bytes = (int)(length * segments_of(x.dtype) * 2), segment = (int)(length / 64);
         for (int64_t first = 0; first < x.rows; first += kBlockTokens) {
             const Matrix some = x.part(first, x.rows - first < kBlockTokens ? x.rows - first : kBlockTokens);
             fo::Operand rows;
-            if (int rc = operand_of<false>(some, nullptr, base + at.x, nullptr, rows, s, what)) return rc;
+            if (int rc = operand_of(some, false, nullptr, some.rows, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
             const fo::TileCost tile = tile_for(some.rows, weight.rows, row_bytes / 2, cus);
-            const fo::LogitsArgs a{rows, w, row_bytes, t, first, (fo::f32x2*)(base + at.stats), smoothing > 0.0f ? (float*)(base + at.sums) : nullptr, (float*)(base + at.picked)};
+            const fo::LogitsArgs a{rows, w, row_bytes, segment, t, first, (fo::f32x2*)(base + at.stats), smoothing > 0.0f ? (float*)(base + at.sums) : nullptr, (float*)(base + at.picked)};
             if (int rc = launch_tiles<LogitsLaunch<Product>>(tile, a, s, what)) return rc;
             const fo::JoinArgs join{a.stats, a.sums, a.picked, t, first, ignore, weight.rows, kept + first, losses + first, labels + first, (int)some.rows,
                                     (int)((weight.rows + tile.wt - 1) / tile.wt), smoothing};
@@ -715,37 +726,60 @@ struct Backward {
 
     template <int DT, class Product> int run() const {
         const char* what = "fo_linear_cross_entropy_backward";
-        const int parts = parts_of(x.dtype);
         const int* labels = (const int*)(kept + x.rows + 1);
-        float *factors = (float*)(base + at.factors), *scale = (float*)(base + at.scale), *sums = (float*)(base + at.sums), *partial = (float*)(base + at.partial);
+        float *factors = (float*)(base + at.factors), *lost = (float*)(base + at.lost), *scale = (float*)(base + at.scale);
+        float *sums = (float*)(base + at.sums), *partial = (float*)(base + at.partial);
         fo::loss_factors_kernel<<<dim3(1), dim3(1024), 0, s>>>(upstream, upstream_stride, labels, x.rows, reduction, kept + x.rows, x.dtype == FO_F16 ? 32768.0f : 1.0f,
-                                                               factors, scale);
+                                                               factors, lost, scale);
         if (int rc = check_hip(hipGetLastError(), what)) return rc;
+        const int dtype = x.dtype;
+        const int64_t tokens_length = length_of(dtype, x.rows), cols_length = length_of(dtype, x.cols), segments = segments_of(dtype);
         fo::Operand rows;
-        if (int rc = operand_of<false>(x, labels, base + at.x, dw ? base + at.turned_x : nullptr, rows, s, what)) return rc;
-        const int64_t tokens_length = length_of(x.rows);
-        const int row_bytes = (int)(length_of(x.cols) * parts * 2);
+        if (int rc = operand_of(x, dw != nullptr, labels, tokens_length, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
+        fo::Operand x_turned = turned(rows, cols_length, tokens_length);
+        x_turned.order = fo::kRightOrder;
         for (int64_t first = 0; first < weight.rows; first += at.piece) {
-            const int64_t n = weight.rows - first < at.piece ? weight.rows - first : at.piece, length = length_of(n);
+            const int64_t n = weight.rows - first < at.piece ? weight.rows - first : at.piece, length = length_of(dtype, n);
             const bool last = first + n == weight.rows;
             fo::Operand w;
-            if (int rc = operand_of<true>(weight.part(first, n), nullptr, base + at.weight, dx ? base + at.turned_weight : nullptr, w, s, what)) return rc;
-            const fo::GradArgs grad{rows, w, row_bytes, labels, kept, factors, dx ? base + at.grad : nullptr, dw ? base + at.turned_grad : nullptr, (int)length,
-                                    (int)tokens_length, (int)first, 1.0f - smoothing, smoothing / (float)weight.rows};
-            if (int rc = launch_tiles<GradLaunch<DT, Product>>(tile_for(x.rows, n, row_bytes / 2, cus), grad, s, what)) return rc;
+            if (int rc = operand_of(weight.part(first, n), false, nullptr, n, base + at.weight, fo::kRightOrder, w, s, what)) return rc;
+            const fo::Operand g = operand(base + at.grad, length, x.rows, x.rows * length * 2, fo::kLeftOrder);
+            const fo::GradArgs grad{rows, w, (int)(cols_length * segments * 2), (int)(cols_length / 64), labels, kept, factors, base + at.grad, lost, g.part_stride, (int)length,
+                                    (int)first, 1.0f - smoothing, smoothing / (float)weight.rows};
+            if (int rc = launch_tiles<GradLaunch<DT, Product>>(tile_for(x.rows, n, (double)(cols_length * segments), cus), grad, s, what)) return rc;
+            fo::GradProductArgs p{};
+            p.cols = (int)x.cols;
+            p.scale = scale;
+            p.stride = x.cols;
+            p.dtype = dtype;
             if (dx) {
-                const int64_t bytes = length * parts * 2;
+                p.left = g;
+                p.right = turned(w, cols_length, n);
+                p.rows = (int)x.rows;
+                p.row_bytes = (int)(length * segments * 2);
+                p.segment_stages = (int)(length / 64);
+                p.more = first ? sums : nullptr;
+                p.sums = last ? nullptr : sums;
+                p.out = last ? dx : nullptr;
+                p.lost = dtype == FO_F32 ? nullptr : lost;
+                p.labels = labels;
+                p.weight = weight.p;
+                p.weight_stride = weight.stride;
                 Cut cut = at.dx_cut;
-                cut.parts = (int)((bytes / 2 + cut.part - 1) / cut.part);
-                const fo::GradProductArgs p{operand(base + at.grad, bytes, x.rows), operand(base + at.turned_weight, bytes, x.cols), (int)bytes, 0, 0, first ? sums : nullptr,
-                                            last ? nullptr : sums, last ? dx : nullptr, scale, x.cols, x.dtype};
-                if (int rc = product<Product>(p, cut, partial, s, what)) return rc;
+                cut.parts = (int)((length * segments + cut.part - 1) / cut.part);
+                if (int rc = product<Product, false>(p, cut, partial, s, what)) return rc;
             }
             if (dw) {
-                const int64_t bytes = tokens_length * parts * 2;
-                const fo::GradProductArgs p{operand(base + at.turned_grad, bytes, n), operand(base + at.turned_x, bytes, x.cols), (int)bytes, 0, 0, nullptr, nullptr,
-                                            dw + first * x.cols * x.width(), scale, x.cols, x.dtype};
-                if (int rc = product<Product>(p, at.dw_cut, partial, s, what)) return rc;
+                p.left = turned(g, length, x.rows);
+                p.right = x_turned;
+                p.rows = (int)n;
+                p.row_bytes = (int)(tokens_length * segments * 2);
+                p.segment_stages = (int)(tokens_length / 64);
+                p.more = nullptr;
+                p.sums = nullptr;
+                p.out = dw + first * x.cols * x.width();
+                p.lost = nullptr;
+                if (int rc = product<Product, true>(p, at.dw_cut, partial, s, what)) return rc;
             }
         }
         return 0;
