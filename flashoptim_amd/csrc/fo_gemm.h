@@ -29,11 +29,11 @@
 // their conflicts are hidden: an order without them took as long.
 // The order is applied to the address that a lane loads from.
 //
-// Either operand of 16-bit values may lie the other way round in memory, the contracted axis down the rows: A[k][i], B[k][j] with i and j adjacent (KA, KB).  Its stage
-// is then 64 rows of a tile's width, of the same number of bytes, and the operand of an instruction comes out of LDS through two transposing reads: sixteen lanes
-// read four rows of sixteen values and get four values of a column each.  A 32-byte piece of a row is what one such read takes; row k keeps its pieces shifted by
-// turned_shift(k), so that the sixteen rows that a wavefront reads at a time lie in all banks.  Rows need not be filled up to whole stages: those behind the last are read as
-// copies of it, the other operand holds zeros for them.
+// Either operand (not codes) may lie the other way round in memory, the contracted axis down the rows: A[k][i], B[k][j] with i and j adjacent (KA, KB).  Its stage
+// is then 64 rows (32 of fp32) of a tile's width, of the same number of bytes.  The operand of a 16-bit instruction comes out of LDS through two transposing reads: sixteen
+// lanes read four rows of sixteen values and get four values of a column each; fp32 ones are read value by value, which is as they are wanted.  Sixteen values of a
+// row are a piece; row k keeps its pieces shifted by turned_shift(k), so that the rows that a wavefront reads at a time lie in all banks.  Rows need not be
+// filled up to whole stages: those behind the last are read as copies of it, the other operand holds zeros for them.
 #pragma once
 
 #include "fo_device.h"
@@ -115,6 +115,8 @@ struct Operand {
     int depth;              // turned operands: how many rows there are along the contracted axis; `rows`, a multiple of 8, is how long they are
     int64_t part_stride;    // products in parts: bytes from a part of the values to the next
     u32 order;              // and which part each segment of the contraction takes, two bits each
+    int pieces;             // 16-byte pieces of a row that there are, where it is not filled up (0: it is); the others are read as copies of the last one, and the
+                            // other operand holds zeros for them
 };
 
 // The matrix instructions are inline asm so that an accumulator stays in the registers it is in (the compiler's own form lets
@@ -123,6 +125,7 @@ struct Operand {
 // multiply().  Results feed the next instruction on the same accumulator without a wait, at least three others lie between.
 struct F16Product {
     static constexpr bool kScaled = false, kParts = false;
+    static constexpr int kBytes = 2;
     typedef f16x8 Frag;
     template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int, int) {
         asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
@@ -131,9 +134,21 @@ struct F16Product {
 
 struct Bf16Product {
     static constexpr bool kScaled = false, kParts = false;
+    static constexpr int kBytes = 2;
     typedef bf16x8 Frag;
     template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int, int) {
         asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    }
+};
+
+// fp32 values on the matrix cores' fp32 instructions, a sixteenth of the 16-bit rate: a lane's 16 bytes are one value for each of four instructions.
+struct F32Product {
+    static constexpr bool kScaled = false, kParts = false;
+    static constexpr int kBytes = 4;
+    typedef f32x4 Frag;
+    template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int, int) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) asm("v_mfma_f32_16x16x4_f32 %0, %1, %2, %0" : "+a"(c) : "v"(a[k]), "v"(b[k]));
     }
 };
 
@@ -146,6 +161,7 @@ constexpr int kSegments = 6;
 // HALF: which byte of the two scales is meant.
 struct Mx4Product {
     static constexpr bool kScaled = true, kParts = false;
+    static constexpr int kBytes = 2;    // of no meaning: two values to a byte
     typedef i32x4 Frag;
     template <int HALF> __device__ __forceinline__ static void multiply(const Frag& a, const Frag& b, f32x4& c, int a_scales, int b_scales) {
         if constexpr (HALF == 0)
@@ -196,7 +212,8 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
     static_assert(kStages * kBuffer <= 163840 && (kStages - 1) * kLoads <= 63, "what LDS holds, what the counter of loads under way counts to");
     static constexpr int kLds = kStages * kBuffer > 4 * kStripBytes ? kStages * kBuffer : 4 * kStripBytes;
 
-    static constexpr int kPieces32 = WT / 8;      // of 32 bytes, in a stage row of a turned operand
+    static constexpr int kPieces = kTile / 16;    // of sixteen values, in a stage row of a turned operand
+    static constexpr int kElement = Product::kBytes, kTurnedRow = kElement * kTile, kTurnedRows = kStageBytes / kElement;
     static_assert(!Product::kScaled || (!KA && !KB), "codes have no transposing read");
 
     typedef typename Product::Frag Frag;
@@ -215,18 +232,20 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
     __device__ __forceinline__ static int buffer_of(int stage) { return (kStages == 3 ? stage % 3 : stage & (kStages - 1)) * kBuffer; }
     __device__ __forceinline__ static int place_of(int row) { return (row >> 1) & 7; }
     __device__ __forceinline__ static int turned_shift(int k) {
-        return kPieces32 % 8 == 0 ? (k & 3) | (k >> 3 & 1) << 2 : (k >> 1 & 1) | (k >> 3 & 1) << 1;
+        if constexpr (kElement == 4) return k >> 2 & 3;
+        return kPieces % 8 == 0 ? (k & 3) | (k >> 3 & 1) << 2 : (k >> 1 & 1) | (k >> 3 & 1) << 1;
     }
+    static constexpr bool kShiftByXor = kElement == 4 || kPieces % 8 == 0;
     // Where piece `at` of stage row k lies in that row.
     __device__ __forceinline__ static int turned_place(int at, int k) {
-        if constexpr (kPieces32 % 8 == 0) return at ^ turned_shift(k);
+        if constexpr (kShiftByXor) return at ^ turned_shift(k);
         const int place = at + turned_shift(k);
-        return place < kPieces32 ? place : place - kPieces32;
+        return place < kPieces ? place : place - kPieces;
     }
     __device__ __forceinline__ static int turned_piece(int place, int k) {    // and back
-        if constexpr (kPieces32 % 8 == 0) return place ^ turned_shift(k);
+        if constexpr (kShiftByXor) return place ^ turned_shift(k);
         const int at = place - turned_shift(k);
-        return at < 0 ? at + kPieces32 : at;
+        return at < 0 ? at + kPieces : at;
     }
     struct Loader {
         unsigned row[kRowLoads];
@@ -237,7 +256,10 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
         unsigned line;           // turned: bytes from a row to the next, and the rows that there are
         int depth;
         unsigned scale[kScaleLoads > 0 ? kScaleLoads : 1];
-        unsigned past_half, past_half_scale;   // what a lane steps back by when the last stage is half of one
+        int piece;               // the lane's piece of a row in even loads; in odd ones, eight rows on, the halves have changed places
+        int whole_stages;        // stages whose pieces are all there
+        int pieces;
+        unsigned past_half_scale;   // what a lane steps back by when the last stage is half of one
         const char* base;
         const char* scale_base;
     };
@@ -247,23 +269,25 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
         const int64_t stride = first ? a.stride : b.stride;
         const int at = first ? row0 : col0, left = (first ? a.rows : b.rows) - at;
         l.turned = first ? KA : KB;
-        l.step = l.turned ? 64 * stride : kStageBytes;
+        l.step = l.turned ? kTurnedRows * stride : kStageBytes;
+        l.pieces = first ? a.pieces : b.pieces;
+        l.whole_stages = l.pieces ? l.pieces / 8 : INT32_MAX;
         l.line = (unsigned)stride;
         l.depth = first ? a.depth : b.depth;
         l.part_stride = first ? a.part_stride : b.part_stride;
         l.order = first ? a.order : b.order;
         if ((KA || KB) && l.turned) {
-            l.base = uniform(data + at * 2);
+            l.base = uniform(data + at * kElement);
 #pragma unroll
             for (int i = 0; i < kRowLoads; ++i) {
-                const int k = turned_row(i), byte = turned_byte(i) % (2 * kTile);
-                const int chunk = turned_piece(byte >> 5, k) * 2 + (byte >> 4 & 1), last = left / 8 - 1;    // of 16 bytes
+                const int k = turned_row(i), byte = turned_byte(i) % kTurnedRow;
+                const int chunk = turned_piece(byte / (16 * kElement), k) * kElement + (byte >> 4) % kElement, last = left * kElement / 16 - 1;    // of 16 bytes
                 l.row[i] = (unsigned)(k * stride) + (chunk < last ? chunk : last) * 16;
             }
             return;
         }
         l.base = uniform(data + at * stride);
-        l.past_half = ((lane & 7) ^ place_of(lane >> 3)) >= 4 ? kHalfBytes : 0;
+        l.piece = (lane & 7) ^ place_of(lane >> 3);
 #pragma unroll
         for (int i = 0; i < kRowLoads; ++i) {
             const int row = i * 8 + (lane >> 3), piece = (lane & 7) ^ place_of(row);   // the other wavefronts' rows are multiples of 16 away
@@ -285,7 +309,7 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
     }
     // Turned operands: which byte of the wavefront's operand in a stage the lane's part of load i is, and in which row that is.
     __device__ __forceinline__ int turned_byte(int i) const { return (wave & 1) * (kRowLoads * 1024) + i * 1024 + lane * 16; }
-    __device__ __forceinline__ int turned_row(int i) const { return turned_byte(i) / (2 * kTile); }
+    __device__ __forceinline__ int turned_row(int i) const { return turned_byte(i) / kTurnedRow; }
 
     // The i-th load of a stage.  half: the rows end in the middle of the stage, its second half repeats the first.
     __device__ __forceinline__ void load(const Loader& l, int i, int stage, bool half) const {
@@ -300,9 +324,9 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
             base += (int64_t)(l.order >> 2 * segment & 3) * l.part_stride;
         }
         if ((KA || KB) && l.turned) {
-            const int last = l.depth - 1 - stage * 64;    // row of the stage
+            const int last = l.depth - 1 - stage * kTurnedRows;    // row of the stage
             unsigned at = l.row[i];
-            if (last < 63) {
+            if (last < kTurnedRows - 1) {
                 const int k = turned_row(i);
                 at -= k > last ? (unsigned)(k - last) * l.line : 0u;
             }
@@ -310,8 +334,13 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
             return;
         }
         if (i < kRowLoads) {
-            const unsigned past = i & 1 ? kHalfBytes - l.past_half : l.past_half;   // eight rows on the halves change places
-            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, l.row[i] - (half ? past : 0), base + (int64_t)stage * kStageBytes);
+            unsigned at = l.row[i];
+            if (half || stage >= l.whole_stages) {    // pieces behind the last one there is, or behind the half, repeat the last before
+                const int piece = i & 1 ? l.piece ^ 4 : l.piece, left = l.pieces ? l.pieces - stage * 8 : 8;
+                const int last = (half && left > 4 ? 4 : left) - 1;
+                at -= piece > last ? (unsigned)(piece - last) * 16 : 0u;
+            }
+            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, at, base + (int64_t)stage * kStageBytes);
         } else if constexpr (Product::kScaled) {
             const int k = i - kRowLoads;
             load_to_lds4(buffer + kScaleOffset + (wave * kScaleLoads + k) * 256, l.scale[k] - (half ? l.past_half_scale : 0),
@@ -334,12 +363,20 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
         const bool is_b = f < kFrags;
         const int i = is_b ? f : f - kFrags, group = lane >> 4;
         if ((KA && !is_b) || (KB && is_b)) {
-            const int k = half * 32 + group * 8 + (lane >> 2 & 3), piece = (is_b ? wave & 1 : wave >> 1) * kFrags + i;
-            const char* from = smem + buffer_of(stage) + (is_b ? kTile * kStageBytes : 0) + (lane & 3) * 8;
-            const i16x4 lo = transposed(from + k * (2 * kTile) + turned_place(piece, k) * 32);
-            const i16x4 hi = transposed(from + (k + 4) * (2 * kTile) + turned_place(piece, k + 4) * 32);
-            const i16x8 all = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            (is_b ? to.b[i] : to.a[i]) = __builtin_bit_cast(Frag, all);
+            const int piece = (is_b ? wave & 1 : wave >> 1) * kFrags + i;
+            const char* from = smem + buffer_of(stage) + (is_b ? kTile * kStageBytes : 0);
+            Frag all;
+            if constexpr (kElement == 4) {
+                const int k = half * 16 + group * 4;
+                const float* p = reinterpret_cast<const float*>(from + k * kTurnedRow + turned_place(piece, k) * 64) + (lane & 15);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) all[e] = p[e * (kTurnedRow / 4)];
+            } else {
+                const int k = half * 32 + group * 8 + (lane >> 2 & 3);
+                from += k * kTurnedRow + turned_place(piece, k) * 32 + (lane & 3) * 8;    // rows k and k + 4 are shifted alike
+                all = __builtin_bit_cast(Frag, __builtin_shufflevector(transposed(from), transposed(from + 4 * kTurnedRow), 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+            (is_b ? to.b[i] : to.a[i]) = all;
             return;
         }
         const int row = (is_b ? kTile + (wave & 1) * WT : (wave >> 1) * WT) + i * 16 + (lane & 15);

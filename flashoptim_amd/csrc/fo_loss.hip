@@ -15,12 +15,13 @@
 // other operand of its products is; the factors f_i are first divided by the largest of them (and multiplied by 2^15 for fp16, so that probabilities down to 2^-39
 // survive), which the products' results are multiplied by at the end: where all are equal, as in a mean, they are 1, and the entry p - 1 of an unlikely
 // target rounds to almost itself.  What the target's entry, by far the largest of most rows, loses in its rounding goes into dx all the same: that times the
-// target's row of W is added in fp32.  fp32 operands are cut into three bf16 parts of 8 bits each, a = a1 + a2 + a3
+// target's row of W is added in fp32.  fp32 operands go into the fp32 instructions, a sixteenth of the rate; or, where the work is large enough to pay for laying
+// them out (in_parts), they are cut into three bf16 parts of 8 bits each, a = a1 + a2 + a3
 // exactly, and the six products a3 b1, a2 b2, a1 b3, a2 b1, a1 b2, a1 b1 are one contraction over six times the length: what is left
 // out is below 2^-23 of a product.  The small ones come first, so that the sums are small while most of the additions round.
 //
-// Rows of operands are whole multiples of 32 values (64 in parts), filled up with zeros: matrices that are so already are read in place, others are laid out
-// first.  G = f (p - ...) is written once, by rows, and read by rows for dx and by columns for dW, W by rows for the logits and by columns for dx: the product core reads
+// Operands are read in place where their rows are whole 16-byte pieces, aligned; others are laid out first.  The contracted axis is filled up to half a stage with zeros on
+// one side of a product.  G = f (p - ...) is written once, by rows, and read by rows for dx and by columns for dW, W by rows for the logits and by columns for dx: the product core reads
 // either way.  Rows of ignored targets are left out of dW by zeros on both sides, so that what stands in them (infinities, NaN) does not matter: x is copied for that.
 #include "fo_gemm.h"
 #include "fo_host.h"
@@ -34,10 +35,10 @@ constexpr int kIgnored = -1, kNone = -2;    // labels
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // ------------------------------------------------------------------------------------------- operands
-// Eight neighbouring values of a row as the matrix instructions' operands have them: rounded to a 16-bit type, or the three parts of each, `part_stride` bytes apart.
+// Eight neighbouring values of a row as a product's operands have them: rounded to a 16-bit type, as they are, or the three parts of each, `part_stride` bytes apart.
 // Returned is what was lost of v[at] by that (0 where at is none of them).
-template <int DT> struct OperandOf {
-    static constexpr int kParts = 1;
+template <int DT, class Product> struct OperandOf {
+    static constexpr int kBytes = 2;
     __device__ __forceinline__ static float store(const float (&v)[8], char* p, int64_t, int at) {
         Pack<2, 8> d;
         float lost = 0.0f;
@@ -52,8 +53,15 @@ template <int DT> struct OperandOf {
         return lost;
     }
 };
-template <> struct OperandOf<DT_F32> {
-    static constexpr int kParts = 3;
+template <> struct OperandOf<DT_F32, F32Product> {
+    static constexpr int kBytes = 4;
+    __device__ __forceinline__ static float store(const float (&v)[8], char* p, int64_t, int) {
+        store_values<DT_F32>(v, p, 8);
+        return 0.0f;
+    }
+};
+template <> struct OperandOf<DT_F32, Bf16PartsProduct> {
+    static constexpr int kBytes = 2;
     __device__ __forceinline__ static float store(const float (&v)[8], char* p, int64_t part_stride, int) {
         u32x4 part[3];
 #pragma unroll
@@ -91,14 +99,15 @@ struct FormArgs {
     int out_rows, length;     // of out: filled up with zeros
 };
 // Rows as operand rows, eight values a thread.  Bound by memory: 8192 x 4096 bf16 in TODO us.
-template <int DT> __global__ __launch_bounds__(256) void form_kernel(FormArgs a) {
+template <int DT, class Product> __global__ __launch_bounds__(256) void form_kernel(FormArgs a) {
+    typedef OperandOf<DT, Product> To;
     const int pieces = a.length / 8;
     const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, r = k / pieces;
     const int c = (int)(k - r * pieces) * 8;
     if (r >= a.out_rows) return;
     float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if (r < a.rows && c < a.cols && !(a.labels && a.labels[r] == kIgnored)) load_values<DT>(v, a.x + (r * a.stride + c) * DTypeInfo<DT>::bytes, a.cols - c);
-    OperandOf<DT>::store(v, a.out + (r * a.length + c) * 2, a.part_stride, -1);
+    To::store(v, a.out + (r * a.length + c) * To::kBytes, a.part_stride, -1);
 }
 
 // ------------------------------------------------------------------------------------------- forward
@@ -312,8 +321,9 @@ struct GradArgs {
     int first;             // the piece's first token of the vocabulary
     float kept, even;      // 1 - e, e / V
 };
-template <int DT> struct GradOut {
+template <int DT, class Product> struct GradOut {
     static constexpr bool kColumns = false;
+    typedef OperandOf<DT, Product> To;
     const GradArgs& a;
     struct In { float lse, factor; int label; };
     __device__ __forceinline__ void begin(int) const {}
@@ -329,7 +339,7 @@ template <int DT> struct GradOut {
             if (at == k) g -= a.kept;
             v[k] = in.label == kIgnored || j + k >= a.weight.rows ? 0.0f : g * in.factor;
         }
-        const float lost = OperandOf<DT>::store(v, a.grad + ((int64_t)i * a.length + j) * 2, a.part_stride, at);
+        const float lost = To::store(v, a.grad + ((int64_t)i * a.length + j) * To::kBytes, a.part_stride, at);
         if (at >= 0 && at < 8) a.lost[i] = lost;
     }
 };
@@ -341,7 +351,7 @@ template <int DT, class Product, int WT, int STAGES> __global__ __launch_bounds_
     Tile tile(smem);
     tile.segment_stages = a.segment_stages;
     tile.multiply(a.x, a.weight, row0, col0, a.row_bytes);
-    GradOut<DT> out{a};
+    GradOut<DT, Product> out{a};
     tile.finish(row0, col0, out);
 }
 
@@ -466,14 +476,24 @@ constexpr int64_t kPieceValues = 1 << 27;        // of G, as rows and as columns
 constexpr fo::TileCost kTileCosts[] = {
     {128, 2, 1, 20.0, 0.0216, 20.0, 0.0216}, {96, 3, 1, 15.0, 0.0137, 15.0, 0.0137}, {64, 2, 2, 6.8, 0.0099, 9.9, 0.0130},
     {32, 2, 5, 3.2, 0.0071, 7.4, 0.0161}, {32, 4, 2, 4.6, 0.0034, 5.5, 0.0054}};
+constexpr fo::TileCost kTileCostsF32[] = {
+    {128, 2, 1, 20.0, 0.22, 20.0, 0.22}, {96, 3, 1, 15.0, 0.124, 15.0, 0.124}, {64, 2, 2, 8.0, 0.055, 10.0, 0.110},
+    {32, 2, 5, 3.5, 0.0142, 8.0, 0.069}, {32, 4, 2, 4.6, 0.0139, 6.0, 0.0277}};
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t aligned(int64_t bytes) { return round_up(bytes, 256); }
-// An operand's rows; those in parts are contracted segment after segment, each of whole stages.
-int64_t length_of(int dtype, int64_t n) { return round_up(n, dtype == FO_F32 ? 64 : 32); }
-int parts_of(int dtype) { return dtype == FO_F32 ? 3 : 1; }
-int64_t segments_of(int dtype) { return dtype == FO_F32 ? fo::kSegments : 1; }
-int64_t form_bytes(int dtype, int64_t rows, int64_t inner) { return aligned(rows * length_of(dtype, inner) * parts_of(dtype) * 2); }
+// How operands are held: in their own type, or fp32 in three bf16 parts, contracted segment after segment, each of whole stages.
+struct Mode {
+    int dtype;
+    bool in_parts;
+    int bytes() const { return dtype == FO_F32 && !in_parts ? 4 : 2; }
+    int parts() const { return in_parts ? 3 : 1; }
+    int segments() const { return in_parts ? fo::kSegments : 1; }
+    int64_t length(int64_t n) const { return round_up(n, in_parts ? 64 : 64 / bytes()); }                     // of an operand's row
+    int64_t form(int64_t rows, int64_t inner) const { return aligned(rows * length(inner) * parts() * bytes()); }
+    int stages(int64_t values) const { return (int)(values * bytes() / fo::kStageBytes); }
+    const fo::TileCost (&costs() const)[5] { return dtype == FO_F32 && !in_parts ? kTileCostsF32 : kTileCosts; }
+};
 
 int validate(const char* what, int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
     if (tokens < 0 || cols < 0 || vocabulary < 0) return fail(FO_ERR_INVALID_ARGUMENT, "%s: negative size", what);
@@ -494,14 +514,27 @@ template <class K, class A> int launch(K kernel, int64_t grid, int threads, int 
 }
 
 // ---- products in tiles of a size that suits the result
-fo::TileCost tile_for(int64_t rows, int64_t cols, double inner, int cus) {
+fo::TileCost tile_for(const Mode& mode, int64_t rows, int64_t cols, double inner, int cus, double* time_of = nullptr) {
     fo::TileCost best{};
     double least = 0.0;
-    for (const fo::TileCost& t : kTileCosts) {
+    for (const fo::TileCost& t : mode.costs()) {
         const double time = fo::tiles_time(t, (double)fo::tiles_of(rows, cols, t.wt), inner, cus);
         if (!best.wt || time < least) { best = t; least = time; }
     }
+    if (time_of) *time_of = least;
     return best;
+}
+
+// fp32 in parts where that takes less: the logits in six times the length with what laying out both operands moves (10 bytes a value, at 4 TB/s) against fp32
+// instructions.  TODO
+Mode mode_of(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int cus) {
+    if (dtype != FO_F32) return {dtype, false};
+    const Mode whole{dtype, false}, parts{dtype, true};
+    double by_whole, by_parts;
+    (void)tile_for(whole, tokens, vocabulary, (double)whole.length(cols), cus, &by_whole);
+    (void)tile_for(parts, tokens, vocabulary, (double)(parts.length(cols) * parts.segments()), cus, &by_parts);
+    by_parts += (double)(tokens + vocabulary) * (double)cols * 10e-6 / 4.0;
+    return by_parts < by_whole ? parts : whole;
 }
 
 // A product of few tiles over a long contraction is cut along it: parts of whole stages, their fp32 results joined by another launch.  1003 x 1000 over
@@ -509,9 +542,9 @@ fo::TileCost tile_for(int64_t rows, int64_t cols, double inner, int cus) {
 struct Cut { fo::TileCost tile; int parts; int64_t part; double time; };
 constexpr int kMostParts = 32;
 constexpr int64_t kLeastPartValues = 512;
-Cut cut_for(int64_t rows, int64_t cols, int64_t inner, int cus) {
+Cut cut_for(const Mode& mode, int64_t rows, int64_t cols, int64_t inner, int cus) {
     Cut best{};
-    for (const fo::TileCost& t : kTileCosts) {
+    for (const fo::TileCost& t : mode.costs()) {
         const double tiles = (double)fo::tiles_of(rows, cols, t.wt);
         for (int parts = 1; parts <= kMostParts; parts = parts < 4 ? parts + 1 : parts + parts / 2) {
             if (parts > 1 && inner < parts * kLeastPartValues) break;
@@ -570,34 +603,46 @@ struct Matrix {
     int dtype;
     int64_t width() const { return dtype == FO_F32 ? 4 : 2; }
     Matrix part(int64_t first, int64_t n) const { return {p + first * stride * width(), stride, n, cols, dtype}; }
-    // Whether the rows are operand rows as they are.
-    bool ready() const { return dtype != FO_F32 && cols % 32 == 0 && stride % 8 == 0 && stride >= 0 && stride < (1 << 22) && ((uintptr_t)p & 15) == 0; }
+    // Whether the rows can be operand rows where they are: whole pieces, aligned.
+    bool ready(const Mode& m) const {
+        const int64_t per = 16 / width();
+        return !m.in_parts && cols % per == 0 && stride % per == 0 && stride >= 0 && stride < (1 << 22) && ((uintptr_t)p & 15) == 0;
+    }
 };
-// The rows of an operand, or (turned) `depth` rows whose columns are it.  part_stride: see fo_gemm.h.
-fo::Operand operand(const void* p, int64_t length, int64_t rows, int64_t part_stride, u32 order) { return {(const char*)p, length * 2, nullptr, 0, (int)rows, 0, part_stride, order}; }
+// Rows of an operand, `stride` bytes apart.  part_stride, order: see fo_gemm.h.
+fo::Operand operand(const void* p, int64_t stride, int64_t rows, int64_t part_stride, u32 order) { return {(const char*)p, stride, nullptr, 0, (int)rows, 0, part_stride, order, 0}; }
+// The same whose columns are the operand: `depth` rows of `length` values.
 fo::Operand turned(fo::Operand o, int64_t length, int64_t depth) {
     o.rows = (int)length;
     o.depth = (int)depth;
+    o.pieces = 0;
     return o;
 }
 
-// The rows of m as an operand: in place where they are one and `copy` does not ask for more, else laid out at `space`, filled up to out_rows rows.  labels: see FormArgs.
-int operand_of(const Matrix& m, bool copy, const int* labels, int64_t out_rows, char* space, u32 order, fo::Operand& to, hipStream_t s, const char* what) {
-    if (m.ready() && !copy) { to = operand(m.p, m.stride, m.rows, 0, order); return 0; }
-    const int64_t length = length_of(m.dtype, m.cols), part_stride = out_rows * length * 2;
-    to = operand(space, length, m.rows, part_stride, order);
+// The rows of m as an operand: in place where they can be and `copy` does not ask for more, else laid out at `space`, filled up to out_rows rows.  labels: see FormArgs.
+int operand_of(const Mode& mode, const Matrix& m, bool copy, const int* labels, int64_t out_rows, char* space, u32 order, fo::Operand& to, hipStream_t s, const char* what) {
+    const int64_t length = mode.length(m.cols);
+    if (m.ready(mode) && !copy) {
+        to = operand(m.p, m.stride * m.width(), m.rows, 0, order);
+        to.pieces = m.cols == length ? 0 : (int)(m.cols * m.width() / 16);
+        return 0;
+    }
+    const int64_t part_stride = out_rows * length * mode.bytes();
+    to = operand(space, length * mode.bytes(), m.rows, part_stride, order);
     const fo::FormArgs a{m.p, space, labels, m.stride, part_stride, (int)m.rows, (int)m.cols, (int)out_rows, (int)length};
     const int64_t grid = (out_rows * (length / 8) + 255) / 256;
     switch (m.dtype) {
-        case FO_F32: return launch(fo::form_kernel<fo::DT_F32>, grid, 256, 0, s, what, a);
-        case FO_BF16: return launch(fo::form_kernel<fo::DT_BF16>, grid, 256, 0, s, what, a);
-        default: return launch(fo::form_kernel<fo::DT_F16>, grid, 256, 0, s, what, a);
+        case FO_F32:
+            return mode.in_parts ? launch(fo::form_kernel<fo::DT_F32, fo::Bf16PartsProduct>, grid, 256, 0, s, what, a)
+                                 : launch(fo::form_kernel<fo::DT_F32, fo::F32Product>, grid, 256, 0, s, what, a);
+        case FO_BF16: return launch(fo::form_kernel<fo::DT_BF16, fo::Bf16Product>, grid, 256, 0, s, what, a);
+        default: return launch(fo::form_kernel<fo::DT_F16, fo::F16Product>, grid, 256, 0, s, what, a);
     }
 }
 
-template <class Product, bool TURNED> int product(fo::GradProductArgs a, const Cut& cut, float* partial, hipStream_t s, const char* what) {
+template <class Product, bool TURNED> int product(const Mode& mode, fo::GradProductArgs a, const Cut& cut, float* partial, hipStream_t s, const char* what) {
     a.parts = cut.parts;
-    a.part_stages = (int)(cut.part / 64);
+    a.part_stages = mode.stages(cut.part);
     if (cut.parts == 1) return launch_tiles<ProductLaunch<Product, TURNED>>(cut.tile, a, s, what);
     fo::GradProductArgs some = a;
     some.more = nullptr;
@@ -610,9 +655,10 @@ template <class Product, bool TURNED> int product(fo::GradProductArgs a, const C
     return check_hip(hipGetLastError(), what);
 }
 
-template <class F> int by_product(int dtype, const F& f) {
-    if (dtype == FO_F32) return f.template run<fo::DT_F32, fo::Bf16PartsProduct>();
-    return dtype == FO_BF16 ? f.template run<fo::DT_BF16, fo::Bf16Product>() : f.template run<fo::DT_F16, fo::F16Product>();
+template <class F> int by_product(const Mode& mode, const F& f) {
+    if (mode.in_parts) return f.template run<fo::DT_F32, fo::Bf16PartsProduct>();
+    if (mode.dtype == FO_F32) return f.template run<fo::DT_F32, fo::F32Product>();
+    return mode.dtype == FO_BF16 ? f.template run<fo::DT_BF16, fo::Bf16Product>() : f.template run<fo::DT_F16, fo::F16Product>();
 }
 
 // Compute units to plan for; without a device those of this part, so that sizes can be asked for anywhere.
@@ -633,15 +679,15 @@ int check_common(const char* what, const void* x, const void* weight, int reduct
 constexpr int kLeastPart = 32;    // columns of the smallest tile's wavefront
 struct ForwardSpace {
     int64_t picked, losses, stats, sums, x, weight, total;
-    ForwardSpace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
+    ForwardSpace(const Mode& mode, int64_t tokens, int64_t cols, int64_t vocabulary) {
         const int64_t rows = tokens < kBlockTokens ? tokens : kBlockTokens, parts = (vocabulary + kLeastPart - 1) / kLeastPart;
         picked = 0;
         losses = picked + aligned(rows * 4);
         stats = losses + aligned(tokens * 4);
         sums = stats + aligned(rows * parts * 8);
         x = sums + aligned(rows * parts * 4);
-        weight = x + form_bytes(dtype, rows, cols);
-        total = weight + form_bytes(dtype, vocabulary, cols);
+        weight = x + mode.form(rows, cols);
+        total = weight + mode.form(vocabulary, cols);
     }
 };
 
@@ -649,21 +695,21 @@ struct BackwardSpace {
     int64_t piece;    // tokens of the vocabulary at a time
     int64_t factors, lost, scale, x, weight, grad, sums, partial, total;
     Cut dx_cut, dw_cut;
-    BackwardSpace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, bool dx, bool dw, int cus) {
-        const int64_t most = round_up(kPieceValues / parts_of(dtype) / tokens + 1, 256);
+    BackwardSpace(const Mode& mode, int64_t tokens, int64_t cols, int64_t vocabulary, bool dx, bool dw, int cus) {
+        const int64_t most = round_up(kPieceValues * 2 / (mode.parts() * mode.bytes()) / tokens + 1, 256);
         const int64_t pieces = (vocabulary + most - 1) / most;
         piece = round_up((vocabulary + pieces - 1) / pieces, 256);
         if (piece > vocabulary) piece = vocabulary;
         // a last piece that is shorter goes by the same cuts: its parts are fewer
-        dx_cut = dx ? cut_for(tokens, cols, length_of(dtype, piece) * segments_of(dtype), cus) : Cut{};
-        dw_cut = dw ? cut_for(piece, cols, length_of(dtype, tokens) * segments_of(dtype), cus) : Cut{};
+        dx_cut = dx ? cut_for(mode, tokens, cols, mode.length(piece) * mode.segments(), cus) : Cut{};
+        dw_cut = dw ? cut_for(mode, piece, cols, mode.length(tokens) * mode.segments(), cus) : Cut{};
         factors = 0;
         lost = factors + aligned(tokens * 4);
         scale = lost + aligned(tokens * 4);
         x = scale + 256;
-        weight = x + form_bytes(dtype, length_of(dtype, tokens), cols);
-        grad = weight + form_bytes(dtype, piece, cols);
-        sums = grad + form_bytes(dtype, tokens, piece);
+        weight = x + mode.form(mode.length(tokens), cols);
+        grad = weight + mode.form(piece, cols);
+        sums = grad + mode.form(tokens, piece);
         partial = sums + (dx && piece < vocabulary ? aligned(tokens * cols * 4) : 0);
         const int64_t of_dx = dx_cut.parts > 1 ? dx_cut.parts * tokens * cols : 0, of_dw = dw_cut.parts > 1 ? dw_cut.parts * piece * cols : 0;
         total = partial + aligned((of_dx > of_dw ? of_dx : of_dw) * 4);
@@ -671,6 +717,7 @@ struct BackwardSpace {
 };
 
 struct Forward {
+    Mode mode;
     Matrix x, weight;
     const void* targets;
     int index_bytes, reduction;
@@ -678,25 +725,24 @@ struct Forward {
     float smoothing;
     float *loss, *kept;
     char* base;
+    int cus;
     hipStream_t s;
 
     template <int DT, class Product> int run() const {
         const char* what = "fo_linear_cross_entropy";
-        const int cus = compute_units();
-        if (cus <= 0) return fail(FO_ERR_NO_DEVICE, "no device");
-        const ForwardSpace at(x.dtype, x.rows, x.cols, weight.rows);
+        const ForwardSpace at(mode, x.rows, x.cols, weight.rows);
         int* labels = (int*)(kept + x.rows + 1);
         const fo::Targets t{targets, index_bytes};
         float* losses = reduction == FO_REDUCE_NONE ? loss : (float*)(base + at.losses);
         fo::Operand w;
-        if (int rc = operand_of(weight, false, nullptr, weight.rows, base + at.weight, fo::kRightOrder, w, s, what)) return rc;
-        const int64_t length = length_of(x.dtype, x.cols);
-        const int row_bytes = (int)(length * segments_of(x.dtype) * 2), segment = (int)(length / 64);
+        if (int rc = operand_of(mode, weight, false, nullptr, weight.rows, base + at.weight, fo::kRightOrder, w, s, what)) return rc;
+        const int64_t length = mode.length(x.cols), inner = length * mode.segments();
+        const int row_bytes = (int)(inner * mode.bytes()), segment = mode.stages(length);
         for (int64_t first = 0; first < x.rows; first += kBlockTokens) {
             const Matrix some = x.part(first, x.rows - first < kBlockTokens ? x.rows - first : kBlockTokens);
             fo::Operand rows;
-            if (int rc = operand_of(some, false, nullptr, some.rows, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
-            const fo::TileCost tile = tile_for(some.rows, weight.rows, row_bytes / 2, cus);
+            if (int rc = operand_of(mode, some, x.cols != length, nullptr, some.rows, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
+            const fo::TileCost tile = tile_for(mode, some.rows, weight.rows, (double)inner, cus);
             const fo::LogitsArgs a{rows, w, row_bytes, segment, t, first, (fo::f32x2*)(base + at.stats), smoothing > 0.0f ? (float*)(base + at.sums) : nullptr, (float*)(base + at.picked)};
             if (int rc = launch_tiles<LogitsLaunch<Product>>(tile, a, s, what)) return rc;
             const fo::JoinArgs join{a.stats, a.sums, a.picked, t, first, ignore, weight.rows, kept + first, losses + first, labels + first, (int)some.rows,
@@ -714,6 +760,7 @@ struct Forward {
 };
 
 struct Backward {
+    Mode mode;
     Matrix x, weight;
     int reduction;
     float smoothing;
@@ -732,54 +779,54 @@ struct Backward {
         fo::loss_factors_kernel<<<dim3(1), dim3(1024), 0, s>>>(upstream, upstream_stride, labels, x.rows, reduction, kept + x.rows, x.dtype == FO_F16 ? 32768.0f : 1.0f,
                                                                factors, lost, scale);
         if (int rc = check_hip(hipGetLastError(), what)) return rc;
-        const int dtype = x.dtype;
-        const int64_t tokens_length = length_of(dtype, x.rows), cols_length = length_of(dtype, x.cols), segments = segments_of(dtype);
+        const int64_t tokens_length = mode.length(x.rows), cols_length = mode.length(x.cols), cols_inner = cols_length * mode.segments();
         fo::Operand rows;
-        if (int rc = operand_of(x, dw != nullptr, labels, tokens_length, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
+        if (int rc = operand_of(mode, x, dw != nullptr || x.cols != cols_length, labels, tokens_length, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
         fo::Operand x_turned = turned(rows, cols_length, tokens_length);
         x_turned.order = fo::kRightOrder;
         for (int64_t first = 0; first < weight.rows; first += at.piece) {
-            const int64_t n = weight.rows - first < at.piece ? weight.rows - first : at.piece, length = length_of(dtype, n);
+            const int64_t n = weight.rows - first < at.piece ? weight.rows - first : at.piece, length = mode.length(n);
             const bool last = first + n == weight.rows;
+            const Matrix some = weight.part(first, n);
             fo::Operand w;
-            if (int rc = operand_of(weight.part(first, n), false, nullptr, n, base + at.weight, fo::kRightOrder, w, s, what)) return rc;
-            const fo::Operand g = operand(base + at.grad, length, x.rows, x.rows * length * 2, fo::kLeftOrder);
-            const fo::GradArgs grad{rows, w, (int)(cols_length * segments * 2), (int)(cols_length / 64), labels, kept, factors, base + at.grad, lost, g.part_stride, (int)length,
+            if (int rc = operand_of(mode, some, false, nullptr, n, base + at.weight, fo::kRightOrder, w, s, what)) return rc;
+            const fo::Operand g = operand(base + at.grad, length * mode.bytes(), x.rows, x.rows * length * mode.bytes(), fo::kLeftOrder);
+            const fo::GradArgs grad{rows, w, (int)(cols_inner * mode.bytes()), mode.stages(cols_length), labels, kept, factors, base + at.grad, lost, g.part_stride, (int)length,
                                     (int)first, 1.0f - smoothing, smoothing / (float)weight.rows};
-            if (int rc = launch_tiles<GradLaunch<DT, Product>>(tile_for(x.rows, n, (double)(cols_length * segments), cus), grad, s, what)) return rc;
+            if (int rc = launch_tiles<GradLaunch<DT, Product>>(tile_for(mode, x.rows, n, (double)cols_inner, cus), grad, s, what)) return rc;
             fo::GradProductArgs p{};
             p.cols = (int)x.cols;
             p.scale = scale;
             p.stride = x.cols;
-            p.dtype = dtype;
+            p.dtype = x.dtype;
             if (dx) {
                 p.left = g;
-                p.right = turned(w, cols_length, n);
+                p.right = turned(w, some.ready(mode) ? x.cols : cols_length, n);
                 p.rows = (int)x.rows;
-                p.row_bytes = (int)(length * segments * 2);
-                p.segment_stages = (int)(length / 64);
+                p.row_bytes = (int)(length * mode.segments() * mode.bytes());
+                p.segment_stages = mode.stages(length);
                 p.more = first ? sums : nullptr;
                 p.sums = last ? nullptr : sums;
                 p.out = last ? dx : nullptr;
-                p.lost = dtype == FO_F32 ? nullptr : lost;
+                p.lost = x.dtype == FO_F32 ? nullptr : lost;
                 p.labels = labels;
                 p.weight = weight.p;
                 p.weight_stride = weight.stride;
                 Cut cut = at.dx_cut;
-                cut.parts = (int)((length * segments + cut.part - 1) / cut.part);
-                if (int rc = product<Product, false>(p, cut, partial, s, what)) return rc;
+                cut.parts = (int)((length * mode.segments() + cut.part - 1) / cut.part);
+                if (int rc = product<Product, false>(mode, p, cut, partial, s, what)) return rc;
             }
             if (dw) {
                 p.left = turned(g, length, x.rows);
                 p.right = x_turned;
                 p.rows = (int)n;
-                p.row_bytes = (int)(tokens_length * segments * 2);
-                p.segment_stages = (int)(tokens_length / 64);
+                p.row_bytes = (int)(tokens_length * mode.segments() * mode.bytes());
+                p.segment_stages = mode.stages(tokens_length);
                 p.more = nullptr;
                 p.sums = nullptr;
                 p.out = dw + first * x.cols * x.width();
                 p.lost = nullptr;
-                if (int rc = product<Product, true>(p, at.dw_cut, partial, s, what)) return rc;
+                if (int rc = product<Product, true>(mode, p, at.dw_cut, partial, s, what)) return rc;
             }
         }
         return 0;
@@ -792,7 +839,7 @@ extern "C" {
 
 int64_t fo_linear_cross_entropy_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
     if (int rc = validate("fo_linear_cross_entropy", dtype, tokens, cols, vocabulary)) return rc;
-    return ForwardSpace(dtype, tokens, cols, vocabulary).total;
+    return ForwardSpace(mode_of(dtype, tokens, cols, vocabulary, units()), tokens, cols, vocabulary).total;
 }
 
 int fo_linear_cross_entropy(const void* x, int dtype, int64_t tokens, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t vocabulary, int64_t cols,
@@ -803,16 +850,18 @@ int fo_linear_cross_entropy(const void* x, int dtype, int64_t tokens, int64_t x_
     if (int rc = check_common(what, x, weight, reduction, smoothing, workspace)) return rc;
     if (!targets || !loss || !kept) return fail(FO_ERR_INVALID_ARGUMENT, "%s: targets, loss and kept must not be NULL", what);
     if (index_bytes != 4 && index_bytes != 8) return fail(FO_ERR_INVALID_ARGUMENT, "%s: targets of %d bytes", what, index_bytes);
-    if (workspace_bytes < ForwardSpace(dtype, tokens, cols, vocabulary).total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
-    const Forward f{{(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, targets, index_bytes, reduction,
-                    ignore, smoothing, loss, kept, (char*)workspace, (hipStream_t)stream};
-    return by_product(dtype, f);
+    const int cus = units();
+    const Mode mode = mode_of(dtype, tokens, cols, vocabulary, cus);
+    if (workspace_bytes < ForwardSpace(mode, tokens, cols, vocabulary).total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+    const Forward f{mode, {(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, targets, index_bytes, reduction,
+                    ignore, smoothing, loss, kept, (char*)workspace, cus, (hipStream_t)stream};
+    return by_product(mode, f);
 }
 
 int64_t fo_linear_cross_entropy_backward_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int want_dx, int want_dw) {
     if (int rc = validate("fo_linear_cross_entropy_backward", dtype, tokens, cols, vocabulary)) return rc;
     const int cus = units();
-    return BackwardSpace(dtype, tokens, cols, vocabulary, want_dx != 0, want_dw != 0, cus).total;
+    return BackwardSpace(mode_of(dtype, tokens, cols, vocabulary, cus), tokens, cols, vocabulary, want_dx != 0, want_dw != 0, cus).total;
 }
 
 int fo_linear_cross_entropy_backward(const void* x, int dtype, int64_t tokens, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t vocabulary,
@@ -823,11 +872,12 @@ int fo_linear_cross_entropy_backward(const void* x, int dtype, int64_t tokens, i
     if (int rc = check_common(what, x, weight, reduction, smoothing, workspace)) return rc;
     if (!kept || !upstream || (!dx && !dw)) return fail(FO_ERR_INVALID_ARGUMENT, "%s: kept, upstream and a result must be given", what);
     const int cus = units();
-    const BackwardSpace at(dtype, tokens, cols, vocabulary, dx != nullptr, dw != nullptr, cus);
+    const Mode mode = mode_of(dtype, tokens, cols, vocabulary, cus);
+    const BackwardSpace at(mode, tokens, cols, vocabulary, dx != nullptr, dw != nullptr, cus);
     if (workspace_bytes < at.total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
-    const Backward b{{(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, reduction, smoothing, kept, upstream,
+    const Backward b{mode, {(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, reduction, smoothing, kept, upstream,
                      upstream_stride, (char*)dx, (char*)dw, (char*)workspace, at, cus, (hipStream_t)stream};
-    return by_product(dtype, b);
+    return by_product(mode, b);
 }
 
 }  // extern "C"
