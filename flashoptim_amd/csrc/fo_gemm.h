@@ -311,8 +311,8 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
     __device__ __forceinline__ int turned_byte(int i) const { return (wave & 1) * (kRowLoads * 1024) + i * 1024 + lane * 16; }
     __device__ __forceinline__ int turned_row(int i) const { return turned_byte(i) / kTurnedRow; }
 
-    // The i-th load of a stage.  half: the rows end in the middle of the stage, its second half repeats the first.
-    __device__ __forceinline__ void load(const Loader& l, int i, int stage, bool half) const {
+    // The i-th load of a stage.  LAST: it may be the last one of the contraction, where rows end; half: in the middle of the stage, its second half repeats the first.
+    template <bool LAST> __device__ __forceinline__ void load(const Loader& l, int i, int stage, bool half) const {
         const unsigned buffer = smem_address + buffer_of(stage);
         const char* base = l.base;
         stage += first_stage;
@@ -323,27 +323,22 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
             stage -= segment * segment_stages;
             base += (int64_t)(l.order >> 2 * segment & 3) * l.part_stride;
         }
-        if ((KA || KB) && l.turned) {
-            const int last = l.depth - 1 - stage * kTurnedRows;    // row of the stage
-            unsigned at = l.row[i];
-            if (last < kTurnedRows - 1) {
-                const int k = turned_row(i);
-                at -= k > last ? (unsigned)(k - last) * l.line : 0u;
-            }
-            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, at, base + stage * l.step);
-            return;
-        }
         if (i < kRowLoads) {
             unsigned at = l.row[i];
-            if (half || stage >= l.whole_stages) {    // pieces behind the last one there is, or behind the half, repeat the last before
-                const int piece = i & 1 ? l.piece ^ 4 : l.piece, left = l.pieces ? l.pieces - stage * 8 : 8;
-                const int last = (half && left > 4 ? 4 : left) - 1;
-                at -= piece > last ? (unsigned)(piece - last) * 16 : 0u;
+            if constexpr (LAST || Product::kParts) {    // a segment's end may be anywhere
+                if ((KA || KB) && l.turned) {
+                    const int last = l.depth - 1 - stage * kTurnedRows, k = turned_row(i);    // rows of the stage
+                    at -= k > last ? (unsigned)(k - last) * l.line : 0u;
+                } else if (half || stage >= l.whole_stages) {    // pieces behind the last one there is, or behind the half, repeat the last before
+                    const int piece = i & 1 ? l.piece ^ 4 : l.piece, left = l.pieces ? l.pieces - stage * 8 : 8;
+                    const int last = (half && left > 4 ? 4 : left) - 1;
+                    at -= piece > last ? (unsigned)(piece - last) * 16 : 0u;
+                }
             }
-            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, at, base + (int64_t)stage * kStageBytes);
+            load_to_lds16(buffer + (wave * kRowLoads + i) * 1024, at, base + stage * l.step);
         } else if constexpr (Product::kScaled) {
             const int k = i - kRowLoads;
-            load_to_lds4(buffer + kScaleOffset + (wave * kScaleLoads + k) * 256, l.scale[k] - (half ? l.past_half_scale : 0),
+            load_to_lds4(buffer + kScaleOffset + (wave * kScaleLoads + k) * 256, l.scale[k] - (LAST && half ? l.past_half_scale : 0),
                          l.scale_base + (int64_t)stage * (kStageBytes / 16));
         }
     }
@@ -401,10 +396,11 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
         }
     }
 
-    // Phase HALF of a stage: multiplies `now` while reading the operands of the next phase and, with LOAD, issuing a stage's loads:
+    // Phase HALF of a stage: multiplies `now` while reading the operands of the next phase and, where LOAD says so, issuing a stage's loads:
     // at most one of each between two matrix instructions, fenced so that they stay there (in clumps they hold the wavefront
     // up: 5 % of the rate at 4096 x 4096 x 8192).  The reads end a quarter before the phase does, so the next finds its operands.
-    template <int HALF, bool LOAD>
+    enum { kNoLoad = 0, kLoad = 1, kLoadLast = 2 };
+    template <int HALF, int LOAD>
     __device__ __forceinline__ void phase(const Operands& now, const Scales& scales, Operands& next, Scales& next_scales, int read_stage,
                                           bool read_short, const Loader& l, int load_stage, bool load_half) {
         constexpr int kAll = kFrags * kFrags;
@@ -413,10 +409,10 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
         constexpr int kReadWithin = kAll >= 16 ? kAll - kAll / 4 : kAll;
 #pragma unroll
         for (int q = 0; q < kAll; ++q) {
-            if constexpr (LOAD) {
+            if constexpr (LOAD != kNoLoad) {
 #pragma unroll
                 for (int k = q * kLoads / kAll; k < (q + 1) * kLoads / kAll; ++k) {
-                    load(l, k, load_stage, load_half);
+                    load<LOAD == kLoadLast>(l, k, load_stage, load_half);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -468,7 +464,7 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
         for (int stage = 0; stage < kStages; ++stage) {
             if (stage >= stages) break;
 #pragma unroll
-            for (int k = 0; k < kLoads; ++k) load(l, k, stage, odd && stages == stage + 1);
+            for (int k = 0; k < kLoads; ++k) load<true>(l, k, stage, odd && stages == stage + 1);
         }
         wait_behind(stages - 1);
         meet();
@@ -481,21 +477,29 @@ template <class Product, int WT, int STAGES, bool KA = false, bool KB = false> s
             if constexpr (Product::kScaled) read_scales(raw, f, 0, first_short);
         }
         int s = 0;
-        for (; s + kStages < stages; ++s) {
+        for (; s + kStages + 1 < stages; ++s) {
             settle(scales, raw, false);
-            phase<0, false>(even, scales, uneven, raw, s, false, l, 0, false);
+            phase<0, kNoLoad>(even, scales, uneven, raw, s, false, l, 0, false);
             wait_loads_and_lds<(kStages - 2) * kLoads>();  // stage s is in registers, stage s + 1 in LDS
             meet();
-            phase<1, true>(uneven, scales, even, raw, s + 1, odd && s + 2 == stages, l, s + kStages, odd && s + kStages + 1 == stages);
+            phase<1, kLoad>(uneven, scales, even, raw, s + 1, false, l, s + kStages, false);
+        }
+        if (s + kStages < stages) {   // the same with the loads of the last stage
+            settle(scales, raw, false);
+            phase<0, kNoLoad>(even, scales, uneven, raw, s, false, l, 0, false);
+            wait_loads_and_lds<(kStages - 2) * kLoads>();
+            meet();
+            phase<1, kLoadLast>(uneven, scales, even, raw, s + 1, odd && s + 2 == stages, l, s + kStages, odd);
+            ++s;
         }
         for (;; ++s) {
             const bool last = s + 1 == stages;
             settle(scales, raw, odd && last);
-            phase<0, false>(even, scales, uneven, raw, s, false, l, 0, false);
+            phase<0, kNoLoad>(even, scales, uneven, raw, s, false, l, 0, false);
             wait_behind(stages - s - 2);
             meet();
             if (last && odd) break;
-            phase<1, false>(uneven, scales, even, raw, s + 1, odd && s + 2 == stages, l, 0, false);
+            phase<1, kNoLoad>(uneven, scales, even, raw, s + 1, odd && s + 2 == stages, l, 0, false);
             if (last) break;
         }
         asm volatile("s_nop 15\n\ts_nop 3" : : : "memory");  // the last results are written
