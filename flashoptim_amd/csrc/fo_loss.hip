@@ -14,7 +14,7 @@
 // Types.  bf16 and fp16 operands go into the matrix cores as they are, sums are fp32.  G is rounded to the operands' type once, as the
 // other operand of its products is; the factors f_i are first divided by the largest of them (and multiplied by 2^15 for fp16, so that probabilities down to 2^-39
 // survive), which the products' results are multiplied by at the end: where all are equal, as in a mean, they are 1, and the entry p - 1 of an unlikely
-// target rounds to almost itself.  What the target's entry, by far the largest of most rows, loses in its rounding goes into dx all the same: that times the
+// target rounds to almost itself.  Of few rows, what the target's entry, by far the largest of most, loses in its rounding goes into dx all the same: that times the
 // target's row of W is added in fp32.  fp32 operands go into the fp32 instructions, a sixteenth of the rate; or, where the work is large enough to pay for laying
 // them out (in_parts), they are cut into three bf16 parts of 8 bits each, a = a1 + a2 + a3
 // exactly, and the six products a3 b1, a2 b2, a1 b3, a2 b1, a1 b2, a1 b1 are one contraction over six times the length: what is left
@@ -285,9 +285,21 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* losses, 
 }
 
 // ------------------------------------------------------------------------------------------- backward
-// factors[i]: f_i over the largest magnitude among them, times `top` (a power of two); scale[0]: what that is to be multiplied by.
+// What the products' results are multiplied by at the end: f_i over the factors that went into G.  One upstream for all rows is that itself, over the number of
+// targets where the loss is a mean; the factors are 1 then, and no launch is needed for them.
+struct Scale {
+    const float* p;         // the upstream, or what loss_factors_kernel made of many
+    const float* count;     // or null
+    float over;             // `top`
+    __device__ __forceinline__ float value() const {
+        if (!count) return p[0] * over;
+        return count[0] > 0.0f ? p[0] * (1.0f / count[0]) * over : 0.0f;    // no targets, no gradients
+    }
+};
+
+// factors[i]: f_i over the largest magnitude among them, times `top` (a power of two); scale[0]: that magnitude.
 __global__ __launch_bounds__(1024) void loss_factors_kernel(const float* upstream, int64_t stride, const int* labels, int64_t n, int reduction, const float* count,
-                                                            float top, float* factors, float* lost, float* scale) {
+                                                            float top, float* factors, float* scale) {
     __shared__ float mosts[16];
     const float share = reduction == FO_REDUCE_MEAN ? 1.0f / count[0] : 1.0f;
     float most = 0.0f;
@@ -304,18 +316,18 @@ __global__ __launch_bounds__(1024) void loss_factors_kernel(const float* upstrea
     for (int64_t i = threadIdx.x; i < n; i += 1024) {
         const float f = upstream[i * stride] * share / most * top;
         factors[i] = labels[i] == kIgnored ? 0.0f : labels[i] == kNone ? __builtin_nanf("") : f;
-        lost[i] = 0.0f;
     }
-    if (threadIdx.x == 0) scale[0] = most / top;
+    if (threadIdx.x == 0) scale[0] = most;
 }
 
 struct GradArgs {
     Operand x, weight;     // of a piece of the vocabulary
     int row_bytes, segment_stages;
     const int* labels;
-    const float *lse, *factors;
+    const float *lse, *factors;    // no factors: `top` for every row
+    float top;
     char* grad;            // G as operand rows over the piece
-    float* lost;           // of each row: what its target's entry lost in its rounding
+    float* lost;           // of each row with a target: what its target's entry lost in its rounding; or null
     int64_t part_stride;
     int length;            // of G's rows
     int first;             // the piece's first token of the vocabulary
@@ -328,7 +340,10 @@ template <int DT, class Product> struct GradOut {
     struct In { float lse, factor; int label; };
     __device__ __forceinline__ void begin(int) const {}
     __device__ __forceinline__ void load(int i, int, In& in) const {
-        if (i < a.x.rows) in = {a.lse[i], a.factors[i], a.labels[i]};
+        if (i >= a.x.rows) return;
+        in.lse = a.lse[i];
+        in.label = a.labels[i];
+        in.factor = a.factors ? a.factors[i] : in.label == kNone ? __builtin_nanf("") : a.top;
     }
     __device__ __forceinline__ void row(int i, int j, In in, float (&v)[8]) const {
         if (i >= a.x.rows || j >= a.length) return;
@@ -340,7 +355,7 @@ template <int DT, class Product> struct GradOut {
             v[k] = in.label == kIgnored || j + k >= a.weight.rows ? 0.0f : g * in.factor;
         }
         const float lost = To::store(v, a.grad + ((int64_t)i * a.length + j) * To::kBytes, a.part_stride, at);
-        if (at >= 0 && at < 8) a.lost[i] = lost;
+        if (a.lost && at >= 0 && at < 8) a.lost[i] = lost;
     }
 };
 template <int DT, class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void grad_kernel(GradArgs a) {
@@ -362,8 +377,8 @@ struct GradProductArgs {
     int row_bytes, segment_stages, part_stages, parts;
     const float* more;     // what is added, fp32, as far apart as out's rows; or null
     float* sums;           // fp32 results that go on; or
-    char* out;             // the last one, of type `dtype`, times scale[0]
-    const float* scale;
+    char* out;             // the last one, of type `dtype`, times the scale
+    Scale scale;
     const float* lost;     // dx: what the rows' targets lost, times their rows of the weight, is added before that; or null
     const int* labels;
     const char* weight;
@@ -372,7 +387,7 @@ struct GradProductArgs {
     int dtype;
 };
 __device__ __forceinline__ void store_result(float (&v)[8], const GradProductArgs& a, int i, int j, int valid) {
-    const float scale = a.scale[0];
+    const float scale = a.scale.value();
     if (a.lost) {
         const int label = a.labels[i];
         if (label >= 0) {
@@ -468,17 +483,18 @@ using fo::u32;
 constexpr int64_t kMostWorkgroups = (1 << 24) - 1;    // of 256 threads: a launch has less than 2^32 threads
 constexpr int64_t kMostTokens = 1 << 20, kMostCols = 1 << 16, kMostVocabulary = 1 << 24;    // 32-bit offsets into a tile's rows
 constexpr int64_t kBlockTokens = 16384;          // rows of one forward launch: bounds the parts' memory
+constexpr int64_t kFewRows = 256;
 constexpr int64_t kPieceValues = 1 << 27;        // of G, as rows and as columns: 256 MiB each in 16 bits
 
-// Times of bf16 tiles in logits_kernel and grad_product_kernel, which differ by a tenth, over 1024 and 4096 values: a 256 x 256 tile takes 42 and 109 us, 192 x 192
-// 29 and 72, two 128 x 128 on a compute unit 23 and 63 (alone 17 and 48), five 64 x 64 24 and 74 (alone 10 and 32; in four stages 9 and 19, two of
-// those 11 and 27).
+// Times of tiles, middle between the three kinds of products, which differ by a tenth.  bf16 over 1024 and 4096 values: a 256 x 256 tile takes 42 and 108 us, 192 x 192
+// 32 and 78, two 128 x 128 on a compute unit 24 and 63 (alone 17 and 48), five 64 x 64 25 and 76 (alone 10 and 32; in four stages 9 and 20, two of
+// those 12 and 32).  fp32, where large tiles gain nothing, over 512 and 1024: two 128 x 128 74 and 133 (43 and 74), five 64 x 64 54 and 95 (15 and 24; 15 and 24, 23 and 38).
 constexpr fo::TileCost kTileCosts[] = {
-    {128, 2, 1, 20.0, 0.0216, 20.0, 0.0216}, {96, 3, 1, 15.0, 0.0137, 15.0, 0.0137}, {64, 2, 2, 6.8, 0.0099, 9.9, 0.0130},
-    {32, 2, 5, 3.2, 0.0071, 7.4, 0.0161}, {32, 4, 2, 4.6, 0.0034, 5.5, 0.0054}};
+    {128, 2, 1, 20.0, 0.0216, 20.0, 0.0216}, {96, 3, 1, 16.5, 0.0150, 16.5, 0.0150}, {64, 2, 2, 6.8, 0.0101, 10.9, 0.0127},
+    {32, 2, 5, 3.2, 0.0071, 7.6, 0.0168}, {32, 4, 2, 5.2, 0.0035, 5.4, 0.0064}};
 constexpr fo::TileCost kTileCostsF32[] = {
-    {128, 2, 1, 20.0, 0.22, 20.0, 0.22}, {96, 3, 1, 15.0, 0.124, 15.0, 0.124}, {64, 2, 2, 8.0, 0.055, 10.0, 0.110},
-    {32, 2, 5, 3.5, 0.0142, 8.0, 0.069}, {32, 4, 2, 4.6, 0.0139, 6.0, 0.0277}};
+    {64, 2, 2, 11.0, 0.061, 14.0, 0.116}, {32, 2, 5, 5.8, 0.0171, 16.0, 0.0765}, {32, 4, 2, 6.5, 0.0168, 7.0, 0.0305}};
+struct Costs { const fo::TileCost *first, *last; const fo::TileCost* begin() const { return first; } const fo::TileCost* end() const { return last; } };
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t aligned(int64_t bytes) { return round_up(bytes, 256); }
@@ -492,7 +508,7 @@ struct Mode {
     int64_t length(int64_t n) const { return round_up(n, in_parts ? 64 : 64 / bytes()); }                     // of an operand's row
     int64_t form(int64_t rows, int64_t inner) const { return aligned(rows * length(inner) * parts() * bytes()); }
     int stages(int64_t values) const { return (int)(values * bytes() / fo::kStageBytes); }
-    const fo::TileCost (&costs() const)[5] { return dtype == FO_F32 && !in_parts ? kTileCostsF32 : kTileCosts; }
+    Costs costs() const { return dtype == FO_F32 && !in_parts ? Costs{kTileCostsF32, kTileCostsF32 + 3} : Costs{kTileCosts, kTileCosts + 5}; }
 };
 
 int validate(const char* what, int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
@@ -560,6 +576,7 @@ Cut cut_for(const Mode& mode, int64_t rows, int64_t cols, int64_t inner, int cus
 
 template <class Product> struct LogitsLaunch {
     typedef fo::LogitsArgs Args;
+    static constexpr bool kF32 = Product::kBytes == 4;
     template <int WT, int STAGES> static auto kernel() { return fo::logits_kernel<Product, WT, STAGES>; }
     template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES>::kLds; }
     static int64_t rows(const Args& a) { return a.x.rows; }
@@ -568,6 +585,7 @@ template <class Product> struct LogitsLaunch {
 };
 template <int DT, class Product> struct GradLaunch {
     typedef fo::GradArgs Args;
+    static constexpr bool kF32 = Product::kBytes == 4;
     template <int WT, int STAGES> static auto kernel() { return fo::grad_kernel<DT, Product, WT, STAGES>; }
     template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES>::kLds; }
     static int64_t rows(const Args& a) { return a.x.rows; }
@@ -576,6 +594,7 @@ template <int DT, class Product> struct GradLaunch {
 };
 template <class Product, bool TURNED> struct ProductLaunch {
     typedef fo::GradProductArgs Args;
+    static constexpr bool kF32 = Product::kBytes == 4;
     template <int WT, int STAGES> static auto kernel() { return fo::grad_product_kernel<Product, TURNED, WT, STAGES>; }
     template <int WT, int STAGES> static constexpr int lds() { return fo::GemmTile<Product, WT, STAGES, TURNED, true>::kLds; }
     static int64_t rows(const Args& a) { return a.rows; }
@@ -588,9 +607,11 @@ template <class L, int WT, int STAGES> int launch_tiles(const typename L::Args& 
     return launch(L::template kernel<WT, STAGES>(), 8 * fo::seats_of(tiles), 256, L::template lds<WT, STAGES>(), s, what, a);
 }
 template <class L> int launch_tiles(const fo::TileCost& t, const typename L::Args& a, hipStream_t s, const char* what) {
+    if constexpr (!L::kF32) {
+        if (t.wt == 128) return launch_tiles<L, 128, 2>(a, s, what);
+        if (t.wt == 96) return launch_tiles<L, 96, 3>(a, s, what);
+    }
     switch (t.wt) {
-        case 128: return launch_tiles<L, 128, 2>(a, s, what);
-        case 96: return launch_tiles<L, 96, 3>(a, s, what);
         case 64: return launch_tiles<L, 64, 2>(a, s, what);
         default: return t.stages == 4 ? launch_tiles<L, 32, 4>(a, s, what) : launch_tiles<L, 32, 2>(a, s, what);
     }
@@ -774,11 +795,19 @@ struct Backward {
     template <int DT, class Product> int run() const {
         const char* what = "fo_linear_cross_entropy_backward";
         const int* labels = (const int*)(kept + x.rows + 1);
-        float *factors = (float*)(base + at.factors), *lost = (float*)(base + at.lost), *scale = (float*)(base + at.scale);
-        float *sums = (float*)(base + at.sums), *partial = (float*)(base + at.partial);
-        fo::loss_factors_kernel<<<dim3(1), dim3(1024), 0, s>>>(upstream, upstream_stride, labels, x.rows, reduction, kept + x.rows, x.dtype == FO_F16 ? 32768.0f : 1.0f,
-                                                               factors, lost, scale);
-        if (int rc = check_hip(hipGetLastError(), what)) return rc;
+        float *sums = (float*)(base + at.sums), *partial = (float*)(base + at.partial), *factors = nullptr;
+        // With many rows the entries' errors are independent of one another, and what they add to dx is as large as its own rounding at most; few rows are put right, which costs a
+        // read of W beside every piece of the result (20 us of 59 for 4096 x 4096 over 1024).
+        float* lost = x.dtype != FO_F32 && dx && x.rows <= kFewRows ? (float*)(base + at.lost) : nullptr;
+        const float top = x.dtype == FO_F16 ? 32768.0f : 1.0f;
+        fo::Scale scale{upstream, reduction == FO_REDUCE_MEAN ? kept + x.rows : nullptr, 1.0f / top};
+        if (upstream_stride != 0 && x.rows > 1) {
+            factors = (float*)(base + at.factors);
+            float* most = (float*)(base + at.scale);
+            fo::loss_factors_kernel<<<dim3(1), dim3(1024), 0, s>>>(upstream, upstream_stride, labels, x.rows, reduction, kept + x.rows, top, factors, most);
+            if (int rc = check_hip(hipGetLastError(), what)) return rc;
+            scale = {most, nullptr, 1.0f / top};
+        }
         const int64_t tokens_length = mode.length(x.rows), cols_length = mode.length(x.cols), cols_inner = cols_length * mode.segments();
         fo::Operand rows;
         if (int rc = operand_of(mode, x, dw != nullptr || x.cols != cols_length, labels, tokens_length, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
@@ -791,7 +820,7 @@ struct Backward {
             fo::Operand w;
             if (int rc = operand_of(mode, some, false, nullptr, n, base + at.weight, fo::kRightOrder, w, s, what)) return rc;
             const fo::Operand g = operand(base + at.grad, length * mode.bytes(), x.rows, x.rows * length * mode.bytes(), fo::kLeftOrder);
-            const fo::GradArgs grad{rows, w, (int)(cols_inner * mode.bytes()), mode.stages(cols_length), labels, kept, factors, base + at.grad, lost, g.part_stride, (int)length,
+            const fo::GradArgs grad{rows, w, (int)(cols_inner * mode.bytes()), mode.stages(cols_length), labels, kept, factors, top, base + at.grad, lost, g.part_stride, (int)length,
                                     (int)first, 1.0f - smoothing, smoothing / (float)weight.rows};
             if (int rc = launch_tiles<GradLaunch<DT, Product>>(tile_for(mode, x.rows, n, (double)cols_inner, cus), grad, s, what)) return rc;
             fo::GradProductArgs p{};
@@ -808,7 +837,7 @@ struct Backward {
                 p.more = first ? sums : nullptr;
                 p.sums = last ? nullptr : sums;
                 p.out = last ? dx : nullptr;
-                p.lost = x.dtype == FO_F32 ? nullptr : lost;
+                p.lost = lost;
                 p.labels = labels;
                 p.weight = weight.p;
                 p.weight_stride = weight.stride;

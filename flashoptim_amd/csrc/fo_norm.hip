@@ -101,13 +101,13 @@ template <int THREADS, class T> __device__ __forceinline__ T group_sum(T x, T (&
 
 // 1 / sqrt(mean(s^2) + eps).  Squares are added in fp64, which costs nothing beside the loads and holds the squares of every fp32 number, and rounded to fp32 as a
 // mean; only where that is no normal number is the root taken in fp64 too.
-template <int THREADS, int V> __device__ __forceinline__ float inverse_root(const float (&s)[V][8], int cols, float eps, double (&places)[2][16], int& turn, double& sum) {
-    sum = 0.0;
+template <int THREADS, int V> __device__ __forceinline__ float inverse_root(const float (&s)[V][8], int cols, float eps, double (&places)[2][16], int& turn) {
+    double sum = 0.0;
 #pragma unroll
     for (int p = 0; p < V; ++p)
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum = __builtin_fma((double)s[p][k], (double)s[p][k], sum);
-    sum = group_sum<THREADS>(sum, places, turn) / cols;    // the mean, exact to fp64
+    sum = group_sum<THREADS>(sum, places, turn) / cols;
     const float mean = (float)sum + eps;
     if (mean >= 0x1p-120f && mean <= 0x1p126f) return rsqrtf(mean);
     return (float)(1.0 / __builtin_sqrt(sum + (double)eps));
@@ -131,17 +131,6 @@ template <int DT, int THREADS, int V, bool WHOLE> struct Raw {
     }
     __device__ __forceinline__ float value(int p, int k) const { return widen<DT, EPL>(d[p][k / EPL], k % EPL); }
 };
-
-// A norm's output on its way into four bits.  Where the fp32 product is next to a number of three bits or fewer (a border between two codes, or the power of two
-// from which the group's scale would be another), which side of it the exact product lies on is asked of fp64, and the result is put there; one value in
-// 10^5 takes that way.  So the codes are those of the exact norm, however its factors round.
-__device__ __forceinline__ float beside_borders(float y, float s, float w, double mean, float eps) {
-    if (((as_u32(y) + 4u) & 0xfffffu) > 8u || y == 0.0f) return y;
-    const double exact = (double)s * (double)w / __builtin_sqrt(mean + (double)eps);
-    const float near = (float)exact;
-    if ((as_u32(near) & 0xfffffu) != 0u || (double)near == exact) return near;
-    return as_f32(__builtin_fabs(exact) > (double)__builtin_fabsf(near) ? as_u32(near) + 1u : as_u32(near) - 1u);
-}
 
 // XT: type of x and y, RT: of the residual and the stream.  THREADS hold V pieces of eight values each, THREADS * V * 8 >= cols.  A workgroup takes every
 // gridDim.x-th row and asks for the next one before it adds up the squares of this one (rows of up to 8192 values; longer ones leave no registers
@@ -182,8 +171,7 @@ template <int XT, int RT, int THREADS, int V, bool MX, bool WHOLE> __global__ __
             x.load(a.x + next * a.x_stride * XB, cols);
             if (a.residual) r.load(a.residual + next * a.residual_stride * RB, cols);
         }
-        double mean;
-        const float inverse = inverse_root<THREADS, V>(s, cols, a.eps, places, turn, mean);
+        const float inverse = inverse_root<THREADS, V>(s, cols, a.eps, places, turn);
         if (a.inverse && threadIdx.x == 0) a.inverse[row] = inverse;
 #pragma unroll
         for (int p = 0; p < V; ++p) {
@@ -194,8 +182,6 @@ template <int XT, int RT, int THREADS, int V, bool MX, bool WHOLE> __global__ __
             if constexpr (MX) {
                 const int blocks = (cols + kBlock - 1) / kBlock;
                 if (c >= blocks * kBlock) continue;    // quads stay together: blocks are sixteen lanes
-#pragma unroll
-                for (int k = 0; k < 8; ++k) y[k] = beside_borders(y[k], s[p][k], w[p][k], mean, a.eps);
                 Pair<DT_F32> q[4];
                 u32 m = 0;
 #pragma unroll

@@ -150,7 +150,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
 def rms_norm_mxfp4(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                    eps: float = 1e-6) -> Union[MXFP4Tensor, tuple[MXFP4Tensor, torch.Tensor]]:
     """:func:`rms_norm` of a matrix's rows with the output in MXFP4, as :func:`mxfp4_matmul` reads it: one launch in place of the norm and
-    the quantiser; the codes are those of the exact norm of the stream.  No gradient flows through.
+    the quantiser, the output quantised from fp32.  No gradient flows through.
     """
     if _autograd.rms_norm_mxfp4 is not None:
         got = _autograd.rms_norm_mxfp4(x, weight, residual, eps)

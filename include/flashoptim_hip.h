@@ -314,8 +314,8 @@ int fo_mxfp4_linear_backward(const void *dy, int dy_dtype, int64_t tokens, int64
  * Root-mean-square norm of the rows of s = x + residual (rounded to the residual's type and written to out_stream; s = x where
  * residual is NULL):  y = s / sqrt(mean(s^2) + eps) * weight.  x and y are of x_dtype, residual and out_stream of stream_dtype (x_dtype or
  * fp32), weight of any type or NULL (ones); y and out_stream are contiguous.  inverse (NULL, or `rows` fp32 numbers) gets
- * 1 / sqrt(mean(s^2) + eps), which the backward pass takes.  The second form writes y in MXFP4 as fo_mxfp4_quantize lays
- * it out, with the codes of the exact y.
+ * 1 / sqrt(mean(s^2) + eps), which the backward pass takes.  The second form writes y, in fp32 up to there, in MXFP4 as
+ * fo_mxfp4_quantize lays it out.
  */
 #define FO_RMS_NORM_MOST_COLS 16384
 int fo_rms_norm(const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t x_stride, const void *residual, int stream_dtype,
