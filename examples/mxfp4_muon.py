@@ -2,16 +2,18 @@
 
     python -m examples.mxfp4_muon [--steps 400] [--width 512] [--tokens 4096]
 
-The model predicts a token from the two before it: embeddings, residual blocks of two MXFP4 linear layers, an output layer.  The
+The model predicts a token from the two before it: embeddings, residual blocks of two MXFP4 linear layers behind a norm that takes the
+residual's addition along, an output matrix whose logits training never writes to memory.  The
 blocks' matrices are stepped by FlashMuon (8-bit momentum, orthogonalised updates), everything else by FlashAdamW; the text
 comes from a random second-order chain, so the best possible loss is known.  Afterwards the blocks' weights are kept in
-MXFP4 alone (17/32 bytes each) and sequences are continued one token at a time.
+MXFP4 alone (17/32 bytes each), the norms hand over MXFP4 too, and sequences are continued one token at a time.
 """
 
 from __future__ import annotations
 
 import argparse
 import time
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -26,27 +28,31 @@ CHOICES = 4       # tokens that may follow a pair
 class Block(nn.Module):
     def __init__(self, width: int):
         super().__init__()
-        self.norm = nn.LayerNorm(width)
+        self.norm = fo.FlashRMSNorm(width)
         self.up = fo.MXFP4Linear(width, 4 * width, bias=False)
         self.down = fo.MXFP4Linear(4 * width, width, bias=False)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return x + self.down(F.gelu(self.up(self.norm(x))))
+    def forward(self, branch: torch.Tensor, stream: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+        """What the block adds to the stream, and the stream with what the block before added."""
+        y, stream = (self.norm(branch), branch) if stream is None else self.norm(branch, stream)
+        return self.down(F.gelu(self.up(y))), stream
 
 
 class Model(nn.Module):
     def __init__(self, width: int, blocks: int):
         super().__init__()
-        self.embed = nn.Embedding(VOCABULARY, width // 2)
+        self.embed = fo.FlashEmbedding(VOCABULARY, width // 2)
         self.blocks = nn.ModuleList(Block(width) for _ in range(blocks))
-        self.norm = nn.LayerNorm(width)
-        self.head = nn.Linear(width, VOCABULARY)
+        self.norm = fo.FlashRMSNorm(width)
+        self.head = nn.Linear(width, VOCABULARY, bias=False)
 
-    def forward(self, pairs: torch.Tensor) -> torch.Tensor:
-        x = self.embed(pairs).flatten(1)
+    def forward(self, pairs: torch.Tensor, target: torch.Tensor) -> torch.Tensor:
+        """The loss."""
+        branch, stream = self.embed(pairs).flatten(1), None
         for block in self.blocks:
-            x = block(x)
-        return self.head(self.norm(x))
+            branch, stream = block(branch, stream)
+        y, _ = self.norm(branch, stream)
+        return fo.linear_cross_entropy(y, self.head.weight, target)
 
 
 class Served:
@@ -58,10 +64,14 @@ class Served:
 
     @torch.no_grad()
     def __call__(self, pairs: torch.Tensor) -> torch.Tensor:
-        x = self.model.embed(pairs).flatten(1)
+        """The next token's logits."""
+        branch, stream = self.model.embed(pairs).flatten(1), None
         for block, (up, down) in zip(self.model.blocks, self.weights):
-            x = x + fo.mxfp4_linear(F.gelu(fo.mxfp4_linear(block.norm(x), up)), down)
-        return self.model.head(self.model.norm(x))
+            q = fo.rms_norm_mxfp4(branch, block.norm.weight, stream, eps=block.norm.eps)
+            q, stream = (q, branch) if stream is None else q
+            branch = fo.mxfp4_linear(F.gelu(fo.mxfp4_matmul(q, up)), down)
+        y, _ = self.model.norm(branch, stream)
+        return self.model.head(y)
 
 
 class Chain:
@@ -91,7 +101,7 @@ def train(model: Model, chain: Chain, steps: int, tokens: int) -> list:
             opt.param_groups[0]["lr"] = opt.defaults["lr"] * (1.0 - step / steps)
             opt.zero_grad()
         pairs, target = chain.draw(tokens)
-        loss = F.cross_entropy(model(pairs).float(), target)
+        loss = model(pairs, target)
         loss.backward()
         for opt in optimizers:
             opt.step()
