@@ -115,9 +115,9 @@ SIGNATURES = {
     "fo_embedding": (_i32, [_vp, _i32, _i64, _vp, _i32] + [_i64] * 3 + [_f32, _vp, _vp]),
     "fo_embedding_backward_workspace": (_i64, [_i64] * 3),
     "fo_embedding_backward": (_i32, [_vp, _i32, _i64, _vp, _i32] + [_i64] * 3 + [_f32, _i64, _vp, _vp, _i64, _vp]),
-    "fo_linear_cross_entropy_workspace": (_i64, [_i32] + [_i64] * 3),
+    "fo_linear_cross_entropy_workspace": (_i64, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _f32]),
     "fo_linear_cross_entropy": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _i64, _i32, _f32, _vp, _vp, _vp, _i64, _vp]),
-    "fo_linear_cross_entropy_backward_workspace": (_i64, [_i32] + [_i64] * 3 + [_i32, _i32]),
+    "fo_linear_cross_entropy_backward_workspace": (_i64, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _i32]),
     "fo_linear_cross_entropy_backward": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _f32, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp]),
     "fo_muon_step": (_i32, [_vp, _vp, _i64, _i32, _i32, _i32, _f32, _f32, _i32, _i32, _vp, _f32, _vp, _i64, _vp]),
 }

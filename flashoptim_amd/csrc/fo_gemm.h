@@ -142,8 +142,8 @@ struct Bf16Product {
 };
 
 // fp32 values on the matrix cores' fp32 instructions, a sixteenth of the 16-bit rate: a lane's 16 bytes are one value for each of four instructions.  An instruction adds four
-// products, so sums of thousands are as many roundings as would show: every four stages (128 values) they are added to a second set, in vector registers, and begin
-// anew (one token's loss over 2195 values: off by 9e-6 of itself without, TODO with; 5 % of the time of 64 x 64 tiles).
+// products, so a sum of thousands is rounded often enough to show (one token's loss over 2195 values was off by 9e-6 of itself, by 1e-6 in sums of another order): every
+// four stages (128 values) the sums are added to a second set, in vector registers, and begin anew.  That is 5 % of the time (512 x 1000 over 5003: 220 -> 230 us).
 struct F32Product {
     static constexpr bool kScaled = false, kParts = false;
     static constexpr int kBytes = 4;

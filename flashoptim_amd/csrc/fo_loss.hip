@@ -98,7 +98,7 @@ struct FormArgs {
     int rows, cols;           // of x
     int out_rows, length;     // of out: filled up with zeros
 };
-// Rows as operand rows, eight values a thread.  Bound by memory: 8192 x 4096 bf16 in TODO us.
+// Rows as operand rows, eight values a thread.  Bound by memory: 8192 x 4096 bf16 in 22 us (6.0 TB/s).
 template <int DT, class Product> __global__ __launch_bounds__(256) void form_kernel(FormArgs a) {
     typedef OperandOf<DT, Product> To;
     const int pieces = a.length / 8;
@@ -157,6 +157,9 @@ template <class Tile> __device__ __forceinline__ bool my_tile(int rows, int cols
     return true;
 }
 
+// A tile of z, then out of the accumulators each row's maximum and sum over a wavefront's WT columns: a lane has four rows of every sixteen and every sixteenth column, so both
+// are a few operations in registers and four exchanges between sixteen neighbouring lanes.  Bound by the matrix cores: 8192 x 4096 over 128256 in 6.6 ms, 1300 TFLOP/s (a library
+// product of that size, which writes its result, 6.0); 17 of a tile's 105 us are its first loads and this.  With few rows bound by the weight's bytes: 5 rows 171 us, 6.1 TB/s.
 template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void logits_kernel(LogitsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmTile<Product, WT, STAGES> Tile;
@@ -358,6 +361,7 @@ template <int DT, class Product> struct GradOut {
         if (a.lost && at >= 0 && at < 8) a.lost[i] = lost;
     }
 };
+// The logits again and G of them.  8192 rows, 16128 tokens of a vocabulary: 890 us (1210 TFLOP/s), 50 more than the product alone.
 template <int DT, class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void grad_kernel(GradArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmTile<Product, WT, STAGES> Tile;
@@ -428,7 +432,8 @@ struct GradProductOut {
         else store_values<DT_F32>(v, a.sums + part * a.rows * a.stride + i * a.stride + j, a.cols - j);
     }
 };
-// TURNED: the left operand comes by columns too (dW = G' x).
+// TURNED: the left operand comes by columns too (dW = G' x).  Bound by the matrix cores: dx of 8192 x 4096 over 16128 in 809 us (1340 TFLOP/s), dW the same sizes in 824.  With operands
+// turned by launches of their own instead of by their reads (64 us a piece, and G written twice) the loss of 1003 x 1000 over 32003 took 496 us, so 398.
 template <class Product, bool TURNED, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void grad_product_kernel(GradProductArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmTile<Product, WT, STAGES, TURNED, true> Tile;
@@ -542,7 +547,8 @@ fo::TileCost tile_for(const Mode& mode, int64_t rows, int64_t cols, double inner
 }
 
 // fp32 in parts where that takes less: the logits in six times the length with what laying out both operands moves (10 bytes a value, at 4 TB/s) against fp32
-// instructions.  TODO
+// instructions.  With gradients 512 x 1000 over 5003 takes 240 us whole and 302 in parts, 64 x 1024 over 32768 223 and 438, 1024 x 1024 over 8192 599 and 521, 8192 x 4096 over 16000
+// 31.3 and 22.8 ms.
 Mode mode_of(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int cus) {
     if (dtype != FO_F32) return {dtype, false};
     const Mode whole{dtype, false}, parts{dtype, true};
@@ -554,7 +560,7 @@ Mode mode_of(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int cu
 }
 
 // A product of few tiles over a long contraction is cut along it: parts of whole stages, their fp32 results joined by another launch.  1003 x 1000 over
-// 32003 values: 157 us in 64 x 64 tiles, TODO in parts.
+// 32003 values: 157 us in 64 x 64 tiles, 86 + 6 in parts (the loss with gradients 433 and 366); 64 x 4096 over 128256 1885 and 1367.
 struct Cut { fo::TileCost tile; int parts; int64_t part; double time; };
 constexpr int kMostParts = 32;
 constexpr int64_t kLeastPartValues = 512;
@@ -696,19 +702,23 @@ int check_common(const char* what, const void* x, const void* weight, int reduct
     return 0;
 }
 
-// ---- what a call keeps in its workspace.  Matrices that are operands in place leave their space unused.
-constexpr int kLeastPart = 32;    // columns of the smallest tile's wavefront
+// ---- what a call keeps in its workspace
 struct ForwardSpace {
+    fo::TileCost tile;    // of a full block of tokens
+    int64_t rows, parts;
     int64_t picked, losses, stats, sums, x, weight, total;
-    ForwardSpace(const Mode& mode, int64_t tokens, int64_t cols, int64_t vocabulary) {
-        const int64_t rows = tokens < kBlockTokens ? tokens : kBlockTokens, parts = (vocabulary + kLeastPart - 1) / kLeastPart;
+    ForwardSpace(const Mode& mode, const Matrix& of_x, const Matrix& of_weight, bool smooth, int cus) {
+        const int64_t tokens = of_x.rows, length = mode.length(of_x.cols);
+        rows = tokens < kBlockTokens ? tokens : kBlockTokens;
+        tile = tile_for(mode, rows, of_weight.rows, (double)(length * mode.segments()), cus);
+        parts = (of_weight.rows + tile.wt - 1) / tile.wt;
         picked = 0;
         losses = picked + aligned(rows * 4);
         stats = losses + aligned(tokens * 4);
         sums = stats + aligned(rows * parts * 8);
-        x = sums + aligned(rows * parts * 4);
-        weight = x + mode.form(rows, cols);
-        total = weight + mode.form(vocabulary, cols);
+        x = sums + (smooth ? aligned(rows * parts * 4) : 0);
+        weight = x + (of_x.ready(mode) && of_x.cols == length ? 0 : mode.form(rows, of_x.cols));
+        total = weight + (of_weight.ready(mode) ? 0 : mode.form(of_weight.rows, of_weight.cols));
     }
 };
 
@@ -716,7 +726,10 @@ struct BackwardSpace {
     int64_t piece;    // tokens of the vocabulary at a time
     int64_t factors, lost, scale, x, weight, grad, sums, partial, total;
     Cut dx_cut, dw_cut;
-    BackwardSpace(const Mode& mode, int64_t tokens, int64_t cols, int64_t vocabulary, bool dx, bool dw, int cus) {
+    // dW reads x with the rows of ignored targets left out; and the logits, where nothing fills up the rows, filled up
+    static bool copies(const Mode& mode, const Matrix& of_x, bool dw) { return dw || of_x.cols != mode.length(of_x.cols) || !of_x.ready(mode); }
+    BackwardSpace(const Mode& mode, const Matrix& of_x, const Matrix& of_weight, bool dx, bool dw, int cus) {
+        const int64_t tokens = of_x.rows, cols = of_x.cols, vocabulary = of_weight.rows;
         const int64_t most = round_up(kPieceValues * 2 / (mode.parts() * mode.bytes()) / tokens + 1, 256);
         const int64_t pieces = (vocabulary + most - 1) / most;
         piece = round_up((vocabulary + pieces - 1) / pieces, 256);
@@ -728,8 +741,8 @@ struct BackwardSpace {
         lost = factors + aligned(tokens * 4);
         scale = lost + aligned(tokens * 4);
         x = scale + 256;
-        weight = x + mode.form(mode.length(tokens), cols);
-        grad = weight + mode.form(piece, cols);
+        weight = x + (copies(mode, of_x, dw) ? mode.form(mode.length(tokens), cols) : 0);
+        grad = weight + (of_weight.ready(mode) ? 0 : mode.form(piece, cols));
         sums = grad + mode.form(tokens, piece);
         partial = sums + (dx && piece < vocabulary ? aligned(tokens * cols * 4) : 0);
         const int64_t of_dx = dx_cut.parts > 1 ? dx_cut.parts * tokens * cols : 0, of_dw = dw_cut.parts > 1 ? dw_cut.parts * piece * cols : 0;
@@ -746,12 +759,12 @@ struct Forward {
     float smoothing;
     float *loss, *kept;
     char* base;
+    const ForwardSpace& at;
     int cus;
     hipStream_t s;
 
     template <int DT, class Product> int run() const {
         const char* what = "fo_linear_cross_entropy";
-        const ForwardSpace at(mode, x.rows, x.cols, weight.rows);
         int* labels = (int*)(kept + x.rows + 1);
         const fo::Targets t{targets, index_bytes};
         float* losses = reduction == FO_REDUCE_NONE ? loss : (float*)(base + at.losses);
@@ -763,7 +776,9 @@ struct Forward {
             const Matrix some = x.part(first, x.rows - first < kBlockTokens ? x.rows - first : kBlockTokens);
             fo::Operand rows;
             if (int rc = operand_of(mode, some, x.cols != length, nullptr, some.rows, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
-            const fo::TileCost tile = tile_for(mode, some.rows, weight.rows, (double)inner, cus);
+            // a last block is shorter, and its tiles may be smaller only where its parts need no more space
+            fo::TileCost tile = tile_for(mode, some.rows, weight.rows, (double)inner, cus);
+            if (some.rows * ((weight.rows + tile.wt - 1) / tile.wt) > at.rows * at.parts) tile = at.tile;
             const fo::LogitsArgs a{rows, w, row_bytes, segment, t, first, (fo::f32x2*)(base + at.stats), smoothing > 0.0f ? (float*)(base + at.sums) : nullptr, (float*)(base + at.picked)};
             if (int rc = launch_tiles<LogitsLaunch<Product>>(tile, a, s, what)) return rc;
             const fo::JoinArgs join{a.stats, a.sums, a.picked, t, first, ignore, weight.rows, kept + first, losses + first, labels + first, (int)some.rows,
@@ -810,7 +825,7 @@ struct Backward {
         }
         const int64_t tokens_length = mode.length(x.rows), cols_length = mode.length(x.cols), cols_inner = cols_length * mode.segments();
         fo::Operand rows;
-        if (int rc = operand_of(mode, x, dw != nullptr || x.cols != cols_length, labels, tokens_length, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
+        if (int rc = operand_of(mode, x, BackwardSpace::copies(mode, x, dw != nullptr), labels, tokens_length, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
         fo::Operand x_turned = turned(rows, cols_length, tokens_length);
         x_turned.order = fo::kRightOrder;
         for (int64_t first = 0; first < weight.rows; first += at.piece) {
@@ -866,9 +881,12 @@ struct Backward {
 
 extern "C" {
 
-int64_t fo_linear_cross_entropy_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
+int64_t fo_linear_cross_entropy_workspace(const void* x, int dtype, int64_t tokens, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t vocabulary, int64_t cols,
+                                          float smoothing) {
     if (int rc = validate("fo_linear_cross_entropy", dtype, tokens, cols, vocabulary)) return rc;
-    return ForwardSpace(mode_of(dtype, tokens, cols, vocabulary, units()), tokens, cols, vocabulary).total;
+    const int cus = units();
+    return ForwardSpace(mode_of(dtype, tokens, cols, vocabulary, cus), {(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype},
+                        smoothing > 0.0f, cus).total;
 }
 
 int fo_linear_cross_entropy(const void* x, int dtype, int64_t tokens, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t vocabulary, int64_t cols,
@@ -881,16 +899,19 @@ int fo_linear_cross_entropy(const void* x, int dtype, int64_t tokens, int64_t x_
     if (index_bytes != 4 && index_bytes != 8) return fail(FO_ERR_INVALID_ARGUMENT, "%s: targets of %d bytes", what, index_bytes);
     const int cus = units();
     const Mode mode = mode_of(dtype, tokens, cols, vocabulary, cus);
-    if (workspace_bytes < ForwardSpace(mode, tokens, cols, vocabulary).total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
-    const Forward f{mode, {(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, targets, index_bytes, reduction,
-                    ignore, smoothing, loss, kept, (char*)workspace, cus, (hipStream_t)stream};
+    const Matrix of_x{(const char*)x, x_stride, tokens, cols, dtype}, of_weight{(const char*)weight, weight_stride, vocabulary, cols, dtype};
+    const ForwardSpace at(mode, of_x, of_weight, smoothing > 0.0f, cus);
+    if (workspace_bytes < at.total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
+    const Forward f{mode, of_x, of_weight, targets, index_bytes, reduction, ignore, smoothing, loss, kept, (char*)workspace, at, cus, (hipStream_t)stream};
     return by_product(mode, f);
 }
 
-int64_t fo_linear_cross_entropy_backward_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int want_dx, int want_dw) {
+int64_t fo_linear_cross_entropy_backward_workspace(const void* x, int dtype, int64_t tokens, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t vocabulary,
+                                                   int64_t cols, int want_dx, int want_dw) {
     if (int rc = validate("fo_linear_cross_entropy_backward", dtype, tokens, cols, vocabulary)) return rc;
     const int cus = units();
-    return BackwardSpace(mode_of(dtype, tokens, cols, vocabulary, cus), tokens, cols, vocabulary, want_dx != 0, want_dw != 0, cus).total;
+    return BackwardSpace(mode_of(dtype, tokens, cols, vocabulary, cus), {(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype},
+                         want_dx != 0, want_dw != 0, cus).total;
 }
 
 int fo_linear_cross_entropy_backward(const void* x, int dtype, int64_t tokens, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t vocabulary,
@@ -902,10 +923,10 @@ int fo_linear_cross_entropy_backward(const void* x, int dtype, int64_t tokens, i
     if (!kept || !upstream || (!dx && !dw)) return fail(FO_ERR_INVALID_ARGUMENT, "%s: kept, upstream and a result must be given", what);
     const int cus = units();
     const Mode mode = mode_of(dtype, tokens, cols, vocabulary, cus);
-    const BackwardSpace at(mode, tokens, cols, vocabulary, dx != nullptr, dw != nullptr, cus);
+    const Matrix of_x{(const char*)x, x_stride, tokens, cols, dtype}, of_weight{(const char*)weight, weight_stride, vocabulary, cols, dtype};
+    const BackwardSpace at(mode, of_x, of_weight, dx != nullptr, dw != nullptr, cus);
     if (workspace_bytes < at.total) return fail(FO_ERR_INVALID_ARGUMENT, "%s: workspace too small", what);
-    const Backward b{mode, {(const char*)x, x_stride, tokens, cols, dtype}, {(const char*)weight, weight_stride, vocabulary, cols, dtype}, reduction, smoothing, kept, upstream,
-                     upstream_stride, (char*)dx, (char*)dw, (char*)workspace, at, cus, (hipStream_t)stream};
+    const Backward b{mode, of_x, of_weight, reduction, smoothing, kept, upstream, upstream_stride, (char*)dx, (char*)dw, (char*)workspace, at, cus, (hipStream_t)stream};
     return by_product(mode, b);
 }
 

@@ -335,7 +335,8 @@ struct LossNode : Node {
             const int64_t width = x.size(-1), tokens = leading(x), vocabulary = weight.size(0);
             Tensor upstream = grads[0].is_neg() ? grads[0].resolve_neg() : grads[0];
             if (upstream.dim() > 1) upstream = upstream.reshape({tokens});
-            const int64_t size = api.fo_linear_cross_entropy_backward_workspace(code_of(x), tokens, width, vocabulary, need_dx, need_dw);
+            const int64_t size = api.fo_linear_cross_entropy_backward_workspace(x.data_ptr(), code_of(x), tokens, row_stride(x), weight.data_ptr(), weight.stride(0), vocabulary,
+                                                                                width, need_dx, need_dw);
             check_size(size, "fo_linear_cross_entropy_backward");
             const Tensor workspace = bytes(size, x);
             if (need_dx) out[0] = at::empty(x.sizes(), x.options());
@@ -370,7 +371,8 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
             const auto numbers = x->options().dtype(at::kFloat);
             loss = reduction == FO_REDUCE_NONE ? at::empty(target->sizes(), numbers) : at::empty({}, numbers);
             kept = at::empty({2 * tokens + 1}, numbers);
-            const int64_t size = api.fo_linear_cross_entropy_workspace(code_of(*x), tokens, width, vocabulary);
+            const int64_t size = api.fo_linear_cross_entropy_workspace(x->data_ptr(), code_of(*x), tokens, row_stride(*x), weight->data_ptr(), weight->stride(0), vocabulary, width,
+                                                                       (float)smoothing);
             check_size(size, "fo_linear_cross_entropy");
             const Tensor workspace = bytes(size, *x);
             check(api.fo_linear_cross_entropy(x->data_ptr(), code_of(*x), tokens, row_stride(*x), weight->data_ptr(), weight->stride(0), vocabulary, width, target->data_ptr(),

@@ -23,7 +23,8 @@ def _forward(x, weight, target, how):
     loss = torch.empty(tokens if reduction == 0 else (), dtype=torch.float32, device=device)
     kept = torch.empty(2 * tokens + 1, dtype=torch.float32, device=device)
     with _native.device_guard(device):
-        size = lib.fo_linear_cross_entropy_workspace(DTYPE_CODE[x.dtype], tokens, width, vocabulary)
+        size = lib.fo_linear_cross_entropy_workspace(x.data_ptr(), DTYPE_CODE[x.dtype], tokens, x.stride(0), weight.data_ptr(), weight.stride(0), vocabulary, width,
+                                                     smoothing)
         if size < 0:
             _native.check(size, "fo_linear_cross_entropy")
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
@@ -58,7 +59,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         dx = torch.empty((tokens, width), dtype=x.dtype, device=device) if need_dx else None
         dw = torch.empty((vocabulary, width), dtype=x.dtype, device=device) if need_dw else None
         with _native.device_guard(device):
-            size = lib.fo_linear_cross_entropy_backward_workspace(DTYPE_CODE[x.dtype], tokens, width, vocabulary, need_dx, need_dw)
+            size = lib.fo_linear_cross_entropy_backward_workspace(x.data_ptr(), DTYPE_CODE[x.dtype], tokens, x.stride(0), weight.data_ptr(), weight.stride(0),
+                                                                  vocabulary, width, need_dx, need_dw)
             if size < 0:
                 _native.check(size, "fo_linear_cross_entropy_backward")
             workspace = torch.empty(size, dtype=torch.uint8, device=device)

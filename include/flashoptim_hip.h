@@ -357,14 +357,17 @@ int fo_embedding_backward(const void *tokens, int index_bytes, int64_t n_tokens,
  *   kept: 2 * tokens + 1 fp32 numbers that the backward pass takes: log sum exp of each row, that number, and the rows' targets as int32 (-1: ignored,
  *   -2: none of the vocabulary)
  * Backward: upstream: the loss's gradient, fp32, upstream_stride elements apart (0: one for all); dx (tokens x cols) and dw (vocabulary
- * x cols) of `dtype`, contiguous, either may be NULL.  workspace: device memory, aligned to 256.
+ * x cols) of `dtype`, contiguous, either may be NULL.  workspace: device memory, aligned to 256; its size goes by the operands' addresses and
+ * strides too (what the matrix cores cannot read in place is laid out there).
  */
 enum fo_reduction { FO_REDUCE_NONE = 0, FO_REDUCE_SUM = 1, FO_REDUCE_MEAN = 2 };
-int64_t fo_linear_cross_entropy_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary);
+int64_t fo_linear_cross_entropy_workspace(const void *x, int dtype, int64_t tokens, int64_t x_stride, const void *weight, int64_t weight_stride,
+                                          int64_t vocabulary, int64_t cols, float smoothing);
 int fo_linear_cross_entropy(const void *x, int dtype, int64_t tokens, int64_t x_stride, const void *weight, int64_t weight_stride,
                             int64_t vocabulary, int64_t cols, const void *targets, int index_bytes, int64_t ignore, int reduction,
                             float smoothing, float *loss, float *kept, void *workspace, int64_t workspace_bytes, void *stream);
-int64_t fo_linear_cross_entropy_backward_workspace(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int want_dx, int want_dw);
+int64_t fo_linear_cross_entropy_backward_workspace(const void *x, int dtype, int64_t tokens, int64_t x_stride, const void *weight,
+                                                   int64_t weight_stride, int64_t vocabulary, int64_t cols, int want_dx, int want_dw);
 int fo_linear_cross_entropy_backward(const void *x, int dtype, int64_t tokens, int64_t x_stride, const void *weight, int64_t weight_stride,
                                      int64_t vocabulary, int64_t cols, int reduction, float smoothing, const float *kept,
                                      const float *upstream, int64_t upstream_stride, void *dx, void *dw, void *workspace,

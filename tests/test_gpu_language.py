@@ -210,10 +210,10 @@ def test_rows_behind_the_results_are_left_alone():
     buffers = {n: torch.full((size + 512,), 77.0, device=DEV) for n, size in dict(y=120, loss=5, kept=11, dx=120, dw=264, rows=120, table=264).items()}
     at = {n: b.data_ptr() + 1024 for n, b in buffers.items()}
     assert lib.fo_rms_norm(x.data_ptr(), 0, 5, 24, 24, None, 0, 0, None, 0, 1e-6, None, at["y"], None, s) == 0
-    size = lib.fo_linear_cross_entropy_workspace(0, 5, 24, 11)
+    size = lib.fo_linear_cross_entropy_workspace(x.data_ptr(), 0, 5, 24, w.data_ptr(), 24, 11, 24, 0.0)
     space = torch.empty(size, dtype=torch.uint8, device=DEV)
     assert lib.fo_linear_cross_entropy(x.data_ptr(), 0, 5, 24, w.data_ptr(), 24, 11, 24, target.data_ptr(), 8, -100, 0, 0.0, at["loss"], at["kept"], space.data_ptr(), size, s) == 0
-    size = lib.fo_linear_cross_entropy_backward_workspace(0, 5, 24, 11, 1, 1)
+    size = lib.fo_linear_cross_entropy_backward_workspace(x.data_ptr(), 0, 5, 24, w.data_ptr(), 24, 11, 24, 1, 1)
     back, ones = torch.empty(size, dtype=torch.uint8, device=DEV), torch.ones(5, device=DEV)
     assert lib.fo_linear_cross_entropy_backward(x.data_ptr(), 0, 5, 24, w.data_ptr(), 24, 11, 24, 0, 0.0, at["kept"], ones.data_ptr(), 1, at["dx"], at["dw"], back.data_ptr(), size, s) == 0
     assert lib.fo_embedding(target.data_ptr(), 8, 5, w.data_ptr(), 0, 11, 24, 24, 1.0, at["rows"], s) == 0

@@ -84,12 +84,24 @@ def test_loss_checks_its_arguments():
     assert call(loss=None) == INVALID and call(targets=None) == INVALID and call(index=1) == INVALID and back(upstream=None) == INVALID and back(dx=None) == INVALID
     for other in (dict(tokens=0), dict(cols=0), dict(vocabulary=0), dict(tokens=(1 << 20) + 1), dict(cols=65537), dict(vocabulary=(1 << 24) + 1)):
         assert call(**other) == UNSUPPORTED and back(**other) == UNSUPPORTED, other
-    forward, backward = lib.fo_linear_cross_entropy_workspace, lib.fo_linear_cross_entropy_backward_workspace
-    assert forward(1, -1, 5, 7) == INVALID and forward(1, 0, 5, 7) == UNSUPPORTED and backward(5, 3, 5, 7, 1, 1) == INVALID
-    # a piece's gradient, 2^27 values, not the logits
+
+    def forward(dtype, tokens, cols, vocabulary, smoothing=0.0, x=SOME, x_stride=None, weight=SOME, weight_stride=None):
+        return lib.fo_linear_cross_entropy_workspace(x, dtype, tokens, x_stride or cols, weight, weight_stride or cols, vocabulary, cols, smoothing)
+
+    def backward(dtype, tokens, cols, vocabulary, dx=1, dw=1, weight=SOME):
+        return lib.fo_linear_cross_entropy_backward_workspace(SOME, dtype, tokens, cols, weight, cols, vocabulary, cols, dx, dw)
+
+    assert forward(1, -1, 5, 7) == INVALID and forward(1, 0, 5, 7) == UNSUPPORTED and backward(5, 3, 5, 7) == INVALID
+    # some bytes a row of a tile's part forward, a piece's gradient of 2^27 values, x and sums between pieces backward: not the logits, and not the weight
     logits = 8192 * 128256 * 2
-    assert backward(1, 8192, 4096, 128256, 1, 1) < logits // 2 and forward(1, 8192, 4096, 128256) < 2 * logits
-    assert backward(1, 8192, 4096, 128256, 1, 0) > backward(1, 8192, 4096, 128256, 0, 1)    # the sums between pieces
+    assert forward(1, 8192, 4096, 128256) < logits // 20 and backward(1, 8192, 4096, 128256) < logits // 4
+    assert backward(1, 8192, 4096, 128256, 1, 0) > backward(1, 8192, 4096, 128256, 0, 1)    # the sums
+    assert forward(1, 8192, 4096, 128256, smoothing=0.1) > forward(1, 8192, 4096, 128256)
+    # what cannot be read in place is laid out
+    weight = 128256 * 4096 * 2
+    for other in (dict(weight=SOME + 2), dict(weight_stride=4097)):
+        assert forward(1, 8192, 4096, 128256, **other) >= forward(1, 8192, 4096, 128256) + weight, other
+    assert forward(1, 8192, 4096, 128256, x=SOME + 2) >= forward(1, 8192, 4096, 128256) + 8192 * 4096 * 2
 
 
 def test_without_a_gpu():
