@@ -1,7 +1,7 @@
 """Loader of the optional C++ calls and autograd nodes (flashoptim_amd/hostscan/fo_autograd.cpp).
 
 Its functions (``rms_norm``, ``rms_norm_mxfp4``, ``embedding``, ``linear_cross_entropy``) are None when the module has not been built (``make -C
-flashoptim_amd/hostscan``) or was built against another torch; they give None for operands out of the ordinary, and until the HIP
+flashoptim_amd/hostscan``) or was built against another torch or another C interface; they give None for operands out of the ordinary, and until the HIP
 library has been loaded.  The Python functions around them (norm.py, embed.py, loss.py) then do the same host work themselves, to the same bits.
 ``FLASHOPTIM_NO_HOSTSCAN=1`` keeps the Python path.
 """
@@ -23,6 +23,13 @@ _PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_fo_aut
 _module = None
 
 
+def _called() -> dict:
+    """The C entry points that the module calls, with the types that the binding passes, in the module's letters."""
+    letters = {ctypes.c_void_p: "P", ctypes.c_char_p: "P", ctypes.c_float: "f", ctypes.c_double: "d", ctypes.c_int32: "i", ctypes.c_int64: "q"}
+    names = [n for n in _native.SIGNATURES if n == "fo_last_error" or n.startswith(("fo_rms_norm", "fo_embedding", "fo_linear_cross_entropy"))]
+    return {n: "".join(letters[t] for t in (_native.SIGNATURES[n][0], *_native.SIGNATURES[n][1])) for n in names}
+
+
 def _load() -> None:
     global _module, rms_norm, rms_norm_mxfp4, embedding, linear_cross_entropy
     if os.environ.get("FLASHOPTIM_NO_HOSTSCAN", "").strip() not in ("", "0") or not os.path.exists(_PATH):
@@ -32,6 +39,8 @@ def _load() -> None:
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
     except (ImportError, OSError):  # built against another torch or python
+        return
+    if getattr(module, "kinds", None) != _called():  # left over from another version of the library
         return
     _module = module
     rms_norm, rms_norm_mxfp4 = module.rms_norm, module.rms_norm_mxfp4
@@ -48,8 +57,7 @@ def bind() -> None:
     if _module is None:
         return
     lib = _native.lib()
-    names = [n for n in _native.SIGNATURES if n == "fo_last_error" or n.startswith(("fo_rms_norm", "fo_embedding", "fo_linear_cross_entropy"))]
-    _module.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names})
+    _module.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _called()})
     _module = None  # once
 
 

@@ -7,6 +7,7 @@
 // (flashoptim_amd/norm.py, embed.py, loss.py), and for every call that is out of the ordinary: a function here gives None, and has done nothing, for
 // operands that are not plain strided tensors of this device with adjacent values; the Python path checks, converts and raises.
 //
+// kinds                                                dict from the name of a C entry point to the types it was built to call it with
 // bind(addresses)                                      dict from the name of a C entry point to its address
 // rms_norm(x, weight, residual, eps)                   None | y | (y, stream)
 // rms_norm_mxfp4(x, weight, residual, eps)             None | (codes, scales) | (codes, scales, stream)
@@ -25,6 +26,8 @@
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <cmath>
+#include <string>
+#include <type_traits>
 
 #include "../../include/flashoptim_hip.h"
 
@@ -395,6 +398,28 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// The result's and the arguments' types, a letter each, as the struct module names them; P: a pointer.
+template <class T> constexpr char kind_of() {
+    if (std::is_pointer<T>::value) return 'P';
+    if (std::is_same<T, float>::value) return 'f';
+    if (std::is_same<T, double>::value) return 'd';
+    return std::is_integral<T>::value && sizeof(T) == 8 ? 'q' : std::is_integral<T>::value && sizeof(T) == 4 ? 'i' : '?';
+}
+template <class R, class... A> std::string kinds_of(R (*)(A...)) { return {kind_of<R>(), kind_of<A>()...}; }
+
+PyObject* all_kinds() {
+    PyObject* kinds = PyDict_New();
+#define FO_KINDS(name)                                                                              \
+    {                                                                                               \
+        PyObject* o = kinds ? PyUnicode_FromString(kinds_of(api.name).c_str()) : nullptr;           \
+        if (!o || PyDict_SetItemString(kinds, #name, o) < 0) Py_CLEAR(kinds);                       \
+        Py_XDECREF(o);                                                                              \
+    }
+    FO_ENTRIES(FO_KINDS)
+#undef FO_KINDS
+    return kinds;
+}
+
 PyObject* bind(PyObject*, PyObject* addresses) {
     if (!PyDict_Check(addresses)) return PyErr_Format(PyExc_TypeError, "bind takes a dict");
 #define FO_BIND(name)                                                                                         \
@@ -425,4 +450,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fo_autograd", "calls and autograd
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fo_autograd(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__fo_autograd(void) {
+    PyObject *m = PyModule_Create(&module), *kinds = m ? all_kinds() : nullptr;
+    if (kinds && PyModule_AddObject(m, "kinds", kinds) == 0) return m;
+    Py_XDECREF(kinds);
+    Py_XDECREF(m);
+    return nullptr;
+}

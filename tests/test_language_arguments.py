@@ -1,10 +1,12 @@
 """What the embedding, the norm and the loss refuse before any device work, through their C entry points and through Python."""
 
+import os
+
 import pytest
 import torch
 
 import flashoptim_amd as fo
-from flashoptim_amd import _native
+from flashoptim_amd import _autograd, _native
 
 INVALID, UNSUPPORTED = -1, -2
 SOME = 1 << 20    # an address that no call here gets to use
@@ -111,3 +113,18 @@ def test_without_a_gpu():
                  lambda: fo.FlashEmbedding(4, 8)(torch.zeros(2, dtype=torch.int64))):
         with pytest.raises(NotImplementedError):
             call()
+
+
+@pytest.mark.skipif(not os.path.exists(_autograd.library_path()), reason="the C++ calls are not built")
+def test_calls_built_for_another_interface_are_left_out(monkeypatch):
+    names = ("rms_norm", "rms_norm_mxfp4", "embedding", "linear_cross_entropy")
+    for name in (*names, "_module"):
+        monkeypatch.setattr(_autograd, name, None)
+    monkeypatch.delenv("FLASHOPTIM_NO_HOSTSCAN", raising=False)
+    result, arguments = _native.SIGNATURES["fo_embedding"]
+    with monkeypatch.context() as other:
+        other.setitem(_native.SIGNATURES, "fo_embedding", (result, arguments[:-1]))
+        _autograd._load()
+        assert all(getattr(_autograd, name) is None for name in names) and _autograd._module is None
+    _autograd._load()
+    assert all(getattr(_autograd, name) is not None for name in names)
