@@ -294,9 +294,11 @@ struct Scale {
     const float* p;         // the upstream, or what loss_factors_kernel made of many
     const float* count;     // or null
     float over;             // `top`
+    bool mean;
     __device__ __forceinline__ float value() const {
         if (!count) return p[0] * over;
-        return count[0] > 0.0f ? p[0] * (1.0f / count[0]) * over : 0.0f;    // no targets, no gradients
+        if (count[0] == 0.0f) return 0.0f;    // no targets, no gradients
+        return mean ? p[0] * (1.0f / count[0]) * over : p[0] * over;
     }
 };
 
@@ -384,7 +386,7 @@ struct GradProductArgs {
     char* out;             // the last one, of type `dtype`, times the scale
     Scale scale;
     const float* lost;     // dx: what the rows' targets lost, times their rows of the weight, is added before that; or null
-    const int* labels;
+    const int* labels;     // dx: of its rows; or null
     const char* weight;
     int64_t weight_stride;
     int64_t stride;
@@ -403,8 +405,10 @@ __device__ __forceinline__ void store_result(float (&v)[8], const GradProductArg
             for (int k = 0; k < 8; ++k) v[k] = fmaf(lost, w[k], v[k]);
         }
     }
+    // rows of ignored targets are zeros up to here, and stay so
+    const bool none = a.labels && !(fabsf(scale) < __builtin_inff()) && a.labels[i] == kIgnored;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= scale;
+    for (int k = 0; k < 8; ++k) v[k] = none ? v[k] : v[k] * scale;
     const int64_t at = i * a.stride + j;
     if (a.dtype == DT_BF16) store_values<DT_BF16>(v, a.out + at * 2, valid);
     else if (a.dtype == DT_F16) store_values<DT_F16>(v, a.out + at * 2, valid);
@@ -815,13 +819,13 @@ struct Backward {
         // read of W beside every piece of the result (20 us of 59 for 4096 x 4096 over 1024).
         float* lost = x.dtype != FO_F32 && dx && x.rows <= kFewRows ? (float*)(base + at.lost) : nullptr;
         const float top = x.dtype == FO_F16 ? 32768.0f : 1.0f;
-        fo::Scale scale{upstream, reduction == FO_REDUCE_MEAN ? kept + x.rows : nullptr, 1.0f / top};
+        fo::Scale scale{upstream, reduction != FO_REDUCE_NONE ? kept + x.rows : nullptr, 1.0f / top, reduction == FO_REDUCE_MEAN};
         if (upstream_stride != 0 && x.rows > 1) {
             factors = (float*)(base + at.factors);
             float* most = (float*)(base + at.scale);
             fo::loss_factors_kernel<<<dim3(1), dim3(1024), 0, s>>>(upstream, upstream_stride, labels, x.rows, reduction, kept + x.rows, top, factors, most);
             if (int rc = check_hip(hipGetLastError(), what)) return rc;
-            scale = {most, nullptr, 1.0f / top};
+            scale = {most, nullptr, 1.0f / top, false};
         }
         const int64_t tokens_length = mode.length(x.rows), cols_length = mode.length(x.cols), cols_inner = cols_length * mode.segments();
         fo::Operand rows;
@@ -866,6 +870,7 @@ struct Backward {
                 p.rows = (int)n;
                 p.row_bytes = (int)(tokens_length * mode.segments() * mode.bytes());
                 p.segment_stages = mode.stages(tokens_length);
+                p.labels = nullptr;
                 p.more = nullptr;
                 p.sums = nullptr;
                 p.out = dw + first * x.cols * x.width();

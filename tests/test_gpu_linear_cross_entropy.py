@@ -198,6 +198,21 @@ def test_what_stands_in_ignored_rows_does_not_matter():
         assert not got[1][rows].any()
 
 
+@pytest.mark.parametrize("upstream", [float("inf"), float("nan")])
+def test_ignored_rows_have_no_gradient_whatever_comes_back(upstream):
+    fo = _fo()
+    for dtype in (BF16, F16, F32):
+        for tokens in (30, 300):
+            for reduction in ("mean", "sum"):
+                x, w, target = _inputs(tokens, 40, 90, dtype, ignored=0.4)
+                loss = fo.linear_cross_entropy(x.requires_grad_(), w.requires_grad_(), target, reduction=reduction)
+                dx, _ = torch.autograd.grad(loss, (x, w), torch.full_like(loss, upstream))
+                assert (dx[target == IGNORE] == 0).all() and not dx[target != IGNORE].isfinite().any(), (dtype, tokens, reduction)
+                loss = fo.linear_cross_entropy(x, w, torch.full_like(target, IGNORE), reduction=reduction)
+                dx, dw = torch.autograd.grad(loss, (x, w), torch.full_like(loss, upstream))
+                assert (dx == 0).all() and (dw == 0).all(), (dtype, tokens, reduction)
+
+
 def test_all_ignored():
     fo = _fo()
     x, w, target = _inputs(10, 32, 50, BF16)
