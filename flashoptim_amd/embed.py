@@ -156,6 +156,15 @@ class FlashEmbedding(torch.nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
         self.scale = scale
 
+    @classmethod
+    def from_pretrained(cls, embeddings: torch.Tensor, freeze: bool = True, padding_idx: Optional[int] = None, scale: float = 1.0) -> "FlashEmbedding":
+        """A module whose weight is `embeddings`, without a gradient where `freeze` says so."""
+        if embeddings.dim() != 2:
+            raise ValueError(f"FlashEmbedding expects a matrix, got shape {tuple(embeddings.shape)}.")
+        made = cls(*embeddings.shape, padding_idx=padding_idx, scale=scale, device="meta", dtype=embeddings.dtype)
+        made.weight = torch.nn.Parameter(embeddings, requires_grad=not freeze)
+        return made
+
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         return embedding(input, self.weight, self.scale, self.padding_idx)
 

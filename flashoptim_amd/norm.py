@@ -6,6 +6,7 @@ The reference package has nothing of the kind.  ``torch.nn.functional.rms_norm``
 from __future__ import annotations
 
 import math
+import operator
 from typing import Optional, Union
 
 import torch
@@ -181,7 +182,9 @@ class FlashRMSNorm(torch.nn.RMSNorm):
     """``torch.nn.RMSNorm`` over the last axis through :func:`rms_norm`: ``norm(x)``, or ``y, stream = norm(x, stream)``."""
 
     def __init__(self, width: int, eps: float = 1e-6, elementwise_affine: bool = True, device=None, dtype=None):
-        super().__init__(width, eps=eps, elementwise_affine=elementwise_affine, device=device, dtype=dtype)
+        super().__init__(operator.index(width), eps=eps, elementwise_affine=elementwise_affine, device=device, dtype=dtype)
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        if self.weight is None and x.shape[-1:] != self.normalized_shape:
+            raise ValueError(f"FlashRMSNorm: x of shape {tuple(x.shape)} does not have rows of {self.normalized_shape[0]} values")
         return rms_norm(x, self.weight, residual, self.eps)

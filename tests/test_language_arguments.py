@@ -115,6 +115,23 @@ def test_without_a_gpu():
             call()
 
 
+def test_modules_check_what_they_are_made_of():
+    table = torch.randn(7, 5, dtype=torch.bfloat16)
+    frozen, free = fo.FlashEmbedding.from_pretrained(table, scale=2.0), fo.FlashEmbedding.from_pretrained(table, freeze=False, padding_idx=-1)
+    assert torch.equal(frozen.weight, table) and not frozen.weight.requires_grad and frozen.scale == 2.0 and frozen.padding_idx is None
+    assert free.weight.requires_grad and free.padding_idx == 6 and (free.num_embeddings, free.embedding_dim) == (7, 5)
+    assert frozen.weight.data_ptr() == table.data_ptr()
+    with pytest.raises(ValueError):
+        fo.FlashEmbedding.from_pretrained(table[0])
+    with pytest.raises(TypeError):
+        fo.FlashRMSNorm((4, 5))
+    norm = fo.FlashRMSNorm(8, elementwise_affine=False)
+    with pytest.raises(ValueError):
+        norm(torch.randn(3, 4))
+    with pytest.raises(ValueError):
+        norm(torch.tensor(1.0))
+
+
 @pytest.mark.skipif(not os.path.exists(_autograd.library_path()), reason="the C++ calls are not built")
 def test_calls_built_for_another_interface_are_left_out(monkeypatch):
     names = ("rms_norm", "rms_norm_mxfp4", "embedding", "linear_cross_entropy")
