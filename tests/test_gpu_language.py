@@ -246,3 +246,62 @@ def test_cast_models_keep_their_head_in_fp32():
     assert head.weight.grad.dtype == torch.float32 and body.weight.grad.dtype == torch.bfloat16
     with pytest.raises(ValueError, match="type"):
         fo.linear_cross_entropy(y, head.weight, target)
+
+
+@pytest.fixture(params=["nodes", "python"])
+def host(request, monkeypatch):
+    """Through the C++ calls and nodes, and through the Python ones that stand in for them."""
+    from flashoptim_amd import _autograd
+
+    _autograd.bind()
+    if request.param == "python":
+        for name in ("rms_norm", "rms_norm_mxfp4", "embedding", "linear_cross_entropy"):
+            monkeypatch.setattr(_autograd, name, None)
+    return request.param
+
+
+def test_under_checkpoints_and_hooks_on_what_is_saved(host):
+    from torch.utils.checkpoint import checkpoint
+
+    model = Model(torch.bfloat16)
+    tokens, target = _data(11)
+    parameters = list(model.parameters())
+    want = torch.autograd.grad(model(tokens, target), parameters)
+
+    def same(got):
+        return all(torch.equal(a, b) for a, b in zip(want, got))
+
+    assert same(torch.autograd.grad(checkpoint(model, tokens, target, use_reentrant=False), parameters))
+    with torch.autograd.graph.save_on_cpu():
+        loss = model(tokens, target)
+    assert same(torch.autograd.grad(loss, parameters))
+    checkpoint(lambda table: model(tokens, target) + 0.0 * table.sum(), model.embed.weight, use_reentrant=True).backward()
+    assert same([p.grad for p in parameters])
+    # a graph that is kept gives the same again, and adds up
+    loss = model(tokens, target)
+    for _ in range(2):
+        loss.backward(retain_graph=True)
+    for p, g in zip(parameters, want):    # two additions, each rounded by at most half a step of at most three times the gradient
+        assert (p.grad.float() - 3 * g.float()).abs().max() <= 3 * 2.0 ** -7 * g.float().abs().max()
+
+
+def test_modes_without_a_graph_and_transforms(host):
+    fo = _fo()
+    model = Model(torch.bfloat16)
+    tokens, target = _data(12)
+    loss = model(tokens, target)
+    with torch.no_grad():
+        assert torch.equal(model(tokens, target), loss)
+    with torch.inference_mode():
+        assert torch.equal(model(tokens, target), loss)
+        y, stream = fo.rms_norm(torch.ones(3, 8, device=DEV), None, torch.ones(3, 8, device=DEV))
+        assert y.is_inference() and stream.is_inference()
+    x, w = torch.randn(5, 8, device=DEV), torch.randn(9, 8, device=DEV)
+    at = torch.tensor([1, 2, 3, 4, 5], device=DEV)
+    with torch.autocast("cuda", dtype=torch.bfloat16):    # nothing is converted
+        assert fo.rms_norm(x).dtype == torch.float32 and fo.linear_cross_entropy(x, w, at).dtype == torch.float32
+    for f in (lambda t: fo.rms_norm(t).sum(), lambda t: fo.linear_cross_entropy(t, w, at), lambda t: fo.embedding(at, t).sum()):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(f)(x)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(x.expand(2, 5, 8).contiguous())
