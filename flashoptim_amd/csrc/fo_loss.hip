@@ -255,15 +255,18 @@ template <int ROWS> __global__ __launch_bounds__(1024) void loss_join_kernel(Joi
         __syncthreads();
     }
     if (slice != 0 || row >= a.rows) return;
-    const float lse = e.most + __builtin_logf(e.sum);
+    const float log_sum = __builtin_logf(e.sum);
     const int64_t target = a.targets[a.first + row];
     const int label = target == a.ignore ? kIgnored : target >= 0 && target < a.vocabulary ? (int)target : kNone;
     float loss = 0.0f;
     if (label == kNone) loss = __builtin_nanf("");
     else if (label != kIgnored) {
-        loss = lse - (a.smoothing > 0.0f ? (1.0f - a.smoothing) * a.picked[row] + a.smoothing * (logits / (float)a.vocabulary) : a.picked[row]);
+        // from the maximum, not from lse, whose rounding is as large as the loss of a target that is likely among large logits
+        loss = e.most - a.picked[row];
+        if (a.smoothing > 0.0f) loss = (1.0f - a.smoothing) * loss + a.smoothing * (e.most - logits / (float)a.vocabulary);
+        loss += log_sum;
     }
-    a.lse[row] = lse;
+    a.lse[row] = e.most + log_sum;
     a.loss[row] = loss;
     a.labels[row] = label;
 }

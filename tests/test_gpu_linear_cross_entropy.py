@@ -213,6 +213,23 @@ def test_ignored_rows_have_no_gradient_whatever_comes_back(upstream):
                 assert (dx == 0).all() and (dw == 0).all(), (dtype, tokens, reduction)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_small_losses_among_large_logits(dtype):
+    """One logit of 1000 and 99 of 992, all exact.  exp(-8) is off by 2^-19 of itself (its exponent, 12, by 2^-20), the sum of exponentials, 1.03, by the rounding of fewer than 16 additions
+    besides, the logarithm by as much: below 2^-19 in all.  With smoothing the mean of the logits, 992.08, is rounded to 2^-15."""
+    fo = _fo()
+    x, w = torch.zeros(3, 16, device=DEV, dtype=dtype), torch.zeros(100, 16, device=DEV, dtype=dtype)
+    x[:, 0], w[:, 0] = 1.0, 992.0
+    target = torch.tensor([0, 41, 99], device=DEV)
+    for row, likely in enumerate(target.tolist()):
+        weight = w.clone()
+        weight[likely, 0] = 1000.0
+        for smoothing in (0.0, 0.1):
+            want = F.cross_entropy(x.double() @ weight.double().t(), target, label_smoothing=smoothing, reduction="none")
+            got = fo.linear_cross_entropy(x, weight, target, label_smoothing=smoothing, reduction="none")
+            assert abs(float(got[row]) - float(want[row])) <= 2.0 ** -19 + smoothing * 2.0 ** -14, (row, smoothing)
+
+
 def test_all_ignored():
     fo = _fo()
     x, w, target = _inputs(10, 32, 50, BF16)
