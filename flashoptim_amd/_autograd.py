@@ -30,6 +30,10 @@ def _called() -> dict:
     return {n: "".join(letters[t] for t in (_native.SIGNATURES[n][0], *_native.SIGNATURES[n][1])) for n in names}
 
 
+def _agreed() -> dict:
+    return {**_called(), "FO_LINEAR_CROSS_ENTROPY_KEPT": str(_native.LOSS_NUMBERS_A_TOKEN + 1)}
+
+
 def _load() -> None:
     global _module, rms_norm, rms_norm_mxfp4, embedding, linear_cross_entropy
     if os.environ.get("FLASHOPTIM_NO_HOSTSCAN", "").strip() not in ("", "0") or not os.path.exists(_PATH):
@@ -40,7 +44,7 @@ def _load() -> None:
         spec.loader.exec_module(module)
     except (ImportError, OSError):  # built against another torch or python
         return
-    if getattr(module, "kinds", None) != _called():  # left over from another version of the library
+    if getattr(module, "kinds", None) != _agreed():  # left over from another version of the library
         return
     _module = module
     rms_norm, rms_norm_mxfp4 = module.rms_norm, module.rms_norm_mxfp4

@@ -23,6 +23,7 @@ _LIB_PATH = os.environ.get("FLASHOPTIM_HIP_LIBRARY") or os.path.join(
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 TILE_ELEMS = 4096
+LOSS_NUMBERS_A_TOKEN = 3  # FO_LINEAR_CROSS_ENTROPY_KEPT, one more beside
 
 
 class FoTensorDesc(ctypes.Structure):

@@ -213,7 +213,7 @@ struct JoinArgs {
     const float *sums, *picked;
     Targets targets;
     int64_t first, ignore, vocabulary;
-    float *lse, *loss;
+    float *most, *log_sum, *loss;    // of each row the largest logit, the log of the sum of exponentials relative to it
     int* labels;
     int rows, parts;
     float smoothing;
@@ -266,7 +266,8 @@ template <int ROWS> __global__ __launch_bounds__(1024) void loss_join_kernel(Joi
         if (a.smoothing > 0.0f) loss = (1.0f - a.smoothing) * loss + a.smoothing * (e.most - logits / (float)a.vocabulary);
         loss += log_sum;
     }
-    a.lse[row] = e.most + log_sum;
+    a.most[row] = e.most;
+    a.log_sum[row] = log_sum;
     a.loss[row] = loss;
     a.labels[row] = label;
 }
@@ -332,7 +333,7 @@ struct GradArgs {
     Operand x, weight;     // of a piece of the vocabulary
     int row_bytes, segment_stages;
     const int* labels;
-    const float *lse, *factors;    // no factors: `top` for every row
+    const float *most, *log_sum, *factors;    // no factors: `top` for every row
     float top;
     char* grad;            // G as operand rows over the piece
     float* lost;           // of each row with a target: what its target's entry lost in its rounding; or null
@@ -345,11 +346,12 @@ template <int DT, class Product> struct GradOut {
     static constexpr bool kColumns = false;
     typedef OperandOf<DT, Product> To;
     const GradArgs& a;
-    struct In { float lse, factor; int label; };
+    struct In { float most, over, factor; int label; };
     __device__ __forceinline__ void begin(int) const {}
     __device__ __forceinline__ void load(int i, int, In& in) const {
         if (i >= a.x.rows) return;
-        in.lse = a.lse[i];
+        in.most = a.most[i];
+        in.over = a.log_sum[i] * kLog2e;
         in.label = a.labels[i];
         in.factor = a.factors ? a.factors[i] : in.label == kNone ? __builtin_nanf("") : a.top;
     }
@@ -358,7 +360,7 @@ template <int DT, class Product> struct GradOut {
         const int at = in.label - a.first - j;    // among the eight, if the target is
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            float g = exp_of(v[k] - in.lse) - a.even;
+            float g = __builtin_amdgcn_exp2f(fmaf(v[k] - in.most, kLog2e, -in.over)) - a.even;    // lse would be rounded to the step of large logits
             if (at == k) g -= a.kept;
             v[k] = in.label == kIgnored || j + k >= a.weight.rows ? 0.0f : g * in.factor;
         }
@@ -772,7 +774,8 @@ struct Forward {
 
     template <int DT, class Product> int run() const {
         const char* what = "fo_linear_cross_entropy";
-        int* labels = (int*)(kept + x.rows + 1);
+        float *most = kept, *log_sum = most + x.rows, *count = log_sum + x.rows;
+        int* labels = (int*)(count + 1);
         const fo::Targets t{targets, index_bytes};
         float* losses = reduction == FO_REDUCE_NONE ? loss : (float*)(base + at.losses);
         fo::Operand w;
@@ -788,7 +791,7 @@ struct Forward {
             if (some.rows * ((weight.rows + tile.wt - 1) / tile.wt) > at.rows * at.parts) tile = at.tile;
             const fo::LogitsArgs a{rows, w, row_bytes, segment, t, first, (fo::f32x2*)(base + at.stats), smoothing > 0.0f ? (float*)(base + at.sums) : nullptr, (float*)(base + at.picked)};
             if (int rc = launch_tiles<LogitsLaunch<Product>>(tile, a, s, what)) return rc;
-            const fo::JoinArgs join{a.stats, a.sums, a.picked, t, first, ignore, weight.rows, kept + first, losses + first, labels + first, (int)some.rows,
+            const fo::JoinArgs join{a.stats, a.sums, a.picked, t, first, ignore, weight.rows, most + first, log_sum + first, losses + first, labels + first, (int)some.rows,
                                     (int)((weight.rows + tile.wt - 1) / tile.wt), smoothing};
             int rc;
             if (some.rows >= 64 * 128) rc = launch(fo::loss_join_kernel<64>, (some.rows + 63) / 64, 1024, 0, s, what, join);
@@ -797,7 +800,7 @@ struct Forward {
             if (rc) return rc;
         }
         if (reduction == FO_REDUCE_NONE) return 0;
-        fo::loss_reduce_kernel<<<dim3(1), dim3(1024), 0, s>>>(losses, labels, x.rows, reduction, loss, kept + x.rows);
+        fo::loss_reduce_kernel<<<dim3(1), dim3(1024), 0, s>>>(losses, labels, x.rows, reduction, loss, count);
         return check_hip(hipGetLastError(), what);
     }
 };
@@ -816,19 +819,20 @@ struct Backward {
 
     template <int DT, class Product> int run() const {
         const char* what = "fo_linear_cross_entropy_backward";
-        const int* labels = (const int*)(kept + x.rows + 1);
+        const float *most = kept, *log_sum = most + x.rows, *count = log_sum + x.rows;
+        const int* labels = (const int*)(count + 1);
         float *sums = (float*)(base + at.sums), *partial = (float*)(base + at.partial), *factors = nullptr;
         // With many rows the entries' errors are independent of one another, and what they add to dx is as large as its own rounding at most; few rows are put right, which costs a
         // read of W beside every piece of the result (20 us of 59 for 4096 x 4096 over 1024).
         float* lost = x.dtype != FO_F32 && dx && x.rows <= kFewRows ? (float*)(base + at.lost) : nullptr;
         const float top = x.dtype == FO_F16 ? 32768.0f : 1.0f;
-        fo::Scale scale{upstream, reduction != FO_REDUCE_NONE ? kept + x.rows : nullptr, 1.0f / top, reduction == FO_REDUCE_MEAN};
+        fo::Scale scale{upstream, reduction != FO_REDUCE_NONE ? count : nullptr, 1.0f / top, reduction == FO_REDUCE_MEAN};
         if (upstream_stride != 0 && x.rows > 1) {
             factors = (float*)(base + at.factors);
-            float* most = (float*)(base + at.scale);
-            fo::loss_factors_kernel<<<dim3(1), dim3(1024), 0, s>>>(upstream, upstream_stride, labels, x.rows, reduction, kept + x.rows, top, factors, most);
+            float* largest = (float*)(base + at.scale);
+            fo::loss_factors_kernel<<<dim3(1), dim3(1024), 0, s>>>(upstream, upstream_stride, labels, x.rows, reduction, count, top, factors, largest);
             if (int rc = check_hip(hipGetLastError(), what)) return rc;
-            scale = {most, nullptr, 1.0f / top, false};
+            scale = {largest, nullptr, 1.0f / top, false};
         }
         const int64_t tokens_length = mode.length(x.rows), cols_length = mode.length(x.cols), cols_inner = cols_length * mode.segments();
         fo::Operand rows;
@@ -842,7 +846,7 @@ struct Backward {
             fo::Operand w;
             if (int rc = operand_of(mode, some, false, nullptr, n, base + at.weight, fo::kRightOrder, w, s, what)) return rc;
             const fo::Operand g = operand(base + at.grad, length * mode.bytes(), x.rows, x.rows * length * mode.bytes(), fo::kLeftOrder);
-            const fo::GradArgs grad{rows, w, (int)(cols_inner * mode.bytes()), mode.stages(cols_length), labels, kept, factors, top, base + at.grad, lost, g.part_stride, (int)length,
+            const fo::GradArgs grad{rows, w, (int)(cols_inner * mode.bytes()), mode.stages(cols_length), labels, most, log_sum, factors, top, base + at.grad, lost, g.part_stride, (int)length,
                                     (int)first, 1.0f - smoothing, smoothing / (float)weight.rows};
             if (int rc = launch_tiles<GradLaunch<DT, Product>>(tile_for(mode, x.rows, n, (double)cols_inner, cus), grad, s, what)) return rc;
             fo::GradProductArgs p{};

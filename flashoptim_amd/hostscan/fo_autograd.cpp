@@ -7,7 +7,7 @@
 // (flashoptim_amd/norm.py, embed.py, loss.py), and for every call that is out of the ordinary: a function here gives None, and has done nothing, for
 // operands that are not plain strided tensors of this device with adjacent values; the Python path checks, converts and raises.
 //
-// kinds                                                dict from the name of a C entry point to the types it was built to call it with
+// kinds                                                dict from the name of a C entry point to the types it was built to call it with, and of sizes
 // bind(addresses)                                      dict from the name of a C entry point to its address
 // rms_norm(x, weight, residual, eps)                   None | y | (y, stream)
 // rms_norm_mxfp4(x, weight, residual, eps)             None | (codes, scales) | (codes, scales, stream)
@@ -373,7 +373,7 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
             at::NoGradGuard none;
             const auto numbers = x->options().dtype(at::kFloat);
             loss = reduction == FO_REDUCE_NONE ? at::empty(target->sizes(), numbers) : at::empty({}, numbers);
-            kept = at::empty({2 * tokens + 1}, numbers);
+            kept = at::empty({FO_LINEAR_CROSS_ENTROPY_KEPT(tokens)}, numbers);
             const int64_t size = api.fo_linear_cross_entropy_workspace(x->data_ptr(), code_of(*x), tokens, row_stride(*x), weight->data_ptr(), weight->stride(0), vocabulary, width,
                                                                        (float)smoothing);
             check_size(size, "fo_linear_cross_entropy");
@@ -417,6 +417,9 @@ PyObject* all_kinds() {
     }
     FO_ENTRIES(FO_KINDS)
 #undef FO_KINDS
+    PyObject* o = kinds ? PyUnicode_FromString(std::to_string(FO_LINEAR_CROSS_ENTROPY_KEPT(1)).c_str()) : nullptr;    // sizes that the two sides have to agree upon
+    if (!o || PyDict_SetItemString(kinds, "FO_LINEAR_CROSS_ENTROPY_KEPT", o) < 0) Py_CLEAR(kinds);
+    Py_XDECREF(o);
     return kinds;
 }
 

@@ -21,7 +21,7 @@ def _forward(x, weight, target, how):
     device, lib = x.device, _native.lib()
     ignore, reduction, smoothing = how
     loss = torch.empty(tokens if reduction == 0 else (), dtype=torch.float32, device=device)
-    kept = torch.empty(2 * tokens + 1, dtype=torch.float32, device=device)
+    kept = torch.empty(_native.LOSS_NUMBERS_A_TOKEN * tokens + 1, dtype=torch.float32, device=device)
     with _native.device_guard(device):
         size = lib.fo_linear_cross_entropy_workspace(x.data_ptr(), DTYPE_CODE[x.dtype], tokens, x.stride(0), weight.data_ptr(), weight.stride(0), vocabulary, width,
                                                      smoothing)
@@ -38,7 +38,7 @@ def _forward(x, weight, target, how):
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
-    """Keeps its operands and two numbers a row."""
+    """Keeps its operands and three numbers a row."""
 
     @staticmethod
     def forward(ctx, x, weight, target, how):
@@ -89,7 +89,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 
     Logits are summed in fp32 and not rounded.  The backward pass computes them again, a piece of the vocabulary at a time, so that of size tokens
     x vocabulary there is only a piece of their gradient; the sums have a fixed order, so results repeat to the bit.  Between the passes
-    `x`, `weight` and two numbers a row are kept.  A target outside the vocabulary makes a NaN (the call does not wait for
+    `x`, `weight` and three numbers a row are kept.  A target outside the vocabulary makes a NaN (the call does not wait for
     the GPU to look at the targets).
 
     Raises:

@@ -354,12 +354,13 @@ int fo_embedding_backward(const void *tokens, int index_bytes, int64_t n_tokens,
  * x: tokens x cols, weight: vocabulary x cols, both of `dtype`; targets: index_bytes 4 or 8 each, contiguous.  A target outside the
  * vocabulary makes a NaN.
  *   loss: fp32, `tokens` of them, or one: their sum or their sum over the number of targets that are not ignored
- *   kept: 2 * tokens + 1 fp32 numbers that the backward pass takes: log sum exp of each row, that number, and the rows' targets as int32 (-1: ignored,
- *   -2: none of the vocabulary)
+ *   kept: FO_LINEAR_CROSS_ENTROPY_KEPT fp32 numbers that the backward pass takes: of each row the largest logit, of each the log of the sum of exp(logit - largest), the
+ *   number of targets that are not ignored, and the rows' targets as int32 (-1: ignored, -2: none of the vocabulary)
  * Backward: upstream: the loss's gradient, fp32, upstream_stride elements apart (0: one for all); dx (tokens x cols) and dw (vocabulary
  * x cols) of `dtype`, contiguous, either may be NULL.  workspace: device memory, aligned to 256; its size goes by the operands' addresses and
  * strides too (what the matrix cores cannot read in place is laid out there).
  */
+#define FO_LINEAR_CROSS_ENTROPY_KEPT(tokens) (3 * (tokens) + 1)
 enum fo_reduction { FO_REDUCE_NONE = 0, FO_REDUCE_SUM = 1, FO_REDUCE_MEAN = 2 };
 int64_t fo_linear_cross_entropy_workspace(const void *x, int dtype, int64_t tokens, int64_t x_stride, const void *weight, int64_t weight_stride,
                                           int64_t vocabulary, int64_t cols, float smoothing);

@@ -207,7 +207,7 @@ def test_rows_behind_the_results_are_left_alone():
     lib, s = _native.lib(), _native.current_stream_ptr(torch.device(DEV))
     x, w = torch.randn(5, 24, device=DEV), torch.randn(11, 24, device=DEV)
     target = torch.tensor([1, 2, 3, 10, 0], device=DEV)
-    buffers = {n: torch.full((size + 512,), 77.0, device=DEV) for n, size in dict(y=120, loss=5, kept=11, dx=120, dw=264, rows=120, table=264).items()}
+    buffers = {n: torch.full((size + 512,), 77.0, device=DEV) for n, size in dict(y=120, loss=5, kept=16, dx=120, dw=264, rows=120, table=264).items()}
     at = {n: b.data_ptr() + 1024 for n, b in buffers.items()}
     assert lib.fo_rms_norm(x.data_ptr(), 0, 5, 24, 24, None, 0, 0, None, 0, 1e-6, None, at["y"], None, s) == 0
     size = lib.fo_linear_cross_entropy_workspace(x.data_ptr(), 0, 5, 24, w.data_ptr(), 24, 11, 24, 0.0)

@@ -228,6 +228,13 @@ def test_small_losses_among_large_logits(dtype):
             want = F.cross_entropy(x.double() @ weight.double().t(), target, label_smoothing=smoothing, reduction="none")
             got = fo.linear_cross_entropy(x, weight, target, label_smoothing=smoothing, reduction="none")
             assert abs(float(got[row]) - float(want[row])) <= 2.0 ** -19 + smoothing * 2.0 ** -14, (row, smoothing)
+        # the first value of each row of the matrix's gradient is the logit's: p - 1, where p is off by 2^-19 as well, and rounded to half a step of the type
+        weight.requires_grad_()
+        fo.linear_cross_entropy(x[row:row + 1], weight, target[row:row + 1]).backward()
+        want = torch.softmax(weight.detach().double()[:, 0], 0)
+        want[likely] -= 1.0
+        off = (weight.grad[:, 0].double() - want).abs()
+        assert bool((off <= 2.0 ** -19 * (want.abs() + (want < 0)) + 2 * HALF_STEP[dtype] * want.abs()).all()), (row, off)
 
 
 def test_all_ignored():
