@@ -59,7 +59,7 @@ template <int LOG, class F> __device__ __forceinline__ int below(u32 limit, cons
 __global__ __launch_bounds__(kRun) void embed_sort_kernel(Tokens tokens, int n, int64_t vocabulary, int64_t skip, u64* keys, int sorting, char* filled, int64_t fill_bytes) {
     if ((int)blockIdx.x >= sorting) { fill<kRun>(filled, fill_bytes, (int64_t)blockIdx.x - sorting); return; }
     __shared__ u32 run[kRun];
-    const int first = (int)blockIdx.x * kRun, at = threadIdx.x, lane = at & 63, wave = at >> 6;
+    const int first = (int)blockIdx.x * kRun, at = threadIdx.x, wave = at >> 6;
     u32 t = kNoToken;
     if (first + at < n) {
         const int64_t token = tokens[first + at];
@@ -70,7 +70,6 @@ __global__ __launch_bounds__(kRun) void embed_sort_kernel(Tokens tokens, int n, 
 #pragma unroll
     for (int i = 0; i < 64; ++i) place += (u32)__builtin_amdgcn_readlane((int)mine, i) < mine;
     run[wave * 64 + place] = mine;
-    (void)lane;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kRun / 64; ++w) {
