@@ -158,7 +158,7 @@ template <class Tile> __device__ __forceinline__ bool my_tile(int rows, int cols
 }
 
 // A tile of z, then out of the accumulators each row's maximum and sum over a wavefront's WT columns: a lane has four rows of every sixteen and every sixteenth column, so both
-// are a few operations in registers and four exchanges between sixteen neighbouring lanes.  Bound by the matrix cores: 8192 x 4096 over 128256 in 6.6 ms, 1300 TFLOP/s (a library
+// are a few operations in registers and four exchanges between sixteen neighbouring lanes.  Bound by the matrix cores: 8192 x 4096 over 128256 in 6.4 ms, 1350 TFLOP/s (a library
 // product of that size, which writes its result, 6.0); 17 of a tile's 105 us are its first loads and this.  With few rows bound by the weight's bytes: 5 rows 171 us, 6.1 TB/s.
 template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void logits_kernel(LogitsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -172,8 +172,18 @@ template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, W
     const int r0 = row0 + (tile.wave >> 1) * WT + (tile.lane >> 4) * 4, part0 = col0 + (tile.wave & 1) * WT, mine = tile.lane & 15;
     if (part0 >= cols) return;
     const int64_t part = part0 / WT;
+    // which column each row's target is: looked up before anything is stored, or every row waits for its own
+    int* wanted = reinterpret_cast<int*>(smem) + tile.wave * WT;
 #pragma unroll
-    for (int i = 0; i < Tile::kFrags; ++i)
+    for (int k = tile.lane; k < WT; k += 64) {
+        const int r = row0 + (tile.wave >> 1) * WT + k;
+        const int64_t at = a.targets[a.first + (r < rows ? r : rows - 1)] - part0;    // one that is ignored, or none, may be found too: nobody asks for it
+        wanted[k] = r < rows && at >= 0 && at < WT ? (int)at : -1;
+    }
+    Tile::same_wave();
+#pragma unroll
+    for (int i = 0; i < Tile::kFrags; ++i) {
+        const i32x4 picks = *reinterpret_cast<const i32x4*>(wanted + i * 16 + (tile.lane >> 4) * 4);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int r = r0 + i * 16 + k;
@@ -189,15 +199,12 @@ template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, W
 #pragma unroll
             for (int j = 0; j < Tile::kFrags; ++j) sum += exp_of(v[j] - base);
             sum = sum_of_16(sum);
-            if (r < rows) {
-                const int64_t at = a.targets[a.first + r] - part0;    // one that is ignored, or none, may be found too: nobody asks for it
-                if (at >= 0 && at < WT && (at & 15) == mine) {
+            if (picks[k] >= 0 && (picks[k] & 15) == mine) {
 #pragma unroll
-                    for (int j = 0; j < Tile::kFrags; ++j)
-                        if (j == at >> 4) a.picked[r] = v[j];
-                }
-                if (mine == 0) a.stats[part * rows + r] = f32x2{most, sum};
+                for (int j = 0; j < Tile::kFrags; ++j)
+                    if (j == picks[k] >> 4) a.picked[r] = v[j];
             }
+            if (mine == 0 && r < rows) a.stats[part * rows + r] = f32x2{most, sum};
             if (a.sums) {
                 float all = 0.0f;
 #pragma unroll
@@ -206,6 +213,7 @@ template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, W
                 if (mine == 0 && r < rows) a.sums[part * rows + r] = all;
             }
         }
+    }
 }
 
 struct JoinArgs {
@@ -397,8 +405,7 @@ struct GradProductArgs {
     int64_t stride;
     int dtype;
 };
-__device__ __forceinline__ void store_result(float (&v)[8], const GradProductArgs& a, int i, int j, int valid) {
-    const float scale = a.scale.value();
+__device__ __forceinline__ void store_result(float (&v)[8], const GradProductArgs& a, float scale, int i, int j, int valid) {
     if (a.lost) {
         const int label = a.labels[i];
         if (label >= 0) {
@@ -423,6 +430,7 @@ struct GradProductOut {
     static constexpr bool kColumns = false;
     const GradProductArgs& a;
     int64_t part;
+    float scale;    // read once: behind a store every piece would wait for it again
     struct In { f32x4 lo, hi; };
     __device__ __forceinline__ void begin(int) const {}
     __device__ __forceinline__ void load(int i, int j, In& in) const {
@@ -437,7 +445,7 @@ struct GradProductOut {
         if (i >= a.rows || j >= a.cols) return;
 #pragma unroll
         for (int k = 0; k < 4; ++k) { v[k] += in.lo[k]; v[4 + k] += in.hi[k]; }
-        if (a.out) store_result(v, a, i, j, a.cols - j);
+        if (a.out) store_result(v, a, scale, i, j, a.cols - j);
         else store_values<DT_F32>(v, a.sums + part * a.rows * a.stride + i * a.stride + j, a.cols - j);
     }
 };
@@ -452,11 +460,11 @@ template <class Product, bool TURNED, int WT, int STAGES> __global__ __launch_bo
     const int part = (int)(t / (down * across));
     int i, j;
     tile_at((int)(t - (int64_t)part * down * across), down, across, i, j);
+    GradProductOut out{a, part, a.out ? a.scale.value() : 1.0f};
     Tile tile(smem);
     tile.segment_stages = a.segment_stages;
     tile.first_stage = part * a.part_stages;
     tile.multiply(a.left, a.right, i * Tile::kTile, j * Tile::kTile, part + 1 < a.parts ? a.part_stages * kStageBytes : a.row_bytes - tile.first_stage * kStageBytes);
-    GradProductOut out{a, part};
     tile.finish(i * Tile::kTile, j * Tile::kTile, out);
 }
 // The parts' results and `more`, added up in their order.  A thread takes eight values of a row.
@@ -481,7 +489,7 @@ __global__ __launch_bounds__(256) void grad_join_kernel(GradProductArgs a, const
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] += v[e];
     }
-    if (a.out) store_result(sum, a, (int)i, j, valid);
+    if (a.out) store_result(sum, a, a.scale.value(), (int)i, j, valid);
     else store_values<DT_F32>(sum, a.sums + at, valid);
 }
 
