@@ -159,7 +159,7 @@ template <class Tile> __device__ __forceinline__ bool my_tile(int rows, int cols
 
 // A tile of z, then out of the accumulators each row's maximum and sum over a wavefront's WT columns: a lane has four rows of every sixteen and every sixteenth column, so both
 // are a few operations in registers and four exchanges between sixteen neighbouring lanes.  Bound by the matrix cores: 8192 x 4096 over 128256 in 6.4 ms, 1350 TFLOP/s (a library
-// product of that size, which writes its result, 6.0); 17 of a tile's 105 us are its first loads and this.  With few rows bound by the weight's bytes: 5 rows 171 us, 6.1 TB/s.
+// product of that size, which writes its result, 6.0); 13 of a tile's 101 us are its first loads and this.  With few rows bound by the weight's bytes: 5 rows 171 us, 6.1 TB/s.
 template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void logits_kernel(LogitsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmTile<Product, WT, STAGES> Tile;
@@ -449,7 +449,7 @@ struct GradProductOut {
         else store_values<DT_F32>(v, a.sums + part * a.rows * a.stride + i * a.stride + j, a.cols - j);
     }
 };
-// TURNED: the left operand comes by columns too (dW = G' x).  Bound by the matrix cores: dx of 8192 x 4096 over 16128 in 809 us (1340 TFLOP/s), dW the same sizes in 824.  With operands
+// TURNED: the left operand comes by columns too (dW = G' x).  Bound by the matrix cores: dx of 8192 x 4096 over 16128 in 777 us (1390 TFLOP/s), dW the same sizes in 805.  With operands
 // turned by launches of their own instead of by their reads (64 us a piece, and G written twice) the loss of 1003 x 1000 over 32003 took 496 us, so 398.
 template <class Product, bool TURNED, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void grad_product_kernel(GradProductArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -508,12 +508,15 @@ constexpr int64_t kBlockTokens = 16384;          // rows of one forward launch: 
 constexpr int64_t kFewRows = 256;
 constexpr int64_t kPieceValues = 1 << 27;        // of G, as rows and as columns: 256 MiB each in 16 bits
 
-// Times of tiles, middle between the three kinds of products, which differ by a tenth.  bf16 over 1024 and 4096 values: a 256 x 256 tile takes 42 and 108 us, 192 x 192
-// 32 and 78, two 128 x 128 on a compute unit 24 and 63 (alone 17 and 48), five 64 x 64 25 and 76 (alone 10 and 32; in four stages 9 and 20, two of
-// those 12 and 32).  fp32, where large tiles gain nothing, over 512 and 1024: two 128 x 128 74 and 133 (43 and 74), five 64 x 64 54 and 95 (15 and 24; 15 and 24, 23 and 38).
+// Times of tiles, middle between the three products that write their results (bf16 over 32, 1024 and 2048 values: a 256 x 256 tile takes 19, 46 and 68 us, 192 x 192 -, 32 and
+// 46, two 128 x 128 on a compute unit 7, 22 and 36, five 64 x 64 4, 18 and 34, two of those in four stages 3, 9 and 15), and of the logits, whose large tiles have less to do at
+// their end (256 x 256 37 and 62 us over 1000 and 2048, 192 x 192 25 and 38).  fp32, where large tiles gain nothing, over 512 and 1024: two 128 x 128 74 and 133 (43 and 74), five 64 x 64 54 and 95 (15 and 24; 15 and 24, 23 and 38).
 constexpr fo::TileCost kTileCosts[] = {
-    {128, 2, 1, 20.0, 0.0216, 20.0, 0.0216}, {96, 3, 1, 16.5, 0.0150, 16.5, 0.0150}, {64, 2, 2, 6.8, 0.0101, 10.9, 0.0127},
-    {32, 2, 5, 3.2, 0.0071, 7.6, 0.0168}, {32, 4, 2, 5.2, 0.0035, 5.4, 0.0064}};
+    {128, 2, 1, 23.0, 0.0216, 23.0, 0.0216}, {96, 3, 1, 16.5, 0.0150, 16.5, 0.0150}, {64, 2, 2, 6.8, 0.0101, 8.3, 0.0133},
+    {32, 2, 5, 3.2, 0.0071, 3.9, 0.0150}, {32, 4, 2, 3.4, 0.0038, 3.4, 0.0060}};
+constexpr fo::TileCost kTileCostsLogits[] = {
+    {128, 2, 1, 16.0, 0.0216, 16.0, 0.0216}, {96, 3, 1, 10.0, 0.0145, 10.0, 0.0145}, {64, 2, 2, 6.5, 0.0101, 7.5, 0.0133},
+    {32, 2, 5, 3.2, 0.0071, 3.9, 0.0150}, {32, 4, 2, 3.4, 0.0038, 3.4, 0.0060}};
 constexpr fo::TileCost kTileCostsF32[] = {
     {64, 2, 2, 11.0, 0.061, 14.0, 0.116}, {32, 2, 5, 5.8, 0.0171, 16.0, 0.0765}, {32, 4, 2, 6.5, 0.0168, 7.0, 0.0305}};
 struct Costs { const fo::TileCost *first, *last; const fo::TileCost* begin() const { return first; } const fo::TileCost* end() const { return last; } };
@@ -530,7 +533,10 @@ struct Mode {
     int64_t length(int64_t n) const { return round_up(n, in_parts ? 64 : 64 / bytes()); }                     // of an operand's row
     int64_t form(int64_t rows, int64_t inner) const { return aligned(rows * length(inner) * parts() * bytes()); }
     int stages(int64_t values) const { return (int)(values * bytes() / fo::kStageBytes); }
-    Costs costs() const { return dtype == FO_F32 && !in_parts ? Costs{kTileCostsF32, kTileCostsF32 + 3} : Costs{kTileCosts, kTileCosts + 5}; }
+    Costs costs(bool logits = false) const {
+        if (dtype == FO_F32 && !in_parts) return {kTileCostsF32, kTileCostsF32 + 3};
+        return logits ? Costs{kTileCostsLogits, kTileCostsLogits + 5} : Costs{kTileCosts, kTileCosts + 5};
+    }
 };
 
 int validate(const char* what, int dtype, int64_t tokens, int64_t cols, int64_t vocabulary) {
@@ -552,10 +558,10 @@ template <class K, class A> int launch(K kernel, int64_t grid, int threads, int 
 }
 
 // ---- products in tiles of a size that suits the result
-fo::TileCost tile_for(const Mode& mode, int64_t rows, int64_t cols, double inner, int cus, double* time_of = nullptr) {
+fo::TileCost tile_for(const Mode& mode, bool logits, int64_t rows, int64_t cols, double inner, int cus, double* time_of = nullptr) {
     fo::TileCost best{};
     double least = 0.0;
-    for (const fo::TileCost& t : mode.costs()) {
+    for (const fo::TileCost& t : mode.costs(logits)) {
         const double time = fo::tiles_time(t, (double)fo::tiles_of(rows, cols, t.wt), inner, cus);
         if (!best.wt || time < least) { best = t; least = time; }
     }
@@ -570,8 +576,8 @@ Mode mode_of(int dtype, int64_t tokens, int64_t cols, int64_t vocabulary, int cu
     if (dtype != FO_F32) return {dtype, false};
     const Mode whole{dtype, false}, parts{dtype, true};
     double by_whole, by_parts;
-    (void)tile_for(whole, tokens, vocabulary, (double)whole.length(cols), cus, &by_whole);
-    (void)tile_for(parts, tokens, vocabulary, (double)(parts.length(cols) * parts.segments()), cus, &by_parts);
+    (void)tile_for(whole, true, tokens, vocabulary, (double)whole.length(cols), cus, &by_whole);
+    (void)tile_for(parts, true, tokens, vocabulary, (double)(parts.length(cols) * parts.segments()), cus, &by_parts);
     by_parts += (double)(tokens + vocabulary) * (double)cols * 10e-6 / 4.0;
     return by_parts < by_whole ? parts : whole;
 }
@@ -727,7 +733,7 @@ struct ForwardSpace {
     ForwardSpace(const Mode& mode, const Matrix& of_x, const Matrix& of_weight, bool smooth, int cus) {
         const int64_t tokens = of_x.rows, length = mode.length(of_x.cols);
         rows = tokens < kBlockTokens ? tokens : kBlockTokens;
-        tile = tile_for(mode, rows, of_weight.rows, (double)(length * mode.segments()), cus);
+        tile = tile_for(mode, true, rows, of_weight.rows, (double)(length * mode.segments()), cus);
         parts = (of_weight.rows + tile.wt - 1) / tile.wt;
         picked = 0;
         losses = picked + aligned(rows * 4);
@@ -795,7 +801,7 @@ struct Forward {
             fo::Operand rows;
             if (int rc = operand_of(mode, some, x.cols != length, nullptr, some.rows, base + at.x, fo::kLeftOrder, rows, s, what)) return rc;
             // a last block is shorter, and its tiles may be smaller only where its parts need no more space
-            fo::TileCost tile = tile_for(mode, some.rows, weight.rows, (double)inner, cus);
+            fo::TileCost tile = tile_for(mode, true, some.rows, weight.rows, (double)inner, cus);
             if (some.rows * ((weight.rows + tile.wt - 1) / tile.wt) > at.rows * at.parts) tile = at.tile;
             const fo::LogitsArgs a{rows, w, row_bytes, segment, t, first, (fo::f32x2*)(base + at.stats), smoothing > 0.0f ? (float*)(base + at.sums) : nullptr, (float*)(base + at.picked)};
             if (int rc = launch_tiles<LogitsLaunch<Product>>(tile, a, s, what)) return rc;
@@ -856,7 +862,7 @@ struct Backward {
             const fo::Operand g = operand(base + at.grad, length * mode.bytes(), x.rows, x.rows * length * mode.bytes(), fo::kLeftOrder);
             const fo::GradArgs grad{rows, w, (int)(cols_inner * mode.bytes()), mode.stages(cols_length), labels, most, log_sum, factors, top, base + at.grad, lost, g.part_stride, (int)length,
                                     (int)first, 1.0f - smoothing, smoothing / (float)weight.rows};
-            if (int rc = launch_tiles<GradLaunch<DT, Product>>(tile_for(mode, x.rows, n, (double)cols_inner, cus), grad, s, what)) return rc;
+            if (int rc = launch_tiles<GradLaunch<DT, Product>>(tile_for(mode, false, x.rows, n, (double)cols_inner, cus), grad, s, what)) return rc;
             fo::GradProductArgs p{};
             p.cols = (int)x.cols;
             p.scale = scale;
