@@ -159,7 +159,7 @@ template <class Tile> __device__ __forceinline__ bool my_tile(int rows, int cols
 
 // A tile of z, then out of the accumulators each row's maximum and sum over a wavefront's WT columns: a lane has four rows of every sixteen and every sixteenth column, so both
 // are a few operations in registers and four exchanges between sixteen neighbouring lanes.  Bound by the matrix cores: 8192 x 4096 over 128256 in 6.4 ms, 1350 TFLOP/s (a library
-// product of that size, which writes its result, 6.0); 13 of a tile's 101 us are its first loads and this.  With few rows bound by the weight's bytes: 5 rows 171 us, 6.1 TB/s.
+// product of that size, which writes its result, 6.0); 13 of a tile's 101 us are its first loads and this.  With few rows bound by the weight's bytes: 5 rows 163 us, 6.4 TB/s.
 template <class Product, int WT, int STAGES> __global__ __launch_bounds__(256, WT >= 96 ? 1 : 2) void logits_kernel(LogitsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmTile<Product, WT, STAGES> Tile;
