@@ -401,14 +401,14 @@ struct GradProductArgs {
     const float* lost;     // dx: what the rows' targets lost, times their rows of the weight, is added before that; or null
     const int* labels;     // dx: of its rows; or null
     const char* weight;
-    int64_t weight_stride;
+    int64_t weight_stride, vocabulary;
     int64_t stride;
     int dtype;
 };
 __device__ __forceinline__ void store_result(float (&v)[8], const GradProductArgs& a, float scale, int i, int j, int valid) {
     if (a.lost) {
         const int label = a.labels[i];
-        if (label >= 0) {
+        if (label >= 0 && label < a.vocabulary) {    // what is kept between the passes has been out of these kernels' hands
             const float lost = a.lost[i];
             const char* row = a.weight + (label * a.weight_stride + j) * 2;
             float w[8];
@@ -881,6 +881,7 @@ struct Backward {
                 p.labels = labels;
                 p.weight = weight.p;
                 p.weight_stride = weight.stride;
+                p.vocabulary = weight.rows;
                 Cut cut = at.dx_cut;
                 cut.parts = (int)((length * mode.segments() + cut.part - 1) / cut.part);
                 if (int rc = product<Product, false>(mode, p, cut, partial, s, what)) return rc;

@@ -373,7 +373,8 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
             at::NoGradGuard none;
             const auto numbers = x->options().dtype(at::kFloat);
             loss = reduction == FO_REDUCE_NONE ? at::empty(target->sizes(), numbers) : at::empty({}, numbers);
-            kept = at::empty({FO_LINEAR_CROSS_ENTROPY_KEPT(tokens)}, numbers);
+            // fp32 numbers and int32 labels.  Hooks on saved tensors may convert what is floating-point; these are bits.
+            kept = at::empty({FO_LINEAR_CROSS_ENTROPY_KEPT(tokens)}, x->options().dtype(at::kInt));
             const int64_t size = api.fo_linear_cross_entropy_workspace(x->data_ptr(), code_of(*x), tokens, row_stride(*x), weight->data_ptr(), weight->stride(0), vocabulary, width,
                                                                        (float)smoothing);
             check_size(size, "fo_linear_cross_entropy");

@@ -21,7 +21,8 @@ def _forward(x, weight, target, how):
     device, lib = x.device, _native.lib()
     ignore, reduction, smoothing = how
     loss = torch.empty(tokens if reduction == 0 else (), dtype=torch.float32, device=device)
-    kept = torch.empty(_native.LOSS_NUMBERS_A_TOKEN * tokens + 1, dtype=torch.float32, device=device)
+    # fp32 numbers and int32 labels.  Hooks on saved tensors may convert what is floating-point; these are bits.
+    kept = torch.empty(_native.LOSS_NUMBERS_A_TOKEN * tokens + 1, dtype=torch.int32, device=device)
     with _native.device_guard(device):
         size = lib.fo_linear_cross_entropy_workspace(x.data_ptr(), DTYPE_CODE[x.dtype], tokens, x.stride(0), weight.data_ptr(), weight.stride(0), vocabulary, width,
                                                      smoothing)
