@@ -47,6 +47,21 @@ def _plain(x: torch.Tensor) -> torch.Tensor:
     return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
 
 
+def _save(ctx, *tensors: Optional[torch.Tensor]) -> None:
+    ctx.save_for_backward(*tensors)
+    ctx.saved_as = [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+
+
+def _saved(ctx, what: str) -> list:
+    """What _save was given, as the kernels read it.  Hooks on saved tensors may lay them out anew, but not give back other ones."""
+    out = []
+    for t, was in zip(ctx.saved_tensors, ctx.saved_as):
+        if (None if t is None else (t.shape, t.dtype, t.device)) != was:
+            raise RuntimeError(f"{what}: a hook on saved tensors gave back {(tuple(t.shape), t.dtype, t.device)} in place of {(tuple(was[0]), *was[1:])}.")
+        out.append(None if t is None else _plain(t))
+    return out
+
+
 def _differentiable_once(backward):
     """A backward pass without a derivative of its own: in a graph that records it, its results lead to an error."""
 
@@ -81,13 +96,13 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, tokens, scale, padding):
         ctx.shape, ctx.scale, ctx.padding = weight.shape, scale, padding
-        ctx.save_for_backward(tokens)
+        _save(ctx, tokens)
         return _lookup(tokens, weight, scale)
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, dy):
-        (tokens,) = ctx.saved_tensors
+        (tokens,) = _saved(ctx, "embedding")
         vocabulary, width = ctx.shape
         dy = _plain(dy)
         device, lib = dy.device, _native.lib()

@@ -96,6 +96,30 @@ bool records(std::initializer_list<const Tensor*> tensors) {
     return false;
 }
 
+// A tensor kept for the backward pass.  Hooks on saved tensors may lay it out anew, but not give back another one.
+struct Kept {
+    SavedVariable saved;
+    c10::SmallVector<int64_t, 6> sizes;
+    at::ScalarType type = at::kFloat;
+    c10::Device device = c10::Device(at::kCPU);
+
+    void keep(const Tensor& t, bool is_output = false) {
+        saved = SavedVariable(t, is_output);
+        sizes.assign(t.sizes().begin(), t.sizes().end());
+        type = t.scalar_type();
+        device = t.device();
+    }
+    void release() { saved.reset_data(); }
+    // As the kernels read it.
+    Tensor take(const char* what, std::shared_ptr<Node> owner = nullptr) const {
+        const Tensor t = saved.unpack(std::move(owner));
+        TORCH_CHECK(t.defined() && t.sizes() == at::IntArrayRef(sizes) && t.scalar_type() == type && t.device() == device && t.layout() == at::kStrided, what,
+                    ": a hook on saved tensors gave back another tensor than the one it was given");
+        at::NoGradGuard none;
+        return as_rows(t);
+    }
+};
+
 // Gradients have no derivative here: in a graph that records the backward pass they lead to an error.
 variable_list once(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -109,15 +133,15 @@ variable_list once(variable_list grads) {
 
 // ---------------------------------------------------------------------------------------------------- norm
 struct NormNode : Node {
-    SavedVariable s, weight, inverse;
+    Kept s, weight, inverse;
     bool has_weight = false, has_residual = false;
     at::ScalarType x_type;
     std::vector<int64_t> sizes;
 
     void release_variables() override {
-        s.reset_data();
-        weight.reset_data();
-        inverse.reset_data();
+        s.release();
+        weight.release();
+        inverse.release();
     }
     std::string name() const override { return "RMSNormBackward"; }
 
@@ -125,8 +149,8 @@ struct NormNode : Node {
         variable_list out(3);    // x, weight, residual
         const bool with_stream = grads.size() > 1 && grads[1].defined();
         if (!grads[0].defined() && !with_stream) return out;
-        const Tensor s = this->s.unpack(has_residual ? getptr() : nullptr), inverse = this->inverse.unpack();
-        const Tensor weight = has_weight ? this->weight.unpack() : Tensor();
+        const Tensor s = this->s.take("rms_norm", has_residual ? getptr() : nullptr), inverse = this->inverse.take("rms_norm");
+        const Tensor weight = has_weight ? this->weight.take("rms_norm") : Tensor();
         {
             at::NoGradGuard none;
             const c10::DeviceGuard guard(s.device());
@@ -197,9 +221,9 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
             node->has_residual = residual != nullptr;
             torch::autograd::set_history(y, node);
             if (residual) torch::autograd::set_history(stream, node);
-            node->s = SavedVariable(residual ? stream : *x, residual != nullptr);
-            if (weight) node->weight = SavedVariable(*weight, false);
-            node->inverse = SavedVariable(inverse, false);
+            node->s.keep(residual ? stream : *x, residual != nullptr);
+            if (weight) node->weight.keep(*weight);
+            node->inverse.keep(inverse);
         }
     }
     if (!residual) return THPVariable_Wrap(y);
@@ -247,17 +271,17 @@ PyObject* rms_norm_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // ---------------------------------------------------------------------------------------------------- embedding
 struct EmbeddingNode : Node {
-    SavedVariable tokens;
+    Kept tokens;
     int64_t vocabulary = 0, width = 0, padding = -1;
     float scale = 1.0f;
 
-    void release_variables() override { tokens.reset_data(); }
+    void release_variables() override { tokens.release(); }
     std::string name() const override { return "EmbeddingBackward"; }
 
     variable_list apply(variable_list&& grads) override {
         variable_list out(1);
         if (!grads[0].defined()) return out;
-        const Tensor tokens = this->tokens.unpack();
+        const Tensor tokens = this->tokens.take("embedding").contiguous();
         {
             at::NoGradGuard none;
             const c10::DeviceGuard guard(tokens.device());
@@ -301,7 +325,7 @@ PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (records({weight})) {
             auto node = std::shared_ptr<EmbeddingNode>(new EmbeddingNode(), torch::autograd::deleteNode);
             node->set_next_edges(torch::autograd::collect_next_edges(*weight));
-            node->tokens = SavedVariable(*tokens, false);
+            node->tokens.keep(*tokens);
             node->vocabulary = vocabulary;
             node->width = width;
             node->padding = padding;
@@ -315,21 +339,22 @@ PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // ---------------------------------------------------------------------------------------------------- loss
 struct LossNode : Node {
-    SavedVariable x, weight, kept;
+    Kept x, weight, kept;
     int reduction = 0;
     float smoothing = 0.0f;
 
     void release_variables() override {
-        x.reset_data();
-        weight.reset_data();
-        kept.reset_data();
+        x.release();
+        weight.release();
+        kept.release();
     }
     std::string name() const override { return "LinearCrossEntropyBackward"; }
 
     variable_list apply(variable_list&& grads) override {
         variable_list out(2);
         if (!grads[0].defined()) return out;
-        const Tensor x = this->x.unpack(), weight = this->weight.unpack(), kept = this->kept.unpack();
+        const char* what = "linear_cross_entropy";
+        const Tensor x = this->x.take(what), weight = this->weight.take(what), kept = this->kept.take(what);
         const bool need_dx = task_should_compute_output(0), need_dw = task_should_compute_output(1);
         if (!need_dx && !need_dw) return out;
         {
@@ -387,9 +412,9 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (records({x, weight})) {
             auto node = std::shared_ptr<LossNode>(new LossNode(), torch::autograd::deleteNode);
             node->set_next_edges(torch::autograd::collect_next_edges(*x, *weight));
-            node->x = SavedVariable(*x, false);
-            node->weight = SavedVariable(*weight, false);
-            node->kept = SavedVariable(kept, false);
+            node->x.keep(*x);
+            node->weight.keep(*weight);
+            node->kept.keep(kept);
             node->reduction = (int)reduction;
             node->smoothing = (float)smoothing;
             torch::autograd::set_history(loss, node);

@@ -10,7 +10,7 @@ import torch
 
 from . import _autograd, _native
 from ._native import DTYPE_CODE
-from .embed import _INDEX_BYTES, _check_tokens, _check_values, _differentiable_once, _plain
+from .embed import _INDEX_BYTES, _check_tokens, _check_values, _differentiable_once, _plain, _save, _saved
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}  # fo_reduction
 
@@ -45,14 +45,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, x, weight, target, how):
         x, weight = _plain(x), _plain(weight)
         loss, kept = _forward(x, weight, target, how)
-        ctx.save_for_backward(x, weight, kept)
+        _save(ctx, x, weight, kept)
         _, ctx.reduction, ctx.smoothing = how
         return loss
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, upstream):
-        x, weight, kept = ctx.saved_tensors
+        x, weight, kept = _saved(ctx, "linear_cross_entropy")
         need_dx, need_dw = ctx.needs_input_grad[:2]
         (tokens, width), vocabulary = x.shape, weight.shape[0]
         device, lib = x.device, _native.lib()

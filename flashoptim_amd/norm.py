@@ -13,7 +13,7 @@ import torch
 
 from . import _autograd, _native
 from ._native import DTYPE_CODE
-from .embed import _check_values, _differentiable_once, _plain
+from .embed import _check_values, _differentiable_once, _plain, _save, _saved
 from .mxfp4 import MXFP4Tensor, _empty
 
 
@@ -49,7 +49,7 @@ class _RMSNorm(torch.autograd.Function):
         plain = None if weight is None else _plain(weight)
         x_rows = _rows(x, x.shape[-1])
         y, stream, inverse = _forward(x_rows, plain, None if residual is None else _rows(residual, x.shape[-1]), eps, True)
-        ctx.save_for_backward(x_rows if residual is None else stream, plain, inverse)
+        _save(ctx, x_rows if residual is None else stream, plain, inverse)
         ctx.shape = x.shape
         y = y.view(x.shape)
         return y if residual is None else (y, stream.view(x.shape))
@@ -57,7 +57,7 @@ class _RMSNorm(torch.autograd.Function):
     @staticmethod
     @_differentiable_once
     def backward(ctx, dy, dstream=None):
-        s, weight, inverse = ctx.saved_tensors
+        s, weight, inverse = _saved(ctx, "rms_norm")
         need_dx, need_dw, need_dresidual, _ = ctx.needs_input_grad
         rows, width = s.shape
         device, lib = s.device, _native.lib()

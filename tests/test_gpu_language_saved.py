@@ -78,3 +78,62 @@ def test_labels_beyond_the_vocabulary_are_no_addresses(dtype):
     assert torch.equal(got[others], clean[others])
     p = torch.softmax(x.double() @ w.double().t(), 1)    # 64 products of fp32, probabilities rounded to the type, the result too: 2^-6 of the magnitudes' sum is far above
     assert bool(((got.double() - p @ w.double()).abs() <= 2.0 ** -6 * (p @ w.double().abs()))[[2, 4, 6]].all())
+
+
+def _laid_out(how):
+    """Hooks that give back the same values, another way round in memory."""
+
+    def other(t):
+        if t.dim() == 0 or t.numel() == 0:
+            return t.clone()
+        if how == "turned":    # the last axis is the one that lies apart
+            return t.transpose(0, -1).contiguous().transpose(0, -1)
+        if how == "apart":     # neither values nor rows are neighbours
+            wide = torch.zeros(*t.shape[:-1], 2 * t.shape[-1] + 3, dtype=t.dtype, device=t.device)
+            wide[..., 1:2 * t.shape[-1]:2] = t
+            return wide[..., 1:2 * t.shape[-1]:2]
+        wide = torch.zeros(*t.shape[:-1], t.shape[-1] + 5, dtype=t.dtype, device=t.device)
+        wide[..., 2:-3] = t
+        return wide[..., 2:-3]
+
+    return saved_tensors_hooks(lambda t: t.clone(), other)
+
+
+def _calls():
+    """Each operator with its leaves, matrices and batches of them."""
+    fo = _fo()
+    g = torch.Generator(device=DEV).manual_seed(5)
+
+    def values(*shape, dtype=BF16):
+        return torch.randn(*shape, generator=g, device=DEV).to(dtype).requires_grad_()
+
+    target = torch.randint(0, 33, (4, 6), generator=g, device=DEV)
+    table, x, r, scale, dy = values(33, 40), values(4, 6, 40), values(4, 6, 40, dtype=F32), values(40), values(4, 6, 40).detach()
+    flat, flat_r = values(24, 40), values(24, 40, dtype=F32)
+    yield "embedding", lambda: fo.embedding(target, table), (table,), dy
+    yield "embedding of a row", lambda: fo.embedding(target[0], table), (table,), dy[0]
+    yield "norm", lambda: fo.rms_norm(x, scale), (x, scale), dy
+    yield "norm with a residual", lambda: fo.rms_norm(x, scale, r)[0], (x, scale, r), dy
+    yield "norm of a matrix", lambda: fo.rms_norm(flat, scale), (flat, scale), dy.view(24, 40)
+    yield "norm of a matrix with a residual", lambda: fo.rms_norm(flat, scale, flat_r)[0], (flat, scale, flat_r), dy.view(24, 40)
+    yield "loss", lambda: fo.linear_cross_entropy(x, table, target, label_smoothing=0.1), (x, table), None
+    yield "loss of a matrix", lambda: fo.linear_cross_entropy(flat, table, target.view(24)), (flat, table), None
+
+
+@pytest.mark.parametrize("how", ["turned", "apart", "rows apart"])
+def test_what_hooks_lay_out_anew_is_read_right(how):
+    for what, call, leaves, dy in _calls():
+        want = torch.autograd.grad(call(), leaves, dy)
+        with _laid_out(how):
+            out = call()
+        got = torch.autograd.grad(out, leaves, dy)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), (how, what)
+
+
+def test_other_tensors_than_those_that_were_saved_are_refused():
+    for change in (lambda t: t.double() if t.is_floating_point() else t.short(), lambda t: t[:-1], lambda t: t.unsqueeze(0), lambda t: t.cpu()):
+        for what, call, leaves, dy in _calls():
+            with saved_tensors_hooks(lambda t: t, change):
+                out = call()
+            with pytest.raises(RuntimeError, match="hook on saved tensors"):
+                torch.autograd.grad(out, leaves, dy)
