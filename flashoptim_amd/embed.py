@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import functools
 import math
+import sys
 from typing import Optional
 
 import torch
@@ -47,17 +48,31 @@ def _plain(x: torch.Tensor) -> torch.Tensor:
     return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
 
 
+def _traced(what: str) -> bool:
+    """Whether torch.jit.trace records.  It sees torch's operations, of which a launch is none: a call goes into the trace as one operation, a Function's.  A tracer into
+    an fx graph has no such thing, and is refused."""
+    fx = sys.modules.get("torch.fx.experimental.proxy_tensor")
+    if fx is not None and fx.get_proxy_mode() is not None:
+        raise NotImplementedError(f"{what} cannot be traced into an fx graph: it is not made of torch's operations")
+    return torch.jit.is_tracing()
+
+
+def _sizes(x: torch.Tensor) -> tuple:
+    """The shape of `x` in numbers; under torch.jit.trace it is made of tensors."""
+    return tuple(map(int, x.shape))
+
+
 def _save(ctx, *tensors: Optional[torch.Tensor]) -> None:
     ctx.save_for_backward(*tensors)
-    ctx.saved_as = [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+    ctx.saved_as = [None if t is None else (_sizes(t), t.dtype, t.device) for t in tensors]
 
 
 def _saved(ctx, what: str) -> list:
     """What _save was given, as the kernels read it.  Hooks on saved tensors may lay them out anew, but not give back other ones."""
     out = []
     for t, was in zip(ctx.saved_tensors, ctx.saved_as):
-        if (None if t is None else (t.shape, t.dtype, t.device)) != was:
-            raise RuntimeError(f"{what}: a hook on saved tensors gave back {(tuple(t.shape), t.dtype, t.device)} in place of {(tuple(was[0]), *was[1:])}.")
+        if (None if t is None else (tuple(t.shape), t.dtype, t.device)) != was:
+            raise RuntimeError(f"{what}: a hook on saved tensors gave back {(tuple(t.shape), t.dtype, t.device)} in place of {was}.")
         out.append(None if t is None else _plain(t))
     return out
 
@@ -80,10 +95,10 @@ def _differentiable_once(backward):
 def _lookup(tokens: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
     """tokens: flat.  Every argument is checked."""
     weight = _plain(weight)
-    vocabulary, width = weight.shape
-    y = torch.empty((tokens.numel(), width), dtype=weight.dtype, device=weight.device)
+    (vocabulary, width), n = _sizes(weight), int(tokens.numel())
+    y = torch.empty((n, width), dtype=weight.dtype, device=weight.device)
     with _native.device_guard(weight.device):
-        rc = _native.lib().fo_embedding(tokens.data_ptr(), _INDEX_BYTES[tokens.dtype], tokens.numel(), weight.data_ptr(), DTYPE_CODE[weight.dtype], vocabulary,
+        rc = _native.lib().fo_embedding(tokens.data_ptr(), _INDEX_BYTES[tokens.dtype], n, weight.data_ptr(), DTYPE_CODE[weight.dtype], vocabulary,
                                         width, weight.stride(0), scale, y.data_ptr(), _native.current_stream_ptr(weight.device))
     if rc:
         _native.check(rc, "fo_embedding")
@@ -95,7 +110,7 @@ class _Embedding(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, weight, tokens, scale, padding):
-        ctx.shape, ctx.scale, ctx.padding = weight.shape, scale, padding
+        ctx.shape, ctx.scale, ctx.padding = _sizes(weight), scale, padding
         _save(ctx, tokens)
         return _lookup(tokens, weight, scale)
 
@@ -154,9 +169,9 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
     if padding_idx is not None:
         if not -vocabulary <= padding_idx < vocabulary:
             raise ValueError(f"padding_idx must be within the vocabulary of {vocabulary}, got {padding_idx}.")
-        padding = padding_idx % vocabulary
+        padding = int(padding_idx % vocabulary)
     flat = _check_tokens(tokens, weight.device, "embedding")
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if _traced("embedding") or (torch.is_grad_enabled() and weight.requires_grad):
         y = _Embedding.apply(weight, flat, scale, padding)
     else:
         y = _lookup(flat, weight, scale)

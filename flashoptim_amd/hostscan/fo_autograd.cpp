@@ -5,7 +5,8 @@
 // allocations are C++ and the backward pass runs in the engine's thread without the interpreter.  It is host code only; the kernels are reached through the
 // addresses of the C entry points that the Python binding hands over.  The package does the same in Python when the module has not been built
 // (flashoptim_amd/norm.py, embed.py, loss.py), and for every call that is out of the ordinary: a function here gives None, and has done nothing, for
-// operands that are not plain strided tensors of this device with adjacent values; the Python path checks, converts and raises.
+// operands that are not plain strided tensors of this device with adjacent values, and where torch's operations are recorded, of which a launch is none; the Python
+// path checks, converts, records and raises.
 //
 // kinds                                                dict from the name of a C entry point to the types it was built to call it with, and of sizes
 // bind(addresses)                                      dict from the name of a C entry point to its address
@@ -17,6 +18,8 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
@@ -24,6 +27,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <string>
@@ -60,6 +64,11 @@ int index_bytes(const Tensor& t) { return t.scalar_type() == at::kLong ? 8 : 4; 
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
+
+// Whether somebody may be looking at the operations that are called here.
+bool watched() {
+    return torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::any_modes_set() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+}
 
 // An ordinary tensor on a GPU; null for any other object.
 const Tensor* tensor_of(PyObject* o) {
@@ -183,7 +192,7 @@ struct NormNode : Node {
 
 PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 4 || !api.bound) Py_RETURN_NONE;
+    if (n != 4 || !api.bound || watched()) Py_RETURN_NONE;
     const Tensor *x = values_of(args[0]), *weight, *residual;
     if (!x || !optional_values(args[1], weight) || !optional_values(args[2], residual)) Py_RETURN_NONE;
     const double eps = PyFloat_AsDouble(args[3]);
@@ -237,7 +246,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyObject* rms_norm_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 4 || !api.bound) Py_RETURN_NONE;
+    if (n != 4 || !api.bound || watched()) Py_RETURN_NONE;
     const Tensor *x = values_of(args[0]), *weight, *residual;
     if (!x || !optional_values(args[1], weight) || !optional_values(args[2], residual)) Py_RETURN_NONE;
     const double eps = PyFloat_AsDouble(args[3]);
@@ -300,7 +309,7 @@ struct EmbeddingNode : Node {
 
 PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 4 || !api.bound) Py_RETURN_NONE;
+    if (n != 4 || !api.bound || watched()) Py_RETURN_NONE;
     const Tensor *tokens = tensor_of(args[0]), *weight = values_of(args[1]);
     if (!tokens || !weight) Py_RETURN_NONE;
     const double scale = PyFloat_AsDouble(args[2]);
@@ -380,7 +389,7 @@ struct LossNode : Node {
 
 PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 6 || !api.bound) Py_RETURN_NONE;
+    if (n != 6 || !api.bound || watched()) Py_RETURN_NONE;
     const Tensor *x = values_of(args[0]), *weight = values_of(args[1]), *target = tensor_of(args[2]);
     if (!x || !weight || !target) Py_RETURN_NONE;
     const int64_t ignore = PyLong_AsLongLong(args[3]), reduction = PyLong_AsLongLong(args[4]);

@@ -10,14 +10,14 @@ import torch
 
 from . import _autograd, _native
 from ._native import DTYPE_CODE
-from .embed import _INDEX_BYTES, _check_tokens, _check_values, _differentiable_once, _plain, _save, _saved
+from .embed import _INDEX_BYTES, _check_tokens, _check_values, _differentiable_once, _plain, _save, _saved, _sizes, _traced
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}  # fo_reduction
 
 
 def _forward(x, weight, target, how):
     """The loss, and what the backward pass takes beside the operands."""
-    (tokens, width), vocabulary = x.shape, weight.shape[0]
+    (tokens, width), (vocabulary, _) = _sizes(x), _sizes(weight)
     device, lib = x.device, _native.lib()
     ignore, reduction, smoothing = how
     loss = torch.empty(tokens if reduction == 0 else (), dtype=torch.float32, device=device)
@@ -122,7 +122,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         raise ValueError("linear_cross_entropy: no rows")
     how = (int(ignore_index), _REDUCTIONS[reduction], float(label_smoothing))
     rows = x if x.dim() == 2 else x.reshape(flat.numel(), x.shape[-1])
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    if _traced("linear_cross_entropy") or (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
         loss = _LinearCrossEntropy.apply(rows, weight, flat, how)
     else:
         loss, _ = _forward(_plain(rows), _plain(weight), flat, how)

@@ -13,18 +13,18 @@ import torch
 
 from . import _autograd, _native
 from ._native import DTYPE_CODE
-from .embed import _check_values, _differentiable_once, _plain, _save, _saved
+from .embed import _check_values, _differentiable_once, _plain, _save, _saved, _sizes, _traced
 from .mxfp4 import MXFP4Tensor, _empty
 
 
 def _rows(x: torch.Tensor, width: int) -> torch.Tensor:
     x = _plain(x)
-    return x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), width)
+    return x if x.dim() == 2 else x.reshape(math.prod(_sizes(x)[:-1]), width)
 
 
 def _forward(x, weight, residual, eps, keep):
     """x and residual as matrices of adjacent values.  y, the stream, and the number a row that the backward pass takes."""
-    rows, width = x.shape
+    rows, width = _sizes(x)
     device = x.device
     y = torch.empty((rows, width), dtype=x.dtype, device=device)
     stream = None if residual is None else torch.empty((rows, width), dtype=residual.dtype, device=device)
@@ -50,7 +50,7 @@ class _RMSNorm(torch.autograd.Function):
         x_rows = _rows(x, x.shape[-1])
         y, stream, inverse = _forward(x_rows, plain, None if residual is None else _rows(residual, x.shape[-1]), eps, True)
         _save(ctx, x_rows if residual is None else stream, plain, inverse)
-        ctx.shape = x.shape
+        ctx.shape = _sizes(x)
         y = y.view(x.shape)
         return y if residual is None else (y, stream.view(x.shape))
 
@@ -140,7 +140,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
             return got
     _autograd.bind()
     eps = _check(x, weight, residual, eps, "rms_norm")
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (residual is not None and residual.requires_grad)):
+    needed = x.requires_grad or (weight is not None and weight.requires_grad) or (residual is not None and residual.requires_grad)
+    if _traced("rms_norm") or (torch.is_grad_enabled() and needed):
         return _RMSNorm.apply(x, weight, residual, eps)
     width = x.shape[-1]
     y, stream, _ = _forward(_rows(x, width), None if weight is None else _plain(weight), None if residual is None else _rows(residual, width), eps, False)
@@ -161,6 +162,8 @@ def rms_norm_mxfp4(x: torch.Tensor, weight: Optional[torch.Tensor] = None, resid
             return y if residual is None else (y, got[2])
     _autograd.bind()
     eps = _check(x, weight, residual, eps, "rms_norm_mxfp4")
+    if _traced("rms_norm_mxfp4"):
+        raise NotImplementedError("rms_norm_mxfp4 cannot be traced: what it makes is not a tensor")
     if x.dim() != 2:
         raise ValueError(f"rms_norm_mxfp4 expects a matrix, got shape {tuple(x.shape)}.")
     x, weight, residual = _plain(x), None if weight is None else _plain(weight), None if residual is None else _plain(residual)
