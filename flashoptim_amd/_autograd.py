@@ -56,13 +56,14 @@ def library_path() -> str:
 
 
 def bind() -> None:
-    """Hands the C entry points of the loaded HIP library to the module."""
+    """Hands the C entry points of the loaded HIP library to the module, once; of threads that come here together each does, the same ones."""
     global _module
-    if _module is None:
+    module = _module
+    if module is None:
         return
     lib = _native.lib()
-    _module.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _called()})
-    _module = None  # once
+    module.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _called()})
+    _module = None
 
 
 _load()

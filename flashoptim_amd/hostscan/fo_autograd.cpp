@@ -460,6 +460,7 @@ PyObject* all_kinds() {
 
 PyObject* bind(PyObject*, PyObject* addresses) {
     if (!PyDict_Check(addresses)) return PyErr_Format(PyExc_TypeError, "bind takes a dict");
+    if (api.bound) Py_RETURN_NONE;    // calls may be under way in other threads
 #define FO_BIND(name)                                                                                         \
     {                                                                                                         \
         PyObject* o = PyDict_GetItemString(addresses, #name);                                                 \

@@ -1,6 +1,7 @@
 """What the embedding, the norm and the loss refuse before any device work, through their C entry points and through Python."""
 
 import os
+import threading
 
 import pytest
 import torch
@@ -145,3 +146,33 @@ def test_calls_built_for_another_interface_are_left_out(monkeypatch):
         assert all(getattr(_autograd, name) is None for name in names) and _autograd._module is None
     _autograd._load()
     assert all(getattr(_autograd, name) is not None for name in names)
+
+
+def test_first_calls_of_several_threads(monkeypatch):
+    """Threads that call first, together: every one finds the module bound, or binds it."""
+    bound, failed, together, lib = [], [], threading.Barrier(4, timeout=30), _native.lib()
+
+    class Module:
+        def bind(self, addresses):
+            bound.append(addresses)
+
+    def load():
+        together.wait()    # every thread has seen that nothing is bound
+        return lib
+
+    monkeypatch.setattr(_autograd, "_module", Module())
+    monkeypatch.setattr(_native, "lib", load)
+
+    def call():
+        try:
+            _autograd.bind()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=call) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and _autograd._module is None
+    assert bound and all(b == bound[0] and all(b.values()) for b in bound)
