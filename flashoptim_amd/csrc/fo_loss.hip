@@ -300,7 +300,7 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* losses, 
 }
 
 // ------------------------------------------------------------------------------------------- backward
-// What the products' results are multiplied by at the end: f_i over the factors that went into G.  One upstream for all rows is that itself, over the number of
+// What the products' results are multiplied by at the end: f_i over the factors that went into G.  The upstream of a sum or a mean is that itself, over the number of
 // targets where the loss is a mean; the factors are 1 then, and no launch is needed for them.
 struct Scale {
     const float* p;         // the upstream, or what loss_factors_kernel made of many
@@ -841,7 +841,8 @@ struct Backward {
         float* lost = x.dtype != FO_F32 && dx && x.rows <= kFewRows ? (float*)(base + at.lost) : nullptr;
         const float top = x.dtype == FO_F16 ? 32768.0f : 1.0f;
         fo::Scale scale{upstream, reduction != FO_REDUCE_NONE ? count : nullptr, 1.0f / top, reduction == FO_REDUCE_MEAN};
-        if (upstream_stride != 0 && x.rows > 1) {
+        // rows of their own losses have factors also where all come back with the same: zeros for ignored rows, so that no product's result needs to know of an infinite one
+        if (reduction == FO_REDUCE_NONE || (upstream_stride != 0 && x.rows > 1)) {
             factors = (float*)(base + at.factors);
             float* largest = (float*)(base + at.scale);
             fo::loss_factors_kernel<<<dim3(1), dim3(1024), 0, s>>>(upstream, upstream_stride, labels, x.rows, reduction, count, top, factors, largest);

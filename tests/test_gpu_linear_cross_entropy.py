@@ -393,3 +393,17 @@ def test_one_derivative_only(host):
     with pytest.raises(RuntimeError, match="differentiate twice"):
         (first.sum() + (leaf * leaf).sum()).backward()
     assert (out.grad_fn.name() == "LinearCrossEntropyBackward") == (host == "nodes")
+
+
+@pytest.mark.parametrize("upstream", [float("inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_ignored_rows_of_single_losses_have_no_gradient_whatever_comes_back(dtype, upstream):
+    """Losses of single rows that come back with the same infinity: one number for all of them, one for each, one row."""
+    fo = _fo()
+    for tokens in (1, 30, 300):
+        x, w, target = _inputs(tokens, 40, 90, dtype, ignored=0.4)
+        for back in (torch.full((), upstream, device=DEV).expand(tokens), torch.full((tokens,), upstream, device=DEV), torch.full((2 * tokens,), upstream, device=DEV)[::2]):
+            dx, dw = torch.autograd.grad(fo.linear_cross_entropy(x, w, torch.full_like(target, IGNORE), reduction="none"), (x, w), back)
+            assert not dx.any() and not dw.any(), (tokens, back.stride())
+            dx, _ = torch.autograd.grad(fo.linear_cross_entropy(x, w, target, reduction="none"), (x, w), back)
+            assert not dx[target == IGNORE].any() and not dx[target != IGNORE].isfinite().any(), (tokens, back.stride())
