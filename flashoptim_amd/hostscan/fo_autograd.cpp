@@ -157,17 +157,25 @@ struct NormNode : Node {
     variable_list apply(variable_list&& grads) override {
         variable_list out(3);    // x, weight, residual
         const bool with_stream = grads.size() > 1 && grads[1].defined();
-        if (!grads[0].defined() && !with_stream) return out;
+        const bool need_dx = task_should_compute_output(0), need_dw = has_weight && task_should_compute_output(1), need_dresidual = has_residual && task_should_compute_output(2);
+        if (!grads[0].defined()) {    // nothing comes from the norm, whatever stands in its rows
+            if (!with_stream) return out;
+            {
+                at::NoGradGuard none;
+                if (need_dx) out[0] = grads[1].to(x_type);
+                if (need_dw) out[1] = at::zeros(weight.sizes, grads[1].options().dtype(weight.type));
+                if (need_dresidual) out[2] = grads[1];
+            }
+            return once(std::move(out));
+        }
         const Tensor s = this->s.take("rms_norm", has_residual ? getptr() : nullptr), inverse = this->inverse.take("rms_norm");
         const Tensor weight = has_weight ? this->weight.take("rms_norm") : Tensor();
         {
             at::NoGradGuard none;
             const c10::DeviceGuard guard(s.device());
             const int64_t width = s.size(-1), rows = inverse.numel();
-            const Tensor dy = grads[0].defined() ? as_rows(grads[0]) : at::zeros(sizes, s.options().dtype(x_type));
-            const Tensor dstream = with_stream ? as_rows(grads[1]) : Tensor();
-            const bool same = s.scalar_type() == x_type, need_dx = task_should_compute_output(0), need_dw = has_weight && task_should_compute_output(1);
-            const bool need_dresidual = has_residual && task_should_compute_output(2);
+            const bool same = s.scalar_type() == x_type;
+            const Tensor dy = as_rows(grads[0]), dstream = with_stream ? as_rows(grads[1]) : Tensor();
             Tensor dx, dresidual, dw, workspace;
             if (need_dx || (need_dresidual && same)) dx = at::empty(sizes, s.options().dtype(x_type));
             if (need_dresidual && !same) dresidual = at::empty(sizes, s.options());

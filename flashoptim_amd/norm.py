@@ -57,14 +57,18 @@ class _RMSNorm(torch.autograd.Function):
     @staticmethod
     @_differentiable_once
     def backward(ctx, dy, dstream=None):
-        s, weight, inverse = _saved(ctx, "rms_norm")
         need_dx, need_dw, need_dresidual, _ = ctx.needs_input_grad
-        rows, width = s.shape
-        device, lib = s.device, _native.lib()
-        if dy is None:
+        if dy is None:    # nothing comes from the norm, whatever stands in its rows
             if dstream is None:
                 return None, None, None, None
-            dy = torch.zeros((rows, width), dtype=ctx.x_dtype, device=device)
+            dw = None
+            if need_dw:
+                shape, dtype, device = ctx.saved_as[1]
+                dw = torch.zeros(shape, dtype=dtype, device=device)
+            return dstream.to(ctx.x_dtype) if need_dx else None, dw, dstream if need_dresidual else None, None
+        s, weight, inverse = _saved(ctx, "rms_norm")
+        rows, width = s.shape
+        device, lib = s.device, _native.lib()
         dy = _rows(dy, width)
         dstream = None if dstream is None else _rows(dstream, width)
         same = s.dtype == ctx.x_dtype

@@ -300,3 +300,30 @@ def test_one_derivative_only(host):
     with pytest.raises(RuntimeError, match="differentiate twice"):
         (first.sum() + (leaf * leaf).sum()).backward()
     assert (out.grad_fn.name() == "RMSNormBackward") == (host == "nodes")
+
+
+def test_a_stream_alone_brings_its_gradient_alone():
+    """Where the norm's output is not used, what stands in its rows does not reach the gradients: infinities, NaN, rows of zeros without eps."""
+    fo = _fo()
+    for dtype, stream_dtype in TYPES:
+        x, r = torch.randn(6, 77, device=DEV).to(dtype), torch.randn(6, 77, device=DEV).to(stream_dtype)
+        w, ds = torch.randn(77, device=DEV).to(dtype), torch.randn(6, 77, device=DEV).to(stream_dtype)
+        x[1, 3], r[2, 70], x[4], r[4] = float("inf"), float("nan"), 0.0, 0.0
+        for shape in ((6, 77), (2, 3, 77)):
+            for eps in (0.0, 1e-6):
+                leaves = [x.clone().view(shape).requires_grad_(), w.clone().requires_grad_(), r.clone().view(shape).requires_grad_()]
+                y, s = fo.rms_norm(*leaves, eps=eps)
+                dx, dw, dr = torch.autograd.grad(s, leaves, ds.view(shape))
+                assert torch.equal(dx, ds.view(shape).to(dtype)) and torch.equal(dr, ds.view(shape)) and dw.shape == w.shape and dw.dtype == dtype and not dw.any()
+                for k in (0, 2):
+                    some = [t.detach().clone().requires_grad_(i == k) for i, t in enumerate(leaves)]
+                    s = fo.rms_norm(*some, eps=eps)[1]
+                    assert torch.equal(torch.autograd.grad(s, some[k], ds.view(shape))[0], dx if k == 0 else dr)
+    leaves = [torch.randn(6, 77, device=DEV, requires_grad=True) for _ in range(2)]
+    s = fo.rms_norm(leaves[0], None, leaves[1])[1]
+    s.sum().backward()
+    assert leaves[0].grad.data_ptr() != leaves[1].grad.data_ptr()
+    s = fo.rms_norm(leaves[0], None, leaves[1])[1]
+    (first,) = torch.autograd.grad(s, leaves[0], torch.ones_like(s), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        first.sum().backward()
