@@ -14,8 +14,9 @@
 // Types.  bf16 and fp16 operands go into the matrix cores as they are, sums are fp32.  G is rounded to the operands' type once, as the
 // other operand of its products is; the factors f_i are first divided by the largest of them (and multiplied by 2^15 for fp16, so that probabilities down to 2^-39
 // survive), which the products' results are multiplied by at the end: where all are equal, as in a mean, they are 1, and the entry p - 1 of an unlikely
-// target rounds to almost itself.  Of few rows, what the target's entry, by far the largest of most, loses in its rounding goes into dx all the same: that times the
-// target's row of W is added in fp32.  fp32 operands go into the fp32 instructions, a sixteenth of the rate; or, where the work is large enough to pay for laying
+// target rounds to almost itself.  What the target's entry, by far the largest of most rows, loses in its rounding goes into dx all the same: that times the
+// target's row of W is added in fp32, which reads a row of W beside every row of dx (of a backward pass of 4096 x 4096 over 1024 6 us in 164, of 4096 x 512 over 64 1 in 29, of
+// 8192 x 4096 over 128256 less than is measured).  dW has the entries as they were rounded.  fp32 operands go into the fp32 instructions, a sixteenth of the rate; or, where the work is large enough to pay for laying
 // them out (in_parts), they are cut into three bf16 parts of 8 bits each, a = a1 + a2 + a3
 // exactly, and the six products a3 b1, a2 b2, a1 b3, a2 b1, a1 b2, a1 b1 are one contraction over six times the length: what is left
 // out is below 2^-23 of a product.  The small ones come first, so that the sums are small while most of the additions round.
@@ -505,7 +506,6 @@ using fo::u32;
 constexpr int64_t kMostWorkgroups = (1 << 24) - 1;    // of 256 threads: a launch has less than 2^32 threads
 constexpr int64_t kMostTokens = 1 << 20, kMostCols = 1 << 16, kMostVocabulary = 1 << 24;    // 32-bit offsets into a tile's rows
 constexpr int64_t kBlockTokens = 16384;          // rows of one forward launch: bounds the parts' memory
-constexpr int64_t kFewRows = 256;
 constexpr int64_t kPieceValues = 1 << 27;        // of G, as rows and as columns: 256 MiB each in 16 bits
 
 // Times of tiles, middle between the three products that write their results (bf16 over 32, 1024 and 2048 values: a 256 x 256 tile takes 19, 46 and 68 us, 192 x 192 -, 32 and
@@ -836,9 +836,7 @@ struct Backward {
         const float *most = kept, *log_sum = most + x.rows, *count = log_sum + x.rows;
         const int* labels = (const int*)(count + 1);
         float *sums = (float*)(base + at.sums), *partial = (float*)(base + at.partial), *factors = nullptr;
-        // With many rows the entries' errors are independent of one another, and what they add to dx is as large as its own rounding at most; few rows are put right, which costs a
-        // read of W beside every piece of the result (20 us of 59 for 4096 x 4096 over 1024).
-        float* lost = x.dtype != FO_F32 && dx && x.rows <= kFewRows ? (float*)(base + at.lost) : nullptr;
+        float* lost = x.dtype != FO_F32 && dx ? (float*)(base + at.lost) : nullptr;
         const float top = x.dtype == FO_F16 ? 32768.0f : 1.0f;
         fo::Scale scale{upstream, reduction != FO_REDUCE_NONE ? count : nullptr, 1.0f / top, reduction == FO_REDUCE_MEAN};
         // rows of their own losses have factors also where all come back with the same: zeros for ignored rows, so that no product's result needs to know of an infinite one

@@ -407,3 +407,36 @@ def test_ignored_rows_of_single_losses_have_no_gradient_whatever_comes_back(dtyp
             assert not dx.any() and not dw.any(), (tokens, back.stride())
             dx, _ = torch.autograd.grad(fo.linear_cross_entropy(x, w, target, reduction="none"), (x, w), back)
             assert not dx[target == IGNORE].any() and not dx[target != IGNORE].isfinite().any(), (tokens, back.stride())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tokens,pieces", [(1, False), (256, False), (257, False), (1000, False), (2100, True)])
+def test_what_the_target_loses_is_in_dx_for_any_number_of_rows(tokens, pieces, dtype):
+    """p - 1 of every row stands almost in the middle between two numbers of the type, the other words' p next to one, and three quarters of the target's part of dx go up
+    against the others'.  Allowed are what the others' p lose, the error of p, 2^-19 as elsewhere here, a contraction over 511 values that are not zero, and one rounding of the result: less than
+    0.6 half steps of the target's part in all.  p - 1 rounded as well would be 0.85 to 0.97 more.  The last case has its vocabulary in pieces."""
+    fo = _fo()
+    half = HALF_STEP[dtype]
+    others = 65280 if dtype == BF16 and pieces else 510 if dtype == BF16 else 65504 if pieces else 2047    # powers of two times 1 - 2^-8 and 1 - 2^-11
+    g = torch.tensor([2.0 ** -(1 + i % 3) * (1.0 + half * (0.85 + 0.01 * (i % 13))) for i in range(tokens)], dtype=torch.float64)
+    logit = torch.log(others * (1 - g) / g)
+    x, w = torch.zeros(tokens, 256, dtype=dtype), torch.zeros(others + 1, 256, dtype=dtype)
+    x[:, 0] = logit.to(dtype)    # two values, so that their sum has more digits than the type
+    x[:, 1] = ((logit - x[:, 0].double()) * 256.0).to(dtype)
+    w[0] = torch.randn(256, generator=torch.Generator().manual_seed(tokens)).to(dtype)
+    w[1:511] = (0.75 * w[0].float() * others / 510).to(dtype)
+    w[:, :2] = 0.0
+    w[0, 0], w[0, 1] = 1.0, 2.0 ** -8
+    x, w = x.to(DEV), w.to(DEV)
+    w64 = w.double()
+    p = torch.softmax(x.double() @ w64.t(), 1)
+    entry, p = p[:, :1] - 1.0, p[:, 1:2]
+    lost, loses = (entry.to(dtype).double() - entry).abs() / entry.abs(), ((32768 * p).to(dtype).double() / 32768 - p).abs()    # of the first, and of each of the others
+    assert bool((lost > 0.8 * half).all()) and bool((loses < 0.2 * half * p).all())    # the entries are what they are meant to be
+    want = entry * w64[:1] + p * w64[1:511].sum(0)
+    error = loses * w64[1:511].abs().sum(0) + 2.0 ** -19 * (w64[:1].abs() + p * w64[1:511].abs().sum(0)) + _slack(511, dtype) * (entry.abs() * w64[:1].abs() + p * w64[1:511].abs().sum(0))
+    bound = error + half * (want.abs() + error) + SMALLEST[dtype]
+    assert bool((bound < 0.6 * half * entry.abs() * w64[:1].abs() + 2 * SMALLEST[dtype])[:, 2:].all())
+    dx = torch.autograd.grad(fo.linear_cross_entropy(x.requires_grad_(), w, torch.zeros(tokens, dtype=torch.int64, device=DEV), reduction="sum"), x)[0]
+    far = (dx.double() - want).abs()
+    assert bool((far <= bound).all()), float((far / bound).max())
