@@ -30,6 +30,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
+#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -105,6 +106,9 @@ bool records(std::initializer_list<const Tensor*> tensors) {
     return false;
 }
 
+// A node's tensors are taken and released under its mutex_: backward passes of one graph may run in several threads.
+typedef std::lock_guard<std::mutex> Lock;
+
 // A tensor kept for the backward pass.  Hooks on saved tensors may lay it out anew, but not give back another one.
 struct Kept {
     SavedVariable saved;
@@ -148,6 +152,7 @@ struct NormNode : Node {
     std::vector<int64_t> sizes;
 
     void release_variables() override {
+        const Lock lock(mutex_);
         s.release();
         weight.release();
         inverse.release();
@@ -168,8 +173,13 @@ struct NormNode : Node {
             }
             return once(std::move(out));
         }
-        const Tensor s = this->s.take("rms_norm", has_residual ? getptr() : nullptr), inverse = this->inverse.take("rms_norm");
-        const Tensor weight = has_weight ? this->weight.take("rms_norm") : Tensor();
+        Tensor s, weight, inverse;
+        {
+            const Lock lock(mutex_);
+            s = this->s.take("rms_norm", has_residual ? getptr() : nullptr);
+            if (has_weight) weight = this->weight.take("rms_norm");
+            inverse = this->inverse.take("rms_norm");
+        }
         {
             at::NoGradGuard none;
             const c10::DeviceGuard guard(s.device());
@@ -292,13 +302,20 @@ struct EmbeddingNode : Node {
     int64_t vocabulary = 0, width = 0, padding = -1;
     float scale = 1.0f;
 
-    void release_variables() override { tokens.release(); }
+    void release_variables() override {
+        const Lock lock(mutex_);
+        tokens.release();
+    }
     std::string name() const override { return "EmbeddingBackward"; }
 
     variable_list apply(variable_list&& grads) override {
         variable_list out(1);
         if (!grads[0].defined()) return out;
-        const Tensor tokens = this->tokens.take("embedding").contiguous();
+        Tensor tokens;
+        {
+            const Lock lock(mutex_);
+            tokens = this->tokens.take("embedding").contiguous();
+        }
         {
             at::NoGradGuard none;
             const c10::DeviceGuard guard(tokens.device());
@@ -361,6 +378,7 @@ struct LossNode : Node {
     float smoothing = 0.0f;
 
     void release_variables() override {
+        const Lock lock(mutex_);
         x.release();
         weight.release();
         kept.release();
@@ -370,8 +388,14 @@ struct LossNode : Node {
     variable_list apply(variable_list&& grads) override {
         variable_list out(2);
         if (!grads[0].defined()) return out;
-        const char* what = "linear_cross_entropy";
-        const Tensor x = this->x.take(what), weight = this->weight.take(what), kept = this->kept.take(what);
+        Tensor x, weight, kept;
+        {
+            const Lock lock(mutex_);
+            const char* what = "linear_cross_entropy";
+            x = this->x.take(what);
+            weight = this->weight.take(what);
+            kept = this->kept.take(what);
+        }
         const bool need_dx = task_should_compute_output(0), need_dw = task_should_compute_output(1);
         if (!need_dx && !need_dw) return out;
         {

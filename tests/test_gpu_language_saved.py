@@ -1,5 +1,7 @@
 """GPU tests of the embedding's, the norm's and the loss's backward passes when what was saved for them has been through a user's hands: hooks on saved tensors."""
 
+import threading
+
 import pytest
 import torch
 from torch.autograd.graph import saved_tensors_hooks
@@ -137,3 +139,28 @@ def test_other_tensors_than_those_that_were_saved_are_refused():
                 out = call()
             with pytest.raises(RuntimeError, match="hook on saved tensors"):
                 torch.autograd.grad(out, leaves, dy)
+
+
+def test_backward_passes_of_one_graph_in_several_threads():
+    """Of a graph that is kept every thread gets the gradients; of one that is not, each gets them or hears that they are gone."""
+    for what, call, leaves, dy in _calls():
+        out = call()
+        want = torch.autograd.grad(out, leaves, dy, retain_graph=True)
+        torch.cuda.synchronize()
+        for keep in (True, False):
+            got, gone, other = [], [], []
+
+            def backward():
+                for _ in range(10):
+                    try:
+                        got.append(torch.autograd.grad(out, leaves, dy, retain_graph=keep))
+                    except RuntimeError as e:
+                        (gone if "second time" in str(e) or "freed" in str(e) else other).append(e)
+
+            threads = [threading.Thread(target=backward) for _ in range(4)]
+            for t in threads:
+                t.start()
+            for t in threads:
+                t.join()
+            assert not other and len(got) + len(gone) == 40 and len(got) >= (40 if keep else 1), (what, other)
+            assert all(torch.equal(a, b) for g in got for a, b in zip(g, want)), what
