@@ -327,3 +327,21 @@ def test_a_stream_alone_brings_its_gradient_alone():
     (first,) = torch.autograd.grad(s, leaves[0], torch.ones_like(s), create_graph=True)
     with pytest.raises(RuntimeError, match="differentiate twice"):
         first.sum().backward()
+
+
+@pytest.mark.parametrize("width", [1, 33, 128, 250, 512, 2730, 4096, 5000, 16300])
+@pytest.mark.parametrize("types", TYPES, ids=str)
+def test_mxfp4_form_writes_the_stream_of_every_row(width, types):
+    """The stream is one fp32 addition and one rounding, in every row, NaN among them too; the codes are those of that stream, formed apart from the call."""
+    fo = _fo()
+    dtype, stream_dtype = types
+    for rows in (2, 9, 1100):
+        x = (3.0 * torch.randn(rows, width, device=DEV)).to(dtype)
+        residual = torch.randn(rows, width, device=DEV).to(stream_dtype)
+        w = (1.0 + 0.3 * torch.randn(width, device=DEV)).to(dtype)
+        x[rows // 2, width // 2] = float("nan")
+        want = (x.float() + residual.float()).to(stream_dtype)
+        q, s = fo.rms_norm_mxfp4(x, w, residual, eps=1e-5)
+        torch.testing.assert_close(s, want, rtol=0, atol=0, equal_nan=True)
+        codes = fo.mxfp4_quantize(fo.rms_norm(want.float(), w, eps=1e-5))
+        assert torch.equal(q.scales, codes.scales) and torch.equal(q.codes, codes.codes), (width, types, rows)
