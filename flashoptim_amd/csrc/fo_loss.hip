@@ -506,7 +506,7 @@ using fo::u32;
 constexpr int64_t kMostWorkgroups = (1 << 24) - 1;    // of 256 threads: a launch has less than 2^32 threads
 constexpr int64_t kMostTokens = 1 << 20, kMostCols = 1 << 16, kMostVocabulary = 1 << 24;    // 32-bit offsets into a tile's rows
 constexpr int64_t kBlockTokens = 16384;          // rows of one forward launch: bounds the parts' memory
-constexpr int64_t kPieceValues = 1 << 27;        // of G, as rows and as columns: 256 MiB each in 16 bits
+constexpr int64_t kPieceValues = 1 << 27;        // of G in 16 bits: 256 MiB, and up to 256 words of every token more, since pieces are whole multiples of that
 
 // Times of tiles, middle between the three products that write their results (bf16 over 32, 1024 and 2048 values: a 256 x 256 tile takes 19, 46 and 68 us, 192 x 192 -, 32 and
 // 46, two 128 x 128 on a compute unit 7, 22 and 36, five 64 x 64 4, 18 and 34, two of those in four stages 3, 9 and 15), and of the logits, whose large tiles have less to do at

@@ -176,3 +176,16 @@ def test_first_calls_of_several_threads(monkeypatch):
         t.join()
     assert not failed and _autograd._module is None
     assert bound and all(b == bound[0] and all(b.values()) for b in bound)
+
+
+def test_the_loss_gradient_takes_a_bounded_workspace():
+    """2^28 bytes of G, up to 256 words more of every token, since pieces are whole multiples of that; beside it dx in fp32 between pieces, or in parts where rows are few, two
+    numbers a token, and fp32 operands that are laid out."""
+    lib = _native.lib()
+    for dtype, bytes_a_word in ((0, 6), (1, 2), (2, 2)):    # of fp32 at most three parts
+        for tokens in (1, 1000, 8192, 50000, 300000, 1 << 20):
+            for vocabulary in (33, 128256, 1 << 24):
+                size = lib.fo_linear_cross_entropy_backward_workspace(SOME, dtype, tokens, 64, SOME, 64, vocabulary, 64, 1, 0)
+                operands = 0 if dtype else 6 * 64 * (tokens + 64 + (1 << 28) // (6 * tokens) + 512)    # fp32 in parts: x and a piece of the matrix
+                sums, parts = 4 * 64 * tokens, 4 * 64 * tokens * 32 if tokens <= 8192 else 0
+                assert 0 < size <= (1 << 28) + 257 * tokens * bytes_a_word + sums + parts + 8 * tokens + operands + (1 << 20), (dtype, tokens, vocabulary)
