@@ -134,7 +134,8 @@ template <int DT, int THREADS, int V, bool WHOLE> struct Raw {
 
 // XT: type of x and y, RT: of the residual and the stream.  THREADS hold V pieces of eight values each, THREADS * V * 8 >= cols.  A workgroup takes every
 // gridDim.x-th row and asks for the next one before it adds up the squares of this one (rows of up to 8192 values; longer ones leave no registers
-// for that).  Bound by memory: 8192 x 4096 bf16 with a residual in 42 us (6.4 TB/s; 56 without the next row ahead), into MXFP4 4096 of them in 18; one row 2.8 us, a launch.
+// for that: 2048 x 16384 and 4096 x 8200 bf16 in 45 us, as 4096 x 8192, and back in 57 where 4096 x 8192 takes 51).
+// Bound by memory: 8192 x 4096 bf16 with a residual in 42 us (6.4 TB/s; 56 without the next row ahead), into MXFP4 4096 of them in 18; one row 2.8 us, a launch.
 template <int XT, int RT, int THREADS, int V, bool MX, bool WHOLE> __global__ __launch_bounds__(THREADS) void norm_kernel(NormArgs a) {
     constexpr int XB = DTypeInfo<XT>::bytes, RB = DTypeInfo<RT>::bytes;
     constexpr bool kAhead = THREADS <= 256;

@@ -88,7 +88,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     Returns:
         The loss in fp32: a number, or of the shape of `target`.
 
-    Logits are summed in fp32 and not rounded.  The backward pass computes them again, a piece of the vocabulary at a time, so that of size tokens
+    Logits are summed in fp32 and not rounded.  Their gradient is rounded once to the type of `x`, between the products; what the target's entry, by far the largest of most rows, loses in
+    that goes into the gradient of `x` all the same, not into that of `weight`.  The backward pass computes them again, a piece of the vocabulary at a time, so that of size tokens
     x vocabulary there is only a piece of their gradient; the sums have a fixed order, so results repeat to the bit.  Between the passes
     `x`, `weight` and three numbers a row are kept.  A target outside the vocabulary makes a NaN (the call does not wait for
     the GPU to look at the targets).

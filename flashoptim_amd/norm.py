@@ -133,7 +133,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
         The norm's output in the type of `x`; with a residual ``(output, s)``, `s` being the stream that goes on, rounded to the residual's
         type.  The norm is taken of the rounded `s`.
 
-    Sums are fp32 (fp64 for rows whose squares fp32 does not hold); outputs and gradients are rounded once and repeat to the bit.
+    The mean of the squares is summed in fp64, the gradients' sums in fp32; outputs and gradients are rounded once and repeat to the bit.  Where only `s` has a
+    gradient, that is handed on as it is, whatever the norm of its rows.
 
     Raises:
         NotImplementedError: no ROCm device, or an operand with a forward-mode tangent (there is no such derivative here).

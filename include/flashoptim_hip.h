@@ -355,7 +355,8 @@ int fo_embedding_backward(const void *tokens, int index_bytes, int64_t n_tokens,
  * vocabulary makes a NaN.
  *   loss: fp32, `tokens` of them, or one: their sum or their sum over the number of targets that are not ignored
  *   kept: FO_LINEAR_CROSS_ENTROPY_KEPT fp32 numbers that the backward pass takes: of each row the largest logit, of each the log of the sum of exp(logit - largest), the
- *   number of targets that are not ignored, and the rows' targets as int32 (-1: ignored, -2: none of the vocabulary)
+ *   number of targets that are not ignored, and the rows' targets as int32 (-1: ignored, -2: none of the vocabulary; anything else outside the vocabulary
+ *   is read as no target)
  * Backward: upstream: the loss's gradient, fp32, upstream_stride elements apart (0: one for all); dx (tokens x cols) and dw (vocabulary
  * x cols) of `dtype`, contiguous, either may be NULL.  workspace: device memory, aligned to 256; its size goes by the operands' addresses and
  * strides too (what the matrix cores cannot read in place is laid out there).
