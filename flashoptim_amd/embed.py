@@ -34,6 +34,8 @@ def _check_values(x: torch.Tensor, what: str, name: str) -> torch.Tensor:
     kernels._require_device(x, what)
     if x.dtype not in DTYPE_CODE:
         raise ValueError(f"{what} expects fp32, bf16 or fp16 as {name}, got {x.dtype}.")
+    if x.numel() and not x.data_ptr():    # to the C entry points an operand without an address is one that was left out
+        raise NotImplementedError(f"{what} expects {name} in memory, got a {type(x).__name__} that has none of its own.")
     if forward_ad.unpack_dual(x).tangent is not None:
         raise NotImplementedError(f"{what} has no forward-mode derivative")
     return x

@@ -75,7 +75,7 @@ bool watched() {
 const Tensor* tensor_of(PyObject* o) {
     if (!THPVariable_CheckExact(o)) return nullptr;
     const Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.is_neg() || t._fw_grad(0).defined()) return nullptr;
+    if (!t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t._is_zerotensor() || t.is_neg() || t._fw_grad(0).defined()) return nullptr;
     return &t;
 }
 bool is_values(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }

@@ -345,3 +345,22 @@ def test_mxfp4_form_writes_the_stream_of_every_row(width, types):
         torch.testing.assert_close(s, want, rtol=0, atol=0, equal_nan=True)
         codes = fo.mxfp4_quantize(fo.rms_norm(want.float(), w, eps=1e-5))
         assert torch.equal(q.scales, codes.scales) and torch.equal(q.codes, codes.codes), (width, types, rows)
+
+
+def test_operands_without_memory_are_refused():
+    """Wrappers and zeros that torch keeps no memory for have no address, which is how the C entry points are told that there is no weight: not ones in its place."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    fo = _fo()
+    x, w = torch.randn(4, 40, device=DEV), torch.randn(40, device=DEV)
+    with FakeTensorMode():
+        fake, fake_x = torch.ones(40, device=DEV), torch.ones(4, 40, device=DEV)
+    zeros, zeros_x = torch._efficientzerotensor(40, device=DEV), torch._efficientzerotensor((4, 40), device=DEV)
+    for args in ((x, fake), (x, zeros), (fake_x, w), (zeros_x, w), (x, w, fake_x), (x, w, zeros_x)):
+        for call in (fo.rms_norm, fo.rms_norm_mxfp4):
+            with pytest.raises(NotImplementedError, match="in memory"):
+                call(*args)
+    with pytest.raises(NotImplementedError, match="in memory"):
+        fo.linear_cross_entropy(x, fake_x, torch.zeros(4, dtype=torch.int64, device=DEV))
+    with pytest.raises(NotImplementedError, match="in memory"):
+        fo.embedding(torch.zeros(4, dtype=torch.int64, device=DEV), zeros_x)
